@@ -10,3 +10,18 @@ from .engine import (  # noqa: F401
     gen_uniform_alg, pad_to_tiles, row_blocks, balanced_row_blocks,
 )
 from ._lib import SpammError, SpammStats  # noqa: F401
+
+# attention over selected blocks works on torch tensors: torch is imported when one of these is first asked for
+_ATTENTION = ("PagedCache", "block_sparse_attention", "select_blocks")
+
+
+def __getattr__(name):
+    if name in _ATTENTION:
+        from . import attention
+
+        return getattr(attention, name)
+    raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
+
+
+def __dir__():
+    return sorted([*globals(), *_ATTENTION])

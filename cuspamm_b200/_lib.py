@@ -36,6 +36,19 @@ class SpammStats(C.Structure):
         return {n: getattr(self, n) for n, _ in self._fields_}
 
 
+class SpammAttn(C.Structure):
+    """Mirror of `spamm_attn` in include/spamm.h."""
+
+    _fields_ = (
+        [(n, C.c_int32) for n in ("dtype", "batch", "heads", "kv_heads", "dim", "block", "query_block", "n_select", "causal",
+                                  "max_q", "tokens", "n_pages", "table_width", "zero_tail")]
+        + [("scale", C.c_float), ("d_cu", C.c_void_p), ("d_lengths", C.c_void_p), ("d_table", C.c_void_p),
+           ("table_stride", C.c_int64), ("d_lists", C.c_void_p)]
+        + [f for x in "qkvo" for f in ((f"d_{x}", C.c_void_p), (f"{x}_token", C.c_int64), (f"{x}_head", C.c_int64))]
+        + [("d_lse", C.c_void_p), ("d_status", C.c_void_p)]
+    )
+
+
 _vp, _i, _i64, _f, _sz = C.c_void_p, C.c_int, C.c_int64, C.c_float, C.c_size_t
 _pp = C.POINTER(C.c_void_p)
 
@@ -103,6 +116,13 @@ SIGNATURES = {
     "spamm_pack_half_dev": (_i, [_vp, _vp, _i, _i, _i, _vp, _vp, _vp, _vp, _vp]),
     "spamm_gated_multiply_dev": (_i, [_vp] * 7 + [_i, _i, _i, _vp, _i64, _vp]),
     "spamm_macro_tile_order": (_i, [_i, _i, _vp]),
+    "spamm_attn_append_dev": (_i, [C.POINTER(SpammAttn), _vp, _vp, _vp, _vp, _i, _i, _vp]),
+    "spamm_attn_select_scratch_bytes": (_sz, [C.POINTER(SpammAttn)]),
+    "spamm_attn_select_dev": (_i, [C.POINTER(SpammAttn), _vp, _i, _i, _vp, _vp, _sz, _vp]),
+    "spamm_attn_forward_scratch_bytes": (_sz, [C.POINTER(SpammAttn)]),
+    "spamm_attn_forward_dev": (_i, [C.POINTER(SpammAttn), _vp, _sz, _vp]),
+    "spamm_attn_backward_scratch_bytes": (_sz, [C.POINTER(SpammAttn)]),
+    "spamm_attn_backward_dev": (_i, [C.POINTER(SpammAttn), _vp, _i64, _i64, _vp, _vp, _vp, _vp, _sz, _vp]),
     "spamm_gen_decay_exp": (_i, [_vp, _f, _f, _i64, _i64, _i64]),
     "spamm_gen_decay_alg": (_i, [_vp, _f, _f, _i64, _i64, _i64]),
     "spamm_gen_ones": (_i, [_vp, _i64, _i64, _i64]),
@@ -143,7 +163,7 @@ class SpammError(RuntimeError):
         lib = load()
         msg = lib.spamm_status_string(status).decode()
         detail = lib.spamm_last_cuda_error().decode()
-        super().__init__(f"{where}: {msg} (status {status})" + (f": {detail}" if detail and status in (2, 3) else ""))
+        super().__init__(f"{where}: {msg} (status {status})" + (f": {detail}" if detail and (status in (2, 3) or where.startswith("spamm_attn")) else ""))
         self.status = status
 
 

@@ -1,0 +1,392 @@
+"""Attention over selected blocks: the engine's scheme (a cheap score for every block, lists of the blocks worth
+multiplying, products of the listed blocks only) for queries, keys and values on the GPU.
+
+    lists = select_blocks(q, k, cu_seqlens, max_seqlen, n_select)
+    o = block_sparse_attention(q, k, v, lists, cu_seqlens, max_seqlen)        # differentiable in q, k and v
+
+and, for serving, over a paged cache whose pages are the blocks:
+
+    cache = PagedCache.empty(n_pages, kv_heads, head_dim)
+    q = cache.append(k, v, cu_seqlens, max_new, page_table, lengths, inv_freq=inv_freq, q=q)
+    lists = cache.select(q, cu_seqlens, max_new, page_table, lengths, n_select)
+    o = cache.attend(q, cu_seqlens, max_new, page_table, lengths, lists=lists)   # or lists=None: all pages
+
+Tensors are torch tensors on one GPU, bf16 or half; work is queued on torch's current stream of that GPU, memory comes
+from torch's allocator, nothing is read back, and every call may be captured into a CUDA graph.  Tokens of all sequences
+lie one behind the other: q is [tokens, heads, head_dim], k and v [tokens, kv_heads, head_dim], sequence s the rows
+cu_seqlens[s] .. cu_seqlens[s+1] - 1 (int32 on the GPU).  Views are fine as long as the last dimension is contiguous and
+rows begin on 16-byte boundaries.  There is no counterpart in the reference.
+"""
+from __future__ import annotations
+
+import ctypes as C
+from typing import Optional
+
+import torch
+
+from . import _lib
+from ._lib import SpammAttn, SpammError, check
+
+_DTYPES = {torch.bfloat16: 0, torch.float16: 1}
+_BLOCKS = (16, 32, 64, 128)
+
+
+def _rows(name: str, x: torch.Tensor, heads: Optional[int] = None, like: Optional[torch.Tensor] = None) -> torch.Tensor:
+    if not isinstance(x, torch.Tensor):
+        raise TypeError(f"{name} must be a torch tensor")
+    if x.dim() != 3:
+        raise ValueError(f"{name} must be [tokens, heads, head_dim], got {tuple(x.shape)}")
+    if x.dtype not in _DTYPES:
+        raise ValueError(f"{name} must be bfloat16 or float16, got {x.dtype}")
+    if x.shape[2] not in (64, 128):
+        raise ValueError(f"{name}: head_dim must be 64 or 128, got {x.shape[2]}")
+    if heads is not None and x.shape[1] != heads:
+        raise ValueError(f"{name} must have {heads} heads, got {x.shape[1]}")
+    if like is not None and (x.shape[0] != like.shape[0] or x.shape[2] != like.shape[2] or x.dtype != like.dtype
+                             or x.device != like.device):
+        raise ValueError(f"{name} must match in tokens, head_dim, dtype and device: {tuple(x.shape)} {x.dtype} {x.device} "
+                         f"against {tuple(like.shape)} {like.dtype} {like.device}")
+    if x.numel() and x.stride(2) != 1:
+        raise ValueError(f"{name}: the last dimension must be contiguous")
+    return x
+
+
+def _ints(name: str, x: torch.Tensor, shape, device) -> torch.Tensor:
+    if not isinstance(x, torch.Tensor) or x.dtype != torch.int32:
+        raise ValueError(f"{name} must be an int32 tensor")
+    if tuple(x.shape) != tuple(shape):
+        raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(x.shape)}")
+    if x.device != device:
+        raise ValueError(f"{name} must be on {device}, is on {x.device}")
+    if x.numel() and not x.is_contiguous():
+        raise ValueError(f"{name} must be contiguous")
+    return x
+
+
+def _host_int(name: str, x, least: int = 0) -> int:
+    if isinstance(x, torch.Tensor):
+        raise TypeError(f"{name} is a host-side number, not a tensor")
+    v = int(x)
+    if v != x or not least <= v < 2 ** 31:
+        raise ValueError(f"{name} must be a whole number of at least {least}, got {x}")
+    return v
+
+
+def _batch(cu_seqlens: torch.Tensor, device) -> int:
+    if not isinstance(cu_seqlens, torch.Tensor) or cu_seqlens.dim() != 1 or cu_seqlens.shape[0] < 1:
+        raise ValueError("cu_seqlens must be a tensor [batch + 1]")
+    _ints("cu_seqlens", cu_seqlens, cu_seqlens.shape, device)
+    return cu_seqlens.shape[0] - 1
+
+
+def _on_gpu(x: torch.Tensor) -> None:
+    if x.device.type != "cuda":
+        raise ValueError(f"tensors must be on a GPU, got {x.device}")
+
+
+def _strides(x: torch.Tensor):
+    """Token and head stride; those of a dimension of one element are never used and may be anything."""
+    return (x.stride(0) if x.shape[0] > 1 else 0), (x.stride(1) if x.shape[1] > 1 else 0)
+
+
+def _problem(q: torch.Tensor, kv_heads: int, cu_seqlens: torch.Tensor, max_q: int, block: int, query_block: int,
+             n_select: int, causal: bool) -> SpammAttn:
+    if block not in _BLOCKS:
+        raise ValueError(f"block must be one of {_BLOCKS}, got {block}")
+    if kv_heads < 1 or q.shape[1] % kv_heads or not 1 <= q.shape[1] // kv_heads <= 128:
+        raise ValueError(f"{q.shape[1]} query heads for {kv_heads} key heads: must be a multiple, 1 to 128 times")
+    a = SpammAttn()
+    a.dtype = _DTYPES[q.dtype]
+    a.batch = _batch(cu_seqlens, q.device)
+    a.heads, a.kv_heads, a.dim = q.shape[1], kv_heads, q.shape[2]
+    a.block, a.query_block, a.n_select = block, query_block, n_select
+    a.causal, a.max_q, a.tokens, a.zero_tail = bool(causal), max_q, q.shape[0], 1
+    a.scale = 1.0
+    a.d_cu = cu_seqlens.data_ptr()
+    a.d_q = q.data_ptr()
+    a.q_token, a.q_head = _strides(q)
+    return a
+
+
+def _set_keys(a: SpammAttn, k: torch.Tensor, v: Optional[torch.Tensor]) -> None:
+    a.d_k = k.data_ptr()
+    a.k_token, a.k_head = _strides(k)
+    if v is not None:
+        a.d_v = v.data_ptr()
+        a.v_token, a.v_head = _strides(v)
+
+
+def _set_out(a: SpammAttn, o: torch.Tensor) -> None:
+    a.d_o = o.data_ptr()
+    a.o_token, a.o_head = _strides(o)
+
+
+def _set_lists(a: SpammAttn, lists: torch.Tensor, device) -> None:
+    if not isinstance(lists, torch.Tensor) or lists.dim() != 4:
+        raise ValueError("lists must be a tensor [batch, query blocks, kv_heads, n_select]")
+    if not 1 <= lists.shape[3] <= 1024:
+        raise ValueError(f"lists of {lists.shape[3]} entries: 1 to 1024 are possible")
+    _ints("lists", lists, (a.batch, -(-a.max_q // a.query_block), a.kv_heads, lists.shape[3]), device)
+    a.n_select = lists.shape[3]
+    a.d_lists = lists.data_ptr()
+
+
+def _scratch(nbytes: int, device):
+    t = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+    return t, (t.data_ptr() if nbytes else None)
+
+
+def _scale(scale, head_dim: int) -> float:
+    s = head_dim ** -0.5 if scale is None else float(scale)
+    if not 0.0 < s < 3e38:
+        raise ValueError(f"scale must be a positive number, got {scale}")
+    return s
+
+
+def _stream(device) -> int:
+    return torch.cuda.current_stream(device).cuda_stream
+
+
+def _select(a: SpammAttn, q: torch.Tensor, key_sums: Optional[torch.Tensor], n_select, n_first, n_local) -> torch.Tensor:
+    lib = _lib.load()
+    forced = n_first + (n_local + (a.query_block + a.block - 2) // a.block if n_local else 0)
+    if not 1 <= n_select <= 1024 or n_select < forced:
+        raise ValueError(f"n_select must be 1 to 1024 and hold the {forced} first and local blocks, got {n_select}")
+    _on_gpu(q)
+    with torch.cuda.device(q.device):
+        lists = torch.empty((a.batch, -(-a.max_q // a.query_block), a.kv_heads, n_select), dtype=torch.int32, device=q.device)
+        n = lib.spamm_attn_select_scratch_bytes(C.byref(a))
+        scratch, ptr = _scratch(n, q.device)
+        check(lib.spamm_attn_select_dev(C.byref(a), key_sums.data_ptr() if key_sums is not None else None, n_first, n_local,
+                                        lists.data_ptr(), ptr, n, _stream(q.device)), "spamm_attn_select_dev")
+    return lists
+
+
+def _forward(a: SpammAttn, device) -> None:
+    lib = _lib.load()
+    n = lib.spamm_attn_forward_scratch_bytes(C.byref(a))
+    scratch, ptr = _scratch(n, device)
+    check(lib.spamm_attn_forward_dev(C.byref(a), ptr, n, _stream(device)), "spamm_attn_forward_dev")
+
+
+def select_blocks(q: torch.Tensor, k: torch.Tensor, cu_seqlens: torch.Tensor, max_seqlen: int, n_select: int, *,
+                  block: int = 64, query_block: int = 64, n_first: int = 1, n_local: int = 1,
+                  causal: bool = True) -> torch.Tensor:
+    """Lists of the `n_select` blocks of `block` keys with the largest scores, one list for every `query_block`
+    consecutive queries (1: every query its own) and key head: int32 [batch, ceil(max_seqlen / query_block), kv_heads,
+    n_select], ascending, -1 behind.  The score of a block is the sum of the queries (over the query block and the heads
+    of the key head) times the block's mean key; it is taken in double, ties go to the lower block.  The first `n_first`
+    blocks and those from `n_local` - 1 before the first query's to the last query's own are always taken.  No sequence
+    may be longer than `max_seqlen`.  The choice is not differentiable."""
+    _rows("q", q)
+    _rows("k", k)
+    _rows("k", k, like=q)
+    a = _problem(q, k.shape[1], cu_seqlens, _host_int("max_seqlen", max_seqlen), _host_int("block", block),
+                 _host_int("query_block", query_block, 1), _host_int("n_select", n_select, 1), causal)
+    _set_keys(a, k, None)
+    return _select(a, q, None, a.n_select, _host_int("n_first", n_first), _host_int("n_local", n_local))
+
+
+class _BlockSparseAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, lists, cu_seqlens, max_seqlen, block, query_block, causal, scale):
+        a = _problem(q, k.shape[1], cu_seqlens, max_seqlen, block, query_block, 0, causal)
+        a.scale = scale
+        _set_keys(a, k, v)
+        _set_lists(a, lists, q.device)
+        _on_gpu(q)
+        with torch.cuda.device(q.device):
+            o = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+            lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device)
+            _set_out(a, o)
+            a.d_lse = lse.data_ptr()
+            if not a.batch or not a.max_q:
+                o.zero_()
+                lse.fill_(float("-inf"))
+            _forward(a, q.device)
+        ctx.save_for_backward(q, k, v, lists, cu_seqlens, o, lse)
+        ctx.how = (max_seqlen, block, query_block, causal, scale)
+        ctx.mark_non_differentiable(lse)
+        return o, lse
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, d_o, _):
+        q, k, v, lists, cu_seqlens, o, lse = ctx.saved_tensors
+        max_seqlen, block, query_block, causal, scale = ctx.how
+        a = _problem(q, k.shape[1], cu_seqlens, max_seqlen, block, query_block, 0, causal)
+        a.scale = scale
+        _set_keys(a, k, v)
+        _set_lists(a, lists, q.device)
+        _set_out(a, o)
+        a.d_lse = lse.data_ptr()
+        # an expanded or oddly laid out gradient (the sum's, for one) is brought into rows first
+        if d_o.numel() and (d_o.stride(2) != 1 or d_o.data_ptr() % 16 or any(st % 8 for st in _strides(d_o))):
+            d_o = d_o.contiguous()
+        lib = _lib.load()
+        with torch.cuda.device(q.device):
+            dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+            dk = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+            dv = torch.empty(v.shape, dtype=v.dtype, device=v.device)
+            n = lib.spamm_attn_backward_scratch_bytes(C.byref(a))
+            scratch, ptr = _scratch(n, q.device)
+            check(lib.spamm_attn_backward_dev(C.byref(a), d_o.data_ptr(), *_strides(d_o), dq.data_ptr(), dk.data_ptr(),
+                                              dv.data_ptr(), ptr, n, _stream(q.device)), "spamm_attn_backward_dev")
+        return dq, dk, dv, None, None, None, None, None, None, None
+
+
+def block_sparse_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lists: torch.Tensor, cu_seqlens: torch.Tensor,
+                           max_seqlen: int, *, block: int = 64, query_block: int = 64, causal: bool = True,
+                           scale: Optional[float] = None, return_lse: bool = False):
+    """Attention of every query over the keys of the blocks on its query block's list (`lists` as `select_blocks` gives
+    them; an entry that is no block of the sequence, or not above every entry before it, is skipped), with `causal` over
+    those up to its own position.  `scale` multiplies q.k (default head_dim ** -0.5).  A query that sees no key gets
+    zeros.  Returns o [tokens, heads, head_dim], with `return_lse` also the log of the sum of exp(scale * q.k) per query
+    and head (float, not differentiable).  Differentiable once in q, k and v; two backward passes give the same bits."""
+    _rows("q", q)
+    _rows("k", k)
+    _rows("k", k, like=q)
+    _rows("v", v, heads=k.shape[1], like=q)
+    o, lse = _BlockSparseAttention.apply(q, k, v, lists, cu_seqlens, _host_int("max_seqlen", max_seqlen),
+                                         _host_int("block", block), _host_int("query_block", query_block, 1), bool(causal),
+                                         _scale(scale, q.shape[2]))
+    return (o, lse) if return_lse else o
+
+
+class PagedCache:
+    """Keys and values of many sequences in pages of `page_size` tokens, with the sum of the keys of every page.
+
+    k, v: [n_pages, kv_heads, page_size, head_dim]; key_sums: float [n_pages, kv_heads, head_dim].  The caller hands out
+    the pages: the page of tokens b * page_size .. of sequence s is page_table[s, b] (int32 [batch, width]), and
+    lengths[s] (int32) tokens are held, counting the new ones of the call: the same two tensors serve `append`, `select`
+    and `attend` of one step.
+
+    What the tables say is checked on the GPU: a page outside the cache is read as masked and never written, a length
+    beyond the table's width is cut, more new tokens than `max_new` or than the length holds are left out; `check()`
+    reports any of these since the last report.  No two sequences may append to the same page in one call; reading a
+    shared page is fine."""
+
+    def __init__(self, k: torch.Tensor, v: torch.Tensor, key_sums: Optional[torch.Tensor] = None):
+        for name, x in (("k", k), ("v", v)):
+            if not isinstance(x, torch.Tensor) or x.dim() != 4 or x.dtype not in _DTYPES or not x.is_contiguous():
+                raise ValueError(f"{name} must be a contiguous bfloat16 or float16 tensor [n_pages, kv_heads, page_size, head_dim]")
+        if k.shape != v.shape or k.dtype != v.dtype or k.device != v.device:
+            raise ValueError("k and v must match in shape, dtype and device")
+        if k.shape[0] < 1 or k.shape[1] < 1 or k.shape[2] not in _BLOCKS or k.shape[3] not in (64, 128):
+            raise ValueError(f"page size must be one of {_BLOCKS}, head_dim 64 or 128, got {tuple(k.shape)}")
+        sums = (k.shape[0], k.shape[1], k.shape[3])
+        if key_sums is not None and (key_sums.dtype != torch.float32 or tuple(key_sums.shape) != sums
+                                     or key_sums.device != k.device or not key_sums.is_contiguous()):
+            raise ValueError(f"key_sums must be a contiguous float32 tensor {sums} beside k")
+        _on_gpu(k)
+        self.k, self.v = k, v
+        self.key_sums = torch.zeros(sums, dtype=torch.float32, device=k.device) if key_sums is None else key_sums
+        self.status = torch.zeros(1, dtype=torch.int32, device=k.device)
+
+    @classmethod
+    def empty(cls, n_pages: int, kv_heads: int, head_dim: int, page_size: int = 64, dtype=torch.bfloat16,
+              device="cuda") -> "PagedCache":
+        shape = (n_pages, kv_heads, page_size, head_dim)
+        return cls(torch.zeros(shape, dtype=dtype, device=device), torch.zeros(shape, dtype=dtype, device=device))
+
+    @property
+    def page_size(self) -> int:
+        return self.k.shape[2]
+
+    def check(self) -> None:
+        """Waits for the GPU and raises SpammError when a call met a page, a length or a number of new tokens out of
+        range since the last report."""
+        st = int(self.status.item())
+        if st:
+            self.status.zero_()
+            raise SpammError(st, "PagedCache")
+
+    def _problem(self, q, cu_seqlens, max_new, page_table, lengths, query_block, n_select, causal) -> SpammAttn:
+        if q.dtype != self.k.dtype or q.shape[2] != self.k.shape[3] or q.device != self.k.device:
+            raise ValueError("tokens must match the cache in dtype, head_dim and device")
+        a = _problem(q, self.k.shape[1], cu_seqlens, _host_int("max_new", max_new), self.page_size,
+                     _host_int("query_block", query_block, 1), n_select, causal)
+        _ints("lengths", lengths, (a.batch,), q.device)
+        if not isinstance(page_table, torch.Tensor) or page_table.dim() != 2 or page_table.dtype != torch.int32 \
+                or page_table.shape[0] != a.batch or page_table.device != q.device:
+            raise ValueError("page_table must be an int32 tensor [batch, pages of the longest sequence] beside the tokens")
+        if page_table.shape[1] > 1 and page_table.stride(1) != 1:
+            raise ValueError("page_table: the last dimension must be contiguous")
+        if page_table.shape[0] > 1 and page_table.shape[1] and page_table.stride(0) < page_table.shape[1]:
+            raise ValueError("page_table: rows must not overlap")
+        a.n_pages, a.table_width = self.k.shape[0], page_table.shape[1]
+        a.table_stride = max(page_table.stride(0), page_table.shape[1]) if page_table.shape[0] > 1 else page_table.shape[1]
+        a.d_table, a.d_lengths, a.d_status = page_table.data_ptr(), lengths.data_ptr(), self.status.data_ptr()
+        return a
+
+    def append(self, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor, max_new: int, page_table: torch.Tensor,
+               lengths: torch.Tensor, inv_freq: Optional[torch.Tensor] = None, interleaved: bool = False,
+               q: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
+        """Writes the new tokens' keys and values to their pages: token i of n new ones of sequence s to position
+        lengths[s] - n + i.  With `inv_freq` (float32 [n], n a multiple of 8, 2 n <= head_dim) keys are rotated by
+        position * inv_freq on the way, pairs (j, j + n) of each head or, `interleaved`, (2j, 2j + 1); `q` is rotated
+        likewise and returned as a new tensor.  The key sums of the touched pages are taken anew from all keys that they
+        hold, so that tokens may be appended again after `lengths` went back."""
+        _rows("k", k, heads=self.k.shape[1])
+        _rows("v", v, heads=self.k.shape[1], like=k)
+        if q is not None:
+            _rows("q", q, like=k)
+        if inv_freq is not None:
+            if not isinstance(inv_freq, torch.Tensor) or inv_freq.dtype != torch.float32 or inv_freq.dim() != 1 \
+                    or not inv_freq.is_contiguous() or inv_freq.device != k.device:
+                raise ValueError("inv_freq must be a contiguous float32 tensor beside the tokens")
+            if inv_freq.shape[0] % 8 or 2 * inv_freq.shape[0] > k.shape[2] or not inv_freq.shape[0]:
+                raise ValueError(f"inv_freq must have a multiple of 8 values, at most head_dim / 2, got {inv_freq.shape[0]}")
+        a = self._problem(k if q is None else q, cu_seqlens, max_new, page_table, lengths, 1, 0, True)
+        _set_keys(a, k, v)
+        lib = _lib.load()
+        with torch.cuda.device(k.device):
+            out = None
+            if q is not None:
+                out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+                _set_out(a, out)
+                if not a.batch or not a.max_q:
+                    out.zero_()
+            check(lib.spamm_attn_append_dev(C.byref(a), self.k.data_ptr(), self.v.data_ptr(), self.key_sums.data_ptr(),
+                                            inv_freq.data_ptr() if inv_freq is not None else None,
+                                            inv_freq.shape[0] if inv_freq is not None else 0, int(bool(interleaved)),
+                                            _stream(k.device)), "spamm_attn_append_dev")
+        return out
+
+    def select(self, q: torch.Tensor, cu_seqlens: torch.Tensor, max_new: int, page_table: torch.Tensor, lengths: torch.Tensor,
+               n_select: int, query_block: int = 1, n_first: int = 1, n_local: int = 1) -> torch.Tensor:
+        """`select_blocks` for the newest tokens over the cached pages, by the cache's key sums."""
+        _rows("q", q)
+        a = self._problem(q, cu_seqlens, max_new, page_table, lengths, query_block, _host_int("n_select", n_select, 1), True)
+        a.d_k = self.k.data_ptr()
+        return _select(a, q, self.key_sums, a.n_select, _host_int("n_first", n_first), _host_int("n_local", n_local))
+
+    def attend(self, q: torch.Tensor, cu_seqlens: torch.Tensor, max_new: int, page_table: torch.Tensor, lengths: torch.Tensor,
+               lists: Optional[torch.Tensor] = None, query_block: int = 1, scale: Optional[float] = None,
+               out: Optional[torch.Tensor] = None, return_lse: bool = False):
+        """Attention of the newest tokens (one of each sequence or a whole chunk) over the cached keys up to their own,
+        of all pages or, with `lists` (as `select` gives them, for the same `query_block`), of the listed ones.  With
+        `out` the result goes there, and its rows that belong to no sequence are left as they are; else they are zero."""
+        _rows("q", q)
+        a = self._problem(q, cu_seqlens, max_new, page_table, lengths, query_block, 0, True)
+        a.scale = _scale(scale, q.shape[2])
+        a.d_k, a.d_v = self.k.data_ptr(), self.v.data_ptr()
+        if lists is not None:
+            _set_lists(a, lists, q.device)
+        with torch.cuda.device(q.device):
+            if out is None:
+                out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+                if not a.batch or not a.max_q:
+                    out.zero_()
+            else:
+                _rows("out", out, heads=q.shape[1], like=q)
+                if any(n > 1 and st == 0 for n, st in zip(out.shape, out.stride())):
+                    raise ValueError("out: rows must not overlap")
+                a.zero_tail = 0
+            _set_out(a, out)
+            lse = None
+            if return_lse:
+                lse = torch.full(q.shape[:2], float("-inf"), dtype=torch.float32, device=q.device)
+                a.d_lse = lse.data_ptr()
+            _forward(a, q.device)
+        return (out, lse) if return_lse else out

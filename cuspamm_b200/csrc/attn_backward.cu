@@ -1,0 +1,657 @@
+// Attention over listed blocks, backward.  With p_ij = exp(scale q_i.k_j - lse_i) again (nothing of the forward is kept
+// but o and lse) and delta_i = do_i.o_i:
+//
+//   ds_ij = p_ij (do_i.v_j - delta_i) scale,   dq_i = sum_j ds_ij k_j,   dk_j = sum_i ds_ij q_i,   dv_j = sum_i p_ij do_i
+//
+// dq walks the lists as the forward does.  dk and dv need, for every block of keys, the query blocks that list it: the
+// lists are turned over into one bit per (block of keys, query block), so that every block of keys is one work item that
+// sums over its queries in ascending order and writes its rows once.  No atomics on gradients: the same inputs give the
+// same bits.  A block that very many queries list (the first one often is on every list) is cut into items of `chunk`
+// query blocks each, whose float partial sums a last kernel adds up in order.
+#include "attn.cuh"
+
+namespace spamm {
+
+struct BackwardPlan {
+    int nqb, nkb, words;        // query blocks, blocks of keys, 32-bit words of a block's bits
+    int chunk;                  // query blocks of a work item
+    int item_cap, slot_cap;     // items and partial sums of one (sequence, key head)
+    int64_t groups;             // batch * kv_heads
+    size_t delta, bits, counts, slots, items, n_items, partial, bytes;   // scratch offsets
+};
+
+struct Item {
+    int kb, chunk, slot, pad;   // block of keys, which chunk of its query blocks, partial sum to write (-1: the rows)
+};
+
+static BackwardPlan backward_plan(const spamm_attn &a)
+{
+    BackwardPlan p;
+    const int G = a.heads / a.kv_heads;
+    p.nqb = attn_query_blocks(a);
+    p.nkb = ceil_div(a.max_q, a.block);
+    p.words = ceil_div(p.nqb, 32);
+    const int64_t rows = (int64_t)min(a.query_block, a.max_q) * G;
+    p.chunk = (int)max((int64_t)1, min((int64_t)1024, 8192 / rows));
+    const int64_t pairs = (int64_t)p.nqb * min(a.n_select, p.nkb);
+    p.item_cap = (int)min((int64_t)INT32_MAX / 4, p.nkb + pairs / p.chunk);
+    p.slot_cap = (int)min((int64_t)INT32_MAX / 4, 2 * pairs / p.chunk);
+    p.groups = (int64_t)a.batch * a.kv_heads;
+    size_t at = 0;
+    auto take = [&](size_t n) { const size_t o = at; at += (n + 255) / 256 * 256; return o; };
+    p.delta = take((size_t)a.tokens * a.heads * 4);
+    p.bits = take((size_t)p.groups * p.nkb * p.words * 4);          // bits and counts are cleared together
+    p.counts = take((size_t)p.groups * p.nkb * 4);
+    p.slots = take((size_t)p.groups * p.nkb * 4);
+    p.items = take((size_t)p.groups * p.item_cap * sizeof(Item));
+    p.n_items = take((size_t)p.groups * 4);
+    p.partial = take((size_t)p.groups * p.slot_cap * a.block * a.dim * 2 * 4);
+    p.bytes = at;
+    return p;
+}
+
+// delta = do.o for every row; a quarter of a warp for each.  Rows of no sequence get zero gradients here.
+template <typename T, int D>
+__global__ __launch_bounds__(256) void attn_delta_kernel(const __grid_constant__ spamm_attn a, const T *d_do, int64_t do_token,
+                                                         int64_t do_head, float *delta, T *dq, T *dk, T *dv)
+{
+    const int sub = threadIdx.x & 7;
+    const int64_t w = (int64_t)blockIdx.x * 32 + (threadIdx.x >> 3);
+    if (w >= (int64_t)a.tokens * a.heads) return;
+    const int row = (int)(w / a.heads), head = (int)(w % a.heads);
+    // the sequence that holds the row
+    int lo = 0, hi = a.batch;
+    while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (a.d_cu[mid + 1] > row) hi = mid; else lo = mid + 1;
+    }
+    bool held = lo < a.batch;
+    if (held) {
+        const Seq sq = attn_seq(a, lo);
+        held = row >= sq.row0 && row < sq.row0 + sq.nq;
+    }
+    if (!held) {
+        const uint4 z = make_uint4(0, 0, 0, 0);
+        const int G = a.heads / a.kv_heads;
+        for (int c = sub; c < D / 8; c += 8) {
+            reinterpret_cast<uint4 *>(dq + ((int64_t)row * a.heads + head) * D)[c] = z;
+            if (head % G == 0) {
+                reinterpret_cast<uint4 *>(dk + ((int64_t)row * a.kv_heads + head / G) * D)[c] = z;
+                reinterpret_cast<uint4 *>(dv + ((int64_t)row * a.kv_heads + head / G) * D)[c] = z;
+            }
+        }
+        return;
+    }
+    float sum = 0.f;
+#pragma unroll
+    for (int c = 0; c < D / 64; c++) {
+        const int d = (c * 8 + sub) * 8;
+        const uint4 x = *reinterpret_cast<const uint4 *>(d_do + row * do_token + head * do_head + d);
+        const uint4 y = *reinterpret_cast<const uint4 *>(static_cast<const T *>(a.d_o) + row * a.o_token + head * a.o_head + d);
+        const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const float2 u = Pack<T>::to2(xs[i]), v = Pack<T>::to2(ys[i]);
+            sum = fmaf(u.x, v.x, fmaf(u.y, v.y, sum));
+        }
+    }
+#pragma unroll
+    for (int d = 1; d < 8; d <<= 1) sum += __shfl_xor_sync(~0u, sum, d, 8);
+    if (sub == 0) delta[w] = sum;
+}
+
+// Turns the lists over: one warp reads a list and sets the bit of its query block in every listed block of keys.
+__global__ __launch_bounds__(128) void attn_turn_kernel(const __grid_constant__ spamm_attn a, int nqb, int nkb, int words,
+                                                        unsigned *bits, int *counts)
+{
+    __shared__ int lists[4][SPAMM_ATTN_MAX_SELECT];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t w = (int64_t)blockIdx.x * 4 + warp;
+    if (w >= (int64_t)a.batch * nqb * a.kv_heads) return;
+    const int h = (int)(w % a.kv_heads), qb = (int)(w / a.kv_heads % nqb), s = (int)(w / a.kv_heads / nqb);
+    const Seq sq = attn_seq(a, s);
+    const int last = min((int)min((int64_t)(qb + 1) * a.query_block, (int64_t)sq.nq), sq.nq) - 1;
+    if ((int64_t)qb * a.query_block >= sq.nq) return;
+    const int n = attn_load_list(a, s, qb, nqb, h, ceil_div(attn_limit(a, sq, last), a.block), lists[warp], lane);
+    const int64_t group = (int64_t)s * a.kv_heads + h;
+    for (int i = lane; i < n; i += 32) {
+        const int64_t at = group * nkb + lists[warp][i];
+        atomicOr(bits + at * words + (qb >> 5), 1u << (qb & 31));
+        atomicAdd(counts + at, 1);
+    }
+}
+
+// The work items of one (sequence, key head), in the order of the blocks: a running sum over the blocks of how many
+// items and partial sums each needs.
+__global__ __launch_bounds__(1024) void attn_items_kernel(const __grid_constant__ spamm_attn a, const BackwardPlan p,
+                                                          const int *counts, int *slots, Item *items, int *n_items)
+{
+    __shared__ int2 warp_sum[32];
+    __shared__ int2 carry;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int64_t group = blockIdx.x;
+    const int s = (int)(group / a.kv_heads);
+    const int n_blocks = ceil_div(attn_seq(a, s).nk, a.block);
+    if (tid == 0) carry = make_int2(0, 0);
+    __syncthreads();
+    for (int b0 = 0; b0 < n_blocks; b0 += 1024) {
+        const int b = b0 + tid;
+        const int n = b < n_blocks ? counts[group * p.nkb + b] : 0;
+        const int chunks = b < n_blocks ? max(1, ceil_div(n, p.chunk)) : 0;
+        int x = chunks, y = chunks > 1 ? chunks : 0;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const int u = __shfl_up_sync(~0u, x, d), v = __shfl_up_sync(~0u, y, d);
+            if (lane >= d) { x += u; y += v; }
+        }
+        if (lane == 31) warp_sum[warp] = make_int2(x, y);
+        __syncthreads();
+        if (warp == 0) {
+            int2 t = warp_sum[lane];
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) {
+                const int u = __shfl_up_sync(~0u, t.x, d), v = __shfl_up_sync(~0u, t.y, d);
+                if (lane >= d) { t.x += u; t.y += v; }
+            }
+            warp_sum[lane] = t;
+        }
+        __syncthreads();
+        const int2 c = carry, before = warp ? warp_sum[warp - 1] : make_int2(0, 0);
+        int at = c.x + before.x + x - chunks, slot = c.y + before.y + y - (chunks > 1 ? chunks : 0);
+        if (b < n_blocks) {
+            slots[group * p.nkb + b] = slot;
+            for (int i = 0; i < chunks; i++)
+                if (at + i < p.item_cap) items[group * p.item_cap + at + i] = Item{b, i, chunks > 1 ? slot + i : -1, 0};
+        }
+        __syncthreads();
+        if (tid == 0) carry = make_int2(c.x + warp_sum[31].x, c.y + warp_sum[31].y);
+        __syncthreads();
+    }
+    if (tid == 0) n_items[group] = min(carry.x, p.item_cap);
+}
+
+constexpr int DQ_STAGES = 3;
+constexpr int DQ_WARPS = 4;
+
+// dq of 16 rows (queries x heads) of one key head; the layout of attn_rows_kernel.
+template <typename T, int D>
+__global__ __launch_bounds__(128) void attn_dq_rows_kernel(const __grid_constant__ spamm_attn a, int nqb, int tiles, const T *d_do,
+                                                           int64_t do_token, int64_t do_head, const float *delta, T *dq)
+{
+    extern __shared__ __align__(128) uint8_t smem[];
+    constexpr int TILE16 = 16 * D * 2;
+    uint8_t *ring = smem;
+    uint8_t *q_tile = ring + DQ_WARPS * DQ_STAGES * 2 * TILE16;
+    uint8_t *do_tile = q_tile + TILE16;
+    int *blk = reinterpret_cast<int *>(do_tile + TILE16);
+    __shared__ int shared_count;
+
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    unsigned idx = blockIdx.x;
+    const int tile = idx % tiles; idx /= tiles;
+    const int qb = idx % nqb; idx /= nqb;
+    const int h = idx % a.kv_heads;
+    const int s = idx / a.kv_heads;
+    const int G = a.heads / a.kv_heads;
+    const Seq sq = attn_seq(a, s);
+    const int bq = min(a.query_block, a.max_q);
+    const int n_tok = min(bq, sq.nq - qb * bq);
+    const int64_t n_rows = (int64_t)max(n_tok, 0) * G;
+    if ((int64_t)tile * 16 >= n_rows) return;
+    const int rows = (int)min((int64_t)16, n_rows - tile * 16);
+    const int first_query = qb * bq + tile * 16 / G, last_query = qb * bq + (tile * 16 + rows - 1) / G;
+    const int limit_max = attn_limit(a, sq, last_query), limit_min = attn_limit(a, sq, first_query);
+
+    for (int i = tid; i < 16 * D / 8; i += 128) {
+        const int r = i / (D / 8), c = i % (D / 8);
+        const int x = tile * 16 + r;
+        const bool ok = r < rows;
+        const int64_t row = sq.row0 + qb * bq + (int64_t)(ok ? x / G : 0), head = h * G + (ok ? x % G : 0);
+        cp_async16(smem_addr(q_tile) + tile_off<D>(r, c), static_cast<const T *>(a.d_q) + row * a.q_token + head * a.q_head + c * 8, ok);
+        cp_async16(smem_addr(do_tile) + tile_off<D>(r, c), d_do + row * do_token + head * do_head + c * 8, ok);
+    }
+    cp_commit();
+    if (warp == 0) {
+        const int n = attn_load_list(a, s, qb, nqb, h, ceil_div(limit_max, a.block), blk, lane);
+        if (lane == 0) shared_count = n;
+    }
+    __syncthreads();
+    const int chunks_per_block = a.block >> 4;
+    const int n_chunks = shared_count * chunks_per_block;
+    const uint32_t my_ring = smem_addr(ring) + warp * DQ_STAGES * 2 * TILE16;
+
+    auto issue = [&](int c, int stage) {
+        if (c < n_chunks) {
+            const int e = c / chunks_per_block;
+            const int pos = blk[e] * a.block + (c - e * chunks_per_block) * 16;
+            const int n = min(16, limit_max - pos);
+            const T *kp = static_cast<const T *>(a.d_k) + (int64_t)(sq.row0 + pos) * a.k_token + h * a.k_head;
+            const T *vp = static_cast<const T *>(a.d_v) + (int64_t)(sq.row0 + pos) * a.v_token + h * a.v_head;
+            const uint32_t kt = my_ring + stage * 2 * TILE16, vt = kt + TILE16;
+#pragma unroll
+            for (int i = 0; i < 16 * D / 8 / 32; i++) {
+                const int x = i * 32 + lane, r = x / (D / 8), c8 = x % (D / 8);
+                const bool ok = r < n;
+                cp_async16(kt + tile_off<D>(r, c8), (ok ? kp + r * a.k_token : static_cast<const T *>(a.d_k)) + c8 * 8, ok);
+                cp_async16(vt + tile_off<D>(r, c8), (ok ? vp + r * a.v_token : static_cast<const T *>(a.d_v)) + c8 * 8, ok);
+            }
+        }
+        cp_commit();
+    };
+    for (int i = 0; i < DQ_STAGES - 1; i++) issue(warp + DQ_WARPS * i, i);
+    cp_wait<DQ_STAGES - 1>();
+    __syncthreads();
+    uint32_t qf[D / 16][4], df[D / 16][4];
+#pragma unroll
+    for (int ks = 0; ks < D / 16; ks++) {
+        a_frag<D>(smem_addr(q_tile), 0, ks, lane, qf[ks]);
+        a_frag<D>(smem_addr(do_tile), 0, ks, lane, df[ks]);
+    }
+    int limit[2];
+    float lse2[2], dl[2];
+#pragma unroll
+    for (int x = 0; x < 2; x++) {
+        const int r = (lane >> 2) + 8 * x;
+        const int y = tile * 16 + min(r, rows - 1);
+        const int64_t row = sq.row0 + qb * bq + y / G;
+        const int64_t at = row * a.heads + h * G + y % G;
+        limit[x] = attn_limit(a, sq, qb * bq + y / G);
+        const float z = a.d_lse[at];
+        lse2[x] = z == -CUDART_INF_F ? CUDART_INF_F : z * LOG2E;       // a row without keys: every p zero
+        dl[x] = delta[at];
+    }
+    const float scale2 = a.scale * LOG2E;
+    float o[D / 8][4] = {};
+    int stage = 0;
+    for (int c = warp; c < n_chunks; c += DQ_WARPS) {
+        issue(c + DQ_WARPS * (DQ_STAGES - 1), (stage + DQ_STAGES - 1) % DQ_STAGES);
+        cp_wait<DQ_STAGES - 1>();
+        __syncwarp();
+        const uint32_t kt = my_ring + stage * 2 * TILE16, vt = kt + TILE16;
+        stage = stage + 1 == DQ_STAGES ? 0 : stage + 1;
+        float sc[2][4] = {}, dp[2][4] = {};
+#pragma unroll
+        for (int ks = 0; ks < D / 16; ks++) {
+            uint32_t b[4];
+            b_frag2<D>(kt, 0, ks, lane, b);
+            mma16816<T>(sc[0], qf[ks], b[0], b[1]);
+            mma16816<T>(sc[1], qf[ks], b[2], b[3]);
+            b_frag2<D>(vt, 0, ks, lane, b);
+            mma16816<T>(dp[0], df[ks], b[0], b[1]);
+            mma16816<T>(dp[1], df[ks], b[2], b[3]);
+        }
+        const int p0 = blk[c / chunks_per_block] * a.block + (c % chunks_per_block) * 16;
+        const bool masked = p0 > limit_min - 16;
+#pragma unroll
+        for (int nt = 0; nt < 2; nt++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const int x = i >> 1;
+                float pr = fast_exp2(sc[nt][i] * scale2 - lse2[x]);
+                float ds = pr * (dp[nt][i] - dl[x]) * a.scale;
+                if (masked && p0 + nt * 8 + (lane & 3) * 2 + (i & 1) >= limit[x]) ds = 0.f;
+                sc[nt][i] = ds;
+            }
+        const uint32_t pf[4] = {Pack<T>::two(sc[0][0], sc[0][1]), Pack<T>::two(sc[0][2], sc[0][3]),
+                                Pack<T>::two(sc[1][0], sc[1][1]), Pack<T>::two(sc[1][2], sc[1][3])};
+#pragma unroll
+        for (int n = 0; n < D / 16; n++) {
+            uint32_t b[4];
+            bt_frag2<D>(kt, 0, n * 16, lane, b);
+            mma16816<T>(o[2 * n], pf, b[0], b[1]);
+            mma16816<T>(o[2 * n + 1], pf, b[2], b[3]);
+        }
+        __syncwarp();
+    }
+    cp_wait<0>();
+    __syncthreads();
+    float *so = reinterpret_cast<float *>(ring);
+#pragma unroll
+    for (int n = 0; n < D / 8; n++)
+#pragma unroll
+        for (int x = 0; x < 2; x++)
+            *reinterpret_cast<float2 *>(so + ((warp * 16 + (lane >> 2) + 8 * x) * D + n * 8 + (lane & 3) * 2)) =
+                make_float2(o[n][2 * x], o[n][2 * x + 1]);
+    __syncthreads();
+    const int r = tid >> 3, c0 = (tid & 7) * (D / 8);
+    if (r < rows) {
+        float y[D / 8] = {};
+#pragma unroll
+        for (int w = 0; w < DQ_WARPS; w++)
+#pragma unroll
+            for (int i = 0; i < D / 8; i++) y[i] += so[(w * 16 + r) * D + c0 + i];
+        uint32_t out[D / 16];
+#pragma unroll
+        for (int i = 0; i < D / 16; i++) out[i] = Pack<T>::two(y[2 * i], y[2 * i + 1]);
+        const int x = tile * 16 + r;
+        T *dst = dq + (((int64_t)sq.row0 + qb * bq + x / G) * a.heads + h * G + x % G) * D + c0;
+#pragma unroll
+        for (int i = 0; i < D / 64; i++) reinterpret_cast<uint4 *>(dst)[i] = *reinterpret_cast<uint4 *>(out + 4 * i);
+    }
+}
+
+constexpr int DKV_ROWS = 64;      // query rows of a shared-memory tile
+constexpr int DKV_STAGES = 2;
+
+// dk and dv of one block of keys from one chunk of the query blocks that list it.  A warp has 16 keys (and, when the
+// block is shorter than 64 keys, a share of the rows of every tile); it takes the transposed scores, keys x queries, so
+// that p and ds leave the products in the layout in which they enter the next ones.
+template <typename T, int D, int KEYS>
+__global__ __launch_bounds__(KEYS == 128 ? 256 : 128) void attn_dkv_kernel(
+    const __grid_constant__ spamm_attn a, const BackwardPlan p, const T *d_do, int64_t do_token, int64_t do_head,
+    const float *delta, const unsigned *bits, const Item *items, const int *n_items, float *partial, T *dk, T *dv)
+{
+    constexpr int THREADS = KEYS == 128 ? 256 : 128, WARPS = THREADS / 32;
+    constexpr int KG = KEYS / 16, RG = WARPS / KG;                 // groups of keys, groups of rows
+    constexpr int STEPS = DKV_ROWS / RG / 16;
+    constexpr int KT = KEYS * D * 2, RT = DKV_ROWS * D * 2;
+    extern __shared__ __align__(128) uint8_t smem[];
+    uint8_t *k_tile = smem, *v_tile = smem + KT;
+    uint8_t *ring = smem + 2 * KT;                                  // [stage][q | do]
+    float *row_lse = reinterpret_cast<float *>(ring + DKV_STAGES * 2 * RT);      // [stage][64]
+    float *row_delta = row_lse + DKV_STAGES * DKV_ROWS;
+    int *row_pos = reinterpret_cast<int *>(row_delta + DKV_STAGES * DKV_ROWS);
+    int *list = row_pos + DKV_STAGES * DKV_ROWS;                    // [chunk] query blocks
+    __shared__ int warp_sum[WARPS];
+
+    const int64_t group = blockIdx.x / p.item_cap;
+    const int item_i = blockIdx.x % p.item_cap;
+    if (item_i >= n_items[group]) return;
+    const Item item = items[group * p.item_cap + item_i];
+    const int s = (int)(group / a.kv_heads), h = (int)(group % a.kv_heads);
+    const Seq sq = attn_seq(a, s);
+    const int G = a.heads / a.kv_heads;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int pos0 = item.kb * KEYS;
+    const int keys = min(KEYS, sq.nk - pos0);
+
+    for (int i = tid; i < KEYS * D / 8; i += THREADS) {
+        const int r = i / (D / 8), c = i % (D / 8);
+        const bool ok = r < keys;
+        const int64_t row = sq.row0 + pos0 + (ok ? r : 0);
+        cp_async16(smem_addr(k_tile) + tile_off<D>(r, c), static_cast<const T *>(a.d_k) + row * a.k_token + h * a.k_head + c * 8, ok);
+        cp_async16(smem_addr(v_tile) + tile_off<D>(r, c), static_cast<const T *>(a.d_v) + row * a.v_token + h * a.v_head + c * 8, ok);
+    }
+    // the query blocks [chunk * p.chunk, ...) among the set bits
+    const unsigned *my_bits = bits + (group * p.nkb + item.kb) * p.words;
+    const int want0 = item.chunk * p.chunk, want1 = want0 + p.chunk;
+    int found = 0;
+    for (int w0 = 0; w0 < p.words && found < want1; w0 += THREADS) {
+        unsigned word = w0 + tid < p.words ? my_bits[w0 + tid] : 0;
+        const int n = __popc(word);
+        int run = n;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const int u = __shfl_up_sync(~0u, run, d);
+            if (lane >= d) run += u;
+        }
+        __syncthreads();
+        if (lane == 31) warp_sum[warp] = run;
+        __syncthreads();
+        int at = found + run - n, all = 0;
+        for (int w = 0; w < WARPS; w++) {
+            if (w < warp) at += warp_sum[w];
+            all += warp_sum[w];
+        }
+        while (word && at < want1) {
+            const int bit = __ffs(word) - 1;
+            word &= word - 1;
+            if (at >= want0) list[at - want0] = (w0 + tid) * 32 + bit;
+            at++;
+        }
+        found += all;
+    }
+    const int n_list = min(max(found - want0, 0), p.chunk);
+    __syncthreads();
+    const int bq = min(a.query_block, a.max_q);
+    const int per = bq * G;                                         // rows of a full query block
+    // all listed query blocks are full but the sequence's last one, which can only be the last of the list
+    const int64_t n_rows = n_list ? (int64_t)(n_list - 1) * per + (int64_t)min(bq, sq.nq - list[n_list - 1] * bq) * G : 0;
+    const int n_tiles = (int)((n_rows + DKV_ROWS - 1) / DKV_ROWS);
+
+    auto issue = [&](int t, int stage) {
+        if (t < n_tiles) {
+            const uint32_t qt = smem_addr(ring) + stage * 2 * RT, dt = qt + RT;
+            for (int i = tid; i < DKV_ROWS * D / 8; i += THREADS) {
+                const int r = i / (D / 8), c = i % (D / 8);
+                const int64_t x = (int64_t)t * DKV_ROWS + r;
+                const bool ok = x < n_rows;
+                const int e = ok ? (int)(x / per) : 0, y = ok ? (int)(x - (int64_t)e * per) : 0;
+                const int query = list[e] * bq + y / G, head = h * G + y % G;
+                const int64_t row = sq.row0 + query;
+                cp_async16(qt + tile_off<D>(r, c), static_cast<const T *>(a.d_q) + row * a.q_token + head * a.q_head + c * 8, ok);
+                cp_async16(dt + tile_off<D>(r, c), d_do + row * do_token + head * do_head + c * 8, ok);
+                if (c == 0) {
+                    const float z = ok ? a.d_lse[row * a.heads + head] : -CUDART_INF_F;
+                    row_lse[stage * DKV_ROWS + r] = z == -CUDART_INF_F ? CUDART_INF_F : z * LOG2E;
+                    row_delta[stage * DKV_ROWS + r] = ok ? delta[row * a.heads + head] : 0.f;
+                    row_pos[stage * DKV_ROWS + r] = ok ? (a.causal ? query : INT32_MAX) : -1;
+                }
+            }
+        }
+        cp_commit();
+    };
+    const int kg = warp % KG, rg = warp / KG;
+    const float scale2 = a.scale * LOG2E;
+    float ak[D / 8][4] = {}, av[D / 8][4] = {};
+    issue(0, 0);
+    for (int t = 0; t < n_tiles; t++) {
+        issue(t + 1, (t + 1) & 1);
+        cp_wait<1>();
+        __syncthreads();
+        const int stage = t & 1;
+        const uint32_t qt = smem_addr(ring) + stage * 2 * RT, dt = qt + RT;
+        const uint32_t kt = smem_addr(k_tile), vt = smem_addr(v_tile);
+#pragma unroll 1
+        for (int step = 0; step < STEPS; step++) {
+            const int r0 = (rg * STEPS + step) * 16;
+            float sc[2][4] = {}, dp[2][4] = {};
+#pragma unroll
+            for (int ks = 0; ks < D / 16; ks++) {
+                uint32_t x[4], b[4];
+                a_frag<D>(kt, kg * 16, ks, lane, x);
+                b_frag2<D>(qt, r0, ks, lane, b);
+                mma16816<T>(sc[0], x, b[0], b[1]);
+                mma16816<T>(sc[1], x, b[2], b[3]);
+                a_frag<D>(vt, kg * 16, ks, lane, x);
+                b_frag2<D>(dt, r0, ks, lane, b);
+                mma16816<T>(dp[0], x, b[0], b[1]);
+                mma16816<T>(dp[1], x, b[2], b[3]);
+            }
+#pragma unroll
+            for (int nt = 0; nt < 2; nt++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const int r = stage * DKV_ROWS + r0 + nt * 8 + (lane & 3) * 2 + (i & 1);
+                    const int key = kg * 16 + (lane >> 2) + 8 * (i >> 1);
+                    const bool ok = key < keys && pos0 + key <= row_pos[r];
+                    const float pr = ok ? fast_exp2(sc[nt][i] * scale2 - row_lse[r]) : 0.f;
+                    dp[nt][i] = ok ? pr * (dp[nt][i] - row_delta[r]) * a.scale : 0.f;
+                    sc[nt][i] = pr;
+                }
+            const uint32_t pf[4] = {Pack<T>::two(sc[0][0], sc[0][1]), Pack<T>::two(sc[0][2], sc[0][3]),
+                                    Pack<T>::two(sc[1][0], sc[1][1]), Pack<T>::two(sc[1][2], sc[1][3])};
+            const uint32_t sf[4] = {Pack<T>::two(dp[0][0], dp[0][1]), Pack<T>::two(dp[0][2], dp[0][3]),
+                                    Pack<T>::two(dp[1][0], dp[1][1]), Pack<T>::two(dp[1][2], dp[1][3])};
+#pragma unroll
+            for (int n = 0; n < D / 16; n++) {
+                uint32_t b[4];
+                bt_frag2<D>(dt, r0, n * 16, lane, b);
+                mma16816<T>(av[2 * n], pf, b[0], b[1]);
+                mma16816<T>(av[2 * n + 1], pf, b[2], b[3]);
+                bt_frag2<D>(qt, r0, n * 16, lane, b);
+                mma16816<T>(ak[2 * n], sf, b[0], b[1]);
+                mma16816<T>(ak[2 * n + 1], sf, b[2], b[3]);
+            }
+        }
+        __syncthreads();
+    }
+    cp_wait<0>();
+    __syncthreads();
+    // the row groups' sums are added in order through shared memory: [KEYS][D] of dk, then of dv (in place of the tiles)
+    float *sk = reinterpret_cast<float *>(smem), *sv = sk + KEYS * D;
+    for (int g = 0; g < RG; g++) {
+        if (rg == g)
+#pragma unroll
+            for (int n = 0; n < D / 8; n++)
+#pragma unroll
+                for (int x = 0; x < 2; x++) {
+                    const int at = (kg * 16 + (lane >> 2) + 8 * x) * D + n * 8 + (lane & 3) * 2;
+                    float2 *pk = reinterpret_cast<float2 *>(sk + at), *pv = reinterpret_cast<float2 *>(sv + at);
+                    float2 k2 = make_float2(ak[n][2 * x], ak[n][2 * x + 1]), v2 = make_float2(av[n][2 * x], av[n][2 * x + 1]);
+                    if (g) {
+                        k2.x += pk->x; k2.y += pk->y;
+                        v2.x += pv->x; v2.y += pv->y;
+                    }
+                    *pk = k2;
+                    *pv = v2;
+                }
+        __syncthreads();
+    }
+    if (item.slot >= 0) {
+        float *dst = partial + (group * p.slot_cap + item.slot) * (int64_t)(2 * KEYS * D);
+        for (int i = tid; i < 2 * KEYS * D / 4; i += THREADS)
+            reinterpret_cast<float4 *>(dst)[i] = reinterpret_cast<float4 *>(sk)[i];
+        return;
+    }
+    for (int i = tid; i < keys * D / 8; i += THREADS) {
+        const int r = i / (D / 8), c = i % (D / 8) * 8;
+        const int64_t at = ((int64_t)(sq.row0 + pos0 + r) * a.kv_heads + h) * D + c;
+        uint32_t x[4], y[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            x[j] = Pack<T>::two(sk[r * D + c + 2 * j], sk[r * D + c + 2 * j + 1]);
+            y[j] = Pack<T>::two(sv[r * D + c + 2 * j], sv[r * D + c + 2 * j + 1]);
+        }
+        *reinterpret_cast<uint4 *>(dk + at) = *reinterpret_cast<uint4 *>(x);
+        *reinterpret_cast<uint4 *>(dv + at) = *reinterpret_cast<uint4 *>(y);
+    }
+}
+
+// Adds up the partial sums of the blocks of keys that were cut into several items.
+template <typename T>
+__global__ __launch_bounds__(128) void attn_dkv_join_kernel(const __grid_constant__ spamm_attn a, const BackwardPlan p,
+                                                            const int *counts, const int *slots, const float *partial,
+                                                            T *dk, T *dv)
+{
+    const int64_t group = blockIdx.x / p.nkb;
+    const int kb = blockIdx.x % p.nkb;
+    const int s = (int)(group / a.kv_heads), h = (int)(group % a.kv_heads);
+    const Seq sq = attn_seq(a, s);
+    const int keys = min(a.block, sq.nk - kb * a.block);
+    const int chunks = keys > 0 ? ceil_div(counts[group * p.nkb + kb], p.chunk) : 0;
+    if (chunks <= 1) return;
+    const int64_t tile = 2 * (int64_t)a.block * a.dim;
+    const float *src = partial + (group * p.slot_cap + slots[group * p.nkb + kb]) * tile;
+    for (int i = threadIdx.x; i < 2 * keys * a.dim / 4; i += 128) {
+        const int which = i >= keys * a.dim / 4;
+        const int x = (i - which * (keys * a.dim / 4)) * 4;
+        float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int c = 0; c < chunks; c++) {
+            const float4 z = *reinterpret_cast<const float4 *>(src + c * tile + which * a.block * a.dim + x);
+            y.x += z.x; y.y += z.y; y.z += z.z; y.w += z.w;
+        }
+        T *dst = (which ? dv : dk) + ((int64_t)(sq.row0 + kb * a.block + x / a.dim) * a.kv_heads + h) * a.dim + x % a.dim;
+        *reinterpret_cast<uint2 *>(dst) = make_uint2(Pack<T>::two(y.x, y.y), Pack<T>::two(y.z, y.w));
+    }
+}
+
+template <typename T, int D, int KEYS>
+static int dkv_launch(const spamm_attn &a, const BackwardPlan &p, const T *d_do, int64_t do_token, int64_t do_head,
+                      const float *delta, const unsigned *bits, const Item *items, const int *n_items, float *partial, T *dk,
+                      T *dv, cudaStream_t stream)
+{
+    const size_t tiles = (size_t)2 * KEYS * D * 2 + DKV_STAGES * 2 * DKV_ROWS * D * 2 + DKV_STAGES * DKV_ROWS * 12 + p.chunk * 4;
+    const size_t sums = (size_t)2 * KEYS * D * 4;
+    const size_t smem = max(tiles, sums);
+    int st = attn_set_smem((const void *)attn_dkv_kernel<T, D, KEYS>, smem);
+    if (st) return st;
+    attn_dkv_kernel<T, D, KEYS><<<(unsigned)(p.groups * p.item_cap), KEYS == 128 ? 256 : 128, smem, stream>>>(
+        a, p, d_do, do_token, do_head, delta, bits, items, n_items, partial, dk, dv);
+    return SPAMM_OK;
+}
+
+template <typename T, int D>
+static int backward_launch(const spamm_attn &a, const BackwardPlan &p, const T *d_do, int64_t do_token, int64_t do_head, T *dq,
+                           T *dk, T *dv, uint8_t *scratch, cudaStream_t stream)
+{
+    float *delta = reinterpret_cast<float *>(scratch + p.delta);
+    unsigned *bits = reinterpret_cast<unsigned *>(scratch + p.bits);
+    int *counts = reinterpret_cast<int *>(scratch + p.counts), *slots = reinterpret_cast<int *>(scratch + p.slots);
+    Item *items = reinterpret_cast<Item *>(scratch + p.items);
+    int *n_items = reinterpret_cast<int *>(scratch + p.n_items);
+    float *partial = reinterpret_cast<float *>(scratch + p.partial);
+    const int64_t rows = (int64_t)a.tokens * a.heads, lists = (int64_t)a.batch * p.nqb * a.kv_heads;
+    const int bq = min(a.query_block, a.max_q);
+    const int tiles = (int)(((int64_t)bq * (a.heads / a.kv_heads) + 15) / 16);
+    const int64_t dq_grid = p.groups * p.nqb * tiles;
+    if ((rows + 31) / 32 > INT32_MAX || (lists + 3) / 4 > INT32_MAX || dq_grid > INT32_MAX || p.groups * p.item_cap > INT32_MAX ||
+        p.groups * p.nkb > INT32_MAX)
+        return attn_too_large();
+
+    SPAMM_CUDA_TRY(cudaMemsetAsync(bits, 0, p.slots - p.bits, stream));
+    attn_delta_kernel<T, D><<<(unsigned)((rows + 31) / 32), 256, 0, stream>>>(a, d_do, do_token, do_head, delta, dq, dk, dv);
+    attn_turn_kernel<<<(unsigned)((lists + 3) / 4), 128, 0, stream>>>(a, p.nqb, p.nkb, p.words, bits, counts);
+    attn_items_kernel<<<(unsigned)p.groups, 1024, 0, stream>>>(a, p, counts, slots, items, n_items);
+
+    const size_t dq_smem = (size_t)DQ_WARPS * DQ_STAGES * 2 * 16 * D * 2 + 2 * 16 * D * 2 + a.n_select * 4;
+    int st = attn_set_smem((const void *)attn_dq_rows_kernel<T, D>, dq_smem);
+    if (st) return st;
+    attn_dq_rows_kernel<T, D><<<(unsigned)dq_grid, 128, dq_smem, stream>>>(a, p.nqb, tiles, d_do, do_token, do_head, delta, dq);
+
+    switch (a.block) {
+    case 16: st = dkv_launch<T, D, 16>(a, p, d_do, do_token, do_head, delta, bits, items, n_items, partial, dk, dv, stream); break;
+    case 32: st = dkv_launch<T, D, 32>(a, p, d_do, do_token, do_head, delta, bits, items, n_items, partial, dk, dv, stream); break;
+    case 64: st = dkv_launch<T, D, 64>(a, p, d_do, do_token, do_head, delta, bits, items, n_items, partial, dk, dv, stream); break;
+    default: st = dkv_launch<T, D, 128>(a, p, d_do, do_token, do_head, delta, bits, items, n_items, partial, dk, dv, stream); break;
+    }
+    if (st) return st;
+    if (p.nqb > p.chunk)
+        attn_dkv_join_kernel<T><<<(unsigned)(p.groups * p.nkb), 128, 0, stream>>>(a, p, counts, slots, partial, dk, dv);
+    SPAMM_CUDA_TRY(cudaGetLastError());
+    return SPAMM_OK;
+}
+
+}  // namespace spamm
+
+using namespace spamm;
+
+extern "C" size_t spamm_attn_backward_scratch_bytes(const spamm_attn *a)
+{
+    if (attn_check(a, false) || !a->batch || !a->max_q || !a->tokens) return 0;
+    return backward_plan(*a).bytes;
+}
+
+extern "C" int spamm_attn_backward_dev(const spamm_attn *a, const void *d_do, int64_t do_token, int64_t do_head, void *d_dq,
+                                       void *d_dk, void *d_dv, void *d_scratch, size_t scratch_bytes, void *stream)
+{
+    int st = attn_check(a, true);
+    if (st) return st;
+    if (a->n_pages || !a->n_select)
+        return attn_refuse("gradients need packed keys and lists");
+    if (!(a->scale > 0.f) || !(a->scale <= 3e38f))
+        return attn_refuse("scale is not a positive number");
+    if (!a->tokens) return SPAMM_OK;
+    if (!attn_rows_ok(a->d_q, a->q_token, a->q_head) || !attn_rows_ok(a->d_k, a->k_token, a->k_head) ||
+        !attn_rows_ok(a->d_v, a->v_token, a->v_head) || !attn_rows_ok(a->d_o, a->o_token, a->o_head) || !a->d_lse ||
+        !attn_rows_ok(d_do, do_token, do_head) || !attn_rows_ok(d_dq, 0, 0) || !attn_rows_ok(d_dk, 0, 0) || !attn_rows_ok(d_dv, 0, 0))
+        return attn_refuse("q, k, v, o, lse and the gradients need rows on 16-byte boundaries");
+    if (!a->batch || !a->max_q) {        // no sequence: all rows belong to none
+        const size_t row = (size_t)a->tokens * a->dim * 2;
+        SPAMM_CUDA_TRY(cudaMemsetAsync(d_dq, 0, row * a->heads, (cudaStream_t)stream));
+        SPAMM_CUDA_TRY(cudaMemsetAsync(d_dk, 0, row * a->kv_heads, (cudaStream_t)stream));
+        SPAMM_CUDA_TRY(cudaMemsetAsync(d_dv, 0, row * a->kv_heads, (cudaStream_t)stream));
+        return SPAMM_OK;
+    }
+    const BackwardPlan p = backward_plan(*a);
+    if (!d_scratch || scratch_bytes < p.bytes || (reinterpret_cast<uintptr_t>(d_scratch) & 15))
+        return attn_refuse("scratch too small or not on a 16-byte boundary");
+    uint8_t *scratch = static_cast<uint8_t *>(d_scratch);
+    cudaStream_t str = (cudaStream_t)stream;
+#define SPAMM_BACKWARD(T, D)                                                                                            \
+    backward_launch<T, D>(*a, p, static_cast<const T *>(d_do), do_token, do_head, static_cast<T *>(d_dq),               \
+                          static_cast<T *>(d_dk), static_cast<T *>(d_dv), scratch, str)
+    if (a->dtype == SPAMM_ATTN_BF16) return a->dim == 64 ? SPAMM_BACKWARD(__nv_bfloat16, 64) : SPAMM_BACKWARD(__nv_bfloat16, 128);
+    return a->dim == 64 ? SPAMM_BACKWARD(__half, 64) : SPAMM_BACKWARD(__half, 128);
+#undef SPAMM_BACKWARD
+}

@@ -1,0 +1,445 @@
+// Attention over listed blocks, forward.
+//
+//   o_i = sum_j p_ij v_j,  p_ij = exp(scale q_i.k_j - lse_i),  lse_i = log sum_j exp(scale q_i.k_j)
+//
+// over the keys j of the blocks on the list of query i's block that i may see.  One pass over the keys with a running
+// maximum and sum (both float); p is rounded to the type of v for the product, as v itself is.
+#include <stdio.h>
+#include "attn.cuh"
+
+namespace spamm {
+
+bool attn_rows_ok(const void *p, int64_t token, int64_t head)
+{
+    return p && !(reinterpret_cast<uintptr_t>(p) & 15) && !(token & 7) && !(head & 7);
+}
+
+int attn_refuse(const char *why)
+{
+    static thread_local char msg[160];
+    snprintf(msg, sizeof(msg), "spamm_attn: %s", why);
+    record_error_text(msg);
+    return SPAMM_ERR_INVALID;
+}
+
+int attn_too_large()
+{
+    record_error_text("spamm_attn: more blocks of threads than a launch can have");
+    return SPAMM_ERR_UNSUPPORTED;
+}
+
+int attn_check(const spamm_attn *a, bool need_lists)
+{
+    if (!a) return SPAMM_ERR_INVALID;
+    if (a->dtype != SPAMM_ATTN_BF16 && a->dtype != SPAMM_ATTN_HALF) return attn_refuse("dtype is neither bf16 nor half");
+    if (a->dim != 64 && a->dim != 128) return attn_refuse("dim is neither 64 nor 128");
+    if (a->block != 16 && a->block != 32 && a->block != 64 && a->block != 128)
+        return attn_refuse("block is none of 16, 32, 64, 128");
+    if (a->batch < 0 || a->tokens < 0 || a->max_q < 0) return attn_refuse("negative size");
+    if (a->kv_heads < 1 || a->heads < a->kv_heads || a->heads % a->kv_heads || a->heads / a->kv_heads > 128)
+        return attn_refuse("heads is no multiple of kv_heads, or more than 128 times it");
+    if (a->query_block < 1) return attn_refuse("query_block below 1");
+    if (a->n_select < 0 || a->n_select > SPAMM_ATTN_MAX_SELECT) return attn_refuse("n_select outside 0..1024");
+    if (a->n_pages < 0 || a->table_width < 0 || (int64_t)a->table_width * a->block > INT32_MAX)
+        return attn_refuse("n_pages or table_width out of range");
+    if (!a->d_cu) return attn_refuse("d_cu is null");
+    if (a->n_pages && ((a->batch && !a->d_lengths) || (a->batch && a->table_width && !a->d_table) || a->table_stride < a->table_width || !a->d_status))
+        return attn_refuse("paged keys need d_lengths, d_table, a table_stride and d_status");
+    if (need_lists && a->n_select && a->batch && a->max_q && !a->d_lists) return attn_refuse("d_lists is null");
+    return SPAMM_OK;
+}
+
+int attn_set_smem(const void *kernel, size_t bytes)
+{
+    if (bytes > 48 * 1024) SPAMM_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+    return SPAMM_OK;
+}
+
+// Output rows that belong to no sequence become zero: part `part` of `parts` of those that lie before, inside (beyond
+// max_q) and, for the last sequence, behind sequence s, for the query heads of key head h.
+template <typename T>
+static __device__ void zero_tail(const spamm_attn &a, const Seq &sq, int s, int h, int part, int parts)
+{
+    const int G = a.heads / a.kv_heads, vecs = G * a.dim / 8;
+    const int end_own = min(max(a.d_cu[s + 1], sq.row0), a.tokens);
+    const int end = s == a.batch - 1 ? a.tokens : end_own;
+    const int begin = sq.row0 + sq.nq;
+    const int lead = s == 0 ? sq.row0 : 0;
+    const int rows = lead + (end - begin);
+    for (int i = part; i < rows; i += parts) {
+        const int row = i < lead ? i : begin + (i - lead);
+        for (int x = threadIdx.x; x < vecs; x += blockDim.x) {
+            const int head = h * G + x / (a.dim / 8), d = x % (a.dim / 8) * 8;
+            *reinterpret_cast<uint4 *>(static_cast<T *>(a.d_o) + row * a.o_token + head * a.o_head + d) = make_uint4(0, 0, 0, 0);
+        }
+        if (a.d_lse)
+            for (int g = threadIdx.x; g < G; g += blockDim.x) a.d_lse[(int64_t)row * a.heads + h * G + g] = -CUDART_INF_F;
+    }
+}
+
+// How a call is cut: tiles of rows over the (queries x heads of a key head) of a query block, and ranges of keys.
+struct RowsPlan {
+    int bq, nqb;            // queries per query block (all of them without lists), query blocks
+    int tiles;              // tiles of a query block
+    int n_split;            // ranges of keys
+    int split_keys;         // keys of a range, a multiple of the block
+    int max_entries;        // blocks of a range
+};
+
+constexpr int ROWS_STAGES = 3;
+constexpr int ROWS_WARPS = 4;
+
+// 16 rows (queries x heads) of one key head against one range of its keys.  Each of the four warps takes every fourth
+// chunk of 16 keys with a ring of three chunks of its own, so that nothing but the end synchronises the block; the four
+// results are joined in shared memory.  Bound by the reading of keys and values when rows are few.
+template <typename T, int D>
+__global__ __launch_bounds__(128) void attn_rows_kernel(const __grid_constant__ spamm_attn a, const RowsPlan p,
+                                                        float *part_o, float *part_lse)
+{
+    extern __shared__ __align__(128) uint8_t smem[];
+    constexpr int TILE16 = 16 * D * 2;
+    uint8_t *ring = smem;                                              // [warp][stage][K | V]
+    uint8_t *q_tile = ring + ROWS_WARPS * ROWS_STAGES * 2 * TILE16;
+    int *blk = reinterpret_cast<int *>(q_tile + TILE16);               // the list; then this range's blocks
+    int64_t *base = reinterpret_cast<int64_t *>(blk + max(a.n_select, p.max_entries) + (max(a.n_select, p.max_entries) & 1));
+    __shared__ int shared_count;
+
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    unsigned idx = blockIdx.x;
+    const int split = idx % p.n_split; idx /= p.n_split;
+    const int tile = idx % p.tiles; idx /= p.tiles;
+    const int qb = idx % p.nqb; idx /= p.nqb;
+    const int h = idx % a.kv_heads;
+    const int s = idx / a.kv_heads;
+    const int G = a.heads / a.kv_heads;
+    const Seq sq = attn_seq(a, s);
+    if (a.zero_tail && split == 0) zero_tail<T>(a, sq, s, h, qb * p.tiles + tile, p.nqb * p.tiles);
+    const int n_tok = min(p.bq, sq.nq - qb * p.bq);                    // queries of this query block
+    const int64_t n_rows = (int64_t)max(n_tok, 0) * G;
+    if ((int64_t)tile * 16 >= n_rows) return;
+    const int rows = (int)min((int64_t)16, n_rows - tile * 16);
+    const int tok0 = tile * 16 / G;
+    const int first_query = qb * p.bq + tok0, last_query = qb * p.bq + (tile * 16 + rows - 1) / G;
+    const int limit_max = attn_limit(a, sq, sq.pos0 + last_query);
+    const int limit_min = attn_limit(a, sq, sq.pos0 + first_query);
+
+    // Q tile: row r is query (tile*16 + r) / G of the block, head (tile*16 + r) % G of the group
+    for (int i = tid; i < 16 * D / 8; i += 128) {
+        const int r = i / (D / 8), c = i % (D / 8);
+        const int x = tile * 16 + r;
+        const bool ok = r < rows;
+        const int64_t off = (sq.row0 + qb * p.bq + (int64_t)(ok ? x / G : 0)) * a.q_token + (int64_t)(h * G + (ok ? x % G : 0)) * a.q_head;
+        cp_async16(smem_addr(q_tile) + tile_off<D>(r, c), static_cast<const T *>(a.d_q) + off + c * 8, ok);
+    }
+    cp_commit();
+
+    const int n_blocks = ceil_div(limit_max, a.block);
+    const int per_split = p.split_keys / a.block;
+    int e0, e1;
+    if (a.n_select) {
+        if (warp == 0) {
+            const int n = attn_load_list(a, s, qb, p.nqb, h, n_blocks, blk, lane);
+            if (lane == 0) shared_count = n;
+        }
+        __syncthreads();
+        e0 = min(split * per_split, shared_count);
+        e1 = min(e0 + per_split, shared_count);
+    } else {
+        e0 = min(split * per_split, n_blocks);
+        e1 = min(e0 + per_split, n_blocks);
+    }
+    // where each block's rows begin: for k; for v they begin at the same place in pages
+    for (int e = e0 + tid; e < e1; e += 128) {
+        const int b = a.n_select ? blk[e] : e;
+        base[e - e0] = attn_block_base(a, sq, s, h, b, a.k_token, a.k_head);
+    }
+    __syncthreads();
+
+    const int chunks_per_block = a.block >> 4;
+    const int n_chunks = (e1 - e0) * chunks_per_block;
+    const int64_t k_tok = a.n_pages ? D : a.k_token, v_tok = a.n_pages ? D : a.v_token;
+    const uint32_t my_ring = smem_addr(ring) + warp * ROWS_STAGES * 2 * TILE16;
+
+    auto chunk_pos = [&](int c) {
+        const int e = c / chunks_per_block;
+        const int b = a.n_select ? blk[e0 + e] : e0 + e;
+        return b * a.block + (c - e * chunks_per_block) * 16;
+    };
+    auto issue = [&](int c, int stage) {
+        if (c < n_chunks) {
+            const int e = c / chunks_per_block;
+            const int b = a.n_select ? blk[e0 + e] : e0 + e;
+            const int off = (c - e * chunks_per_block) * 16;
+            const int64_t kb = base[e];
+            const int64_t vb = a.n_pages ? kb : (int64_t)(sq.row0 + b * a.block) * a.v_token + h * a.v_head;
+            const int n = min(16, limit_max - (b * a.block + off));            // rows that some query may see
+            const T *kp = static_cast<const T *>(a.d_k) + (kb >= 0 ? kb + off * k_tok : 0);
+            const T *vp = static_cast<const T *>(a.d_v) + (kb >= 0 ? vb + off * v_tok : 0);
+            const uint32_t kt = my_ring + stage * 2 * TILE16, vt = kt + TILE16;
+#pragma unroll
+            for (int i = 0; i < 16 * D / 8 / 32; i++) {
+                const int x = i * 32 + lane, r = x / (D / 8), c8 = x % (D / 8);
+                const bool ok = kb >= 0 && r < n;
+                cp_async16(kt + tile_off<D>(r, c8), kp + (ok ? r * k_tok : 0) + c8 * 8, ok);
+                cp_async16(vt + tile_off<D>(r, c8), vp + (ok ? r * v_tok : 0) + c8 * 8, ok);
+            }
+        }
+        cp_commit();
+    };
+    for (int i = 0; i < ROWS_STAGES - 1; i++) issue(warp + ROWS_WARPS * i, i);
+
+    cp_wait<ROWS_STAGES - 1>();
+    __syncthreads();                       // the Q tile, loaded by all threads
+    uint32_t qf[D / 16][4];
+#pragma unroll
+    for (int ks = 0; ks < D / 16; ks++) a_frag<D>(smem_addr(q_tile), 0, ks, lane, qf[ks]);
+
+    int limit[2];
+#pragma unroll
+    for (int x = 0; x < 2; x++) {
+        const int r = (lane >> 2) + 8 * x;
+        limit[x] = r < rows ? attn_limit(a, sq, sq.pos0 + qb * p.bq + (tile * 16 + r) / G) : limit_max;
+    }
+    const float scale2 = a.scale * LOG2E;
+    float o[D / 8][4] = {};
+    float m[2] = {-CUDART_INF_F, -CUDART_INF_F}, l[2] = {0.f, 0.f};
+
+    int stage = 0;
+    for (int c = warp; c < n_chunks; c += ROWS_WARPS) {
+        issue(c + ROWS_WARPS * (ROWS_STAGES - 1), (stage + ROWS_STAGES - 1) % ROWS_STAGES);
+        cp_wait<ROWS_STAGES - 1>();
+        __syncwarp();
+        const uint32_t kt = my_ring + stage * 2 * TILE16, vt = kt + TILE16;
+        stage = stage + 1 == ROWS_STAGES ? 0 : stage + 1;
+        float sc[2][4] = {};
+#pragma unroll
+        for (int ks = 0; ks < D / 16; ks++) {
+            uint32_t b[4];
+            b_frag2<D>(kt, 0, ks, lane, b);
+            mma16816<T>(sc[0], qf[ks], b[0], b[1]);
+            mma16816<T>(sc[1], qf[ks], b[2], b[3]);
+        }
+        const int p0 = base[c / chunks_per_block] < 0 ? INT32_MAX - 64 : chunk_pos(c);
+        const bool masked = p0 > limit_min - 16;
+        float top[2] = {m[0], m[1]};
+#pragma unroll
+        for (int nt = 0; nt < 2; nt++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                float v = sc[nt][i] * scale2;
+                if (masked && p0 + nt * 8 + (lane & 3) * 2 + (i & 1) >= limit[i >> 1]) v = -CUDART_INF_F;
+                sc[nt][i] = v;
+                top[i >> 1] = fmaxf(top[i >> 1], v);
+            }
+#pragma unroll
+        for (int x = 0; x < 2; x++) {
+            top[x] = fmaxf(top[x], __shfl_xor_sync(~0u, top[x], 1));
+            top[x] = fmaxf(top[x], __shfl_xor_sync(~0u, top[x], 2));
+        }
+        if (__any_sync(~0u, top[0] != m[0] || top[1] != m[1])) {
+#pragma unroll
+            for (int x = 0; x < 2; x++) {
+                const float f = m[x] == top[x] ? 1.f : fast_exp2(m[x] - top[x]);   // equal: also -inf against -inf
+                l[x] *= f;
+                m[x] = top[x];
+#pragma unroll
+                for (int n = 0; n < D / 8; n++) { o[n][2 * x] *= f; o[n][2 * x + 1] *= f; }
+            }
+        }
+        const float m0 = m[0] == -CUDART_INF_F ? 0.f : m[0], m1 = m[1] == -CUDART_INF_F ? 0.f : m[1];
+#pragma unroll
+        for (int nt = 0; nt < 2; nt++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                sc[nt][i] = fast_exp2(sc[nt][i] - (i < 2 ? m0 : m1));
+                l[i >> 1] += sc[nt][i];
+            }
+        const uint32_t pf[4] = {Pack<T>::two(sc[0][0], sc[0][1]), Pack<T>::two(sc[0][2], sc[0][3]),
+                                Pack<T>::two(sc[1][0], sc[1][1]), Pack<T>::two(sc[1][2], sc[1][3])};
+#pragma unroll
+        for (int n = 0; n < D / 16; n++) {
+            uint32_t b[4];
+            bt_frag2<D>(vt, 0, n * 16, lane, b);
+            mma16816<T>(o[2 * n], pf, b[0], b[1]);
+            mma16816<T>(o[2 * n + 1], pf, b[2], b[3]);
+        }
+        __syncwarp();
+    }
+    cp_wait<0>();
+#pragma unroll
+    for (int x = 0; x < 2; x++) {
+        l[x] += __shfl_xor_sync(~0u, l[x], 1);
+        l[x] += __shfl_xor_sync(~0u, l[x], 2);
+    }
+    __syncthreads();
+    // join the four warps: [warp][16][D] sums, then maxima and sums of the rows
+    float *so = reinterpret_cast<float *>(ring);
+    float *sm = so + ROWS_WARPS * 16 * D, *sl = sm + ROWS_WARPS * 16;
+#pragma unroll
+    for (int n = 0; n < D / 8; n++)
+#pragma unroll
+        for (int x = 0; x < 2; x++)
+            *reinterpret_cast<float2 *>(so + ((warp * 16 + (lane >> 2) + 8 * x) * D + n * 8 + (lane & 3) * 2)) =
+                make_float2(o[n][2 * x], o[n][2 * x + 1]);
+    if ((lane & 3) == 0)
+#pragma unroll
+        for (int x = 0; x < 2; x++) {
+            sm[warp * 16 + (lane >> 2) + 8 * x] = m[x];
+            sl[warp * 16 + (lane >> 2) + 8 * x] = l[x];
+        }
+    __syncthreads();
+    const int r = tid >> 3, c0 = (tid & 7) * (D / 8);
+    if (r < rows) {
+        float top = -CUDART_INF_F, f[ROWS_WARPS], total = 0.f;
+#pragma unroll
+        for (int w = 0; w < ROWS_WARPS; w++) top = fmaxf(top, sm[w * 16 + r]);
+        const float t0 = top == -CUDART_INF_F ? 0.f : top;
+#pragma unroll
+        for (int w = 0; w < ROWS_WARPS; w++) {
+            f[w] = fast_exp2(sm[w * 16 + r] - t0);
+            total += sl[w * 16 + r] * f[w];
+        }
+        // no visible key: no sum, output zero.  (A NaN among the scores stays: total is then NaN, not zero.)
+        const float inv = total == 0.f ? 0.f : 1.f / total;
+        const float lse2 = total == 0.f ? -CUDART_INF_F : t0 + log2f(total);
+        float y[D / 8] = {};
+#pragma unroll
+        for (int w = 0; w < ROWS_WARPS; w++)
+#pragma unroll
+            for (int i = 0; i < D / 8; i++) y[i] += so[(w * 16 + r) * D + c0 + i] * f[w];
+        const int x = tile * 16 + r;
+        const int64_t row = sq.row0 + qb * p.bq + x / G;
+        const int head = h * G + x % G;
+        if (p.n_split == 1) {
+            uint32_t out[D / 16];
+#pragma unroll
+            for (int i = 0; i < D / 16; i++) out[i] = Pack<T>::two(y[2 * i] * inv, y[2 * i + 1] * inv);
+            T *dst = static_cast<T *>(a.d_o) + row * a.o_token + head * a.o_head + c0;
+#pragma unroll
+            for (int i = 0; i < D / 64; i++) reinterpret_cast<uint4 *>(dst)[i] = *reinterpret_cast<uint4 *>(out + 4 * i);
+            if (a.d_lse && (tid & 7) == 0) a.d_lse[row * a.heads + head] = lse2 * LN2;
+        } else {
+            const int64_t at = (row * a.heads + head) * p.n_split + split;
+#pragma unroll
+            for (int i = 0; i < D / 8; i++) part_o[at * D + c0 + i] = y[i] * inv;
+            if ((tid & 7) == 0) part_lse[at] = lse2;
+        }
+    }
+}
+
+// Joins the ranges of keys of every row: o = sum_i 2^(lse_i - lse) o_i.  One warp for a row and head.
+template <typename T, int D>
+__global__ __launch_bounds__(128) void attn_join_kernel(const __grid_constant__ spamm_attn a, int n_split,
+                                                        const float *part_o, const float *part_lse)
+{
+    const int lane = threadIdx.x & 31;
+    const int64_t w = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
+    const int64_t per_seq = (int64_t)a.max_q * a.heads;
+    if (w >= per_seq * a.batch) return;
+    const int s = (int)(w / per_seq);
+    const int i = (int)(w % per_seq / a.heads), head = (int)(w % a.heads);
+    const Seq sq = attn_seq(a, s);
+    if (i >= sq.nq) return;
+    const int64_t row = sq.row0 + i, at = (row * a.heads + head) * n_split;
+    float top = -CUDART_INF_F;
+    for (int j = lane; j < n_split; j += 32) top = fmaxf(top, part_lse[at + j]);
+#pragma unroll
+    for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
+    const float t0 = top == -CUDART_INF_F ? 0.f : top;
+    float y[D / 32] = {}, total = 0.f;
+    for (int j = 0; j < n_split; j++) {
+        const float z = part_lse[at + j];
+        if (z == -CUDART_INF_F) continue;
+        const float f = fast_exp2(z - t0);
+        total += f;
+        const float *src = part_o + (at + j) * D + lane * (D / 32);
+#pragma unroll
+        for (int d = 0; d < D / 32; d++) y[d] += f * src[d];
+    }
+    const float inv = total == 0.f ? 0.f : 1.f / total;
+    T *dst = static_cast<T *>(a.d_o) + row * a.o_token + head * a.o_head + lane * (D / 32);
+#pragma unroll
+    for (int d = 0; d < D / 32; d += 2) *reinterpret_cast<uint32_t *>(dst + d) = Pack<T>::two(y[d] * inv, y[d + 1] * inv);
+    if (a.d_lse && lane == 0) a.d_lse[row * a.heads + head] = total == 0.f ? -CUDART_INF_F : (t0 + log2f(total)) * LN2;
+}
+
+static int64_t longest_list(const spamm_attn &a)
+{
+    return a.n_select ? min(a.n_select, attn_max_blocks(a)) : attn_max_blocks(a);
+}
+
+static RowsPlan rows_plan(const spamm_attn &a, int tile_rows)
+{
+    RowsPlan p;
+    const int G = a.heads / a.kv_heads;
+    p.bq = a.n_select ? min(a.query_block, a.max_q) : a.max_q;
+    p.nqb = ceil_div(a.max_q, p.bq);
+    p.tiles = (int)(((int64_t)p.bq * G + tile_rows - 1) / tile_rows);
+    const int64_t blocks = max((int64_t)1, longest_list(a));
+    const int64_t units = (int64_t)a.batch * a.kv_heads * p.nqb * p.tiles;
+    // enough blocks of threads to fill 148 SMs twice over, ranges of 256 keys at the least
+    int64_t want = (600 + units - 1) / units;
+    want = max((int64_t)1, min(want, (blocks * a.block + 255) / 256));
+    int64_t per = min((int64_t)SPAMM_ATTN_MAX_SELECT, (blocks + want - 1) / want);
+    p.n_split = (int)((blocks + per - 1) / per);
+    p.max_entries = (int)per;
+    p.split_keys = (int)(per * a.block);
+    return p;
+}
+
+static size_t rows_smem(const spamm_attn &a, const RowsPlan &p)
+{
+    const int n = max(a.n_select, p.max_entries);
+    return (size_t)ROWS_WARPS * ROWS_STAGES * 2 * 16 * a.dim * 2 + 16 * a.dim * 2 + 4 * (n + (n & 1)) + 8 * (size_t)p.max_entries;
+}
+
+template <typename T, int D>
+static int forward_launch(const spamm_attn &a, float *scratch, cudaStream_t stream)
+{
+    const RowsPlan p = rows_plan(a, 16);
+    const int64_t grid = (int64_t)a.batch * a.kv_heads * p.nqb * p.tiles * p.n_split;
+    const int64_t rows = (int64_t)a.batch * a.max_q * a.heads;
+    if (grid > INT32_MAX || (rows + 3) / 4 > INT32_MAX) return attn_too_large();
+    float *part_o = scratch;
+    float *part_lse = scratch + (size_t)a.tokens * a.heads * p.n_split * D;
+    const size_t smem = rows_smem(a, p);
+    int st = attn_set_smem((const void *)attn_rows_kernel<T, D>, smem);
+    if (st) return st;
+    attn_rows_kernel<T, D><<<(unsigned)grid, 128, smem, stream>>>(a, p, part_o, part_lse);
+    if (p.n_split > 1)
+        attn_join_kernel<T, D><<<(unsigned)((rows + 3) / 4), 128, 0, stream>>>(a, p.n_split, part_o, part_lse);
+    SPAMM_CUDA_TRY(cudaGetLastError());
+    return SPAMM_OK;
+}
+
+}  // namespace spamm
+
+using namespace spamm;
+
+extern "C" size_t spamm_attn_forward_scratch_bytes(const spamm_attn *a)
+{
+    if (attn_check(a, false) || !a->batch || !a->max_q || !a->tokens) return 0;
+    const RowsPlan p = rows_plan(*a, 16);
+    return p.n_split > 1 ? (size_t)a->tokens * a->heads * p.n_split * (a->dim + 1) * sizeof(float) : 0;
+}
+
+extern "C" int spamm_attn_forward_dev(const spamm_attn *a, void *d_scratch, size_t scratch_bytes, void *stream)
+{
+    int st = attn_check(a, true);
+    if (st) return st;
+    if (!(a->scale > 0.f) || !(a->scale <= 3e38f)) return attn_refuse("scale is not a positive number");
+    if (!a->tokens || !a->batch || !a->max_q) return SPAMM_OK;
+    const bool k_ok = a->n_pages ? attn_rows_ok(a->d_k, 0, 0) && attn_rows_ok(a->d_v, 0, 0)
+                                 : attn_rows_ok(a->d_k, a->k_token, a->k_head) && attn_rows_ok(a->d_v, a->v_token, a->v_head);
+    if (!k_ok || !attn_rows_ok(a->d_q, a->q_token, a->q_head) || !attn_rows_ok(a->d_o, a->o_token, a->o_head))
+        return attn_refuse("q, k, v and o need rows on 16-byte boundaries");
+    const size_t need = spamm_attn_forward_scratch_bytes(a);
+    if (need && (!d_scratch || scratch_bytes < need || (reinterpret_cast<uintptr_t>(d_scratch) & 15)))
+        return attn_refuse("scratch too small or not on a 16-byte boundary");
+    float *scratch = static_cast<float *>(d_scratch);
+    if (a->dtype == SPAMM_ATTN_BF16)
+        return a->dim == 64 ? forward_launch<__nv_bfloat16, 64>(*a, scratch, (cudaStream_t)stream)
+                            : forward_launch<__nv_bfloat16, 128>(*a, scratch, (cudaStream_t)stream);
+    return a->dim == 64 ? forward_launch<__half, 64>(*a, scratch, (cudaStream_t)stream)
+                        : forward_launch<__half, 128>(*a, scratch, (cudaStream_t)stream);
+}

@@ -26,7 +26,7 @@ __host__ __device__ inline uint32_t step_cols(uint32_t s) { return (s >> 20) & 0
 __host__ __device__ inline int step_count_of(int32_t v) { return v & SPAMM_STEPS_MASK; }
 __host__ __device__ inline bool step_list_dense(int32_t v) { return (v & SPAMM_STEPS_DENSE) != 0; }
 
-inline int ceil_div(int a, int b) { return (a + b - 1) / b; }
+__host__ __device__ inline int ceil_div(int a, int b) { return (a + b - 1) / b; }
 
 // Records a CUDA error for spamm_last_cuda_error and maps it to a status.
 int record_cuda_error(cudaError_t e, const char *what);

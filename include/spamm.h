@@ -457,6 +457,114 @@ int spamm_count_valid_static(const float *d_norm_a, const float *d_norm_b, int r
                              float tau, unsigned long long *d_count, double *d_sum, void *stream);
 int spamm_count_valid_static_max_blocks(void);
 
+/* ---------------------------------------------------------------- attention over selected blocks ---- */
+
+/*
+ * The engine's scheme -- a cheap score per block, lists of the blocks worth multiplying, products of the listed blocks
+ * only -- applied to attention.  Queries, keys and values are bf16 or half; keys are taken in blocks of `block` tokens;
+ * `query_block` consecutive queries of a sequence share one list per key head.
+ *
+ *   spamm_attn_append_dev     new keys and values into the pages of a cache, rotated by position on the way
+ *   spamm_attn_select_dev     the lists: the n_select best blocks of every query block
+ *   spamm_attn_forward_dev    attention over the listed blocks, or over all of them
+ *   spamm_attn_backward_dev   gradients of q, k and v (packed keys, listed blocks)
+ *
+ * There is no counterpart in the reference.  All four work on device memory of the caller (tensors, lists, scratch) on
+ * the caller's stream, allocate nothing, may be captured into a graph, and are safe to call from several threads.
+ * The current device must be the one that holds the memory.
+ *
+ * Tokens of all sequences lie one behind the other ("packed"): sequence s has the rows [cu[s], cu[s+1]) of q, of o and,
+ * without pages, of k and v.  Query heads h*G .. h*G+G-1 (G = heads / kv_heads) read key head h.  The last value of a
+ * row is contiguous, rows are 16-byte aligned, and token and head strides are given in elements (multiples of 8).
+ *
+ * Keys are either packed (n_pages == 0; self attention, query i of a sequence has position i), or in a paged cache:
+ * k and v are [n_pages][kv_heads][block][dim] with no gaps, the page of block b of sequence s is table[s][b], and
+ * lengths[s] keys are held, the new ones among them (query i of n new ones has position lengths[s] - n + i).
+ *
+ * What device memory says is never trusted with an address: cu is clamped to [0, tokens], lengths to the table's width,
+ * a page outside [0, n_pages) is treated as masked (append: not written) and SPAMM_ERR_INVALID is stored to *d_status;
+ * a list entry that is no block of the sequence, or not above every entry before it, is skipped.  Queries of a
+ * sequence from max_q on are not computed (their rows count as rows behind the last sequence).
+ */
+#define SPAMM_ATTN_BF16 0
+#define SPAMM_ATTN_HALF 1
+#define SPAMM_ATTN_MAX_SELECT 1024      /* longest list */
+#define SPAMM_ATTN_MAX_BLOCKS 16384     /* most blocks of a sequence that spamm_attn_select_dev ranks */
+
+typedef struct spamm_attn {
+    int32_t dtype;              /* of q, k, v, o and their gradients: SPAMM_ATTN_* */
+    int32_t batch;              /* sequences */
+    int32_t heads, kv_heads;    /* heads a multiple of kv_heads, at most 128 times */
+    int32_t dim;                /* of a head: 64 or 128 */
+    int32_t block;              /* keys of a block, tokens of a page: 16, 32, 64 or 128 */
+    int32_t query_block;        /* queries that share a list: 1 or more */
+    int32_t n_select;           /* entries of a list; 0: no lists, every block is read */
+    int32_t causal;             /* non-zero: a query sees the keys up to its own position */
+    int32_t max_q;              /* no sequence has more new tokens (a host-side bound; sizes the grids and d_lists) */
+    int32_t tokens;             /* rows of q, o and packed k, v */
+    int32_t n_pages;            /* pages of the cache; 0: packed keys */
+    int32_t table_width;        /* entries of a row of d_table */
+    int32_t zero_tail;          /* non-zero: output rows that belong to no sequence become zero; else they are left */
+    float scale;                /* of the scores, above zero */
+    const int32_t *d_cu;        /* [batch + 1] */
+    const int32_t *d_lengths;   /* [batch], pages only */
+    const int32_t *d_table;     /* [batch][table_stride], pages only */
+    int64_t table_stride;
+    const int32_t *d_lists;     /* [batch][ceil(max_q / query_block)][kv_heads][n_select], ascending, -1 behind */
+    const void *d_q;
+    int64_t q_token, q_head;
+    const void *d_k;            /* packed keys, or the pages (strides not read) */
+    int64_t k_token, k_head;
+    const void *d_v;
+    int64_t v_token, v_head;
+    void *d_o;
+    int64_t o_token, o_head;
+    float *d_lse;               /* [tokens][heads] log of the sum of exp(scale * q.k) over the keys read, -inf for none;
+                                   output of the forward (NULL: not wanted), input of the backward */
+    int32_t *d_status;          /* one word, kept until the caller clears it; may be NULL without pages */
+} spamm_attn;
+
+/*
+ * New keys and values (k and v of `a`, packed, d_k/d_v with their strides) go to the pages: token i of n new ones of
+ * sequence s to position p = lengths[s] - n + i.  d_k_pages, d_v_pages: [n_pages][kv_heads][block][dim].  With
+ * d_inv_freq ([n_freq] float, 2 * n_freq <= dim) the first 2 * n_freq values of every key head are turned by the angles
+ * p * inv_freq[j], pairs (j, j + n_freq) or, with interleaved, (2j, 2j + 1); d_q, when given, is turned likewise into
+ * d_o.  The angle is taken in double, its cosine and sine rounded to float, the products and their sum rounded to float
+ * one by one, the result once to the type.  d_key_sums ([n_pages][kv_heads][dim] float, may be NULL) gets for every page
+ * written to the sum of all the keys that the page now holds, taken in double: appending again after a rollback of
+ * `lengths` leaves right sums.  No two sequences may append to the same page in one call.
+ */
+int spamm_attn_append_dev(const spamm_attn *a, void *d_k_pages, void *d_v_pages, float *d_key_sums,
+                          const float *d_inv_freq, int n_freq, int interleaved, void *stream);
+
+/*
+ * Lists of the n_select blocks with the largest score for every query block and key head, ascending, -1 behind:
+ *   score(b) = (sum of the query block's queries, all G heads) . (sum of the keys of b) / (keys held by b)
+ * Key sums are rounded to float (d_key_sums with pages, computed here from packed keys otherwise); everything else is
+ * done in double, so that the choice does not depend on an order of summation.  Ties go to the lower block; a score
+ * that is NaN comes last.  Blocks with no key that some query of the query block sees are not candidates.  The first
+ * n_first blocks and the blocks from (n_local - 1) before that of the first query to that of the last one (n_local 0:
+ * none) are taken whatever their score: n_select >= n_first + n_local + (query_block + block - 2) / block (without the
+ * last two terms when n_local is 0).  d_lists_out has the layout of d_lists; rows of query blocks that do not exist
+ * become -1.
+ */
+size_t spamm_attn_select_scratch_bytes(const spamm_attn *a);
+int spamm_attn_select_dev(const spamm_attn *a, const float *d_key_sums, int n_first, int n_local,
+                          int32_t *d_lists_out, void *d_scratch, size_t scratch_bytes, void *stream);
+
+/* o = softmax(scale * q k^T) v over the keys of the listed blocks that a query may see; zero where there are none. */
+size_t spamm_attn_forward_scratch_bytes(const spamm_attn *a);
+int spamm_attn_forward_dev(const spamm_attn *a, void *d_scratch, size_t scratch_bytes, void *stream);
+
+/*
+ * Gradients for the output gradient d_do ([tokens][heads][dim], strides given): d_dq [tokens][heads][dim], d_dk and
+ * d_dv [tokens][kv_heads][dim], without gaps.  `a` holds q, k, v, o, lse and the lists as the forward had them.  Sums
+ * run in a fixed order: the same inputs give the same bits.
+ */
+size_t spamm_attn_backward_scratch_bytes(const spamm_attn *a);
+int spamm_attn_backward_dev(const spamm_attn *a, const void *d_do, int64_t do_token, int64_t do_head,
+                            void *d_dq, void *d_dk, void *d_dv, void *d_scratch, size_t scratch_bytes, void *stream);
+
 /* ---------------------------------------------------------------- generators and misc ------------- */
 
 /*
