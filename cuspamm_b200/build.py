@@ -16,7 +16,7 @@ CSRC = PKG_DIR / "csrc"
 LIB_PATH = PKG_DIR / "libspamm.so"
 SOURCES = ["norm_map.cu", "skip_lists.cu", "pack_half.cu", "gated_multiply.cu", "gated_multiply_pair.cu", "gated_multiply_gpair.cu", "plan.cu", "group.cu", "extras.cu",
            "attn_append.cu", "attn_select.cu", "attn_forward.cu", "attn_backward.cu", "generators.cpp"]
-HEADERS = [CSRC / "common.cuh", CSRC / "tc_utils.cuh", CSRC / "plan.cuh", CSRC / "attn.cuh", PKG_DIR.parent / "include" / "spamm.h"]
+HEADERS = [CSRC / "common.cuh", CSRC / "tc_utils.cuh", CSRC / "plan.cuh", CSRC / "attn.cuh", CSRC / "attn_tc.cuh", PKG_DIR.parent / "include" / "spamm.h"]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",

@@ -6,6 +6,7 @@
 // maximum and sum (both float); p is rounded to the type of v for the product, as v itself is.
 #include <stdio.h>
 #include "attn.cuh"
+#include "attn_tc.cuh"
 
 namespace spamm {
 
@@ -327,6 +328,334 @@ __global__ __launch_bounds__(128) void attn_rows_kernel(const __grid_constant__ 
     }
 }
 
+// ---- tiles of 128 rows on the tensor memory path
+//
+// Per block of threads: 128 rows (queries x heads of a key head) against a range of its keys, 128 keys (the listed blocks
+// one behind the other) at a time.  S = Q K^T goes to tensor memory; four warps, a thread for each row, take the running
+// maximum and write p over S in the type of v; O += P V takes p from tensor memory.  A block uses half of the tensor
+// memory and under half of the shared memory, so that two of them share an SM: one's exponentials run beside the other's
+// products.  Four warps feed K and V with 16-byte copies (rows gathered block by block, keys behind the end zero).
+//
+// The running maximum is only raised when a row's scores exceed it by more than 2^8: until then p stays below 2^8, which
+// both types and the float sums hold without loss, and O need not be rescaled in tensor memory.
+constexpr int TC_ROWS = 128, TC_KEYS = 128;
+constexpr int TC_SOFTMAX = 128, TC_LOADERS = 128, TC_THREADS = TC_SOFTMAX + 32 + TC_LOADERS;
+constexpr int TC_COLS = 256;            // S (P over it) in columns 0..127, O behind
+
+struct TcCtrl {
+    uint64_t q_full, k_full, k_empty, v_full, v_empty, s_full, p_full, pv_done;
+    uint32_t tmem_base;
+    uint32_t abort_flag;
+    int32_t err;
+    int32_t count;
+};
+
+template <typename T, int D>
+__global__ __launch_bounds__(TC_THREADS, 2) void attn_tc_kernel(const __grid_constant__ spamm_attn a, const RowsPlan p,
+                                                                float *part_o, float *part_lse)
+{
+    extern __shared__ __align__(16) uint8_t smem_raw[];
+    constexpr int TILE = 128 * D * 2;
+    const uint32_t raw = smem_u32(smem_raw);
+    uint8_t *smem = smem_raw + ((1024 - (raw & 1023)) & 1023);
+    const uint32_t q_tile = smem_u32(smem), k_tile = q_tile + TILE, v_tile = k_tile + TILE;
+    TcCtrl *ctrl = reinterpret_cast<TcCtrl *>(smem + 3 * TILE);
+    int64_t *base = reinterpret_cast<int64_t *>(ctrl + 1);
+    int *blk = reinterpret_cast<int *>(base + p.max_entries);
+
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    unsigned idx = blockIdx.x;
+    // tiles that read the same keys run side by side, those with the longest causal rows first
+    const int tile = p.tiles - 1 - idx % p.tiles; idx /= p.tiles;
+    const int qb = p.nqb - 1 - idx % p.nqb; idx /= p.nqb;
+    const int split = idx % p.n_split; idx /= p.n_split;
+    const int h = idx % a.kv_heads;
+    const int s = idx / a.kv_heads;
+    const int G = a.heads / a.kv_heads;
+    const Seq sq = attn_seq(a, s);
+    if (a.zero_tail && split == 0) zero_tail<T>(a, sq, s, h, qb * p.tiles + tile, p.nqb * p.tiles);
+    const int n_tok = min(p.bq, sq.nq - qb * p.bq);
+    const int64_t n_rows = (int64_t)max(n_tok, 0) * G;
+    if ((int64_t)tile * TC_ROWS >= n_rows) return;
+    const int rows = (int)min((int64_t)TC_ROWS, n_rows - tile * TC_ROWS);
+    const int query0 = qb * p.bq;
+    const int first_query = query0 + tile * TC_ROWS / G, last_query = query0 + (tile * TC_ROWS + rows - 1) / G;
+    const int limit_max = attn_limit(a, sq, sq.pos0 + last_query);
+    const int limit_min = attn_limit(a, sq, sq.pos0 + first_query);
+
+    if (warp == 0) {
+        if (a.n_select) {
+            const int n = attn_load_list(a, s, qb, p.nqb, h, ceil_div(limit_max, a.block), blk, lane);
+            if (lane == 0) ctrl->count = n;
+        } else if (lane == 0)
+            ctrl->count = ceil_div(limit_max, a.block);
+    } else if (warp == 4) {
+        if (lane == 0) {
+            mbar_init(smem_u32(&ctrl->q_full), TC_LOADERS);
+            mbar_init(smem_u32(&ctrl->k_full), TC_LOADERS);
+            mbar_init(smem_u32(&ctrl->v_full), TC_LOADERS);
+            mbar_init(smem_u32(&ctrl->k_empty), 1);
+            mbar_init(smem_u32(&ctrl->v_empty), 1);
+            mbar_init(smem_u32(&ctrl->s_full), 1);
+            mbar_init(smem_u32(&ctrl->pv_done), 1);
+            mbar_init(smem_u32(&ctrl->p_full), TC_SOFTMAX);
+            ctrl->abort_flag = 0;
+            ctrl->err = 0;
+            asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        }
+        __syncwarp();
+        tmem_alloc<TC_COLS>(smem_u32(&ctrl->tmem_base));
+        tc_fence_before();
+    }
+    __syncthreads();
+    tc_fence_after();
+    const int per_split = p.split_keys / a.block;
+    const int e0 = min(split * per_split, ctrl->count), n_entries = min(per_split, ctrl->count - e0);
+    // first position of every block of the range (far behind every limit for a page that does not exist) and where its
+    // rows of k begin
+    int my_pos[4];
+    for (int i = 0, e = tid; e < n_entries; e += TC_THREADS, i++) {
+        const int b = a.n_select ? blk[e0 + e] : e0 + e;
+        const int64_t at = attn_block_base(a, sq, s, h, b, a.k_token, a.k_head);
+        base[e] = at;
+        my_pos[i] = at < 0 ? INT32_MAX / 2 : b * a.block;
+    }
+    __syncthreads();
+    for (int i = 0, e = tid; e < n_entries; e += TC_THREADS, i++) blk[e] = my_pos[i];
+    __syncthreads();
+    const int log_block = 31 - __clz(a.block);
+    const int n_keys = n_entries << log_block;
+    const int n_tiles = (n_keys + TC_KEYS - 1) / TC_KEYS;
+    const uint32_t tmem = ctrl->tmem_base, tmem_o = tmem + TC_KEYS;
+    const WaitState ws{&ctrl->abort_flag, &ctrl->err};
+
+    if (warp >= 5) {
+        // ---- loaders
+        const int t = tid - (TC_SOFTMAX + 32);
+        constexpr int PER = 128 * (D / 8) / TC_LOADERS;
+        for (int i = 0; i < PER; i++) {
+            const int x = i * TC_LOADERS + t, r = x / (D / 8), c = x % (D / 8);
+            const bool ok = r < rows;
+            const int y = tile * TC_ROWS + (ok ? r : 0);
+            const int64_t off = (int64_t)(sq.row0 + query0 + y / G) * a.q_token + (int64_t)(h * G + y % G) * a.q_head;
+            cp_async16(q_tile + panel_off(128, r, c), static_cast<const T *>(a.d_q) + off + c * 8, ok);
+        }
+        cp_commit();
+        const int64_t k_tok = a.n_pages ? D : a.k_token, v_tok = a.n_pages ? D : a.v_token;
+        // signals that the copies before the last `left` groups have arrived
+        auto signal = [&](uint64_t *bar) {
+            fence_async_smem();
+            mbar_arrive(smem_u32(bar));
+        };
+        auto load = [&](int j, bool value) {
+            const uint32_t dst = value ? v_tile : k_tile;
+            const int64_t tok = value ? v_tok : k_tok;
+            const T *src = static_cast<const T *>(value ? a.d_v : a.d_k);
+#pragma unroll 4
+            for (int i = 0; i < PER; i++) {
+                const int x = i * TC_LOADERS + t, r = x / (D / 8), c = x % (D / 8);
+                const int key = j * TC_KEYS + r, e = key >> log_block, off = key & (a.block - 1);
+                const bool ok = e < n_entries && blk[e] + off < limit_max;
+                int64_t at = 0;
+                if (ok) at = (value && !a.n_pages ? (int64_t)(sq.row0 + blk[e]) * a.v_token + h * a.v_head : base[e]) + off * tok;
+                cp_async16(dst + panel_off(128, r, c), src + at + c * 8, ok);
+            }
+            cp_commit();
+        };
+        bool fine = true;
+        for (int j = 0; j < n_tiles && fine; j++) {
+            if (j) fine = ws.wait(smem_u32(&ctrl->k_empty), j - 1, 1);
+            if (!fine) break;
+            load(j, false);
+            // the group before this one: the queries, or the values of the tile before
+            cp_wait<1>();
+            signal(j ? &ctrl->v_full : &ctrl->q_full);
+            if (j) fine = ws.wait(smem_u32(&ctrl->v_empty), j - 1, 2);
+            if (!fine) break;
+            load(j, true);
+            cp_wait<1>();
+            signal(&ctrl->k_full);
+        }
+        cp_wait<0>();
+        if (n_tiles && fine) signal(&ctrl->v_full);
+    } else if (warp == 4) {
+        // ---- products
+        if (lane == 0 && n_tiles) {
+            constexpr uint32_t s_desc = mma_desc<T>(128, TC_KEYS, false, false), o_desc = mma_desc<T>(128, D, false, true);
+            bool fine = ws.wait(smem_u32(&ctrl->q_full), 0, 3);
+            for (int j = 0; j <= n_tiles && fine; j++) {
+                if (j) {
+                    fine = ws.wait(smem_u32(&ctrl->p_full), j - 1, 4) && ws.wait(smem_u32(&ctrl->v_full), j - 1, 5);
+                    if (!fine) break;
+                    tc_fence_after();
+#pragma unroll
+                    for (int ks = 0; ks < TC_KEYS / 16; ks++)
+                        mma_ts(tmem_o, tmem + ks * 8, desc_mn_major(v_tile, 128, ks), o_desc, j > 1 || ks);
+                    umma_commit(smem_u32(&ctrl->v_empty));
+                    umma_commit(smem_u32(&ctrl->pv_done));
+                }
+                if (j < n_tiles) {
+                    // products of one block run in order: S may be written where p is still being read
+                    fine = ws.wait(smem_u32(&ctrl->k_full), j, 6);
+                    if (!fine) break;
+                    tc_fence_after();
+#pragma unroll
+                    for (int ks = 0; ks < D / 16; ks++)
+                        mma_ss(tmem, desc_k_major(q_tile, 128, ks), desc_k_major(k_tile, 128, ks), s_desc, ks != 0);
+                    umma_commit(smem_u32(&ctrl->k_empty));
+                    umma_commit(smem_u32(&ctrl->s_full));
+                }
+            }
+        }
+        __syncwarp();
+    } else {
+        // ---- softmax: thread = row
+        const uint32_t lane_base = tmem + ((uint32_t)(warp * 32) << 16), lane_o = tmem_o + ((uint32_t)(warp * 32) << 16);
+        const int r = tid;
+        const int y = tile * TC_ROWS + min(r, rows - 1);
+        const int limit = attn_limit(a, sq, sq.pos0 + query0 + y / G);
+        const float scale2 = a.scale * LOG2E;
+        float m = -CUDART_INF_F, l = 0.f;
+        bool fine = true;
+        for (int j = 0; j < n_tiles; j++) {
+            fine = __all_sync(~0u, ws.wait(smem_u32(&ctrl->s_full), j, 7));
+            if (!fine) break;
+            tc_fence_after();
+            // positions of the tile's eight groups of 16 keys; all visible to all rows in most tiles
+            int group_pos = INT32_MAX / 2;
+            if (lane < TC_KEYS / 16) {
+                const int key = j * TC_KEYS + lane * 16, e = key >> log_block;
+                if (e < n_entries) group_pos = blk[e] + (key & (a.block - 1));
+            }
+            const bool masked = __any_sync(~0u, lane < TC_KEYS / 16 && group_pos > limit_min - 16);
+            float top = -CUDART_INF_F;
+            uint32_t v[32];
+#pragma unroll 1
+            for (int c = 0; c < TC_KEYS / 32; c++) {
+                tmem_ld32(lane_base + c * 32, v);
+                tmem_wait_ld();
+                if (masked) {
+                    const int n0 = limit - __shfl_sync(~0u, group_pos, 2 * c), n1 = limit - __shfl_sync(~0u, group_pos, 2 * c + 1);
+#pragma unroll
+                    for (int i = 0; i < 32; i++)
+                        if ((i & 15) >= (i < 16 ? n0 : n1)) v[i] = 0xff800000u;
+                }
+                float t0 = __uint_as_float(v[0]), t1 = __uint_as_float(v[1]);
+#pragma unroll
+                for (int i = 2; i < 32; i += 2) {
+                    t0 = fmaxf(t0, __uint_as_float(v[i]));
+                    t1 = fmaxf(t1, __uint_as_float(v[i + 1]));
+                }
+                top = fmaxf(top, fmaxf(t0, t1));
+            }
+            top *= scale2;
+            const bool raise = top > m + 8.f || (m == -CUDART_INF_F && top > m);
+            if (__any_sync(~0u, raise)) {
+                const float f = raise ? fast_exp2(m - top) : 1.f;
+                if (raise) { m = top; l *= f; }
+                if (j) {
+                    // O of the tiles before must be complete before it is rescaled
+                    fine = __all_sync(~0u, ws.wait(smem_u32(&ctrl->pv_done), j - 1, 8));
+                    if (!fine) break;
+                    tc_fence_after();
+#pragma unroll 1
+                    for (int c = 0; c < D / 32; c++) {
+                        tmem_ld32(lane_o + c * 32, v);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int i = 0; i < 32; i++) v[i] = __float_as_uint(__uint_as_float(v[i]) * f);
+                        tmem_st32(lane_o + c * 32, v);
+                    }
+                    tmem_wait_st();
+                }
+            }
+            const float m0 = m == -CUDART_INF_F ? 0.f : m;
+            float l0 = 0.f, l1 = 0.f;
+#pragma unroll 1
+            for (int c = 0; c < TC_KEYS / 32; c++) {
+                tmem_ld32(lane_base + c * 32, v);
+                tmem_wait_ld();
+                if (masked) {
+                    const int n0 = limit - __shfl_sync(~0u, group_pos, 2 * c), n1 = limit - __shfl_sync(~0u, group_pos, 2 * c + 1);
+#pragma unroll
+                    for (int i = 0; i < 32; i++)
+                        if ((i & 15) >= (i < 16 ? n0 : n1)) v[i] = 0xff800000u;
+                }
+                uint32_t w[16];
+#pragma unroll
+                for (int i = 0; i < 16; i++) {
+                    const float x0 = fast_exp2(fmaf(__uint_as_float(v[2 * i]), scale2, -m0));
+                    const float x1 = fast_exp2(fmaf(__uint_as_float(v[2 * i + 1]), scale2, -m0));
+                    l0 += x0;
+                    l1 += x1;
+                    w[i] = Pack<T>::two(x0, x1);
+                }
+                tmem_st16(lane_base + c * 16, w);           // over columns whose scores have been read
+            }
+            l += l0 + l1;
+            tmem_wait_st();
+            tc_fence_before();
+            mbar_arrive(smem_u32(&ctrl->p_full));
+        }
+        if (n_tiles && fine) fine = __all_sync(~0u, ws.wait(smem_u32(&ctrl->pv_done), n_tiles - 1, 9));
+        tc_fence_after();
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        const float lse2 = l == 0.f ? -CUDART_INF_F : (m == -CUDART_INF_F ? 0.f : m) + log2f(l);
+        const int64_t row = sq.row0 + query0 + y / G;
+        const int head = h * G + y % G;
+        const int64_t at = (row * a.heads + head) * p.n_split + split;
+#pragma unroll 1
+        for (int c = 0; c < D / 32; c++) {
+            uint32_t v[32];
+            if (n_tiles) {
+                tmem_ld32(lane_o + c * 32, v);
+                tmem_wait_ld();
+            }
+#pragma unroll
+            for (int i = 0; i < 32; i++)
+                v[i] = !fine ? 0x7fc00000u : n_tiles ? __float_as_uint(__uint_as_float(v[i]) * inv) : 0u;
+            if (r < rows) {
+                if (p.n_split == 1) {
+                    T *dst = static_cast<T *>(a.d_o) + row * a.o_token + head * a.o_head + c * 32;
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        uint4 x;
+                        uint32_t *xs = reinterpret_cast<uint32_t *>(&x);
+#pragma unroll
+                        for (int k = 0; k < 4; k++)
+                            xs[k] = Pack<T>::two(__uint_as_float(v[8 * i + 2 * k]), __uint_as_float(v[8 * i + 2 * k + 1]));
+                        reinterpret_cast<uint4 *>(dst)[i] = x;
+                    }
+                } else {
+                    float4 *dst = reinterpret_cast<float4 *>(part_o + at * D + c * 32);
+#pragma unroll
+                    for (int i = 0; i < 8; i++)
+                        dst[i] = make_float4(__uint_as_float(v[4 * i]), __uint_as_float(v[4 * i + 1]),
+                                             __uint_as_float(v[4 * i + 2]), __uint_as_float(v[4 * i + 3]));
+                }
+            }
+        }
+        if (r < rows) {
+            if (p.n_split > 1) part_lse[at] = fine ? lse2 : CUDART_NAN_F;
+            else if (a.d_lse) a.d_lse[row * a.heads + head] = fine ? lse2 * LN2 : CUDART_NAN_F;
+        }
+        if (!fine && a.d_status) *a.d_status = SPAMM_ERR_DEVICE_WAIT;
+        tc_fence_before();
+    }
+    __syncthreads();
+    if (warp == 4) {
+        // after an aborted wait products may still be in flight: they end before the tensor memory is given back
+        if (ctrl->abort_flag) {
+            if (lane == 0) umma_commit(smem_u32(&ctrl->q_full));
+            const unsigned long long t0 = global_ns();
+            while (global_ns() - t0 < 1000000ull) {}
+        }
+        __syncwarp();
+        tc_fence_after();
+        tmem_free<TC_COLS>(tmem);
+    }
+}
+
 // Joins the ranges of keys of every row: o = sum_i 2^(lse_i - lse) o_i.  One warp for a row and head.
 template <typename T, int D>
 __global__ __launch_bounds__(128) void attn_join_kernel(const __grid_constant__ spamm_attn a, int n_split,
@@ -368,18 +697,29 @@ static int64_t longest_list(const spamm_attn &a)
     return a.n_select ? min(a.n_select, attn_max_blocks(a)) : attn_max_blocks(a);
 }
 
-static RowsPlan rows_plan(const spamm_attn &a, int tile_rows)
+// Rows that share keys: the queries of a query block times the heads of a key head.  From MIN_TC_ROWS on they go to the
+// kernel with tiles of 128 rows.
+constexpr int MIN_TC_ROWS = 48;
+static bool use_tc(const spamm_attn &a)
+{
+    const int64_t bq = a.n_select ? min(a.query_block, a.max_q) : a.max_q;
+    return bq * (a.heads / a.kv_heads) >= MIN_TC_ROWS;
+}
+
+static RowsPlan rows_plan(const spamm_attn &a)
 {
     RowsPlan p;
     const int G = a.heads / a.kv_heads;
+    const bool tc = use_tc(a);
+    const int tile_rows = tc ? TC_ROWS : 16;
     p.bq = a.n_select ? min(a.query_block, a.max_q) : a.max_q;
     p.nqb = ceil_div(a.max_q, p.bq);
     p.tiles = (int)(((int64_t)p.bq * G + tile_rows - 1) / tile_rows);
     const int64_t blocks = max((int64_t)1, longest_list(a));
     const int64_t units = (int64_t)a.batch * a.kv_heads * p.nqb * p.tiles;
     // enough blocks of threads to fill 148 SMs twice over, ranges of 256 keys at the least
-    int64_t want = (600 + units - 1) / units;
-    want = max((int64_t)1, min(want, (blocks * a.block + 255) / 256));
+    int64_t want = ((tc ? 1200 : 600) + units - 1) / units;
+    want = max((int64_t)1, min(want, (blocks * a.block + (tc ? 1023 : 255)) / (tc ? 1024 : 256)));
     int64_t per = min((int64_t)SPAMM_ATTN_MAX_SELECT, (blocks + want - 1) / want);
     p.n_split = (int)((blocks + per - 1) / per);
     p.max_entries = (int)per;
@@ -396,16 +736,23 @@ static size_t rows_smem(const spamm_attn &a, const RowsPlan &p)
 template <typename T, int D>
 static int forward_launch(const spamm_attn &a, float *scratch, cudaStream_t stream)
 {
-    const RowsPlan p = rows_plan(a, 16);
+    const RowsPlan p = rows_plan(a);
     const int64_t grid = (int64_t)a.batch * a.kv_heads * p.nqb * p.tiles * p.n_split;
     const int64_t rows = (int64_t)a.batch * a.max_q * a.heads;
     if (grid > INT32_MAX || (rows + 3) / 4 > INT32_MAX) return attn_too_large();
     float *part_o = scratch;
     float *part_lse = scratch + (size_t)a.tokens * a.heads * p.n_split * D;
-    const size_t smem = rows_smem(a, p);
-    int st = attn_set_smem((const void *)attn_rows_kernel<T, D>, smem);
-    if (st) return st;
-    attn_rows_kernel<T, D><<<(unsigned)grid, 128, smem, stream>>>(a, p, part_o, part_lse);
+    if (use_tc(a)) {
+        const size_t smem = 1024 + 3 * TC_ROWS * D * 2 + sizeof(TcCtrl) + 8 * (size_t)p.max_entries + 4 * (size_t)max(a.n_select, p.max_entries);
+        int st = attn_set_smem((const void *)attn_tc_kernel<T, D>, smem);
+        if (st) return st;
+        attn_tc_kernel<T, D><<<(unsigned)grid, TC_THREADS, smem, stream>>>(a, p, part_o, part_lse);
+    } else {
+        const size_t smem = rows_smem(a, p);
+        int st = attn_set_smem((const void *)attn_rows_kernel<T, D>, smem);
+        if (st) return st;
+        attn_rows_kernel<T, D><<<(unsigned)grid, 128, smem, stream>>>(a, p, part_o, part_lse);
+    }
     if (p.n_split > 1)
         attn_join_kernel<T, D><<<(unsigned)((rows + 3) / 4), 128, 0, stream>>>(a, p.n_split, part_o, part_lse);
     SPAMM_CUDA_TRY(cudaGetLastError());
@@ -419,7 +766,7 @@ using namespace spamm;
 extern "C" size_t spamm_attn_forward_scratch_bytes(const spamm_attn *a)
 {
     if (attn_check(a, false) || !a->batch || !a->max_q || !a->tokens) return 0;
-    const RowsPlan p = rows_plan(*a, 16);
+    const RowsPlan p = rows_plan(*a);
     return p.n_split > 1 ? (size_t)a->tokens * a->heads * p.n_split * (a->dim + 1) * sizeof(float) : 0;
 }
 

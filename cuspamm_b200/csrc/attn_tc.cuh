@@ -1,0 +1,95 @@
+// What the tcgen05 attention kernels share.  Operand tiles lie in shared memory as panels of 64 values: rows of 128 bytes
+// whose 16-byte pieces are XORed with the row number (the 128-byte swizzle), groups of 8 rows 1024 bytes apart.  The same
+// tile serves as an operand whose rows are M or N (K-major: values along K) and as one whose rows are K (MN-major).
+#pragma once
+#include "attn.cuh"
+#include "tc_utils.cuh"
+
+namespace spamm {
+
+// Byte offset of 16-byte piece c (0 .. D/8-1) of row r in a tile of `rows` rows.
+__device__ __forceinline__ uint32_t panel_off(int rows, int r, int c)
+{
+    return (c >> 3) * (rows * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4);
+}
+
+constexpr uint32_t DESC_HI = (1024u >> 4) | (1u << 14) | (2u << 29);     // 8-row groups 1024 bytes apart, 128-byte swizzle
+// Rows are M or N; K step ks of 16 values.
+__device__ __forceinline__ uint64_t desc_k_major(uint32_t tile, int rows, int ks)
+{
+    const uint32_t addr = tile + (ks >> 2) * (rows * 128) + (ks & 3) * 32;
+    return ((uint64_t)DESC_HI << 32) | ((addr & 0x3ffffu) >> 4) | (1u << 16);
+}
+// Rows are K; K step ks of 16 rows; panels of 64 values of M or N lie rows * 128 bytes apart.
+__device__ __forceinline__ uint64_t desc_mn_major(uint32_t tile, int rows, int ks)
+{
+    const uint32_t addr = tile + ks * 2048;
+    return ((uint64_t)DESC_HI << 32) | ((addr & 0x3ffffu) >> 4) | ((uint32_t)(rows * 128) >> 4 << 16);
+}
+
+template <typename T> struct IsBf { static constexpr uint32_t value = 0; };
+template <> struct IsBf<__nv_bfloat16> { static constexpr uint32_t value = 1; };
+// Instruction descriptor: float accumulator, A and B of type T, M x N; a_mn / b_mn: the operand's rows are K.
+template <typename T> __host__ __device__ constexpr uint32_t mma_desc(uint32_t m, uint32_t n, bool a_mn, bool b_mn)
+{
+    return (1u << 4) | (IsBf<T>::value << 7) | (IsBf<T>::value << 10) | ((uint32_t)a_mn << 15) | ((uint32_t)b_mn << 16) |
+           ((n >> 3) << 17) | ((m >> 4) << 24);
+}
+
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add)
+{
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc),
+                 "r"((uint32_t)add)
+                 : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a_tmem, uint64_t b, uint32_t idesc, bool add)
+{
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a_tmem), "l"(b), "r"(idesc),
+                 "r"((uint32_t)add)
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t *v)
+{
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+                 "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
+                 "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+                 "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t *v)
+{
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+                 "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, "
+                 "%24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
+                 "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+                 "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]),
+                 "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]),
+                 "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
+                 : "memory");
+}
+template <int COLS> __device__ __forceinline__ void tmem_alloc(uint32_t smem_slot)
+{
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_slot), "r"(COLS) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+}
+template <int COLS> __device__ __forceinline__ void tmem_free(uint32_t base)
+{
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(base), "r"(COLS) : "memory");
+}
+// What this thread's ordinary stores (cp.async, st.shared) left in shared memory becomes visible to tcgen05.mma.
+__device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+// Barriers of a kernel and its abort flag: a wait that runs out (never, unless the kernel is wrong) sets the flag, every
+// role leaves its loop, and the results of the tile become NaN.
+struct WaitState {
+    volatile uint32_t *abort_flag;
+    int32_t *err;                       // in shared memory
+    __device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, int code) const
+    {
+        return wait_bounded(bar, parity & 1u, abort_flag, err, code);
+    }
+};
+
+}  // namespace spamm
