@@ -5,6 +5,8 @@
 // over the keys j of the blocks on the list of query i's block that i may see.  One pass over the keys with a running
 // maximum and sum (both float); p is rounded to the type of v for the product, as v itself is.
 #include <stdio.h>
+#include <string.h>
+#include <cudaTypedefs.h>
 #include "attn.cuh"
 #include "attn_tc.cuh"
 
@@ -334,12 +336,13 @@ __global__ __launch_bounds__(128) void attn_rows_kernel(const __grid_constant__ 
 // one behind the other) at a time.  S = Q K^T goes to tensor memory; four warps, a thread for each row, take the running
 // maximum and write p over S in the type of v; O += P V takes p from tensor memory.  A block uses half of the tensor
 // memory and under half of the shared memory, so that two of them share an SM: one's exponentials run beside the other's
-// products.  Four warps feed K and V with 16-byte copies (rows gathered block by block, keys behind the end zero).
+// products.  One warp feeds K and V, a tensor copy for each block of keys and 64 values; the block in which the sequence
+// ends is copied 16 bytes a time with zeros behind the last key (what lies there may be NaN).
 //
 // The running maximum is only raised when a row's scores exceed it by more than 2^8: until then p stays below 2^8, which
 // both types and the float sums hold without loss, and O need not be rescaled in tensor memory.
 constexpr int TC_ROWS = 128, TC_KEYS = 128;
-constexpr int TC_SOFTMAX = 128, TC_LOADERS = 128, TC_THREADS = TC_SOFTMAX + 32 + TC_LOADERS;
+constexpr int TC_SOFTMAX = 128, TC_THREADS = TC_SOFTMAX + 64;
 constexpr int TC_COLS = 256;            // S (P over it) in columns 0..127, O behind
 
 struct TcCtrl {
@@ -352,7 +355,9 @@ struct TcCtrl {
 
 template <typename T, int D>
 __global__ __launch_bounds__(TC_THREADS, 2) void attn_tc_kernel(const __grid_constant__ spamm_attn a, const RowsPlan p,
-                                                                float *part_o, float *part_lse)
+                                                                const __grid_constant__ RowMap k_map,
+                                                                const __grid_constant__ RowMap v_map, float *part_o,
+                                                                float *part_lse)
 {
     extern __shared__ __align__(16) uint8_t smem_raw[];
     constexpr int TILE = 128 * D * 2;
@@ -391,9 +396,9 @@ __global__ __launch_bounds__(TC_THREADS, 2) void attn_tc_kernel(const __grid_con
             ctrl->count = ceil_div(limit_max, a.block);
     } else if (warp == 4) {
         if (lane == 0) {
-            mbar_init(smem_u32(&ctrl->q_full), TC_LOADERS);
-            mbar_init(smem_u32(&ctrl->k_full), TC_LOADERS);
-            mbar_init(smem_u32(&ctrl->v_full), TC_LOADERS);
+            mbar_init(smem_u32(&ctrl->q_full), TC_SOFTMAX);
+            mbar_init(smem_u32(&ctrl->k_full), 32);
+            mbar_init(smem_u32(&ctrl->v_full), 32);
             mbar_init(smem_u32(&ctrl->k_empty), 1);
             mbar_init(smem_u32(&ctrl->v_empty), 1);
             mbar_init(smem_u32(&ctrl->s_full), 1);
@@ -413,10 +418,11 @@ __global__ __launch_bounds__(TC_THREADS, 2) void attn_tc_kernel(const __grid_con
     const int e0 = min(split * per_split, ctrl->count), n_entries = min(per_split, ctrl->count - e0);
     // first position of every block of the range (far behind every limit for a page that does not exist) and where its
     // rows of k begin
-    int my_pos[4];
+    int my_pos[6];
     for (int i = 0, e = tid; e < n_entries; e += TC_THREADS, i++) {
         const int b = a.n_select ? blk[e0 + e] : e0 + e;
-        const int64_t at = attn_block_base(a, sq, s, h, b, a.k_token, a.k_head);
+        int64_t at = attn_block_base(a, sq, s, h, b, a.k_token, a.k_head);
+        if (a.n_pages && at >= 0) at /= a.block * D;                   // pages: page * kv_heads + h
         base[e] = at;
         my_pos[i] = at < 0 ? INT32_MAX / 2 : b * a.block;
     }
@@ -429,55 +435,62 @@ __global__ __launch_bounds__(TC_THREADS, 2) void attn_tc_kernel(const __grid_con
     const uint32_t tmem = ctrl->tmem_base, tmem_o = tmem + TC_KEYS;
     const WaitState ws{&ctrl->abort_flag, &ctrl->err};
 
-    if (warp >= 5) {
-        // ---- loaders
-        const int t = tid - (TC_SOFTMAX + 32);
-        constexpr int PER = 128 * (D / 8) / TC_LOADERS;
-        for (int i = 0; i < PER; i++) {
-            const int x = i * TC_LOADERS + t, r = x / (D / 8), c = x % (D / 8);
-            const bool ok = r < rows;
-            const int y = tile * TC_ROWS + (ok ? r : 0);
-            const int64_t off = (int64_t)(sq.row0 + query0 + y / G) * a.q_token + (int64_t)(h * G + y % G) * a.q_head;
-            cp_async16(q_tile + panel_off(128, r, c), static_cast<const T *>(a.d_q) + off + c * 8, ok);
-        }
-        cp_commit();
+    if (warp == 5) {
+        // ---- K and V
         const int64_t k_tok = a.n_pages ? D : a.k_token, v_tok = a.n_pages ? D : a.v_token;
-        // signals that the copies before the last `left` groups have arrived
-        auto signal = [&](uint64_t *bar) {
-            fence_async_smem();
-            mbar_arrive(smem_u32(bar));
-        };
-        auto load = [&](int j, bool value) {
-            const uint32_t dst = value ? v_tile : k_tile;
+        const int per_tile = max(1, TC_KEYS >> log_block);
+        // every lane takes part in the barrier's phase with the bytes of its tensor copies and one arrival
+        auto load = [&](int j, bool value, uint64_t *full) {
+            const uint32_t dst = value ? v_tile : k_tile, bar = smem_u32(full);
+            const RowMap &rm = value ? v_map : k_map;
+            const T *src0 = static_cast<const T *>(value ? a.d_v : a.d_k);
             const int64_t tok = value ? v_tok : k_tok;
-            const T *src = static_cast<const T *>(value ? a.d_v : a.d_k);
-#pragma unroll 4
-            for (int i = 0; i < PER; i++) {
-                const int x = i * TC_LOADERS + t, r = x / (D / 8), c = x % (D / 8);
-                const int key = j * TC_KEYS + r, e = key >> log_block, off = key & (a.block - 1);
-                const bool ok = e < n_entries && blk[e] + off < limit_max;
-                int64_t at = 0;
-                if (ok) at = (value && !a.n_pages ? (int64_t)(sq.row0 + blk[e]) * a.v_token + h * a.v_head : base[e]) + off * tok;
-                cp_async16(dst + panel_off(128, r, c), src + at + c * 8, ok);
+            bool by_hand = false;
+            for (int x = lane; x < per_tile * (D / 64); x += 32) {
+                const int i = x / (D / 64), panel = x % (D / 64), e = j * per_tile + i;
+                if (e >= n_entries) continue;
+                const int pos = blk[e];
+                if (!rm.usable || pos + a.block > sq.nk) { by_hand = true; continue; }
+                int y = 0, z = (int)base[e];
+                if (!a.n_pages) {
+                    y = rm.swapped ? sq.row0 + pos : h;
+                    z = rm.swapped ? h : sq.row0 + pos;
+                }
+                mbar_expect_tx(bar, a.block * 128);
+                tma_box(dst + panel * (128 * 128) + (i << log_block) * 128, &rm.map, panel * 64, y, z, bar);
             }
-            cp_commit();
+            if (__any_sync(~0u, by_hand)) {
+                for (int i = 0; i < per_tile; i++) {
+                    const int e = j * per_tile + i;
+                    if (e >= n_entries) break;
+                    const int pos = blk[e];
+                    if (rm.usable && pos + a.block <= sq.nk) continue;
+                    const int n = sq.nk - pos;                         // none of a page that does not exist
+                    int64_t at = 0;
+                    if (n > 0) {
+                        if (a.n_pages) at = base[e] * a.block * D;
+                        else at = (int64_t)(sq.row0 + pos) * tok + h * (value ? a.v_head : a.k_head);
+                    }
+                    for (int x = lane; x < a.block * (D / 8); x += 32) {
+                        const int r = x / (D / 8), c = x % (D / 8);
+                        cp_async16(dst + panel_off(128, (i << log_block) + r, c), src0 + (r < n ? at + r * tok : 0) + c * 8, r < n);
+                    }
+                }
+                cp_commit();
+                cp_wait<0>();
+                fence_async_smem();
+            }
+            mbar_arrive(bar);
         };
         bool fine = true;
-        for (int j = 0; j < n_tiles && fine; j++) {
-            if (j) fine = ws.wait(smem_u32(&ctrl->k_empty), j - 1, 1);
+        for (int j = 0; j < n_tiles; j++) {
+            if (j) fine = __all_sync(~0u, ws.wait(smem_u32(&ctrl->k_empty), j - 1, 1));
             if (!fine) break;
-            load(j, false);
-            // the group before this one: the queries, or the values of the tile before
-            cp_wait<1>();
-            signal(j ? &ctrl->v_full : &ctrl->q_full);
-            if (j) fine = ws.wait(smem_u32(&ctrl->v_empty), j - 1, 2);
+            load(j, false, &ctrl->k_full);
+            if (j) fine = __all_sync(~0u, ws.wait(smem_u32(&ctrl->v_empty), j - 1, 2));
             if (!fine) break;
-            load(j, true);
-            cp_wait<1>();
-            signal(&ctrl->k_full);
+            load(j, true, &ctrl->v_full);
         }
-        cp_wait<0>();
-        if (n_tiles && fine) signal(&ctrl->v_full);
     } else if (warp == 4) {
         // ---- products
         if (lane == 0 && n_tiles) {
@@ -488,9 +501,11 @@ __global__ __launch_bounds__(TC_THREADS, 2) void attn_tc_kernel(const __grid_con
                     fine = ws.wait(smem_u32(&ctrl->p_full), j - 1, 4) && ws.wait(smem_u32(&ctrl->v_full), j - 1, 5);
                     if (!fine) break;
                     tc_fence_after();
+                    // keys behind the last block of the range take no part: their rows of V were never written
+                    const int steps = min(TC_KEYS, n_keys - (j - 1) * TC_KEYS) / 16;
 #pragma unroll
                     for (int ks = 0; ks < TC_KEYS / 16; ks++)
-                        mma_ts(tmem_o, tmem + ks * 8, desc_mn_major(v_tile, 128, ks), o_desc, j > 1 || ks);
+                        if (ks < steps) mma_ts(tmem_o, tmem + ks * 8, desc_mn_major(v_tile, 128, ks), o_desc, j > 1 || ks);
                     umma_commit(smem_u32(&ctrl->v_empty));
                     umma_commit(smem_u32(&ctrl->pv_done));
                 }
@@ -510,6 +525,17 @@ __global__ __launch_bounds__(TC_THREADS, 2) void attn_tc_kernel(const __grid_con
         __syncwarp();
     } else {
         // ---- softmax: thread = row
+        for (int i = 0; i < D / 8; i++) {
+            const int x = i * TC_SOFTMAX + tid, qr = x / (D / 8), c = x % (D / 8);
+            const bool ok = qr < rows;
+            const int qy = tile * TC_ROWS + (ok ? qr : 0);
+            const int64_t off = (int64_t)(sq.row0 + query0 + qy / G) * a.q_token + (int64_t)(h * G + qy % G) * a.q_head;
+            cp_async16(q_tile + panel_off(128, qr, c), static_cast<const T *>(a.d_q) + off + c * 8, ok);
+        }
+        cp_commit();
+        cp_wait<0>();
+        fence_async_smem();
+        mbar_arrive(smem_u32(&ctrl->q_full));
         const uint32_t lane_base = tmem + ((uint32_t)(warp * 32) << 16), lane_o = tmem_o + ((uint32_t)(warp * 32) << 16);
         const int r = tid;
         const int y = tile * TC_ROWS + min(r, rows - 1);
@@ -521,6 +547,9 @@ __global__ __launch_bounds__(TC_THREADS, 2) void attn_tc_kernel(const __grid_con
             fine = __all_sync(~0u, ws.wait(smem_u32(&ctrl->s_full), j, 7));
             if (!fine) break;
             tc_fence_after();
+            uint32_t v[TC_KEYS];
+#pragma unroll
+            for (int c = 0; c < TC_KEYS / 32; c++) tmem_ld32(lane_base + c * 32, v + c * 32);
             // positions of the tile's eight groups of 16 keys; all visible to all rows in most tiles
             int group_pos = INT32_MAX / 2;
             if (lane < TC_KEYS / 16) {
@@ -528,71 +557,60 @@ __global__ __launch_bounds__(TC_THREADS, 2) void attn_tc_kernel(const __grid_con
                 if (e < n_entries) group_pos = blk[e] + (key & (a.block - 1));
             }
             const bool masked = __any_sync(~0u, lane < TC_KEYS / 16 && group_pos > limit_min - 16);
-            float top = -CUDART_INF_F;
-            uint32_t v[32];
-#pragma unroll 1
-            for (int c = 0; c < TC_KEYS / 32; c++) {
-                tmem_ld32(lane_base + c * 32, v);
-                tmem_wait_ld();
-                if (masked) {
-                    const int n0 = limit - __shfl_sync(~0u, group_pos, 2 * c), n1 = limit - __shfl_sync(~0u, group_pos, 2 * c + 1);
+            tmem_wait_ld();
+            tmem_landed<TC_KEYS>(v);
+            if (masked) {
 #pragma unroll
-                    for (int i = 0; i < 32; i++)
-                        if ((i & 15) >= (i < 16 ? n0 : n1)) v[i] = 0xff800000u;
-                }
-                float t0 = __uint_as_float(v[0]), t1 = __uint_as_float(v[1]);
+                for (int g = 0; g < TC_KEYS / 16; g++) {
+                    const int n = limit - __shfl_sync(~0u, group_pos, g);
 #pragma unroll
-                for (int i = 2; i < 32; i += 2) {
-                    t0 = fmaxf(t0, __uint_as_float(v[i]));
-                    t1 = fmaxf(t1, __uint_as_float(v[i + 1]));
+                    for (int i = 0; i < 16; i++)
+                        if (i >= n) v[g * 16 + i] = 0xff800000u;
                 }
-                top = fmaxf(top, fmaxf(t0, t1));
             }
-            top *= scale2;
+            float t0 = __uint_as_float(v[0]), t1 = __uint_as_float(v[1]), t2 = __uint_as_float(v[2]), t3 = __uint_as_float(v[3]);
+#pragma unroll
+            for (int i = 0; i < TC_KEYS; i += 8) {
+                t0 = fmaxf(t0, fmaxf(__uint_as_float(v[i]), __uint_as_float(v[i + 1])));
+                t1 = fmaxf(t1, fmaxf(__uint_as_float(v[i + 2]), __uint_as_float(v[i + 3])));
+                t2 = fmaxf(t2, fmaxf(__uint_as_float(v[i + 4]), __uint_as_float(v[i + 5])));
+                t3 = fmaxf(t3, fmaxf(__uint_as_float(v[i + 6]), __uint_as_float(v[i + 7])));
+            }
+            const float top = fmaxf(fmaxf(t0, t1), fmaxf(t2, t3)) * scale2;
             const bool raise = top > m + 8.f || (m == -CUDART_INF_F && top > m);
             if (__any_sync(~0u, raise)) {
                 const float f = raise ? fast_exp2(m - top) : 1.f;
                 if (raise) { m = top; l *= f; }
+                // the products before this S are complete, O is at rest
                 if (j) {
-                    // O of the tiles before must be complete before it is rescaled
-                    fine = __all_sync(~0u, ws.wait(smem_u32(&ctrl->pv_done), j - 1, 8));
-                    if (!fine) break;
-                    tc_fence_after();
 #pragma unroll 1
-                    for (int c = 0; c < D / 32; c++) {
-                        tmem_ld32(lane_o + c * 32, v);
+                    for (int c = 0; c < D / 16; c++) {
+                        uint32_t w[16];
+                        tmem_ld16(lane_o + c * 16, w);
                         tmem_wait_ld();
+                        tmem_landed<16>(w);
 #pragma unroll
-                        for (int i = 0; i < 32; i++) v[i] = __float_as_uint(__uint_as_float(v[i]) * f);
-                        tmem_st32(lane_o + c * 32, v);
+                        for (int i = 0; i < 16; i++) w[i] = __float_as_uint(__uint_as_float(w[i]) * f);
+                        tmem_st16(lane_o + c * 16, w);
                     }
-                    tmem_wait_st();
                 }
             }
             const float m0 = m == -CUDART_INF_F ? 0.f : m;
-            float l0 = 0.f, l1 = 0.f;
-#pragma unroll 1
-            for (int c = 0; c < TC_KEYS / 32; c++) {
-                tmem_ld32(lane_base + c * 32, v);
-                tmem_wait_ld();
-                if (masked) {
-                    const int n0 = limit - __shfl_sync(~0u, group_pos, 2 * c), n1 = limit - __shfl_sync(~0u, group_pos, 2 * c + 1);
+            const float2 scale22 = make_float2(scale2, scale2), minus_m = make_float2(-m0, -m0);
+            float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
-                    for (int i = 0; i < 32; i++)
-                        if ((i & 15) >= (i < 16 ? n0 : n1)) v[i] = 0xff800000u;
-                }
+            for (int c = 0; c < TC_KEYS / 32; c++) {
                 uint32_t w[16];
 #pragma unroll
                 for (int i = 0; i < 16; i++) {
-                    const float x0 = fast_exp2(fmaf(__uint_as_float(v[2 * i]), scale2, -m0));
-                    const float x1 = fast_exp2(fmaf(__uint_as_float(v[2 * i + 1]), scale2, -m0));
-                    l0 += x0;
-                    l1 += x1;
-                    w[i] = Pack<T>::two(x0, x1);
+                    const float2 x = fma2(make_float2(__uint_as_float(v[c * 32 + 2 * i]), __uint_as_float(v[c * 32 + 2 * i + 1])), scale22, minus_m);
+                    const float2 e = make_float2(fast_exp2(x.x), fast_exp2(x.y));
+                    sum = add2(sum, e);
+                    w[i] = Pack<T>::two(e.x, e.y);
                 }
-                tmem_st16(lane_base + c * 16, w);           // over columns whose scores have been read
+                tmem_st16(lane_base + c * 16, w);           // over S, which is in registers
             }
-            l += l0 + l1;
+            l += sum.x + sum.y;
             tmem_wait_st();
             tc_fence_before();
             mbar_arrive(smem_u32(&ctrl->p_full));
@@ -610,6 +628,7 @@ __global__ __launch_bounds__(TC_THREADS, 2) void attn_tc_kernel(const __grid_con
             if (n_tiles) {
                 tmem_ld32(lane_o + c * 32, v);
                 tmem_wait_ld();
+                tmem_landed<32>(v);
             }
 #pragma unroll
             for (int i = 0; i < 32; i++)
@@ -692,6 +711,54 @@ __global__ __launch_bounds__(128) void attn_join_kernel(const __grid_constant__ 
     if (a.d_lse && lane == 0) a.d_lse[row * a.heads + head] = total == 0.f ? -CUDART_INF_F : (t0 + log2f(total)) * LN2;
 }
 
+// cuTensorMapEncodeTiled of the driver, looked up once through the runtime (the library does not link the driver).
+static PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder()
+{
+    static PFN_cuTensorMapEncodeTiled_v12000 fn = [] {
+        void *p = nullptr;
+        cudaDriverEntryPointQueryResult found;
+        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &found) != cudaSuccess ||
+            found != cudaDriverEntryPointSuccess)
+            p = nullptr;
+        return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
+    }();
+    return fn;
+}
+
+static void row_map(const spamm_attn &a, const void *p, int64_t token, int64_t head, RowMap *out)
+{
+    memset(out, 0, sizeof(*out));
+    const auto encode = tensor_map_encoder();
+    if (!encode) return;
+    cuuint64_t dims[3] = {(cuuint64_t)a.dim}, strides[2];
+    cuuint32_t box[3] = {64, 1, 1}, step[3] = {1, 1, 1};
+    if (a.n_pages) {
+        if ((int64_t)a.n_pages * a.kv_heads > INT32_MAX) return;
+        dims[1] = a.block; dims[2] = (cuuint64_t)a.n_pages * a.kv_heads;
+        strides[0] = (cuuint64_t)a.dim * 2; strides[1] = (cuuint64_t)a.block * a.dim * 2;
+        box[1] = a.block;
+    } else {
+        // the larger stride last, a multiple of the smaller
+        if (a.kv_heads == 1) head = a.dim;
+        if (token <= 0 || head <= 0 || token >= (1ll << 38) || head >= (1ll << 38)) return;
+        out->swapped = head > token;
+        const int t = out->swapped ? 1 : 2, h = 3 - t;
+        if ((out->swapped ? head % token : token % head) != 0) return;
+        dims[t] = a.tokens; dims[h] = a.kv_heads;
+        strides[t - 1] = (cuuint64_t)token * 2; strides[h - 1] = (cuuint64_t)head * 2;
+        box[t] = a.block;
+    }
+    const CUtensorMapDataType type = a.dtype == SPAMM_ATTN_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+    out->usable = encode(&out->map, type, 3, const_cast<void *>(p), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+void attn_row_maps(const spamm_attn &a, RowMap *k, RowMap *v)
+{
+    row_map(a, a.d_k, a.k_token, a.k_head, k);
+    row_map(a, a.d_v, a.v_token, a.v_head, v);
+}
+
 static int64_t longest_list(const spamm_attn &a)
 {
     return a.n_select ? min(a.n_select, attn_max_blocks(a)) : attn_max_blocks(a);
@@ -746,7 +813,9 @@ static int forward_launch(const spamm_attn &a, float *scratch, cudaStream_t stre
         const size_t smem = 1024 + 3 * TC_ROWS * D * 2 + sizeof(TcCtrl) + 8 * (size_t)p.max_entries + 4 * (size_t)max(a.n_select, p.max_entries);
         int st = attn_set_smem((const void *)attn_tc_kernel<T, D>, smem);
         if (st) return st;
-        attn_tc_kernel<T, D><<<(unsigned)grid, TC_THREADS, smem, stream>>>(a, p, part_o, part_lse);
+        RowMap k_map, v_map;
+        attn_row_maps(a, &k_map, &v_map);
+        attn_tc_kernel<T, D><<<(unsigned)grid, TC_THREADS, smem, stream>>>(a, p, k_map, v_map, part_o, part_lse);
     } else {
         const size_t smem = rows_smem(a, p);
         int st = attn_set_smem((const void *)attn_rows_kernel<T, D>, smem);

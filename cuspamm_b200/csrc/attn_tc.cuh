@@ -2,6 +2,7 @@
 // whose 16-byte pieces are XORed with the row number (the 128-byte swizzle), groups of 8 rows 1024 bytes apart.  The same
 // tile serves as an operand whose rows are M or N (K-major: values along K) and as one whose rows are K (MN-major).
 #pragma once
+#include <cuda.h>
 #include "attn.cuh"
 #include "tc_utils.cuh"
 
@@ -50,6 +51,15 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a_tmem, uint64_t b, 
                  "r"((uint32_t)add)
                  : "memory");
 }
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t *v)
+{
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+                 "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
+                   "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+                 : "r"(taddr)
+                 : "memory");
+}
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t *v)
 {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
@@ -69,6 +79,12 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t *v)
                  "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
                  : "memory");
 }
+// After tmem_wait_ld: keeps the compiler from using loaded values before the wait.
+template <int N> __device__ __forceinline__ void tmem_landed(uint32_t *v)
+{
+#pragma unroll
+    for (int i = 0; i < N; i++) asm volatile("" : "+r"(v[i]));
+}
 template <int COLS> __device__ __forceinline__ void tmem_alloc(uint32_t smem_slot)
 {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_slot), "r"(COLS) : "memory");
@@ -80,6 +96,42 @@ template <int COLS> __device__ __forceinline__ void tmem_free(uint32_t base)
 }
 // What this thread's ordinary stores (cp.async, st.shared) left in shared memory becomes visible to tcgen05.mma.
 __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+// A tensor map over the rows of k or v: boxes of one block of keys x 64 values.  Coordinates (value, y, z) of the block that
+// begins at row `row` of key head h: packed (value, h or row, row or h), pages (value, 0, page * kv_heads + h).
+struct RowMap {
+    CUtensorMap map;
+    int usable;          // 0: the strides do not fit a tensor map, rows are copied 16 bytes at a time
+    int swapped;         // packed: the head is the third coordinate
+};
+// Fills both maps (pages: strides are not read).
+void attn_row_maps(const spamm_attn &a, RowMap *k, RowMap *v);
+
+__device__ __forceinline__ void tma_box(uint32_t dst, const CUtensorMap *map, int x, int y, int z, uint32_t bar)
+{
+    asm volatile("cp.async.bulk.tensor.3d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+                 "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar)
+                 : "memory");
+}
+
+// Two float operations in one instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c)
+{
+    float2 d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;"
+        : "=l"(*reinterpret_cast<unsigned long long *>(&d))
+        : "l"(*reinterpret_cast<unsigned long long *>(&a)), "l"(*reinterpret_cast<unsigned long long *>(&b)),
+          "l"(*reinterpret_cast<unsigned long long *>(&c)));
+    return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b)
+{
+    float2 d;
+    asm("add.rn.f32x2 %0, %1, %2;"
+        : "=l"(*reinterpret_cast<unsigned long long *>(&d))
+        : "l"(*reinterpret_cast<unsigned long long *>(&a)), "l"(*reinterpret_cast<unsigned long long *>(&b)));
+    return d;
+}
 
 // Barriers of a kernel and its abort flag: a wait that runs out (never, unless the kernel is wrong) sets the flag, every
 // role leaves its loop, and the results of the tile become NaN.
