@@ -45,7 +45,7 @@ class SpammAttn(C.Structure):
         + [("scale", C.c_float), ("d_cu", C.c_void_p), ("d_lengths", C.c_void_p), ("d_table", C.c_void_p),
            ("table_stride", C.c_int64), ("d_lists", C.c_void_p)]
         + [f for x in "qkvo" for f in ((f"d_{x}", C.c_void_p), (f"{x}_token", C.c_int64), (f"{x}_head", C.c_int64))]
-        + [("d_lse", C.c_void_p), ("d_status", C.c_void_p)]
+        + [("d_lse", C.c_void_p), ("d_o_low", C.c_void_p), ("d_status", C.c_void_p)]
     )
 
 

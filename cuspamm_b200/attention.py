@@ -200,11 +200,14 @@ class _BlockSparseAttention(torch.autograd.Function):
             lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device)
             _set_out(a, o)
             a.d_lse = lse.data_ptr()
+            # what the rounding of o left, for the backward's do.o: only where there will be one
+            low = torch.empty_like(o) if any(ctx.needs_input_grad[:3]) else None
+            a.d_o_low = low.data_ptr() if low is not None else None
             if not a.batch or not a.max_q:
                 o.zero_()
                 lse.fill_(float("-inf"))
             _forward(a, q.device)
-        ctx.save_for_backward(q, k, v, lists, cu_seqlens, o, lse)
+        ctx.save_for_backward(q, k, v, lists, cu_seqlens, o, low, lse)
         ctx.how = (max_seqlen, block, query_block, causal, scale)
         ctx.mark_non_differentiable(lse)
         return o, lse
@@ -212,14 +215,14 @@ class _BlockSparseAttention(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, d_o, _):
-        q, k, v, lists, cu_seqlens, o, lse = ctx.saved_tensors
+        q, k, v, lists, cu_seqlens, o, low, lse = ctx.saved_tensors
         max_seqlen, block, query_block, causal, scale = ctx.how
         a = _problem(q, k.shape[1], cu_seqlens, max_seqlen, block, query_block, 0, causal)
         a.scale = scale
         _set_keys(a, k, v)
         _set_lists(a, lists, q.device)
         _set_out(a, o)
-        a.d_lse = lse.data_ptr()
+        a.d_lse, a.d_o_low = lse.data_ptr(), low.data_ptr()
         # an expanded or oddly laid out gradient (the sum's, for one) is brought into rows first
         if d_o.numel() and (d_o.stride(2) != 1 or d_o.data_ptr() % 16 or any(st % 8 for st in _strides(d_o))):
             d_o = d_o.contiguous()

@@ -8,7 +8,7 @@
 // sums over its queries in ascending order and writes its rows once.  No atomics on gradients: the same inputs give the
 // same bits.  A block that very many queries list (the first one often is on every list) is cut into items of `chunk`
 // query blocks each, whose float partial sums a last kernel adds up in order.
-#include "attn.cuh"
+#include "attn_tc.cuh"
 
 namespace spamm {
 
@@ -88,10 +88,18 @@ __global__ __launch_bounds__(256) void attn_delta_kernel(const __grid_constant__
         const int d = (c * 8 + sub) * 8;
         const uint4 x = *reinterpret_cast<const uint4 *>(d_do + row * do_token + head * do_head + d);
         const uint4 y = *reinterpret_cast<const uint4 *>(static_cast<const T *>(a.d_o) + row * a.o_token + head * a.o_head + d);
+        uint4 z = make_uint4(0, 0, 0, 0);
+        if (a.d_o_low) z = *reinterpret_cast<const uint4 *>(static_cast<const T *>(a.d_o_low) + w * D + d);
         const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            const float2 u = Pack<T>::to2(xs[i]), v = Pack<T>::to2(ys[i]);
+            const float2 u = Pack<T>::to2(xs[i]);
+            float2 v = Pack<T>::to2(ys[i]);
+            if (a.d_o_low) {
+                const float2 w = Pack<T>::to2(reinterpret_cast<const uint32_t *>(&z)[i]);
+                v.x += w.x;
+                v.y += w.y;
+            }
             sum = fmaf(u.x, v.x, fmaf(u.y, v.y, sum));
         }
     }
@@ -330,6 +338,41 @@ __global__ __launch_bounds__(128) void attn_dq_rows_kernel(const __grid_constant
     }
 }
 
+// The set bits [want0, want0 + room) of a block's query blocks, in order, to `list`; how many there are.  All threads.
+template <int THREADS>
+static __device__ __forceinline__ int expand_bits(const unsigned *my_bits, int words, int want0, int room, int *list, int *warp_sum)
+{
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, want1 = want0 + room;
+    int found = 0;
+    for (int w0 = 0; w0 < words && found < want1; w0 += THREADS) {
+        unsigned word = w0 + tid < words ? my_bits[w0 + tid] : 0;
+        const int n = __popc(word);
+        int run = n;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const int u = __shfl_up_sync(~0u, run, d);
+            if (lane >= d) run += u;
+        }
+        __syncthreads();
+        if (lane == 31) warp_sum[warp] = run;
+        __syncthreads();
+        int at = found + run - n, all = 0;
+        for (int w = 0; w < THREADS / 32; w++) {
+            if (w < warp) at += warp_sum[w];
+            all += warp_sum[w];
+        }
+        while (word && at < want1) {
+            const int bit = __ffs(word) - 1;
+            word &= word - 1;
+            if (at >= want0) list[at - want0] = (w0 + tid) * 32 + bit;
+            at++;
+        }
+        found += all;
+    }
+    __syncthreads();
+    return min(max(found - want0, 0), room);
+}
+
 constexpr int DKV_ROWS = 64;      // query rows of a shared-memory tile
 constexpr int DKV_STAGES = 2;
 
@@ -372,37 +415,8 @@ __global__ __launch_bounds__(KEYS == 128 ? 256 : 128) void attn_dkv_kernel(
         cp_async16(smem_addr(k_tile) + tile_off<D>(r, c), static_cast<const T *>(a.d_k) + row * a.k_token + h * a.k_head + c * 8, ok);
         cp_async16(smem_addr(v_tile) + tile_off<D>(r, c), static_cast<const T *>(a.d_v) + row * a.v_token + h * a.v_head + c * 8, ok);
     }
-    // the query blocks [chunk * p.chunk, ...) among the set bits
-    const unsigned *my_bits = bits + (group * p.nkb + item.kb) * p.words;
-    const int want0 = item.chunk * p.chunk, want1 = want0 + p.chunk;
-    int found = 0;
-    for (int w0 = 0; w0 < p.words && found < want1; w0 += THREADS) {
-        unsigned word = w0 + tid < p.words ? my_bits[w0 + tid] : 0;
-        const int n = __popc(word);
-        int run = n;
-#pragma unroll
-        for (int d = 1; d < 32; d <<= 1) {
-            const int u = __shfl_up_sync(~0u, run, d);
-            if (lane >= d) run += u;
-        }
-        __syncthreads();
-        if (lane == 31) warp_sum[warp] = run;
-        __syncthreads();
-        int at = found + run - n, all = 0;
-        for (int w = 0; w < WARPS; w++) {
-            if (w < warp) at += warp_sum[w];
-            all += warp_sum[w];
-        }
-        while (word && at < want1) {
-            const int bit = __ffs(word) - 1;
-            word &= word - 1;
-            if (at >= want0) list[at - want0] = (w0 + tid) * 32 + bit;
-            at++;
-        }
-        found += all;
-    }
-    const int n_list = min(max(found - want0, 0), p.chunk);
-    __syncthreads();
+    const int n_list = expand_bits<THREADS>(bits + (group * p.nkb + item.kb) * p.words, p.words, item.chunk * p.chunk, p.chunk, list,
+                                            warp_sum);
     const int bq = min(a.query_block, a.max_q);
     const int per = bq * G;                                         // rows of a full query block
     // all listed query blocks are full but the sequence's last one, which can only be the last of the list
@@ -528,6 +542,551 @@ __global__ __launch_bounds__(KEYS == 128 ? 256 : 128) void attn_dkv_kernel(
     }
 }
 
+// ---- tiles of 128 rows on the tensor memory path
+//
+// dq: 128 rows (queries x heads of a key head), 64 listed keys at a time.  S = Q K^T and dP = dO V^T go to tensor memory, a
+// thread for each row writes ds over S, dQ += ds K takes it from there.  Half the tensor memory and half the shared memory:
+// two blocks of threads share an SM, one's exponentials run beside the other's products.
+constexpr int TQ_ROWS = 128, TQ_KEYS = 64, TQ_THREADS = 192, TQ_COLS = 256;
+
+struct TqCtrl {
+    uint64_t q_full, k_full[2], k_empty[2], v_full, v_empty, s_full, ds_full, dq_done;
+    uint32_t tmem_base;
+    uint32_t abort_flag;
+    int32_t err;
+    int32_t count;
+};
+
+template <typename T, int D>
+__global__ __launch_bounds__(TQ_THREADS, 2) void attn_dq_tc_kernel(const __grid_constant__ spamm_attn a, int nqb, int tiles,
+                                                                   const __grid_constant__ RowMap k_map,
+                                                                   const __grid_constant__ RowMap v_map, const T *d_do,
+                                                                   int64_t do_token, int64_t do_head, const float *delta, T *dq)
+{
+    extern __shared__ __align__(1024) uint8_t smem_tc[];
+    uint8_t *const smem = smem_tc;
+    constexpr int RT = TQ_ROWS * D * 2, KT = TQ_KEYS * D * 2;
+    const uint32_t q_tile = smem_u32(smem), do_tile = q_tile + RT, k_ring = do_tile + RT, v_tile = k_ring + 2 * KT;
+    TqCtrl *ctrl = reinterpret_cast<TqCtrl *>(smem + 2 * RT + 3 * KT);
+    int *blk = reinterpret_cast<int *>(ctrl + 1);
+
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    unsigned idx = blockIdx.x;
+    const int tile = idx % tiles; idx /= tiles;
+    const int qb = nqb - 1 - idx % nqb; idx /= nqb;
+    const int h = idx % a.kv_heads;
+    const int s = idx / a.kv_heads;
+    const int G = a.heads / a.kv_heads;
+    const Seq sq = attn_seq(a, s);
+    const int bq = min(a.query_block, a.max_q);
+    const int n_tok = min(bq, sq.nq - qb * bq);
+    const int64_t n_rows = (int64_t)max(n_tok, 0) * G;
+    if ((int64_t)tile * TQ_ROWS >= n_rows) return;
+    const int rows = (int)min((int64_t)TQ_ROWS, n_rows - tile * TQ_ROWS);
+    const int query0 = qb * bq;
+    const int limit_max = attn_limit(a, sq, query0 + (tile * TQ_ROWS + rows - 1) / G);
+    const int limit_min = attn_limit(a, sq, query0 + tile * TQ_ROWS / G);
+
+    if (warp == 0) {
+        const int n = attn_load_list(a, s, qb, nqb, h, ceil_div(limit_max, a.block), blk, lane);
+        if (lane == 0) ctrl->count = n;
+    } else if (warp == 4) {
+        if (lane == 0) {
+            mbar_init(smem_u32(&ctrl->q_full), 128);
+            for (int i = 0; i < 2; i++) {
+                mbar_init(smem_u32(&ctrl->k_full[i]), 32);
+                mbar_init(smem_u32(&ctrl->k_empty[i]), 1);
+            }
+            mbar_init(smem_u32(&ctrl->v_full), 32);
+            mbar_init(smem_u32(&ctrl->v_empty), 1);
+            mbar_init(smem_u32(&ctrl->s_full), 1);
+            mbar_init(smem_u32(&ctrl->ds_full), 128);
+            mbar_init(smem_u32(&ctrl->dq_done), 1);
+            ctrl->abort_flag = 0;
+            ctrl->err = 0;
+            asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        }
+        __syncwarp();
+        tmem_alloc<TQ_COLS>(smem_u32(&ctrl->tmem_base));
+        tc_fence_before();
+    }
+    __syncthreads();
+    tc_fence_after();
+    const int log_block = 31 - __clz(a.block);
+    const int n_entries = ctrl->count, n_keys = n_entries << log_block;
+    const int n_tiles = (n_keys + TQ_KEYS - 1) / TQ_KEYS;
+    const uint32_t tmem = ctrl->tmem_base, tmem_dp = tmem + TQ_KEYS, tmem_dq = tmem + 2 * TQ_KEYS;
+    const WaitState ws{&ctrl->abort_flag, &ctrl->err};
+
+    if (warp == 5) {
+        const int piece = min(a.block, TQ_KEYS), pieces = TQ_KEYS / piece;     // a piece: keys of one block, one tensor copy
+        auto load = [&](int j, uint32_t dst, bool value, uint64_t *full) {
+            const uint32_t bar = smem_u32(full);
+            const RowMap &rm = value ? v_map : k_map;
+            bool by_hand = false;
+            for (int x = lane; x < pieces * (D / 64); x += 32) {
+                const int i = x / (D / 64), panel = x % (D / 64), key = j * TQ_KEYS + i * piece, e = key >> log_block;
+                if (e >= n_entries) continue;
+                const int pos = blk[e] * a.block + (key & (a.block - 1));
+                if (!rm.usable || pos + piece > sq.nk) { by_hand = true; continue; }
+                mbar_expect_tx(bar, piece * 128);
+                tma_box(dst + panel * (TQ_KEYS * 128) + i * piece * 128, &rm.map, panel * 64, rm.swapped ? sq.row0 + pos : h,
+                        rm.swapped ? h : sq.row0 + pos, bar);
+            }
+            if (__any_sync(~0u, by_hand)) {
+                const T *src = static_cast<const T *>(value ? a.d_v : a.d_k);
+                const int64_t tok = value ? a.v_token : a.k_token, head = value ? a.v_head : a.k_head;
+                for (int i = 0; i < pieces; i++) {
+                    const int key = j * TQ_KEYS + i * piece, e = key >> log_block;
+                    if (e >= n_entries) break;
+                    const int pos = blk[e] * a.block + (key & (a.block - 1));
+                    if (rm.usable && pos + piece <= sq.nk) continue;
+                    const int n = sq.nk - pos;
+                    const int64_t at = n > 0 ? (int64_t)(sq.row0 + pos) * tok + h * head : 0;
+                    for (int x = lane; x < piece * (D / 8); x += 32) {
+                        const int r = x / (D / 8), c = x % (D / 8);
+                        cp_async16(dst + panel_off(TQ_KEYS, i * piece + r, c), src + (r < n ? at + r * tok : 0) + c * 8, r < n);
+                    }
+                }
+                cp_commit();
+                cp_wait<0>();
+                fence_async_smem();
+            }
+            mbar_arrive(bar);
+        };
+        bool fine = true;
+        for (int j = 0; j < n_tiles; j++) {
+            if (j > 1) fine = __all_sync(~0u, ws.wait(smem_u32(&ctrl->k_empty[j & 1]), (j >> 1) - 1, 1));
+            if (!fine) break;
+            load(j, k_ring + (j & 1) * KT, false, &ctrl->k_full[j & 1]);
+            if (j) fine = __all_sync(~0u, ws.wait(smem_u32(&ctrl->v_empty), j - 1, 2));
+            if (!fine) break;
+            load(j, v_tile, true, &ctrl->v_full);
+        }
+    } else if (warp == 4) {
+        if (lane == 0 && n_tiles) {
+            constexpr uint32_t s_desc = mma_desc<T>(128, TQ_KEYS, false, false), q_desc = mma_desc<T>(128, D, false, true);
+            bool fine = ws.wait(smem_u32(&ctrl->q_full), 0, 3);
+            for (int j = 0; j < n_tiles && fine; j++) {
+                const uint32_t k_tile = k_ring + (j & 1) * KT;
+                fine = ws.wait(smem_u32(&ctrl->k_full[j & 1]), j >> 1, 4) && ws.wait(smem_u32(&ctrl->v_full), j, 5);
+                if (!fine) break;
+                tc_fence_after();
+#pragma unroll
+                for (int ks = 0; ks < D / 16; ks++)
+                    mma_ss(tmem, desc_k_major(q_tile, TQ_ROWS, ks), desc_k_major(k_tile, TQ_KEYS, ks), s_desc, ks != 0);
+#pragma unroll
+                for (int ks = 0; ks < D / 16; ks++)
+                    mma_ss(tmem_dp, desc_k_major(do_tile, TQ_ROWS, ks), desc_k_major(v_tile, TQ_KEYS, ks), s_desc, ks != 0);
+                umma_commit(smem_u32(&ctrl->v_empty));
+                umma_commit(smem_u32(&ctrl->s_full));
+                fine = ws.wait(smem_u32(&ctrl->ds_full), j, 6);
+                if (!fine) break;
+                tc_fence_after();
+                const int steps = min(TQ_KEYS, n_keys - j * TQ_KEYS) / 16;      // rows of K behind were never written
+#pragma unroll
+                for (int ks = 0; ks < TQ_KEYS / 16; ks++)
+                    if (ks < steps) mma_ts(tmem_dq, tmem + ks * 8, desc_mn_major(k_tile, TQ_KEYS, ks), q_desc, j || ks);
+                umma_commit(smem_u32(&ctrl->k_empty[j & 1]));
+                umma_commit(smem_u32(&ctrl->dq_done));
+            }
+        }
+        __syncwarp();
+    } else {
+        for (int i = 0; i < D / 8; i++) {
+            const int x = i * 128 + tid, qr = x / (D / 8), c = x % (D / 8);
+            const bool ok = qr < rows;
+            const int qy = tile * TQ_ROWS + (ok ? qr : 0);
+            const int64_t row = sq.row0 + query0 + qy / G, head = h * G + qy % G;
+            cp_async16(q_tile + panel_off(TQ_ROWS, qr, c), static_cast<const T *>(a.d_q) + row * a.q_token + head * a.q_head + c * 8, ok);
+            cp_async16(do_tile + panel_off(TQ_ROWS, qr, c), d_do + row * do_token + head * do_head + c * 8, ok);
+        }
+        cp_commit();
+        const int r = tid, y = tile * TQ_ROWS + min(r, rows - 1);
+        const int limit = attn_limit(a, sq, query0 + y / G);
+        const int64_t at = (int64_t)(sq.row0 + query0 + y / G) * a.heads + h * G + y % G;
+        const float z = a.d_lse[at];
+        const float minus_lse = z == -CUDART_INF_F ? -CUDART_INF_F : -z * LOG2E;       // a row without keys: every p zero
+        const float minus_delta = -delta[at] * a.scale;
+        cp_wait<0>();
+        fence_async_smem();
+        mbar_arrive(smem_u32(&ctrl->q_full));
+        const uint32_t lane_s = tmem + ((uint32_t)(warp * 32) << 16), lane_dp = lane_s + TQ_KEYS, lane_dq = lane_s + 2 * TQ_KEYS;
+        const float scale2 = a.scale * LOG2E;
+        const float2 sc2 = make_float2(scale2, scale2), ml2 = make_float2(minus_lse, minus_lse);
+        const float2 sc = make_float2(a.scale, a.scale), md = make_float2(minus_delta, minus_delta);
+        bool fine = true;
+        for (int j = 0; j < n_tiles; j++) {
+            fine = __all_sync(~0u, ws.wait(smem_u32(&ctrl->s_full), j, 7));
+            if (!fine) break;
+            tc_fence_after();
+            int group_pos = INT32_MAX / 2;
+            if (lane < TQ_KEYS / 16) {
+                const int key = j * TQ_KEYS + lane * 16, e = key >> log_block;
+                if (e < n_entries) group_pos = blk[e] * a.block + (key & (a.block - 1));
+            }
+            const bool masked = __any_sync(~0u, lane < TQ_KEYS / 16 && group_pos > limit_min - 16);
+#pragma unroll
+            for (int c = 0; c < TQ_KEYS / 32; c++) {
+                uint32_t v[32], d[32], w[16];
+                tmem_ld32(lane_s + c * 32, v);
+                tmem_ld32(lane_dp + c * 32, d);
+                tmem_wait_ld();
+                tmem_landed<32>(v);
+                tmem_landed<32>(d);
+#pragma unroll
+                for (int i = 0; i < 16; i++) {
+                    const float2 x = fma2(make_float2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), sc2, ml2);
+                    const float2 g = fma2(make_float2(__uint_as_float(d[2 * i]), __uint_as_float(d[2 * i + 1])), sc, md);
+                    v[2 * i] = __float_as_uint(fast_exp2(x.x) * g.x);
+                    v[2 * i + 1] = __float_as_uint(fast_exp2(x.y) * g.y);
+                }
+                if (masked) {
+                    const int n0 = limit - __shfl_sync(~0u, group_pos, 2 * c), n1 = limit - __shfl_sync(~0u, group_pos, 2 * c + 1);
+#pragma unroll
+                    for (int i = 0; i < 32; i++)
+                        if ((i & 15) >= (i < 16 ? n0 : n1)) v[i] = 0u;
+                }
+#pragma unroll
+                for (int i = 0; i < 16; i++) w[i] = Pack<T>::two(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]));
+                tmem_st16(lane_s + c * 16, w);                  // over columns whose scores have been read
+            }
+            tmem_wait_st();
+            tc_fence_before();
+            mbar_arrive(smem_u32(&ctrl->ds_full));
+        }
+        if (n_tiles && fine) fine = __all_sync(~0u, ws.wait(smem_u32(&ctrl->dq_done), n_tiles - 1, 8));
+        tc_fence_after();
+        T *dst = dq + at * D;
+#pragma unroll 1
+        for (int c = 0; c < D / 32; c++) {
+            uint32_t v[32];
+            if (n_tiles) {
+                tmem_ld32(lane_dq + c * 32, v);
+                tmem_wait_ld();
+                tmem_landed<32>(v);
+            }
+#pragma unroll
+            for (int i = 0; i < 32; i++) v[i] = !fine ? 0x7fc00000u : n_tiles ? v[i] : 0u;
+            if (r < rows)
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    uint32_t x[4];
+#pragma unroll
+                    for (int k = 0; k < 4; k++)
+                        x[k] = Pack<T>::two(__uint_as_float(v[8 * i + 2 * k]), __uint_as_float(v[8 * i + 2 * k + 1]));
+                    reinterpret_cast<uint4 *>(dst + c * 32)[i] = *reinterpret_cast<uint4 *>(x);
+                }
+        }
+        if (!fine && a.d_status) *a.d_status = SPAMM_ERR_DEVICE_WAIT;
+        tc_fence_before();
+    }
+    __syncthreads();
+    if (warp == 4) {
+        if (ctrl->abort_flag) drain_products();
+        __syncwarp();
+        tc_fence_after();
+        tmem_free<TQ_COLS>(tmem);
+    }
+}
+
+// dk and dv of 64 keys of a block from one chunk of the query blocks that list it, 128 gathered rows at a time.
+//
+//   S = Q K^T, dP = dO V^T   [128 rows x 64 keys]        from shared memory, two buffers each in tensor memory
+//   dV^T += dO^T P,  dK^T += Q^T ds   [D x 64 keys]      the tiles of dO and Q once more, as operands whose rows are K
+//
+// P and ds pass through shared memory.  One block of threads per SM: while eight warps work on the exponentials of one
+// tile, the products of the tile before and of the one behind it run, and four warps gather the rows of the one after.
+// With D = 64 the tiles of dO and Q together are the 128 rows of the second products' A: dV^T comes out in the upper half
+// of one accumulator, dK^T in the lower half of the other (the other halves are not used).
+constexpr int TK_ROWS = 128, TK_KEYS = 64, TK_SOFTMAX = 256, TK_THREADS = TK_SOFTMAX + 32 + 128, TK_COLS = 512;
+
+struct TkCtrl {
+    uint64_t kv_full, r_full[2], r_empty[2], s_full[2], p_full, dv_done, ds_full, dk_done;
+    uint32_t tmem_base;
+    uint32_t abort_flag;
+    int32_t err;
+    int32_t pad;
+};
+
+template <typename T, int D>
+__global__ __launch_bounds__(TK_THREADS, 1) void attn_dkv_tc_kernel(const __grid_constant__ spamm_attn a, const BackwardPlan p,
+                                                                    const T *d_do, int64_t do_token, int64_t do_head,
+                                                                    const float *delta, const unsigned *bits, const Item *items,
+                                                                    const int *n_items, float *partial, T *dk, T *dv)
+{
+    extern __shared__ __align__(1024) uint8_t smem_tc[];
+    uint8_t *const smem = smem_tc;
+    constexpr int KT = TK_KEYS * D * 2, RT = TK_ROWS * D * 2, PT = TK_ROWS * TK_KEYS * 2;
+    const uint32_t k_tile = smem_u32(smem), v_tile = k_tile + KT, ring = v_tile + KT;      // ring: [stage][do | q]
+    const uint32_t p_tile = ring + 4 * RT, ds_tile = p_tile + PT;
+    TkCtrl *ctrl = reinterpret_cast<TkCtrl *>(smem + 2 * KT + 4 * RT + 2 * PT);
+    int *list = reinterpret_cast<int *>(ctrl + 1);
+    __shared__ int warp_sum[TK_THREADS / 32];
+
+    const int halves = a.block / TK_KEYS;
+    const int half = blockIdx.x % halves;
+    const unsigned rest = blockIdx.x / halves;
+    const int64_t group = rest / p.item_cap;
+    const int item_i = rest % p.item_cap;
+    if (item_i >= n_items[group]) return;
+    const Item item = items[group * p.item_cap + item_i];
+    const int s = (int)(group / a.kv_heads), h = (int)(group % a.kv_heads);
+    const Seq sq = attn_seq(a, s);
+    const int G = a.heads / a.kv_heads;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int pos0 = item.kb * a.block + half * TK_KEYS;
+    const int keys = min(TK_KEYS, sq.nk - pos0);
+    if (keys <= 0) return;
+
+    if (warp == 8) {
+        if (lane == 0) {
+            mbar_init(smem_u32(&ctrl->kv_full), 128);
+            for (int i = 0; i < 2; i++) {
+                mbar_init(smem_u32(&ctrl->r_full[i]), 128);
+                mbar_init(smem_u32(&ctrl->r_empty[i]), 1);
+                mbar_init(smem_u32(&ctrl->s_full[i]), 1);
+            }
+            mbar_init(smem_u32(&ctrl->p_full), TK_SOFTMAX);
+            mbar_init(smem_u32(&ctrl->ds_full), TK_SOFTMAX);
+            mbar_init(smem_u32(&ctrl->dv_done), 1);
+            mbar_init(smem_u32(&ctrl->dk_done), 1);
+            ctrl->abort_flag = 0;
+            ctrl->err = 0;
+            asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        }
+        __syncwarp();
+        tmem_alloc<TK_COLS>(smem_u32(&ctrl->tmem_base));
+        tc_fence_before();
+    }
+    const int n_list = expand_bits<TK_THREADS>(bits + (group * p.nkb + item.kb) * p.words, p.words, item.chunk * p.chunk, p.chunk,
+                                               list, warp_sum);
+    tc_fence_after();
+    const int bq = min(a.query_block, a.max_q), per = bq * G;
+    // all listed query blocks are full but the sequence's last one, which can only be the last of the list
+    const int64_t n_rows = n_list ? (int64_t)(n_list - 1) * per + (int64_t)min(bq, sq.nq - list[n_list - 1] * bq) * G : 0;
+    const int n_tiles = (int)((n_rows + TK_ROWS - 1) / TK_ROWS);
+    const uint32_t tmem = ctrl->tmem_base, tmem_dv = tmem + 4 * TK_KEYS, tmem_dk = tmem_dv + TK_KEYS;
+    const WaitState ws{&ctrl->abort_flag, &ctrl->err};
+    // row x of the gathered rows: its row of q and its head; false when there is none
+    auto locate = [&](int64_t x, int *query, int *head) {
+        if (x >= n_rows) return false;
+        const int e = (int)(x / per), y = (int)(x - (int64_t)e * per);
+        *query = list[e] * bq + y / G;
+        *head = h * G + y % G;
+        return true;
+    };
+
+    if (warp > 8) {
+        // ---- rows of Q and dO; K and V first
+        const int t = tid - TK_SOFTMAX - 32, lw = t >> 5;
+        for (int x = t; x < TK_KEYS * (D / 8); x += 128) {
+            const int r = x / (D / 8), c = x % (D / 8);
+            const bool ok = r < keys;
+            const int64_t row = sq.row0 + pos0 + (ok ? r : 0);
+            cp_async16(k_tile + panel_off(TK_KEYS, r, c), static_cast<const T *>(a.d_k) + row * a.k_token + h * a.k_head + c * 8, ok);
+            cp_async16(v_tile + panel_off(TK_KEYS, r, c), static_cast<const T *>(a.d_v) + row * a.v_token + h * a.v_head + c * 8, ok);
+        }
+        cp_commit();
+        constexpr int PASS = 32 / (D / 8);                      // rows of a warp's copy
+        const int col = lane % (D / 8), sub = lane / (D / 8);
+        bool fine = true;
+        auto signal = [&](uint64_t *bar) {
+            fence_async_smem();
+            mbar_arrive(smem_u32(bar));
+        };
+        for (int j = 0; j <= n_tiles; j++) {
+            if (j > 1) {
+                // the buffer comes free only when the tile before has been worked on: announce that one first
+                cp_wait<0>();
+                signal(&ctrl->r_full[(j - 1) & 1]);
+            }
+            if (j < n_tiles) {
+                if (j > 1) fine = __all_sync(~0u, ws.wait(smem_u32(&ctrl->r_empty[j & 1]), (j >> 1) - 1, 1));
+                if (!fine) break;
+                // each lane finds one of the warp's 32 rows, the copies take the addresses from it
+                int query = 0, head = 0;
+                const bool there = locate((int64_t)j * TK_ROWS + lw * 32 + lane, &query, &head);
+                const int64_t q_at = there ? (int64_t)(sq.row0 + query) * a.q_token + head * a.q_head : -1;
+                const int64_t do_at = (int64_t)(sq.row0 + query) * do_token + head * do_head;
+                const uint32_t do_dst = ring + (j & 1) * 2 * RT, q_dst = do_dst + RT;
+#pragma unroll 4
+                for (int i = 0; i < 32; i += PASS) {
+                    const int r = i + sub;
+                    const int64_t qa = __shfl_sync(~0u, q_at, r), da = __shfl_sync(~0u, do_at, r);
+                    const uint32_t off = panel_off(TK_ROWS, lw * 32 + r, col);
+                    cp_async16(q_dst + off, static_cast<const T *>(a.d_q) + (qa < 0 ? 0 : qa) + col * 8, qa >= 0);
+                    cp_async16(do_dst + off, d_do + (qa < 0 ? 0 : da) + col * 8, qa >= 0);
+                }
+            }
+            cp_commit();
+            if (j <= 1) {
+                cp_wait<1>();                                   // the group before: K and V, or the rows of the first tile
+                signal(j ? &ctrl->r_full[0] : &ctrl->kv_full);
+            }
+        }
+        cp_wait<0>();
+    } else if (warp == 8) {
+        // ---- products
+        if (lane == 0 && n_tiles) {
+            constexpr uint32_t s_desc = mma_desc<T>(128, TK_KEYS, false, false), o_desc = mma_desc<T>(128, TK_KEYS, true, true);
+            bool fine = ws.wait(smem_u32(&ctrl->kv_full), 0, 2);
+            for (int j = 0; j <= n_tiles && fine; j++) {
+                if (j < n_tiles) {
+                    fine = ws.wait(smem_u32(&ctrl->r_full[j & 1]), j >> 1, 3);
+                    if (!fine) break;
+                    tc_fence_after();
+                    const uint32_t do_tile = ring + (j & 1) * 2 * RT, q_tile = do_tile + RT, s_at = tmem + (j & 1) * 2 * TK_KEYS;
+#pragma unroll
+                    for (int ks = 0; ks < D / 16; ks++)
+                        mma_ss(s_at, desc_k_major(q_tile, TK_ROWS, ks), desc_k_major(k_tile, TK_KEYS, ks), s_desc, ks != 0);
+#pragma unroll
+                    for (int ks = 0; ks < D / 16; ks++)
+                        mma_ss(s_at + TK_KEYS, desc_k_major(do_tile, TK_ROWS, ks), desc_k_major(v_tile, TK_KEYS, ks), s_desc, ks != 0);
+                    umma_commit(smem_u32(&ctrl->s_full[j & 1]));
+                }
+                if (j) {
+                    // A: 128 values of dO (of Q) x 128 rows; with D = 64 the tiles of dO and Q one behind the other
+                    const uint32_t do_tile = ring + ((j - 1) & 1) * 2 * RT, q_tile = D == 64 ? do_tile : do_tile + RT;
+                    fine = ws.wait(smem_u32(&ctrl->p_full), j - 1, 4);
+                    if (!fine) break;
+                    tc_fence_after();
+#pragma unroll
+                    for (int ks = 0; ks < TK_ROWS / 16; ks++)
+                        mma_ss(tmem_dv, desc_mn_major(do_tile, TK_ROWS, ks), desc_mn_major(p_tile, TK_ROWS, ks), o_desc, j > 1 || ks);
+                    umma_commit(smem_u32(&ctrl->dv_done));
+                    fine = ws.wait(smem_u32(&ctrl->ds_full), j - 1, 5);
+                    if (!fine) break;
+                    tc_fence_after();
+#pragma unroll
+                    for (int ks = 0; ks < TK_ROWS / 16; ks++)
+                        mma_ss(tmem_dk, desc_mn_major(q_tile, TK_ROWS, ks), desc_mn_major(ds_tile, TK_ROWS, ks), o_desc, j > 1 || ks);
+                    umma_commit(smem_u32(&ctrl->r_empty[(j - 1) & 1]));
+                    umma_commit(smem_u32(&ctrl->dk_done));
+                }
+            }
+        }
+        __syncwarp();
+    } else {
+        // ---- p and ds: thread = row, the upper four warps the keys 32..63
+        const int r = tid & 127, part = warp >> 2;
+        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+        const float scale2 = a.scale * LOG2E;
+        const float2 sc2 = make_float2(scale2, scale2), sc = make_float2(a.scale, a.scale);
+        auto row_of = [&](int j, float *minus_lse, float *minus_delta, int *n_visible) {
+            int query, head;
+            *minus_lse = -CUDART_INF_F;                         // a row that is none, or has no keys: every p zero
+            *minus_delta = 0.f;
+            *n_visible = 0;
+            if (j < n_tiles && locate((int64_t)j * TK_ROWS + r, &query, &head)) {
+                const int64_t at = (int64_t)(sq.row0 + query) * a.heads + head;
+                const float z = a.d_lse[at];
+                if (z != -CUDART_INF_F) *minus_lse = -z * LOG2E;
+                *minus_delta = -delta[at] * a.scale;
+                *n_visible = min(a.causal ? query + 1 - pos0 : TK_KEYS, keys) - part * 32;
+            }
+        };
+        float minus_lse, minus_delta;
+        int n_visible;
+        row_of(0, &minus_lse, &minus_delta, &n_visible);
+        bool fine = true;
+        for (int j = 0; j < n_tiles; j++) {
+            float next_lse, next_delta;
+            int next_visible;
+            row_of(j + 1, &next_lse, &next_delta, &next_visible);
+            fine = __all_sync(~0u, ws.wait(smem_u32(&ctrl->s_full[j & 1]), j >> 1, 6));
+            if (!fine) break;
+            tc_fence_after();
+            const uint32_t s_at = tmem + (j & 1) * 2 * TK_KEYS + lanes + part * 32;
+            uint32_t v[32], d[32], w[16];
+            tmem_ld32(s_at, v);
+            tmem_ld32(s_at + TK_KEYS, d);
+            tmem_wait_ld();
+            tmem_landed<32>(v);
+            tmem_landed<32>(d);
+            const float2 ml2 = make_float2(minus_lse, minus_lse), md = make_float2(minus_delta, minus_delta);
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+                const float2 x = fma2(make_float2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), sc2, ml2);
+                const float2 g = fma2(make_float2(__uint_as_float(d[2 * i]), __uint_as_float(d[2 * i + 1])), sc, md);
+                const float e0 = fast_exp2(x.x), e1 = fast_exp2(x.y);
+                v[2 * i] = __float_as_uint(e0);
+                v[2 * i + 1] = __float_as_uint(e1);
+                d[2 * i] = __float_as_uint(e0 * g.x);
+                d[2 * i + 1] = __float_as_uint(e1 * g.y);
+            }
+            if (__any_sync(~0u, n_visible < 32)) {
+#pragma unroll
+                for (int i = 0; i < 32; i++)
+                    if (i >= n_visible) { v[i] = 0u; d[i] = 0u; }
+            }
+#pragma unroll
+            for (int i = 0; i < 16; i++) w[i] = Pack<T>::two(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]));
+            if (j) fine = __all_sync(~0u, ws.wait(smem_u32(&ctrl->dv_done), j - 1, 7));
+            if (!fine) break;
+#pragma unroll
+            for (int c = 0; c < 4; c++)
+                *reinterpret_cast<uint4 *>(smem + (p_tile - k_tile) + panel_off(TK_ROWS, r, part * 4 + c)) =
+                    make_uint4(w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]);
+            fence_async_smem();
+            tc_fence_before();
+            mbar_arrive(smem_u32(&ctrl->p_full));
+#pragma unroll
+            for (int i = 0; i < 16; i++) w[i] = Pack<T>::two(__uint_as_float(d[2 * i]), __uint_as_float(d[2 * i + 1]));
+            if (j) fine = __all_sync(~0u, ws.wait(smem_u32(&ctrl->dk_done), j - 1, 8));
+            if (!fine) break;
+#pragma unroll
+            for (int c = 0; c < 4; c++)
+                *reinterpret_cast<uint4 *>(smem + (ds_tile - k_tile) + panel_off(TK_ROWS, r, part * 4 + c)) =
+                    make_uint4(w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]);
+            fence_async_smem();
+            tc_fence_before();
+            mbar_arrive(smem_u32(&ctrl->ds_full));
+            minus_lse = next_lse;
+            minus_delta = next_delta;
+            n_visible = next_visible;
+        }
+        if (n_tiles && fine) fine = __all_sync(~0u, ws.wait(smem_u32(&ctrl->dk_done), n_tiles - 1, 9));
+        tc_fence_after();
+        // rows of the accumulators are the D values, columns the keys: four warps write dv, four dk
+        const bool is_k = part != 0;
+        const int row = r, d0 = D == 64 && is_k ? row - 64 : row;
+        const bool mine = D == 128 || (is_k ? row >= 64 : row < 64);            // whole warps
+#pragma unroll 1
+        for (int c = 0; c < TK_KEYS / 32; c++) {
+            uint32_t v[32];
+            if (n_tiles) {
+                tmem_ld32((is_k ? tmem_dk : tmem_dv) + lanes + c * 32, v);
+                tmem_wait_ld();
+                tmem_landed<32>(v);
+            }
+#pragma unroll
+            for (int i = 0; i < 32; i++) v[i] = !fine ? 0x7fc00000u : n_tiles ? v[i] : 0u;
+            if (!mine) continue;
+            if (item.slot >= 0) {
+                float *dst = partial + (group * p.slot_cap + item.slot) * (int64_t)(2 * a.block * D) + (is_k ? 0 : a.block * D) +
+                             (half * TK_KEYS + c * 32) * D + d0;
+#pragma unroll
+                for (int i = 0; i < 32; i++) dst[i * D] = __uint_as_float(v[i]);
+            } else {
+                T *dst = (is_k ? dk : dv) + ((int64_t)(sq.row0 + pos0 + c * 32) * a.kv_heads + h) * D + d0;
+#pragma unroll
+                for (int i = 0; i < 32; i++)
+                    if (c * 32 + i < keys) dst[(int64_t)i * a.kv_heads * D] = Pack<T>::one(__uint_as_float(v[i]));
+            }
+        }
+        if (!fine && a.d_status) *a.d_status = SPAMM_ERR_DEVICE_WAIT;
+        tc_fence_before();
+    }
+    __syncthreads();
+    if (warp == 8) {
+        if (ctrl->abort_flag) drain_products();
+        __syncwarp();
+        tc_fence_after();
+        tmem_free<TK_COLS>(tmem);
+    }
+}
+
 // Adds up the partial sums of the blocks of keys that were cut into several items.
 template <typename T>
 __global__ __launch_bounds__(128) void attn_dkv_join_kernel(const __grid_constant__ spamm_attn a, const BackwardPlan p,
@@ -585,7 +1144,7 @@ static int backward_launch(const spamm_attn &a, const BackwardPlan &p, const T *
     const int bq = min(a.query_block, a.max_q);
     const int tiles = (int)(((int64_t)bq * (a.heads / a.kv_heads) + 15) / 16);
     const int64_t dq_grid = p.groups * p.nqb * tiles;
-    if ((rows + 31) / 32 > INT32_MAX || (lists + 3) / 4 > INT32_MAX || dq_grid > INT32_MAX || p.groups * p.item_cap > INT32_MAX ||
+    if ((rows + 31) / 32 > INT32_MAX || (lists + 3) / 4 > INT32_MAX || dq_grid > INT32_MAX || p.groups * p.item_cap > INT32_MAX / 2 ||
         p.groups * p.nkb > INT32_MAX)
         return attn_too_large();
 
@@ -594,16 +1153,33 @@ static int backward_launch(const spamm_attn &a, const BackwardPlan &p, const T *
     attn_turn_kernel<<<(unsigned)((lists + 3) / 4), 128, 0, stream>>>(a, p.nqb, p.nkb, p.words, bits, counts);
     attn_items_kernel<<<(unsigned)p.groups, 1024, 0, stream>>>(a, p, counts, slots, items, n_items);
 
+    // from 48 rows that share a list on, tiles of 128 rows; below, tiles of 16
+    int st;
+    if ((int64_t)bq * (a.heads / a.kv_heads) >= 48) {
+        const int tq = (int)(((int64_t)bq * (a.heads / a.kv_heads) + TQ_ROWS - 1) / TQ_ROWS);
+        RowMap k_map, v_map;
+        attn_row_maps(a, min(a.block, TQ_KEYS), &k_map, &v_map);
+        const size_t smem = 2 * TQ_ROWS * D * 2 + 3 * TQ_KEYS * D * 2 + sizeof(TqCtrl) + a.n_select * 4;
+        st = attn_set_smem((const void *)attn_dq_tc_kernel<T, D>, smem);
+        if (st) return st;
+        attn_dq_tc_kernel<T, D><<<(unsigned)(p.groups * p.nqb * tq), TQ_THREADS, smem, stream>>>(
+            a, p.nqb, tq, k_map, v_map, d_do, do_token, do_head, delta, dq);
+    } else {
     const size_t dq_smem = (size_t)DQ_WARPS * DQ_STAGES * 2 * 16 * D * 2 + 2 * 16 * D * 2 + a.n_select * 4;
-    int st = attn_set_smem((const void *)attn_dq_rows_kernel<T, D>, dq_smem);
+    st = attn_set_smem((const void *)attn_dq_rows_kernel<T, D>, dq_smem);
     if (st) return st;
     attn_dq_rows_kernel<T, D><<<(unsigned)dq_grid, 128, dq_smem, stream>>>(a, p.nqb, tiles, d_do, do_token, do_head, delta, dq);
+    }
 
-    switch (a.block) {
+    if (a.block >= TK_KEYS) {
+        const size_t smem = 2 * TK_KEYS * D * 2 + 4 * TK_ROWS * D * 2 + 2 * TK_ROWS * TK_KEYS * 2 + sizeof(TkCtrl) + p.chunk * 4;
+        st = attn_set_smem((const void *)attn_dkv_tc_kernel<T, D>, smem);
+        if (st) return st;
+        attn_dkv_tc_kernel<T, D><<<(unsigned)(p.groups * p.item_cap * (a.block / TK_KEYS)), TK_THREADS, smem, stream>>>(
+            a, p, d_do, do_token, do_head, delta, bits, items, n_items, partial, dk, dv);
+    } else switch (a.block) {
     case 16: st = dkv_launch<T, D, 16>(a, p, d_do, do_token, do_head, delta, bits, items, n_items, partial, dk, dv, stream); break;
-    case 32: st = dkv_launch<T, D, 32>(a, p, d_do, do_token, do_head, delta, bits, items, n_items, partial, dk, dv, stream); break;
-    case 64: st = dkv_launch<T, D, 64>(a, p, d_do, do_token, do_head, delta, bits, items, n_items, partial, dk, dv, stream); break;
-    default: st = dkv_launch<T, D, 128>(a, p, d_do, do_token, do_head, delta, bits, items, n_items, partial, dk, dv, stream); break;
+    default: st = dkv_launch<T, D, 32>(a, p, d_do, do_token, do_head, delta, bits, items, n_items, partial, dk, dv, stream); break;
     }
     if (st) return st;
     if (p.nqb > p.chunk)
@@ -643,6 +1219,7 @@ extern "C" int spamm_attn_backward_dev(const spamm_attn *a, const void *d_do, in
         SPAMM_CUDA_TRY(cudaMemsetAsync(d_dv, 0, row * a->kv_heads, (cudaStream_t)stream));
         return SPAMM_OK;
     }
+    if (reinterpret_cast<uintptr_t>(a->d_o_low) & 15) return attn_refuse("d_o_low is not on a 16-byte boundary");
     const BackwardPlan p = backward_plan(*a);
     if (!d_scratch || scratch_bytes < p.bytes || (reinterpret_cast<uintptr_t>(d_scratch) & 15))
         return attn_refuse("scratch too small or not on a 16-byte boundary");

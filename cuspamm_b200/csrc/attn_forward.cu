@@ -80,6 +80,23 @@ static __device__ void zero_tail(const spamm_attn &a, const Seq &sq, int s, int 
     }
 }
 
+// Eight values to o, and what their rounding left to `low` (when given).
+template <typename T> static __device__ __forceinline__ void store8(T *dst, T *low, const float *y)
+{
+    uint32_t x[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) x[i] = Pack<T>::two(y[2 * i], y[2 * i + 1]);
+    *reinterpret_cast<uint4 *>(dst) = *reinterpret_cast<uint4 *>(x);
+    if (low) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const float2 back = Pack<T>::to2(x[i]);
+            x[i] = Pack<T>::two(y[2 * i] - back.x, y[2 * i + 1] - back.y);
+        }
+        *reinterpret_cast<uint4 *>(low) = *reinterpret_cast<uint4 *>(x);
+    }
+}
+
 // How a call is cut: tiles of rows over the (queries x heads of a key head) of a query block, and ranges of keys.
 struct RowsPlan {
     int bq, nqb;            // queries per query block (all of them without lists), query blocks
@@ -314,12 +331,12 @@ __global__ __launch_bounds__(128) void attn_rows_kernel(const __grid_constant__ 
         const int64_t row = sq.row0 + qb * p.bq + x / G;
         const int head = h * G + x % G;
         if (p.n_split == 1) {
-            uint32_t out[D / 16];
 #pragma unroll
-            for (int i = 0; i < D / 16; i++) out[i] = Pack<T>::two(y[2 * i] * inv, y[2 * i + 1] * inv);
+            for (int i = 0; i < D / 8; i++) y[i] *= inv;
             T *dst = static_cast<T *>(a.d_o) + row * a.o_token + head * a.o_head + c0;
+            T *low = a.d_o_low ? static_cast<T *>(a.d_o_low) + (row * a.heads + head) * D + c0 : nullptr;
 #pragma unroll
-            for (int i = 0; i < D / 64; i++) reinterpret_cast<uint4 *>(dst)[i] = *reinterpret_cast<uint4 *>(out + 4 * i);
+            for (int i = 0; i < D / 64; i++) store8<T>(dst + 8 * i, low ? low + 8 * i : nullptr, y + 8 * i);
             if (a.d_lse && (tid & 7) == 0) a.d_lse[row * a.heads + head] = lse2 * LN2;
         } else {
             const int64_t at = (row * a.heads + head) * p.n_split + split;
@@ -636,15 +653,9 @@ __global__ __launch_bounds__(TC_THREADS, 2) void attn_tc_kernel(const __grid_con
             if (r < rows) {
                 if (p.n_split == 1) {
                     T *dst = static_cast<T *>(a.d_o) + row * a.o_token + head * a.o_head + c * 32;
+                    T *low = a.d_o_low ? static_cast<T *>(a.d_o_low) + (row * a.heads + head) * D + c * 32 : nullptr;
 #pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        uint4 x;
-                        uint32_t *xs = reinterpret_cast<uint32_t *>(&x);
-#pragma unroll
-                        for (int k = 0; k < 4; k++)
-                            xs[k] = Pack<T>::two(__uint_as_float(v[8 * i + 2 * k]), __uint_as_float(v[8 * i + 2 * k + 1]));
-                        reinterpret_cast<uint4 *>(dst)[i] = x;
-                    }
+                    for (int i = 0; i < 4; i++) store8<T>(dst + 8 * i, low ? low + 8 * i : nullptr, reinterpret_cast<float *>(v) + 8 * i);
                 } else {
                     float4 *dst = reinterpret_cast<float4 *>(part_o + at * D + c * 32);
 #pragma unroll
@@ -663,12 +674,7 @@ __global__ __launch_bounds__(TC_THREADS, 2) void attn_tc_kernel(const __grid_con
     }
     __syncthreads();
     if (warp == 4) {
-        // after an aborted wait products may still be in flight: they end before the tensor memory is given back
-        if (ctrl->abort_flag) {
-            if (lane == 0) umma_commit(smem_u32(&ctrl->q_full));
-            const unsigned long long t0 = global_ns();
-            while (global_ns() - t0 < 1000000ull) {}
-        }
+        if (ctrl->abort_flag) drain_products();
         __syncwarp();
         tc_fence_after();
         tmem_free<TC_COLS>(tmem);
@@ -706,8 +712,16 @@ __global__ __launch_bounds__(128) void attn_join_kernel(const __grid_constant__ 
     }
     const float inv = total == 0.f ? 0.f : 1.f / total;
     T *dst = static_cast<T *>(a.d_o) + row * a.o_token + head * a.o_head + lane * (D / 32);
+    T *low = a.d_o_low ? static_cast<T *>(a.d_o_low) + (row * a.heads + head) * D + lane * (D / 32) : nullptr;
 #pragma unroll
-    for (int d = 0; d < D / 32; d += 2) *reinterpret_cast<uint32_t *>(dst + d) = Pack<T>::two(y[d] * inv, y[d + 1] * inv);
+    for (int d = 0; d < D / 32; d += 2) {
+        const uint32_t x = Pack<T>::two(y[d] * inv, y[d + 1] * inv);
+        *reinterpret_cast<uint32_t *>(dst + d) = x;
+        if (low) {
+            const float2 back = Pack<T>::to2(x);
+            *reinterpret_cast<uint32_t *>(low + d) = Pack<T>::two(y[d] * inv - back.x, y[d + 1] * inv - back.y);
+        }
+    }
     if (a.d_lse && lane == 0) a.d_lse[row * a.heads + head] = total == 0.f ? -CUDART_INF_F : (t0 + log2f(total)) * LN2;
 }
 
@@ -725,7 +739,7 @@ static PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder()
     return fn;
 }
 
-static void row_map(const spamm_attn &a, const void *p, int64_t token, int64_t head, RowMap *out)
+static void row_map(const spamm_attn &a, int box_rows, const void *p, int64_t token, int64_t head, RowMap *out)
 {
     memset(out, 0, sizeof(*out));
     const auto encode = tensor_map_encoder();
@@ -736,7 +750,7 @@ static void row_map(const spamm_attn &a, const void *p, int64_t token, int64_t h
         if ((int64_t)a.n_pages * a.kv_heads > INT32_MAX) return;
         dims[1] = a.block; dims[2] = (cuuint64_t)a.n_pages * a.kv_heads;
         strides[0] = (cuuint64_t)a.dim * 2; strides[1] = (cuuint64_t)a.block * a.dim * 2;
-        box[1] = a.block;
+        box[1] = box_rows;
     } else {
         // the larger stride last, a multiple of the smaller
         if (a.kv_heads == 1) head = a.dim;
@@ -746,17 +760,17 @@ static void row_map(const spamm_attn &a, const void *p, int64_t token, int64_t h
         if ((out->swapped ? head % token : token % head) != 0) return;
         dims[t] = a.tokens; dims[h] = a.kv_heads;
         strides[t - 1] = (cuuint64_t)token * 2; strides[h - 1] = (cuuint64_t)head * 2;
-        box[t] = a.block;
+        box[t] = box_rows;
     }
     const CUtensorMapDataType type = a.dtype == SPAMM_ATTN_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
     out->usable = encode(&out->map, type, 3, const_cast<void *>(p), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
                          CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-void attn_row_maps(const spamm_attn &a, RowMap *k, RowMap *v)
+void attn_row_maps(const spamm_attn &a, int box_rows, RowMap *k, RowMap *v)
 {
-    row_map(a, a.d_k, a.k_token, a.k_head, k);
-    row_map(a, a.d_v, a.v_token, a.v_head, v);
+    row_map(a, box_rows, a.d_k, a.k_token, a.k_head, k);
+    row_map(a, box_rows, a.d_v, a.v_token, a.v_head, v);
 }
 
 static int64_t longest_list(const spamm_attn &a)
@@ -814,7 +828,7 @@ static int forward_launch(const spamm_attn &a, float *scratch, cudaStream_t stre
         int st = attn_set_smem((const void *)attn_tc_kernel<T, D>, smem);
         if (st) return st;
         RowMap k_map, v_map;
-        attn_row_maps(a, &k_map, &v_map);
+        attn_row_maps(a, a.block, &k_map, &v_map);
         attn_tc_kernel<T, D><<<(unsigned)grid, TC_THREADS, smem, stream>>>(a, p, k_map, v_map, part_o, part_lse);
     } else {
         const size_t smem = rows_smem(a, p);
@@ -847,6 +861,7 @@ extern "C" int spamm_attn_forward_dev(const spamm_attn *a, void *d_scratch, size
     if (!a->tokens || !a->batch || !a->max_q) return SPAMM_OK;
     const bool k_ok = a->n_pages ? attn_rows_ok(a->d_k, 0, 0) && attn_rows_ok(a->d_v, 0, 0)
                                  : attn_rows_ok(a->d_k, a->k_token, a->k_head) && attn_rows_ok(a->d_v, a->v_token, a->v_head);
+    if (reinterpret_cast<uintptr_t>(a->d_o_low) & 15) return attn_refuse("d_o_low is not on a 16-byte boundary");
     if (!k_ok || !attn_rows_ok(a->d_q, a->q_token, a->q_head) || !attn_rows_ok(a->d_o, a->o_token, a->o_head))
         return attn_refuse("q, k, v and o need rows on 16-byte boundaries");
     const size_t need = spamm_attn_forward_scratch_bytes(a);

@@ -97,15 +97,15 @@ template <int COLS> __device__ __forceinline__ void tmem_free(uint32_t base)
 // What this thread's ordinary stores (cp.async, st.shared) left in shared memory becomes visible to tcgen05.mma.
 __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
-// A tensor map over the rows of k or v: boxes of one block of keys x 64 values.  Coordinates (value, y, z) of the block that
+// A tensor map over the rows of k or v: boxes of box_rows keys x 64 values.  Coordinates (value, y, z) of the block that
 // begins at row `row` of key head h: packed (value, h or row, row or h), pages (value, 0, page * kv_heads + h).
 struct RowMap {
     CUtensorMap map;
     int usable;          // 0: the strides do not fit a tensor map, rows are copied 16 bytes at a time
     int swapped;         // packed: the head is the third coordinate
 };
-// Fills both maps (pages: strides are not read).
-void attn_row_maps(const spamm_attn &a, RowMap *k, RowMap *v);
+// Fills both maps (pages: strides are not read); box_rows keys at a time, at most a block.
+void attn_row_maps(const spamm_attn &a, int box_rows, RowMap *k, RowMap *v);
 
 __device__ __forceinline__ void tma_box(uint32_t dst, const CUtensorMap *map, int x, int y, int z, uint32_t bar)
 {
@@ -143,5 +143,12 @@ struct WaitState {
         return wait_bounded(bar, parity & 1u, abort_flag, err, code);
     }
 };
+
+// After an aborted wait products may still be in flight; they end before their tensor memory is given back.
+static __device__ __noinline__ void drain_products()
+{
+    const unsigned long long t0 = global_ns();
+    while (global_ns() - t0 < 1000000ull) {}
+}
 
 }  // namespace spamm

@@ -521,6 +521,9 @@ typedef struct spamm_attn {
     int64_t o_token, o_head;
     float *d_lse;               /* [tokens][heads] log of the sum of exp(scale * q.k) over the keys read, -inf for none;
                                    output of the forward (NULL: not wanted), input of the backward */
+    void *d_o_low;              /* [tokens][heads][dim] without gaps, may be NULL: what the rounding of o left, rounded
+                                   to the type; output of the forward, read by the backward, whose gradients of q and
+                                   k are then as near as if o had been kept in float */
     int32_t *d_status;          /* one word, kept until the caller clears it; may be NULL without pages */
 } spamm_attn;
 
