@@ -20,6 +20,22 @@ int attn_set_smem(const void *kernel, size_t bytes);
 int attn_refuse(const char *why);     // records the text, gives SPAMM_ERR_INVALID
 int attn_too_large();                 // the same for a grid beyond 2^31 - 1, SPAMM_ERR_UNSUPPORTED
 
+// Division of numbers below 2^31 by a fixed one: n / d = (n * m) >> (32 + s) with m = ceil(2^(32+s) / d), s = ceil(log2 d) - 1
+// (m < 2^32 and the excess m*d - 2^(32+s) < d <= 2^(s+1) keeps the quotient exact for n < 2^31).
+struct FastDiv {
+    uint32_t d, m, s;
+    __device__ __forceinline__ uint32_t quotient(uint32_t n) const { return d == 1 ? n : __umulhi(n, m) >> s; }
+};
+inline FastDiv fast_div(uint32_t d)
+{
+    FastDiv f{d, 0, 0};
+    if (d > 1) {
+        while ((2u << f.s) < d) f.s++;
+        f.m = (uint32_t)((((uint64_t)1 << (32 + f.s)) + d - 1) / d);
+    }
+    return f;
+}
+
 struct Seq {
     int row0;     // first row of q (and of packed k, v)
     int nq;       // queries that are computed

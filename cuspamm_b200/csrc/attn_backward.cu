@@ -17,6 +17,8 @@ struct BackwardPlan {
     int chunk;                  // query blocks of a work item
     int item_cap, slot_cap;     // items and partial sums of one (sequence, key head)
     int64_t groups;             // batch * kv_heads
+    FastDiv per, G;             // rows of a full query block, heads of a key head
+    int box_tokens;             // queries of a tensor copy of q and do (0: rows are copied one by one)
     size_t delta, bits, counts, slots, items, n_items, partial, bytes;   // scratch offsets
 };
 
@@ -33,6 +35,12 @@ static BackwardPlan backward_plan(const spamm_attn &a)
     p.words = ceil_div(p.nqb, 32);
     const int64_t rows = (int64_t)min(a.query_block, a.max_q) * G;
     p.chunk = (int)max((int64_t)1, min((int64_t)1024, 8192 / rows));
+    p.per = fast_div((uint32_t)rows);
+    p.G = fast_div((uint32_t)G);
+    // a tensor copy takes the heads of a key head of as many queries as fit a tile or make up a query block, when that
+    // cuts tiles of 128 rows evenly and begins on a group of 8 rows
+    const int64_t fit = G <= 128 && 128 % G == 0 ? min((int64_t)min(a.query_block, a.max_q), (int64_t)128 / G) : 0;
+    p.box_tokens = fit && 128 % (fit * G) == 0 && fit * G % 8 == 0 && min(a.query_block, a.max_q) % fit == 0 ? (int)fit : 0;
     const int64_t pairs = (int64_t)p.nqb * min(a.n_select, p.nkb);
     p.item_cap = (int)min((int64_t)INT32_MAX / 4, p.nkb + pairs / p.chunk);
     p.slot_cap = (int)min((int64_t)INT32_MAX / 4, 2 * pairs / p.chunk);
@@ -810,7 +818,9 @@ struct TkCtrl {
 };
 
 template <typename T, int D>
-__global__ __launch_bounds__(TK_THREADS, 1) void attn_dkv_tc_kernel(const __grid_constant__ spamm_attn a, const BackwardPlan p,
+__global__ __launch_bounds__(TK_THREADS, 1) void attn_dkv_tc_kernel(const __grid_constant__ spamm_attn a, const __grid_constant__ BackwardPlan p,
+                                                                    const __grid_constant__ RowMap q_map,
+                                                                    const __grid_constant__ RowMap do_map,
                                                                     const T *d_do, int64_t do_token, int64_t do_head,
                                                                     const float *delta, const unsigned *bits, const Item *items,
                                                                     const int *n_items, float *partial, T *dk, T *dv)
@@ -864,16 +874,16 @@ __global__ __launch_bounds__(TK_THREADS, 1) void attn_dkv_tc_kernel(const __grid
     tc_fence_after();
     const int bq = min(a.query_block, a.max_q), per = bq * G;
     // all listed query blocks are full but the sequence's last one, which can only be the last of the list
-    const int64_t n_rows = n_list ? (int64_t)(n_list - 1) * per + (int64_t)min(bq, sq.nq - list[n_list - 1] * bq) * G : 0;
-    const int n_tiles = (int)((n_rows + TK_ROWS - 1) / TK_ROWS);
+    const int n_rows = n_list ? (n_list - 1) * per + min(bq, sq.nq - list[n_list - 1] * bq) * G : 0;
+    const int n_tiles = (n_rows + TK_ROWS - 1) / TK_ROWS;
     const uint32_t tmem = ctrl->tmem_base, tmem_dv = tmem + 4 * TK_KEYS, tmem_dk = tmem_dv + TK_KEYS;
     const WaitState ws{&ctrl->abort_flag, &ctrl->err};
     // row x of the gathered rows: its row of q and its head; false when there is none
-    auto locate = [&](int64_t x, int *query, int *head) {
+    auto locate = [&](int x, int *query, int *head) {
         if (x >= n_rows) return false;
-        const int e = (int)(x / per), y = (int)(x - (int64_t)e * per);
-        *query = list[e] * bq + y / G;
-        *head = h * G + y % G;
+        const int e = (int)p.per.quotient(x), y = x - e * per, tok = (int)p.G.quotient(y);
+        *query = list[e] * bq + tok;
+        *head = h * G + y - tok * G;
         return true;
     };
 
@@ -895,8 +905,31 @@ __global__ __launch_bounds__(TK_THREADS, 1) void attn_dkv_tc_kernel(const __grid
             fence_async_smem();
             mbar_arrive(smem_u32(bar));
         };
-        for (int j = 0; j <= n_tiles; j++) {
-            if (j > 1) {
+        // whole tiles by tensor copies; the one in which the rows end, or all when the strides do not allow it, row by row
+        const int by_map = p.box_tokens && q_map.usable && do_map.usable && !q_map.swapped && !do_map.swapped ? n_rows / TK_ROWS : 0;
+        if (by_map) {
+            cp_wait<0>();
+            signal(&ctrl->kv_full);
+            const int box_rows = p.box_tokens * G, boxes = TK_ROWS / box_rows;
+            for (int j = 0; j < by_map; j++) {
+                if (j > 1) fine = __all_sync(~0u, ws.wait(smem_u32(&ctrl->r_empty[j & 1]), (j >> 1) - 1, 1));
+                if (!fine) break;
+                const uint32_t do_dst = ring + (j & 1) * 2 * RT, q_dst = do_dst + RT, bar = smem_u32(&ctrl->r_full[j & 1]);
+                const int i = t % boxes, what = t / boxes;          // box; panel and tensor
+                if (what < 2 * (D / 64)) {
+                    const int panel = what >> 1;
+                    int query, head;
+                    locate(j * TK_ROWS + i * box_rows, &query, &head);
+                    const uint32_t off = panel * (TK_ROWS * 128) + i * box_rows * 128;
+                    mbar_expect_tx(bar, box_rows * 128);
+                    if (what & 1) tma_box(do_dst + off, &do_map.map, panel * 64, head, sq.row0 + query, bar);
+                    else tma_box(q_dst + off, &q_map.map, panel * 64, head, sq.row0 + query, bar);
+                }
+                mbar_arrive(bar);
+            }
+        }
+        for (int j = by_map; j <= n_tiles && fine; j++) {
+            if (j > 1 && j > by_map) {
                 // the buffer comes free only when the tile before has been worked on: announce that one first
                 cp_wait<0>();
                 signal(&ctrl->r_full[(j - 1) & 1]);
@@ -906,7 +939,7 @@ __global__ __launch_bounds__(TK_THREADS, 1) void attn_dkv_tc_kernel(const __grid
                 if (!fine) break;
                 // each lane finds one of the warp's 32 rows, the copies take the addresses from it
                 int query = 0, head = 0;
-                const bool there = locate((int64_t)j * TK_ROWS + lw * 32 + lane, &query, &head);
+                const bool there = locate(j * TK_ROWS + lw * 32 + lane, &query, &head);
                 const int64_t q_at = there ? (int64_t)(sq.row0 + query) * a.q_token + head * a.q_head : -1;
                 const int64_t do_at = (int64_t)(sq.row0 + query) * do_token + head * do_head;
                 const uint32_t do_dst = ring + (j & 1) * 2 * RT, q_dst = do_dst + RT;
@@ -920,7 +953,7 @@ __global__ __launch_bounds__(TK_THREADS, 1) void attn_dkv_tc_kernel(const __grid
                 }
             }
             cp_commit();
-            if (j <= 1) {
+            if (j <= 1 && !by_map) {
                 cp_wait<1>();                                   // the group before: K and V, or the rows of the first tile
                 signal(j ? &ctrl->r_full[0] : &ctrl->kv_full);
             }
@@ -931,38 +964,49 @@ __global__ __launch_bounds__(TK_THREADS, 1) void attn_dkv_tc_kernel(const __grid
         if (lane == 0 && n_tiles) {
             constexpr uint32_t s_desc = mma_desc<T>(128, TK_KEYS, false, false), o_desc = mma_desc<T>(128, TK_KEYS, true, true);
             bool fine = ws.wait(smem_u32(&ctrl->kv_full), 0, 2);
-            for (int j = 0; j <= n_tiles && fine; j++) {
-                if (j < n_tiles) {
-                    fine = ws.wait(smem_u32(&ctrl->r_full[j & 1]), j >> 1, 3);
-                    if (!fine) break;
+            // whichever of the two is ready: the first products of the next tile, when its rows are there and at most one
+            // tile is under way, or the second products of the oldest tile under way.  (In a fixed order the second
+            // products would wait for the copies of the next tile, which wait for their buffer, which they free.)
+            int first = 0, second = 0;
+            unsigned long long t0 = 0;
+            while (second < n_tiles) {
+                if (first < n_tiles && first - second < 2 && mbar_test(smem_u32(&ctrl->r_full[first & 1]), (first >> 1) & 1)) {
                     tc_fence_after();
-                    const uint32_t do_tile = ring + (j & 1) * 2 * RT, q_tile = do_tile + RT, s_at = tmem + (j & 1) * 2 * TK_KEYS;
+                    const uint32_t do_tile = ring + (first & 1) * 2 * RT, q_tile = do_tile + RT, s_at = tmem + (first & 1) * 2 * TK_KEYS;
 #pragma unroll
                     for (int ks = 0; ks < D / 16; ks++)
                         mma_ss(s_at, desc_k_major(q_tile, TK_ROWS, ks), desc_k_major(k_tile, TK_KEYS, ks), s_desc, ks != 0);
 #pragma unroll
                     for (int ks = 0; ks < D / 16; ks++)
                         mma_ss(s_at + TK_KEYS, desc_k_major(do_tile, TK_ROWS, ks), desc_k_major(v_tile, TK_KEYS, ks), s_desc, ks != 0);
-                    umma_commit(smem_u32(&ctrl->s_full[j & 1]));
-                }
-                if (j) {
+                    umma_commit(smem_u32(&ctrl->s_full[first & 1]));
+                    first++;
+                    t0 = 0;
+                } else if (second < first && mbar_test(smem_u32(&ctrl->p_full), second & 1)) {
                     // A: 128 values of dO (of Q) x 128 rows; with D = 64 the tiles of dO and Q one behind the other
-                    const uint32_t do_tile = ring + ((j - 1) & 1) * 2 * RT, q_tile = D == 64 ? do_tile : do_tile + RT;
-                    fine = ws.wait(smem_u32(&ctrl->p_full), j - 1, 4);
-                    if (!fine) break;
+                    const uint32_t do_tile = ring + (second & 1) * 2 * RT, q_tile = D == 64 ? do_tile : do_tile + RT;
                     tc_fence_after();
 #pragma unroll
                     for (int ks = 0; ks < TK_ROWS / 16; ks++)
-                        mma_ss(tmem_dv, desc_mn_major(do_tile, TK_ROWS, ks), desc_mn_major(p_tile, TK_ROWS, ks), o_desc, j > 1 || ks);
+                        mma_ss(tmem_dv, desc_mn_major(do_tile, TK_ROWS, ks), desc_mn_major(p_tile, TK_ROWS, ks), o_desc, second || ks);
                     umma_commit(smem_u32(&ctrl->dv_done));
-                    fine = ws.wait(smem_u32(&ctrl->ds_full), j - 1, 5);
+                    fine = ws.wait(smem_u32(&ctrl->ds_full), second, 5);
                     if (!fine) break;
                     tc_fence_after();
 #pragma unroll
                     for (int ks = 0; ks < TK_ROWS / 16; ks++)
-                        mma_ss(tmem_dk, desc_mn_major(q_tile, TK_ROWS, ks), desc_mn_major(ds_tile, TK_ROWS, ks), o_desc, j > 1 || ks);
-                    umma_commit(smem_u32(&ctrl->r_empty[(j - 1) & 1]));
+                        mma_ss(tmem_dk, desc_mn_major(q_tile, TK_ROWS, ks), desc_mn_major(ds_tile, TK_ROWS, ks), o_desc, second || ks);
+                    umma_commit(smem_u32(&ctrl->r_empty[second & 1]));
                     umma_commit(smem_u32(&ctrl->dk_done));
+                    second++;
+                    t0 = 0;
+                } else {
+                    if (!fine || ctrl->abort_flag) break;
+                    if (!t0) t0 = global_ns();
+                    else if (global_ns() - t0 > WAIT_LIMIT_NS) {
+                        *ws.abort_flag = 1;
+                        break;
+                    }
                 }
             }
         }
@@ -978,7 +1022,7 @@ __global__ __launch_bounds__(TK_THREADS, 1) void attn_dkv_tc_kernel(const __grid
             *minus_lse = -CUDART_INF_F;                         // a row that is none, or has no keys: every p zero
             *minus_delta = 0.f;
             *n_visible = 0;
-            if (j < n_tiles && locate((int64_t)j * TK_ROWS + r, &query, &head)) {
+            if (j < n_tiles && locate(j * TK_ROWS + r, &query, &head)) {
                 const int64_t at = (int64_t)(sq.row0 + query) * a.heads + head;
                 const float z = a.d_lse[at];
                 if (z != -CUDART_INF_F) *minus_lse = -z * LOG2E;
@@ -1145,7 +1189,7 @@ static int backward_launch(const spamm_attn &a, const BackwardPlan &p, const T *
     const int tiles = (int)(((int64_t)bq * (a.heads / a.kv_heads) + 15) / 16);
     const int64_t dq_grid = p.groups * p.nqb * tiles;
     if ((rows + 31) / 32 > INT32_MAX || (lists + 3) / 4 > INT32_MAX || dq_grid > INT32_MAX || p.groups * p.item_cap > INT32_MAX / 2 ||
-        p.groups * p.nkb > INT32_MAX)
+        p.groups * p.nkb > INT32_MAX || (int64_t)bq * (a.heads / a.kv_heads) > (1 << 28))
         return attn_too_large();
 
     SPAMM_CUDA_TRY(cudaMemsetAsync(bits, 0, p.slots - p.bits, stream));
@@ -1175,8 +1219,12 @@ static int backward_launch(const spamm_attn &a, const BackwardPlan &p, const T *
         const size_t smem = 2 * TK_KEYS * D * 2 + 4 * TK_ROWS * D * 2 + 2 * TK_ROWS * TK_KEYS * 2 + sizeof(TkCtrl) + p.chunk * 4;
         st = attn_set_smem((const void *)attn_dkv_tc_kernel<T, D>, smem);
         if (st) return st;
+        RowMap q_map, do_map;
+        const int G = a.heads / a.kv_heads;
+        attn_row_map(a, a.d_q, a.q_token, a.q_head, a.heads, G, max(1, p.box_tokens), &q_map);
+        attn_row_map(a, d_do, do_token, do_head, a.heads, G, max(1, p.box_tokens), &do_map);
         attn_dkv_tc_kernel<T, D><<<(unsigned)(p.groups * p.item_cap * (a.block / TK_KEYS)), TK_THREADS, smem, stream>>>(
-            a, p, d_do, do_token, do_head, delta, bits, items, n_items, partial, dk, dv);
+            a, p, q_map, do_map, d_do, do_token, do_head, delta, bits, items, n_items, partial, dk, dv);
     } else switch (a.block) {
     case 16: st = dkv_launch<T, D, 16>(a, p, d_do, do_token, do_head, delta, bits, items, n_items, partial, dk, dv, stream); break;
     default: st = dkv_launch<T, D, 32>(a, p, d_do, do_token, do_head, delta, bits, items, n_items, partial, dk, dv, stream); break;

@@ -739,38 +739,51 @@ static PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder()
     return fn;
 }
 
-static void row_map(const spamm_attn &a, int box_rows, const void *p, int64_t token, int64_t head, RowMap *out)
+static bool encode_map(const spamm_attn &a, const void *p, const cuuint64_t *dims, const cuuint64_t *strides, const cuuint32_t *box,
+                       RowMap *out)
+{
+    const auto encode = tensor_map_encoder();
+    if (!encode) return false;
+    const cuuint32_t step[3] = {1, 1, 1};
+    const CUtensorMapDataType type = a.dtype == SPAMM_ATTN_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+    return encode(&out->map, type, 3, const_cast<void *>(p), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+void attn_row_map(const spamm_attn &a, const void *p, int64_t token, int64_t head, int heads, int box_heads, int box_tokens,
+                  RowMap *out)
 {
     memset(out, 0, sizeof(*out));
-    const auto encode = tensor_map_encoder();
-    if (!encode) return;
+    // the larger stride last, a multiple of the smaller; a dimension of one element has any stride
+    if (heads == 1) head = a.dim;
+    if (a.tokens == 1) token = head * heads;
+    if (token <= 0 || head <= 0 || token >= (1ll << 38) || head >= (1ll << 38)) return;
+    out->swapped = head > token;
+    const int t = out->swapped ? 1 : 2, h = 3 - t;
+    if ((out->swapped ? head % token : token % head) != 0) return;
     cuuint64_t dims[3] = {(cuuint64_t)a.dim}, strides[2];
-    cuuint32_t box[3] = {64, 1, 1}, step[3] = {1, 1, 1};
-    if (a.n_pages) {
-        if ((int64_t)a.n_pages * a.kv_heads > INT32_MAX) return;
-        dims[1] = a.block; dims[2] = (cuuint64_t)a.n_pages * a.kv_heads;
-        strides[0] = (cuuint64_t)a.dim * 2; strides[1] = (cuuint64_t)a.block * a.dim * 2;
-        box[1] = box_rows;
-    } else {
-        // the larger stride last, a multiple of the smaller
-        if (a.kv_heads == 1) head = a.dim;
-        if (token <= 0 || head <= 0 || token >= (1ll << 38) || head >= (1ll << 38)) return;
-        out->swapped = head > token;
-        const int t = out->swapped ? 1 : 2, h = 3 - t;
-        if ((out->swapped ? head % token : token % head) != 0) return;
-        dims[t] = a.tokens; dims[h] = a.kv_heads;
-        strides[t - 1] = (cuuint64_t)token * 2; strides[h - 1] = (cuuint64_t)head * 2;
-        box[t] = box_rows;
-    }
-    const CUtensorMapDataType type = a.dtype == SPAMM_ATTN_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
-    out->usable = encode(&out->map, type, 3, const_cast<void *>(p), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+    cuuint32_t box[3] = {64, 1, 1};
+    dims[t] = a.tokens; dims[h] = heads;
+    strides[t - 1] = (cuuint64_t)token * 2; strides[h - 1] = (cuuint64_t)head * 2;
+    box[t] = box_tokens; box[h] = box_heads;
+    out->usable = encode_map(a, p, dims, strides, box, out);
 }
 
 void attn_row_maps(const spamm_attn &a, int box_rows, RowMap *k, RowMap *v)
 {
-    row_map(a, box_rows, a.d_k, a.k_token, a.k_head, k);
-    row_map(a, box_rows, a.d_v, a.v_token, a.v_head, v);
+    if (!a.n_pages) {
+        attn_row_map(a, a.d_k, a.k_token, a.k_head, a.kv_heads, 1, box_rows, k);
+        attn_row_map(a, a.d_v, a.v_token, a.v_head, a.kv_heads, 1, box_rows, v);
+        return;
+    }
+    memset(k, 0, sizeof(*k));
+    memset(v, 0, sizeof(*v));
+    if ((int64_t)a.n_pages * a.kv_heads > INT32_MAX) return;
+    const cuuint64_t dims[3] = {(cuuint64_t)a.dim, (cuuint64_t)a.block, (cuuint64_t)a.n_pages * a.kv_heads};
+    const cuuint64_t strides[2] = {(cuuint64_t)a.dim * 2, (cuuint64_t)a.block * a.dim * 2};
+    const cuuint32_t box[3] = {64, (cuuint32_t)box_rows, 1};
+    k->usable = encode_map(a, a.d_k, dims, strides, box, k);
+    v->usable = encode_map(a, a.d_v, dims, strides, box, v);
 }
 
 static int64_t longest_list(const spamm_attn &a)

@@ -94,17 +94,28 @@ template <int COLS> __device__ __forceinline__ void tmem_free(uint32_t base)
 {
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(base), "r"(COLS) : "memory");
 }
+// Whether the phase with this parity is complete, without waiting.
+__device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity)
+{
+    uint32_t ok;
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                 : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+    return ok != 0;
+}
 // What this thread's ordinary stores (cp.async, st.shared) left in shared memory becomes visible to tcgen05.mma.
 __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
-// A tensor map over the rows of k or v: boxes of box_rows keys x 64 values.  Coordinates (value, y, z) of the block that
-// begins at row `row` of key head h: packed (value, h or row, row or h), pages (value, 0, page * kv_heads + h).
+// A tensor map over rows of q, k, v or do.  Packed: boxes of box_tokens x box_heads rows x 64 values, coordinates (value,
+// head, token) or, swapped, (value, token, head).  Pages: boxes of box_tokens keys x 64 values, coordinates (value, 0,
+// page * kv_heads + head).
 struct RowMap {
     CUtensorMap map;
     int usable;          // 0: the strides do not fit a tensor map, rows are copied 16 bytes at a time
-    int swapped;         // packed: the head is the third coordinate
+    int swapped;         // packed: the token is the second coordinate
 };
-// Fills both maps (pages: strides are not read); box_rows keys at a time, at most a block.
+void attn_row_map(const spamm_attn &a, const void *p, int64_t token, int64_t head, int heads, int box_heads, int box_tokens,
+                  RowMap *out);
+// Both maps of the keys, box_rows at a time, at most a block.
 void attn_row_maps(const spamm_attn &a, int box_rows, RowMap *k, RowMap *v);
 
 __device__ __forceinline__ void tma_box(uint32_t dst, const CUtensorMap *map, int x, int y, int z, uint32_t bar)
