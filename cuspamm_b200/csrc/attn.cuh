@@ -90,10 +90,10 @@ __device__ __forceinline__ int64_t attn_block_base(const spamm_attn &a, const Se
     return (int64_t)(sq.row0 + b * a.block) * token + h * head;
 }
 
-// One warp copies the list of (s, qb, h) to `out` (room for n_select), leaving out what is no block below n_blocks or
-// not above every entry before it.  Returns how many there are.
-__device__ __forceinline__ int attn_load_list(const spamm_attn &a, int s, int qb, int nqb, int h, int n_blocks, int *out,
-                                              int lane)
+// One warp walks the list of (s, qb, h) and calls f(entry, how many kept before it) for every entry that counts: no f for
+// what is no block below n_blocks or not above every entry before it.  Returns how many there are.
+template <typename F>
+__device__ __forceinline__ int attn_for_list(const spamm_attn &a, int s, int qb, int nqb, int h, int n_blocks, int lane, F f)
 {
     const int32_t *list = a.d_lists + (((int64_t)s * nqb + qb) * a.kv_heads + h) * a.n_select;
     int count = 0, top = -1;
@@ -110,12 +110,17 @@ __device__ __forceinline__ int attn_load_list(const spamm_attn &a, int s, int qb
         before = max(lane ? before : -1, top);
         const bool keep = v > before;
         const unsigned m = __ballot_sync(~0u, keep);
-        if (keep) out[count + __popc(m & ((1u << lane) - 1))] = v;
+        if (keep) f(v, count + __popc(m & ((1u << lane) - 1)));
         count += __popc(m);
         top = max(top, __shfl_sync(~0u, run, 31));
     }
     __syncwarp();
     return count;
+}
+// The same into an array with room for n_select.
+__device__ __forceinline__ int attn_load_list(const spamm_attn &a, int s, int qb, int nqb, int h, int n_blocks, int *out, int lane)
+{
+    return attn_for_list(a, s, qb, nqb, h, n_blocks, lane, [&](int v, int i) { out[i] = v; });
 }
 
 // ---- types

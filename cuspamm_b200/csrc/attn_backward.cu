@@ -553,9 +553,9 @@ __global__ __launch_bounds__(KEYS == 128 ? 256 : 128) void attn_dkv_kernel(
 // ---- tiles of 128 rows on the tensor memory path
 //
 // dq: 128 rows (queries x heads of a key head), 64 listed keys at a time.  S = Q K^T and dP = dO V^T go to tensor memory, a
-// thread for each row writes ds over S, dQ += ds K takes it from there.  Half the tensor memory and half the shared memory:
+// pair of threads for each row writes ds over S, dQ += ds K takes it from there.  Half the tensor memory and half the shared memory:
 // two blocks of threads share an SM, one's exponentials run beside the other's products.
-constexpr int TQ_ROWS = 128, TQ_KEYS = 64, TQ_THREADS = 192, TQ_COLS = 256;
+constexpr int TQ_ROWS = 128, TQ_KEYS = 64, TQ_SOFTMAX = 256, TQ_THREADS = TQ_SOFTMAX + 64, TQ_COLS = 256;
 
 struct TqCtrl {
     uint64_t q_full, k_full[2], k_empty[2], v_full, v_empty, s_full, ds_full, dq_done;
@@ -566,7 +566,8 @@ struct TqCtrl {
 };
 
 template <typename T, int D>
-__global__ __launch_bounds__(TQ_THREADS, 2) void attn_dq_tc_kernel(const __grid_constant__ spamm_attn a, int nqb, int tiles,
+__global__ __launch_bounds__(TQ_THREADS, 2) void attn_dq_tc_kernel(const __grid_constant__ spamm_attn a, int tiles,
+                                                                   int max_entries,
                                                                    const __grid_constant__ RowMap k_map,
                                                                    const __grid_constant__ RowMap v_map, const T *d_do,
                                                                    int64_t do_token, int64_t do_head, const float *delta, T *dq)
@@ -576,31 +577,24 @@ __global__ __launch_bounds__(TQ_THREADS, 2) void attn_dq_tc_kernel(const __grid_
     constexpr int RT = TQ_ROWS * D * 2, KT = TQ_KEYS * D * 2;
     const uint32_t q_tile = smem_u32(smem), do_tile = q_tile + RT, k_ring = do_tile + RT, v_tile = k_ring + 2 * KT;
     TqCtrl *ctrl = reinterpret_cast<TqCtrl *>(smem + 2 * RT + 3 * KT);
-    int *blk = reinterpret_cast<int *>(ctrl + 1);
+    uint32_t *bits = reinterpret_cast<uint32_t *>(ctrl + 1);           // [max_entries]
+    uint16_t *blk = reinterpret_cast<uint16_t *>(bits + max_entries);
 
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     unsigned idx = blockIdx.x;
-    const int tile = idx % tiles; idx /= tiles;
-    const int qb = nqb - 1 - idx % nqb; idx /= nqb;
+    const int tile = tiles - 1 - idx % tiles; idx /= tiles;
     const int h = idx % a.kv_heads;
     const int s = idx / a.kv_heads;
     const int G = a.heads / a.kv_heads;
     const Seq sq = attn_seq(a, s);
-    const int bq = min(a.query_block, a.max_q);
-    const int n_tok = min(bq, sq.nq - qb * bq);
-    const int64_t n_rows = (int64_t)max(n_tok, 0) * G;
-    if ((int64_t)tile * TQ_ROWS >= n_rows) return;
-    const int rows = (int)min((int64_t)TQ_ROWS, n_rows - tile * TQ_ROWS);
-    const int query0 = qb * bq;
-    const int limit_max = attn_limit(a, sq, query0 + (tile * TQ_ROWS + rows - 1) / G);
-    const int limit_min = attn_limit(a, sq, query0 + tile * TQ_ROWS / G);
+    TileRows tr;
+    if (!attn_tile(a, sq, tile, &tr)) return;
+    const int rows = tr.rows;
+    const int limit_max = attn_limit(a, sq, tr.last), limit_min = attn_limit(a, sq, tr.first);
 
-    if (warp == 0) {
-        const int n = attn_load_list(a, s, qb, nqb, h, ceil_div(limit_max, a.block), blk, lane);
-        if (lane == 0) ctrl->count = n;
-    } else if (warp == 4) {
+    if (warp == 8) {
         if (lane == 0) {
-            mbar_init(smem_u32(&ctrl->q_full), 128);
+            mbar_init(smem_u32(&ctrl->q_full), TQ_SOFTMAX);
             for (int i = 0; i < 2; i++) {
                 mbar_init(smem_u32(&ctrl->k_full[i]), 32);
                 mbar_init(smem_u32(&ctrl->k_empty[i]), 1);
@@ -608,7 +602,7 @@ __global__ __launch_bounds__(TQ_THREADS, 2) void attn_dq_tc_kernel(const __grid_
             mbar_init(smem_u32(&ctrl->v_full), 32);
             mbar_init(smem_u32(&ctrl->v_empty), 1);
             mbar_init(smem_u32(&ctrl->s_full), 1);
-            mbar_init(smem_u32(&ctrl->ds_full), 128);
+            mbar_init(smem_u32(&ctrl->ds_full), TQ_SOFTMAX);
             mbar_init(smem_u32(&ctrl->dq_done), 1);
             ctrl->abort_flag = 0;
             ctrl->err = 0;
@@ -618,15 +612,16 @@ __global__ __launch_bounds__(TQ_THREADS, 2) void attn_dq_tc_kernel(const __grid_
         tmem_alloc<TQ_COLS>(smem_u32(&ctrl->tmem_base));
         tc_fence_before();
     }
-    __syncthreads();
+    const int n_entries = attn_union<TQ_THREADS>(a, sq, s, h, tr, 0, ceil_div(limit_max, a.block), reinterpret_cast<uint32_t *>(smem),
+                                                 blk, bits, &ctrl->count);
     tc_fence_after();
     const int log_block = 31 - __clz(a.block);
-    const int n_entries = ctrl->count, n_keys = n_entries << log_block;
+    const int n_keys = n_entries << log_block;
     const int n_tiles = (n_keys + TQ_KEYS - 1) / TQ_KEYS;
     const uint32_t tmem = ctrl->tmem_base, tmem_dp = tmem + TQ_KEYS, tmem_dq = tmem + 2 * TQ_KEYS;
     const WaitState ws{&ctrl->abort_flag, &ctrl->err};
 
-    if (warp == 5) {
+    if (warp == 9) {
         const int piece = min(a.block, TQ_KEYS), pieces = TQ_KEYS / piece;     // a piece: keys of one block, one tensor copy
         auto load = [&](int j, uint32_t dst, bool value, uint64_t *full) {
             const uint32_t bar = smem_u32(full);
@@ -671,7 +666,7 @@ __global__ __launch_bounds__(TQ_THREADS, 2) void attn_dq_tc_kernel(const __grid_
             if (!fine) break;
             load(j, v_tile, true, &ctrl->v_full);
         }
-    } else if (warp == 4) {
+    } else if (warp == 8) {
         if (lane == 0 && n_tiles) {
             constexpr uint32_t s_desc = mma_desc<T>(128, TQ_KEYS, false, false), q_desc = mma_desc<T>(128, D, false, true);
             bool fine = ws.wait(smem_u32(&ctrl->q_full), 0, 3);
@@ -680,13 +675,14 @@ __global__ __launch_bounds__(TQ_THREADS, 2) void attn_dq_tc_kernel(const __grid_
                 fine = ws.wait(smem_u32(&ctrl->k_full[j & 1]), j >> 1, 4) && ws.wait(smem_u32(&ctrl->v_full), j, 5);
                 if (!fine) break;
                 tc_fence_after();
-#pragma unroll
-                for (int ks = 0; ks < D / 16; ks++)
-                    mma_ss(tmem, desc_k_major(q_tile, TQ_ROWS, ks), desc_k_major(k_tile, TQ_KEYS, ks), s_desc, ks != 0);
+                // dP first: the buffer of V comes free the earlier
 #pragma unroll
                 for (int ks = 0; ks < D / 16; ks++)
                     mma_ss(tmem_dp, desc_k_major(do_tile, TQ_ROWS, ks), desc_k_major(v_tile, TQ_KEYS, ks), s_desc, ks != 0);
                 umma_commit(smem_u32(&ctrl->v_empty));
+#pragma unroll
+                for (int ks = 0; ks < D / 16; ks++)
+                    mma_ss(tmem, desc_k_major(q_tile, TQ_ROWS, ks), desc_k_major(k_tile, TQ_KEYS, ks), s_desc, ks != 0);
                 umma_commit(smem_u32(&ctrl->s_full));
                 fine = ws.wait(smem_u32(&ctrl->ds_full), j, 6);
                 if (!fine) break;
@@ -694,80 +690,88 @@ __global__ __launch_bounds__(TQ_THREADS, 2) void attn_dq_tc_kernel(const __grid_
                 const int steps = min(TQ_KEYS, n_keys - j * TQ_KEYS) / 16;      // rows of K behind were never written
 #pragma unroll
                 for (int ks = 0; ks < TQ_KEYS / 16; ks++)
-                    if (ks < steps) mma_ts(tmem_dq, tmem + ks * 8, desc_mn_major(k_tile, TQ_KEYS, ks), q_desc, j || ks);
+                    if (ks < steps) mma_ts(tmem_dq, tmem + (ks >> 1) * 32 + (ks & 1) * 8, desc_mn_major(k_tile, TQ_KEYS, ks), q_desc, j || ks);
                 umma_commit(smem_u32(&ctrl->k_empty[j & 1]));
                 umma_commit(smem_u32(&ctrl->dq_done));
             }
         }
         __syncwarp();
     } else {
-        for (int i = 0; i < D / 8; i++) {
-            const int x = i * 128 + tid, qr = x / (D / 8), c = x % (D / 8);
+        for (int i = 0; i < D / 16; i++) {
+            const int x = i * TQ_SOFTMAX + tid, qr = x / (D / 8), c = x % (D / 8);
             const bool ok = qr < rows;
-            const int qy = tile * TQ_ROWS + (ok ? qr : 0);
-            const int64_t row = sq.row0 + query0 + qy / G, head = h * G + qy % G;
+            const int qy = tr.row0 + (ok ? qr : 0);
+            const int64_t row = sq.row0 + qy / G, head = h * G + qy % G;
             cp_async16(q_tile + panel_off(TQ_ROWS, qr, c), static_cast<const T *>(a.d_q) + row * a.q_token + head * a.q_head + c * 8, ok);
             cp_async16(do_tile + panel_off(TQ_ROWS, qr, c), d_do + row * do_token + head * do_head + c * 8, ok);
         }
         cp_commit();
-        const int r = tid, y = tile * TQ_ROWS + min(r, rows - 1);
-        const int limit = attn_limit(a, sq, query0 + y / G);
-        const int64_t at = (int64_t)(sq.row0 + query0 + y / G) * a.heads + h * G + y % G;
+        const int r = tid & 127, half = warp >> 2, y = tr.row0 + min(r, rows - 1);
+        const int limit = attn_limit(a, sq, y / G);
+        const uint32_t my_bit = 1u << (y / G / a.query_block - tr.qb0), all_bits = tr.n_qb == 32 ? ~0u : (1u << tr.n_qb) - 1;
+        const int64_t at = (int64_t)(sq.row0 + y / G) * a.heads + h * G + y % G;
         const float z = a.d_lse[at];
         const float minus_lse = z == -CUDART_INF_F ? -CUDART_INF_F : -z * LOG2E;       // a row without keys: every p zero
         const float minus_delta = -delta[at] * a.scale;
         cp_wait<0>();
         fence_async_smem();
         mbar_arrive(smem_u32(&ctrl->q_full));
-        const uint32_t lane_s = tmem + ((uint32_t)(warp * 32) << 16), lane_dp = lane_s + TQ_KEYS, lane_dq = lane_s + 2 * TQ_KEYS;
+        const uint32_t lane_s = tmem + ((uint32_t)((warp & 3) * 32) << 16) + half * 32, lane_dp = lane_s + TQ_KEYS;
+        const uint32_t lane_dq = tmem_dq + ((uint32_t)((warp & 3) * 32) << 16) + half * (D / 2);
         const float scale2 = a.scale * LOG2E;
         const float2 sc2 = make_float2(scale2, scale2), ml2 = make_float2(minus_lse, minus_lse);
         const float2 sc = make_float2(a.scale, a.scale), md = make_float2(minus_delta, minus_delta);
         bool fine = true;
         for (int j = 0; j < n_tiles; j++) {
+            // lanes 0 and 1: position and lists of this half's groups of 16 keys
+            int group_pos = INT32_MAX / 2;
+            uint32_t group_bits = all_bits;
+            if (lane < 2) {
+                const int key = j * TQ_KEYS + half * 32 + lane * 16, e = key >> log_block;
+                if (e < n_entries) {
+                    group_pos = blk[e] * a.block + (key & (a.block - 1));
+                    group_bits = bits[e];
+                }
+            }
+            const bool masked = __any_sync(~0u, (lane < 2 && group_pos > limit_min - 16) || group_bits != all_bits);
             fine = __all_sync(~0u, ws.wait(smem_u32(&ctrl->s_full), j, 7));
             if (!fine) break;
             tc_fence_after();
-            int group_pos = INT32_MAX / 2;
-            if (lane < TQ_KEYS / 16) {
-                const int key = j * TQ_KEYS + lane * 16, e = key >> log_block;
-                if (e < n_entries) group_pos = blk[e] * a.block + (key & (a.block - 1));
+            uint32_t v[32], d[32], w[16];
+            tmem_ld32(lane_s, v);
+            tmem_ld32(lane_dp, d);
+            tmem_wait_ld();
+            tmem_landed<32>(v);
+            tmem_landed<32>(d);
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+                const float2 x = fma2(make_float2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), sc2, ml2);
+                const float2 g = fma2(make_float2(__uint_as_float(d[2 * i]), __uint_as_float(d[2 * i + 1])), sc, md);
+                v[2 * i] = __float_as_uint(fast_exp2(x.x) * g.x);
+                v[2 * i + 1] = __float_as_uint(fast_exp2(x.y) * g.y);
             }
-            const bool masked = __any_sync(~0u, lane < TQ_KEYS / 16 && group_pos > limit_min - 16);
+            if (masked) {
 #pragma unroll
-            for (int c = 0; c < TQ_KEYS / 32; c++) {
-                uint32_t v[32], d[32], w[16];
-                tmem_ld32(lane_s + c * 32, v);
-                tmem_ld32(lane_dp + c * 32, d);
-                tmem_wait_ld();
-                tmem_landed<32>(v);
-                tmem_landed<32>(d);
+                for (int g = 0; g < 2; g++) {
+                    const int pos = __shfl_sync(~0u, group_pos, g);
+                    const int n = __shfl_sync(~0u, group_bits, g) & my_bit ? limit - pos : 0;
 #pragma unroll
-                for (int i = 0; i < 16; i++) {
-                    const float2 x = fma2(make_float2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), sc2, ml2);
-                    const float2 g = fma2(make_float2(__uint_as_float(d[2 * i]), __uint_as_float(d[2 * i + 1])), sc, md);
-                    v[2 * i] = __float_as_uint(fast_exp2(x.x) * g.x);
-                    v[2 * i + 1] = __float_as_uint(fast_exp2(x.y) * g.y);
+                    for (int i = 0; i < 16; i++)
+                        if (i >= n) v[g * 16 + i] = 0u;
                 }
-                if (masked) {
-                    const int n0 = limit - __shfl_sync(~0u, group_pos, 2 * c), n1 = limit - __shfl_sync(~0u, group_pos, 2 * c + 1);
-#pragma unroll
-                    for (int i = 0; i < 32; i++)
-                        if ((i & 15) >= (i < 16 ? n0 : n1)) v[i] = 0u;
-                }
-#pragma unroll
-                for (int i = 0; i < 16; i++) w[i] = Pack<T>::two(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]));
-                tmem_st16(lane_s + c * 16, w);                  // over columns whose scores have been read
             }
+#pragma unroll
+            for (int i = 0; i < 16; i++) w[i] = Pack<T>::two(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]));
+            tmem_st16(lane_s, w);                               // over this thread's scores, which have been read
             tmem_wait_st();
             tc_fence_before();
             mbar_arrive(smem_u32(&ctrl->ds_full));
         }
         if (n_tiles && fine) fine = __all_sync(~0u, ws.wait(smem_u32(&ctrl->dq_done), n_tiles - 1, 8));
         tc_fence_after();
-        T *dst = dq + at * D;
+        T *dst = dq + at * D + half * (D / 2);
 #pragma unroll 1
-        for (int c = 0; c < D / 32; c++) {
+        for (int c = 0; c < D / 64; c++) {
             uint32_t v[32];
             if (n_tiles) {
                 tmem_ld32(lane_dq + c * 32, v);
@@ -790,7 +794,7 @@ __global__ __launch_bounds__(TQ_THREADS, 2) void attn_dq_tc_kernel(const __grid_
         tc_fence_before();
     }
     __syncthreads();
-    if (warp == 4) {
+    if (warp == 8) {
         if (ctrl->abort_flag) drain_products();
         __syncwarp();
         tc_fence_after();
@@ -1197,17 +1201,19 @@ static int backward_launch(const spamm_attn &a, const BackwardPlan &p, const T *
     attn_turn_kernel<<<(unsigned)((lists + 3) / 4), 128, 0, stream>>>(a, p.nqb, p.nkb, p.words, bits, counts);
     attn_items_kernel<<<(unsigned)p.groups, 1024, 0, stream>>>(a, p, counts, slots, items, n_items);
 
-    // from 48 rows that share a list on, tiles of 128 rows; below, tiles of 16
+    // from 48 rows of a sequence and key head on, tiles of 128 rows; below, and over more blocks than a union is built
+    // over, tiles of 16
     int st;
-    if ((int64_t)bq * (a.heads / a.kv_heads) >= 48) {
-        const int tq = (int)(((int64_t)bq * (a.heads / a.kv_heads) + TQ_ROWS - 1) / TQ_ROWS);
+    const int tq = attn_tiles(a);
+    if ((int64_t)a.max_q * (a.heads / a.kv_heads) >= 48 && p.nkb <= UNION_BLOCKS && p.groups * tq <= INT32_MAX) {
         RowMap k_map, v_map;
         attn_row_maps(a, min(a.block, TQ_KEYS), &k_map, &v_map);
-        const size_t smem = 2 * TQ_ROWS * D * 2 + 3 * TQ_KEYS * D * 2 + sizeof(TqCtrl) + a.n_select * 4;
+        const int entries = (int)min((int64_t)p.nkb, (int64_t)attn_tile_lists(a) * a.n_select);
+        const size_t smem = 2 * TQ_ROWS * D * 2 + 3 * TQ_KEYS * D * 2 + sizeof(TqCtrl) + 6 * (size_t)entries;
         st = attn_set_smem((const void *)attn_dq_tc_kernel<T, D>, smem);
         if (st) return st;
-        attn_dq_tc_kernel<T, D><<<(unsigned)(p.groups * p.nqb * tq), TQ_THREADS, smem, stream>>>(
-            a, p.nqb, tq, k_map, v_map, d_do, do_token, do_head, delta, dq);
+        attn_dq_tc_kernel<T, D><<<(unsigned)(p.groups * tq), TQ_THREADS, smem, stream>>>(
+            a, tq, entries, k_map, v_map, d_do, do_token, do_head, delta, dq);
     } else {
     const size_t dq_smem = (size_t)DQ_WARPS * DQ_STAGES * 2 * 16 * D * 2 + 2 * 16 * D * 2 + a.n_select * 4;
     st = attn_set_smem((const void *)attn_dq_rows_kernel<T, D>, dq_smem);

@@ -350,7 +350,7 @@ __global__ __launch_bounds__(128) void attn_rows_kernel(const __grid_constant__ 
 // ---- tiles of 128 rows on the tensor memory path
 //
 // Per block of threads: 128 rows (queries x heads of a key head) against a range of its keys, 128 keys (the listed blocks
-// one behind the other) at a time.  S = Q K^T goes to tensor memory; four warps, a thread for each row, take the running
+// one behind the other) at a time.  S = Q K^T goes to tensor memory; eight warps, two threads for each row, take the running
 // maximum and write p over S in the type of v; O += P V takes p from tensor memory.  A block uses half of the tensor
 // memory and under half of the shared memory, so that two of them share an SM: one's exponentials run beside the other's
 // products.  One warp feeds K and V, a tensor copy for each block of keys and 64 values; the block in which the sequence
@@ -358,16 +358,20 @@ __global__ __launch_bounds__(128) void attn_rows_kernel(const __grid_constant__ 
 //
 // The running maximum is only raised when a row's scores exceed it by more than 2^8: until then p stays below 2^8, which
 // both types and the float sums hold without loss, and O need not be rescaled in tensor memory.
-constexpr int TC_ROWS = 128, TC_KEYS = 128;
-constexpr int TC_SOFTMAX = 128, TC_THREADS = TC_SOFTMAX + 64;
-constexpr int TC_COLS = 256;            // S (P over it) in columns 0..127, O behind
+constexpr int TC_ROWS = 128, TC_KEYS = 128, TC_HALF = TC_KEYS / 2;
+constexpr int TC_SOFTMAX = 256, TC_THREADS = TC_SOFTMAX + 64;
+constexpr int TC_COLS = 256;            // S (P over each half of it) in columns 0..127, O behind
 
 struct TcCtrl {
     uint64_t q_full, k_full, k_empty, v_full, v_empty, s_full, p_full, pv_done;
+    uint64_t met[4];                    // the two warps of 32 rows have left their maxima
     uint32_t tmem_base;
     uint32_t abort_flag;
     int32_t err;
     int32_t count;
+    int32_t bad_page;
+    int32_t pad[3];
+    float top[2][2][TC_ROWS];           // [tile & 1][half][row]
 };
 
 template <typename T, int D>
@@ -376,42 +380,30 @@ __global__ __launch_bounds__(TC_THREADS, 2) void attn_tc_kernel(const __grid_con
                                                                 const __grid_constant__ RowMap v_map, float *part_o,
                                                                 float *part_lse)
 {
-    extern __shared__ __align__(16) uint8_t smem_raw[];
+    extern __shared__ __align__(1024) uint8_t smem_tc[];
     constexpr int TILE = 128 * D * 2;
-    const uint32_t raw = smem_u32(smem_raw);
-    uint8_t *smem = smem_raw + ((1024 - (raw & 1023)) & 1023);
+    uint8_t *const smem = smem_tc;
     const uint32_t q_tile = smem_u32(smem), k_tile = q_tile + TILE, v_tile = k_tile + TILE;
     TcCtrl *ctrl = reinterpret_cast<TcCtrl *>(smem + 3 * TILE);
-    int64_t *base = reinterpret_cast<int64_t *>(ctrl + 1);
-    int *blk = reinterpret_cast<int *>(base + p.max_entries);
+    uint32_t *bits = reinterpret_cast<uint32_t *>(ctrl + 1);           // [max_entries], with lists
+    uint16_t *idx = reinterpret_cast<uint16_t *>(bits + (a.n_select ? p.max_entries : 0));
 
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    unsigned idx = blockIdx.x;
+    unsigned where = blockIdx.x;
     // tiles that read the same keys run side by side, those with the longest causal rows first
-    const int tile = p.tiles - 1 - idx % p.tiles; idx /= p.tiles;
-    const int qb = p.nqb - 1 - idx % p.nqb; idx /= p.nqb;
-    const int split = idx % p.n_split; idx /= p.n_split;
-    const int h = idx % a.kv_heads;
-    const int s = idx / a.kv_heads;
+    const int tile = p.tiles - 1 - where % p.tiles; where /= p.tiles;
+    const int split = where % p.n_split; where /= p.n_split;
+    const int h = where % a.kv_heads;
+    const int s = where / a.kv_heads;
     const int G = a.heads / a.kv_heads;
     const Seq sq = attn_seq(a, s);
-    if (a.zero_tail && split == 0) zero_tail<T>(a, sq, s, h, qb * p.tiles + tile, p.nqb * p.tiles);
-    const int n_tok = min(p.bq, sq.nq - qb * p.bq);
-    const int64_t n_rows = (int64_t)max(n_tok, 0) * G;
-    if ((int64_t)tile * TC_ROWS >= n_rows) return;
-    const int rows = (int)min((int64_t)TC_ROWS, n_rows - tile * TC_ROWS);
-    const int query0 = qb * p.bq;
-    const int first_query = query0 + tile * TC_ROWS / G, last_query = query0 + (tile * TC_ROWS + rows - 1) / G;
-    const int limit_max = attn_limit(a, sq, sq.pos0 + last_query);
-    const int limit_min = attn_limit(a, sq, sq.pos0 + first_query);
+    if (a.zero_tail && split == 0) zero_tail<T>(a, sq, s, h, tile, p.tiles);
+    TileRows tr;
+    if (!attn_tile(a, sq, tile, &tr)) return;
+    const int rows = tr.rows;
+    const int limit_max = attn_limit(a, sq, sq.pos0 + tr.last), limit_min = attn_limit(a, sq, sq.pos0 + tr.first);
 
-    if (warp == 0) {
-        if (a.n_select) {
-            const int n = attn_load_list(a, s, qb, p.nqb, h, ceil_div(limit_max, a.block), blk, lane);
-            if (lane == 0) ctrl->count = n;
-        } else if (lane == 0)
-            ctrl->count = ceil_div(limit_max, a.block);
-    } else if (warp == 4) {
+    if (warp == 8) {
         if (lane == 0) {
             mbar_init(smem_u32(&ctrl->q_full), TC_SOFTMAX);
             mbar_init(smem_u32(&ctrl->k_full), 32);
@@ -421,76 +413,99 @@ __global__ __launch_bounds__(TC_THREADS, 2) void attn_tc_kernel(const __grid_con
             mbar_init(smem_u32(&ctrl->s_full), 1);
             mbar_init(smem_u32(&ctrl->pv_done), 1);
             mbar_init(smem_u32(&ctrl->p_full), TC_SOFTMAX);
+            for (int i = 0; i < 4; i++) mbar_init(smem_u32(&ctrl->met[i]), 64);
             ctrl->abort_flag = 0;
             ctrl->err = 0;
+            ctrl->bad_page = 0;
             asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         }
         __syncwarp();
         tmem_alloc<TC_COLS>(smem_u32(&ctrl->tmem_base));
         tc_fence_before();
     }
-    __syncthreads();
-    tc_fence_after();
-    const int per_split = p.split_keys / a.block;
-    const int e0 = min(split * per_split, ctrl->count), n_entries = min(per_split, ctrl->count - e0);
-    // first position of every block of the range (far behind every limit for a page that does not exist) and where its
-    // rows of k begin
-    int my_pos[6];
-    for (int i = 0, e = tid; e < n_entries; e += TC_THREADS, i++) {
-        const int b = a.n_select ? blk[e0 + e] : e0 + e;
-        int64_t at = attn_block_base(a, sq, s, h, b, a.k_token, a.k_head);
-        if (a.n_pages && at >= 0) at /= a.block * D;                   // pages: page * kv_heads + h
-        base[e] = at;
-        my_pos[i] = at < 0 ? INT32_MAX / 2 : b * a.block;
-    }
-    __syncthreads();
-    for (int i = 0, e = tid; e < n_entries; e += TC_THREADS, i++) blk[e] = my_pos[i];
-    __syncthreads();
     const int log_block = 31 - __clz(a.block);
+    const int b0 = min(split * (p.split_keys >> log_block), ceil_div(limit_max, a.block));
+    const int b1 = min(b0 + (p.split_keys >> log_block), ceil_div(limit_max, a.block));
+    int n_entries = b1 - b0;
+    if (a.n_select) {
+        n_entries = attn_union<TC_THREADS>(a, sq, s, h, tr, b0, b1, reinterpret_cast<uint32_t *>(smem), idx, bits, &ctrl->count);
+    } else {
+        __syncthreads();
+        if (a.n_pages) {
+            for (int e = tid; e < n_entries; e += TC_THREADS) {
+                const int page = a.d_table[(int64_t)s * a.table_stride + b0 + e];
+                if (page < 0 || page >= a.n_pages) {
+                    ctrl->bad_page = 1;
+                    *a.d_status = SPAMM_ERR_INVALID;
+                }
+            }
+            __syncthreads();
+        }
+    }
+    tc_fence_after();
+    // block of keys of entry e
+    auto block_of = [&](int e) { return b0 + (a.n_select ? (int)idx[e] : e); };
+    auto page_of = [&](int b) { return a.d_table[(int64_t)s * a.table_stride + b]; };
     const int n_keys = n_entries << log_block;
     const int n_tiles = (n_keys + TC_KEYS - 1) / TC_KEYS;
     const uint32_t tmem = ctrl->tmem_base, tmem_o = tmem + TC_KEYS;
     const WaitState ws{&ctrl->abort_flag, &ctrl->err};
 
-    if (warp == 5) {
+    if (warp == 9) {
         // ---- K and V
-        const int64_t k_tok = a.n_pages ? D : a.k_token, v_tok = a.n_pages ? D : a.v_token;
-        const int per_tile = max(1, TC_KEYS >> log_block);
-        // every lane takes part in the barrier's phase with the bytes of its tensor copies and one arrival
-        auto load = [&](int j, bool value, uint64_t *full) {
+        const int per_tile = TC_KEYS >> log_block;
+        // lane's copies of a tile: entry j * per_tile + my_i, values 64 * my_panel ..
+        const int my_i = lane / (D / 64), my_panel = lane % (D / 64);
+        // where they begin: the row of packed keys, or page * kv_heads + head; -1: not there, -2: to be copied by hand
+        struct At { int row, pos; };
+        auto look_up = [&](int j) {
+            At at{-1, 0};
+            const int e = j * per_tile + my_i;
+            if (my_i < per_tile && e < n_entries) {
+                const int b = block_of(e);
+                at.pos = b * a.block;
+                at.row = sq.row0 + at.pos;
+                if (a.n_pages) {
+                    const int page = page_of(b);
+                    at.row = page < 0 || page >= a.n_pages ? -2 : page * a.kv_heads + h;
+                }
+                if (at.pos + a.block > sq.nk) at.row = -2;
+            }
+            return at;
+        };
+        // every lane takes part in the barrier's phase with the bytes of its tensor copy and one arrival
+        auto load = [&](int j, const At &at, bool value, uint64_t *full) {
             const uint32_t dst = value ? v_tile : k_tile, bar = smem_u32(full);
             const RowMap &rm = value ? v_map : k_map;
-            const T *src0 = static_cast<const T *>(value ? a.d_v : a.d_k);
-            const int64_t tok = value ? v_tok : k_tok;
-            bool by_hand = false;
-            for (int x = lane; x < per_tile * (D / 64); x += 32) {
-                const int i = x / (D / 64), panel = x % (D / 64), e = j * per_tile + i;
-                if (e >= n_entries) continue;
-                const int pos = blk[e];
-                if (!rm.usable || pos + a.block > sq.nk) { by_hand = true; continue; }
-                int y = 0, z = (int)base[e];
-                if (!a.n_pages) {
-                    y = rm.swapped ? sq.row0 + pos : h;
-                    z = rm.swapped ? h : sq.row0 + pos;
-                }
+            if (at.row >= 0 && rm.usable) {
                 mbar_expect_tx(bar, a.block * 128);
-                tma_box(dst + panel * (128 * 128) + (i << log_block) * 128, &rm.map, panel * 64, y, z, bar);
+                int y = 0, z = at.row;
+                if (!a.n_pages) {
+                    y = rm.swapped ? at.row : h;
+                    z = rm.swapped ? h : at.row;
+                }
+                tma_box(dst + my_panel * (128 * 128) + (my_i << log_block) * 128, &rm.map, my_panel * 64, y, z, bar);
             }
-            if (__any_sync(~0u, by_hand)) {
+            if (__any_sync(~0u, at.row == -2 || (at.row >= 0 && !rm.usable))) {
+                const T *src0 = static_cast<const T *>(value ? a.d_v : a.d_k);
+                const int64_t tok = a.n_pages ? D : value ? a.v_token : a.k_token;
                 for (int i = 0; i < per_tile; i++) {
                     const int e = j * per_tile + i;
                     if (e >= n_entries) break;
-                    const int pos = blk[e];
-                    if (rm.usable && pos + a.block <= sq.nk) continue;
-                    const int n = sq.nk - pos;                         // none of a page that does not exist
-                    int64_t at = 0;
-                    if (n > 0) {
-                        if (a.n_pages) at = base[e] * a.block * D;
-                        else at = (int64_t)(sq.row0 + pos) * tok + h * (value ? a.v_head : a.k_head);
+                    const int b = block_of(e), pos = b * a.block;
+                    int n = sq.nk - pos;                               // keys of the block that are there
+                    int64_t from = (int64_t)(sq.row0 + pos) * tok + h * (value ? a.v_head : a.k_head);
+                    bool page_ok = true;
+                    if (a.n_pages) {
+                        const int page = page_of(b);
+                        page_ok = page >= 0 && page < a.n_pages;
+                        from = ((int64_t)page * a.kv_heads + h) * a.block * D;
                     }
+                    if (page_ok && rm.usable && n >= a.block) continue;
+                    if (!page_ok) n = 0;
                     for (int x = lane; x < a.block * (D / 8); x += 32) {
                         const int r = x / (D / 8), c = x % (D / 8);
-                        cp_async16(dst + panel_off(128, (i << log_block) + r, c), src0 + (r < n ? at + r * tok : 0) + c * 8, r < n);
+                        cp_async16(dst + panel_off(128, (i << log_block) + r, c), src0 + (r < n ? from + r * tok : 0) + c * 8, r < n);
                     }
                 }
                 cp_commit();
@@ -500,15 +515,18 @@ __global__ __launch_bounds__(TC_THREADS, 2) void attn_tc_kernel(const __grid_con
             mbar_arrive(bar);
         };
         bool fine = true;
+        At at = look_up(0);
         for (int j = 0; j < n_tiles; j++) {
+            const At next = look_up(j + 1);
             if (j) fine = __all_sync(~0u, ws.wait(smem_u32(&ctrl->k_empty), j - 1, 1));
             if (!fine) break;
-            load(j, false, &ctrl->k_full);
+            load(j, at, false, &ctrl->k_full);
             if (j) fine = __all_sync(~0u, ws.wait(smem_u32(&ctrl->v_empty), j - 1, 2));
             if (!fine) break;
-            load(j, true, &ctrl->v_full);
+            load(j, at, true, &ctrl->v_full);
+            at = next;
         }
-    } else if (warp == 4) {
+    } else if (warp == 8) {
         // ---- products
         if (lane == 0 && n_tiles) {
             constexpr uint32_t s_desc = mma_desc<T>(128, TC_KEYS, false, false), o_desc = mma_desc<T>(128, D, false, true);
@@ -522,7 +540,7 @@ __global__ __launch_bounds__(TC_THREADS, 2) void attn_tc_kernel(const __grid_con
                     const int steps = min(TC_KEYS, n_keys - (j - 1) * TC_KEYS) / 16;
 #pragma unroll
                     for (int ks = 0; ks < TC_KEYS / 16; ks++)
-                        if (ks < steps) mma_ts(tmem_o, tmem + ks * 8, desc_mn_major(v_tile, 128, ks), o_desc, j > 1 || ks);
+                        if (ks < steps) mma_ts(tmem_o, tmem + (ks >> 2) * TC_HALF + (ks & 3) * 8, desc_mn_major(v_tile, 128, ks), o_desc, j > 1 || ks);
                     umma_commit(smem_u32(&ctrl->v_empty));
                     umma_commit(smem_u32(&ctrl->pv_done));
                 }
@@ -541,67 +559,92 @@ __global__ __launch_bounds__(TC_THREADS, 2) void attn_tc_kernel(const __grid_con
         }
         __syncwarp();
     } else {
-        // ---- softmax: thread = row
-        for (int i = 0; i < D / 8; i++) {
+        // ---- softmax: two threads for a row, each half of the keys
+        for (int i = 0; i < D / 16; i++) {
             const int x = i * TC_SOFTMAX + tid, qr = x / (D / 8), c = x % (D / 8);
             const bool ok = qr < rows;
-            const int qy = tile * TC_ROWS + (ok ? qr : 0);
-            const int64_t off = (int64_t)(sq.row0 + query0 + qy / G) * a.q_token + (int64_t)(h * G + qy % G) * a.q_head;
+            const int qy = tr.row0 + (ok ? qr : 0);
+            const int64_t off = (int64_t)(sq.row0 + qy / G) * a.q_token + (int64_t)(h * G + qy % G) * a.q_head;
             cp_async16(q_tile + panel_off(128, qr, c), static_cast<const T *>(a.d_q) + off + c * 8, ok);
         }
         cp_commit();
+        const int r = tid & 127, half = warp >> 2, quad = warp & 3;
+        const int y = tr.row0 + min(r, rows - 1);
+        const int limit = attn_limit(a, sq, sq.pos0 + y / G);
+        const uint32_t my_bit = a.n_select ? 1u << (y / G / a.query_block - tr.qb0) : 1u;
+        const uint32_t all_bits = tr.n_qb == 32 ? ~0u : (1u << tr.n_qb) - 1;
+        const float scale2 = a.scale * LOG2E;
+        const uint32_t lane_s = tmem + ((uint32_t)(quad * 32) << 16) + half * TC_HALF;
+        const uint32_t lane_o = tmem_o + ((uint32_t)(quad * 32) << 16) + half * (D / 2);
+        const uint32_t met = smem_u32(&ctrl->met[quad]);
         cp_wait<0>();
         fence_async_smem();
         mbar_arrive(smem_u32(&ctrl->q_full));
-        const uint32_t lane_base = tmem + ((uint32_t)(warp * 32) << 16), lane_o = tmem_o + ((uint32_t)(warp * 32) << 16);
-        const int r = tid;
-        const int y = tile * TC_ROWS + min(r, rows - 1);
-        const int limit = attn_limit(a, sq, sq.pos0 + query0 + y / G);
-        const float scale2 = a.scale * LOG2E;
         float m = -CUDART_INF_F, l = 0.f;
         bool fine = true;
         for (int j = 0; j < n_tiles; j++) {
+            // lanes 0..3: position and lists of this half's groups of 16 keys (far behind every limit: none there)
+            int group_pos = INT32_MAX / 2;
+            uint32_t group_bits = all_bits;
+            if (lane < TC_HALF / 16) {
+                const int key = j * TC_KEYS + half * TC_HALF + lane * 16, e = key >> log_block;
+                if (e < n_entries) {
+                    const int b = block_of(e);
+                    group_pos = b * a.block + (key & (a.block - 1));
+                    if (a.n_select) group_bits = bits[e];
+                    else if (ctrl->bad_page) {
+                        const int page = page_of(b);
+                        if (page < 0 || page >= a.n_pages) group_pos = INT32_MAX / 2;
+                    }
+                }
+            }
+            const bool masked = __any_sync(~0u, lane < TC_HALF / 16 && group_pos > limit_min - 16);
+            const bool partly = __any_sync(~0u, group_bits != all_bits);
             fine = __all_sync(~0u, ws.wait(smem_u32(&ctrl->s_full), j, 7));
             if (!fine) break;
             tc_fence_after();
-            uint32_t v[TC_KEYS];
-#pragma unroll
-            for (int c = 0; c < TC_KEYS / 32; c++) tmem_ld32(lane_base + c * 32, v + c * 32);
-            // positions of the tile's eight groups of 16 keys; all visible to all rows in most tiles
-            int group_pos = INT32_MAX / 2;
-            if (lane < TC_KEYS / 16) {
-                const int key = j * TC_KEYS + lane * 16, e = key >> log_block;
-                if (e < n_entries) group_pos = blk[e] + (key & (a.block - 1));
-            }
-            const bool masked = __any_sync(~0u, lane < TC_KEYS / 16 && group_pos > limit_min - 16);
+            uint32_t v[TC_HALF];
+            tmem_ld32(lane_s, v);
+            tmem_ld32(lane_s + 32, v + 32);
             tmem_wait_ld();
-            tmem_landed<TC_KEYS>(v);
+            tmem_landed<TC_HALF>(v);
             if (masked) {
 #pragma unroll
-                for (int g = 0; g < TC_KEYS / 16; g++) {
+                for (int g = 0; g < TC_HALF / 16; g++) {
                     const int n = limit - __shfl_sync(~0u, group_pos, g);
 #pragma unroll
                     for (int i = 0; i < 16; i++)
                         if (i >= n) v[g * 16 + i] = 0xff800000u;
                 }
             }
-            float t0 = __uint_as_float(v[0]), t1 = __uint_as_float(v[1]), t2 = __uint_as_float(v[2]), t3 = __uint_as_float(v[3]);
+            if (partly) {
 #pragma unroll
-            for (int i = 0; i < TC_KEYS; i += 8) {
+                for (int g = 0; g < TC_HALF / 16; g++) {
+                    if (!(__shfl_sync(~0u, group_bits, g) & my_bit))
+#pragma unroll
+                        for (int i = 0; i < 16; i++) v[g * 16 + i] = 0xff800000u;
+                }
+            }
+            float t0 = __uint_as_float(v[0]), t1 = __uint_as_float(v[1]);
+#pragma unroll
+            for (int i = 0; i < TC_HALF; i += 4) {
                 t0 = fmaxf(t0, fmaxf(__uint_as_float(v[i]), __uint_as_float(v[i + 1])));
                 t1 = fmaxf(t1, fmaxf(__uint_as_float(v[i + 2]), __uint_as_float(v[i + 3])));
-                t2 = fmaxf(t2, fmaxf(__uint_as_float(v[i + 4]), __uint_as_float(v[i + 5])));
-                t3 = fmaxf(t3, fmaxf(__uint_as_float(v[i + 6]), __uint_as_float(v[i + 7])));
             }
-            const float top = fmaxf(fmaxf(t0, t1), fmaxf(t2, t3)) * scale2;
+            float top = fmaxf(t0, t1);
+            ctrl->top[j & 1][half][r] = top;
+            mbar_arrive(met);
+            fine = __all_sync(~0u, ws.wait(met, j, 10));
+            if (!fine) break;
+            top = fmaxf(top, ctrl->top[j & 1][half ^ 1][r]) * scale2;
             const bool raise = top > m + 8.f || (m == -CUDART_INF_F && top > m);
             if (__any_sync(~0u, raise)) {
                 const float f = raise ? fast_exp2(m - top) : 1.f;
                 if (raise) { m = top; l *= f; }
-                // the products before this S are complete, O is at rest
+                // the products before this S are complete, O is at rest; each thread takes half of its columns
                 if (j) {
 #pragma unroll 1
-                    for (int c = 0; c < D / 16; c++) {
+                    for (int c = 0; c < D / 32; c++) {
                         uint32_t w[16];
                         tmem_ld16(lane_o + c * 16, w);
                         tmem_wait_ld();
@@ -616,7 +659,7 @@ __global__ __launch_bounds__(TC_THREADS, 2) void attn_tc_kernel(const __grid_con
             const float2 scale22 = make_float2(scale2, scale2), minus_m = make_float2(-m0, -m0);
             float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
-            for (int c = 0; c < TC_KEYS / 32; c++) {
+            for (int c = 0; c < TC_HALF / 32; c++) {
                 uint32_t w[16];
 #pragma unroll
                 for (int i = 0; i < 16; i++) {
@@ -625,7 +668,7 @@ __global__ __launch_bounds__(TC_THREADS, 2) void attn_tc_kernel(const __grid_con
                     sum = add2(sum, e);
                     w[i] = Pack<T>::two(e.x, e.y);
                 }
-                tmem_st16(lane_base + c * 16, w);           // over S, which is in registers
+                tmem_st16(lane_s + c * 16, w);              // over this thread's S, which is in registers
             }
             l += sum.x + sum.y;
             tmem_wait_st();
@@ -634,14 +677,22 @@ __global__ __launch_bounds__(TC_THREADS, 2) void attn_tc_kernel(const __grid_con
         }
         if (n_tiles && fine) fine = __all_sync(~0u, ws.wait(smem_u32(&ctrl->pv_done), n_tiles - 1, 9));
         tc_fence_after();
+        // the row's sum: both halves (in the same order for both threads)
+        if (n_tiles && fine) {
+            ctrl->top[n_tiles & 1][half][r] = l;
+            mbar_arrive(met);
+            fine = __all_sync(~0u, ws.wait(met, n_tiles, 11));
+            l = ctrl->top[n_tiles & 1][0][r] + ctrl->top[n_tiles & 1][1][r];
+        }
         const float inv = l == 0.f ? 0.f : 1.f / l;
         const float lse2 = l == 0.f ? -CUDART_INF_F : (m == -CUDART_INF_F ? 0.f : m) + log2f(l);
-        const int64_t row = sq.row0 + query0 + y / G;
+        const int64_t row = sq.row0 + y / G;
         const int head = h * G + y % G;
         const int64_t at = (row * a.heads + head) * p.n_split + split;
 #pragma unroll 1
-        for (int c = 0; c < D / 32; c++) {
+        for (int c = 0; c < D / 64; c++) {
             uint32_t v[32];
+            const int d0 = half * (D / 2) + c * 32;
             if (n_tiles) {
                 tmem_ld32(lane_o + c * 32, v);
                 tmem_wait_ld();
@@ -652,12 +703,12 @@ __global__ __launch_bounds__(TC_THREADS, 2) void attn_tc_kernel(const __grid_con
                 v[i] = !fine ? 0x7fc00000u : n_tiles ? __float_as_uint(__uint_as_float(v[i]) * inv) : 0u;
             if (r < rows) {
                 if (p.n_split == 1) {
-                    T *dst = static_cast<T *>(a.d_o) + row * a.o_token + head * a.o_head + c * 32;
-                    T *low = a.d_o_low ? static_cast<T *>(a.d_o_low) + (row * a.heads + head) * D + c * 32 : nullptr;
+                    T *dst = static_cast<T *>(a.d_o) + row * a.o_token + head * a.o_head + d0;
+                    T *low = a.d_o_low ? static_cast<T *>(a.d_o_low) + (row * a.heads + head) * D + d0 : nullptr;
 #pragma unroll
                     for (int i = 0; i < 4; i++) store8<T>(dst + 8 * i, low ? low + 8 * i : nullptr, reinterpret_cast<float *>(v) + 8 * i);
                 } else {
-                    float4 *dst = reinterpret_cast<float4 *>(part_o + at * D + c * 32);
+                    float4 *dst = reinterpret_cast<float4 *>(part_o + at * D + d0);
 #pragma unroll
                     for (int i = 0; i < 8; i++)
                         dst[i] = make_float4(__uint_as_float(v[4 * i]), __uint_as_float(v[4 * i + 1]),
@@ -665,7 +716,7 @@ __global__ __launch_bounds__(TC_THREADS, 2) void attn_tc_kernel(const __grid_con
                 }
             }
         }
-        if (r < rows) {
+        if (r < rows && half == 0) {
             if (p.n_split > 1) part_lse[at] = fine ? lse2 : CUDART_NAN_F;
             else if (a.d_lse) a.d_lse[row * a.heads + head] = fine ? lse2 * LN2 : CUDART_NAN_F;
         }
@@ -673,7 +724,7 @@ __global__ __launch_bounds__(TC_THREADS, 2) void attn_tc_kernel(const __grid_con
         tc_fence_before();
     }
     __syncthreads();
-    if (warp == 4) {
+    if (warp == 8) {
         if (ctrl->abort_flag) drain_products();
         __syncwarp();
         tc_fence_after();
@@ -791,32 +842,35 @@ static int64_t longest_list(const spamm_attn &a)
     return a.n_select ? min(a.n_select, attn_max_blocks(a)) : attn_max_blocks(a);
 }
 
-// Rows that share keys: the queries of a query block times the heads of a key head.  From MIN_TC_ROWS on they go to the
-// kernel with tiles of 128 rows.
+// From 48 rows of a sequence and key head on, tiles of 128 rows are used; below (decoding), tiles of 16.
 constexpr int MIN_TC_ROWS = 48;
-static bool use_tc(const spamm_attn &a)
-{
-    const int64_t bq = a.n_select ? min(a.query_block, a.max_q) : a.max_q;
-    return bq * (a.heads / a.kv_heads) >= MIN_TC_ROWS;
-}
+static bool use_tc(const spamm_attn &a) { return (int64_t)a.max_q * (a.heads / a.kv_heads) >= MIN_TC_ROWS; }
 
 static RowsPlan rows_plan(const spamm_attn &a)
 {
     RowsPlan p;
     const int G = a.heads / a.kv_heads;
     const bool tc = use_tc(a);
-    const int tile_rows = tc ? TC_ROWS : 16;
-    p.bq = a.n_select ? min(a.query_block, a.max_q) : a.max_q;
-    p.nqb = ceil_div(a.max_q, p.bq);
-    p.tiles = (int)(((int64_t)p.bq * G + tile_rows - 1) / tile_rows);
-    const int64_t blocks = max((int64_t)1, longest_list(a));
+    if (tc) {
+        p.bq = 0;
+        p.nqb = 1;
+        p.tiles = attn_tiles(a);
+    } else {
+        p.bq = a.n_select ? min(a.query_block, a.max_q) : a.max_q;
+        p.nqb = ceil_div(a.max_q, p.bq);
+        p.tiles = (int)(((int64_t)p.bq * G + 15) / 16);
+    }
+    // tiles of 128 rows cut the sequence's blocks into ranges (they look through the lists for those in theirs), tiles of
+    // 16 rows the list
+    const int64_t blocks = max((int64_t)1, tc ? (int64_t)attn_max_blocks(a) : longest_list(a));
+    const int64_t most = !tc ? SPAMM_ATTN_MAX_SELECT : a.n_select ? UNION_BLOCKS : blocks;
     const int64_t units = (int64_t)a.batch * a.kv_heads * p.nqb * p.tiles;
-    // enough blocks of threads to fill 148 SMs twice over, ranges of 256 keys at the least
-    int64_t want = ((tc ? 1200 : 600) + units - 1) / units;
+    // enough blocks of threads to fill 148 SMs several times over, ranges of 1024 (256) keys at the least
+    int64_t want = (tc ? a.n_select ? 148 : 1200 : 600) / units + 1;
     want = max((int64_t)1, min(want, (blocks * a.block + (tc ? 1023 : 255)) / (tc ? 1024 : 256)));
-    int64_t per = min((int64_t)SPAMM_ATTN_MAX_SELECT, (blocks + want - 1) / want);
+    int64_t per = min(most, (blocks + want - 1) / want);
     p.n_split = (int)((blocks + per - 1) / per);
-    p.max_entries = (int)per;
+    p.max_entries = (int)(tc && a.n_select ? min(per, (int64_t)attn_tile_lists(a) * a.n_select) : per);
     p.split_keys = (int)(per * a.block);
     return p;
 }
@@ -837,7 +891,7 @@ static int forward_launch(const spamm_attn &a, float *scratch, cudaStream_t stre
     float *part_o = scratch;
     float *part_lse = scratch + (size_t)a.tokens * a.heads * p.n_split * D;
     if (use_tc(a)) {
-        const size_t smem = 1024 + 3 * TC_ROWS * D * 2 + sizeof(TcCtrl) + 8 * (size_t)p.max_entries + 4 * (size_t)max(a.n_select, p.max_entries);
+        const size_t smem = 3 * TC_ROWS * D * 2 + sizeof(TcCtrl) + (a.n_select ? 6 * (size_t)p.max_entries : 0);
         int st = attn_set_smem((const void *)attn_tc_kernel<T, D>, smem);
         if (st) return st;
         RowMap k_map, v_map;

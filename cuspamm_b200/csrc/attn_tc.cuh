@@ -102,8 +102,6 @@ __device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity)
                  : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
     return ok != 0;
 }
-// What this thread's ordinary stores (cp.async, st.shared) left in shared memory becomes visible to tcgen05.mma.
-__device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
 // A tensor map over rows of q, k, v or do.  Packed: boxes of box_tokens x box_heads rows x 64 values, coordinates (value,
 // head, token) or, swapped, (value, token, head).  Pages: boxes of box_tokens keys x 64 values, coordinates (value, 0,
@@ -123,6 +121,101 @@ __device__ __forceinline__ void tma_box(uint32_t dst, const CUtensorMap *map, in
     asm volatile("cp.async.bulk.tensor.3d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
                  "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar)
                  : "memory");
+}
+
+// What this thread's ordinary stores (cp.async, st.shared) left in shared memory becomes visible to tcgen05.mma.
+__device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+// ---- tiles of rows that span several query blocks
+//
+// A tile of 128 rows (queries x heads of a key head) reads the union of its query blocks' lists, at most 32 lists to a
+// tile; a bit for each of them says which rows a block of keys counts for.  Neighbouring queries share most of their blocks,
+// and where they do not, the union is still never more to copy than the lists one by one.
+constexpr int UNION_LISTS = 32;
+constexpr int UNION_BLOCKS = 8192;           // blocks of keys that a tile's union is built over at a time
+
+struct TileRows {
+    int rows;                 // of the tile
+    int row0;                 // first of the sequence's rows (query * G + head)
+    int first, last;          // its first and last query
+    int qb0, n_qb;            // its query blocks
+};
+__host__ __device__ inline int attn_tile_rows(const spamm_attn &a)
+{
+    if (!a.n_select) return 128;
+    const int64_t most = (int64_t)UNION_LISTS * a.query_block * (a.heads / a.kv_heads);
+    return most < 128 ? (int)most : 128;
+}
+__host__ __device__ inline int attn_tiles(const spamm_attn &a)
+{
+    const int rows = attn_tile_rows(a);
+    return (int)(((int64_t)a.max_q * (a.heads / a.kv_heads) + rows - 1) / rows);
+}
+// Lists that meet in a tile, at most.
+inline int attn_tile_lists(const spamm_attn &a)
+{
+    const int64_t per = (int64_t)a.query_block * (a.heads / a.kv_heads);
+    const int64_t n = attn_tile_rows(a) % per == 0 || per % attn_tile_rows(a) == 0 ? (attn_tile_rows(a) + per - 1) / per
+                                                                                    : (attn_tile_rows(a) + per - 1) / per + 1;
+    return (int)(n < UNION_LISTS ? n : UNION_LISTS);
+}
+// False when the tile has no rows.
+__device__ __forceinline__ bool attn_tile(const spamm_attn &a, const Seq &sq, int tile, TileRows *t)
+{
+    const int G = a.heads / a.kv_heads, per_tile = attn_tile_rows(a);
+    const int64_t all = (int64_t)sq.nq * G, row0 = (int64_t)tile * per_tile;
+    if (row0 >= all) return false;
+    t->rows = (int)min((int64_t)per_tile, all - row0);
+    t->row0 = (int)row0;
+    t->first = (int)(row0 / G);
+    t->last = (int)((row0 + t->rows - 1) / G);
+    t->qb0 = a.n_select ? t->first / a.query_block : 0;
+    t->n_qb = a.n_select ? t->last / a.query_block - t->qb0 + 1 : 1;
+    return true;
+}
+// The union of the tile's lists within the blocks [b0, b1): idx[e] = block - b0, ascending, bits[e] = the lists that have
+// it.  `marks`: room for b1 - b0 words that nothing else uses until the return.  All threads call; `count` is shared.
+// (Room of idx and bits: the sum of the lists' lengths, or b1 - b0.)
+template <int THREADS>
+__device__ __forceinline__ int attn_union(const spamm_attn &a, const Seq &sq, int s, int h, const TileRows &t, int b0, int b1,
+                                          uint32_t *marks, uint16_t *idx, uint32_t *bits, int *count)
+{
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n = b1 - b0;
+    const int nqb = ceil_div(a.max_q, a.query_block);
+    for (int i = tid; i < n; i += THREADS) marks[i] = 0;
+    __syncthreads();
+    for (int q = warp; q < t.n_qb; q += THREADS / 32) {
+        const int qb = t.qb0 + q;
+        const int last = (int)min((int64_t)(qb + 1) * a.query_block, (int64_t)sq.nq) - 1;
+        attn_for_list(a, s, qb, nqb, h, ceil_div(attn_limit(a, sq, sq.pos0 + last), a.block), lane, [&](int v, int) {
+            if (v >= b0 && v < b1) atomicOr(marks + v - b0, 1u << q);
+        });
+    }
+    __syncthreads();
+    if (warp == 0) {
+        int found = 0;
+        for (int i0 = 0; i0 < n; i0 += 32) {
+            uint32_t m = i0 + lane < n ? marks[i0 + lane] : 0;
+            if (m && a.n_pages) {
+                const int page = a.d_table[(int64_t)s * a.table_stride + b0 + i0 + lane];
+                if (page < 0 || page >= a.n_pages) {
+                    m = 0;
+                    *a.d_status = SPAMM_ERR_INVALID;
+                }
+            }
+            const unsigned there = __ballot_sync(~0u, m != 0);
+            const int at = found + __popc(there & ((1u << lane) - 1));
+            if (m) {
+                idx[at] = (uint16_t)(i0 + lane);
+                bits[at] = m;
+            }
+            found += __popc(there);
+        }
+        if (lane == 0) *count = found;
+    }
+    fence_async_smem();                      // tensor copies may now write where the marks were
+    __syncthreads();
+    return *count;
 }
 
 // Two float operations in one instruction.
