@@ -6,6 +6,7 @@
 // now and then.  Sums and products are therefore taken in double: bf16 and half values add up without any rounding
 // there (short of wildly different magnitudes), and the double rate of this GPU is half its float rate.  Only the key
 // sums, which a cache keeps, are rounded to float.
+#include <type_traits>
 #include "attn.cuh"
 
 namespace spamm {
@@ -15,6 +16,60 @@ __device__ __forceinline__ int64_t sums_row(const spamm_attn &a, const Seq &sq, 
 {
     return (int64_t)sq.row0 / a.block + s + b;
 }
+
+// Eight double sums of values that come 16 bytes at a time.  The conversion to double is slow (8 values a clock and SM), so
+// the bits of the float are put where the double has them instead: read as a double they stand for the value times 2^-896,
+// zeros and subnormals included, and sums of them are scaled back once at the end.  Infinities and NaN alone would be read as
+// finite; `odd` notices them and the sums are then taken again with conversions.
+template <typename T> struct Sum8 {
+    double y[8];
+    uint32_t odd;
+    __device__ __forceinline__ Sum8() : odd(0)
+    {
+#pragma unroll
+        for (int i = 0; i < 8; i++) y[i] = 0.0;
+    }
+    static __device__ __forceinline__ double moved(float f)
+    {
+        const uint32_t x = __float_as_uint(f);
+        return __hiloint2double((int)((x & 0x80000000u) | ((x & 0x7fffffffu) >> 3)), 0);   // the low 13 bits are zero
+    }
+    __device__ __forceinline__ void add(uint4 x)
+    {
+        const uint32_t xs[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            // an exponent of all ones carries into the sign's place
+            odd |= (xs[i] & 0x7fff7fffu) + (std::is_same<T, __nv_bfloat16>::value ? 0x00800080u : 0x04000400u);
+            const float2 f = Pack<T>::to2(xs[i]);
+            y[2 * i] += moved(f.x);
+            y[2 * i + 1] += moved(f.y);
+        }
+    }
+    __device__ __forceinline__ void add_slowly(uint4 x)
+    {
+        const uint32_t xs[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const float2 f = Pack<T>::to2(xs[i]);
+            y[2 * i] += (double)f.x;
+            y[2 * i + 1] += (double)f.y;
+        }
+    }
+    // Sums what `at(r)` points to for r = first, first + step, ... below n.
+    template <typename At> __device__ __forceinline__ void all(int first, int step, int n, At at)
+    {
+#pragma unroll 8
+        for (int r = first; r < n; r += step) add(*reinterpret_cast<const uint4 *>(at(r)));
+#pragma unroll
+        for (int i = 0; i < 8; i++) y[i] *= 0x1p896;
+        if (odd & 0x80008000u) {
+#pragma unroll
+            for (int i = 0; i < 8; i++) y[i] = 0.0;
+            for (int r = first; r < n; r += step) add_slowly(*reinterpret_cast<const uint4 *>(at(r)));
+        }
+    }
+};
 
 template <typename T, int D>
 __global__ __launch_bounds__(256) void attn_key_sums_kernel(const __grid_constant__ spamm_attn a, int nkb, float *key_sums)
@@ -30,22 +85,11 @@ __global__ __launch_bounds__(256) void attn_key_sums_kernel(const __grid_constan
         const int cols = min(256, a.kv_heads * V - c0), groups = 256 / cols;
         const int col = tid % cols, g = tid / cols, h = (c0 + col) / V, c = (c0 + col) % V;
         const T *src = static_cast<const T *>(a.d_k) + (int64_t)(sq.row0 + b * a.block) * a.k_token + h * a.k_head + c * 8;
-        double y[8] = {};
-        if (g < groups)
-#pragma unroll 4
-            for (int r = g; r < held; r += groups) {
-                const uint4 x = *reinterpret_cast<const uint4 *>(src + r * a.k_token);
-                const uint32_t xs[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const float2 f = Pack<T>::to2(xs[i]);
-                    y[2 * i] += (double)f.x;
-                    y[2 * i + 1] += (double)f.y;
-                }
-            }
+        Sum8<T> sum;
+        if (g < groups) sum.all(g, groups, held, [&](int r) { return src + r * a.k_token; });
         __syncthreads();
 #pragma unroll
-        for (int i = 0; i < 8; i++) sums[tid * 8 + i] = y[i];
+        for (int i = 0; i < 8; i++) sums[tid * 8 + i] = sum.y[i];
         __syncthreads();
         for (int i = tid; i < cols * 8; i += 256) {
             double z = 0.0;
@@ -63,70 +107,326 @@ __device__ __forceinline__ unsigned long long order_key(double x)
     return b >> 63 ? ~b : b | (1ull << 63);
 }
 
-// One query block and key head per block of threads.
+// What a query block may and must read: blocks [0, n) are candidates, those below n_first and in (lo, hi] are taken.
+struct Reach { int n, lo, hi; };
+__device__ __forceinline__ Reach reach_of(const spamm_attn &a, const Seq &sq, int64_t q0, int n_tok, int n_local)
+{
+    Reach r{0, 0, -1};
+    if (n_tok <= 0) return r;
+    const int first = sq.pos0 + (int)q0, last = first + n_tok - 1;
+    r.n = ceil_div(attn_limit(a, sq, last), a.block);
+    if (n_local > 0) {
+        r.lo = (first >= 0 ? first / a.block : -1) - n_local;
+        r.hi = last >= 0 ? last / a.block : -1;
+    }
+    return r;
+}
+__device__ __forceinline__ bool taken(const Reach &r, int b, int n_first) { return b < n_first || (b > r.lo && b <= r.hi); }
+
+// Row of the key sums of block b; -1 for a page that does not exist.
+__device__ __forceinline__ int64_t key_sum_row(const spamm_attn &a, const Seq &sq, int s, int b)
+{
+    if (!a.n_pages) return sums_row(a, sq, s, b);
+    const int page = a.d_table[(int64_t)s * a.table_stride + b];
+    if (page < 0 || page >= a.n_pages) {
+        *a.d_status = SPAMM_ERR_INVALID;
+        return -1;
+    }
+    return page;
+}
+
+// The sum of a query block's queries over the heads of key head h, by all threads: qsum[D].  part: room for THREADS * 8.
+template <typename T, int D, int THREADS>
+static __device__ void query_sum(const spamm_attn &a, const Seq &sq, int64_t q0, int n_tok, int h, double *part, double *qsum)
+{
+    constexpr int V = D / 8, GROUPS = THREADS / V;
+    const int tid = threadIdx.x, c = tid % V, g = tid / V, G = a.heads / a.kv_heads;
+    const T *src = static_cast<const T *>(a.d_q) + (sq.row0 + q0) * a.q_token + (int64_t)h * G * a.q_head + c * 8;
+    Sum8<T> sum;
+    sum.all(g, GROUPS, n_tok * G, [&](int r) { return src + r / G * a.q_token + r % G * a.q_head; });
+#pragma unroll
+    for (int i = 0; i < 8; i++) part[(g * V + c) * 8 + i] = sum.y[i];
+    __syncthreads();
+    for (int d = tid; d < D; d += THREADS) {
+        double z = 0.0;
+        for (int k = 0; k < GROUPS; k++) z += part[k * D + d];
+        qsum[d] = z;
+    }
+    __syncthreads();
+}
+
+// The bits in which ordered keys can differ: all below the first one in which `low` and `high` do.
+__device__ __forceinline__ int differing_bits(unsigned long long low, unsigned long long high) { return 64 - __clzll(low ^ high); }
+
+// One warp writes the keys above the threshold, and of its equals the first `left`, as an ascending list.
+static __device__ __forceinline__ void write_list(const unsigned long long *keys, int n, unsigned long long threshold, int left, int n_select,
+                                  int32_t *out, int lane)
+{
+    int count = 0;
+    for (int b0 = 0; b0 < n; b0 += 32) {
+        const int b = b0 + lane;
+        const unsigned long long key = b < n ? keys[b] : 0;
+        const unsigned eq = __ballot_sync(~0u, key == threshold && key != 0);
+        const bool tie = key == threshold && key != 0 && __popc(eq & ((1u << lane) - 1)) < left;
+        const unsigned m = __ballot_sync(~0u, key > threshold || tie);
+        const int at = count + __popc(m & ((1u << lane) - 1));
+        if ((m >> lane & 1) && at < n_select) out[at] = b;
+        count += __popc(m);
+        left -= min(left, __popc(eq));
+    }
+    for (int i = min(count, n_select) + lane; i < n_select; i += 32) out[i] = -1;
+}
+
+// Writes the n_select largest of keys[0, n) in shared memory (0: no candidate) as an ascending list, by all threads.  The
+// n_select-th largest key is found bit by bit; the search ends as soon as exactly n_select keys are at or above it.
+template <int THREADS>
+static __device__ void write_largest(const unsigned long long *keys, int n, int n_select, int32_t *out)
+{
+    __shared__ int counts[66];
+    __shared__ unsigned long long ends[2];
+    const int tid = threadIdx.x, lane = tid & 31;
+    if (tid < 66) counts[tid] = 0;
+    if (tid == 0) { ends[0] = ~0ull; ends[1] = 0; }
+    __syncthreads();
+    auto count = [&](int slot, auto pred) {
+        int c = 0;
+        for (int b = tid; b < n; b += THREADS) c += pred(keys[b]);
+        c = __reduce_add_sync(~0u, c);
+        if (lane == 0 && c) atomicAdd(&counts[slot], c);
+        __syncthreads();
+        return counts[slot];
+    };
+    unsigned long long threshold = 1;
+    int left = INT32_MAX;
+    if (n > n_select) {
+        // blocks that are taken in any case have the key ~0 and are left out of the range of the search
+        unsigned long long low = ~0ull, high = 0;
+        for (int b = tid; b < n; b += THREADS) {
+            low = min(low, keys[b]);
+            if (keys[b] != ~0ull) high = max(high, keys[b]);
+        }
+#pragma unroll
+        for (int d = 16; d; d >>= 1) {
+            low = min(low, __shfl_xor_sync(~0u, low, d));
+            high = max(high, __shfl_xor_sync(~0u, high, d));
+        }
+        if (lane == 0) {
+            atomicMin(&ends[0], low);
+            atomicMax(&ends[1], high);
+        }
+        __syncthreads();
+        const int bits = differing_bits(ends[0], ends[1]);
+        threshold = bits == 64 ? 0 : ends[1] >> bits << bits;
+        bool exact = false;
+        for (int bit = bits - 1; bit >= 0 && !exact; bit--) {
+            const unsigned long long want = threshold | (1ull << bit);
+            const int c = count(bit, [&](unsigned long long k) { return k >= want; });
+            if (c >= n_select) threshold = want;
+            exact = c == n_select;
+        }
+        if (!exact) left = n_select - count(65, [&](unsigned long long k) { return k > threshold; });
+    }
+    if (tid < 32) write_list(keys, n, threshold, left, n_select, out, lane);
+}
+
+// ---- QT query blocks and one key head per block of threads, scores as double products on the tensor cores (m8n8k4).  Many
+// query blocks: all blocks of keys, the lists picked from shared memory.  Few of them (decoding; SPREAD): SPREAD_BLOCKS
+// blocks of keys, so that the reading of the key sums spreads over the GPU, and the ordered scores to global memory.
+constexpr int SPREAD_BLOCKS = 64;
+
+__device__ __forceinline__ void mma_double(double *c, double a, double b)
+{
+    asm volatile("mma.sync.aligned.m8n8k4.row.col.f64.f64.f64.f64 {%0, %1}, {%2}, {%3}, {%0, %1};"
+                 : "+d"(c[0]), "+d"(c[1]) : "d"(a), "d"(b));
+}
+
+template <typename T, int D, int QT, bool SPREAD>
+__global__ __launch_bounds__(256) void attn_select_tile_kernel(const __grid_constant__ spamm_attn a, int nqb, int nkb, int n_first,
+                                                               int n_local, const float *key_sums, int32_t *lists,
+                                                               unsigned long long *spread_keys)
+{
+    constexpr int V = D / 8, LD = D + 4;                    // rows 4 doubles apart from a multiple of the banks
+    constexpr int MG = QT / 8, NG = 8 / MG, KT = QT == 8 ? 64 : 32, NT = KT / NG / 8;
+    extern __shared__ __align__(16) uint8_t smem[];
+    double *qs = reinterpret_cast<double *>(smem);          // [QT][LD]
+    double *ks = qs + QT * LD;                              // [KT][LD]
+    unsigned long long *keys = reinterpret_cast<unsigned long long *>(ks + KT * LD);    // [QT][nkb]
+    __shared__ Reach reach[QT];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int q_tiles = (nqb + QT - 1) / QT;
+    unsigned idx = blockIdx.x;
+    const int spans = SPREAD ? (nkb + SPREAD_BLOCKS - 1) / SPREAD_BLOCKS : 1;
+    const int span = idx % spans; idx /= spans;
+    const int qt = q_tiles - 1 - idx % q_tiles; idx /= q_tiles;
+    const int h = idx % a.kv_heads, s = idx / a.kv_heads;
+    const int G = a.heads / a.kv_heads;
+    const Seq sq = attn_seq(a, s);
+    if (SPREAD) {
+        // the last query block there is reaches furthest
+        const int last_qb = min((qt + 1) * QT, ceil_div(sq.nq, a.query_block)) - 1;
+        const int64_t q0 = (int64_t)last_qb * a.query_block;
+        if (last_qb < qt * QT ||
+            span * SPREAD_BLOCKS >= reach_of(a, sq, q0, (int)min((int64_t)a.query_block, sq.nq - q0), 0).n) return;
+    }
+    if (tid < QT) {
+        const int64_t q0 = (int64_t)(qt * QT + tid) * a.query_block;
+        reach[tid] = reach_of(a, sq, q0, qt * QT + tid < nqb ? (int)min((int64_t)a.query_block, sq.nq - q0) : 0, n_local);
+    }
+    // sums of the queries: a group of V threads for a query block, or the block's rows dealt out to several groups
+    {
+        constexpr int GROUPS = 256 / V, PER = GROUPS > QT ? GROUPS / QT : 1;
+        const int c = tid % V, g = tid / V;
+        for (int i = g / PER; i < QT; i += GROUPS / PER) {
+            const int64_t q0 = (int64_t)(qt * QT + i) * a.query_block;
+            const int n_tok = qt * QT + i < nqb ? (int)min((int64_t)a.query_block, sq.nq - q0) : 0;
+            const T *src = static_cast<const T *>(a.d_q) + (sq.row0 + q0) * a.q_token + (int64_t)h * G * a.q_head + c * 8;
+            int tok = 0, head = g % PER;
+            while (head >= G) { head -= G; tok++; }
+            const int tok0 = tok, head0 = head;
+            Sum8<T> sum;
+            sum.all(g % PER, PER, n_tok * G, [&](int r) {
+                if (r == g % PER) { tok = tok0; head = head0; }
+                const T *p = src + tok * a.q_token + head * a.q_head;
+                head += PER;
+                while (head >= G) { head -= G; tok++; }
+                return p;
+            });
+            // the PER partial sums lie in neighbouring lanes of one warp
+#pragma unroll
+            for (int d = V; d < PER * V; d <<= 1)
+#pragma unroll
+                for (int k = 0; k < 8; k++) sum.y[k] += __shfl_xor_sync(~0u, sum.y[k], d);
+            if (g % PER == 0)
+#pragma unroll
+                for (int k = 0; k < 8; k++) qs[i * LD + c * 8 + k] = sum.y[k];
+        }
+    }
+    __syncthreads();
+    int n_most = 0;
+#pragma unroll 1
+    for (int i = 0; i < QT; i++) n_most = max(n_most, reach[i].n);
+    const int mg = warp % MG, ng = warp / MG;
+    const double per_key = 1.0 / (double)a.block;
+    const int b_end = SPREAD ? min(n_most, (span + 1) * SPREAD_BLOCKS) : n_most;
+    for (int b0 = SPREAD ? span * SPREAD_BLOCKS : 0; b0 < b_end; b0 += KT) {
+        for (int i = tid; i < KT * (D / 4); i += 256) {
+            const int r = i / (D / 4), c = i % (D / 4) * 4, b = b0 + r;
+            float4 k = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (b < n_most) {
+                const int64_t row = key_sum_row(a, sq, s, b);
+                if (row >= 0) k = *reinterpret_cast<const float4 *>(key_sums + (row * a.kv_heads + h) * D + c);
+            }
+            double *dst = ks + r * LD + c;
+            *reinterpret_cast<double2 *>(dst) = make_double2((double)k.x, (double)k.y);
+            *reinterpret_cast<double2 *>(dst + 2) = make_double2((double)k.z, (double)k.w);
+        }
+        __syncthreads();
+        double acc[NT][2] = {};
+        const double *qa = qs + (mg * 8 + (lane >> 2)) * LD + (lane & 3);
+        const double *kb = ks + (ng * NT * 8 + (lane >> 2)) * LD + (lane & 3);
+#pragma unroll 8
+        for (int k = 0; k < D; k += 4) {
+            const double x = qa[k];
+#pragma unroll
+            for (int n = 0; n < NT; n++) mma_double(acc[n], x, kb[n * 8 * LD + k]);
+        }
+        const int i = mg * 8 + (lane >> 2);
+        const Reach rr = reach[i];
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                const int b = b0 + (ng * NT + n) * 8 + (lane & 3) * 2 + e;
+                if (b >= nkb || (SPREAD && qt * QT + i >= nqb)) continue;
+                unsigned long long key = 0;
+                if (b < rr.n && (!a.n_pages || key_sum_row(a, sq, s, b) >= 0)) {
+                    // every block but the last is full, and 1 / block a power of two
+                    const int held = sq.nk - b * a.block;
+                    key = taken(rr, b, n_first) ? ~0ull : order_key(held < a.block ? acc[n][e] / (double)held : acc[n][e] * per_key);
+                }
+                if (SPREAD) spread_keys[(((int64_t)s * nqb + qt * QT + i) * a.kv_heads + h) * nkb + b] = key;
+                else keys[i * nkb + b] = key;
+            }
+        __syncthreads();
+    }
+    // a warp for a list, as write_largest does it
+    if constexpr (!SPREAD) for (int i = warp; i < QT; i += 8) {
+        const int qb = qt * QT + i;
+        if (qb >= nqb) break;
+        int32_t *out = lists + (((int64_t)s * nqb + qb) * a.kv_heads + h) * a.n_select;
+        const unsigned long long *mine = keys + i * nkb;
+        const int n = reach[i].n;
+        unsigned long long threshold = 1;
+        int left = INT32_MAX;
+        if (n > a.n_select) {
+            unsigned long long low = ~0ull, high = 0;
+            for (int b = lane; b < n; b += 32) {
+                low = min(low, mine[b]);
+                if (mine[b] != ~0ull) high = max(high, mine[b]);
+            }
+#pragma unroll
+            for (int d = 16; d; d >>= 1) {
+                low = min(low, __shfl_xor_sync(~0u, low, d));
+                high = max(high, __shfl_xor_sync(~0u, high, d));
+            }
+            const int bits = differing_bits(low, high);
+            threshold = bits == 64 ? 0 : high >> bits << bits;
+            bool exact = false;
+            for (int bit = bits - 1; bit >= 0 && !exact; bit--) {
+                const unsigned long long want = threshold | (1ull << bit);
+                int count = 0;
+                for (int b = lane; b < n; b += 32) count += mine[b] >= want;
+                count = __reduce_add_sync(~0u, count);
+                if (count >= a.n_select) threshold = want;
+                exact = count == a.n_select;
+            }
+            if (!exact) {
+                int above = 0;
+                for (int b = lane; b < n; b += 32) above += mine[b] > threshold;
+                left = a.n_select - __reduce_add_sync(~0u, above);
+            }
+        }
+        write_list(mine, n, threshold, left, a.n_select, out, lane);
+    }
+}
+
+template <int THREADS>
+__global__ __launch_bounds__(THREADS) void attn_largest_kernel(const __grid_constant__ spamm_attn a, int nqb, int nkb,
+                                                               const unsigned long long *keys, int32_t *lists)
+{
+    extern __shared__ __align__(16) unsigned long long copy[];
+    const int s = blockIdx.x / a.kv_heads / nqb, qb = blockIdx.x / a.kv_heads % nqb;
+    const Seq sq = attn_seq(a, s);
+    const int64_t q0 = (int64_t)qb * a.query_block;
+    const Reach reach = reach_of(a, sq, q0, (int)min((int64_t)a.query_block, sq.nq - q0), 0);
+    for (int i = threadIdx.x; i < reach.n; i += THREADS) copy[i] = keys[(int64_t)blockIdx.x * nkb + i];
+    write_largest<THREADS>(copy, reach.n, a.n_select, lists + (int64_t)blockIdx.x * a.n_select);
+}
+
+// ---- many query blocks of sequences too long for that: one list per block of threads
 template <typename T, int D>
 __global__ __launch_bounds__(128) void attn_select_kernel(const __grid_constant__ spamm_attn a, int nqb, int n_first, int n_local,
                                                           const float *key_sums, int32_t *lists)
 {
     extern __shared__ __align__(16) uint8_t smem[];
-    constexpr int V = D / 8;
     unsigned long long *keys = reinterpret_cast<unsigned long long *>(smem);
     __shared__ double part[128 * 8];
     __shared__ double qsum[D];
-    __shared__ int hist[256];
-    __shared__ unsigned long long s_prefix;
-    __shared__ int s_left;
-    const int tid = threadIdx.x, lane = tid & 31;
+    const int tid = threadIdx.x;
     unsigned idx = blockIdx.x;
     const int h = idx % a.kv_heads; idx /= a.kv_heads;
-    const int qb = idx % nqb;
-    const int s = idx / nqb;
-    const int G = a.heads / a.kv_heads;
+    const int qb = idx % nqb, s = idx / nqb;
     const Seq sq = attn_seq(a, s);
-    int32_t *out = lists + (((int64_t)s * nqb + qb) * a.kv_heads + h) * a.n_select;
     const int64_t q0 = (int64_t)qb * a.query_block;
     const int n_tok = (int)min((int64_t)a.query_block, sq.nq - q0);
-    const int first = sq.pos0 + (int)min(q0, (int64_t)sq.nq), last = first + max(n_tok, 0) - 1;
-    const int n_blocks = n_tok > 0 ? ceil_div(attn_limit(a, sq, last), a.block) : 0;
-    if (n_blocks <= 0) {
-        for (int i = tid; i < a.n_select; i += 128) out[i] = -1;
-        return;
-    }
-    // sum of the queries
-    {
-        const int c = tid % V, g = tid / V;
-        double y[8] = {};
-        const T *src = static_cast<const T *>(a.d_q) + (sq.row0 + q0) * a.q_token + (int64_t)h * G * a.q_head + c * 8;
-        for (int r = g; r < n_tok * G; r += 128 / V) {
-            const uint4 x = *reinterpret_cast<const uint4 *>(src + r / G * a.q_token + r % G * a.q_head);
-            const uint32_t xs[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const float2 f = Pack<T>::to2(xs[i]);
-                y[2 * i] += (double)f.x;
-                y[2 * i + 1] += (double)f.y;
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < 8; i++) part[(g * V + c) * 8 + i] = y[i];
-    }
-    __syncthreads();
-    for (int d = tid; d < D; d += 128) {
-        double z = 0.0;
-        for (int g = 0; g < 128 / V; g++) z += part[g * D + d];
-        qsum[d] = z;
-    }
-    __syncthreads();
-    // scores as ordered integers
-    const int first_block = first >= 0 ? first / a.block : -1, last_block = last >= 0 ? last / a.block : -1;
-    for (int b = tid; b < n_blocks; b += 128) {
-        const bool forced = b < n_first || (b > first_block - n_local && b <= last_block && n_local > 0);
+    const Reach reach = reach_of(a, sq, q0, n_tok, n_local);
+    if (n_tok > 0) query_sum<T, D, 128>(a, sq, q0, n_tok, h, part, qsum);
+    for (int b = tid; b < reach.n; b += 128) {
         unsigned long long key = ~0ull;
-        const int64_t row = a.n_pages ? (int64_t)a.d_table[(int64_t)s * a.table_stride + b] : sums_row(a, sq, s, b);
-        if (a.n_pages && (row < 0 || row >= a.n_pages)) {
-            *a.d_status = SPAMM_ERR_INVALID;
+        const int64_t row = key_sum_row(a, sq, s, b);
+        if (row < 0) {
             key = 0;
-        } else if (!forced) {
+        } else if (!taken(reach, b, n_first)) {
             const float4 *ks = reinterpret_cast<const float4 *>(key_sums + (row * a.kv_heads + h) * D);
             double z = 0.0;
 #pragma unroll 8
@@ -141,59 +441,45 @@ __global__ __launch_bounds__(128) void attn_select_kernel(const __grid_constant_
         }
         keys[b] = key;
     }
-    if (tid == 0) { s_prefix = 0; s_left = a.n_select; }
-    __syncthreads();
-    // the n_select-th largest key, eight bits at a time; all candidates when there are no more than n_select blocks
-    unsigned long long mask = 0;
-    if (n_blocks > a.n_select) {
-        for (int shift = 56; shift >= 0; shift -= 8) {
-            for (int i = tid; i < 256; i += 128) hist[i] = 0;
-            __syncthreads();
-            const unsigned long long prefix = s_prefix;
-            for (int b = tid; b < n_blocks; b += 128)
-                if ((keys[b] & mask) == prefix) atomicAdd(&hist[(int)(keys[b] >> shift) & 255], 1);
-            __syncthreads();
-            if (tid < 32) {
-                // lane's eight bins from the top: where the running count reaches s_left
-                const int left = s_left;
-                int mine = 0;
-                for (int i = 0; i < 8; i++) mine += hist[255 - lane * 8 - i];
-                int run = mine;
-#pragma unroll
-                for (int d = 1; d < 32; d <<= 1) {
-                    const int u = __shfl_up_sync(~0u, run, d);
-                    if (lane >= d) run += u;
-                }
-                const int before = run - mine;
-                if (before < left && run >= left) {
-                    int rest = left - before, bin = 255 - lane * 8;
-                    while (hist[bin] < rest) rest -= hist[bin--];
-                    s_prefix = prefix | ((unsigned long long)bin << shift);
-                    s_left = rest;
-                }
-            }
-            mask |= 255ull << shift;
-            __syncthreads();
-        }
-    }
-    // keep what is above the threshold, and of its equals the first s_left
-    if (tid < 32) {
-        const unsigned long long threshold = s_prefix;
-        int left = n_blocks > a.n_select ? s_left : INT32_MAX, count = 0;
-        for (int b0 = 0; b0 < n_blocks; b0 += 32) {
-            const int b = b0 + lane;
-            const unsigned long long key = b < n_blocks ? keys[b] : 0;
-            const unsigned eq = __ballot_sync(~0u, key == threshold && key != 0);
-            const bool tie = key == threshold && key != 0 && __popc(eq & ((1u << lane) - 1)) < left;
-            const bool keep = key > threshold || tie;
-            const unsigned m = __ballot_sync(~0u, keep);
-            const int at = count + __popc(m & ((1u << lane) - 1));
-            if (keep && at < a.n_select) out[at] = b;
-            count += __popc(m);
-            left -= min(left, __popc(eq));
-        }
-        for (int i = min(count, a.n_select) + lane; i < a.n_select; i += 32) out[i] = -1;
-    }
+    write_largest<128>(keys, reach.n, a.n_select, lists + (((int64_t)s * nqb + qb) * a.kv_heads + h) * a.n_select);
+}
+
+// Which of the three: by how many lists there are to fill the GPU with, and whether the scores of a tile of query blocks
+// fit shared memory.
+enum SelectWay { SELECT_SPREAD, SELECT_TILE32, SELECT_TILE8, SELECT_ONE };
+static SelectWay select_way(const spamm_attn &a)
+{
+    const int64_t lists = (int64_t)a.batch * attn_query_blocks(a) * a.kv_heads, blocks = attn_max_blocks(a);
+    if (lists < 1184) return SELECT_SPREAD;
+    if (blocks <= 256 && lists >= 32 * 296) return SELECT_TILE32;
+    if (blocks <= 1024) return SELECT_TILE8;
+    return SELECT_ONE;
+}
+
+template <typename T, int D, int QT, bool SPREAD>
+static int select_tile_launch(const spamm_attn &a, int nqb, int nkb, int n_first, int n_local, const float *key_sums, int32_t *lists,
+                              unsigned long long *keys, cudaStream_t stream)
+{
+    const size_t smem = (size_t)(QT + (QT == 8 ? 64 : 32)) * (D + 4) * 8 + (SPREAD ? 0 : (size_t)QT * nkb * 8);
+    const int64_t grid = (int64_t)a.batch * a.kv_heads * ((nqb + QT - 1) / QT) * (SPREAD ? ceil_div(nkb, SPREAD_BLOCKS) : 1);
+    if (grid > INT32_MAX) return attn_too_large();
+    int st = attn_set_smem((const void *)attn_select_tile_kernel<T, D, QT, SPREAD>, smem);
+    if (st) return st;
+    attn_select_tile_kernel<T, D, QT, SPREAD><<<(unsigned)grid, 256, smem, stream>>>(a, nqb, nkb, n_first, n_local, key_sums, lists, keys);
+    return SPAMM_OK;
+}
+
+// No page table: nothing to list.
+static int clear_lists(const spamm_attn &a, int32_t *lists, cudaStream_t stream)
+{
+    SPAMM_CUDA_TRY(cudaMemsetAsync(lists, 0xff, (size_t)a.batch * attn_query_blocks(a) * a.kv_heads * a.n_select * 4, stream));
+    return SPAMM_OK;
+}
+
+static size_t key_sums_bytes(const spamm_attn &a)
+{
+    if (a.n_pages) return 0;
+    return (((size_t)a.tokens / a.block + a.batch + 1) * a.kv_heads * a.dim * sizeof(float) + 15) / 16 * 16;
 }
 
 template <typename T, int D>
@@ -203,14 +489,31 @@ static int select_launch(const spamm_attn &a, const float *key_sums, int n_first
     const int nkb = attn_max_blocks(a), nqb = attn_query_blocks(a);
     const int64_t grid = (int64_t)a.batch * nqb * a.kv_heads, sums_grid = (int64_t)a.batch * nkb;
     if (grid > INT32_MAX || sums_grid > INT32_MAX) return attn_too_large();
-    if (!a.n_pages) {
+    if (!a.n_pages && a.tokens) {
         attn_key_sums_kernel<T, D><<<(unsigned)sums_grid, 256, 0, stream>>>(a, nkb, scratch);
         key_sums = scratch;
     }
-    const size_t smem = (size_t)nkb * 8;
-    int st = attn_set_smem((const void *)attn_select_kernel<T, D>, smem);
+    int st = SPAMM_OK;
+    switch (select_way(a)) {
+    case SELECT_SPREAD: {
+        unsigned long long *keys = reinterpret_cast<unsigned long long *>(reinterpret_cast<uint8_t *>(scratch) + key_sums_bytes(a));
+        if (!nkb) return clear_lists(a, lists, stream);
+        st = select_tile_launch<T, D, 8, true>(a, nqb, nkb, n_first, n_local, key_sums, lists, keys, stream);
+        if (st) return st;
+        st = attn_set_smem((const void *)attn_largest_kernel<256>, (size_t)nkb * 8);
+        if (st) return st;
+        attn_largest_kernel<256><<<(unsigned)grid, 256, (size_t)nkb * 8, stream>>>(a, nqb, nkb, keys, lists);
+        break;
+    }
+    case SELECT_TILE32: st = select_tile_launch<T, D, 32, false>(a, nqb, nkb, n_first, n_local, key_sums, lists, nullptr, stream); break;
+    case SELECT_TILE8: st = select_tile_launch<T, D, 8, false>(a, nqb, nkb, n_first, n_local, key_sums, lists, nullptr, stream); break;
+    case SELECT_ONE:
+        st = attn_set_smem((const void *)attn_select_kernel<T, D>, (size_t)nkb * 8);
+        if (st) return st;
+        attn_select_kernel<T, D><<<(unsigned)grid, 128, (size_t)nkb * 8, stream>>>(a, nqb, n_first, n_local, key_sums, lists);
+        break;
+    }
     if (st) return st;
-    attn_select_kernel<T, D><<<(unsigned)grid, 128, smem, stream>>>(a, nqb, n_first, n_local, key_sums, lists);
     SPAMM_CUDA_TRY(cudaGetLastError());
     return SPAMM_OK;
 }
@@ -221,8 +524,11 @@ using namespace spamm;
 
 extern "C" size_t spamm_attn_select_scratch_bytes(const spamm_attn *a)
 {
-    if (attn_check(a, false) || a->n_pages || !a->batch || !a->max_q || !a->tokens) return 0;
-    return ((size_t)a->tokens / a->block + a->batch + 1) * a->kv_heads * a->dim * sizeof(float);
+    if (attn_check(a, false) || !a->batch || !a->max_q) return 0;
+    size_t n = a->tokens ? key_sums_bytes(*a) : 0;
+    if (select_way(*a) == SELECT_SPREAD)
+        n += (size_t)a->batch * attn_query_blocks(*a) * a->kv_heads * attn_max_blocks(*a) * sizeof(unsigned long long);
+    return n;
 }
 
 extern "C" int spamm_attn_select_dev(const spamm_attn *a, const float *d_key_sums, int n_first, int n_local,

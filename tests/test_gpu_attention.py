@@ -571,3 +571,46 @@ def test_captured_training_step():
         graph.replay()
         for a, b in zip(out, step()):
             assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("lens,H,HK,qb,block", [([700], 4, 4, 1, 16), ([5000], 2, 2, 4, 16), ([2100, 900], 8, 4, 2, 16),
+                                                ([17000], 1, 1, 8, 16)])
+def test_select_many_lists(lens, H, HK, qb, block):
+    """Enough lists for the kernels that work on tiles of them, and on single ones over many blocks; infinities and NaN among
+    the queries and keys."""
+    from cuspamm_b200 import select_blocks
+
+    g = torch.Generator().manual_seed(len(lens) + lens[0])
+    T, D = sum(lens), 64
+    q, k = tokens(g, T, H, D, BF), tokens(g, T, HK, D, BF)
+    k[5, 0, 3], k[40, 0, 7], k[90, HK - 1, 1] = torch.inf, -torch.inf, torch.nan
+    q[60, 0, 2], q[200, H - 1, 9] = torch.inf, torch.nan
+    got = select_blocks(q, k, cu_of(lens), max(lens), 8, block=block, query_block=qb, n_first=1, n_local=2).cpu()
+    at = 0
+    for s, n in enumerate(lens):
+        nb = -(-n // block)
+        sums = torch.stack([k[at + b * block:min(at + (b + 1) * block, at + n)].double().sum(0).float() for b in range(nb)]).double()
+        held = torch.tensor([min(block, n - b * block) for b in range(nb)], device=DEV).double()
+        qs = q[at:at + n].double().view(n, HK, H // HK, D).sum(2)
+        nqb = -(-n // qb)
+        qs = torch.zeros(nqb, HK, D, dtype=torch.float64, device=DEV).index_add_(0, torch.arange(n, device=DEV) // qb, qs)
+        first = torch.arange(nqb, device=DEV) * qb
+        last = torch.clamp(first + qb, max=n) - 1
+        b = torch.arange(nb, device=DEV)
+        for h in range(HK):
+            # the products one by one: infinities times zero and against each other must be NaN in every order of summation
+            score = torch.stack([(x[None] * sums[:, h]).sum(1) for x in qs[:, h]]) / held
+            rank = torch.where(torch.isnan(score), -torch.inf, score)
+            nan = torch.isnan(score)
+            forced = (b < 1)[None] | ((b > (first // block)[:, None] - 2) & (b <= (last // block)[:, None]))
+            ok = b[None] * block <= last[:, None]
+            # by rank: forced, then by score, NaN behind minus infinity, then by index; not candidates last
+            key = torch.where(forced, torch.inf, rank)
+            level = torch.where(ok, torch.where(forced, 3, torch.where(nan, 1, 2)), 0)
+            by = torch.argsort(key, dim=1, descending=True, stable=True)
+            by = torch.gather(by, 1, torch.argsort(torch.gather(level, 1, by), dim=1, descending=True, stable=True))[:, :8]
+            pick = torch.where(torch.gather(level, 1, by) > 0, by, nb).sort(1).values
+            want = torch.full((nqb, 8), -1)
+            want[:, :pick.shape[1]] = torch.where(pick < nb, pick, -1).cpu()
+            assert torch.equal(got[s, :nqb, h].long(), want), (s, h)
+        at += n
