@@ -123,6 +123,15 @@ __device__ __forceinline__ Reach reach_of(const spamm_attn &a, const Seq &sq, in
 }
 __device__ __forceinline__ bool taken(const Reach &r, int b, int n_first) { return b < n_first || (b > r.lo && b <= r.hi); }
 
+// The ordered key of the score z of candidate b.  Every block but the last is full, and 1 / block a power of two.
+__device__ __forceinline__ unsigned long long score_key(const spamm_attn &a, const Seq &sq, const Reach &r, int b, int n_first, double z,
+                                                        double per_key)
+{
+    if (taken(r, b, n_first)) return ~0ull;
+    const int held = sq.nk - b * a.block;
+    return order_key(held < a.block ? z / (double)held : z * per_key);
+}
+
 // Row of the key sums of block b; -1 for a page that does not exist.
 __device__ __forceinline__ int64_t key_sum_row(const spamm_attn &a, const Seq &sq, int s, int b)
 {
@@ -135,28 +144,62 @@ __device__ __forceinline__ int64_t key_sum_row(const spamm_attn &a, const Seq &s
     return page;
 }
 
-// The sum of a query block's queries over the heads of key head h, by all threads: qsum[D].  part: room for THREADS * 8.
-template <typename T, int D, int THREADS>
-static __device__ void query_sum(const spamm_attn &a, const Seq &sq, int64_t q0, int n_tok, int h, double *part, double *qsum)
+// The sums of every query block's queries over the heads of a key head, double [lists][D].  WIDE: a block of threads for a
+// list (many rows), else a group of D / 8 threads.  Bound by the reading of q.
+template <typename T, int D, bool WIDE>
+__global__ __launch_bounds__(256, 4) void attn_query_sums_kernel(const __grid_constant__ spamm_attn a, int nqb, FastDiv div_g,
+                                                              double *query_sums)
 {
-    constexpr int V = D / 8, GROUPS = THREADS / V;
+    constexpr int V = D / 8, GROUPS = 256 / V;
+    __shared__ double part[256 * 8];
     const int tid = threadIdx.x, c = tid % V, g = tid / V, G = a.heads / a.kv_heads;
+    const int64_t list = WIDE ? blockIdx.x : (int64_t)blockIdx.x * GROUPS + g;
+    const int64_t lists = (int64_t)a.batch * nqb * a.kv_heads;
+    if (list >= lists) return;
+    const int h = (int)(list % a.kv_heads), qb = (int)(list / a.kv_heads % nqb), s = (int)(list / a.kv_heads / nqb);
+    const Seq sq = attn_seq(a, s);
+    const int64_t q0 = (int64_t)qb * a.query_block;
+    const int n_tok = (int)min((int64_t)a.query_block, sq.nq - q0);
+    if (n_tok <= 0) return;
     const T *src = static_cast<const T *>(a.d_q) + (sq.row0 + q0) * a.q_token + (int64_t)h * G * a.q_head + c * 8;
     Sum8<T> sum;
-    sum.all(g, GROUPS, n_tok * G, [&](int r) { return src + r / G * a.q_token + r % G * a.q_head; });
+    sum.all(WIDE ? g : 0, WIDE ? GROUPS : 1, n_tok * G, [&](int r) {
+        const int tok = (int)div_g.quotient(r);
+        return src + tok * a.q_token + (r - tok * G) * a.q_head;
+    });
+    double *out = query_sums + list * D;
+    if constexpr (!WIDE) {
 #pragma unroll
-    for (int i = 0; i < 8; i++) part[(g * V + c) * 8 + i] = sum.y[i];
-    __syncthreads();
-    for (int d = tid; d < D; d += THREADS) {
-        double z = 0.0;
-        for (int k = 0; k < GROUPS; k++) z += part[k * D + d];
-        qsum[d] = z;
+        for (int i = 0; i < 4; i++)
+            reinterpret_cast<double2 *>(out + c * 8)[i] = make_double2(sum.y[2 * i], sum.y[2 * i + 1]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; i++) part[(g * V + c) * 8 + i] = sum.y[i];
+        __syncthreads();
+        for (int d = tid; d < D; d += 256) {
+            double z = 0.0;
+            for (int k = 0; k < GROUPS; k++) z += part[k * D + d];
+            out[d] = z;
+        }
     }
-    __syncthreads();
 }
 
-// The bits in which ordered keys can differ: all below the first one in which `low` and `high` do.
-__device__ __forceinline__ int differing_bits(unsigned long long low, unsigned long long high) { return 64 - __clzll(low ^ high); }
+// The number that an ordered key stands for.
+__device__ __forceinline__ double key_value(unsigned long long key)
+{
+    return __longlong_as_double((long long)(key >> 63 ? key & 0x7fffffffffffffffull : ~key));
+}
+// The next key to try between low and high (low < result < high; high - low > 1): halfway between the values for the first
+// rounds, which comes near a rank in few of them, halfway between the keys from then on, which always ends.
+__device__ __forceinline__ unsigned long long key_between(unsigned long long low, unsigned long long high, int round)
+{
+    if (round < 16) {
+        const double x = 0.5 * key_value(low) + 0.5 * key_value(high);
+        const unsigned long long key = order_key(x);
+        if (key > low && key < high) return key;
+    }
+    return low + ((high - low) >> 1);
+}
 
 // One warp writes the keys above the threshold, and of its equals the first `left`, as an ascending list.
 static __device__ __forceinline__ void write_list(const unsigned long long *keys, int n, unsigned long long threshold, int left, int n_select,
@@ -178,23 +221,28 @@ static __device__ __forceinline__ void write_list(const unsigned long long *keys
 }
 
 // Writes the n_select largest of keys[0, n) in shared memory (0: no candidate) as an ascending list, by all threads.  The
-// n_select-th largest key is found bit by bit; the search ends as soon as exactly n_select keys are at or above it.
+// threshold is searched between the smallest and the largest key, until exactly n_select keys are at or above it or it is
+// the n_select-th largest key itself.
 template <int THREADS>
 static __device__ void write_largest(const unsigned long long *keys, int n, int n_select, int32_t *out)
 {
-    __shared__ int counts[66];
+    __shared__ int counts[3];                    // taken in turn, each cleared two rounds ahead
     __shared__ unsigned long long ends[2];
     const int tid = threadIdx.x, lane = tid & 31;
-    if (tid < 66) counts[tid] = 0;
+    if (tid < 3) counts[tid] = 0;
     if (tid == 0) { ends[0] = ~0ull; ends[1] = 0; }
     __syncthreads();
-    auto count = [&](int slot, auto pred) {
+    int round = 0;
+    auto count = [&](auto pred) {
         int c = 0;
         for (int b = tid; b < n; b += THREADS) c += pred(keys[b]);
         c = __reduce_add_sync(~0u, c);
-        if (lane == 0 && c) atomicAdd(&counts[slot], c);
+        if (lane == 0 && c) atomicAdd(&counts[round % 3], c);
         __syncthreads();
-        return counts[slot];
+        c = counts[round % 3];
+        if (tid == 0) counts[(round + 2) % 3] = 0;
+        round++;
+        return c;
     };
     unsigned long long threshold = 1;
     int left = INT32_MAX;
@@ -215,91 +263,92 @@ static __device__ void write_largest(const unsigned long long *keys, int n, int 
             atomicMax(&ends[1], high);
         }
         __syncthreads();
-        const int bits = differing_bits(ends[0], ends[1]);
-        threshold = bits == 64 ? 0 : ends[1] >> bits << bits;
+        low = ends[0];
+        high = ends[1] + 1;                      // all keys are at or above low, fewer than n_select at or above high
         bool exact = false;
-        for (int bit = bits - 1; bit >= 0 && !exact; bit--) {
-            const unsigned long long want = threshold | (1ull << bit);
-            const int c = count(bit, [&](unsigned long long k) { return k >= want; });
-            if (c >= n_select) threshold = want;
+        while (high - low > 1 && !exact) {
+            const unsigned long long want = key_between(low, high, round);
+            const int c = count([&](unsigned long long k) { return k >= want; });
             exact = c == n_select;
+            if (c >= n_select) low = want;
+            else high = want;
         }
-        if (!exact) left = n_select - count(65, [&](unsigned long long k) { return k > threshold; });
+        threshold = low;
+        if (!exact) left = n_select - count([&](unsigned long long k) { return k > threshold; });
     }
-    if (tid < 32) write_list(keys, n, threshold, left, n_select, out, lane);
+    // every warp writes the part of the list that lies in its share of the blocks
+    __shared__ int2 shares[THREADS / 32];
+    const int warp = tid >> 5, share = (n + THREADS - 1) / THREADS * 32;
+    const int from = min(warp * share, n), to = min(from + share, n);
+    int above = 0, equal = 0;
+    for (int b = from + lane; b < to; b += 32) {
+        above += keys[b] > threshold;
+        equal += keys[b] == threshold && threshold != 0;
+    }
+    above = __reduce_add_sync(~0u, above);
+    equal = __reduce_add_sync(~0u, equal);
+    if (lane == 0) shares[warp] = make_int2(above, equal);
+    __syncthreads();
+    int at = 0, all = 0;
+    for (int w = 0; w < THREADS / 32; w++) {
+        const int2 x = shares[w];
+        const int ties = min(x.y, left);
+        if (w < warp) at += x.x + ties;
+        else if (w == warp) equal = ties;                    // of this share's equals, the first so many
+        left -= ties;
+        all += x.x + ties;
+    }
+    for (int b0 = from; b0 < to; b0 += 32) {
+        const int b = b0 + lane;
+        const unsigned long long key = b < to ? keys[b] : 0;
+        const unsigned eq = __ballot_sync(~0u, key == threshold && key != 0);
+        const bool tie = key == threshold && key != 0 && __popc(eq & ((1u << lane) - 1)) < equal;
+        const unsigned m = __ballot_sync(~0u, key > threshold || tie);
+        const int to_at = at + __popc(m & ((1u << lane) - 1));
+        if ((m >> lane & 1) && to_at < n_select) out[to_at] = b;
+        at += __popc(m);
+        equal -= min(equal, __popc(eq));
+    }
+    for (int i = min(all, n_select) + tid; i < n_select; i += THREADS) out[i] = -1;
 }
 
-// ---- QT query blocks and one key head per block of threads, scores as double products on the tensor cores (m8n8k4).  Many
-// query blocks: all blocks of keys, the lists picked from shared memory.  Few of them (decoding; SPREAD): SPREAD_BLOCKS
-// blocks of keys, so that the reading of the key sums spreads over the GPU, and the ordered scores to global memory.
-constexpr int SPREAD_BLOCKS = 64;
-
+// ---- many query blocks: QT of them and one key head per block of threads, scores as double products on the tensor cores
+// (m8n8k4), the lists picked from shared memory
 __device__ __forceinline__ void mma_double(double *c, double a, double b)
 {
     asm volatile("mma.sync.aligned.m8n8k4.row.col.f64.f64.f64.f64 {%0, %1}, {%2}, {%3}, {%0, %1};"
                  : "+d"(c[0]), "+d"(c[1]) : "d"(a), "d"(b));
 }
 
-template <typename T, int D, int QT, bool SPREAD>
+template <int D, int QT>
 __global__ __launch_bounds__(256) void attn_select_tile_kernel(const __grid_constant__ spamm_attn a, int nqb, int nkb, int n_first,
-                                                               int n_local, const float *key_sums, int32_t *lists,
-                                                               unsigned long long *spread_keys)
+                                                               int n_local, const float *key_sums, const double *query_sums,
+                                                               int32_t *lists)
 {
-    constexpr int V = D / 8, LD = D + 4;                    // rows 4 doubles apart from a multiple of the banks
+    constexpr int LD = D + 4;                               // rows 4 doubles apart from a multiple of the banks
     constexpr int MG = QT / 8, NG = 8 / MG, KT = QT == 8 ? 64 : 32, NT = KT / NG / 8;
     extern __shared__ __align__(16) uint8_t smem[];
     double *qs = reinterpret_cast<double *>(smem);          // [QT][LD]
     double *ks = qs + QT * LD;                              // [KT][LD]
     unsigned long long *keys = reinterpret_cast<unsigned long long *>(ks + KT * LD);    // [QT][nkb]
     __shared__ Reach reach[QT];
+    __shared__ bool there[KT];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int q_tiles = (nqb + QT - 1) / QT;
     unsigned idx = blockIdx.x;
-    const int spans = SPREAD ? (nkb + SPREAD_BLOCKS - 1) / SPREAD_BLOCKS : 1;
-    const int span = idx % spans; idx /= spans;
     const int qt = q_tiles - 1 - idx % q_tiles; idx /= q_tiles;
     const int h = idx % a.kv_heads, s = idx / a.kv_heads;
-    const int G = a.heads / a.kv_heads;
     const Seq sq = attn_seq(a, s);
-    if (SPREAD) {
-        // the last query block there is reaches furthest
-        const int last_qb = min((qt + 1) * QT, ceil_div(sq.nq, a.query_block)) - 1;
-        const int64_t q0 = (int64_t)last_qb * a.query_block;
-        if (last_qb < qt * QT ||
-            span * SPREAD_BLOCKS >= reach_of(a, sq, q0, (int)min((int64_t)a.query_block, sq.nq - q0), 0).n) return;
-    }
     if (tid < QT) {
         const int64_t q0 = (int64_t)(qt * QT + tid) * a.query_block;
         reach[tid] = reach_of(a, sq, q0, qt * QT + tid < nqb ? (int)min((int64_t)a.query_block, sq.nq - q0) : 0, n_local);
     }
-    // sums of the queries: a group of V threads for a query block, or the block's rows dealt out to several groups
-    {
-        constexpr int GROUPS = 256 / V, PER = GROUPS > QT ? GROUPS / QT : 1;
-        const int c = tid % V, g = tid / V;
-        for (int i = g / PER; i < QT; i += GROUPS / PER) {
-            const int64_t q0 = (int64_t)(qt * QT + i) * a.query_block;
-            const int n_tok = qt * QT + i < nqb ? (int)min((int64_t)a.query_block, sq.nq - q0) : 0;
-            const T *src = static_cast<const T *>(a.d_q) + (sq.row0 + q0) * a.q_token + (int64_t)h * G * a.q_head + c * 8;
-            int tok = 0, head = g % PER;
-            while (head >= G) { head -= G; tok++; }
-            const int tok0 = tok, head0 = head;
-            Sum8<T> sum;
-            sum.all(g % PER, PER, n_tok * G, [&](int r) {
-                if (r == g % PER) { tok = tok0; head = head0; }
-                const T *p = src + tok * a.q_token + head * a.q_head;
-                head += PER;
-                while (head >= G) { head -= G; tok++; }
-                return p;
-            });
-            // the PER partial sums lie in neighbouring lanes of one warp
-#pragma unroll
-            for (int d = V; d < PER * V; d <<= 1)
-#pragma unroll
-                for (int k = 0; k < 8; k++) sum.y[k] += __shfl_xor_sync(~0u, sum.y[k], d);
-            if (g % PER == 0)
-#pragma unroll
-                for (int k = 0; k < 8; k++) qs[i * LD + c * 8 + k] = sum.y[k];
-        }
+    for (int i = tid; i < QT * (D / 2); i += 256) {
+        const int r = i / (D / 2), c = i % (D / 2) * 2;
+        double2 x = make_double2(0.0, 0.0);
+        if ((int64_t)(qt * QT + r) * a.query_block < sq.nq)
+            x = *reinterpret_cast<const double2 *>(query_sums + (((int64_t)s * nqb + qt * QT + r) * a.kv_heads + h) * D + c);
+        *reinterpret_cast<double2 *>(qs + r * LD + c) = x;
     }
     __syncthreads();
     int n_most = 0;
@@ -307,16 +356,18 @@ __global__ __launch_bounds__(256) void attn_select_tile_kernel(const __grid_cons
     for (int i = 0; i < QT; i++) n_most = max(n_most, reach[i].n);
     const int mg = warp % MG, ng = warp / MG;
     const double per_key = 1.0 / (double)a.block;
-    const int b_end = SPREAD ? min(n_most, (span + 1) * SPREAD_BLOCKS) : n_most;
-    for (int b0 = SPREAD ? span * SPREAD_BLOCKS : 0; b0 < b_end; b0 += KT) {
-        for (int i = tid; i < KT * (D / 4); i += 256) {
-            const int r = i / (D / 4), c = i % (D / 4) * 4, b = b0 + r;
-            float4 k = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (b < n_most) {
-                const int64_t row = key_sum_row(a, sq, s, b);
-                if (row >= 0) k = *reinterpret_cast<const float4 *>(key_sums + (row * a.kv_heads + h) * D + c);
-            }
-            double *dst = ks + r * LD + c;
+    constexpr int PER_ROW = 256 / KT;                       // threads of a row of key sums
+    const int my_row = tid / PER_ROW, my_col = tid % PER_ROW;
+    for (int b0 = 0; b0 < n_most; b0 += KT) {
+        int64_t row = -1;
+        if (b0 + my_row < n_most) row = key_sum_row(a, sq, s, b0 + my_row);
+        const float4 *src = reinterpret_cast<const float4 *>(key_sums + (max(row, (int64_t)0) * a.kv_heads + h) * D);
+        if (my_col == 0) there[my_row] = row >= 0;
+#pragma unroll
+        for (int i = 0; i < D / 4 / PER_ROW; i++) {
+            const int c = i * PER_ROW + my_col;
+            const float4 k = row >= 0 ? src[c] : make_float4(0.f, 0.f, 0.f, 0.f);
+            double *dst = ks + my_row * LD + c * 4;
             *reinterpret_cast<double2 *>(dst) = make_double2((double)k.x, (double)k.y);
             *reinterpret_cast<double2 *>(dst + 2) = make_double2((double)k.z, (double)k.w);
         }
@@ -324,7 +375,7 @@ __global__ __launch_bounds__(256) void attn_select_tile_kernel(const __grid_cons
         double acc[NT][2] = {};
         const double *qa = qs + (mg * 8 + (lane >> 2)) * LD + (lane & 3);
         const double *kb = ks + (ng * NT * 8 + (lane >> 2)) * LD + (lane & 3);
-#pragma unroll 8
+#pragma unroll 16
         for (int k = 0; k < D; k += 4) {
             const double x = qa[k];
 #pragma unroll
@@ -336,21 +387,13 @@ __global__ __launch_bounds__(256) void attn_select_tile_kernel(const __grid_cons
         for (int n = 0; n < NT; n++)
 #pragma unroll
             for (int e = 0; e < 2; e++) {
-                const int b = b0 + (ng * NT + n) * 8 + (lane & 3) * 2 + e;
-                if (b >= nkb || (SPREAD && qt * QT + i >= nqb)) continue;
-                unsigned long long key = 0;
-                if (b < rr.n && (!a.n_pages || key_sum_row(a, sq, s, b) >= 0)) {
-                    // every block but the last is full, and 1 / block a power of two
-                    const int held = sq.nk - b * a.block;
-                    key = taken(rr, b, n_first) ? ~0ull : order_key(held < a.block ? acc[n][e] / (double)held : acc[n][e] * per_key);
-                }
-                if (SPREAD) spread_keys[(((int64_t)s * nqb + qt * QT + i) * a.kv_heads + h) * nkb + b] = key;
-                else keys[i * nkb + b] = key;
+                const int at = (ng * NT + n) * 8 + (lane & 3) * 2 + e, b = b0 + at;
+                if (b < nkb) keys[i * nkb + b] = b < rr.n && there[at] ? score_key(a, sq, rr, b, n_first, acc[n][e], per_key) : 0;
             }
         __syncthreads();
     }
-    // a warp for a list, as write_largest does it
-    if constexpr (!SPREAD) for (int i = warp; i < QT; i += 8) {
+    // a warp for a list, as write_largest does it; the upper halves of the keys, kept in registers, nearly always suffice
+    for (int i = warp; i < QT; i += 8) {
         const int qb = qt * QT + i;
         if (qb >= nqb) break;
         int32_t *out = lists + (((int64_t)s * nqb + qb) * a.kv_heads + h) * a.n_select;
@@ -359,26 +402,53 @@ __global__ __launch_bounds__(256) void attn_select_tile_kernel(const __grid_cons
         unsigned long long threshold = 1;
         int left = INT32_MAX;
         if (n > a.n_select) {
-            unsigned long long low = ~0ull, high = 0;
-            for (int b = lane; b < n; b += 32) {
-                low = min(low, mine[b]);
-                if (mine[b] != ~0ull) high = max(high, mine[b]);
-            }
-#pragma unroll
-            for (int d = 16; d; d >>= 1) {
-                low = min(low, __shfl_xor_sync(~0u, low, d));
-                high = max(high, __shfl_xor_sync(~0u, high, d));
-            }
-            const int bits = differing_bits(low, high);
-            threshold = bits == 64 ? 0 : high >> bits << bits;
             bool exact = false;
-            for (int bit = bits - 1; bit >= 0 && !exact; bit--) {
-                const unsigned long long want = threshold | (1ull << bit);
-                int count = 0;
-                for (int b = lane; b < n; b += 32) count += mine[b] >= want;
-                count = __reduce_add_sync(~0u, count);
-                if (count >= a.n_select) threshold = want;
-                exact = count == a.n_select;
+            constexpr int R = 8;
+            if (n <= 32 * R) {
+                uint32_t k[R], low = ~0u, high = 0;
+#pragma unroll
+                for (int x = 0; x < R; x++) {
+                    k[x] = x * 32 + lane < n ? (uint32_t)(mine[x * 32 + lane] >> 32) : 0;
+                    if (x * 32 + lane < n) low = min(low, k[x]);
+                    if (k[x] != ~0u) high = max(high, k[x]);
+                }
+                low = __reduce_min_sync(~0u, low);
+                high = __reduce_max_sync(~0u, high) + 1;
+                for (int round = 0; high - low > 1 && low < high && !exact; round++) {
+                    uint32_t want = (uint32_t)(key_between((unsigned long long)low << 32, (unsigned long long)high << 32, round) >> 32);
+                    if (want == low) want++;
+                    int c = 0;
+#pragma unroll
+                    for (int x = 0; x < R; x++) c += k[x] >= want;
+                    c = __reduce_add_sync(~0u, c);
+                    exact = c == a.n_select;
+                    if (c >= a.n_select) low = want;
+                    else high = want;
+                }
+                threshold = (unsigned long long)low << 32;
+            }
+            if (!exact) {
+                unsigned long long low = ~0ull, high = 0;
+                for (int b = lane; b < n; b += 32) {
+                    low = min(low, mine[b]);
+                    if (mine[b] != ~0ull) high = max(high, mine[b]);
+                }
+#pragma unroll
+                for (int d = 16; d; d >>= 1) {
+                    low = min(low, __shfl_xor_sync(~0u, low, d));
+                    high = max(high, __shfl_xor_sync(~0u, high, d));
+                }
+                high++;
+                for (int round = 0; high - low > 1 && !exact; round++) {
+                    const unsigned long long want = key_between(low, high, round);
+                    int c = 0;
+                    for (int b = lane; b < n; b += 32) c += mine[b] >= want;
+                    c = __reduce_add_sync(~0u, c);
+                    exact = c == a.n_select;
+                    if (c >= a.n_select) low = want;
+                    else high = want;
+                }
+                threshold = low;
             }
             if (!exact) {
                 int above = 0;
@@ -387,6 +457,94 @@ __global__ __launch_bounds__(256) void attn_select_tile_kernel(const __grid_cons
             }
         }
         write_list(mine, n, threshold, left, a.n_select, out, lane);
+    }
+}
+
+// ---- few query blocks (decoding): SPREAD_GROUPS times eight blocks of keys to a warp, so that the reading of the key sums, which bounds it,
+// spreads over the GPU; up to eight query blocks of a sequence at once.  The key sums go from global memory straight into
+// fragments: a lane reads four neighbouring values, which enter four products in turn (the sum over the values takes them in
+// another order than they lie in, for both operands alike).  With few rows to a query block their sums are taken here.
+constexpr int SPREAD_ROWS = 16, SPREAD_GROUPS = 1, SPREAD_WARPS = 4;
+
+template <typename T, int D>
+__global__ __launch_bounds__(SPREAD_WARPS * 32, 4) void attn_spread_scores_kernel(const __grid_constant__ spamm_attn a, int nqb, int spans, int nkb,
+                                                                 int n_first, int n_local, const float *key_sums,
+                                                                 const double *query_sums, unsigned long long *keys)
+{
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, row = lane >> 2, kk = lane & 3;
+    const int groups = (nqb + 7) / 8;
+    unsigned idx = blockIdx.x;
+    const int span = idx % spans; idx /= spans;
+    const int qg = idx % groups; idx /= groups;
+    const int h = idx % a.kv_heads, s = idx / a.kv_heads;
+    const Seq sq = attn_seq(a, s);
+    const int qb = qg * 8 + row;
+    const int64_t q0 = (int64_t)qb * a.query_block;
+    const int n_tok = qb < nqb ? (int)min((int64_t)a.query_block, sq.nq - q0) : 0;
+    const Reach reach = reach_of(a, sq, q0, n_tok, n_local);
+    int n_most = reach.n;
+#pragma unroll
+    for (int d = 4; d < 32; d <<= 1) n_most = max(n_most, __shfl_xor_sync(~0u, n_most, d));
+    const int first_b = (span * SPREAD_WARPS + warp) * 8 * SPREAD_GROUPS;
+    if (first_b >= n_most) return;
+    int64_t k_row[SPREAD_GROUPS];
+    float4 k[SPREAD_GROUPS][D / 16];
+#pragma unroll
+    for (int x = 0; x < SPREAD_GROUPS; x++) {
+        const int my_b = first_b + 8 * x + row;
+        k_row[x] = my_b < n_most ? key_sum_row(a, sq, s, my_b) : -1;
+    }
+#pragma unroll
+    for (int x = 0; x < SPREAD_GROUPS; x++) {
+        const float4 *ks = reinterpret_cast<const float4 *>(key_sums + (max(k_row[x], (int64_t)0) * a.kv_heads + h) * D) + kk;
+#pragma unroll
+        for (int i = 0; i < D / 16; i++) k[x][i] = k_row[x] >= 0 ? ks[4 * i] : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    const int64_t list = ((int64_t)s * nqb + qb) * a.kv_heads + h;
+    const int G = a.heads / a.kv_heads;
+    double q[D / 4] = {};
+    if (n_tok > 0) {
+        if (query_sums) {
+            const double2 *src = reinterpret_cast<const double2 *>(query_sums + list * D + 4 * kk);
+#pragma unroll
+            for (int i = 0; i < D / 16; i++) {
+                const double2 x = src[8 * i], y = src[8 * i + 1];
+                q[4 * i] = x.x; q[4 * i + 1] = x.y; q[4 * i + 2] = y.x; q[4 * i + 3] = y.y;
+            }
+        } else {
+            for (int r = 0; r < n_tok * G; r++) {
+                const T *src = static_cast<const T *>(a.d_q) + (sq.row0 + q0 + r / G) * a.q_token + (int64_t)(h * G + r % G) * a.q_head + 4 * kk;
+                uint2 x[D / 16];
+#pragma unroll
+                for (int i = 0; i < D / 16; i++) x[i] = *reinterpret_cast<const uint2 *>(src + 16 * i);
+#pragma unroll
+                for (int i = 0; i < D / 16; i++) {
+                    const float2 u = Pack<T>::to2(x[i].x), v = Pack<T>::to2(x[i].y);
+                    q[4 * i] += (double)u.x; q[4 * i + 1] += (double)u.y; q[4 * i + 2] += (double)v.x; q[4 * i + 3] += (double)v.y;
+                }
+            }
+        }
+    }
+    const double per_key = 1.0 / (double)a.block;
+    double acc[SPREAD_GROUPS][2] = {};
+#pragma unroll
+    for (int i = 0; i < D / 16; i++)
+#pragma unroll
+        for (int x = 0; x < SPREAD_GROUPS; x++) {
+            mma_double(acc[x], q[4 * i], (double)k[x][i].x);
+            mma_double(acc[x], q[4 * i + 1], (double)k[x][i].y);
+            mma_double(acc[x], q[4 * i + 2], (double)k[x][i].z);
+            mma_double(acc[x], q[4 * i + 3], (double)k[x][i].w);
+        }
+    // this lane's results: its row's query block, two blocks of each eight
+#pragma unroll
+    for (int x = 0; x < SPREAD_GROUPS; x++) {
+        const unsigned ok = __ballot_sync(~0u, k_row[x] >= 0);     // bit 4 * i: the i-th of the eight is there
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+            const int at = 2 * kk + e, b = first_b + 8 * x + at;
+            if (b < reach.n) keys[list * nkb + b] = ok >> (4 * at) & 1 ? score_key(a, sq, reach, b, n_first, acc[x][e], per_key) : 0;
+        }
     }
 }
 
@@ -406,11 +564,10 @@ __global__ __launch_bounds__(THREADS) void attn_largest_kernel(const __grid_cons
 // ---- many query blocks of sequences too long for that: one list per block of threads
 template <typename T, int D>
 __global__ __launch_bounds__(128) void attn_select_kernel(const __grid_constant__ spamm_attn a, int nqb, int n_first, int n_local,
-                                                          const float *key_sums, int32_t *lists)
+                                                          const float *key_sums, const double *query_sums, int32_t *lists)
 {
     extern __shared__ __align__(16) uint8_t smem[];
     unsigned long long *keys = reinterpret_cast<unsigned long long *>(smem);
-    __shared__ double part[128 * 8];
     __shared__ double qsum[D];
     const int tid = threadIdx.x;
     unsigned idx = blockIdx.x;
@@ -420,7 +577,9 @@ __global__ __launch_bounds__(128) void attn_select_kernel(const __grid_constant_
     const int64_t q0 = (int64_t)qb * a.query_block;
     const int n_tok = (int)min((int64_t)a.query_block, sq.nq - q0);
     const Reach reach = reach_of(a, sq, q0, n_tok, n_local);
-    if (n_tok > 0) query_sum<T, D, 128>(a, sq, q0, n_tok, h, part, qsum);
+    if (n_tok > 0)
+        for (int d = tid; d < D; d += 128) qsum[d] = query_sums[(int64_t)blockIdx.x * D + d];
+    __syncthreads();
     for (int b = tid; b < reach.n; b += 128) {
         unsigned long long key = ~0ull;
         const int64_t row = key_sum_row(a, sq, s, b);
@@ -456,16 +615,15 @@ static SelectWay select_way(const spamm_attn &a)
     return SELECT_ONE;
 }
 
-template <typename T, int D, int QT, bool SPREAD>
-static int select_tile_launch(const spamm_attn &a, int nqb, int nkb, int n_first, int n_local, const float *key_sums, int32_t *lists,
-                              unsigned long long *keys, cudaStream_t stream)
+template <int D, int QT>
+static int select_tile_launch(const spamm_attn &a, int nqb, int nkb, int n_first, int n_local, const float *key_sums,
+                              const double *query_sums, int32_t *lists, cudaStream_t stream)
 {
-    const size_t smem = (size_t)(QT + (QT == 8 ? 64 : 32)) * (D + 4) * 8 + (SPREAD ? 0 : (size_t)QT * nkb * 8);
-    const int64_t grid = (int64_t)a.batch * a.kv_heads * ((nqb + QT - 1) / QT) * (SPREAD ? ceil_div(nkb, SPREAD_BLOCKS) : 1);
-    if (grid > INT32_MAX) return attn_too_large();
-    int st = attn_set_smem((const void *)attn_select_tile_kernel<T, D, QT, SPREAD>, smem);
+    const size_t smem = (size_t)(QT + (QT == 8 ? 64 : 32)) * (D + 4) * 8 + (size_t)QT * nkb * 8;
+    const int64_t grid = (int64_t)a.batch * a.kv_heads * ((nqb + QT - 1) / QT);
+    int st = attn_set_smem((const void *)attn_select_tile_kernel<D, QT>, smem);
     if (st) return st;
-    attn_select_tile_kernel<T, D, QT, SPREAD><<<(unsigned)grid, 256, smem, stream>>>(a, nqb, nkb, n_first, n_local, key_sums, lists, keys);
+    attn_select_tile_kernel<D, QT><<<(unsigned)grid, 256, smem, stream>>>(a, nqb, nkb, n_first, n_local, key_sums, query_sums, lists);
     return SPAMM_OK;
 }
 
@@ -493,24 +651,36 @@ static int select_launch(const spamm_attn &a, const float *key_sums, int n_first
         attn_key_sums_kernel<T, D><<<(unsigned)sums_grid, 256, 0, stream>>>(a, nkb, scratch);
         key_sums = scratch;
     }
+    const int G = a.heads / a.kv_heads;
+    double *query_sums = reinterpret_cast<double *>(reinterpret_cast<uint8_t *>(scratch) + key_sums_bytes(a));
+    if ((int64_t)min(a.query_block, a.max_q) * G > INT32_MAX / 2) return attn_too_large();
+    const SelectWay way = select_way(a);
+    const int rows = min(a.query_block, a.max_q) * G;
+    if (rows >= 64)
+        attn_query_sums_kernel<T, D, true><<<(unsigned)grid, 256, 0, stream>>>(a, nqb, fast_div(G), query_sums);
+    else if (way != SELECT_SPREAD || rows > SPREAD_ROWS)
+        attn_query_sums_kernel<T, D, false><<<(unsigned)((grid + 2048 / D - 1) / (2048 / D)), 256, 0, stream>>>(a, nqb, fast_div(G), query_sums);
     int st = SPAMM_OK;
-    switch (select_way(a)) {
+    switch (way) {
     case SELECT_SPREAD: {
-        unsigned long long *keys = reinterpret_cast<unsigned long long *>(reinterpret_cast<uint8_t *>(scratch) + key_sums_bytes(a));
         if (!nkb) return clear_lists(a, lists, stream);
-        st = select_tile_launch<T, D, 8, true>(a, nqb, nkb, n_first, n_local, key_sums, lists, keys, stream);
-        if (st) return st;
+        unsigned long long *keys = reinterpret_cast<unsigned long long *>(query_sums + grid * D);
+        const int spans = ceil_div(nkb, 8 * SPREAD_GROUPS * SPREAD_WARPS);
+        const int64_t blocks = (int64_t)a.batch * a.kv_heads * ((nqb + 7) / 8) * spans;
+        if (blocks > INT32_MAX) return attn_too_large();
+        attn_spread_scores_kernel<T, D><<<(unsigned)blocks, SPREAD_WARPS * 32, 0, stream>>>(a, nqb, spans, nkb, n_first, n_local, key_sums,
+                                                                              rows > SPREAD_ROWS ? query_sums : nullptr, keys);
         st = attn_set_smem((const void *)attn_largest_kernel<256>, (size_t)nkb * 8);
         if (st) return st;
         attn_largest_kernel<256><<<(unsigned)grid, 256, (size_t)nkb * 8, stream>>>(a, nqb, nkb, keys, lists);
         break;
     }
-    case SELECT_TILE32: st = select_tile_launch<T, D, 32, false>(a, nqb, nkb, n_first, n_local, key_sums, lists, nullptr, stream); break;
-    case SELECT_TILE8: st = select_tile_launch<T, D, 8, false>(a, nqb, nkb, n_first, n_local, key_sums, lists, nullptr, stream); break;
+    case SELECT_TILE32: st = select_tile_launch<D, 32>(a, nqb, nkb, n_first, n_local, key_sums, query_sums, lists, stream); break;
+    case SELECT_TILE8: st = select_tile_launch<D, 8>(a, nqb, nkb, n_first, n_local, key_sums, query_sums, lists, stream); break;
     case SELECT_ONE:
         st = attn_set_smem((const void *)attn_select_kernel<T, D>, (size_t)nkb * 8);
         if (st) return st;
-        attn_select_kernel<T, D><<<(unsigned)grid, 128, (size_t)nkb * 8, stream>>>(a, nqb, n_first, n_local, key_sums, lists);
+        attn_select_kernel<T, D><<<(unsigned)grid, 128, (size_t)nkb * 8, stream>>>(a, nqb, n_first, n_local, key_sums, query_sums, lists);
         break;
     }
     if (st) return st;
@@ -525,9 +695,9 @@ using namespace spamm;
 extern "C" size_t spamm_attn_select_scratch_bytes(const spamm_attn *a)
 {
     if (attn_check(a, false) || !a->batch || !a->max_q) return 0;
-    size_t n = a->tokens ? key_sums_bytes(*a) : 0;
-    if (select_way(*a) == SELECT_SPREAD)
-        n += (size_t)a->batch * attn_query_blocks(*a) * a->kv_heads * attn_max_blocks(*a) * sizeof(unsigned long long);
+    const size_t lists = (size_t)a->batch * attn_query_blocks(*a) * a->kv_heads;
+    size_t n = key_sums_bytes(*a) + lists * a->dim * sizeof(double);
+    if (select_way(*a) == SELECT_SPREAD) n += lists * attn_max_blocks(*a) * sizeof(unsigned long long);
     return n;
 }
 
