@@ -460,17 +460,22 @@ __global__ __launch_bounds__(256) void attn_select_tile_kernel(const __grid_cons
     }
 }
 
-// ---- few query blocks (decoding): SPREAD_GROUPS times eight blocks of keys to a warp, so that the reading of the key sums, which bounds it,
-// spreads over the GPU; up to eight query blocks of a sequence at once.  The key sums go from global memory straight into
-// fragments: a lane reads four neighbouring values, which enter four products in turn (the sum over the values takes them in
-// another order than they lie in, for both operands alike).  With few rows to a query block their sums are taken here.
-constexpr int SPREAD_ROWS = 16, SPREAD_GROUPS = 1, SPREAD_WARPS = 4;
+// ---- few query blocks (decoding): SPREAD_BLOCKS blocks of keys to a warp, so that the reading of the key sums, which bounds
+// it, spreads over the GPU; up to eight query blocks of a sequence at once.  The key sums go from global memory straight into
+// registers, eight blocks at a time and the next eight under way: a lane has every fourth group of four values of one block.
+// One query block (the newest token): plain products, joined by two shuffles.  Several: m8n8k4, where a lane's four values
+// enter four products in turn (the sum then takes the values in another order, for both operands alike).
+constexpr int SPREAD_ROWS = 16;          // rows of a query block up to which their sums are taken here
+constexpr int SPREAD_BLOCKS = 32, SPREAD_WARPS = 4;
 
 template <typename T, int D>
-__global__ __launch_bounds__(SPREAD_WARPS * 32, 4) void attn_spread_scores_kernel(const __grid_constant__ spamm_attn a, int nqb, int spans, int nkb,
-                                                                 int n_first, int n_local, const float *key_sums,
-                                                                 const double *query_sums, unsigned long long *keys)
+__global__ __launch_bounds__(SPREAD_WARPS * 32, 4) void attn_spread_scores_kernel(const __grid_constant__ spamm_attn a, int nqb, int spans,
+                                                                                 int nkb, int n_first, int n_local,
+                                                                                 const float *key_sums, const double *query_sums,
+                                                                                 unsigned long long *keys)
 {
+    constexpr int N = D / 16;            // groups of four values of a lane
+    __shared__ __align__(16) double qs[8][D];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, row = lane >> 2, kk = lane & 3;
     const int groups = (nqb + 7) / 8;
     unsigned idx = blockIdx.x;
@@ -478,73 +483,90 @@ __global__ __launch_bounds__(SPREAD_WARPS * 32, 4) void attn_spread_scores_kerne
     const int qg = idx % groups; idx /= groups;
     const int h = idx % a.kv_heads, s = idx / a.kv_heads;
     const Seq sq = attn_seq(a, s);
-    const int qb = qg * 8 + row;
-    const int64_t q0 = (int64_t)qb * a.query_block;
-    const int n_tok = qb < nqb ? (int)min((int64_t)a.query_block, sq.nq - q0) : 0;
-    const Reach reach = reach_of(a, sq, q0, n_tok, n_local);
-    int n_most = reach.n;
-#pragma unroll
-    for (int d = 4; d < 32; d <<= 1) n_most = max(n_most, __shfl_xor_sync(~0u, n_most, d));
-    const int first_b = (span * SPREAD_WARPS + warp) * 8 * SPREAD_GROUPS;
-    if (first_b >= n_most) return;
-    int64_t k_row[SPREAD_GROUPS];
-    float4 k[SPREAD_GROUPS][D / 16];
-#pragma unroll
-    for (int x = 0; x < SPREAD_GROUPS; x++) {
-        const int my_b = first_b + 8 * x + row;
-        k_row[x] = my_b < n_most ? key_sum_row(a, sq, s, my_b) : -1;
-    }
-#pragma unroll
-    for (int x = 0; x < SPREAD_GROUPS; x++) {
-        const float4 *ks = reinterpret_cast<const float4 *>(key_sums + (max(k_row[x], (int64_t)0) * a.kv_heads + h) * D) + kk;
-#pragma unroll
-        for (int i = 0; i < D / 16; i++) k[x][i] = k_row[x] >= 0 ? ks[4 * i] : make_float4(0.f, 0.f, 0.f, 0.f);
-    }
-    const int64_t list = ((int64_t)s * nqb + qb) * a.kv_heads + h;
     const int G = a.heads / a.kv_heads;
-    double q[D / 4] = {};
-    if (n_tok > 0) {
-        if (query_sums) {
-            const double2 *src = reinterpret_cast<const double2 *>(query_sums + list * D + 4 * kk);
-#pragma unroll
-            for (int i = 0; i < D / 16; i++) {
-                const double2 x = src[8 * i], y = src[8 * i + 1];
-                q[4 * i] = x.x; q[4 * i + 1] = x.y; q[4 * i + 2] = y.x; q[4 * i + 3] = y.y;
-            }
-        } else {
-            for (int r = 0; r < n_tok * G; r++) {
-                const T *src = static_cast<const T *>(a.d_q) + (sq.row0 + q0 + r / G) * a.q_token + (int64_t)(h * G + r % G) * a.q_head + 4 * kk;
-                uint2 x[D / 16];
-#pragma unroll
-                for (int i = 0; i < D / 16; i++) x[i] = *reinterpret_cast<const uint2 *>(src + 16 * i);
-#pragma unroll
-                for (int i = 0; i < D / 16; i++) {
-                    const float2 u = Pack<T>::to2(x[i].x), v = Pack<T>::to2(x[i].y);
-                    q[4 * i] += (double)u.x; q[4 * i + 1] += (double)u.y; q[4 * i + 2] += (double)v.x; q[4 * i + 3] += (double)v.y;
-                }
-            }
-        }
+    const int n_lists = min(8, ceil_div(sq.nq, a.query_block) - qg * 8);      // of this group
+    if (n_lists <= 0) return;
+    {
+        // the last query block reaches furthest
+        const int64_t q0 = (int64_t)(qg * 8 + n_lists - 1) * a.query_block;
+        const Reach last = reach_of(a, sq, q0, (int)min((int64_t)a.query_block, sq.nq - q0), 0);
+        if (span * SPREAD_WARPS * SPREAD_BLOCKS >= last.n) return;
     }
+    const int first_b = (span * SPREAD_WARPS + warp) * SPREAD_BLOCKS;
+    // this lane's block of the warp's 32: the row of its key sums
+    int64_t my_row = -1;
+    if (first_b + lane < ceil_div(sq.nk, a.block)) my_row = key_sum_row(a, sq, s, first_b + lane);
+    const unsigned ok = __ballot_sync(~0u, my_row >= 0);
+    auto fetch = [&](int x, float4 *k) {
+        const int64_t at = __shfl_sync(~0u, my_row, 8 * x + row);
+        const float4 *ks = reinterpret_cast<const float4 *>(key_sums + (max(at, (int64_t)0) * a.kv_heads + h) * D) + kk;
+#pragma unroll
+        for (int i = 0; i < N; i++) k[i] = at >= 0 ? ks[4 * i] : make_float4(0.f, 0.f, 0.f, 0.f);
+    };
+    float4 k[N], next[N];
+    fetch(0, k);
+    for (int i = tid; i < n_lists * D; i += SPREAD_WARPS * 32) {
+        const int l = i / D, d = i % D;
+        const int64_t q0 = (int64_t)(qg * 8 + l) * a.query_block;
+        double z = 0.0;
+        if (query_sums) {
+            z = query_sums[(((int64_t)s * nqb + qg * 8 + l) * a.kv_heads + h) * D + d];
+        } else {
+            const int rows = (int)min((int64_t)a.query_block, sq.nq - q0) * G;
+            const T *src = static_cast<const T *>(a.d_q) + (sq.row0 + q0) * a.q_token + (int64_t)h * G * a.q_head + d;
+#pragma unroll 4
+            for (int r = 0; r < rows; r++) z += (double)(float)src[r / G * a.q_token + r % G * a.q_head];
+        }
+        qs[l][d] = z;
+    }
+    __syncthreads();
     const double per_key = 1.0 / (double)a.block;
-    double acc[SPREAD_GROUPS][2] = {};
-#pragma unroll
-    for (int i = 0; i < D / 16; i++)
-#pragma unroll
-        for (int x = 0; x < SPREAD_GROUPS; x++) {
-            mma_double(acc[x], q[4 * i], (double)k[x][i].x);
-            mma_double(acc[x], q[4 * i + 1], (double)k[x][i].y);
-            mma_double(acc[x], q[4 * i + 2], (double)k[x][i].z);
-            mma_double(acc[x], q[4 * i + 3], (double)k[x][i].w);
+    auto store = [&](int l, int b, bool there, double z) {
+        const int64_t q0 = (int64_t)(qg * 8 + l) * a.query_block;
+        const Reach reach = reach_of(a, sq, q0, (int)min((int64_t)a.query_block, sq.nq - q0), n_local);
+        if (b < reach.n)
+            keys[(((int64_t)s * nqb + qg * 8 + l) * a.kv_heads + h) * nkb + b] = there ? score_key(a, sq, reach, b, n_first, z, per_key) : 0;
+    };
+    // the list whose sums this lane reads (lanes of rows without one: any, their results are not used)
+    const double *q = qs[n_lists == 1 ? 0 : min(row, n_lists - 1)] + 4 * kk;
+#pragma unroll 1
+    for (int x = 0; x < SPREAD_BLOCKS / 8; x++) {
+        if (!(ok >> (8 * x))) {
+            // nothing but blocks that are not there: their keys are written all the same
+            if (first_b + 8 * x >= ceil_div(sq.nk, a.block)) break;
         }
-    // this lane's results: its row's query block, two blocks of each eight
+        if (x + 1 < SPREAD_BLOCKS / 8) fetch(x + 1, next);
+        if (n_lists == 1) {
+            double z0 = 0.0, z1 = 0.0;
 #pragma unroll
-    for (int x = 0; x < SPREAD_GROUPS; x++) {
-        const unsigned ok = __ballot_sync(~0u, k_row[x] >= 0);     // bit 4 * i: the i-th of the eight is there
+            for (int i = 0; i < N; i++) {
+                const double2 u = *reinterpret_cast<const double2 *>(q + 16 * i), v = *reinterpret_cast<const double2 *>(q + 16 * i + 2);
+                z0 = fma(u.x, (double)k[i].x, z0);
+                z1 = fma(u.y, (double)k[i].y, z1);
+                z0 = fma(v.x, (double)k[i].z, z0);
+                z1 = fma(v.y, (double)k[i].w, z1);
+            }
+            z0 += z1;
+            z0 += __shfl_xor_sync(~0u, z0, 1);
+            z0 += __shfl_xor_sync(~0u, z0, 2);
+            if (kk == 0) store(0, first_b + 8 * x + row, ok >> (8 * x + row) & 1, z0);
+        } else {
+            double acc[2][2] = {};
 #pragma unroll
-        for (int e = 0; e < 2; e++) {
-            const int at = 2 * kk + e, b = first_b + 8 * x + at;
-            if (b < reach.n) keys[list * nkb + b] = ok >> (4 * at) & 1 ? score_key(a, sq, reach, b, n_first, acc[x][e], per_key) : 0;
+            for (int i = 0; i < N; i++) {
+                const double2 u = *reinterpret_cast<const double2 *>(q + 16 * i), v = *reinterpret_cast<const double2 *>(q + 16 * i + 2);
+                mma_double(acc[0], u.x, (double)k[i].x);
+                mma_double(acc[1], u.y, (double)k[i].y);
+                mma_double(acc[0], v.x, (double)k[i].z);
+                mma_double(acc[1], v.y, (double)k[i].w);
+            }
+            if (row < n_lists)
+#pragma unroll
+                for (int e = 0; e < 2; e++)
+                    store(row, first_b + 8 * x + 2 * kk + e, ok >> (8 * x + 2 * kk + e) & 1, acc[0][e] + acc[1][e]);
         }
+#pragma unroll
+        for (int i = 0; i < N; i++) k[i] = next[i];
     }
 }
 
@@ -665,7 +687,7 @@ static int select_launch(const spamm_attn &a, const float *key_sums, int n_first
     case SELECT_SPREAD: {
         if (!nkb) return clear_lists(a, lists, stream);
         unsigned long long *keys = reinterpret_cast<unsigned long long *>(query_sums + grid * D);
-        const int spans = ceil_div(nkb, 8 * SPREAD_GROUPS * SPREAD_WARPS);
+        const int spans = ceil_div(nkb, SPREAD_BLOCKS * SPREAD_WARPS);
         const int64_t blocks = (int64_t)a.batch * a.kv_heads * ((nqb + 7) / 8) * spans;
         if (blocks > INT32_MAX) return attn_too_large();
         attn_spread_scores_kernel<T, D><<<(unsigned)blocks, SPREAD_WARPS * 32, 0, stream>>>(a, nqb, spans, nkb, n_first, n_local, key_sums,
