@@ -54,7 +54,7 @@ def _rows(name: str, x: torch.Tensor, heads: Optional[int] = None, like: Optiona
 def _ints(name: str, x: torch.Tensor, shape, device) -> torch.Tensor:
     if not isinstance(x, torch.Tensor) or x.dtype != torch.int32:
         raise ValueError(f"{name} must be an int32 tensor")
-    if tuple(x.shape) != tuple(shape):
+    if x.shape != shape:
         raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(x.shape)}")
     if x.device != device:
         raise ValueError(f"{name} must be on {device}, is on {x.device}")
@@ -64,6 +64,8 @@ def _ints(name: str, x: torch.Tensor, shape, device) -> torch.Tensor:
 
 
 def _host_int(name: str, x, least: int = 0) -> int:
+    if type(x) is int and least <= x < 2 ** 31:
+        return x
     if isinstance(x, torch.Tensor):
         raise TypeError(f"{name} is a host-side number, not a tensor")
     v = int(x)
@@ -86,7 +88,8 @@ def _on_gpu(x: torch.Tensor) -> None:
 
 def _strides(x: torch.Tensor):
     """Token and head stride; those of a dimension of one element are never used and may be anything."""
-    return (x.stride(0) if x.shape[0] > 1 else 0), (x.stride(1) if x.shape[1] > 1 else 0)
+    (tokens, heads, _), (token, head, _) = x.shape, x.stride()
+    return (token if tokens > 1 else 0), (head if heads > 1 else 0)
 
 
 def _problem(q: torch.Tensor, kv_heads: int, cu_seqlens: torch.Tensor, max_q: int, block: int, query_block: int,
@@ -144,7 +147,24 @@ def _scale(scale, head_dim: int) -> float:
 
 
 def _stream(device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
+class _Same:
+    """Stands for torch.cuda.device where the tensors' device is the current one already."""
+
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *exc):
+        return False
+
+
+_SAME = _Same()
+
+
+def _device(device):
+    return _SAME if torch.cuda.current_device() == device.index else torch.cuda.device(device)
 
 
 def _select(a: SpammAttn, q: torch.Tensor, key_sums: Optional[torch.Tensor], n_select, n_first, n_local) -> torch.Tensor:
@@ -153,7 +173,7 @@ def _select(a: SpammAttn, q: torch.Tensor, key_sums: Optional[torch.Tensor], n_s
     if not 1 <= n_select <= 1024 or n_select < forced:
         raise ValueError(f"n_select must be 1 to 1024 and hold the {forced} first and local blocks, got {n_select}")
     _on_gpu(q)
-    with torch.cuda.device(q.device):
+    with _device(q.device):
         lists = torch.empty((a.batch, -(-a.max_q // a.query_block), a.kv_heads, n_select), dtype=torch.int32, device=q.device)
         n = lib.spamm_attn_select_scratch_bytes(C.byref(a))
         scratch, ptr = _scratch(n, q.device)
@@ -195,8 +215,8 @@ class _BlockSparseAttention(torch.autograd.Function):
         _set_keys(a, k, v)
         _set_lists(a, lists, q.device)
         _on_gpu(q)
-        with torch.cuda.device(q.device):
-            o = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        with _device(q.device):
+            o = q.new_empty(q.shape)
             lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device)
             _set_out(a, o)
             a.d_lse = lse.data_ptr()
@@ -227,10 +247,10 @@ class _BlockSparseAttention(torch.autograd.Function):
         if d_o.numel() and (d_o.stride(2) != 1 or d_o.data_ptr() % 16 or any(st % 8 for st in _strides(d_o))):
             d_o = d_o.contiguous()
         lib = _lib.load()
-        with torch.cuda.device(q.device):
-            dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-            dk = torch.empty(k.shape, dtype=k.dtype, device=k.device)
-            dv = torch.empty(v.shape, dtype=v.dtype, device=v.device)
+        with _device(q.device):
+            dq = q.new_empty(q.shape)
+            dk = k.new_empty(k.shape)
+            dv = v.new_empty(v.shape)
             n = lib.spamm_attn_backward_scratch_bytes(C.byref(a))
             scratch, ptr = _scratch(n, q.device)
             check(lib.spamm_attn_backward_dev(C.byref(a), d_o.data_ptr(), *_strides(d_o), dq.data_ptr(), dk.data_ptr(),
@@ -343,10 +363,10 @@ class PagedCache:
         a = self._problem(k if q is None else q, cu_seqlens, max_new, page_table, lengths, 1, 0, True)
         _set_keys(a, k, v)
         lib = _lib.load()
-        with torch.cuda.device(k.device):
+        with _device(k.device):
             out = None
             if q is not None:
-                out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+                out = q.new_empty(q.shape)
                 _set_out(a, out)
                 if not a.batch or not a.max_q:
                     out.zero_()
@@ -376,9 +396,9 @@ class PagedCache:
         a.d_k, a.d_v = self.k.data_ptr(), self.v.data_ptr()
         if lists is not None:
             _set_lists(a, lists, q.device)
-        with torch.cuda.device(q.device):
+        with _device(q.device):
             if out is None:
-                out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+                out = q.new_empty(q.shape)
                 if not a.batch or not a.max_q:
                     out.zero_()
             else:

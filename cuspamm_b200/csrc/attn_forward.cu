@@ -52,9 +52,25 @@ int attn_check(const spamm_attn *a, bool need_lists)
     return SPAMM_OK;
 }
 
+// The attribute is set once for a kernel, device and host thread as long as the size does not grow (the call costs about as
+// much as a launch).
 int attn_set_smem(const void *kernel, size_t bytes)
 {
-    if (bytes > 48 * 1024) SPAMM_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+    if (bytes <= 48 * 1024) return SPAMM_OK;
+    struct Known { const void *kernel; int device; size_t bytes; };
+    constexpr int ROOM = 64;
+    static thread_local Known known[ROOM];
+    static thread_local int n_known = 0;
+    int device = 0;
+    SPAMM_CUDA_TRY(cudaGetDevice(&device));
+    int i = 0;
+    while (i < n_known && (known[i].kernel != kernel || known[i].device != device)) i++;
+    if (i < n_known && known[i].bytes >= bytes) return SPAMM_OK;
+    SPAMM_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+    if (i < ROOM) {
+        known[i] = Known{kernel, device, bytes};
+        if (i == n_known) n_known++;
+    }
     return SPAMM_OK;
 }
 
