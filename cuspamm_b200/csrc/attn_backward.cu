@@ -587,8 +587,8 @@ __global__ __launch_bounds__(TQ_THREADS, 2) void attn_dq_tc_kernel(const __grid_
     const int s = idx / a.kv_heads;
     const int G = a.heads / a.kv_heads;
     const Seq sq = attn_seq(a, s);
-    TileRows tr;
-    if (!attn_tile(a, sq, tile, &tr)) return;
+    const TileRows tr = attn_tile(a, sq, tile);
+    if (!tr.rows) return;
     const int rows = tr.rows;
     const int limit_max = attn_limit(a, sq, tr.last), limit_min = attn_limit(a, sq, tr.first);
 
@@ -612,8 +612,8 @@ __global__ __launch_bounds__(TQ_THREADS, 2) void attn_dq_tc_kernel(const __grid_
         tmem_alloc<TQ_COLS>(smem_u32(&ctrl->tmem_base));
         tc_fence_before();
     }
-    const int n_entries = attn_union<TQ_THREADS>(a, sq, s, h, tr, 0, ceil_div(limit_max, a.block), reinterpret_cast<uint32_t *>(smem),
-                                                 blk, bits, &ctrl->count);
+    const int n_entries = attn_union<TQ_THREADS, 1>(a, sq, s, h, &tr, 0, ceil_div(limit_max, a.block),
+                                                    reinterpret_cast<uint32_t *>(smem), blk, bits, max_entries, &ctrl->count);
     tc_fence_after();
     const int log_block = 31 - __clz(a.block);
     const int n_keys = n_entries << log_block;

@@ -120,6 +120,7 @@ struct RowsPlan {
     int n_split;            // ranges of keys
     int split_keys;         // keys of a range, a multiple of the block
     int max_entries;        // blocks of a range
+    bool pairs;             // pairs of tiles of 128 rows to a block of threads
 };
 
 constexpr int ROWS_STAGES = 3;
@@ -363,80 +364,99 @@ __global__ __launch_bounds__(128) void attn_rows_kernel(const __grid_constant__ 
     }
 }
 
-// ---- tiles of 128 rows on the tensor memory path
+// ---- pairs of tiles of 128 rows on the tensor memory path
 //
-// Per block of threads: 128 rows (queries x heads of a key head) against a range of its keys, 128 keys (the listed blocks
-// one behind the other) at a time.  S = Q K^T goes to tensor memory; eight warps, two threads for each row, take the running
-// maximum and write p over S in the type of v; O += P V takes p from tensor memory.  A block uses half of the tensor
-// memory and under half of the shared memory, so that two of them share an SM: one's exponentials run beside the other's
-// products.  One warp feeds K and V, a tensor copy for each block of keys and 64 values; the block in which the sequence
-// ends is copied 16 bytes a time with zeros behind the last key (what lies there may be NaN).
+// Per block of threads: two tiles of 128 rows (queries x heads of a key head) against a range of their keys, 128 keys (the
+// blocks of the union of their lists one behind the other) at a time.  S = Q K^T goes to tensor memory; two threads for each
+// row, half of the keys each, take the running maximum and write p over S in the type of v (one warp per scheduler and tile
+// would not overlap its exponentials with its other instructions); O += P V takes p from tensor memory.  One warp issues the
+// products of the two tiles in turn, so that one tile's exponentials run beside the other's products (two independent blocks
+// per SM fall into step instead: both multiply, then both exponentiate).  K and V are shared by the pair and double
+// buffered; one warp feeds them, a tensor copy for each block of keys and 64 values; the block in which the sequence ends is
+// copied 16 bytes a time with zeros behind the last key (what lies there may be NaN).
 //
 // The running maximum is only raised when a row's scores exceed it by more than 2^8: until then p stays below 2^8, which
 // both types and the float sums hold without loss, and O need not be rescaled in tensor memory.
+//
+// Where pairs would not fill the GPU, single tiles (TILES 1) with one buffer each for K and V: two blocks of threads per SM.
 constexpr int TC_ROWS = 128, TC_KEYS = 128, TC_HALF = TC_KEYS / 2;
-constexpr int TC_SOFTMAX = 256, TC_THREADS = TC_SOFTMAX + 64;
-constexpr int TC_COLS = 256;            // S (P over each half of it) in columns 0..127, O behind
+constexpr int TC_ENTRIES = 2048;        // blocks of a union, at most
+constexpr int TC_POLY = 6;              // of 16 pairs of exponentials, those that the polynomial takes
 
 struct TcCtrl {
-    uint64_t q_full, k_full, k_empty, v_full, v_empty, s_full, p_full, pv_done;
-    uint64_t met[4];                    // the two warps of 32 rows have left their maxima
+    uint64_t q_full[2], k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], pv_done[2];
+    uint64_t met[8];                    // [tile][32 rows]: the two warps of the rows have left their maxima
     uint32_t tmem_base;
     uint32_t abort_flag;
     int32_t err;
     int32_t count;
     int32_t bad_page;
     int32_t pad[3];
-    float top[2][2][TC_ROWS];           // [tile & 1][half][row]
+    float top[2][2][2][TC_ROWS];        // [tile][step & 1][half][row]
 };
 
-template <typename T, int D>
-__global__ __launch_bounds__(TC_THREADS, 2) void attn_tc_kernel(const __grid_constant__ spamm_attn a, const RowsPlan p,
+template <typename T, int D, int TILES>
+__global__ __launch_bounds__(TILES * 256 + 64, TILES == 1 ? 2 : 1) void attn_tc_kernel(const __grid_constant__ spamm_attn a, const RowsPlan p,
                                                                 const __grid_constant__ RowMap k_map,
                                                                 const __grid_constant__ RowMap v_map, float *part_o,
                                                                 float *part_lse)
 {
     extern __shared__ __align__(1024) uint8_t smem_tc[];
-    constexpr int TILE = 128 * D * 2;
+    constexpr int TILE = 128 * D * 2, STAGES = TILES, THREADS = TILES * 256 + 64, W_MMA = TILES * 8, W_LOAD = W_MMA + 1;
+    constexpr int COLS = TILES * 256;                                  // S (P over it) of the tiles, then O
     uint8_t *const smem = smem_tc;
-    const uint32_t q_tile = smem_u32(smem), k_tile = q_tile + TILE, v_tile = k_tile + TILE;
-    TcCtrl *ctrl = reinterpret_cast<TcCtrl *>(smem + 3 * TILE);
-    uint32_t *bits = reinterpret_cast<uint32_t *>(ctrl + 1);           // [max_entries], with lists
-    uint16_t *idx = reinterpret_cast<uint16_t *>(bits + (a.n_select ? p.max_entries : 0));
+    const uint32_t q_tiles = smem_u32(smem), k_ring = q_tiles + TILES * TILE, v_ring = k_ring + STAGES * TILE;
+    TcCtrl *ctrl = reinterpret_cast<TcCtrl *>(smem + 3 * TILES * TILE);
+    uint32_t *bits = reinterpret_cast<uint32_t *>(ctrl + 1);           // [TILES][max_entries], with lists
+    uint16_t *idx = reinterpret_cast<uint16_t *>(bits + (a.n_select ? TILES * p.max_entries : 0));
 
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     unsigned where = blockIdx.x;
     // tiles that read the same keys run side by side, those with the longest causal rows first
-    const int tile = p.tiles - 1 - where % p.tiles; where /= p.tiles;
+    const int pair = p.tiles - 1 - where % p.tiles; where /= p.tiles;      // of tiles (or one tile)
     const int split = where % p.n_split; where /= p.n_split;
     const int h = where % a.kv_heads;
     const int s = where / a.kv_heads;
     const int G = a.heads / a.kv_heads;
     const Seq sq = attn_seq(a, s);
-    if (a.zero_tail && split == 0) zero_tail<T>(a, sq, s, h, tile, p.tiles);
-    TileRows tr;
-    if (!attn_tile(a, sq, tile, &tr)) return;
-    const int rows = tr.rows;
-    const int limit_max = attn_limit(a, sq, sq.pos0 + tr.last), limit_min = attn_limit(a, sq, sq.pos0 + tr.first);
+    if (a.zero_tail && split == 0) zero_tail<T>(a, sq, s, h, pair, p.tiles);
+    const TileRows tr[2] = {attn_tile(a, sq, TILES * pair), TILES == 2 ? attn_tile(a, sq, 2 * pair + 1) : TileRows{}};
+    if (!tr[0].rows) return;
+    const int limits[2] = {attn_limit(a, sq, sq.pos0 + tr[0].last), tr[1].rows ? attn_limit(a, sq, sq.pos0 + tr[1].last) : 0};
+    const int limit_max = max(limits[0], limits[1]);
 
-    if (warp == 8) {
+    if (warp < W_MMA) {
+        // the queries of the warp's tile
+        const int x0 = warp >> 3, t = tid & 255;
+        const TileRows mine = x0 ? tr[1] : tr[0];
+        for (int i = 0; i < D / 16; i++) {
+            const int x = i * 256 + t, qr = x / (D / 8), c = x % (D / 8);
+            const bool ok = qr < mine.rows;
+            const int qy = mine.row0 + (ok ? qr : 0);
+            const int64_t off = (int64_t)(sq.row0 + qy / G) * a.q_token + (int64_t)(h * G + qy % G) * a.q_head;
+            cp_async16(q_tiles + x0 * TILE + panel_off(128, qr, c), static_cast<const T *>(a.d_q) + off + c * 8, ok);
+        }
+        cp_commit();
+    } else if (warp == W_MMA) {
         if (lane == 0) {
-            mbar_init(smem_u32(&ctrl->q_full), TC_SOFTMAX);
-            mbar_init(smem_u32(&ctrl->k_full), 32);
-            mbar_init(smem_u32(&ctrl->v_full), 32);
-            mbar_init(smem_u32(&ctrl->k_empty), 1);
-            mbar_init(smem_u32(&ctrl->v_empty), 1);
-            mbar_init(smem_u32(&ctrl->s_full), 1);
-            mbar_init(smem_u32(&ctrl->pv_done), 1);
-            mbar_init(smem_u32(&ctrl->p_full), TC_SOFTMAX);
-            for (int i = 0; i < 4; i++) mbar_init(smem_u32(&ctrl->met[i]), 64);
+            for (int i = 0; i < 2; i++) {
+                mbar_init(smem_u32(&ctrl->q_full[i]), 256);
+                mbar_init(smem_u32(&ctrl->k_full[i]), 32);
+                mbar_init(smem_u32(&ctrl->v_full[i]), 32);
+                mbar_init(smem_u32(&ctrl->k_empty[i]), 1);
+                mbar_init(smem_u32(&ctrl->v_empty[i]), 1);
+                mbar_init(smem_u32(&ctrl->s_full[i]), 1);
+                mbar_init(smem_u32(&ctrl->pv_done[i]), 1);
+                mbar_init(smem_u32(&ctrl->p_full[i]), 256);
+            }
+            for (int i = 0; i < 8; i++) mbar_init(smem_u32(&ctrl->met[i]), 64);
             ctrl->abort_flag = 0;
             ctrl->err = 0;
             ctrl->bad_page = 0;
             asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         }
         __syncwarp();
-        tmem_alloc<TC_COLS>(smem_u32(&ctrl->tmem_base));
+        tmem_alloc<COLS>(smem_u32(&ctrl->tmem_base));
         tc_fence_before();
     }
     const int log_block = 31 - __clz(a.block);
@@ -444,11 +464,12 @@ __global__ __launch_bounds__(TC_THREADS, 2) void attn_tc_kernel(const __grid_con
     const int b1 = min(b0 + (p.split_keys >> log_block), ceil_div(limit_max, a.block));
     int n_entries = b1 - b0;
     if (a.n_select) {
-        n_entries = attn_union<TC_THREADS>(a, sq, s, h, tr, b0, b1, reinterpret_cast<uint32_t *>(smem), idx, bits, &ctrl->count);
+        n_entries = attn_union<THREADS, TILES>(a, sq, s, h, tr, b0, b1, reinterpret_cast<uint32_t *>(smem + TILES * TILE), idx, bits,
+                                              p.max_entries, &ctrl->count);
     } else {
         __syncthreads();
         if (a.n_pages) {
-            for (int e = tid; e < n_entries; e += TC_THREADS) {
+            for (int e = tid; e < n_entries; e += THREADS) {
                 const int page = a.d_table[(int64_t)s * a.table_stride + b0 + e];
                 if (page < 0 || page >= a.n_pages) {
                     ctrl->bad_page = 1;
@@ -462,15 +483,26 @@ __global__ __launch_bounds__(TC_THREADS, 2) void attn_tc_kernel(const __grid_con
     // block of keys of entry e
     auto block_of = [&](int e) { return b0 + (a.n_select ? (int)idx[e] : e); };
     auto page_of = [&](int b) { return a.d_table[(int64_t)s * a.table_stride + b]; };
-    const int n_keys = n_entries << log_block;
+    const int n_keys = n_entries << log_block, per_tile = TC_KEYS >> log_block;
     const int n_tiles = (n_keys + TC_KEYS - 1) / TC_KEYS;
-    const uint32_t tmem = ctrl->tmem_base, tmem_o = tmem + TC_KEYS;
+    // whether some row of tile x reads keys of step j
+    auto uses = [&](bool second, int j) {
+        if (second && !tr[1].rows) return false;
+        if (!a.n_select) return (b0 << log_block) + j * TC_KEYS < (second ? limits[1] : limits[0]);
+        const uint32_t *mine = bits + (second ? p.max_entries : 0);
+        bool any = false;
+        for (int i = 0; i < per_tile; i++) {
+            const int e = j * per_tile + i;
+            any |= e < n_entries && mine[e] != 0;
+        }
+        return any;
+    };
+    const uint32_t tmem = ctrl->tmem_base, tmem_o = tmem + TILES * TC_KEYS;
     const WaitState ws{&ctrl->abort_flag, &ctrl->err};
 
-    if (warp == 9) {
+    if (warp == W_LOAD) {
         // ---- K and V
-        const int per_tile = TC_KEYS >> log_block;
-        // lane's copies of a tile: entry j * per_tile + my_i, values 64 * my_panel ..
+        // lane's copies of a step: entry j * per_tile + my_i, values 64 * my_panel ..
         const int my_i = lane / (D / 64), my_panel = lane % (D / 64);
         // where they begin: the row of packed keys, or page * kv_heads + head; -1: not there, -2: to be copied by hand
         struct At { int row, pos; };
@@ -490,8 +522,8 @@ __global__ __launch_bounds__(TC_THREADS, 2) void attn_tc_kernel(const __grid_con
             return at;
         };
         // every lane takes part in the barrier's phase with the bytes of its tensor copy and one arrival
-        auto load = [&](int j, const At &at, bool value, uint64_t *full) {
-            const uint32_t dst = value ? v_tile : k_tile, bar = smem_u32(full);
+        auto load = [&](int j, const At &at, bool value, uint32_t dst, uint64_t *full) {
+            const uint32_t bar = smem_u32(full);
             const RowMap &rm = value ? v_map : k_map;
             if (at.row >= 0 && rm.usable) {
                 mbar_expect_tx(bar, a.block * 128);
@@ -534,71 +566,80 @@ __global__ __launch_bounds__(TC_THREADS, 2) void attn_tc_kernel(const __grid_con
         At at = look_up(0);
         for (int j = 0; j < n_tiles; j++) {
             const At next = look_up(j + 1);
-            if (j) fine = __all_sync(~0u, ws.wait(smem_u32(&ctrl->k_empty), j - 1, 1));
+            const int b = j % STAGES, round = j / STAGES;
+            if (round) fine = __all_sync(~0u, ws.wait(smem_u32(&ctrl->k_empty[b]), round - 1, 1));
             if (!fine) break;
-            load(j, at, false, &ctrl->k_full);
-            if (j) fine = __all_sync(~0u, ws.wait(smem_u32(&ctrl->v_empty), j - 1, 2));
+            load(j, at, false, k_ring + b * TILE, &ctrl->k_full[b]);
+            if (round) fine = __all_sync(~0u, ws.wait(smem_u32(&ctrl->v_empty[b]), round - 1, 2));
             if (!fine) break;
-            load(j, at, true, &ctrl->v_full);
+            load(j, at, true, v_ring + b * TILE, &ctrl->v_full[b]);
             at = next;
         }
-    } else if (warp == 8) {
-        // ---- products
+    } else if (warp == W_MMA) {
+        // ---- products: for each tile in turn, O of the step before, then S of this one.  They run in the order of their
+        // issue: S may be written where p is still being read.
         if (lane == 0 && n_tiles) {
             constexpr uint32_t s_desc = mma_desc<T>(128, TC_KEYS, false, false), o_desc = mma_desc<T>(128, D, false, true);
-            bool fine = ws.wait(smem_u32(&ctrl->q_full), 0, 3);
+            bool fine = ws.wait(smem_u32(&ctrl->q_full[0]), 0, 3) && (!tr[1].rows || ws.wait(smem_u32(&ctrl->q_full[1]), 0, 3));
+            int done[2] = {0, 0};                                      // steps whose O has been issued
+            bool used[2] = {false, false};                             // by the step before
             for (int j = 0; j <= n_tiles && fine; j++) {
-                if (j) {
-                    fine = ws.wait(smem_u32(&ctrl->p_full), j - 1, 4) && ws.wait(smem_u32(&ctrl->v_full), j - 1, 5);
-                    if (!fine) break;
-                    tc_fence_after();
-                    // keys behind the last block of the range take no part: their rows of V were never written
-                    const int steps = min(TC_KEYS, n_keys - (j - 1) * TC_KEYS) / 16;
+                const int kb = j % STAGES, vb = j ? (j - 1) % STAGES : 0;
+                const uint32_t k_tile = k_ring + kb * TILE, v_tile = v_ring + vb * TILE;
+                if (j) fine = ws.wait(smem_u32(&ctrl->v_full[vb]), (j - 1) / STAGES, 5);
 #pragma unroll
-                    for (int ks = 0; ks < TC_KEYS / 16; ks++)
-                        if (ks < steps) mma_ts(tmem_o, tmem + (ks >> 2) * TC_HALF + (ks & 3) * 8, desc_mn_major(v_tile, 128, ks), o_desc, j > 1 || ks);
-                    umma_commit(smem_u32(&ctrl->v_empty));
-                    umma_commit(smem_u32(&ctrl->pv_done));
-                }
-                if (j < n_tiles) {
-                    // products of one block run in order: S may be written where p is still being read
-                    fine = ws.wait(smem_u32(&ctrl->k_full), j, 6);
-                    if (!fine) break;
-                    tc_fence_after();
+                for (int x = 0; x < TILES && fine; x++) {
+                    if (used[x]) {
+                        fine = ws.wait(smem_u32(&ctrl->p_full[x]), done[x], 4);
+                        if (!fine) break;
+                        tc_fence_after();
+                        // keys behind the last block of the range take no part: their rows of V were never written
+                        const int steps = min(TC_KEYS, n_keys - (j - 1) * TC_KEYS) / 16;
 #pragma unroll
-                    for (int ks = 0; ks < D / 16; ks++)
-                        mma_ss(tmem, desc_k_major(q_tile, 128, ks), desc_k_major(k_tile, 128, ks), s_desc, ks != 0);
-                    umma_commit(smem_u32(&ctrl->k_empty));
-                    umma_commit(smem_u32(&ctrl->s_full));
+                        for (int ks = 0; ks < TC_KEYS / 16; ks++)
+                            if (ks < steps)
+                                mma_ts(tmem_o + x * 128, tmem + x * TC_KEYS + (ks >> 2) * TC_HALF + (ks & 3) * 8, desc_mn_major(v_tile, 128, ks), o_desc, done[x] || ks);
+                        umma_commit(smem_u32(&ctrl->pv_done[x]));
+                        done[x]++;
+                    }
+                    if (x == 0 && j < n_tiles) fine = ws.wait(smem_u32(&ctrl->k_full[kb]), j / STAGES, 6);
+                    if (!fine) break;
+                    used[x] = j < n_tiles && uses(x, j);
+                    if (used[x]) {
+                        tc_fence_after();
+#pragma unroll
+                        for (int ks = 0; ks < D / 16; ks++)
+                            mma_ss(tmem + x * TC_KEYS, desc_k_major(q_tiles + x * TILE, 128, ks), desc_k_major(k_tile, 128, ks), s_desc, ks != 0);
+                        umma_commit(smem_u32(&ctrl->s_full[x]));
+                    }
                 }
+                if (fine && j) umma_commit(smem_u32(&ctrl->v_empty[vb]));
+                if (fine && j < n_tiles) umma_commit(smem_u32(&ctrl->k_empty[kb]));
             }
         }
         __syncwarp();
     } else {
-        // ---- softmax: two threads for a row, each half of the keys
-        for (int i = 0; i < D / 16; i++) {
-            const int x = i * TC_SOFTMAX + tid, qr = x / (D / 8), c = x % (D / 8);
-            const bool ok = qr < rows;
-            const int qy = tr.row0 + (ok ? qr : 0);
-            const int64_t off = (int64_t)(sq.row0 + qy / G) * a.q_token + (int64_t)(h * G + qy % G) * a.q_head;
-            cp_async16(q_tile + panel_off(128, qr, c), static_cast<const T *>(a.d_q) + off + c * 8, ok);
-        }
-        cp_commit();
-        const int r = tid & 127, half = warp >> 2, quad = warp & 3;
-        const int y = tr.row0 + min(r, rows - 1);
-        const int limit = attn_limit(a, sq, sq.pos0 + y / G);
-        const uint32_t my_bit = a.n_select ? 1u << (y / G / a.query_block - tr.qb0) : 1u;
-        const uint32_t all_bits = tr.n_qb == 32 ? ~0u : (1u << tr.n_qb) - 1;
-        const float scale2 = a.scale * LOG2E;
-        const uint32_t lane_s = tmem + ((uint32_t)(quad * 32) << 16) + half * TC_HALF;
-        const uint32_t lane_o = tmem_o + ((uint32_t)(quad * 32) << 16) + half * (D / 2);
-        const uint32_t met = smem_u32(&ctrl->met[quad]);
+        // ---- softmax: two threads for a row of the warp's tile, each half of the keys
+        const int x0 = warp >> 3, half = warp >> 2 & 1, quad = warp & 3;
+        const TileRows mine = x0 ? tr[1] : tr[0];
+        const int rows = mine.rows;
         cp_wait<0>();
         fence_async_smem();
-        mbar_arrive(smem_u32(&ctrl->q_full));
+        mbar_arrive(smem_u32(&ctrl->q_full[x0]));
+        const int r = tid & 127;
+        const int y = mine.row0 + min(r, max(rows, 1) - 1);
+        const int limit = attn_limit(a, sq, sq.pos0 + y / G), limit_min = attn_limit(a, sq, sq.pos0 + mine.first);
+        const uint32_t my_bit = a.n_select ? 1u << (y / G / a.query_block - mine.qb0) : 1u;
+        const uint32_t all_bits = mine.n_qb == 32 ? ~0u : (1u << mine.n_qb) - 1;
+        const float scale2 = a.scale * LOG2E;
+        const uint32_t lane_s = tmem + ((uint32_t)(quad * 32) << 16) + x0 * TC_KEYS + half * TC_HALF;
+        const uint32_t lane_o = tmem_o + ((uint32_t)(quad * 32) << 16) + x0 * 128 + half * (D / 2);
+        const uint32_t met = smem_u32(&ctrl->met[x0 * 4 + quad]);
         float m = -CUDART_INF_F, l = 0.f;
         bool fine = true;
-        for (int j = 0; j < n_tiles; j++) {
+        int n_done = 0;
+        for (int j = 0; j < n_tiles && rows; j++) {
+            if (!uses(x0, j)) continue;
             // lanes 0..3: position and lists of this half's groups of 16 keys (far behind every limit: none there)
             int group_pos = INT32_MAX / 2;
             uint32_t group_bits = all_bits;
@@ -607,16 +648,15 @@ __global__ __launch_bounds__(TC_THREADS, 2) void attn_tc_kernel(const __grid_con
                 if (e < n_entries) {
                     const int b = block_of(e);
                     group_pos = b * a.block + (key & (a.block - 1));
-                    if (a.n_select) group_bits = bits[e];
+                    if (a.n_select) group_bits = bits[x0 * p.max_entries + e];
                     else if (ctrl->bad_page) {
                         const int page = page_of(b);
                         if (page < 0 || page >= a.n_pages) group_pos = INT32_MAX / 2;
                     }
                 }
             }
-            const bool masked = __any_sync(~0u, lane < TC_HALF / 16 && group_pos > limit_min - 16);
-            const bool partly = __any_sync(~0u, group_bits != all_bits);
-            fine = __all_sync(~0u, ws.wait(smem_u32(&ctrl->s_full), j, 7));
+            const bool masked = __any_sync(~0u, (lane < TC_HALF / 16 && group_pos > limit_min - 16) || group_bits != all_bits);
+            fine = __all_sync(~0u, ws.wait(smem_u32(&ctrl->s_full[x0]), n_done, 7));
             if (!fine) break;
             tc_fence_after();
             uint32_t v[TC_HALF];
@@ -627,18 +667,11 @@ __global__ __launch_bounds__(TC_THREADS, 2) void attn_tc_kernel(const __grid_con
             if (masked) {
 #pragma unroll
                 for (int g = 0; g < TC_HALF / 16; g++) {
-                    const int n = limit - __shfl_sync(~0u, group_pos, g);
+                    const int pos = __shfl_sync(~0u, group_pos, g);
+                    const int n = __shfl_sync(~0u, group_bits, g) & my_bit ? limit - pos : 0;
 #pragma unroll
                     for (int i = 0; i < 16; i++)
                         if (i >= n) v[g * 16 + i] = 0xff800000u;
-                }
-            }
-            if (partly) {
-#pragma unroll
-                for (int g = 0; g < TC_HALF / 16; g++) {
-                    if (!(__shfl_sync(~0u, group_bits, g) & my_bit))
-#pragma unroll
-                        for (int i = 0; i < 16; i++) v[g * 16 + i] = 0xff800000u;
                 }
             }
             float t0 = __uint_as_float(v[0]), t1 = __uint_as_float(v[1]);
@@ -648,17 +681,17 @@ __global__ __launch_bounds__(TC_THREADS, 2) void attn_tc_kernel(const __grid_con
                 t1 = fmaxf(t1, fmaxf(__uint_as_float(v[i + 2]), __uint_as_float(v[i + 3])));
             }
             float top = fmaxf(t0, t1);
-            ctrl->top[j & 1][half][r] = top;
+            ctrl->top[x0][n_done & 1][half][r] = top;
             mbar_arrive(met);
-            fine = __all_sync(~0u, ws.wait(met, j, 10));
+            fine = __all_sync(~0u, ws.wait(met, n_done, 10));
             if (!fine) break;
-            top = fmaxf(top, ctrl->top[j & 1][half ^ 1][r]) * scale2;
+            top = fmaxf(top, ctrl->top[x0][n_done & 1][half ^ 1][r]) * scale2;
             const bool raise = top > m + 8.f || (m == -CUDART_INF_F && top > m);
             if (__any_sync(~0u, raise)) {
                 const float f = raise ? fast_exp2(m - top) : 1.f;
                 if (raise) { m = top; l *= f; }
                 // the products before this S are complete, O is at rest; each thread takes half of its columns
-                if (j) {
+                if (n_done) {
 #pragma unroll 1
                     for (int c = 0; c < D / 32; c++) {
                         uint32_t w[16];
@@ -679,8 +712,9 @@ __global__ __launch_bounds__(TC_THREADS, 2) void attn_tc_kernel(const __grid_con
                 uint32_t w[16];
 #pragma unroll
                 for (int i = 0; i < 16; i++) {
-                    const float2 x = fma2(make_float2(__uint_as_float(v[c * 32 + 2 * i]), __uint_as_float(v[c * 32 + 2 * i + 1])), scale22, minus_m);
-                    const float2 e = make_float2(fast_exp2(x.x), fast_exp2(x.y));
+                    const float2 z = fma2(make_float2(__uint_as_float(v[c * 32 + 2 * i]), __uint_as_float(v[c * 32 + 2 * i + 1])), scale22, minus_m);
+                    // spread evenly, so that both units are busy all the time
+                    const float2 e = i * TC_POLY / 16 != (i + 1) * TC_POLY / 16 ? poly_exp2(z) : make_float2(fast_exp2(z.x), fast_exp2(z.y));
                     sum = add2(sum, e);
                     w[i] = Pack<T>::two(e.x, e.y);
                 }
@@ -689,34 +723,35 @@ __global__ __launch_bounds__(TC_THREADS, 2) void attn_tc_kernel(const __grid_con
             l += sum.x + sum.y;
             tmem_wait_st();
             tc_fence_before();
-            mbar_arrive(smem_u32(&ctrl->p_full));
+            mbar_arrive(smem_u32(&ctrl->p_full[x0]));
+            n_done++;
         }
-        if (n_tiles && fine) fine = __all_sync(~0u, ws.wait(smem_u32(&ctrl->pv_done), n_tiles - 1, 9));
-        tc_fence_after();
-        // the row's sum: both halves (in the same order for both threads)
-        if (n_tiles && fine) {
-            ctrl->top[n_tiles & 1][half][r] = l;
+        if (n_done && fine) {
+            fine = __all_sync(~0u, ws.wait(smem_u32(&ctrl->pv_done[x0]), n_done - 1, 9));
+            // the row's sum: both halves, in the same order for both threads
+            ctrl->top[x0][n_done & 1][half][r] = l;
             mbar_arrive(met);
-            fine = __all_sync(~0u, ws.wait(met, n_tiles, 11));
-            l = ctrl->top[n_tiles & 1][0][r] + ctrl->top[n_tiles & 1][1][r];
+            fine = fine && __all_sync(~0u, ws.wait(met, n_done, 11));
+            l = ctrl->top[x0][n_done & 1][0][r] + ctrl->top[x0][n_done & 1][1][r];
         }
+        tc_fence_after();
         const float inv = l == 0.f ? 0.f : 1.f / l;
         const float lse2 = l == 0.f ? -CUDART_INF_F : (m == -CUDART_INF_F ? 0.f : m) + log2f(l);
         const int64_t row = sq.row0 + y / G;
         const int head = h * G + y % G;
         const int64_t at = (row * a.heads + head) * p.n_split + split;
 #pragma unroll 1
-        for (int c = 0; c < D / 64; c++) {
+        for (int c = 0; c < D / 64 && rows; c++) {
             uint32_t v[32];
             const int d0 = half * (D / 2) + c * 32;
-            if (n_tiles) {
+            if (n_done) {
                 tmem_ld32(lane_o + c * 32, v);
                 tmem_wait_ld();
                 tmem_landed<32>(v);
             }
 #pragma unroll
             for (int i = 0; i < 32; i++)
-                v[i] = !fine ? 0x7fc00000u : n_tiles ? __float_as_uint(__uint_as_float(v[i]) * inv) : 0u;
+                v[i] = !fine ? 0x7fc00000u : n_done ? __float_as_uint(__uint_as_float(v[i]) * inv) : 0u;
             if (r < rows) {
                 if (p.n_split == 1) {
                     T *dst = static_cast<T *>(a.d_o) + row * a.o_token + head * a.o_head + d0;
@@ -740,11 +775,11 @@ __global__ __launch_bounds__(TC_THREADS, 2) void attn_tc_kernel(const __grid_con
         tc_fence_before();
     }
     __syncthreads();
-    if (warp == 8) {
+    if (warp == W_MMA) {
         if (ctrl->abort_flag) drain_products();
         __syncwarp();
         tc_fence_after();
-        tmem_free<TC_COLS>(tmem);
+        tmem_free<COLS>(tmem);
     }
 }
 
@@ -864,13 +899,16 @@ static bool use_tc(const spamm_attn &a) { return (int64_t)a.max_q * (a.heads / a
 
 static RowsPlan rows_plan(const spamm_attn &a)
 {
-    RowsPlan p;
+    RowsPlan p{};
     const int G = a.heads / a.kv_heads;
     const bool tc = use_tc(a);
     if (tc) {
         p.bq = 0;
         p.nqb = 1;
-        p.tiles = attn_tiles(a);
+        // pairs of tiles once they fill the 148 SMs twice over
+        p.tiles = ceil_div(attn_tiles(a), 2);
+        p.pairs = (int64_t)a.batch * a.kv_heads * p.tiles >= 2 * 148 || !a.n_select;
+        if (!p.pairs) p.tiles = attn_tiles(a);
     } else {
         p.bq = a.n_select ? min(a.query_block, a.max_q) : a.max_q;
         p.nqb = ceil_div(a.max_q, p.bq);
@@ -879,14 +917,15 @@ static RowsPlan rows_plan(const spamm_attn &a)
     // tiles of 128 rows cut the sequence's blocks into ranges (they look through the lists for those in theirs), tiles of
     // 16 rows the list
     const int64_t blocks = max((int64_t)1, tc ? (int64_t)attn_max_blocks(a) : longest_list(a));
-    const int64_t most = !tc ? SPAMM_ATTN_MAX_SELECT : a.n_select ? UNION_BLOCKS : blocks;
+    const int64_t listed = (int64_t)(p.pairs ? 2 : 1) * attn_tile_lists(a) * a.n_select;       // blocks of a union
+    const int64_t most = !tc ? SPAMM_ATTN_MAX_SELECT : !a.n_select ? blocks : listed <= TC_ENTRIES ? UNION_BLOCKS : TC_ENTRIES;
     const int64_t units = (int64_t)a.batch * a.kv_heads * p.nqb * p.tiles;
     // enough blocks of threads to fill 148 SMs several times over, ranges of 1024 (256) keys at the least
-    int64_t want = (tc ? a.n_select ? 148 : 1200 : 600) / units + 1;
+    int64_t want = (tc ? a.n_select ? 148 : 740 : 600) / units + 1;
     want = max((int64_t)1, min(want, (blocks * a.block + (tc ? 1023 : 255)) / (tc ? 1024 : 256)));
     int64_t per = min(most, (blocks + want - 1) / want);
     p.n_split = (int)((blocks + per - 1) / per);
-    p.max_entries = (int)(tc && a.n_select ? min(per, (int64_t)attn_tile_lists(a) * a.n_select) : per);
+    p.max_entries = (int)(tc && a.n_select ? min(per, listed) : per);
     p.split_keys = (int)(per * a.block);
     return p;
 }
@@ -907,12 +946,14 @@ static int forward_launch(const spamm_attn &a, float *scratch, cudaStream_t stre
     float *part_o = scratch;
     float *part_lse = scratch + (size_t)a.tokens * a.heads * p.n_split * D;
     if (use_tc(a)) {
-        const size_t smem = 3 * TC_ROWS * D * 2 + sizeof(TcCtrl) + (a.n_select ? 6 * (size_t)p.max_entries : 0);
-        int st = attn_set_smem((const void *)attn_tc_kernel<T, D>, smem);
+        const int tiles = p.pairs ? 2 : 1;
+        const size_t smem = tiles * 3 * TC_ROWS * D * 2 + sizeof(TcCtrl) + (a.n_select ? (4 * tiles + 2) * (size_t)p.max_entries : 0);
+        const auto kernel = p.pairs ? attn_tc_kernel<T, D, 2> : attn_tc_kernel<T, D, 1>;
+        int st = attn_set_smem((const void *)kernel, smem);
         if (st) return st;
         RowMap k_map, v_map;
         attn_row_maps(a, a.block, &k_map, &v_map);
-        attn_tc_kernel<T, D><<<(unsigned)grid, TC_THREADS, smem, stream>>>(a, p, k_map, v_map, part_o, part_lse);
+        kernel<<<(unsigned)grid, tiles * 256 + 64, smem, stream>>>(a, p, k_map, v_map, part_o, part_lse);
     } else {
         const size_t smem = rows_smem(a, p);
         int st = attn_set_smem((const void *)attn_rows_kernel<T, D>, smem);

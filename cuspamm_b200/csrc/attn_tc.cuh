@@ -132,10 +132,10 @@ __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.a
 // tile; a bit for each of them says which rows a block of keys counts for.  Neighbouring queries share most of their blocks,
 // and where they do not, the union is still never more to copy than the lists one by one.
 constexpr int UNION_LISTS = 32;
-constexpr int UNION_BLOCKS = 8192;           // blocks of keys that a tile's union is built over at a time
+constexpr int UNION_BLOCKS = 8192;           // blocks of keys that a union is built over at a time
 
 struct TileRows {
-    int rows;                 // of the tile
+    int rows;                 // of the tile; 0: there is none
     int row0;                 // first of the sequence's rows (query * G + head)
     int first, last;          // its first and last query
     int qb0, n_qb;            // its query blocks
@@ -154,60 +154,71 @@ __host__ __device__ inline int attn_tiles(const spamm_attn &a)
 // Lists that meet in a tile, at most.
 inline int attn_tile_lists(const spamm_attn &a)
 {
-    const int64_t per = (int64_t)a.query_block * (a.heads / a.kv_heads);
-    const int64_t n = attn_tile_rows(a) % per == 0 || per % attn_tile_rows(a) == 0 ? (attn_tile_rows(a) + per - 1) / per
-                                                                                    : (attn_tile_rows(a) + per - 1) / per + 1;
+    const int64_t per = (int64_t)a.query_block * (a.heads / a.kv_heads), rows = attn_tile_rows(a);
+    const int64_t n = (rows + per - 1) / per + (rows % per && per % rows ? 1 : 0);
     return (int)(n < UNION_LISTS ? n : UNION_LISTS);
 }
-// False when the tile has no rows.
-__device__ __forceinline__ bool attn_tile(const spamm_attn &a, const Seq &sq, int tile, TileRows *t)
+__device__ __forceinline__ TileRows attn_tile(const spamm_attn &a, const Seq &sq, int tile)
 {
+    TileRows t{};
     const int G = a.heads / a.kv_heads, per_tile = attn_tile_rows(a);
     const int64_t all = (int64_t)sq.nq * G, row0 = (int64_t)tile * per_tile;
-    if (row0 >= all) return false;
-    t->rows = (int)min((int64_t)per_tile, all - row0);
-    t->row0 = (int)row0;
-    t->first = (int)(row0 / G);
-    t->last = (int)((row0 + t->rows - 1) / G);
-    t->qb0 = a.n_select ? t->first / a.query_block : 0;
-    t->n_qb = a.n_select ? t->last / a.query_block - t->qb0 + 1 : 1;
-    return true;
+    if (row0 >= all) return t;
+    t.rows = (int)min((int64_t)per_tile, all - row0);
+    t.row0 = (int)row0;
+    t.first = (int)(row0 / G);
+    t.last = (int)((row0 + t.rows - 1) / G);
+    t.qb0 = a.n_select ? t.first / a.query_block : 0;
+    t.n_qb = a.n_select ? t.last / a.query_block - t.qb0 + 1 : 1;
+    return t;
 }
-// The union of the tile's lists within the blocks [b0, b1): idx[e] = block - b0, ascending, bits[e] = the lists that have
-// it.  `marks`: room for b1 - b0 words that nothing else uses until the return.  All threads call; `count` is shared.
-// (Room of idx and bits: the sum of the lists' lengths, or b1 - b0.)
-template <int THREADS>
-__device__ __forceinline__ int attn_union(const spamm_attn &a, const Seq &sq, int s, int h, const TileRows &t, int b0, int b1,
-                                          uint32_t *marks, uint16_t *idx, uint32_t *bits, int *count)
+// The union of the lists of TILES tiles within the blocks [b0, b1): idx[e] = block - b0, ascending, bits[t * room + e] = the
+// lists of tile t that have it.  `marks`: room for TILES * (b1 - b0) words that nothing else uses until the return.  All
+// threads call; `count` is shared.  room: the sum of the lists' lengths, or b1 - b0.
+template <int THREADS, int TILES>
+__device__ __forceinline__ int attn_union(const spamm_attn &a, const Seq &sq, int s, int h, const TileRows *t, int b0, int b1,
+                                          uint32_t *marks, uint16_t *idx, uint32_t *bits, int room, int *count)
 {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n = b1 - b0;
     const int nqb = ceil_div(a.max_q, a.query_block);
-    for (int i = tid; i < n; i += THREADS) marks[i] = 0;
+    for (int i = tid; i < TILES * n; i += THREADS) marks[i] = 0;
     __syncthreads();
-    for (int q = warp; q < t.n_qb; q += THREADS / 32) {
-        const int qb = t.qb0 + q;
-        const int last = (int)min((int64_t)(qb + 1) * a.query_block, (int64_t)sq.nq) - 1;
-        attn_for_list(a, s, qb, nqb, h, ceil_div(attn_limit(a, sq, sq.pos0 + last), a.block), lane, [&](int v, int) {
-            if (v >= b0 && v < b1) atomicOr(marks + v - b0, 1u << q);
-        });
+    int q0 = 0;
+#pragma unroll
+    for (int x = 0; x < TILES; x++) {
+        if (t[x].rows)
+            for (int q = (warp + THREADS / 32 - q0 % (THREADS / 32)) % (THREADS / 32); q < t[x].n_qb; q += THREADS / 32) {
+                const int qb = t[x].qb0 + q;
+                const int last = (int)min((int64_t)(qb + 1) * a.query_block, (int64_t)sq.nq) - 1;
+                attn_for_list(a, s, qb, nqb, h, ceil_div(attn_limit(a, sq, sq.pos0 + last), a.block), lane, [&](int v, int) {
+                    if (v >= b0 && v < b1) atomicOr(marks + x * n + v - b0, 1u << q);
+                });
+            }
+        q0 += t[x].n_qb;
     }
     __syncthreads();
     if (warp == 0) {
         int found = 0;
         for (int i0 = 0; i0 < n; i0 += 32) {
-            uint32_t m = i0 + lane < n ? marks[i0 + lane] : 0;
-            if (m && a.n_pages) {
+            uint32_t m[TILES], any = 0;
+#pragma unroll
+            for (int x = 0; x < TILES; x++) {
+                m[x] = i0 + lane < n ? marks[x * n + i0 + lane] : 0;
+                any |= m[x];
+            }
+            if (any && a.n_pages) {
                 const int page = a.d_table[(int64_t)s * a.table_stride + b0 + i0 + lane];
                 if (page < 0 || page >= a.n_pages) {
-                    m = 0;
+                    any = 0;
                     *a.d_status = SPAMM_ERR_INVALID;
                 }
             }
-            const unsigned there = __ballot_sync(~0u, m != 0);
+            const unsigned there = __ballot_sync(~0u, any != 0);
             const int at = found + __popc(there & ((1u << lane) - 1));
-            if (m) {
+            if (any) {
                 idx[at] = (uint16_t)(i0 + lane);
-                bits[at] = m;
+#pragma unroll
+                for (int x = 0; x < TILES; x++) bits[x * room + at] = m[x];
             }
             found += __popc(there);
         }
@@ -222,19 +233,50 @@ __device__ __forceinline__ int attn_union(const spamm_attn &a, const Seq &sq, in
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c)
 {
     float2 d;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;"
-        : "=l"(*reinterpret_cast<unsigned long long *>(&d))
-        : "l"(*reinterpret_cast<unsigned long long *>(&a)), "l"(*reinterpret_cast<unsigned long long *>(&b)),
-          "l"(*reinterpret_cast<unsigned long long *>(&c)));
+    asm("{\n\t.reg .b64 a, b, c, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
+        "fma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
     return d;
 }
 __device__ __forceinline__ float2 add2(float2 a, float2 b)
 {
     float2 d;
-    asm("add.rn.f32x2 %0, %1, %2;"
-        : "=l"(*reinterpret_cast<unsigned long long *>(&d))
-        : "l"(*reinterpret_cast<unsigned long long *>(&a)), "l"(*reinterpret_cast<unsigned long long *>(&b)));
+    asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tadd.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
     return d;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b)
+{
+    float2 d;
+    asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmul.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+__device__ __forceinline__ float max_nan(float a, float b)
+{
+    float d;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+    return d;
+}
+// 2^x for two values below 128 without the special-function unit, which gives four results a clock and scheduler and would
+// bound the softmax: x = n + r with r in [-1/2, 1/2] (n by adding and subtracting 1.5 * 2^23, whose sum has n in its low
+// bits), 2^r by the polynomial of degree 4 with the smallest largest relative error there (2.7e-6, a Remez exchange), 2^n put
+// together as bits.  At and below -127 the result is zero, and a NaN stays one.
+__device__ __forceinline__ float2 poly_exp2(float2 x)
+{
+    const float2 magic = make_float2(12582912.f, 12582912.f), back = make_float2(-12582912.f, -12582912.f);
+    x.x = max_nan(x.x, -127.f);
+    x.y = max_nan(x.y, -127.f);
+    const float2 t = add2(x, magic);
+    const float2 n = add2(t, back);
+    const float2 r = fma2(n, make_float2(-1.f, -1.f), x);
+    float2 p = fma2(make_float2(0.009570102207362652f, 0.009570102207362652f), r, make_float2(0.05591785907745361f, 0.05591785907745361f));
+    p = fma2(p, r, make_float2(0.240247443318367f, 0.240247443318367f));
+    p = fma2(p, r, make_float2(0.6931217908859253f, 0.6931217908859253f));
+    p = fma2(p, r, make_float2(0.9999992847442627f, 0.9999992847442627f));
+    const float2 s = make_float2(__uint_as_float((__float_as_uint(t.x) << 23) + 0x3f800000u),
+                                 __uint_as_float((__float_as_uint(t.y) << 23) + 0x3f800000u));
+    return mul2(p, s);
 }
 
 // Barriers of a kernel and its abort flag: a wait that runs out (never, unless the kernel is wrong) sets the flag, every
