@@ -618,7 +618,7 @@ __global__ __launch_bounds__(TQ_THREADS, 2) void attn_dq_tc_kernel(const __grid_
     const int log_block = 31 - __clz(a.block);
     const int n_keys = n_entries << log_block;
     const int n_tiles = (n_keys + TQ_KEYS - 1) / TQ_KEYS;
-    const uint32_t tmem = ctrl->tmem_base, tmem_dp = tmem + TQ_KEYS, tmem_dq = tmem + 2 * TQ_KEYS;
+    const uint32_t tmem = ctrl->tmem_base, tmem_dq = tmem + 2 * TQ_KEYS;
     const WaitState ws{&ctrl->abort_flag, &ctrl->err};
 
     if (warp == 9) {
@@ -667,32 +667,42 @@ __global__ __launch_bounds__(TQ_THREADS, 2) void attn_dq_tc_kernel(const __grid_
             load(j, v_tile, true, &ctrl->v_full);
         }
     } else if (warp == 8) {
-        if (lane == 0 && n_tiles) {
-            constexpr uint32_t s_desc = mma_desc<T>(128, TQ_KEYS, false, false), q_desc = mma_desc<T>(128, D, false, true);
-            bool fine = ws.wait(smem_u32(&ctrl->q_full), 0, 3);
+        if (n_tiles) {
+            constexpr uint32_t s_desc = mma_desc<T>(128, TQ_KEYS, false, false), o_desc = mma_desc<T>(128, D, false, true);
+            const uint32_t base = __shfl_sync(~0u, tmem, 0);
+            const uint64_t q_desc = desc_k_major(q_tile), do_desc = desc_k_major(do_tile), v_desc = desc_k_major(v_tile);
+            const uint64_t k_desc = desc_k_major(k_ring), kt_desc = desc_mn_major(k_ring, TQ_KEYS);
+            bool fine = __all_sync(~0u, ws.wait(smem_u32(&ctrl->q_full), 0, 3));
             for (int j = 0; j < n_tiles && fine; j++) {
-                const uint32_t k_tile = k_ring + (j & 1) * KT;
-                fine = ws.wait(smem_u32(&ctrl->k_full[j & 1]), j >> 1, 4) && ws.wait(smem_u32(&ctrl->v_full), j, 5);
+                const uint32_t stage = (j & 1) * (KT >> 4);
+                fine = __all_sync(~0u, ws.wait(smem_u32(&ctrl->k_full[j & 1]), j >> 1, 4) && ws.wait(smem_u32(&ctrl->v_full), j, 5));
                 if (!fine) break;
                 tc_fence_after();
-                // dP first: the buffer of V comes free the earlier
+                if (elect_one()) {
+                    // dP first: the buffer of V comes free the earlier
 #pragma unroll
-                for (int ks = 0; ks < D / 16; ks++)
-                    mma_ss(tmem_dp, desc_k_major(do_tile, TQ_ROWS, ks), desc_k_major(v_tile, TQ_KEYS, ks), s_desc, ks != 0);
-                umma_commit(smem_u32(&ctrl->v_empty));
+                    for (int ks = 0; ks < D / 16; ks++)
+                        mma_ss(base + TQ_KEYS, do_desc + step_k_major(TQ_ROWS, ks), v_desc + step_k_major(TQ_KEYS, ks), s_desc, ks != 0);
+                    umma_commit(smem_u32(&ctrl->v_empty));
 #pragma unroll
-                for (int ks = 0; ks < D / 16; ks++)
-                    mma_ss(tmem, desc_k_major(q_tile, TQ_ROWS, ks), desc_k_major(k_tile, TQ_KEYS, ks), s_desc, ks != 0);
-                umma_commit(smem_u32(&ctrl->s_full));
-                fine = ws.wait(smem_u32(&ctrl->ds_full), j, 6);
+                    for (int ks = 0; ks < D / 16; ks++)
+                        mma_ss(base, q_desc + step_k_major(TQ_ROWS, ks), k_desc + stage + step_k_major(TQ_KEYS, ks), s_desc, ks != 0);
+                    umma_commit(smem_u32(&ctrl->s_full));
+                }
+                __syncwarp();
+                fine = __all_sync(~0u, ws.wait(smem_u32(&ctrl->ds_full), j, 6));
                 if (!fine) break;
                 tc_fence_after();
                 const int steps = min(TQ_KEYS, n_keys - j * TQ_KEYS) / 16;      // rows of K behind were never written
+                if (elect_one()) {
 #pragma unroll
-                for (int ks = 0; ks < TQ_KEYS / 16; ks++)
-                    if (ks < steps) mma_ts(tmem_dq, tmem + (ks >> 1) * 32 + (ks & 1) * 8, desc_mn_major(k_tile, TQ_KEYS, ks), q_desc, j || ks);
-                umma_commit(smem_u32(&ctrl->k_empty[j & 1]));
-                umma_commit(smem_u32(&ctrl->dq_done));
+                    for (int ks = 0; ks < TQ_KEYS / 16; ks++)
+                        if (ks < steps)
+                            mma_ts(base + 2 * TQ_KEYS, base + (ks >> 1) * 32 + (ks & 1) * 8, kt_desc + stage + step_mn_major(ks), o_desc, j || ks);
+                    umma_commit(smem_u32(&ctrl->k_empty[j & 1]));
+                    umma_commit(smem_u32(&ctrl->dq_done));
+                }
+                __syncwarp();
             }
         }
         __syncwarp();
@@ -965,49 +975,63 @@ __global__ __launch_bounds__(TK_THREADS, 1) void attn_dkv_tc_kernel(const __grid
         cp_wait<0>();
     } else if (warp == 8) {
         // ---- products
-        if (lane == 0 && n_tiles) {
+        if (n_tiles) {
             constexpr uint32_t s_desc = mma_desc<T>(128, TK_KEYS, false, false), o_desc = mma_desc<T>(128, TK_KEYS, true, true);
-            bool fine = ws.wait(smem_u32(&ctrl->kv_full), 0, 2);
+            const uint32_t base = __shfl_sync(~0u, tmem, 0);
+            const uint64_t k_desc = desc_k_major(k_tile), v_desc = desc_k_major(v_tile), do_desc = desc_k_major(ring), q_desc = desc_k_major(ring + RT);
+            // A of the second products: 128 values of dO (of Q) x 128 rows; with D = 64 the tiles of dO and Q one behind the other
+            const uint64_t dot_desc = desc_mn_major(ring, TK_ROWS), qt_desc = desc_mn_major(D == 64 ? ring : ring + RT, TK_ROWS);
+            const uint64_t p_desc = desc_mn_major(p_tile, TK_ROWS), ds_desc = desc_mn_major(ds_tile, TK_ROWS);
+            bool fine = __all_sync(~0u, ws.wait(smem_u32(&ctrl->kv_full), 0, 2));
             // whichever of the two is ready: the first products of the next tile, when its rows are there and at most one
             // tile is under way, or the second products of the oldest tile under way.  (In a fixed order the second
             // products would wait for the copies of the next tile, which wait for their buffer, which they free.)
             int first = 0, second = 0;
             unsigned long long t0 = 0;
             while (second < n_tiles) {
-                if (first < n_tiles && first - second < 2 && mbar_test(smem_u32(&ctrl->r_full[first & 1]), (first >> 1) & 1)) {
+                if (first < n_tiles && first - second < 2 &&
+                    __all_sync(~0u, mbar_test(smem_u32(&ctrl->r_full[first & 1]), (first >> 1) & 1))) {
                     tc_fence_after();
-                    const uint32_t do_tile = ring + (first & 1) * 2 * RT, q_tile = do_tile + RT, s_at = tmem + (first & 1) * 2 * TK_KEYS;
+                    const uint32_t stage = (first & 1) * (2 * RT >> 4), s_at = base + (first & 1) * 2 * TK_KEYS;
+                    if (elect_one()) {
 #pragma unroll
-                    for (int ks = 0; ks < D / 16; ks++)
-                        mma_ss(s_at, desc_k_major(q_tile, TK_ROWS, ks), desc_k_major(k_tile, TK_KEYS, ks), s_desc, ks != 0);
+                        for (int ks = 0; ks < D / 16; ks++)
+                            mma_ss(s_at, q_desc + stage + step_k_major(TK_ROWS, ks), k_desc + step_k_major(TK_KEYS, ks), s_desc, ks != 0);
 #pragma unroll
-                    for (int ks = 0; ks < D / 16; ks++)
-                        mma_ss(s_at + TK_KEYS, desc_k_major(do_tile, TK_ROWS, ks), desc_k_major(v_tile, TK_KEYS, ks), s_desc, ks != 0);
-                    umma_commit(smem_u32(&ctrl->s_full[first & 1]));
+                        for (int ks = 0; ks < D / 16; ks++)
+                            mma_ss(s_at + TK_KEYS, do_desc + stage + step_k_major(TK_ROWS, ks), v_desc + step_k_major(TK_KEYS, ks), s_desc, ks != 0);
+                        umma_commit(smem_u32(&ctrl->s_full[first & 1]));
+                    }
+                    __syncwarp();
                     first++;
                     t0 = 0;
-                } else if (second < first && mbar_test(smem_u32(&ctrl->p_full), second & 1)) {
-                    // A: 128 values of dO (of Q) x 128 rows; with D = 64 the tiles of dO and Q one behind the other
-                    const uint32_t do_tile = ring + (second & 1) * 2 * RT, q_tile = D == 64 ? do_tile : do_tile + RT;
+                } else if (second < first && __all_sync(~0u, mbar_test(smem_u32(&ctrl->p_full), second & 1))) {
                     tc_fence_after();
+                    const uint32_t stage = (second & 1) * (2 * RT >> 4);
+                    if (elect_one()) {
 #pragma unroll
-                    for (int ks = 0; ks < TK_ROWS / 16; ks++)
-                        mma_ss(tmem_dv, desc_mn_major(do_tile, TK_ROWS, ks), desc_mn_major(p_tile, TK_ROWS, ks), o_desc, second || ks);
-                    umma_commit(smem_u32(&ctrl->dv_done));
-                    fine = ws.wait(smem_u32(&ctrl->ds_full), second, 5);
+                        for (int ks = 0; ks < TK_ROWS / 16; ks++)
+                            mma_ss(base + 4 * TK_KEYS, dot_desc + stage + step_mn_major(ks), p_desc + step_mn_major(ks), o_desc, second || ks);
+                        umma_commit(smem_u32(&ctrl->dv_done));
+                    }
+                    __syncwarp();
+                    fine = __all_sync(~0u, ws.wait(smem_u32(&ctrl->ds_full), second, 5));
                     if (!fine) break;
                     tc_fence_after();
+                    if (elect_one()) {
 #pragma unroll
-                    for (int ks = 0; ks < TK_ROWS / 16; ks++)
-                        mma_ss(tmem_dk, desc_mn_major(q_tile, TK_ROWS, ks), desc_mn_major(ds_tile, TK_ROWS, ks), o_desc, second || ks);
-                    umma_commit(smem_u32(&ctrl->r_empty[second & 1]));
-                    umma_commit(smem_u32(&ctrl->dk_done));
+                        for (int ks = 0; ks < TK_ROWS / 16; ks++)
+                            mma_ss(base + 5 * TK_KEYS, qt_desc + stage + step_mn_major(ks), ds_desc + step_mn_major(ks), o_desc, second || ks);
+                        umma_commit(smem_u32(&ctrl->r_empty[second & 1]));
+                        umma_commit(smem_u32(&ctrl->dk_done));
+                    }
+                    __syncwarp();
                     second++;
                     t0 = 0;
                 } else {
-                    if (!fine || ctrl->abort_flag) break;
+                    if (__any_sync(~0u, !fine || ctrl->abort_flag)) break;
                     if (!t0) t0 = global_ns();
-                    else if (global_ns() - t0 > WAIT_LIMIT_NS) {
+                    if (__any_sync(~0u, global_ns() - t0 > WAIT_LIMIT_NS)) {
                         *ws.abort_flag = 1;
                         break;
                     }

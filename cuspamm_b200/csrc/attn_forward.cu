@@ -578,43 +578,57 @@ __global__ __launch_bounds__(TILES * 256 + 64, TILES == 1 ? 2 : 1) void attn_tc_
     } else if (warp == W_MMA) {
         // ---- products: for each tile in turn, O of the step before, then S of this one.  They run in the order of their
         // issue: S may be written where p is still being read.
-        if (lane == 0 && n_tiles) {
+        if (n_tiles) {
             constexpr uint32_t s_desc = mma_desc<T>(128, TC_KEYS, false, false), o_desc = mma_desc<T>(128, D, false, true);
-            bool fine = ws.wait(smem_u32(&ctrl->q_full[0]), 0, 3) && (!tr[1].rows || ws.wait(smem_u32(&ctrl->q_full[1]), 0, 3));
+            const uint32_t base = __shfl_sync(~0u, tmem, 0);
+            const uint64_t q_desc = desc_k_major(q_tiles), k_desc = desc_k_major(k_ring), v_desc = desc_mn_major(v_ring, 128);
+            bool fine = __all_sync(~0u, ws.wait(smem_u32(&ctrl->q_full[0]), 0, 3) && (!tr[1].rows || ws.wait(smem_u32(&ctrl->q_full[1]), 0, 3)));
             int done[2] = {0, 0};                                      // steps whose O has been issued
             bool used[2] = {false, false};                             // by the step before
             for (int j = 0; j <= n_tiles && fine; j++) {
                 const int kb = j % STAGES, vb = j ? (j - 1) % STAGES : 0;
-                const uint32_t k_tile = k_ring + kb * TILE, v_tile = v_ring + vb * TILE;
-                if (j) fine = ws.wait(smem_u32(&ctrl->v_full[vb]), (j - 1) / STAGES, 5);
+                if (j) fine = __all_sync(~0u, ws.wait(smem_u32(&ctrl->v_full[vb]), (j - 1) / STAGES, 5));
+                // keys behind the last block of the range take no part: their rows of V were never written
+                const int steps = min(TC_KEYS, n_keys - (j - 1) * TC_KEYS) / 16;
 #pragma unroll
                 for (int x = 0; x < TILES && fine; x++) {
+                    const bool use = j < n_tiles && uses(x, j);
                     if (used[x]) {
-                        fine = ws.wait(smem_u32(&ctrl->p_full[x]), done[x], 4);
+                        fine = __all_sync(~0u, ws.wait(smem_u32(&ctrl->p_full[x]), done[x], 4));
                         if (!fine) break;
                         tc_fence_after();
-                        // keys behind the last block of the range take no part: their rows of V were never written
-                        const int steps = min(TC_KEYS, n_keys - (j - 1) * TC_KEYS) / 16;
+                        const uint64_t vd = v_desc + vb * (TILE >> 4);
+                        if (elect_one()) {
 #pragma unroll
-                        for (int ks = 0; ks < TC_KEYS / 16; ks++)
-                            if (ks < steps)
-                                mma_ts(tmem_o + x * 128, tmem + x * TC_KEYS + (ks >> 2) * TC_HALF + (ks & 3) * 8, desc_mn_major(v_tile, 128, ks), o_desc, done[x] || ks);
-                        umma_commit(smem_u32(&ctrl->pv_done[x]));
+                            for (int ks = 0; ks < TC_KEYS / 16; ks++)
+                                if (ks < steps)
+                                    mma_ts(base + (TILES * TC_KEYS + x * 128), base + x * TC_KEYS + (ks >> 2) * TC_HALF + (ks & 3) * 8,
+                                           vd + step_mn_major(ks), o_desc, done[x] || ks);
+                            umma_commit(smem_u32(&ctrl->pv_done[x]));
+                        }
+                        __syncwarp();
                         done[x]++;
                     }
-                    if (x == 0 && j < n_tiles) fine = ws.wait(smem_u32(&ctrl->k_full[kb]), j / STAGES, 6);
+                    if (x == 0 && j < n_tiles) fine = __all_sync(~0u, ws.wait(smem_u32(&ctrl->k_full[kb]), j / STAGES, 6));
                     if (!fine) break;
-                    used[x] = j < n_tiles && uses(x, j);
-                    if (used[x]) {
+                    if (use) {
                         tc_fence_after();
+                        const uint64_t qd = q_desc + x * (TILE >> 4), kd = k_desc + kb * (TILE >> 4);
+                        if (elect_one()) {
 #pragma unroll
-                        for (int ks = 0; ks < D / 16; ks++)
-                            mma_ss(tmem + x * TC_KEYS, desc_k_major(q_tiles + x * TILE, 128, ks), desc_k_major(k_tile, 128, ks), s_desc, ks != 0);
-                        umma_commit(smem_u32(&ctrl->s_full[x]));
+                            for (int ks = 0; ks < D / 16; ks++)
+                                mma_ss(base + x * TC_KEYS, qd + step_k_major(128, ks), kd + step_k_major(128, ks), s_desc, ks != 0);
+                            umma_commit(smem_u32(&ctrl->s_full[x]));
+                        }
+                        __syncwarp();
                     }
+                    used[x] = use;
                 }
-                if (fine && j) umma_commit(smem_u32(&ctrl->v_empty[vb]));
-                if (fine && j < n_tiles) umma_commit(smem_u32(&ctrl->k_empty[kb]));
+                if (fine && elect_one()) {
+                    if (j) umma_commit(smem_u32(&ctrl->v_empty[vb]));
+                    if (j < n_tiles) umma_commit(smem_u32(&ctrl->k_empty[kb]));
+                }
+                __syncwarp();
             }
         }
         __syncwarp();

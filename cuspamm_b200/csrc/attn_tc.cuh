@@ -15,17 +15,27 @@ __device__ __forceinline__ uint32_t panel_off(int rows, int r, int c)
 }
 
 constexpr uint32_t DESC_HI = (1024u >> 4) | (1u << 14) | (2u << 29);     // 8-row groups 1024 bytes apart, 128-byte swizzle
-// Rows are M or N; K step ks of 16 values.
-__device__ __forceinline__ uint64_t desc_k_major(uint32_t tile, int rows, int ks)
+// Descriptor of a tile whose rows are M or N, and what K step ks of 16 values adds to it.
+__device__ __forceinline__ uint64_t desc_k_major(uint32_t tile)
 {
-    const uint32_t addr = tile + (ks >> 2) * (rows * 128) + (ks & 3) * 32;
-    return ((uint64_t)DESC_HI << 32) | ((addr & 0x3ffffu) >> 4) | (1u << 16);
+    return ((uint64_t)DESC_HI << 32) | ((tile & 0x3ffffu) >> 4) | (1u << 16);
 }
-// Rows are K; K step ks of 16 rows; panels of 64 values of M or N lie rows * 128 bytes apart.
-__device__ __forceinline__ uint64_t desc_mn_major(uint32_t tile, int rows, int ks)
+__host__ __device__ constexpr uint32_t step_k_major(int rows, int ks) { return ((ks >> 2) * (rows * 128) + (ks & 3) * 32) >> 4; }
+// The same for a tile whose rows are K (steps of 16 rows); panels of 64 values of M or N lie rows * 128 bytes apart.
+__device__ __forceinline__ uint64_t desc_mn_major(uint32_t tile, int rows)
 {
-    const uint32_t addr = tile + ks * 2048;
-    return ((uint64_t)DESC_HI << 32) | ((addr & 0x3ffffu) >> 4) | ((uint32_t)(rows * 128) >> 4 << 16);
+    return ((uint64_t)DESC_HI << 32) | ((tile & 0x3ffffu) >> 4) | ((uint32_t)(rows * 128) >> 4 << 16);
+}
+__host__ __device__ constexpr uint32_t step_mn_major(int ks) { return ks * 2048 >> 4; }
+
+// One lane of a converged warp.  The loops that issue products are walked by the whole warp, so that addresses and
+// descriptors stay in uniform registers, and this lane issues: the issuing warp shares its scheduler with the busy ones, and
+// every instruction that it needs for a product delays the next.
+__device__ __forceinline__ bool elect_one()
+{
+    uint32_t ok;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok));
+    return ok != 0;
 }
 
 template <typename T> struct IsBf { static constexpr uint32_t value = 0; };
