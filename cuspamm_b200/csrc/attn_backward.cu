@@ -557,6 +557,9 @@ __global__ __launch_bounds__(KEYS == 128 ? 256 : 128) void attn_dkv_kernel(
 // two blocks of threads share an SM, one's exponentials run beside the other's products.
 constexpr int TQ_ROWS = 128, TQ_KEYS = 64, TQ_SOFTMAX = 256, TQ_THREADS = TQ_SOFTMAX + 64, TQ_COLS = 256;
 
+// Blocks of keys whose marks fit the room of the key tiles.
+template <int D> constexpr int TQ_BLOCKS = 3 * TQ_KEYS * D * 2 / 4 < UNION_BLOCKS ? 3 * TQ_KEYS * D * 2 / 4 : UNION_BLOCKS;
+
 struct TqCtrl {
     uint64_t q_full, k_full[2], k_empty[2], v_full, v_empty, s_full, ds_full, dq_done;
     uint32_t tmem_base;
@@ -592,7 +595,17 @@ __global__ __launch_bounds__(TQ_THREADS, 2) void attn_dq_tc_kernel(const __grid_
     const int rows = tr.rows;
     const int limit_max = attn_limit(a, sq, tr.last), limit_min = attn_limit(a, sq, tr.first);
 
-    if (warp == 8) {
+    if (warp < 8) {
+        for (int i = 0; i < D / 16; i++) {
+            const int x = i * TQ_SOFTMAX + tid, qr = x / (D / 8), c = x % (D / 8);
+            const bool ok = qr < rows;
+            const int qy = tr.row0 + (ok ? qr : 0);
+            const int64_t row = sq.row0 + qy / G, head = h * G + qy % G;
+            cp_async16(q_tile + panel_off(TQ_ROWS, qr, c), static_cast<const T *>(a.d_q) + row * a.q_token + head * a.q_head + c * 8, ok);
+            cp_async16(do_tile + panel_off(TQ_ROWS, qr, c), d_do + row * do_token + head * do_head + c * 8, ok);
+        }
+        cp_commit();
+    } else if (warp == 8) {
         if (lane == 0) {
             mbar_init(smem_u32(&ctrl->q_full), TQ_SOFTMAX);
             for (int i = 0; i < 2; i++) {
@@ -613,7 +626,7 @@ __global__ __launch_bounds__(TQ_THREADS, 2) void attn_dq_tc_kernel(const __grid_
         tc_fence_before();
     }
     const int n_entries = attn_union<TQ_THREADS, 1>(a, sq, s, h, &tr, 0, ceil_div(limit_max, a.block),
-                                                    reinterpret_cast<uint32_t *>(smem), blk, bits, max_entries, &ctrl->count);
+                                                    reinterpret_cast<uint32_t *>(smem + 2 * RT), blk, bits, max_entries, &ctrl->count);
     tc_fence_after();
     const int log_block = 31 - __clz(a.block);
     const int n_keys = n_entries << log_block;
@@ -666,6 +679,7 @@ __global__ __launch_bounds__(TQ_THREADS, 2) void attn_dq_tc_kernel(const __grid_
             if (!fine) break;
             load(j, v_tile, true, &ctrl->v_full);
         }
+        __syncthreads();
     } else if (warp == 8) {
         if (n_tiles) {
             constexpr uint32_t s_desc = mma_desc<T>(128, TQ_KEYS, false, false), o_desc = mma_desc<T>(128, D, false, true);
@@ -706,16 +720,8 @@ __global__ __launch_bounds__(TQ_THREADS, 2) void attn_dq_tc_kernel(const __grid_
             }
         }
         __syncwarp();
+        __syncthreads();
     } else {
-        for (int i = 0; i < D / 16; i++) {
-            const int x = i * TQ_SOFTMAX + tid, qr = x / (D / 8), c = x % (D / 8);
-            const bool ok = qr < rows;
-            const int qy = tr.row0 + (ok ? qr : 0);
-            const int64_t row = sq.row0 + qy / G, head = h * G + qy % G;
-            cp_async16(q_tile + panel_off(TQ_ROWS, qr, c), static_cast<const T *>(a.d_q) + row * a.q_token + head * a.q_head + c * 8, ok);
-            cp_async16(do_tile + panel_off(TQ_ROWS, qr, c), d_do + row * do_token + head * do_head + c * 8, ok);
-        }
-        cp_commit();
         const int r = tid & 127, half = warp >> 2, y = tr.row0 + min(r, rows - 1);
         const int limit = attn_limit(a, sq, y / G);
         const uint32_t my_bit = 1u << (y / G / a.query_block - tr.qb0), all_bits = tr.n_qb == 32 ? ~0u : (1u << tr.n_qb) - 1;
@@ -779,7 +785,7 @@ __global__ __launch_bounds__(TQ_THREADS, 2) void attn_dq_tc_kernel(const __grid_
         }
         if (n_tiles && fine) fine = __all_sync(~0u, ws.wait(smem_u32(&ctrl->dq_done), n_tiles - 1, 8));
         tc_fence_after();
-        T *dst = dq + at * D + half * (D / 2);
+        __syncthreads();                                       // every copy has landed, every product is done
 #pragma unroll 1
         for (int c = 0; c < D / 64; c++) {
             uint32_t v[32];
@@ -790,15 +796,20 @@ __global__ __launch_bounds__(TQ_THREADS, 2) void attn_dq_tc_kernel(const __grid_
             }
 #pragma unroll
             for (int i = 0; i < 32; i++) v[i] = !fine ? 0x7fc00000u : n_tiles ? v[i] : 0u;
-            if (r < rows)
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    uint32_t x[4];
+            for (int i = 0; i < 4; i++) {
+                uint32_t x[4];
 #pragma unroll
-                    for (int k = 0; k < 4; k++)
-                        x[k] = Pack<T>::two(__uint_as_float(v[8 * i + 2 * k]), __uint_as_float(v[8 * i + 2 * k + 1]));
-                    reinterpret_cast<uint4 *>(dst + c * 32)[i] = *reinterpret_cast<uint4 *>(x);
-                }
+                for (int k = 0; k < 4; k++)
+                    x[k] = Pack<T>::two(__uint_as_float(v[8 * i + 2 * k]), __uint_as_float(v[8 * i + 2 * k + 1]));
+                *reinterpret_cast<uint4 *>(smem + row_piece(D * 2, r, half * (D / 16) + c * 4 + i)) = *reinterpret_cast<uint4 *>(x);
+            }
+        }
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+        for (int i = tid; i < rows * (D / 8); i += TQ_SOFTMAX) {
+            const int sr = i / (D / 8), c = i % (D / 8), sy = tr.row0 + sr;
+            *reinterpret_cast<uint4 *>(dq + ((int64_t)(sq.row0 + sy / G) * a.heads + h * G + sy % G) * D + c * 8) =
+                *reinterpret_cast<const uint4 *>(smem + row_piece(D * 2, sr, c));
         }
         if (!fine && a.d_status) *a.d_status = SPAMM_ERR_DEVICE_WAIT;
         tc_fence_before();
@@ -1229,7 +1240,7 @@ static int backward_launch(const spamm_attn &a, const BackwardPlan &p, const T *
     // over, tiles of 16
     int st;
     const int tq = attn_tiles(a);
-    if ((int64_t)a.max_q * (a.heads / a.kv_heads) >= 48 && p.nkb <= UNION_BLOCKS && p.groups * tq <= INT32_MAX) {
+    if ((int64_t)a.max_q * (a.heads / a.kv_heads) >= 48 && p.nkb <= TQ_BLOCKS<D> && p.groups * tq <= INT32_MAX) {
         RowMap k_map, v_map;
         attn_row_maps(a, min(a.block, TQ_KEYS), &k_map, &v_map);
         const int entries = (int)min((int64_t)p.nkb, (int64_t)attn_tile_lists(a) * a.n_select);

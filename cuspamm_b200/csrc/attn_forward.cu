@@ -395,6 +395,12 @@ struct TcCtrl {
     float top[2][2][2][TC_ROWS];        // [tile][step & 1][half][row]
 };
 
+// The 256 threads of a tile meet.
+static __device__ __forceinline__ void tile_barrier(int tile)
+{
+    asm volatile("bar.sync %0, 256;" ::"r"(tile + 1) : "memory");
+}
+
 template <typename T, int D, int TILES>
 __global__ __launch_bounds__(TILES * 256 + 64, TILES == 1 ? 2 : 1) void attn_tc_kernel(const __grid_constant__ spamm_attn a, const RowsPlan p,
                                                                 const __grid_constant__ RowMap k_map,
@@ -575,6 +581,7 @@ __global__ __launch_bounds__(TILES * 256 + 64, TILES == 1 ? 2 : 1) void attn_tc_
             load(j, at, true, v_ring + b * TILE, &ctrl->v_full[b]);
             at = next;
         }
+        __syncthreads();
     } else if (warp == W_MMA) {
         // ---- products: for each tile in turn, O of the step before, then S of this one.  They run in the order of their
         // issue: S may be written where p is still being read.
@@ -632,6 +639,7 @@ __global__ __launch_bounds__(TILES * 256 + 64, TILES == 1 ? 2 : 1) void attn_tc_
             }
         }
         __syncwarp();
+        __syncthreads();
     } else {
         // ---- softmax: two threads for a row of the warp's tile, each half of the keys
         const int x0 = warp >> 3, half = warp >> 2 & 1, quad = warp & 3;
@@ -751,9 +759,10 @@ __global__ __launch_bounds__(TILES * 256 + 64, TILES == 1 ? 2 : 1) void attn_tc_
         tc_fence_after();
         const float inv = l == 0.f ? 0.f : 1.f / l;
         const float lse2 = l == 0.f ? -CUDART_INF_F : (m == -CUDART_INF_F ? 0.f : m) + log2f(l);
-        const int64_t row = sq.row0 + y / G;
-        const int head = h * G + y % G;
-        const int64_t at = (row * a.heads + head) * p.n_split + split;
+        // every copy has landed and every product is done when all roles have come here: the tiles' room is free
+        __syncthreads();
+        uint8_t *const stage = smem + x0 * 3 * TILE;               // rows in the type (and their low parts behind), or in float
+        const bool whole = p.n_split == 1;
 #pragma unroll 1
         for (int c = 0; c < D / 64 && rows; c++) {
             uint32_t v[32];
@@ -766,24 +775,39 @@ __global__ __launch_bounds__(TILES * 256 + 64, TILES == 1 ? 2 : 1) void attn_tc_
 #pragma unroll
             for (int i = 0; i < 32; i++)
                 v[i] = !fine ? 0x7fc00000u : n_done ? __float_as_uint(__uint_as_float(v[i]) * inv) : 0u;
-            if (r < rows) {
-                if (p.n_split == 1) {
-                    T *dst = static_cast<T *>(a.d_o) + row * a.o_token + head * a.o_head + d0;
-                    T *low = a.d_o_low ? static_cast<T *>(a.d_o_low) + (row * a.heads + head) * D + d0 : nullptr;
+            if (whole) {
 #pragma unroll
-                    for (int i = 0; i < 4; i++) store8<T>(dst + 8 * i, low ? low + 8 * i : nullptr, reinterpret_cast<float *>(v) + 8 * i);
-                } else {
-                    float4 *dst = reinterpret_cast<float4 *>(part_o + at * D + d0);
-#pragma unroll
-                    for (int i = 0; i < 8; i++)
-                        dst[i] = make_float4(__uint_as_float(v[4 * i]), __uint_as_float(v[4 * i + 1]),
-                                             __uint_as_float(v[4 * i + 2]), __uint_as_float(v[4 * i + 3]));
+                for (int i = 0; i < 4; i++) {
+                    uint8_t *at = stage + row_piece(D * 2, r, d0 / 8 + i);
+                    store8<T>(reinterpret_cast<T *>(at), a.d_o_low ? reinterpret_cast<T *>(at + TILE) : nullptr, reinterpret_cast<float *>(v) + 8 * i);
                 }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; i++)
+                    *reinterpret_cast<uint4 *>(stage + row_piece(D * 4, r, d0 / 4 + i)) = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
             }
         }
         if (r < rows && half == 0) {
-            if (p.n_split > 1) part_lse[at] = fine ? lse2 : CUDART_NAN_F;
+            const int64_t row = sq.row0 + y / G;
+            const int head = h * G + y % G;
+            if (!whole) part_lse[(row * a.heads + head) * p.n_split + split] = fine ? lse2 : CUDART_NAN_F;
             else if (a.d_lse) a.d_lse[row * a.heads + head] = fine ? lse2 * LN2 : CUDART_NAN_F;
+        }
+        tile_barrier(x0);
+        const int pieces = whole ? D / 8 : D / 4;                  // of a row
+        for (int i = tid & 255; i < rows * pieces; i += 256) {
+            const int sr = i / pieces, c = i % pieces, sy = mine.row0 + sr;
+            const int64_t row = sq.row0 + sy / G;
+            const int head = h * G + sy % G;
+            if (whole) {
+                const uint8_t *from = stage + row_piece(D * 2, sr, c);
+                *reinterpret_cast<uint4 *>(static_cast<T *>(a.d_o) + row * a.o_token + head * a.o_head + c * 8) = *reinterpret_cast<const uint4 *>(from);
+                if (a.d_o_low)
+                    *reinterpret_cast<uint4 *>(static_cast<T *>(a.d_o_low) + (row * a.heads + head) * D + c * 8) = *reinterpret_cast<const uint4 *>(from + TILE);
+            } else {
+                const int64_t at = (row * a.heads + head) * p.n_split + split;
+                *reinterpret_cast<uint4 *>(part_o + at * D + c * 4) = *reinterpret_cast<const uint4 *>(stage + row_piece(D * 4, sr, c));
+            }
         }
         if (!fine && a.d_status) *a.d_status = SPAMM_ERR_DEVICE_WAIT;
         tc_fence_before();

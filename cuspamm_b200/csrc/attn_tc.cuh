@@ -289,6 +289,12 @@ __device__ __forceinline__ float2 poly_exp2(float2 x)
     return mul2(p, s);
 }
 
+// ---- results by way of shared memory
+//
+// A thread has a row of an accumulator; stored from there, every warp instruction would touch 32 lines.  The rows go to
+// shared memory first (16-byte pieces XORed with the row, no bank conflicts either way) and leave as whole rows.
+__device__ __forceinline__ uint32_t row_piece(int row_bytes, int r, int c) { return r * row_bytes + ((c ^ (r & 7)) << 4); }
+
 // Barriers of a kernel and its abort flag: a wait that runs out (never, unless the kernel is wrong) sets the flag, every
 // role leaves its loop, and the results of the tile become NaN.
 struct WaitState {
