@@ -570,7 +570,7 @@ struct TqCtrl {
 
 template <typename T, int D>
 __global__ __launch_bounds__(TQ_THREADS, 2) void attn_dq_tc_kernel(const __grid_constant__ spamm_attn a, int tiles,
-                                                                   int max_entries,
+                                                                   const TileShape shape, int max_entries,
                                                                    const __grid_constant__ RowMap k_map,
                                                                    const __grid_constant__ RowMap v_map, const T *d_do,
                                                                    int64_t do_token, int64_t do_head, const float *delta, T *dq)
@@ -590,19 +590,23 @@ __global__ __launch_bounds__(TQ_THREADS, 2) void attn_dq_tc_kernel(const __grid_
     const int s = idx / a.kv_heads;
     const int G = a.heads / a.kv_heads;
     const Seq sq = attn_seq(a, s);
-    const TileRows tr = attn_tile(a, sq, tile);
+    const TileRows tr = attn_tile(a, shape, sq, tile);
     if (!tr.rows) return;
     const int rows = tr.rows;
     const int limit_max = attn_limit(a, sq, tr.last), limit_min = attn_limit(a, sq, tr.first);
 
     if (warp < 8) {
-        for (int i = 0; i < D / 16; i++) {
-            const int x = i * TQ_SOFTMAX + tid, qr = x / (D / 8), c = x % (D / 8);
+        constexpr int PASS = TQ_SOFTMAX / (D / 8);                     // rows at a time
+        const int c = tid % (D / 8);
+        const T *q_src = static_cast<const T *>(a.d_q) + (int64_t)sq.row0 * a.q_token + (int64_t)h * G * a.q_head + c * 8;
+        const T *do_src = d_do + (int64_t)sq.row0 * do_token + (int64_t)h * G * do_head + c * 8;
+#pragma unroll
+        for (int qr = tid / (D / 8); qr < TQ_ROWS; qr += PASS) {
             const bool ok = qr < rows;
-            const int qy = tr.row0 + (ok ? qr : 0);
-            const int64_t row = sq.row0 + qy / G, head = h * G + qy % G;
-            cp_async16(q_tile + panel_off(TQ_ROWS, qr, c), static_cast<const T *>(a.d_q) + row * a.q_token + head * a.q_head + c * 8, ok);
-            cp_async16(do_tile + panel_off(TQ_ROWS, qr, c), d_do + row * do_token + head * do_head + c * 8, ok);
+            const int qy = tr.row0 + (ok ? qr : 0), tok = (int)shape.G.quotient(qy), head = qy - tok * G;
+            const uint32_t off = panel_off(TQ_ROWS, qr, c);
+            cp_async16(q_tile + off, q_src + tok * a.q_token + head * a.q_head, ok);
+            cp_async16(do_tile + off, do_src + tok * do_token + head * do_head, ok);
         }
         cp_commit();
     } else if (warp == 8) {
@@ -722,10 +726,10 @@ __global__ __launch_bounds__(TQ_THREADS, 2) void attn_dq_tc_kernel(const __grid_
         __syncwarp();
         __syncthreads();
     } else {
-        const int r = tid & 127, half = warp >> 2, y = tr.row0 + min(r, rows - 1);
-        const int limit = attn_limit(a, sq, y / G);
-        const uint32_t my_bit = 1u << (y / G / a.query_block - tr.qb0), all_bits = tr.n_qb == 32 ? ~0u : (1u << tr.n_qb) - 1;
-        const int64_t at = (int64_t)(sq.row0 + y / G) * a.heads + h * G + y % G;
+        const int r = tid & 127, half = warp >> 2, y = tr.row0 + min(r, rows - 1), my_query = (int)shape.G.quotient(y);
+        const int limit = attn_limit(a, sq, my_query);
+        const uint32_t my_bit = 1u << (my_query / a.query_block - tr.qb0), all_bits = tr.n_qb == 32 ? ~0u : (1u << tr.n_qb) - 1;
+        const int64_t at = (int64_t)(sq.row0 + my_query) * a.heads + h * G + y - my_query * G;
         const float z = a.d_lse[at];
         const float minus_lse = z == -CUDART_INF_F ? -CUDART_INF_F : -z * LOG2E;       // a row without keys: every p zero
         const float minus_delta = -delta[at] * a.scale;
@@ -806,9 +810,10 @@ __global__ __launch_bounds__(TQ_THREADS, 2) void attn_dq_tc_kernel(const __grid_
             }
         }
         asm volatile("bar.sync 1, 256;" ::: "memory");
-        for (int i = tid; i < rows * (D / 8); i += TQ_SOFTMAX) {
-            const int sr = i / (D / 8), c = i % (D / 8), sy = tr.row0 + sr;
-            *reinterpret_cast<uint4 *>(dq + ((int64_t)(sq.row0 + sy / G) * a.heads + h * G + sy % G) * D + c * 8) =
+        const int c = tid % (D / 8);
+        for (int sr = tid / (D / 8); sr < rows; sr += TQ_SOFTMAX / (D / 8)) {
+            const int sy = tr.row0 + sr, tok = (int)shape.G.quotient(sy);
+            *reinterpret_cast<uint4 *>(dq + ((int64_t)(sq.row0 + tok) * a.heads + h * G + sy - tok * G) * D + c * 8) =
                 *reinterpret_cast<const uint4 *>(smem + row_piece(D * 2, sr, c));
         }
         if (!fine && a.d_status) *a.d_status = SPAMM_ERR_DEVICE_WAIT;
@@ -1240,7 +1245,7 @@ static int backward_launch(const spamm_attn &a, const BackwardPlan &p, const T *
     // over, tiles of 16
     int st;
     const int tq = attn_tiles(a);
-    if ((int64_t)a.max_q * (a.heads / a.kv_heads) >= 48 && p.nkb <= TQ_BLOCKS<D> && p.groups * tq <= INT32_MAX) {
+    if ((int64_t)a.max_q * (a.heads / a.kv_heads) >= 48 && attn_tile_fits(a) && p.nkb <= TQ_BLOCKS<D> && p.groups * tq <= INT32_MAX) {
         RowMap k_map, v_map;
         attn_row_maps(a, min(a.block, TQ_KEYS), &k_map, &v_map);
         const int entries = (int)min((int64_t)p.nkb, (int64_t)attn_tile_lists(a) * a.n_select);
@@ -1248,7 +1253,7 @@ static int backward_launch(const spamm_attn &a, const BackwardPlan &p, const T *
         st = attn_set_smem((const void *)attn_dq_tc_kernel<T, D>, smem);
         if (st) return st;
         attn_dq_tc_kernel<T, D><<<(unsigned)(p.groups * tq), TQ_THREADS, smem, stream>>>(
-            a, tq, entries, k_map, v_map, d_do, do_token, do_head, delta, dq);
+            a, tq, attn_tile_shape(a), entries, k_map, v_map, d_do, do_token, do_head, delta, dq);
     } else {
     const size_t dq_smem = (size_t)DQ_WARPS * DQ_STAGES * 2 * 16 * D * 2 + 2 * 16 * D * 2 + a.n_select * 4;
     st = attn_set_smem((const void *)attn_dq_rows_kernel<T, D>, dq_smem);

@@ -121,6 +121,7 @@ struct RowsPlan {
     int split_keys;         // keys of a range, a multiple of the block
     int max_entries;        // blocks of a range
     bool pairs;             // pairs of tiles of 128 rows to a block of threads
+    TileShape shape;        // of a tile of 128 rows
 };
 
 constexpr int ROWS_STAGES = 3;
@@ -402,7 +403,7 @@ static __device__ __forceinline__ void tile_barrier(int tile)
 }
 
 template <typename T, int D, int TILES>
-__global__ __launch_bounds__(TILES * 256 + 64, TILES == 1 ? 2 : 1) void attn_tc_kernel(const __grid_constant__ spamm_attn a, const RowsPlan p,
+__global__ __launch_bounds__(TILES * 256 + 64, TILES == 1 ? 2 : 1) void attn_tc_kernel(const __grid_constant__ spamm_attn a, const __grid_constant__ RowsPlan p,
                                                                 const __grid_constant__ RowMap k_map,
                                                                 const __grid_constant__ RowMap v_map, float *part_o,
                                                                 float *part_lse)
@@ -426,7 +427,7 @@ __global__ __launch_bounds__(TILES * 256 + 64, TILES == 1 ? 2 : 1) void attn_tc_
     const int G = a.heads / a.kv_heads;
     const Seq sq = attn_seq(a, s);
     if (a.zero_tail && split == 0) zero_tail<T>(a, sq, s, h, pair, p.tiles);
-    const TileRows tr[2] = {attn_tile(a, sq, TILES * pair), TILES == 2 ? attn_tile(a, sq, 2 * pair + 1) : TileRows{}};
+    const TileRows tr[2] = {attn_tile(a, p.shape, sq, TILES * pair), TILES == 2 ? attn_tile(a, p.shape, sq, 2 * pair + 1) : TileRows{}};
     if (!tr[0].rows) return;
     const int limits[2] = {attn_limit(a, sq, sq.pos0 + tr[0].last), tr[1].rows ? attn_limit(a, sq, sq.pos0 + tr[1].last) : 0};
     const int limit_max = max(limits[0], limits[1]);
@@ -435,12 +436,14 @@ __global__ __launch_bounds__(TILES * 256 + 64, TILES == 1 ? 2 : 1) void attn_tc_
         // the queries of the warp's tile
         const int x0 = warp >> 3, t = tid & 255;
         const TileRows mine = x0 ? tr[1] : tr[0];
-        for (int i = 0; i < D / 16; i++) {
-            const int x = i * 256 + t, qr = x / (D / 8), c = x % (D / 8);
+        constexpr int PASS = 256 / (D / 8);                            // rows at a time
+        const int c = t % (D / 8);
+        const T *src = static_cast<const T *>(a.d_q) + (int64_t)sq.row0 * a.q_token + (int64_t)h * G * a.q_head + c * 8;
+#pragma unroll
+        for (int qr = t / (D / 8); qr < TC_ROWS; qr += PASS) {
             const bool ok = qr < mine.rows;
-            const int qy = mine.row0 + (ok ? qr : 0);
-            const int64_t off = (int64_t)(sq.row0 + qy / G) * a.q_token + (int64_t)(h * G + qy % G) * a.q_head;
-            cp_async16(q_tiles + x0 * TILE + panel_off(128, qr, c), static_cast<const T *>(a.d_q) + off + c * 8, ok);
+            const int qy = mine.row0 + (ok ? qr : 0), tok = (int)p.shape.G.quotient(qy);
+            cp_async16(q_tiles + x0 * TILE + panel_off(128, qr, c), src + tok * a.q_token + (qy - tok * G) * a.q_head, ok);
         }
         cp_commit();
     } else if (warp == W_MMA) {
@@ -649,9 +652,9 @@ __global__ __launch_bounds__(TILES * 256 + 64, TILES == 1 ? 2 : 1) void attn_tc_
         fence_async_smem();
         mbar_arrive(smem_u32(&ctrl->q_full[x0]));
         const int r = tid & 127;
-        const int y = mine.row0 + min(r, max(rows, 1) - 1);
-        const int limit = attn_limit(a, sq, sq.pos0 + y / G), limit_min = attn_limit(a, sq, sq.pos0 + mine.first);
-        const uint32_t my_bit = a.n_select ? 1u << (y / G / a.query_block - mine.qb0) : 1u;
+        const int y = mine.row0 + min(r, max(rows, 1) - 1), my_query = (int)p.shape.G.quotient(y);
+        const int limit = attn_limit(a, sq, sq.pos0 + my_query), limit_min = attn_limit(a, sq, sq.pos0 + mine.first);
+        const uint32_t my_bit = a.n_select ? 1u << (my_query / a.query_block - mine.qb0) : 1u;
         const uint32_t all_bits = mine.n_qb == 32 ? ~0u : (1u << mine.n_qb) - 1;
         const float scale2 = a.scale * LOG2E;
         const uint32_t lane_s = tmem + ((uint32_t)(quad * 32) << 16) + x0 * TC_KEYS + half * TC_HALF;
@@ -788,24 +791,27 @@ __global__ __launch_bounds__(TILES * 256 + 64, TILES == 1 ? 2 : 1) void attn_tc_
             }
         }
         if (r < rows && half == 0) {
-            const int64_t row = sq.row0 + y / G;
-            const int head = h * G + y % G;
+            const int64_t row = sq.row0 + my_query;
+            const int head = h * G + y - my_query * G;
             if (!whole) part_lse[(row * a.heads + head) * p.n_split + split] = fine ? lse2 : CUDART_NAN_F;
             else if (a.d_lse) a.d_lse[row * a.heads + head] = fine ? lse2 * LN2 : CUDART_NAN_F;
         }
         tile_barrier(x0);
-        const int pieces = whole ? D / 8 : D / 4;                  // of a row
-        for (int i = tid & 255; i < rows * pieces; i += 256) {
-            const int sr = i / pieces, c = i % pieces, sy = mine.row0 + sr;
-            const int64_t row = sq.row0 + sy / G;
-            const int head = h * G + sy % G;
-            if (whole) {
+        if (whole) {
+            const int c = (tid & 255) % (D / 8);
+            for (int sr = (tid & 255) / (D / 8); sr < rows; sr += 256 / (D / 8)) {
+                const int sy = mine.row0 + sr, tok = (int)p.shape.G.quotient(sy), head = h * G + sy - tok * G;
+                const int64_t row = sq.row0 + tok;
                 const uint8_t *from = stage + row_piece(D * 2, sr, c);
                 *reinterpret_cast<uint4 *>(static_cast<T *>(a.d_o) + row * a.o_token + head * a.o_head + c * 8) = *reinterpret_cast<const uint4 *>(from);
                 if (a.d_o_low)
                     *reinterpret_cast<uint4 *>(static_cast<T *>(a.d_o_low) + (row * a.heads + head) * D + c * 8) = *reinterpret_cast<const uint4 *>(from + TILE);
-            } else {
-                const int64_t at = (row * a.heads + head) * p.n_split + split;
+            }
+        } else {
+            const int c = (tid & 255) % (D / 4);
+            for (int sr = (tid & 255) / (D / 4); sr < rows; sr += 256 / (D / 4)) {
+                const int sy = mine.row0 + sr, tok = (int)p.shape.G.quotient(sy), head = h * G + sy - tok * G;
+                const int64_t at = ((int64_t)(sq.row0 + tok) * a.heads + head) * p.n_split + split;
                 *reinterpret_cast<uint4 *>(part_o + at * D + c * 4) = *reinterpret_cast<const uint4 *>(stage + row_piece(D * 4, sr, c));
             }
         }
@@ -947,6 +953,7 @@ static RowsPlan rows_plan(const spamm_attn &a)
         p.tiles = ceil_div(attn_tiles(a), 2);
         p.pairs = (int64_t)a.batch * a.kv_heads * p.tiles >= 2 * 148 || !a.n_select;
         if (!p.pairs) p.tiles = attn_tiles(a);
+        p.shape = attn_tile_shape(a);
     } else {
         p.bq = a.n_select ? min(a.query_block, a.max_q) : a.max_q;
         p.nqb = ceil_div(a.max_q, p.bq);
@@ -980,7 +987,7 @@ static int forward_launch(const spamm_attn &a, float *scratch, cudaStream_t stre
     const RowsPlan p = rows_plan(a);
     const int64_t grid = (int64_t)a.batch * a.kv_heads * p.nqb * p.tiles * p.n_split;
     const int64_t rows = (int64_t)a.batch * a.max_q * a.heads;
-    if (grid > INT32_MAX || (rows + 3) / 4 > INT32_MAX) return attn_too_large();
+    if (grid > INT32_MAX || (rows + 3) / 4 > INT32_MAX || (use_tc(a) && !attn_tile_fits(a))) return attn_too_large();
     float *part_o = scratch;
     float *part_lse = scratch + (size_t)a.tokens * a.heads * p.n_split * D;
     if (use_tc(a)) {

@@ -168,16 +168,23 @@ inline int attn_tile_lists(const spamm_attn &a)
     const int64_t n = (rows + per - 1) / per + (rows % per && per % rows ? 1 : 0);
     return (int)(n < UNION_LISTS ? n : UNION_LISTS);
 }
-__device__ __forceinline__ TileRows attn_tile(const spamm_attn &a, const Seq &sq, int tile)
+// Rows of a tile and the heads of a key head, made on the host (rows of a sequence are below 2^30).
+struct TileShape {
+    int rows;
+    FastDiv G;
+};
+inline TileShape attn_tile_shape(const spamm_attn &a) { return TileShape{attn_tile_rows(a), fast_div((uint32_t)(a.heads / a.kv_heads))}; }
+inline bool attn_tile_fits(const spamm_attn &a) { return (int64_t)a.max_q * (a.heads / a.kv_heads) < (1 << 30); }
+
+__device__ __forceinline__ TileRows attn_tile(const spamm_attn &a, const TileShape &shape, const Seq &sq, int tile)
 {
     TileRows t{};
-    const int G = a.heads / a.kv_heads, per_tile = attn_tile_rows(a);
-    const int64_t all = (int64_t)sq.nq * G, row0 = (int64_t)tile * per_tile;
+    const int all = sq.nq * (int)shape.G.d, row0 = tile * shape.rows;
     if (row0 >= all) return t;
-    t.rows = (int)min((int64_t)per_tile, all - row0);
-    t.row0 = (int)row0;
-    t.first = (int)(row0 / G);
-    t.last = (int)((row0 + t.rows - 1) / G);
+    t.rows = min(shape.rows, all - row0);
+    t.row0 = row0;
+    t.first = (int)shape.G.quotient(row0);
+    t.last = (int)shape.G.quotient(row0 + t.rows - 1);
     t.qb0 = a.n_select ? t.first / a.query_block : 0;
     t.n_qb = a.n_select ? t.last / a.query_block - t.qb0 + 1 : 1;
     return t;
@@ -197,7 +204,8 @@ __device__ __forceinline__ int attn_union(const spamm_attn &a, const Seq &sq, in
 #pragma unroll
     for (int x = 0; x < TILES; x++) {
         if (t[x].rows)
-            for (int q = (warp + THREADS / 32 - q0 % (THREADS / 32)) % (THREADS / 32); q < t[x].n_qb; q += THREADS / 32) {
+            // (the last warps first: they are free while the others load the queries)
+            for (int q = (2 * (THREADS / 32) - 1 - warp - q0 % (THREADS / 32)) % (THREADS / 32); q < t[x].n_qb; q += THREADS / 32) {
                 const int qb = t[x].qb0 + q;
                 const int last = (int)min((int64_t)(qb + 1) * a.query_block, (int64_t)sq.nq) - 1;
                 attn_for_list(a, s, qb, nqb, h, ceil_div(attn_limit(a, sq, sq.pos0 + last), a.block), lane, [&](int v, int) {
