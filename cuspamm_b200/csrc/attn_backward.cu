@@ -381,175 +381,6 @@ static __device__ __forceinline__ int expand_bits(const unsigned *my_bits, int w
     return min(max(found - want0, 0), room);
 }
 
-constexpr int DKV_ROWS = 64;      // query rows of a shared-memory tile
-constexpr int DKV_STAGES = 2;
-
-// dk and dv of one block of keys from one chunk of the query blocks that list it.  A warp has 16 keys (and, when the
-// block is shorter than 64 keys, a share of the rows of every tile); it takes the transposed scores, keys x queries, so
-// that p and ds leave the products in the layout in which they enter the next ones.
-template <typename T, int D, int KEYS>
-__global__ __launch_bounds__(KEYS == 128 ? 256 : 128) void attn_dkv_kernel(
-    const __grid_constant__ spamm_attn a, const BackwardPlan p, const T *d_do, int64_t do_token, int64_t do_head,
-    const float *delta, const unsigned *bits, const Item *items, const int *n_items, float *partial, T *dk, T *dv)
-{
-    constexpr int THREADS = KEYS == 128 ? 256 : 128, WARPS = THREADS / 32;
-    constexpr int KG = KEYS / 16, RG = WARPS / KG;                 // groups of keys, groups of rows
-    constexpr int STEPS = DKV_ROWS / RG / 16;
-    constexpr int KT = KEYS * D * 2, RT = DKV_ROWS * D * 2;
-    extern __shared__ __align__(128) uint8_t smem[];
-    uint8_t *k_tile = smem, *v_tile = smem + KT;
-    uint8_t *ring = smem + 2 * KT;                                  // [stage][q | do]
-    float *row_lse = reinterpret_cast<float *>(ring + DKV_STAGES * 2 * RT);      // [stage][64]
-    float *row_delta = row_lse + DKV_STAGES * DKV_ROWS;
-    int *row_pos = reinterpret_cast<int *>(row_delta + DKV_STAGES * DKV_ROWS);
-    int *list = row_pos + DKV_STAGES * DKV_ROWS;                    // [chunk] query blocks
-    __shared__ int warp_sum[WARPS];
-
-    const int64_t group = blockIdx.x / p.item_cap;
-    const int item_i = blockIdx.x % p.item_cap;
-    if (item_i >= n_items[group]) return;
-    const Item item = items[group * p.item_cap + item_i];
-    const int s = (int)(group / a.kv_heads), h = (int)(group % a.kv_heads);
-    const Seq sq = attn_seq(a, s);
-    const int G = a.heads / a.kv_heads;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int pos0 = item.kb * KEYS;
-    const int keys = min(KEYS, sq.nk - pos0);
-
-    for (int i = tid; i < KEYS * D / 8; i += THREADS) {
-        const int r = i / (D / 8), c = i % (D / 8);
-        const bool ok = r < keys;
-        const int64_t row = sq.row0 + pos0 + (ok ? r : 0);
-        cp_async16(smem_addr(k_tile) + tile_off<D>(r, c), static_cast<const T *>(a.d_k) + row * a.k_token + h * a.k_head + c * 8, ok);
-        cp_async16(smem_addr(v_tile) + tile_off<D>(r, c), static_cast<const T *>(a.d_v) + row * a.v_token + h * a.v_head + c * 8, ok);
-    }
-    const int n_list = expand_bits<THREADS>(bits + (group * p.nkb + item.kb) * p.words, p.words, item.chunk * p.chunk, p.chunk, list,
-                                            warp_sum);
-    const int bq = min(a.query_block, a.max_q);
-    const int per = bq * G;                                         // rows of a full query block
-    // all listed query blocks are full but the sequence's last one, which can only be the last of the list
-    const int64_t n_rows = n_list ? (int64_t)(n_list - 1) * per + (int64_t)min(bq, sq.nq - list[n_list - 1] * bq) * G : 0;
-    const int n_tiles = (int)((n_rows + DKV_ROWS - 1) / DKV_ROWS);
-
-    auto issue = [&](int t, int stage) {
-        if (t < n_tiles) {
-            const uint32_t qt = smem_addr(ring) + stage * 2 * RT, dt = qt + RT;
-            for (int i = tid; i < DKV_ROWS * D / 8; i += THREADS) {
-                const int r = i / (D / 8), c = i % (D / 8);
-                const int64_t x = (int64_t)t * DKV_ROWS + r;
-                const bool ok = x < n_rows;
-                const int e = ok ? (int)(x / per) : 0, y = ok ? (int)(x - (int64_t)e * per) : 0;
-                const int query = list[e] * bq + y / G, head = h * G + y % G;
-                const int64_t row = sq.row0 + query;
-                cp_async16(qt + tile_off<D>(r, c), static_cast<const T *>(a.d_q) + row * a.q_token + head * a.q_head + c * 8, ok);
-                cp_async16(dt + tile_off<D>(r, c), d_do + row * do_token + head * do_head + c * 8, ok);
-                if (c == 0) {
-                    const float z = ok ? a.d_lse[row * a.heads + head] : -CUDART_INF_F;
-                    row_lse[stage * DKV_ROWS + r] = z == -CUDART_INF_F ? CUDART_INF_F : z * LOG2E;
-                    row_delta[stage * DKV_ROWS + r] = ok ? delta[row * a.heads + head] : 0.f;
-                    row_pos[stage * DKV_ROWS + r] = ok ? (a.causal ? query : INT32_MAX) : -1;
-                }
-            }
-        }
-        cp_commit();
-    };
-    const int kg = warp % KG, rg = warp / KG;
-    const float scale2 = a.scale * LOG2E;
-    float ak[D / 8][4] = {}, av[D / 8][4] = {};
-    issue(0, 0);
-    for (int t = 0; t < n_tiles; t++) {
-        issue(t + 1, (t + 1) & 1);
-        cp_wait<1>();
-        __syncthreads();
-        const int stage = t & 1;
-        const uint32_t qt = smem_addr(ring) + stage * 2 * RT, dt = qt + RT;
-        const uint32_t kt = smem_addr(k_tile), vt = smem_addr(v_tile);
-#pragma unroll 1
-        for (int step = 0; step < STEPS; step++) {
-            const int r0 = (rg * STEPS + step) * 16;
-            float sc[2][4] = {}, dp[2][4] = {};
-#pragma unroll
-            for (int ks = 0; ks < D / 16; ks++) {
-                uint32_t x[4], b[4];
-                a_frag<D>(kt, kg * 16, ks, lane, x);
-                b_frag2<D>(qt, r0, ks, lane, b);
-                mma16816<T>(sc[0], x, b[0], b[1]);
-                mma16816<T>(sc[1], x, b[2], b[3]);
-                a_frag<D>(vt, kg * 16, ks, lane, x);
-                b_frag2<D>(dt, r0, ks, lane, b);
-                mma16816<T>(dp[0], x, b[0], b[1]);
-                mma16816<T>(dp[1], x, b[2], b[3]);
-            }
-#pragma unroll
-            for (int nt = 0; nt < 2; nt++)
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const int r = stage * DKV_ROWS + r0 + nt * 8 + (lane & 3) * 2 + (i & 1);
-                    const int key = kg * 16 + (lane >> 2) + 8 * (i >> 1);
-                    const bool ok = key < keys && pos0 + key <= row_pos[r];
-                    const float pr = ok ? fast_exp2(sc[nt][i] * scale2 - row_lse[r]) : 0.f;
-                    dp[nt][i] = ok ? pr * (dp[nt][i] - row_delta[r]) * a.scale : 0.f;
-                    sc[nt][i] = pr;
-                }
-            const uint32_t pf[4] = {Pack<T>::two(sc[0][0], sc[0][1]), Pack<T>::two(sc[0][2], sc[0][3]),
-                                    Pack<T>::two(sc[1][0], sc[1][1]), Pack<T>::two(sc[1][2], sc[1][3])};
-            const uint32_t sf[4] = {Pack<T>::two(dp[0][0], dp[0][1]), Pack<T>::two(dp[0][2], dp[0][3]),
-                                    Pack<T>::two(dp[1][0], dp[1][1]), Pack<T>::two(dp[1][2], dp[1][3])};
-#pragma unroll
-            for (int n = 0; n < D / 16; n++) {
-                uint32_t b[4];
-                bt_frag2<D>(dt, r0, n * 16, lane, b);
-                mma16816<T>(av[2 * n], pf, b[0], b[1]);
-                mma16816<T>(av[2 * n + 1], pf, b[2], b[3]);
-                bt_frag2<D>(qt, r0, n * 16, lane, b);
-                mma16816<T>(ak[2 * n], sf, b[0], b[1]);
-                mma16816<T>(ak[2 * n + 1], sf, b[2], b[3]);
-            }
-        }
-        __syncthreads();
-    }
-    cp_wait<0>();
-    __syncthreads();
-    // the row groups' sums are added in order through shared memory: [KEYS][D] of dk, then of dv (in place of the tiles)
-    float *sk = reinterpret_cast<float *>(smem), *sv = sk + KEYS * D;
-    for (int g = 0; g < RG; g++) {
-        if (rg == g)
-#pragma unroll
-            for (int n = 0; n < D / 8; n++)
-#pragma unroll
-                for (int x = 0; x < 2; x++) {
-                    const int at = (kg * 16 + (lane >> 2) + 8 * x) * D + n * 8 + (lane & 3) * 2;
-                    float2 *pk = reinterpret_cast<float2 *>(sk + at), *pv = reinterpret_cast<float2 *>(sv + at);
-                    float2 k2 = make_float2(ak[n][2 * x], ak[n][2 * x + 1]), v2 = make_float2(av[n][2 * x], av[n][2 * x + 1]);
-                    if (g) {
-                        k2.x += pk->x; k2.y += pk->y;
-                        v2.x += pv->x; v2.y += pv->y;
-                    }
-                    *pk = k2;
-                    *pv = v2;
-                }
-        __syncthreads();
-    }
-    if (item.slot >= 0) {
-        float *dst = partial + (group * p.slot_cap + item.slot) * (int64_t)(2 * KEYS * D);
-        for (int i = tid; i < 2 * KEYS * D / 4; i += THREADS)
-            reinterpret_cast<float4 *>(dst)[i] = reinterpret_cast<float4 *>(sk)[i];
-        return;
-    }
-    for (int i = tid; i < keys * D / 8; i += THREADS) {
-        const int r = i / (D / 8), c = i % (D / 8) * 8;
-        const int64_t at = ((int64_t)(sq.row0 + pos0 + r) * a.kv_heads + h) * D + c;
-        uint32_t x[4], y[4];
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            x[j] = Pack<T>::two(sk[r * D + c + 2 * j], sk[r * D + c + 2 * j + 1]);
-            y[j] = Pack<T>::two(sv[r * D + c + 2 * j], sv[r * D + c + 2 * j + 1]);
-        }
-        *reinterpret_cast<uint4 *>(dk + at) = *reinterpret_cast<uint4 *>(x);
-        *reinterpret_cast<uint4 *>(dv + at) = *reinterpret_cast<uint4 *>(y);
-    }
-}
-
 // ---- tiles of 128 rows on the tensor memory path
 //
 // dq: 128 rows (queries x heads of a key head), 64 listed keys at a time.  S = Q K^T and dP = dO V^T go to tensor memory, a
@@ -828,16 +659,17 @@ __global__ __launch_bounds__(TQ_THREADS, 2) void attn_dq_tc_kernel(const __grid_
     }
 }
 
-// dk and dv of 64 keys of a block from one chunk of the query blocks that list it, 128 gathered rows at a time.
+// dk and dv of a block's keys (of half a block of 128) from one chunk of the query blocks that list it, 128 gathered rows at a
+// time.
 //
-//   S = Q K^T, dP = dO V^T   [128 rows x 64 keys]        from shared memory, two buffers each in tensor memory
-//   dV^T += dO^T P,  dK^T += Q^T ds   [D x 64 keys]      the tiles of dO and Q once more, as operands whose rows are K
+//   S = Q K^T, dP = dO V^T   [128 rows x keys]        from shared memory, two buffers each in tensor memory
+//   dV^T += dO^T P,  dK^T += Q^T ds   [D x keys]      the tiles of dO and Q once more, as operands whose rows are K
 //
 // P and ds pass through shared memory.  One block of threads per SM: while eight warps work on the exponentials of one
 // tile, the products of the tile before and of the one behind it run, and four warps gather the rows of the one after.
 // With D = 64 the tiles of dO and Q together are the 128 rows of the second products' A: dV^T comes out in the upper half
 // of one accumulator, dK^T in the lower half of the other (the other halves are not used).
-constexpr int TK_ROWS = 128, TK_KEYS = 64, TK_SOFTMAX = 256, TK_THREADS = TK_SOFTMAX + 32 + 128, TK_COLS = 512;
+constexpr int TK_ROWS = 128, TK_MAX_KEYS = 64, TK_SOFTMAX = 256, TK_THREADS = TK_SOFTMAX + 32 + 128, TK_COLS = 512;
 
 struct TkCtrl {
     uint64_t kv_full, r_full[2], r_empty[2], s_full[2], p_full, dv_done, ds_full, dk_done;
@@ -847,7 +679,7 @@ struct TkCtrl {
     int32_t pad;
 };
 
-template <typename T, int D>
+template <typename T, int D, int TK_KEYS>
 __global__ __launch_bounds__(TK_THREADS, 1) void attn_dkv_tc_kernel(const __grid_constant__ spamm_attn a, const __grid_constant__ BackwardPlan p,
                                                                     const __grid_constant__ RowMap q_map,
                                                                     const __grid_constant__ RowMap do_map,
@@ -857,7 +689,8 @@ __global__ __launch_bounds__(TK_THREADS, 1) void attn_dkv_tc_kernel(const __grid
 {
     extern __shared__ __align__(1024) uint8_t smem_tc[];
     uint8_t *const smem = smem_tc;
-    constexpr int KT = TK_KEYS * D * 2, RT = TK_ROWS * D * 2, PT = TK_ROWS * TK_KEYS * 2;
+    constexpr int KT = TK_KEYS * D * 2, RT = TK_ROWS * D * 2, PT = TK_ROWS * 128;     // rows of p and ds take a panel's 128 bytes
+    constexpr int HALF = TK_KEYS / 2;                           // keys of a thread
     const uint32_t k_tile = smem_u32(smem), v_tile = k_tile + KT, ring = v_tile + KT;      // ring: [stage][do | q]
     const uint32_t p_tile = ring + 4 * RT, ds_tile = p_tile + PT;
     TkCtrl *ctrl = reinterpret_cast<TkCtrl *>(smem + 2 * KT + 4 * RT + 2 * PT);
@@ -1056,7 +889,7 @@ __global__ __launch_bounds__(TK_THREADS, 1) void attn_dkv_tc_kernel(const __grid
         }
         __syncwarp();
     } else {
-        // ---- p and ds: thread = row, the upper four warps the keys 32..63
+        // ---- p and ds: thread = row, the upper four warps the second half of the keys
         const int r = tid & 127, part = warp >> 2;
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         const float scale2 = a.scale * LOG2E;
@@ -1071,7 +904,7 @@ __global__ __launch_bounds__(TK_THREADS, 1) void attn_dkv_tc_kernel(const __grid
                 const float z = a.d_lse[at];
                 if (z != -CUDART_INF_F) *minus_lse = -z * LOG2E;
                 *minus_delta = -delta[at] * a.scale;
-                *n_visible = min(a.causal ? query + 1 - pos0 : TK_KEYS, keys) - part * 32;
+                *n_visible = min(a.causal ? query + 1 - pos0 : TK_KEYS, keys) - part * HALF;
             }
         };
         float minus_lse, minus_delta;
@@ -1085,16 +918,16 @@ __global__ __launch_bounds__(TK_THREADS, 1) void attn_dkv_tc_kernel(const __grid
             fine = __all_sync(~0u, ws.wait(smem_u32(&ctrl->s_full[j & 1]), j >> 1, 6));
             if (!fine) break;
             tc_fence_after();
-            const uint32_t s_at = tmem + (j & 1) * 2 * TK_KEYS + lanes + part * 32;
-            uint32_t v[32], d[32], w[16];
-            tmem_ld32(s_at, v);
-            tmem_ld32(s_at + TK_KEYS, d);
+            const uint32_t s_at = tmem + (j & 1) * 2 * TK_KEYS + lanes + part * HALF;
+            uint32_t v[HALF], d[HALF], w[HALF / 2];
+            tmem_ld<HALF>(s_at, v);
+            tmem_ld<HALF>(s_at + TK_KEYS, d);
             tmem_wait_ld();
-            tmem_landed<32>(v);
-            tmem_landed<32>(d);
+            tmem_landed<HALF>(v);
+            tmem_landed<HALF>(d);
             const float2 ml2 = make_float2(minus_lse, minus_lse), md = make_float2(minus_delta, minus_delta);
 #pragma unroll
-            for (int i = 0; i < 16; i++) {
+            for (int i = 0; i < HALF / 2; i++) {
                 const float2 x = fma2(make_float2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), sc2, ml2);
                 const float2 g = fma2(make_float2(__uint_as_float(d[2 * i]), __uint_as_float(d[2 * i + 1])), sc, md);
                 const float e0 = fast_exp2(x.x), e1 = fast_exp2(x.y);
@@ -1103,29 +936,29 @@ __global__ __launch_bounds__(TK_THREADS, 1) void attn_dkv_tc_kernel(const __grid
                 d[2 * i] = __float_as_uint(e0 * g.x);
                 d[2 * i + 1] = __float_as_uint(e1 * g.y);
             }
-            if (__any_sync(~0u, n_visible < 32)) {
+            if (__any_sync(~0u, n_visible < HALF)) {
 #pragma unroll
-                for (int i = 0; i < 32; i++)
+                for (int i = 0; i < HALF; i++)
                     if (i >= n_visible) { v[i] = 0u; d[i] = 0u; }
             }
 #pragma unroll
-            for (int i = 0; i < 16; i++) w[i] = Pack<T>::two(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]));
+            for (int i = 0; i < HALF / 2; i++) w[i] = Pack<T>::two(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]));
             if (j) fine = __all_sync(~0u, ws.wait(smem_u32(&ctrl->dv_done), j - 1, 7));
             if (!fine) break;
 #pragma unroll
-            for (int c = 0; c < 4; c++)
-                *reinterpret_cast<uint4 *>(smem + (p_tile - k_tile) + panel_off(TK_ROWS, r, part * 4 + c)) =
+            for (int c = 0; c < HALF / 8; c++)
+                *reinterpret_cast<uint4 *>(smem + (p_tile - k_tile) + panel_off(TK_ROWS, r, part * (HALF / 8) + c)) =
                     make_uint4(w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]);
             fence_async_smem();
             tc_fence_before();
             mbar_arrive(smem_u32(&ctrl->p_full));
 #pragma unroll
-            for (int i = 0; i < 16; i++) w[i] = Pack<T>::two(__uint_as_float(d[2 * i]), __uint_as_float(d[2 * i + 1]));
+            for (int i = 0; i < HALF / 2; i++) w[i] = Pack<T>::two(__uint_as_float(d[2 * i]), __uint_as_float(d[2 * i + 1]));
             if (j) fine = __all_sync(~0u, ws.wait(smem_u32(&ctrl->dk_done), j - 1, 8));
             if (!fine) break;
 #pragma unroll
-            for (int c = 0; c < 4; c++)
-                *reinterpret_cast<uint4 *>(smem + (ds_tile - k_tile) + panel_off(TK_ROWS, r, part * 4 + c)) =
+            for (int c = 0; c < HALF / 8; c++)
+                *reinterpret_cast<uint4 *>(smem + (ds_tile - k_tile) + panel_off(TK_ROWS, r, part * (HALF / 8) + c)) =
                     make_uint4(w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]);
             fence_async_smem();
             tc_fence_before();
@@ -1140,27 +973,28 @@ __global__ __launch_bounds__(TK_THREADS, 1) void attn_dkv_tc_kernel(const __grid
         const bool is_k = part != 0;
         const int row = r, d0 = D == 64 && is_k ? row - 64 : row;
         const bool mine = D == 128 || (is_k ? row >= 64 : row < 64);            // whole warps
+        constexpr int COLS = TK_KEYS < 32 ? TK_KEYS : 32;
 #pragma unroll 1
-        for (int c = 0; c < TK_KEYS / 32; c++) {
-            uint32_t v[32];
+        for (int c = 0; c < TK_KEYS / COLS; c++) {
+            uint32_t v[COLS];
             if (n_tiles) {
-                tmem_ld32((is_k ? tmem_dk : tmem_dv) + lanes + c * 32, v);
+                tmem_ld<COLS>((is_k ? tmem_dk : tmem_dv) + lanes + c * COLS, v);
                 tmem_wait_ld();
-                tmem_landed<32>(v);
+                tmem_landed<COLS>(v);
             }
 #pragma unroll
-            for (int i = 0; i < 32; i++) v[i] = !fine ? 0x7fc00000u : n_tiles ? v[i] : 0u;
+            for (int i = 0; i < COLS; i++) v[i] = !fine ? 0x7fc00000u : n_tiles ? v[i] : 0u;
             if (!mine) continue;
             if (item.slot >= 0) {
                 float *dst = partial + (group * p.slot_cap + item.slot) * (int64_t)(2 * a.block * D) + (is_k ? 0 : a.block * D) +
-                             (half * TK_KEYS + c * 32) * D + d0;
+                             (half * TK_KEYS + c * COLS) * D + d0;
 #pragma unroll
-                for (int i = 0; i < 32; i++) dst[i * D] = __uint_as_float(v[i]);
+                for (int i = 0; i < COLS; i++) dst[i * D] = __uint_as_float(v[i]);
             } else {
-                T *dst = (is_k ? dk : dv) + ((int64_t)(sq.row0 + pos0 + c * 32) * a.kv_heads + h) * D + d0;
+                T *dst = (is_k ? dk : dv) + ((int64_t)(sq.row0 + pos0 + c * COLS) * a.kv_heads + h) * D + d0;
 #pragma unroll
-                for (int i = 0; i < 32; i++)
-                    if (c * 32 + i < keys) dst[(int64_t)i * a.kv_heads * D] = Pack<T>::one(__uint_as_float(v[i]));
+                for (int i = 0; i < COLS; i++)
+                    if (c * COLS + i < keys) dst[(int64_t)i * a.kv_heads * D] = Pack<T>::one(__uint_as_float(v[i]));
             }
         }
         if (!fine && a.d_status) *a.d_status = SPAMM_ERR_DEVICE_WAIT;
@@ -1208,13 +1042,15 @@ static int dkv_launch(const spamm_attn &a, const BackwardPlan &p, const T *d_do,
                       const float *delta, const unsigned *bits, const Item *items, const int *n_items, float *partial, T *dk,
                       T *dv, cudaStream_t stream)
 {
-    const size_t tiles = (size_t)2 * KEYS * D * 2 + DKV_STAGES * 2 * DKV_ROWS * D * 2 + DKV_STAGES * DKV_ROWS * 12 + p.chunk * 4;
-    const size_t sums = (size_t)2 * KEYS * D * 4;
-    const size_t smem = max(tiles, sums);
-    int st = attn_set_smem((const void *)attn_dkv_kernel<T, D, KEYS>, smem);
+    const size_t smem = 2 * KEYS * D * 2 + 4 * TK_ROWS * D * 2 + 2 * TK_ROWS * 128 + sizeof(TkCtrl) + p.chunk * 4;
+    int st = attn_set_smem((const void *)attn_dkv_tc_kernel<T, D, KEYS>, smem);
     if (st) return st;
-    attn_dkv_kernel<T, D, KEYS><<<(unsigned)(p.groups * p.item_cap), KEYS == 128 ? 256 : 128, smem, stream>>>(
-        a, p, d_do, do_token, do_head, delta, bits, items, n_items, partial, dk, dv);
+    RowMap q_map, do_map;
+    const int G = a.heads / a.kv_heads;
+    attn_row_map(a, a.d_q, a.q_token, a.q_head, a.heads, G, max(1, p.box_tokens), &q_map);
+    attn_row_map(a, d_do, do_token, do_head, a.heads, G, max(1, p.box_tokens), &do_map);
+    attn_dkv_tc_kernel<T, D, KEYS><<<(unsigned)(p.groups * p.item_cap * (a.block / KEYS)), TK_THREADS, smem, stream>>>(
+        a, p, q_map, do_map, d_do, do_token, do_head, delta, bits, items, n_items, partial, dk, dv);
     return SPAMM_OK;
 }
 
@@ -1261,19 +1097,10 @@ static int backward_launch(const spamm_attn &a, const BackwardPlan &p, const T *
     attn_dq_rows_kernel<T, D><<<(unsigned)dq_grid, 128, dq_smem, stream>>>(a, p.nqb, tiles, d_do, do_token, do_head, delta, dq);
     }
 
-    if (a.block >= TK_KEYS) {
-        const size_t smem = 2 * TK_KEYS * D * 2 + 4 * TK_ROWS * D * 2 + 2 * TK_ROWS * TK_KEYS * 2 + sizeof(TkCtrl) + p.chunk * 4;
-        st = attn_set_smem((const void *)attn_dkv_tc_kernel<T, D>, smem);
-        if (st) return st;
-        RowMap q_map, do_map;
-        const int G = a.heads / a.kv_heads;
-        attn_row_map(a, a.d_q, a.q_token, a.q_head, a.heads, G, max(1, p.box_tokens), &q_map);
-        attn_row_map(a, d_do, do_token, do_head, a.heads, G, max(1, p.box_tokens), &do_map);
-        attn_dkv_tc_kernel<T, D><<<(unsigned)(p.groups * p.item_cap * (a.block / TK_KEYS)), TK_THREADS, smem, stream>>>(
-            a, p, q_map, do_map, d_do, do_token, do_head, delta, bits, items, n_items, partial, dk, dv);
-    } else switch (a.block) {
+    switch (a.block) {
     case 16: st = dkv_launch<T, D, 16>(a, p, d_do, do_token, do_head, delta, bits, items, n_items, partial, dk, dv, stream); break;
-    default: st = dkv_launch<T, D, 32>(a, p, d_do, do_token, do_head, delta, bits, items, n_items, partial, dk, dv, stream); break;
+    case 32: st = dkv_launch<T, D, 32>(a, p, d_do, do_token, do_head, delta, bits, items, n_items, partial, dk, dv, stream); break;
+    default: st = dkv_launch<T, D, TK_MAX_KEYS>(a, p, d_do, do_token, do_head, delta, bits, items, n_items, partial, dk, dv, stream); break;
     }
     if (st) return st;
     if (p.nqb > p.chunk)

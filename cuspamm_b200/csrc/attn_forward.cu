@@ -382,7 +382,7 @@ __global__ __launch_bounds__(128) void attn_rows_kernel(const __grid_constant__ 
 // Where pairs would not fill the GPU, single tiles (TILES 1) with one buffer each for K and V: two blocks of threads per SM.
 constexpr int TC_ROWS = 128, TC_KEYS = 128, TC_HALF = TC_KEYS / 2;
 constexpr int TC_ENTRIES = 2048;        // blocks of a union, at most
-constexpr int TC_POLY = 6;              // of 16 pairs of exponentials, those that the polynomial takes
+constexpr int TC_POLY = 3;              // of 16 pairs of exponentials, those that the polynomial takes
 
 struct TcCtrl {
     uint64_t q_full[2], k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], pv_done[2];

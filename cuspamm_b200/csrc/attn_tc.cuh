@@ -70,6 +70,20 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t *v)
                  : "r"(taddr)
                  : "memory");
 }
+__device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t *v)
+{
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7])
+                 : "r"(taddr)
+                 : "memory");
+}
+template <int N> __device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t *v)
+{
+    static_assert(N == 8 || N == 16 || N == 32, "columns of one load");
+    if constexpr (N == 8) tmem_ld8(taddr, v);
+    else if constexpr (N == 16) tmem_ld16(taddr, v);
+    else tmem_ld32(taddr, v);
+}
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t *v)
 {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
