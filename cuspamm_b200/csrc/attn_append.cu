@@ -40,7 +40,7 @@ template <typename T> static __device__ __forceinline__ void turn_neighbours(uin
 
 template <typename T, int D>
 __global__ __launch_bounds__(APPEND_THREADS) void attn_append_kernel(const __grid_constant__ spamm_attn a, int pages_per_seq,
-                                                                     int heads_per_cta, T *k_pages, T *v_pages,
+                                                                     int heads_per_cta, FastDiv div_k, FastDiv div_q, T *k_pages, T *v_pages,
                                                                      float *key_sums, const float *inv_freq, int n_freq,
                                                                      bool interleaved)
 {
@@ -86,42 +86,52 @@ __global__ __launch_bounds__(APPEND_THREADS) void attn_append_kernel(const __gri
 
     const int64_t row0 = sq.row0 + (lo - sq.pos0);                    // row of the page's first new token
     const int rv = n_freq / 8;                                        // 8-value pieces of half the turned part
-    // values, a plain copy
-    if (page >= 0)
-        for (int i = tid; i < n * hn * V; i += APPEND_THREADS) {
-            const int c = i % V, h = h0 + i / V % hn, t = i / (V * hn);
-            const uint4 x = *reinterpret_cast<const uint4 *>(static_cast<const T *>(a.d_v) + (row0 + t) * a.v_token + h * a.v_head + c * 8);
-            *reinterpret_cast<uint4 *>(v_pages + (((int64_t)page * a.kv_heads + h) * a.block + (lo + t) % a.block) * D + c * 8) = x;
+    // Rows are (token, head), V neighbouring threads to a row; of keys and queries that are turned by halves a thread takes a
+    // pair of pieces, and when that leaves no more than V / 2 of them, V / 2 threads a row.  (The last block of heads may hold
+    // fewer than div_k.d: its rows beyond are skipped.)
+    const int col = tid % V;
+    const int64_t at0 = ((int64_t)page * a.kv_heads + h0) * a.block * D;
+    if (page >= 0) {
+        const T *src = static_cast<const T *>(a.d_v) + row0 * a.v_token + h0 * a.v_head + col * 8;
+#pragma unroll 4
+        for (int i = tid / V; i < n * (int)div_k.d; i += APPEND_THREADS / V) {
+            const int t = (int)div_k.quotient(i), h = i - t * (int)div_k.d;
+            if (h >= hn) continue;
+            const uint4 x = *reinterpret_cast<const uint4 *>(src + t * a.v_token + h * a.v_head);
+            *reinterpret_cast<uint4 *>(v_pages + at0 + (h * a.block + (lo + t) % a.block) * D + col * 8) = x;
         }
-    // keys, then queries: `units` pieces (or pairs of pieces) of a head
-    const int units = interleaved ? V : V - rv;
-    auto turn_head = [&](const T *src, T *dst, int u, const float2 *cs) {
-        if (interleaved) {
-            uint4 x = *reinterpret_cast<const uint4 *>(src + u * 8);
-            if (u < 2 * rv) turn_neighbours<T>(x, cs + u * 4);
-            *reinterpret_cast<uint4 *>(dst + u * 8) = x;
-        } else if (u < rv) {
-            uint4 x = *reinterpret_cast<const uint4 *>(src + u * 8), y = *reinterpret_cast<const uint4 *>(src + n_freq + u * 8);
-            turn_halves<T>(x, y, cs + u * 8);
-            *reinterpret_cast<uint4 *>(dst + u * 8) = x;
-            *reinterpret_cast<uint4 *>(dst + n_freq + u * 8) = y;
-        } else {
-            *reinterpret_cast<uint4 *>(dst + (u + rv) * 8) = *reinterpret_cast<const uint4 *>(src + (u + rv) * 8);
+    }
+    auto turn_rows = [&](const T *src, int64_t token, int64_t head, int rows, const FastDiv &div, int heads, auto to) {
+        const int units = interleaved ? V : V - rv, lanes = units <= V / 2 ? V / 2 : V;
+        const int u = tid % lanes, step = APPEND_THREADS / lanes;
+        if (u >= units) return;
+        const bool pair = !interleaved && u < rv, turned = interleaved ? u < 2 * rv : pair;
+        const int p0 = (interleaved || pair ? u : u + rv) * 8;
+#pragma unroll 4
+        for (int i = tid / lanes; i < rows; i += step) {
+            const int t = (int)div.quotient(i), h = i - t * (int)div.d;
+            if (h >= heads) continue;
+            const T *from = src + t * token + h * head;
+            T *dst = to(t, h);
+            const float2 *cs = turn + t * n_freq;
+            uint4 x = *reinterpret_cast<const uint4 *>(from + p0);
+            if (pair) {
+                uint4 y = *reinterpret_cast<const uint4 *>(from + n_freq + p0);
+                turn_halves<T>(x, y, cs + u * 8);
+                *reinterpret_cast<uint4 *>(dst + n_freq + p0) = y;
+            } else if (turned) {
+                turn_neighbours<T>(x, cs + u * 4);
+            }
+            *reinterpret_cast<uint4 *>(dst + p0) = x;
         }
     };
     if (page >= 0)
-        for (int i = tid; i < n * hn * units; i += APPEND_THREADS) {
-            const int u = i % units, h = h0 + i / units % hn, t = i / (units * hn);
-            turn_head(static_cast<const T *>(a.d_k) + (row0 + t) * a.k_token + h * a.k_head,
-                      k_pages + (((int64_t)page * a.kv_heads + h) * a.block + (lo + t) % a.block) * D, u, turn + t * n_freq);
-        }
+        turn_rows(static_cast<const T *>(a.d_k) + row0 * a.k_token + h0 * a.k_head, a.k_token, a.k_head, n * (int)div_k.d, div_k, hn,
+                  [&](int t, int h) { return k_pages + at0 + (h * a.block + (lo + t) % a.block) * D; });
     if (a.d_o) {
-        const int qh = hn * G;
-        for (int i = tid; i < n * qh * units; i += APPEND_THREADS) {
-            const int u = i % units, h = h0 * G + i / units % qh, t = i / (units * qh);
-            turn_head(static_cast<const T *>(a.d_q) + (row0 + t) * a.q_token + h * a.q_head,
-                      static_cast<T *>(a.d_o) + (row0 + t) * a.o_token + h * a.o_head, u, turn + t * n_freq);
-        }
+        T *out = static_cast<T *>(a.d_o) + row0 * a.o_token + (int64_t)h0 * G * a.o_head;
+        turn_rows(static_cast<const T *>(a.d_q) + row0 * a.q_token + (int64_t)h0 * G * a.q_head, a.q_token, a.q_head, n * (int)div_q.d, div_q,
+                  hn * G, [&](int t, int h) { return out + t * a.o_token + h * a.o_head; });
     }
     if (page < 0 || !key_sums) return;
     // the sum of all keys that the page holds: columns of 8 values, the rows dealt out to groups of threads
@@ -173,7 +183,7 @@ static int append_launch(const spamm_attn &a, void *k_pages, void *v_pages, floa
     int st = attn_set_smem((const void *)attn_append_kernel<T, D>, smem);
     if (st) return st;
     attn_append_kernel<T, D><<<dim3((unsigned)grid, split), APPEND_THREADS, smem, stream>>>(
-        a, (int)per, heads_per_cta, static_cast<T *>(k_pages), static_cast<T *>(v_pages), key_sums, inv_freq, n_freq, interleaved != 0);
+        a, (int)per, heads_per_cta, fast_div(heads_per_cta), fast_div(heads_per_cta * (a.heads / a.kv_heads)), static_cast<T *>(k_pages), static_cast<T *>(v_pages), key_sums, inv_freq, n_freq, interleaved != 0);
     SPAMM_CUDA_TRY(cudaGetLastError());
     return SPAMM_OK;
 }

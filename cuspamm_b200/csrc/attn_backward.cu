@@ -669,7 +669,10 @@ __global__ __launch_bounds__(TQ_THREADS, 2) void attn_dq_tc_kernel(const __grid_
 // tile, the products of the tile before and of the one behind it run, and four warps gather the rows of the one after.
 // With D = 64 the tiles of dO and Q together are the 128 rows of the second products' A: dV^T comes out in the upper half
 // of one accumulator, dK^T in the lower half of the other (the other halves are not used).
-constexpr int TK_ROWS = 128, TK_MAX_KEYS = 64, TK_SOFTMAX = 256, TK_THREADS = TK_SOFTMAX + 32 + 128, TK_COLS = 512;
+constexpr int TK_ROWS = 128, TK_MAX_KEYS = 64, TK_SOFTMAX = 256, TK_THREADS = TK_SOFTMAX + 32 + 128;
+// Tensor memory columns, and blocks of threads per SM: short blocks of small heads leave room for two.
+__host__ __device__ constexpr int tk_cols(int keys) { return keys == 64 ? 512 : keys == 32 ? 256 : 128; }
+__host__ __device__ constexpr int tk_per_sm(int dim, int keys) { return dim == 64 && keys < 64 ? 2 : 1; }
 
 struct TkCtrl {
     uint64_t kv_full, r_full[2], r_empty[2], s_full[2], p_full, dv_done, ds_full, dk_done;
@@ -680,7 +683,7 @@ struct TkCtrl {
 };
 
 template <typename T, int D, int TK_KEYS>
-__global__ __launch_bounds__(TK_THREADS, 1) void attn_dkv_tc_kernel(const __grid_constant__ spamm_attn a, const __grid_constant__ BackwardPlan p,
+__global__ __launch_bounds__(TK_THREADS, tk_per_sm(D, TK_KEYS)) void attn_dkv_tc_kernel(const __grid_constant__ spamm_attn a, const __grid_constant__ BackwardPlan p,
                                                                     const __grid_constant__ RowMap q_map,
                                                                     const __grid_constant__ RowMap do_map,
                                                                     const T *d_do, int64_t do_token, int64_t do_head,
@@ -729,7 +732,7 @@ __global__ __launch_bounds__(TK_THREADS, 1) void attn_dkv_tc_kernel(const __grid
             asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         }
         __syncwarp();
-        tmem_alloc<TK_COLS>(smem_u32(&ctrl->tmem_base));
+        tmem_alloc<tk_cols(TK_KEYS)>(smem_u32(&ctrl->tmem_base));
         tc_fence_before();
     }
     const int n_list = expand_bits<TK_THREADS>(bits + (group * p.nkb + item.kb) * p.words, p.words, item.chunk * p.chunk, p.chunk,
@@ -1005,7 +1008,7 @@ __global__ __launch_bounds__(TK_THREADS, 1) void attn_dkv_tc_kernel(const __grid
         if (ctrl->abort_flag) drain_products();
         __syncwarp();
         tc_fence_after();
-        tmem_free<TK_COLS>(tmem);
+        tmem_free<tk_cols(TK_KEYS)>(tmem);
     }
 }
 

@@ -965,8 +965,11 @@ static RowsPlan rows_plan(const spamm_attn &a)
     const int64_t listed = (int64_t)(p.pairs ? 2 : 1) * attn_tile_lists(a) * a.n_select;       // blocks of a union
     const int64_t most = !tc ? SPAMM_ATTN_MAX_SELECT : !a.n_select ? blocks : listed <= TC_ENTRIES ? UNION_BLOCKS : TC_ENTRIES;
     const int64_t units = (int64_t)a.batch * a.kv_heads * p.nqb * p.tiles;
-    // enough blocks of threads to fill 148 SMs several times over, ranges of 1024 (256) keys at the least
-    int64_t want = (tc ? a.n_select ? 148 : 740 : 600) / units + 1;
+    // Tiles of 128 rows: enough blocks of threads to fill 148 SMs several times over (with lists the work is short as it is:
+    // once), ranges of 1024 keys at the least.  Tiles of 16: two blocks per SM; lists are of one length, so one wave of equal
+    // ranges does (296 blocks: 25 us against 30 us with 600 for 64 lists of 2048 keys), whole sequences are not, and two waves
+    // even them out.
+    int64_t want = (tc ? a.n_select ? 148 : 740 : a.n_select ? 296 : 600) / units + (tc || !a.n_select);
     want = max((int64_t)1, min(want, (blocks * a.block + (tc ? 1023 : 255)) / (tc ? 1024 : 256)));
     int64_t per = min(most, (blocks + want - 1) / want);
     p.n_split = (int)((blocks + per - 1) / per);
