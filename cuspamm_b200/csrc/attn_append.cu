@@ -77,10 +77,26 @@ __global__ __launch_bounds__(APPEND_THREADS) void attn_append_kernel(const __gri
         if (tid == 0) *a.d_status = SPAMM_ERR_INVALID;
         page = -1;
     }
-    for (int i = tid; i < n * n_freq; i += APPEND_THREADS) {
+    // Sines and cosines in double are the dearest part of a prompt's append, so that of position lo + 8 x + y is put together
+    // from those of (lo + 8 x) and y by the sums' formula, in double (11 pairs instead of 32 for a page of 32; every angle is
+    // exact, 24 bits of frequency times the position, and the formula's rounding is 2^-29 of the float's that follows).
+    double2 *far = reinterpret_cast<double2 *>(smem + ((size_t)min(a.max_q, a.block) * n_freq * sizeof(float2) + 15) / 16 * 16);
+    const int n_far = (n + 7) / 8, n_near = min(n, 8);
+    for (int i = tid; i < (n_far + n_near - 1) * n_freq; i += APPEND_THREADS) {
+        const int x = i / n_freq, f = i - x * n_freq;
         double sn, cs;
-        sincos((double)(lo + i / n_freq) * (double)inv_freq[i % n_freq], &sn, &cs);
-        turn[i] = make_float2((float)cs, (float)sn);
+        sincos((double)(x < n_far ? lo + 8 * x : x - n_far + 1) * (double)inv_freq[f], &sn, &cs);
+        far[i] = make_double2(cs, sn);
+    }
+    __syncthreads();
+    for (int i = tid; i < n * n_freq; i += APPEND_THREADS) {
+        const int t = i / n_freq, f = i - t * n_freq;
+        double2 z = far[(t >> 3) * n_freq + f];
+        if (t & 7) {
+            const double2 w = far[(n_far + (t & 7) - 1) * n_freq + f];
+            z = make_double2(z.x * w.x - z.y * w.y, z.y * w.x + z.x * w.y);
+        }
+        turn[i] = make_float2((float)z.x, (float)z.y);
     }
     __syncthreads();
 
@@ -179,7 +195,8 @@ static int append_launch(const spamm_attn &a, void *k_pages, void *v_pages, floa
     const int heads_per_cta = ceil_div(a.kv_heads, split);
     split = ceil_div(a.kv_heads, heads_per_cta);
     const int tokens = min(a.max_q, a.block);
-    const size_t smem = max((size_t)tokens * n_freq * sizeof(float2), (size_t)APPEND_THREADS * 8 * sizeof(double));
+    const size_t turns = ((size_t)tokens * n_freq * sizeof(float2) + 15) / 16 * 16 + (size_t)(ceil_div(tokens, 8) + 7) * n_freq * sizeof(double2);
+    const size_t smem = max(turns, (size_t)APPEND_THREADS * 8 * sizeof(double));
     int st = attn_set_smem((const void *)attn_append_kernel<T, D>, smem);
     if (st) return st;
     attn_append_kernel<T, D><<<dim3((unsigned)grid, split), APPEND_THREADS, smem, stream>>>(
