@@ -675,7 +675,7 @@ __host__ __device__ constexpr int tk_cols(int keys) { return keys == 64 ? 512 : 
 __host__ __device__ constexpr int tk_per_sm(int dim, int keys) { return dim == 64 && keys < 64 ? 2 : 1; }
 
 struct TkCtrl {
-    uint64_t kv_full, r_full[2], r_empty[2], s_full[2], p_full, dv_done, ds_full, dk_done;
+    uint64_t kv_full, q_full[2], q_empty[2], do_full[2], do_empty[2], s_full[2], p_full, dv_done, ds_full, dk_done;
     uint32_t tmem_base;
     uint32_t abort_flag;
     int32_t err;
@@ -719,8 +719,10 @@ __global__ __launch_bounds__(TK_THREADS, tk_per_sm(D, TK_KEYS)) void attn_dkv_tc
         if (lane == 0) {
             mbar_init(smem_u32(&ctrl->kv_full), 128);
             for (int i = 0; i < 2; i++) {
-                mbar_init(smem_u32(&ctrl->r_full[i]), 128);
-                mbar_init(smem_u32(&ctrl->r_empty[i]), 1);
+                mbar_init(smem_u32(&ctrl->q_full[i]), 64);
+                mbar_init(smem_u32(&ctrl->do_full[i]), 64);
+                mbar_init(smem_u32(&ctrl->q_empty[i]), 1);
+                mbar_init(smem_u32(&ctrl->do_empty[i]), 1);
                 mbar_init(smem_u32(&ctrl->s_full[i]), 1);
             }
             mbar_init(smem_u32(&ctrl->p_full), TK_SOFTMAX);
@@ -754,16 +756,24 @@ __global__ __launch_bounds__(TK_THREADS, tk_per_sm(D, TK_KEYS)) void attn_dkv_tc
     };
 
     if (warp > 8) {
-        // ---- rows of Q and dO; K and V first
-        const int t = tid - TK_SOFTMAX - 32, lw = t >> 5;
-        for (int x = t; x < TK_KEYS * (D / 8); x += 128) {
-            const int r = x / (D / 8), c = x % (D / 8);
-            const bool ok = r < keys;
-            const int64_t row = sq.row0 + pos0 + (ok ? r : 0);
-            cp_async16(k_tile + panel_off(TK_KEYS, r, c), static_cast<const T *>(a.d_k) + row * a.k_token + h * a.k_head + c * 8, ok);
-            cp_async16(v_tile + panel_off(TK_KEYS, r, c), static_cast<const T *>(a.d_v) + row * a.v_token + h * a.v_head + c * 8, ok);
+        // ---- rows: two warps bring those of dO (and V first), two those of Q (and K first), each as its buffers come free
+        const int t = (tid - TK_SOFTMAX - 32) & 63, lw = t >> 5;
+        const bool is_q = tid - TK_SOFTMAX - 32 >= 64;
+        const T *src = is_q ? static_cast<const T *>(a.d_q) : d_do;
+        const int64_t token = is_q ? a.q_token : do_token, stride = is_q ? a.q_head : do_head;
+        uint64_t *full = is_q ? ctrl->q_full : ctrl->do_full, *empty = is_q ? ctrl->q_empty : ctrl->do_empty;
+        const uint32_t my_ring = ring + (is_q ? RT : 0);
+        {
+            const T *kv = is_q ? static_cast<const T *>(a.d_k) : static_cast<const T *>(a.d_v);
+            const int64_t kv_token = is_q ? a.k_token : a.v_token, kv_head = is_q ? a.k_head : a.v_head;
+            const uint32_t tile = is_q ? k_tile : v_tile;
+            for (int x = t; x < TK_KEYS * (D / 8); x += 64) {
+                const int r = x / (D / 8), c = x % (D / 8);
+                const bool ok = r < keys;
+                cp_async16(tile + panel_off(TK_KEYS, r, c), kv + (int64_t)(sq.row0 + pos0 + (ok ? r : 0)) * kv_token + h * kv_head + c * 8, ok);
+            }
+            cp_commit();
         }
-        cp_commit();
         constexpr int PASS = 32 / (D / 8);                      // rows of a warp's copy
         const int col = lane % (D / 8), sub = lane / (D / 8);
         bool fine = true;
@@ -772,56 +782,58 @@ __global__ __launch_bounds__(TK_THREADS, tk_per_sm(D, TK_KEYS)) void attn_dkv_tc
             mbar_arrive(smem_u32(bar));
         };
         // whole tiles by tensor copies; the one in which the rows end, or all when the strides do not allow it, row by row
-        const int by_map = p.box_tokens && q_map.usable && do_map.usable && !q_map.swapped && !do_map.swapped ? n_rows / TK_ROWS : 0;
+        const RowMap &map = is_q ? q_map : do_map;
+        const int by_map = p.box_tokens && map.usable && !map.swapped ? n_rows / TK_ROWS : 0;
         if (by_map) {
-            cp_wait<0>();
-            signal(&ctrl->kv_full);
             const int box_rows = p.box_tokens * G, boxes = TK_ROWS / box_rows;
+            const int i = t % boxes, panel = t / boxes;
             for (int j = 0; j < by_map; j++) {
-                if (j > 1) fine = __all_sync(~0u, ws.wait(smem_u32(&ctrl->r_empty[j & 1]), (j >> 1) - 1, 1));
+                if (j > 1) fine = __all_sync(~0u, ws.wait(smem_u32(&empty[j & 1]), (j >> 1) - 1, 1));
                 if (!fine) break;
-                const uint32_t do_dst = ring + (j & 1) * 2 * RT, q_dst = do_dst + RT, bar = smem_u32(&ctrl->r_full[j & 1]);
-                const int i = t % boxes, what = t / boxes;          // box; panel and tensor
-                if (what < 2 * (D / 64)) {
-                    const int panel = what >> 1;
+                const uint32_t bar = smem_u32(&full[j & 1]);
+                if (panel < D / 64) {
                     int query, head;
                     locate(j * TK_ROWS + i * box_rows, &query, &head);
-                    const uint32_t off = panel * (TK_ROWS * 128) + i * box_rows * 128;
                     mbar_expect_tx(bar, box_rows * 128);
-                    if (what & 1) tma_box(do_dst + off, &do_map.map, panel * 64, head, sq.row0 + query, bar);
-                    else tma_box(q_dst + off, &q_map.map, panel * 64, head, sq.row0 + query, bar);
+                    tma_box(my_ring + (j & 1) * 2 * RT + panel * (TK_ROWS * 128) + i * box_rows * 128, &map.map, panel * 64, head,
+                            sq.row0 + query, bar);
                 }
                 mbar_arrive(bar);
+                if (j == 0) {
+                    cp_wait<0>();
+                    signal(&ctrl->kv_full);
+                }
             }
         }
         for (int j = by_map; j <= n_tiles && fine; j++) {
             if (j > 1 && j > by_map) {
                 // the buffer comes free only when the tile before has been worked on: announce that one first
                 cp_wait<0>();
-                signal(&ctrl->r_full[(j - 1) & 1]);
+                signal(&full[(j - 1) & 1]);
             }
             if (j < n_tiles) {
-                if (j > 1) fine = __all_sync(~0u, ws.wait(smem_u32(&ctrl->r_empty[j & 1]), (j >> 1) - 1, 1));
+                if (j > 1) fine = __all_sync(~0u, ws.wait(smem_u32(&empty[j & 1]), (j >> 1) - 1, 1));
                 if (!fine) break;
-                // each lane finds one of the warp's 32 rows, the copies take the addresses from it
-                int query = 0, head = 0;
-                const bool there = locate(j * TK_ROWS + lw * 32 + lane, &query, &head);
-                const int64_t q_at = there ? (int64_t)(sq.row0 + query) * a.q_token + head * a.q_head : -1;
-                const int64_t do_at = (int64_t)(sq.row0 + query) * do_token + head * do_head;
-                const uint32_t do_dst = ring + (j & 1) * 2 * RT, q_dst = do_dst + RT;
+                const uint32_t dst = my_ring + (j & 1) * 2 * RT;
+#pragma unroll 1
+                for (int half_tile = 0; half_tile < 2; half_tile++) {
+                    // each lane finds one of 32 rows, the copies take the addresses from it
+                    const int r0 = lw * 64 + half_tile * 32;
+                    int query = 0, head = 0;
+                    const bool there = locate(j * TK_ROWS + r0 + lane, &query, &head);
+                    const int64_t at = there ? (int64_t)(sq.row0 + query) * token + head * stride : -1;
 #pragma unroll 4
-                for (int i = 0; i < 32; i += PASS) {
-                    const int r = i + sub;
-                    const int64_t qa = __shfl_sync(~0u, q_at, r), da = __shfl_sync(~0u, do_at, r);
-                    const uint32_t off = panel_off(TK_ROWS, lw * 32 + r, col);
-                    cp_async16(q_dst + off, static_cast<const T *>(a.d_q) + (qa < 0 ? 0 : qa) + col * 8, qa >= 0);
-                    cp_async16(do_dst + off, d_do + (qa < 0 ? 0 : da) + col * 8, qa >= 0);
+                    for (int i = 0; i < 32; i += PASS) {
+                        const int r = i + sub;
+                        const int64_t from = __shfl_sync(~0u, at, r);
+                        cp_async16(dst + panel_off(TK_ROWS, r0 + r, col), src + (from < 0 ? 0 : from) + col * 8, from >= 0);
+                    }
                 }
             }
             cp_commit();
             if (j <= 1 && !by_map) {
-                cp_wait<1>();                                   // the group before: K and V, or the rows of the first tile
-                signal(j ? &ctrl->r_full[0] : &ctrl->kv_full);
+                cp_wait<1>();                                   // the group before: K or V, or the rows of the first tile
+                signal(j ? &full[0] : &ctrl->kv_full);
             }
         }
         cp_wait<0>();
@@ -835,35 +847,45 @@ __global__ __launch_bounds__(TK_THREADS, tk_per_sm(D, TK_KEYS)) void attn_dkv_tc
             const uint64_t dot_desc = desc_mn_major(ring, TK_ROWS), qt_desc = desc_mn_major(D == 64 ? ring : ring + RT, TK_ROWS);
             const uint64_t p_desc = desc_mn_major(p_tile, TK_ROWS), ds_desc = desc_mn_major(ds_tile, TK_ROWS);
             bool fine = __all_sync(~0u, ws.wait(smem_u32(&ctrl->kv_full), 0, 2));
-            // whichever of the two is ready: the first products of the next tile, when its rows are there and at most one
-            // tile is under way, or the second products of the oldest tile under way.  (In a fixed order the second
-            // products would wait for the copies of the next tile, which wait for their buffer, which they free.)
-            int first = 0, second = 0;
+            // Whichever is ready: dP of the next tile (at most one tile under way), its S, or the second products of the oldest
+            // tile under way.  dO comes free after dV, before Q does, and returns before it: hence dP before S.  (In a fixed
+            // order the second products would wait for the copies of the next tile, which wait for the buffers that they free.)
+            int next_dp = 0, next_s = 0, second = 0;
             unsigned long long t0 = 0;
             while (second < n_tiles) {
-                if (first < n_tiles && first - second < 2 &&
-                    __all_sync(~0u, mbar_test(smem_u32(&ctrl->r_full[first & 1]), (first >> 1) & 1))) {
+                const uint32_t dp_stage = (next_dp & 1) * (2 * RT >> 4), s_stage = (next_s & 1) * (2 * RT >> 4);
+                if (next_s < next_dp && __all_sync(~0u, mbar_test(smem_u32(&ctrl->q_full[next_s & 1]), (next_s >> 1) & 1))) {
                     tc_fence_after();
-                    const uint32_t stage = (first & 1) * (2 * RT >> 4), s_at = base + (first & 1) * 2 * TK_KEYS;
                     if (elect_one()) {
 #pragma unroll
                         for (int ks = 0; ks < D / 16; ks++)
-                            mma_ss(s_at, q_desc + stage + step_k_major(TK_ROWS, ks), k_desc + step_k_major(TK_KEYS, ks), s_desc, ks != 0);
-#pragma unroll
-                        for (int ks = 0; ks < D / 16; ks++)
-                            mma_ss(s_at + TK_KEYS, do_desc + stage + step_k_major(TK_ROWS, ks), v_desc + step_k_major(TK_KEYS, ks), s_desc, ks != 0);
-                        umma_commit(smem_u32(&ctrl->s_full[first & 1]));
+                            mma_ss(base + (next_s & 1) * 2 * TK_KEYS, q_desc + s_stage + step_k_major(TK_ROWS, ks), k_desc + step_k_major(TK_KEYS, ks),
+                                   s_desc, ks != 0);
+                        umma_commit(smem_u32(&ctrl->s_full[next_s & 1]));
                     }
                     __syncwarp();
-                    first++;
+                    next_s++;
                     t0 = 0;
-                } else if (second < first && __all_sync(~0u, mbar_test(smem_u32(&ctrl->p_full), second & 1))) {
+                } else if (next_dp < n_tiles && next_dp - second < 2 &&
+                           __all_sync(~0u, mbar_test(smem_u32(&ctrl->do_full[next_dp & 1]), (next_dp >> 1) & 1))) {
+                    tc_fence_after();
+                    if (elect_one()) {
+#pragma unroll
+                        for (int ks = 0; ks < D / 16; ks++)
+                            mma_ss(base + (next_dp & 1) * 2 * TK_KEYS + TK_KEYS, do_desc + dp_stage + step_k_major(TK_ROWS, ks),
+                                   v_desc + step_k_major(TK_KEYS, ks), s_desc, ks != 0);
+                    }
+                    __syncwarp();
+                    next_dp++;
+                    t0 = 0;
+                } else if (second < next_s && __all_sync(~0u, mbar_test(smem_u32(&ctrl->p_full), second & 1))) {
                     tc_fence_after();
                     const uint32_t stage = (second & 1) * (2 * RT >> 4);
                     if (elect_one()) {
 #pragma unroll
                         for (int ks = 0; ks < TK_ROWS / 16; ks++)
                             mma_ss(base + 4 * TK_KEYS, dot_desc + stage + step_mn_major(ks), p_desc + step_mn_major(ks), o_desc, second || ks);
+                        if (D == 128) umma_commit(smem_u32(&ctrl->do_empty[second & 1]));
                         umma_commit(smem_u32(&ctrl->dv_done));
                     }
                     __syncwarp();
@@ -874,7 +896,8 @@ __global__ __launch_bounds__(TK_THREADS, tk_per_sm(D, TK_KEYS)) void attn_dkv_tc
 #pragma unroll
                         for (int ks = 0; ks < TK_ROWS / 16; ks++)
                             mma_ss(base + 5 * TK_KEYS, qt_desc + stage + step_mn_major(ks), ds_desc + step_mn_major(ks), o_desc, second || ks);
-                        umma_commit(smem_u32(&ctrl->r_empty[second & 1]));
+                        if (D == 64) umma_commit(smem_u32(&ctrl->do_empty[second & 1]));      // dO is half of this A too
+                        umma_commit(smem_u32(&ctrl->q_empty[second & 1]));
                         umma_commit(smem_u32(&ctrl->dk_done));
                     }
                     __syncwarp();
