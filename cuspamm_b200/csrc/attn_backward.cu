@@ -1050,10 +1050,11 @@ __global__ __launch_bounds__(128) void attn_dkv_join_kernel(const __grid_constan
     if (chunks <= 1) return;
     const int64_t tile = 2 * (int64_t)a.block * a.dim;
     const float *src = partial + (group * p.slot_cap + slots[group * p.nkb + kb]) * tile;
-    for (int i = threadIdx.x; i < 2 * keys * a.dim / 4; i += 128) {
+    for (int i = blockIdx.y * 128 + threadIdx.x; i < 2 * keys * a.dim / 4; i += 128 * gridDim.y) {
         const int which = i >= keys * a.dim / 4;
         const int x = (i - which * (keys * a.dim / 4)) * 4;
         float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
         for (int c = 0; c < chunks; c++) {
             const float4 z = *reinterpret_cast<const float4 *>(src + c * tile + which * a.block * a.dim + x);
             y.x += z.x; y.y += z.y; y.z += z.z; y.w += z.w;
@@ -1130,7 +1131,7 @@ static int backward_launch(const spamm_attn &a, const BackwardPlan &p, const T *
     }
     if (st) return st;
     if (p.nqb > p.chunk)
-        attn_dkv_join_kernel<T><<<(unsigned)(p.groups * p.nkb), 128, 0, stream>>>(a, p, counts, slots, partial, dk, dv);
+        attn_dkv_join_kernel<T><<<dim3((unsigned)(p.groups * p.nkb), 8), 128, 0, stream>>>(a, p, counts, slots, partial, dk, dv);
     SPAMM_CUDA_TRY(cudaGetLastError());
     return SPAMM_OK;
 }
