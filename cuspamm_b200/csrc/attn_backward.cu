@@ -397,6 +397,7 @@ struct TqCtrl {
     uint32_t abort_flag;
     int32_t err;
     int32_t count;
+    uint32_t odd[4];                    // rows whose result is not finite
 };
 
 template <typename T, int D>
@@ -454,6 +455,7 @@ __global__ __launch_bounds__(TQ_THREADS, 2) void attn_dq_tc_kernel(const __grid_
             mbar_init(smem_u32(&ctrl->dq_done), 1);
             ctrl->abort_flag = 0;
             ctrl->err = 0;
+            for (int i = 0; i < 4; i++) ctrl->odd[i] = 0;
             asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         }
         __syncwarp();
@@ -621,6 +623,7 @@ __global__ __launch_bounds__(TQ_THREADS, 2) void attn_dq_tc_kernel(const __grid_
         if (n_tiles && fine) fine = __all_sync(~0u, ws.wait(smem_u32(&ctrl->dq_done), n_tiles - 1, 8));
         tc_fence_after();
         __syncthreads();                                       // every copy has landed, every product is done
+        bool odd = false;
 #pragma unroll 1
         for (int c = 0; c < D / 64; c++) {
             uint32_t v[32];
@@ -632,6 +635,8 @@ __global__ __launch_bounds__(TQ_THREADS, 2) void attn_dq_tc_kernel(const __grid_
 #pragma unroll
             for (int i = 0; i < 32; i++) v[i] = !fine ? 0x7fc00000u : n_tiles ? v[i] : 0u;
 #pragma unroll
+            for (int i = 0; i < 32; i++) odd |= not_finite(v[i]);
+#pragma unroll
             for (int i = 0; i < 4; i++) {
                 uint32_t x[4];
 #pragma unroll
@@ -640,7 +645,38 @@ __global__ __launch_bounds__(TQ_THREADS, 2) void attn_dq_tc_kernel(const __grid_
                 *reinterpret_cast<uint4 *>(smem + row_piece(D * 2, r, half * (D / 16) + c * 4 + i)) = *reinterpret_cast<uint4 *>(x);
             }
         }
+        const unsigned rows_odd = __ballot_sync(~0u, odd && fine && r < rows);
+        if (rows_odd && lane == 0) atomicOr(&ctrl->odd[warp & 3], rows_odd);
         asm volatile("bar.sync 1, 256;" ::: "memory");
+        if (ctrl->odd[0] | ctrl->odd[1] | ctrl->odd[2] | ctrl->odd[3]) {
+#pragma unroll 1
+            for (int sr = warp; sr < rows; sr += 8) {
+                if (!(ctrl->odd[sr >> 5] >> (sr & 31) & 1)) continue;
+                const int sy = tr.row0 + sr, tok = (int)shape.G.quotient(sy), head = h * G + sy - tok * G;
+                const int64_t row = sq.row0 + tok, at_row = row * a.heads + head;
+                const uint32_t bit = 1u << (tok / a.query_block - tr.qb0);
+                const float lse = a.d_lse[at_row], dl = delta[at_row];
+                const float row_lse = lse == -CUDART_INF_F ? -CUDART_INF_F : -lse * LOG2E;
+                float q[D / 32], g[D / 32], kx[D / 32], vx[D / 32], y2[D / 32] = {};
+                row_load<T, D>(static_cast<const T *>(a.d_q) + row * a.q_token + head * a.q_head, lane, q);
+                row_load<T, D>(d_do + row * do_token + head * do_head, lane, g);
+                row_keys<T>(a, sq, s, h, n_entries, attn_limit(a, sq, tok), [&](int e) { return bits[e] & bit ? (int)blk[e] : -1; },
+                            [&](const T *kr, const T *vr) {
+                                row_load<T, D>(kr, lane, kx);
+                                row_load<T, D>(vr, lane, vx);
+                                const float pr = fast_exp2(fmaf(row_dot<D>(q, kx), scale2, row_lse));
+                                const float ds = pr * (row_dot<D>(g, vx) - dl) * a.scale;
+#pragma unroll
+                                for (int i = 0; i < D / 32; i++) y2[i] = fmaf(ds, kx[i], y2[i]);
+                            });
+#pragma unroll
+                for (int i = 0; i < D / 32; i += 2) {
+                    const int piece = (lane * (D / 32) + i) * 2;
+                    *reinterpret_cast<uint32_t *>(smem + row_piece(D * 2, sr, piece >> 4) + (piece & 15)) = Pack<T>::two(y2[i], y2[i + 1]);
+                }
+            }
+            asm volatile("bar.sync 1, 256;" ::: "memory");
+        }
         const int c = tid % (D / 8);
         for (int sr = tid / (D / 8); sr < rows; sr += TQ_SOFTMAX / (D / 8)) {
             const int sy = tr.row0 + sr, tok = (int)shape.G.quotient(sy);

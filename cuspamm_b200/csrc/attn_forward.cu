@@ -392,6 +392,7 @@ struct TcCtrl {
     int32_t err;
     int32_t count;
     int32_t bad_page;
+    uint32_t odd[2][4];                 // [tile]: rows whose result is not finite
     int32_t pad[3];
     float top[2][2][2][TC_ROWS];        // [tile][step & 1][half][row]
 };
@@ -462,6 +463,7 @@ __global__ __launch_bounds__(TILES * 256 + 64, TILES == 1 ? 2 : 1) void attn_tc_
             ctrl->abort_flag = 0;
             ctrl->err = 0;
             ctrl->bad_page = 0;
+            for (int i = 0; i < 8; i++) ctrl->odd[i >> 2][i & 3] = 0;
             asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         }
         __syncwarp();
@@ -766,6 +768,7 @@ __global__ __launch_bounds__(TILES * 256 + 64, TILES == 1 ? 2 : 1) void attn_tc_
         __syncthreads();
         uint8_t *const stage = smem + x0 * 3 * TILE;               // rows in the type (and their low parts behind), or in float
         const bool whole = p.n_split == 1;
+        bool odd = false;
 #pragma unroll 1
         for (int c = 0; c < D / 64 && rows; c++) {
             uint32_t v[32];
@@ -778,6 +781,8 @@ __global__ __launch_bounds__(TILES * 256 + 64, TILES == 1 ? 2 : 1) void attn_tc_
 #pragma unroll
             for (int i = 0; i < 32; i++)
                 v[i] = !fine ? 0x7fc00000u : n_done ? __float_as_uint(__uint_as_float(v[i]) * inv) : 0u;
+#pragma unroll
+            for (int i = 0; i < 32; i++) odd |= not_finite(v[i]);
             if (whole) {
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
@@ -796,7 +801,51 @@ __global__ __launch_bounds__(TILES * 256 + 64, TILES == 1 ? 2 : 1) void attn_tc_
             if (!whole) part_lse[(row * a.heads + head) * p.n_split + split] = fine ? lse2 : CUDART_NAN_F;
             else if (a.d_lse) a.d_lse[row * a.heads + head] = fine ? lse2 * LN2 : CUDART_NAN_F;
         }
+        {
+            const unsigned rows_odd = __ballot_sync(~0u, odd && fine && r < rows);
+            if (rows_odd && lane == 0) atomicOr(&ctrl->odd[x0][quad], rows_odd);
+        }
         tile_barrier(x0);
+        if (ctrl->odd[x0][0] | ctrl->odd[x0][1] | ctrl->odd[x0][2] | ctrl->odd[x0][3]) {
+#pragma unroll 1
+            for (int sr = warp & 7; sr < rows; sr += 8) {
+                if (!(ctrl->odd[x0][sr >> 5] >> (sr & 31) & 1)) continue;
+                const int sy = mine.row0 + sr, tok = (int)p.shape.G.quotient(sy), head = h * G + sy - tok * G;
+                const int64_t row = sq.row0 + tok;
+                const uint32_t bit = a.n_select ? 1u << (tok / a.query_block - mine.qb0) : 1u;
+                float q[D / 32], k[D / 32], v[D / 32], o[D / 32] = {}, top = -CUDART_INF_F, sum = 0.f;
+                row_load<T, D>(static_cast<const T *>(a.d_q) + row * a.q_token + head * a.q_head, lane, q);
+                row_keys<T>(a, sq, s, h, n_entries, attn_limit(a, sq, sq.pos0 + tok),
+                            [&](int e) { return !a.n_select || bits[x0 * p.max_entries + e] & bit ? block_of(e) : -1; },
+                            [&](const T *kr, const T *vr) {
+                                row_load<T, D>(kr, lane, k);
+                                row_load<T, D>(vr, lane, v);
+                                const float z = row_dot<D>(q, k) * scale2, next = fmaxf(top, z);
+                                const float f = top == next ? 1.f : fast_exp2(top - next), w = fast_exp2(z - (next == -CUDART_INF_F ? 0.f : next));
+                                top = next;
+                                sum = sum * f + w;
+#pragma unroll
+                                for (int i = 0; i < D / 32; i++) o[i] = o[i] * f + w * v[i];
+                            });
+                const float scale_o = sum == 0.f ? 0.f : 1.f / sum;
+                const int d0 = lane * (D / 32);
+#pragma unroll
+                for (int i = 0; i < D / 32; i += 2) {
+                    const float y0 = o[i] * scale_o, y1 = o[i + 1] * scale_o;
+                    const int piece = (d0 + i) * (whole ? 2 : 4);
+                    uint8_t *at = stage + row_piece(whole ? D * 2 : D * 4, sr, piece >> 4) + (piece & 15);
+                    if (whole) {
+                        const uint32_t x = Pack<T>::two(y0, y1);
+                        *reinterpret_cast<uint32_t *>(at) = x;
+                        const float2 back = Pack<T>::to2(x);
+                        if (a.d_o_low) *reinterpret_cast<uint32_t *>(at + TILE) = Pack<T>::two(y0 - back.x, y1 - back.y);
+                    } else {
+                        *reinterpret_cast<float2 *>(at) = make_float2(y0, y1);
+                    }
+                }
+            }
+            tile_barrier(x0);
+        }
         if (whole) {
             const int c = (tid & 255) % (D / 8);
             for (int sr = (tid & 255) / (D / 8); sr < rows; sr += 256 / (D / 8)) {

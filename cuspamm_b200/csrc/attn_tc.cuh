@@ -317,6 +317,48 @@ __device__ __forceinline__ float2 poly_exp2(float2 x)
 // shared memory first (16-byte pieces XORed with the row, no bank conflicts either way) and leave as whole rows.
 __device__ __forceinline__ uint32_t row_piece(int row_bytes, int r, int c) { return r * row_bytes + ((c ^ (r & 7)) << 4); }
 
+// ---- rows taken key by key
+//
+// A tile multiplies every row with every key of its steps, those that the row does not read with p (or ds) = 0: a NaN or an
+// infinity among their values would reach the row all the same, as 0 * NaN.  Rows whose result is not finite are therefore
+// taken again over their own keys alone, one warp for a row.  (Rows that read such a key themselves come out the same.)
+
+// Elements lane * D/32 .. of a row of D values.
+template <typename T, int D> __device__ __forceinline__ void row_load(const T *p, int lane, float *x)
+{
+#pragma unroll
+    for (int i = 0; i < D / 32; i += 2) {
+        const float2 f = Pack<T>::to2(*reinterpret_cast<const uint32_t *>(p + lane * (D / 32) + i));
+        x[i] = f.x;
+        x[i + 1] = f.y;
+    }
+}
+template <int D> __device__ __forceinline__ float row_dot(const float *x, const float *y)
+{
+    float z = 0.f;
+#pragma unroll
+    for (int i = 0; i < D / 32; i++) z = fmaf(x[i], y[i], z);
+#pragma unroll
+    for (int d = 16; d; d >>= 1) z += __shfl_xor_sync(~0u, z, d);
+    return z;
+}
+// Calls f(k row, v row) for every key below `limit` of the blocks that block(e) names for e in [0, n) (-1: not the row's).
+template <typename T, typename Block, typename F>
+__device__ __forceinline__ void row_keys(const spamm_attn &a, const Seq &sq, int s, int h, int n, int limit, Block block, F f)
+{
+    for (int e = 0; e < n; e++) {
+        const int b = block(e);
+        if (b < 0) continue;
+        const int64_t k0 = attn_block_base(a, sq, s, h, b, a.k_token, a.k_head);
+        if (k0 < 0) continue;
+        const int64_t v0 = a.n_pages ? k0 : (int64_t)(sq.row0 + b * a.block) * a.v_token + h * a.v_head;
+        const int64_t k_tok = a.n_pages ? a.dim : a.k_token, v_tok = a.n_pages ? a.dim : a.v_token;
+        const int keys = min(a.block, limit - b * a.block);
+        for (int i = 0; i < keys; i++) f(static_cast<const T *>(a.d_k) + k0 + i * k_tok, static_cast<const T *>(a.d_v) + v0 + i * v_tok);
+    }
+}
+__device__ __forceinline__ bool not_finite(uint32_t v) { return (v & 0x7f800000u) == 0x7f800000u; }
+
 // Barriers of a kernel and its abort flag: a wait that runs out (never, unless the kernel is wrong) sets the flag, every
 // role leaves its loop, and the results of the tile become NaN.
 struct WaitState {

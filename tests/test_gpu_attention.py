@@ -614,3 +614,67 @@ def test_select_many_lists(lens, H, HK, qb, block):
             want[:, :pick.shape[1]] = torch.where(pick < nb, pick, -1).cpu()
             assert torch.equal(got[s, :nqb, h].long(), want), (s, h)
         at += n
+
+
+@pytest.mark.parametrize("lens,H,HK,D,qb,block", [([200, 90], 16, 1, 128, 1, 64), ([300], 4, 2, 64, 16, 32), ([800], 4, 4, 64, 64, 64)])
+def test_infinities_and_nan_stay_with_the_rows_that_read_them(lens, H, HK, D, qb, block):
+    """Keys and values that are not finite, in blocks that some queries list and their neighbours do not: only rows that
+    read such a key may notice.  Others equal the plain form over their own keys."""
+    from cuspamm_b200 import block_sparse_attention
+
+    g = torch.Generator().manual_seed(71)
+    T = sum(lens)
+    q, k, v, d_o = (tokens(g, T, n, D, BF) for n in (H, HK, HK, H))
+    lists = random_lists(g, lens, lens, HK, block, qb, 2, True)
+    k[70, 0, 3], k[110, 0, 5], v[75, 0, 1], v[131, 0] = torch.inf, torch.nan, -torch.inf, torch.nan
+    x = [t.clone().requires_grad_() for t in (q, k, v)]
+    o = block_sparse_attention(*x, lists, cu_of(lens), max(lens), block=block, query_block=qb)
+    (dq,) = torch.autograd.grad(o, x[:1], d_o)
+    at, clean = 0, 0
+    for s, n in enumerate(lens):
+        r = slice(at, at + n)
+        for h in range(H):
+            hk = h // (H // HK)
+            ok = plain.mask_of(lists[s].cpu(), n, n, 0, block, qb, True, hk).to(DEV)
+            fine = torch.isfinite(k[r, hk]).all(1) & torch.isfinite(v[r, hk]).all(1)
+            rows = ~(ok & ~fine[None]).any(1)                      # rows that read none of them
+            clean += int(rows.sum())
+            kk, vv = k[r, hk].nan_to_num(0, 0, 0), v[r, hk].nan_to_num(0, 0, 0)
+            val, tol = plain.attend(q[r, h], kk, vv, ok, D ** -0.5, d_o[r, h])
+            near(o[r, h][rows].detach(), val["o"][rows], tol["o"][rows], "o")
+            near(dq[r, h][rows], val["dq"][rows], tol["dq"][rows], "dq")
+        at += n
+    assert clean > T                                              # most rows
+
+
+def test_offsets_beyond_four_gigabytes():
+    """A cache whose last pages lie behind 2^32 bytes and 2^31 elements."""
+    from cuspamm_b200 import PagedCache
+
+    pages, HK, D, page = 36000, 8, 128, 64
+    if torch.cuda.mem_get_info(0)[0] < 24 << 30:
+        pytest.skip("needs 24 GB")
+    g = torch.Generator().manual_seed(81)
+    k = torch.zeros(pages, HK, page, D, dtype=BF, device=DEV)
+    v = torch.zeros_like(k)
+    cache = PagedCache(k, v)
+    held = [150, 70]
+    table = torch.tensor([[35999, 0, 35998], [35997, 35000, 0]], dtype=torch.int32, device=DEV)
+    lengths = torch.tensor(held, dtype=torch.int32, device=DEV)
+    nk, nv, q = tokens(g, 220, HK, D, BF), tokens(g, 220, HK, D, BF), tokens(g, 220, HK, D, BF)
+    cache.append(nk, nv, cu_of(held), 150, table, lengths)
+    for new in ([150, 70], [1, 1]):                               # the kernels of prompts and of single tokens
+        qq = torch.cat([q[150 - new[0]:150], q[220 - new[1]:]])
+        o = cache.attend(qq, cu_of(new), max(new), table, lengths)
+        lists = cache.select(qq, cu_of(new), max(new), table, lengths, 3)
+        assert sorted(set(lists.flatten().tolist())) == ([-1, 0, 1, 2] if new[0] > 1 else [-1, 0, 1, 2])
+        listed = cache.attend(qq, cu_of(new), max(new), table, lengths, lists=lists)
+        at, src = 0, 0
+        for n, m in zip(held, new):
+            for h in range(HK):
+                ok = plain.mask_of(None, m, n, n - m, page, 1, True, h).to(DEV)
+                val, tol = plain.attend(qq[at:at + m, h], nk[src:src + n, h], nv[src:src + n, h], ok, D ** -0.5)
+                near(o[at:at + m, h], val["o"], tol["o"], "o")
+                near(listed[at:at + m, h], val["o"], tol["o"], "listed")
+            at, src = at + m, src + n
+    cache.check()
