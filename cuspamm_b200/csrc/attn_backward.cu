@@ -186,6 +186,26 @@ __global__ __launch_bounds__(1024) void attn_items_kernel(const __grid_constant_
     if (tid == 0) n_items[group] = min(carry.x, p.item_cap);
 }
 
+// dq of one row over its own keys alone, by one warp: y[0 .. D/32).
+template <typename T, int D, typename Block>
+static __device__ __forceinline__ void dq_row(const spamm_attn &a, const Seq &sq, int s, int h, int query, int head, const T *d_do,
+                                              int64_t do_token, int64_t do_head, const float *delta, int n, Block block, int lane, float *y)
+{
+    const int64_t row = sq.row0 + query, at = row * a.heads + head;
+    const float lse = a.d_lse[at], dl = delta[at], minus_lse = lse == -CUDART_INF_F ? -CUDART_INF_F : -lse * LOG2E;
+    float q[D / 32], g[D / 32], k[D / 32], v[D / 32];
+    row_load<T, D>(static_cast<const T *>(a.d_q) + row * a.q_token + head * a.q_head, lane, q);
+    row_load<T, D>(d_do + row * do_token + head * do_head, lane, g);
+    row_keys<T>(a, sq, s, h, n, attn_limit(a, sq, query), block, [&](const T *kr, const T *vr) {
+        row_load<T, D>(kr, lane, k);
+        row_load<T, D>(vr, lane, v);
+        const float p = fast_exp2(fmaf(row_dot<D>(q, k), a.scale * LOG2E, minus_lse));
+        const float ds = p * (row_dot<D>(g, v) - dl) * a.scale;
+#pragma unroll
+        for (int i = 0; i < D / 32; i++) y[i] = fmaf(ds, k[i], y[i]);
+    });
+}
+
 constexpr int DQ_STAGES = 3;
 constexpr int DQ_WARPS = 4;
 
@@ -330,12 +350,17 @@ __global__ __launch_bounds__(128) void attn_dq_rows_kernel(const __grid_constant
                 make_float2(o[n][2 * x], o[n][2 * x + 1]);
     __syncthreads();
     const int r = tid >> 3, c0 = (tid & 7) * (D / 8);
+    __shared__ unsigned odd_rows;
+    if (tid == 0) odd_rows = 0;
+    bool odd = false;
     if (r < rows) {
         float y[D / 8] = {};
 #pragma unroll
         for (int w = 0; w < DQ_WARPS; w++)
 #pragma unroll
             for (int i = 0; i < D / 8; i++) y[i] += so[(w * 16 + r) * D + c0 + i];
+#pragma unroll
+        for (int i = 0; i < D / 8; i++) odd |= not_finite(__float_as_uint(y[i]));
         uint32_t out[D / 16];
 #pragma unroll
         for (int i = 0; i < D / 16; i++) out[i] = Pack<T>::two(y[2 * i], y[2 * i + 1]);
@@ -343,6 +368,20 @@ __global__ __launch_bounds__(128) void attn_dq_rows_kernel(const __grid_constant
         T *dst = dq + (((int64_t)sq.row0 + qb * bq + x / G) * a.heads + h * G + x % G) * D + c0;
 #pragma unroll
         for (int i = 0; i < D / 64; i++) reinterpret_cast<uint4 *>(dst)[i] = *reinterpret_cast<uint4 *>(out + 4 * i);
+    }
+    if (!__syncthreads_or(odd)) return;
+    // rows that are not finite once more, over their own keys alone (see row_keys)
+    if (odd) atomicOr(&odd_rows, 1u << r);
+    __syncthreads();
+#pragma unroll 1
+    for (int sr = warp; sr < rows; sr += DQ_WARPS) {
+        if (!(odd_rows >> sr & 1)) continue;
+        const int x = tile * 16 + sr, query = qb * bq + x / G, head = h * G + x % G;
+        float y[D / 32] = {};
+        dq_row<T, D>(a, sq, s, h, query, head, d_do, do_token, do_head, delta, shared_count, [&](int e) { return blk[e]; }, lane, y);
+        T *dst = dq + (((int64_t)sq.row0 + query) * a.heads + head) * D + lane * (D / 32);
+#pragma unroll
+        for (int i = 0; i < D / 32; i += 2) *reinterpret_cast<uint32_t *>(dst + i) = Pack<T>::two(y[i], y[i + 1]);
     }
 }
 
@@ -653,22 +692,10 @@ __global__ __launch_bounds__(TQ_THREADS, 2) void attn_dq_tc_kernel(const __grid_
             for (int sr = warp; sr < rows; sr += 8) {
                 if (!(ctrl->odd[sr >> 5] >> (sr & 31) & 1)) continue;
                 const int sy = tr.row0 + sr, tok = (int)shape.G.quotient(sy), head = h * G + sy - tok * G;
-                const int64_t row = sq.row0 + tok, at_row = row * a.heads + head;
                 const uint32_t bit = 1u << (tok / a.query_block - tr.qb0);
-                const float lse = a.d_lse[at_row], dl = delta[at_row];
-                const float row_lse = lse == -CUDART_INF_F ? -CUDART_INF_F : -lse * LOG2E;
-                float q[D / 32], g[D / 32], kx[D / 32], vx[D / 32], y2[D / 32] = {};
-                row_load<T, D>(static_cast<const T *>(a.d_q) + row * a.q_token + head * a.q_head, lane, q);
-                row_load<T, D>(d_do + row * do_token + head * do_head, lane, g);
-                row_keys<T>(a, sq, s, h, n_entries, attn_limit(a, sq, tok), [&](int e) { return bits[e] & bit ? (int)blk[e] : -1; },
-                            [&](const T *kr, const T *vr) {
-                                row_load<T, D>(kr, lane, kx);
-                                row_load<T, D>(vr, lane, vx);
-                                const float pr = fast_exp2(fmaf(row_dot<D>(q, kx), scale2, row_lse));
-                                const float ds = pr * (row_dot<D>(g, vx) - dl) * a.scale;
-#pragma unroll
-                                for (int i = 0; i < D / 32; i++) y2[i] = fmaf(ds, kx[i], y2[i]);
-                            });
+                float y2[D / 32] = {};
+                dq_row<T, D>(a, sq, s, h, tok, head, d_do, do_token, do_head, delta, n_entries,
+                             [&](int e) { return bits[e] & bit ? (int)blk[e] : -1; }, lane, y2);
 #pragma unroll
                 for (int i = 0; i < D / 32; i += 2) {
                     const int piece = (lane * (D / 32) + i) * 2;

@@ -327,6 +327,9 @@ __global__ __launch_bounds__(128) void attn_rows_kernel(const __grid_constant__ 
         }
     __syncthreads();
     const int r = tid >> 3, c0 = (tid & 7) * (D / 8);
+    __shared__ unsigned odd_rows;
+    if (tid == 0) odd_rows = 0;
+    bool odd = false;
     if (r < rows) {
         float top = -CUDART_INF_F, f[ROWS_WARPS], total = 0.f;
 #pragma unroll
@@ -345,6 +348,8 @@ __global__ __launch_bounds__(128) void attn_rows_kernel(const __grid_constant__ 
         for (int w = 0; w < ROWS_WARPS; w++)
 #pragma unroll
             for (int i = 0; i < D / 8; i++) y[i] += so[(w * 16 + r) * D + c0 + i] * f[w];
+#pragma unroll
+        for (int i = 0; i < D / 8; i++) odd |= not_finite(__float_as_uint(y[i] * inv));
         const int x = tile * 16 + r;
         const int64_t row = sq.row0 + qb * p.bq + x / G;
         const int head = h * G + x % G;
@@ -361,6 +366,40 @@ __global__ __launch_bounds__(128) void attn_rows_kernel(const __grid_constant__ 
 #pragma unroll
             for (int i = 0; i < D / 8; i++) part_o[at * D + c0 + i] = y[i] * inv;
             if ((tid & 7) == 0) part_lse[at] = lse2;
+        }
+    }
+    if (!__syncthreads_or(odd)) return;
+    // rows that are not finite once more, over their own keys alone (see row_keys)
+    if (odd) atomicOr(&odd_rows, 1u << r);
+    __syncthreads();
+#pragma unroll 1
+    for (int sr = warp; sr < rows; sr += ROWS_WARPS) {
+        if (!(odd_rows >> sr & 1)) continue;
+        const int x = tile * 16 + sr, query = qb * p.bq + x / G, head = h * G + x % G;
+        const int64_t row = sq.row0 + query;
+        float q[D / 32], k[D / 32], v[D / 32], y[D / 32] = {}, top = -CUDART_INF_F, sum = 0.f;
+        row_load<T, D>(static_cast<const T *>(a.d_q) + row * a.q_token + head * a.q_head, lane, q);
+        row_keys<T>(a, sq, s, h, e1 - e0, attn_limit(a, sq, sq.pos0 + query), [&](int e) { return a.n_select ? blk[e0 + e] : e0 + e; },
+                    [&](const T *kr, const T *vr) {
+                        row_load<T, D>(kr, lane, k);
+                        row_load<T, D>(vr, lane, v);
+                        online_row<D>(row_dot<D>(q, k) * scale2, v, y, &top, &sum);
+                    });
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+        const int64_t at = (row * a.heads + head) * p.n_split + split;
+#pragma unroll
+        for (int i = 0; i < D / 32; i += 2) {
+            const int d = lane * (D / 32) + i;
+            if (p.n_split == 1) {
+                const uint32_t z = Pack<T>::two(y[i] * inv, y[i + 1] * inv);
+                *reinterpret_cast<uint32_t *>(static_cast<T *>(a.d_o) + row * a.o_token + head * a.o_head + d) = z;
+                const float2 back = Pack<T>::to2(z);
+                if (a.d_o_low)
+                    *reinterpret_cast<uint32_t *>(static_cast<T *>(a.d_o_low) + (row * a.heads + head) * D + d) =
+                        Pack<T>::two(y[i] * inv - back.x, y[i + 1] * inv - back.y);
+            } else {
+                *reinterpret_cast<float2 *>(part_o + at * D + d) = make_float2(y[i] * inv, y[i + 1] * inv);
+            }
         }
     }
 }
@@ -820,12 +859,7 @@ __global__ __launch_bounds__(TILES * 256 + 64, TILES == 1 ? 2 : 1) void attn_tc_
                             [&](const T *kr, const T *vr) {
                                 row_load<T, D>(kr, lane, k);
                                 row_load<T, D>(vr, lane, v);
-                                const float z = row_dot<D>(q, k) * scale2, next = fmaxf(top, z);
-                                const float f = top == next ? 1.f : fast_exp2(top - next), w = fast_exp2(z - (next == -CUDART_INF_F ? 0.f : next));
-                                top = next;
-                                sum = sum * f + w;
-#pragma unroll
-                                for (int i = 0; i < D / 32; i++) o[i] = o[i] * f + w * v[i];
+                                online_row<D>(row_dot<D>(q, k) * scale2, v, o, &top, &sum);
                             });
                 const float scale_o = sum == 0.f ? 0.f : 1.f / sum;
                 const int d0 = lane * (D / 32);

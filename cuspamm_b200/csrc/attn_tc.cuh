@@ -357,6 +357,16 @@ __device__ __forceinline__ void row_keys(const spamm_attn &a, const Seq &sq, int
         for (int i = 0; i < keys; i++) f(static_cast<const T *>(a.d_k) + k0 + i * k_tok, static_cast<const T *>(a.d_v) + v0 + i * v_tok);
     }
 }
+// One key with the score z (times log2 e) joins a row's running maximum, sum and output.
+template <int D> __device__ __forceinline__ void online_row(float z, const float *v, float *o, float *top, float *sum)
+{
+    const float next = fmaxf(*top, z);
+    const float f = *top == next ? 1.f : fast_exp2(*top - next), w = fast_exp2(z - (next == -CUDART_INF_F ? 0.f : next));
+    *top = next;
+    *sum = *sum * f + w;
+#pragma unroll
+    for (int i = 0; i < D / 32; i++) o[i] = o[i] * f + w * v[i];
+}
 __device__ __forceinline__ bool not_finite(uint32_t v) { return (v & 0x7f800000u) == 0x7f800000u; }
 
 // Barriers of a kernel and its abort flag: a wait that runs out (never, unless the kernel is wrong) sets the flag, every

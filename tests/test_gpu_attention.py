@@ -647,6 +647,36 @@ def test_infinities_and_nan_stay_with_the_rows_that_read_them(lens, H, HK, D, qb
     assert clean > T                                              # most rows
 
 
+def test_nan_of_a_later_token_of_a_short_chunk():
+    """Four new tokens share a tile of rows; what the last one brings is seen by itself alone."""
+    from cuspamm_b200 import PagedCache, block_sparse_attention
+
+    g = torch.Generator().manual_seed(73)
+    H, HK, D, page = 4, 2, 64, 16
+    k, v, table, lengths = build_cache(g, [40], HK, D, HF, page)
+    q, cu = tokens(g, 4, H, D, HF), cu_of([4])
+    v[table[0, 39 // page].long(), :, 39 % page] = torch.nan
+    k[table[0, 38 // page].long(), 1, 38 % page, 5] = torch.inf
+    o = PagedCache(k, v).attend(q, cu, 4, table, lengths)
+    for h in range(H):
+        kk, vv = flat(k, table, 0, 40, h // 2).nan_to_num(0, 0, 0), flat(v, table, 0, 40, h // 2).nan_to_num(0, 0, 0)
+        ok = plain.mask_of(None, 4, 40, 36, page, 1, True, h // 2).to(DEV)
+        val, tol = plain.attend(q[:, h], kk, vv, ok, D ** -0.5)
+        n = 3 if h < 2 else 2
+        near(o[:n, h], val["o"][:n], tol["o"][:n], "o")
+        assert bool(torch.isnan(o[3, h]).any())
+    # the same in training: three tokens of one head
+    q, k, v, d_o = (tokens(g, 3, 1, D, BF) for _ in range(4))
+    v[2] = torch.inf
+    x = q.clone().requires_grad_()
+    lists = torch.zeros(1, 1, 1, 1, dtype=torch.int32, device=DEV)
+    o = block_sparse_attention(x, k, v, lists, cu_of([3]), 3, block=16, query_block=16)
+    (dq,) = torch.autograd.grad(o, x, d_o)
+    val, tol = plain.attend(q[:2, 0], k[:2, 0], v[:2, 0], torch.ones(2, 2, dtype=torch.bool, device=DEV).tril(), D ** -0.5, d_o[:2, 0])
+    near(o[:2, 0].detach(), val["o"], tol["o"], "o")
+    near(dq[:2, 0], val["dq"], tol["dq"], "dq")
+
+
 def test_offsets_beyond_four_gigabytes():
     """A cache whose last pages lie behind 2^32 bytes and 2^31 elements."""
     from cuspamm_b200 import PagedCache
