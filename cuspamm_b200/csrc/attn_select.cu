@@ -266,7 +266,7 @@ static __device__ void write_largest(const unsigned long long *keys, int n, int 
         low = ends[0];
         high = ends[1] + 1;                      // all keys are at or above low, fewer than n_select at or above high
         bool exact = false;
-        while (high - low > 1 && !exact) {
+        while (low < high && high - low > 1 && !exact) {
             const unsigned long long want = key_between(low, high, round);
             const int c = count([&](unsigned long long k) { return k >= want; });
             exact = c == n_select;
@@ -311,6 +311,45 @@ static __device__ void write_largest(const unsigned long long *keys, int n, int 
     }
     for (int i = min(all, n_select) + tid; i < n_select; i += THREADS) out[i] = -1;
 }
+
+// write_largest by one warp.
+static __device__ __noinline__ void pick_by_whole_keys(const unsigned long long *mine, int n, int n_select, int32_t *out, int lane)
+{
+    unsigned long long threshold = 1;
+    int left = INT32_MAX;
+    if (n > n_select) {
+        unsigned long long low = ~0ull, high = 0;
+        for (int b = lane; b < n; b += 32) {
+            low = min(low, mine[b]);
+            if (mine[b] != ~0ull) high = max(high, mine[b]);
+        }
+#pragma unroll
+        for (int d = 16; d; d >>= 1) {
+            low = min(low, __shfl_xor_sync(~0u, low, d));
+            high = max(high, __shfl_xor_sync(~0u, high, d));
+        }
+        high++;
+        bool exact = false;
+        for (int round = 0; low < high && high - low > 1 && !exact; round++) {
+            const unsigned long long want = key_between(low, high, round);
+            int c = 0;
+            for (int b = lane; b < n; b += 32) c += mine[b] >= want;
+            c = __reduce_add_sync(~0u, c);
+            exact = c == n_select;
+            if (c >= n_select) low = want;
+            else high = want;
+        }
+        threshold = low;
+        if (!exact) {
+            int above = 0;
+            for (int b = lane; b < n; b += 32) above += mine[b] > threshold;
+            left = n_select - __reduce_add_sync(~0u, above);
+        }
+    }
+    write_list(mine, n, threshold, left, n_select, out, lane);
+}
+
+constexpr int SELECT_TILE32_BLOCKS = 256;      // blocks of a sequence up to which tiles of 32 query blocks are used
 
 // ---- many query blocks: QT of them and one key head per block of threads, scores as double products on the tensor cores
 // (m8n8k4), the lists picked from shared memory
@@ -392,71 +431,73 @@ __global__ __launch_bounds__(256) void attn_select_tile_kernel(const __grid_cons
             }
         __syncthreads();
     }
-    // a warp for a list, as write_largest does it; the upper halves of the keys, kept in registers, nearly always suffice
-    for (int i = warp; i < QT; i += 8) {
-        const int qb = qt * QT + i;
-        if (qb >= nqb) break;
-        int32_t *out = lists + (((int64_t)s * nqb + qb) * a.kv_heads + h) * a.n_select;
+    if constexpr (QT == 32) {
+        // eight lanes for a list, four lists to a warp, which keeps four searches in flight; the upper halves of the keys,
+        // held in registers, nearly always suffice
+        const int g = lane >> 3, l = lane & 7, i = warp * 4 + g, qb = qt * QT + i, n = reach[i].n;
         const unsigned long long *mine = keys + i * nkb;
-        const int n = reach[i].n;
-        unsigned long long threshold = 1;
-        int left = INT32_MAX;
-        if (n > a.n_select) {
-            bool exact = false;
-            constexpr int R = 8;
-            if (n <= 32 * R) {
-                uint32_t k[R], low = ~0u, high = 0;
+        constexpr int R = SELECT_TILE32_BLOCKS / 8;
+        uint32_t k[R], low = ~0u, high = 0;
 #pragma unroll
-                for (int x = 0; x < R; x++) {
-                    k[x] = x * 32 + lane < n ? (uint32_t)(mine[x * 32 + lane] >> 32) : 0;
-                    if (x * 32 + lane < n) low = min(low, k[x]);
-                    if (k[x] != ~0u) high = max(high, k[x]);
-                }
-                low = __reduce_min_sync(~0u, low);
-                high = __reduce_max_sync(~0u, high) + 1;
-                for (int round = 0; high - low > 1 && low < high && !exact; round++) {
-                    uint32_t want = (uint32_t)(key_between((unsigned long long)low << 32, (unsigned long long)high << 32, round) >> 32);
-                    if (want == low) want++;
-                    int c = 0;
-#pragma unroll
-                    for (int x = 0; x < R; x++) c += k[x] >= want;
-                    c = __reduce_add_sync(~0u, c);
-                    exact = c == a.n_select;
-                    if (c >= a.n_select) low = want;
-                    else high = want;
-                }
-                threshold = (unsigned long long)low << 32;
-            }
-            if (!exact) {
-                unsigned long long low = ~0ull, high = 0;
-                for (int b = lane; b < n; b += 32) {
-                    low = min(low, mine[b]);
-                    if (mine[b] != ~0ull) high = max(high, mine[b]);
-                }
-#pragma unroll
-                for (int d = 16; d; d >>= 1) {
-                    low = min(low, __shfl_xor_sync(~0u, low, d));
-                    high = max(high, __shfl_xor_sync(~0u, high, d));
-                }
-                high++;
-                for (int round = 0; high - low > 1 && !exact; round++) {
-                    const unsigned long long want = key_between(low, high, round);
-                    int c = 0;
-                    for (int b = lane; b < n; b += 32) c += mine[b] >= want;
-                    c = __reduce_add_sync(~0u, c);
-                    exact = c == a.n_select;
-                    if (c >= a.n_select) low = want;
-                    else high = want;
-                }
-                threshold = low;
-            }
-            if (!exact) {
-                int above = 0;
-                for (int b = lane; b < n; b += 32) above += mine[b] > threshold;
-                left = a.n_select - __reduce_add_sync(~0u, above);
+        for (int x = 0; x < R; x++) {
+            const int b = x * 8 + l;
+            k[x] = 0;
+            if (x * 8 < n_most && b < n) {
+                k[x] = (uint32_t)(mine[b] >> 32);
+                low = min(low, k[x]);
+                if (k[x] != ~0u) high = max(high, k[x]);
             }
         }
-        write_list(mine, n, threshold, left, a.n_select, out, lane);
+#pragma unroll
+        for (int d = 1; d < 8; d <<= 1) {
+            low = min(low, __shfl_xor_sync(~0u, low, d));
+            high = max(high, __shfl_xor_sync(~0u, high, d));
+        }
+        high++;
+        const bool all = n <= a.n_select;                    // every candidate is taken
+        bool exact = all;
+        for (int round = 0; __any_sync(~0u, !exact && low < high && high - low > 1); round++) {
+            uint32_t want = (uint32_t)(key_between((unsigned long long)low << 32, (unsigned long long)high << 32, round) >> 32);
+            if (want == low) want++;
+            int c = 0;
+#pragma unroll
+            for (int x = 0; x < R; x++)
+                if (x * 8 < n_most) c += k[x] >= want;
+#pragma unroll
+            for (int d = 1; d < 8; d <<= 1) c += __shfl_xor_sync(~0u, c, d);
+            if (!exact && low < high && high - low > 1) {
+                exact = c == a.n_select;
+                if (c >= a.n_select) low = want;
+                else high = want;
+            }
+        }
+        int32_t *out = lists + (((int64_t)s * nqb + qb) * a.kv_heads + h) * a.n_select;
+        int count = 0;
+#pragma unroll
+        for (int x = 0; x < R; x++) {
+            if (x * 8 >= n_most) break;
+            const int b = x * 8 + l;
+            const bool keep = exact && b < n && (all ? mine[b] != 0 : k[x] >= low);
+            const unsigned m = __ballot_sync(~0u, keep) >> (8 * g) & 255u;
+            if (keep && qb < nqb) out[count + __popc(m & ((1u << l) - 1))] = b;
+            count += __popc(m);
+        }
+        if (exact && qb < nqb)
+            for (int x = count + l; x < a.n_select; x += 8) out[x] = -1;
+        // the rest, where upper halves are alike at the border
+        unsigned rest = __ballot_sync(~0u, !exact && l == 0 && qb < nqb);
+        while (rest) {
+            const int slow = warp * 4 + (__ffs(rest) - 1) / 8;
+            rest &= rest - 1;
+            pick_by_whole_keys(keys + slow * nkb, reach[slow].n, a.n_select,
+                               lists + (((int64_t)s * nqb + qt * QT + slow) * a.kv_heads + h) * a.n_select, lane);
+        }
+    } else {
+        for (int i = warp; i < QT; i += 8) {
+            const int qb = qt * QT + i;
+            if (qb >= nqb) break;
+            pick_by_whole_keys(keys + i * nkb, reach[i].n, a.n_select, lists + (((int64_t)s * nqb + qb) * a.kv_heads + h) * a.n_select, lane);
+        }
     }
 }
 
@@ -632,7 +673,7 @@ static SelectWay select_way(const spamm_attn &a)
 {
     const int64_t lists = (int64_t)a.batch * attn_query_blocks(a) * a.kv_heads, blocks = attn_max_blocks(a);
     if (lists < 1184) return SELECT_SPREAD;
-    if (blocks <= 256 && lists >= 32 * 296) return SELECT_TILE32;
+    if (blocks <= SELECT_TILE32_BLOCKS && lists >= 32 * 296) return SELECT_TILE32;
     if (blocks <= 1024) return SELECT_TILE8;
     return SELECT_ONE;
 }
