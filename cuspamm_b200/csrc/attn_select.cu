@@ -72,11 +72,10 @@ template <typename T> struct Sum8 {
 };
 
 template <typename T, int D>
-__global__ __launch_bounds__(256) void attn_key_sums_kernel(const __grid_constant__ spamm_attn a, int nkb, float *key_sums)
+static __device__ void key_sums_of(const spamm_attn &a, int block, int nkb, double *sums, float *key_sums)
 {
     constexpr int V = D / 8;
-    __shared__ double sums[256 * 8];
-    const int tid = threadIdx.x, s = blockIdx.x / nkb, b = blockIdx.x % nkb;
+    const int tid = threadIdx.x, s = block / nkb, b = block % nkb;
     const Seq sq = attn_seq(a, s);
     const int held = min(a.block, sq.nk - b * a.block);
     if (held <= 0) return;
@@ -147,13 +146,11 @@ __device__ __forceinline__ int64_t key_sum_row(const spamm_attn &a, const Seq &s
 // The sums of every query block's queries over the heads of a key head, double [lists][D].  WIDE: a block of threads for a
 // list (many rows), else a group of D / 8 threads.  Bound by the reading of q.
 template <typename T, int D, bool WIDE>
-__global__ __launch_bounds__(256, 4) void attn_query_sums_kernel(const __grid_constant__ spamm_attn a, int nqb, FastDiv div_g,
-                                                              double *query_sums)
+static __device__ void query_sums_of(const spamm_attn &a, int block, int nqb, const FastDiv &div_g, double *part, double *query_sums)
 {
     constexpr int V = D / 8, GROUPS = 256 / V;
-    __shared__ double part[256 * 8];
     const int tid = threadIdx.x, c = tid % V, g = tid / V, G = a.heads / a.kv_heads;
-    const int64_t list = WIDE ? blockIdx.x : (int64_t)blockIdx.x * GROUPS + g;
+    const int64_t list = WIDE ? block : (int64_t)block * GROUPS + g;
     const int64_t lists = (int64_t)a.batch * nqb * a.kv_heads;
     if (list >= lists) return;
     const int h = (int)(list % a.kv_heads), qb = (int)(list / a.kv_heads % nqb), s = (int)(list / a.kv_heads / nqb);
@@ -182,6 +179,16 @@ __global__ __launch_bounds__(256, 4) void attn_query_sums_kernel(const __grid_co
             out[d] = z;
         }
     }
+}
+
+// Both kinds of sums in one launch: the first key_blocks blocks of threads take those of the keys.
+template <typename T, int D, bool WIDE>
+__global__ __launch_bounds__(256, 4) void attn_sums_kernel(const __grid_constant__ spamm_attn a, int key_blocks, int nkb, int nqb,
+                                                           FastDiv div_g, float *key_sums, double *query_sums)
+{
+    __shared__ double part[256 * 8];
+    if ((int)blockIdx.x < key_blocks) key_sums_of<T, D>(a, blockIdx.x, nkb, part, key_sums);
+    else query_sums_of<T, D, WIDE>(a, blockIdx.x - key_blocks, nqb, div_g, part, query_sums);
 }
 
 // The number that an ordered key stands for.
@@ -382,12 +389,20 @@ __global__ __launch_bounds__(256) void attn_select_tile_kernel(const __grid_cons
         const int64_t q0 = (int64_t)(qt * QT + tid) * a.query_block;
         reach[tid] = reach_of(a, sq, q0, qt * QT + tid < nqb ? (int)min((int64_t)a.query_block, sq.nq - q0) : 0, n_local);
     }
-    for (int i = tid; i < QT * (D / 2); i += 256) {
-        const int r = i / (D / 2), c = i % (D / 2) * 2;
-        double2 x = make_double2(0.0, 0.0);
-        if ((int64_t)(qt * QT + r) * a.query_block < sq.nq)
-            x = *reinterpret_cast<const double2 *>(query_sums + (((int64_t)s * nqb + qt * QT + r) * a.kv_heads + h) * D + c);
-        *reinterpret_cast<double2 *>(qs + r * LD + c) = x;
+    // (loads in batches: the compiler may not move one above a store to shared memory)
+    {
+        constexpr int N = QT * (D / 2) / 256;
+        double2 x[N];
+        const int c = tid % (D / 2) * 2, r0 = tid / (D / 2);
+        const double *src = query_sums + (((int64_t)s * nqb + qt * QT) * a.kv_heads + h) * D + c;
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            const int r = r0 + i * (512 / D);
+            x[i] = make_double2(0.0, 0.0);
+            if ((int64_t)(qt * QT + r) * a.query_block < sq.nq) x[i] = *reinterpret_cast<const double2 *>(src + (int64_t)r * a.kv_heads * D);
+        }
+#pragma unroll
+        for (int i = 0; i < N; i++) *reinterpret_cast<double2 *>(qs + (r0 + i * (512 / D)) * LD + c) = x[i];
     }
     __syncthreads();
     int n_most = 0;
@@ -397,19 +412,26 @@ __global__ __launch_bounds__(256) void attn_select_tile_kernel(const __grid_cons
     const double per_key = 1.0 / (double)a.block;
     constexpr int PER_ROW = 256 / KT;                       // threads of a row of key sums
     const int my_row = tid / PER_ROW, my_col = tid % PER_ROW;
-    for (int b0 = 0; b0 < n_most; b0 += KT) {
-        int64_t row = -1;
-        if (b0 + my_row < n_most) row = key_sum_row(a, sq, s, b0 + my_row);
+    constexpr int KN = D / 4 / PER_ROW;
+    float4 k[KN];
+    int64_t row = -1;
+    auto fetch = [&](int b0) {
+        row = b0 + my_row < n_most ? key_sum_row(a, sq, s, b0 + my_row) : -1;
         const float4 *src = reinterpret_cast<const float4 *>(key_sums + (max(row, (int64_t)0) * a.kv_heads + h) * D);
+#pragma unroll
+        for (int i = 0; i < KN; i++) k[i] = row >= 0 ? src[i * PER_ROW + my_col] : make_float4(0.f, 0.f, 0.f, 0.f);
+    };
+    fetch(0);
+    for (int b0 = 0; b0 < n_most; b0 += KT) {
+        // this step's key sums are in registers already; the next step's are requested before the products
         if (my_col == 0) there[my_row] = row >= 0;
 #pragma unroll
-        for (int i = 0; i < D / 4 / PER_ROW; i++) {
-            const int c = i * PER_ROW + my_col;
-            const float4 k = row >= 0 ? src[c] : make_float4(0.f, 0.f, 0.f, 0.f);
-            double *dst = ks + my_row * LD + c * 4;
-            *reinterpret_cast<double2 *>(dst) = make_double2((double)k.x, (double)k.y);
-            *reinterpret_cast<double2 *>(dst + 2) = make_double2((double)k.z, (double)k.w);
+        for (int i = 0; i < KN; i++) {
+            double *dst = ks + my_row * LD + (i * PER_ROW + my_col) * 4;
+            *reinterpret_cast<double2 *>(dst) = make_double2((double)k[i].x, (double)k[i].y);
+            *reinterpret_cast<double2 *>(dst + 2) = make_double2((double)k[i].z, (double)k[i].w);
         }
+        fetch(b0 + KT);
         __syncthreads();
         double acc[NT][2] = {};
         const double *qa = qs + (mg * 8 + (lane >> 2)) * LD + (lane & 3);
@@ -710,19 +732,22 @@ static int select_launch(const spamm_attn &a, const float *key_sums, int n_first
     const int nkb = attn_max_blocks(a), nqb = attn_query_blocks(a);
     const int64_t grid = (int64_t)a.batch * nqb * a.kv_heads, sums_grid = (int64_t)a.batch * nkb;
     if (grid > INT32_MAX || sums_grid > INT32_MAX) return attn_too_large();
-    if (!a.n_pages && a.tokens) {
-        attn_key_sums_kernel<T, D><<<(unsigned)sums_grid, 256, 0, stream>>>(a, nkb, scratch);
-        key_sums = scratch;
-    }
+    const int key_blocks = !a.n_pages && a.tokens ? (int)sums_grid : 0;
+    if (!a.n_pages) key_sums = scratch;
     const int G = a.heads / a.kv_heads;
     double *query_sums = reinterpret_cast<double *>(reinterpret_cast<uint8_t *>(scratch) + key_sums_bytes(a));
     if ((int64_t)min(a.query_block, a.max_q) * G > INT32_MAX / 2) return attn_too_large();
     const SelectWay way = select_way(a);
     const int rows = min(a.query_block, a.max_q) * G;
-    if (rows >= 64)
-        attn_query_sums_kernel<T, D, true><<<(unsigned)grid, 256, 0, stream>>>(a, nqb, fast_div(G), query_sums);
-    else if (way != SELECT_SPREAD || rows > SPREAD_ROWS)
-        attn_query_sums_kernel<T, D, false><<<(unsigned)((grid + 2048 / D - 1) / (2048 / D)), 256, 0, stream>>>(a, nqb, fast_div(G), query_sums);
+    // the queries' sums: a block of threads for a list of many rows, 2048 / D lists to a block of few, none where the scores'
+    // kernel takes them itself
+    const bool wide = rows >= 64;
+    const int64_t query_blocks = wide ? grid : way != SELECT_SPREAD || rows > SPREAD_ROWS ? (grid + 2048 / D - 1) / (2048 / D) : 0;
+    if (key_blocks + query_blocks > INT32_MAX) return attn_too_large();
+    if (key_blocks + query_blocks) {
+        const auto sums = wide ? attn_sums_kernel<T, D, true> : attn_sums_kernel<T, D, false>;
+        sums<<<(unsigned)(key_blocks + query_blocks), 256, 0, stream>>>(a, key_blocks, nkb, nqb, fast_div(G), scratch, query_sums);
+    }
     int st = SPAMM_OK;
     switch (way) {
     case SELECT_SPREAD: {
