@@ -1167,11 +1167,10 @@ static int backward_launch(const spamm_attn &a, const BackwardPlan &p, const T *
     attn_turn_kernel<<<(unsigned)((lists + 3) / 4), 128, 0, stream>>>(a, p.nqb, p.nkb, p.words, bits, counts);
     attn_items_kernel<<<(unsigned)p.groups, 1024, 0, stream>>>(a, p, counts, slots, items, n_items);
 
-    // from 48 rows of a sequence and key head on, tiles of 128 rows; below, and over more blocks than a union is built
-    // over, tiles of 16
+    // (over more blocks than a union is built over, tiles of 16 rows whatever their number)
     int st;
     const int tq = attn_tiles(a);
-    if ((int64_t)a.max_q * (a.heads / a.kv_heads) >= 48 && attn_tile_fits(a) && p.nkb <= TQ_BLOCKS<D> && p.groups * tq <= INT32_MAX) {
+    if (attn_big_tiles(a, (int64_t)min(a.n_select, p.nkb) * a.block) && attn_tile_fits(a) && p.nkb <= TQ_BLOCKS<D> && p.groups * tq <= INT32_MAX) {
         RowMap k_map, v_map;
         attn_row_maps(a, min(a.block, TQ_KEYS), &k_map, &v_map);
         const int entries = (int)min((int64_t)p.nkb, (int64_t)attn_tile_lists(a) * a.n_select);

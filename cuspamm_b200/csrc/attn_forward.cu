@@ -1020,9 +1020,7 @@ static int64_t longest_list(const spamm_attn &a)
     return a.n_select ? min(a.n_select, attn_max_blocks(a)) : attn_max_blocks(a);
 }
 
-// From 48 rows of a sequence and key head on, tiles of 128 rows are used; below (decoding), tiles of 16.
-constexpr int MIN_TC_ROWS = 48;
-static bool use_tc(const spamm_attn &a) { return (int64_t)a.max_q * (a.heads / a.kv_heads) >= MIN_TC_ROWS; }
+static bool use_tc(const spamm_attn &a) { return attn_big_tiles(a, longest_list(a) * a.block); }
 
 static RowsPlan rows_plan(const spamm_attn &a)
 {
@@ -1032,10 +1030,13 @@ static RowsPlan rows_plan(const spamm_attn &a)
     if (tc) {
         p.bq = 0;
         p.nqb = 1;
-        // pairs of tiles once they fill the 148 SMs twice over
-        p.tiles = ceil_div(attn_tiles(a), 2);
-        p.pairs = (int64_t)a.batch * a.kv_heads * p.tiles >= 2 * 148 || !a.n_select;
-        if (!p.pairs) p.tiles = attn_tiles(a);
+        // Pairs of tiles where they fill the GPU without cutting the keys and the keys are not listed: two chunks of 1024 tokens
+        // over 32768 keys take 898 us in pairs and 944 us in single tiles, but 8 chunks of 64 tokens over 8192 keys (two pairs
+        // for each of 64 heads) 227 us and 186 us, and a training batch with lists of 1024 keys 497 us and 469 us: a pair is
+        // alone on its SM, and nothing runs beside its beginning and its end.
+        p.tiles = attn_tiles(a);
+        p.pairs = !a.n_select && (int64_t)a.batch * a.kv_heads * ceil_div(p.tiles, 2) >= 148;
+        if (p.pairs) p.tiles = ceil_div(p.tiles, 2);
         p.shape = attn_tile_shape(a);
     } else {
         p.bq = a.n_select ? min(a.query_block, a.max_q) : a.max_q;

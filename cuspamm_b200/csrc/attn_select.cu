@@ -688,16 +688,19 @@ __global__ __launch_bounds__(128) void attn_select_kernel(const __grid_constant_
     write_largest<128>(keys, reach.n, a.n_select, lists + (((int64_t)s * nqb + qb) * a.kv_heads + h) * a.n_select);
 }
 
-// Which of the three: by how many lists there are to fill the GPU with, and whether the scores of a tile of query blocks
-// fit shared memory.
+// Which of the four (times with the sums, 8 key heads of 128 unless noted).  A tile of eight query blocks wants eight in a
+// sequence, and tiles enough to fill the GPU when the blocks of keys are many: else the scores are spread (16 sequences of one
+// token over up to 1025 blocks: 17 us and 14 us for the lists; as tiles of one list each seven eighths of the products would be
+// empty).  1024 lists over 32 blocks: tiles of 8 15 us, spread 24 us, one by one 19 us.  Tiles of 32 need 4096 lists: 2048
+// lists over 64 blocks 19 us against 17 us in tiles of 8, 8192 lists 30 us against 42 us (one by one 79 us, spread 103 us).
+// Beyond 1024 blocks the scores of eight query blocks do not fit shared memory.
 enum SelectWay { SELECT_SPREAD, SELECT_TILE32, SELECT_TILE8, SELECT_ONE };
 static SelectWay select_way(const spamm_attn &a)
 {
-    const int64_t lists = (int64_t)a.batch * attn_query_blocks(a) * a.kv_heads, blocks = attn_max_blocks(a);
-    if (lists < 1184) return SELECT_SPREAD;
-    if (blocks <= SELECT_TILE32_BLOCKS && lists >= 32 * 296) return SELECT_TILE32;
-    if (blocks <= 1024) return SELECT_TILE8;
-    return SELECT_ONE;
+    const int64_t groups = (int64_t)a.batch * a.kv_heads, nqb = attn_query_blocks(a), blocks = attn_max_blocks(a);
+    if (nqb < 8 || (blocks > 128 && groups * ((nqb + 7) / 8) < 148) || (blocks > 1024 && groups * nqb < 1184)) return SELECT_SPREAD;
+    if (blocks <= SELECT_TILE32_BLOCKS && groups * nqb >= 4096) return SELECT_TILE32;
+    return blocks <= 1024 ? SELECT_TILE8 : SELECT_ONE;
 }
 
 template <int D, int QT>

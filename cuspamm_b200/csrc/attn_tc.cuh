@@ -158,6 +158,16 @@ __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.a
 constexpr int UNION_LISTS = 32;
 constexpr int UNION_BLOCKS = 8192;           // blocks of keys that a union is built over at a time
 
+// Tiles of 128 rows or of 16, by the rows of a sequence and key head.  64 sequences, 8 key heads of 128, lists of up to 16 blocks
+// of 64: 16 rows of as many keys take 29 us in a tile of 128 against 15 us in one of 16 (dq 26 us, 13 us), 48 rows 31 us
+// against 39 us (dq 27 us, 33 us).  Over long ranges tiles of 16 read the keys once for each: 8 sequences of 8192 keys, 32 rows
+// 71 us against 119 us, 16 rows (one tile either way) about the same.
+inline bool attn_big_tiles(const spamm_attn &a, int64_t keys)
+{
+    const int64_t rows = (int64_t)a.max_q * (a.heads / a.kv_heads);
+    return rows >= 36 || (rows > 16 && keys >= 4096);
+}
+
 struct TileRows {
     int rows;                 // of the tile; 0: there is none
     int row0;                 // first of the sequence's rows (query * G + head)
