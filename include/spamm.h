@@ -485,6 +485,12 @@ int spamm_count_valid_static_max_blocks(void);
  * a page outside [0, n_pages) is treated as masked (append: not written) and SPAMM_ERR_INVALID is stored to *d_status;
  * a list entry that is no block of the sequence, or not above every entry before it, is skipped.  Queries of a
  * sequence from max_q on are not computed (their rows count as rows behind the last sequence).
+ *
+ * A NaN or an infinity in a key or value reaches the rows that read it and no others: what lies behind the last key of a
+ * sequence, in blocks that are not listed or behind a causal limit changes no result.  One in a query or in its output
+ * gradient stays with its own row of o and dq, and may reach dk and dv of all blocks that its query block lists.
+ *
+ * No call waits for the GPU.  The first call of each kind on a GPU loads its kernels: make it outside a capture.
  */
 #define SPAMM_ATTN_BF16 0
 #define SPAMM_ATTN_HALF 1
@@ -530,7 +536,7 @@ typedef struct spamm_attn {
 /*
  * New keys and values (k and v of `a`, packed, d_k/d_v with their strides) go to the pages: token i of n new ones of
  * sequence s to position p = lengths[s] - n + i.  d_k_pages, d_v_pages: [n_pages][kv_heads][block][dim].  With
- * d_inv_freq ([n_freq] float, 2 * n_freq <= dim) the first 2 * n_freq values of every key head are turned by the angles
+ * d_inv_freq ([n_freq] float, n_freq a multiple of 8, 2 * n_freq <= dim) the first 2 * n_freq values of every key head are turned by the angles
  * p * inv_freq[j], pairs (j, j + n_freq) or, with interleaved, (2j, 2j + 1); d_q, when given, is turned likewise into
  * d_o.  The angle is taken in double, its cosine and sine rounded to float, the products and their sum rounded to float
  * one by one, the result once to the type.  d_key_sums ([n_pages][kv_heads][dim] float, may be NULL) gets for every page
