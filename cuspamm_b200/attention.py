@@ -31,24 +31,28 @@ _DTYPES = {torch.bfloat16: 0, torch.float16: 1}
 _BLOCKS = (16, 32, 64, 128)
 
 
-def _rows(name: str, x: torch.Tensor, heads: Optional[int] = None, like: Optional[torch.Tensor] = None) -> torch.Tensor:
+def _rows(name: str, x: torch.Tensor, heads: Optional[int] = None, like: Optional[torch.Tensor] = None):
+    """Checks a tensor of rows; its token and head stride (those of a dimension of one element are never used: 0)."""
     if not isinstance(x, torch.Tensor):
         raise TypeError(f"{name} must be a torch tensor")
     if x.dim() != 3:
         raise ValueError(f"{name} must be [tokens, heads, head_dim], got {tuple(x.shape)}")
     if x.dtype not in _DTYPES:
         raise ValueError(f"{name} must be bfloat16 or float16, got {x.dtype}")
-    if x.shape[2] not in (64, 128):
-        raise ValueError(f"{name}: head_dim must be 64 or 128, got {x.shape[2]}")
-    if heads is not None and x.shape[1] != heads:
-        raise ValueError(f"{name} must have {heads} heads, got {x.shape[1]}")
-    if like is not None and (x.shape[0] != like.shape[0] or x.shape[2] != like.shape[2] or x.dtype != like.dtype
-                             or x.device != like.device):
-        raise ValueError(f"{name} must match in tokens, head_dim, dtype and device: {tuple(x.shape)} {x.dtype} {x.device} "
-                         f"against {tuple(like.shape)} {like.dtype} {like.device}")
-    if x.numel() and x.stride(2) != 1:
+    n_tokens, n_heads, dim = x.shape
+    if dim != 64 and dim != 128:
+        raise ValueError(f"{name}: head_dim must be 64 or 128, got {dim}")
+    if heads is not None and n_heads != heads:
+        raise ValueError(f"{name} must have {heads} heads, got {n_heads}")
+    if like is not None:
+        tokens, _, like_dim = like.shape
+        if n_tokens != tokens or dim != like_dim or x.dtype != like.dtype or x.device != like.device:
+            raise ValueError(f"{name} must match in tokens, head_dim, dtype and device: {tuple(x.shape)} {x.dtype} {x.device} "
+                             f"against {tuple(like.shape)} {like.dtype} {like.device}")
+    token, head, last = x.stride()
+    if last != 1 and x.numel():
         raise ValueError(f"{name}: the last dimension must be contiguous")
-    return x
+    return token if n_tokens > 1 else 0, head if n_heads > 1 else 0
 
 
 def _ints(name: str, x: torch.Tensor, shape, device) -> torch.Tensor:
@@ -58,7 +62,7 @@ def _ints(name: str, x: torch.Tensor, shape, device) -> torch.Tensor:
         raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(x.shape)}")
     if x.device != device:
         raise ValueError(f"{name} must be on {device}, is on {x.device}")
-    if x.numel() and not x.is_contiguous():
+    if not x.is_contiguous():
         raise ValueError(f"{name} must be contiguous")
     return x
 
@@ -74,54 +78,58 @@ def _host_int(name: str, x, least: int = 0) -> int:
     return v
 
 
-def _batch(cu_seqlens: torch.Tensor, device) -> int:
-    if not isinstance(cu_seqlens, torch.Tensor) or cu_seqlens.dim() != 1 or cu_seqlens.shape[0] < 1:
-        raise ValueError("cu_seqlens must be a tensor [batch + 1]")
-    _ints("cu_seqlens", cu_seqlens, cu_seqlens.shape, device)
-    return cu_seqlens.shape[0] - 1
-
-
 def _on_gpu(x: torch.Tensor) -> None:
-    if x.device.type != "cuda":
+    if not x.is_cuda:
         raise ValueError(f"tensors must be on a GPU, got {x.device}")
 
 
-def _strides(x: torch.Tensor):
-    """Token and head stride; those of a dimension of one element are never used and may be anything."""
-    (tokens, heads, _), (token, head, _) = x.shape, x.stride()
-    return (token if tokens > 1 else 0), (head if heads > 1 else 0)
+def _like(x: torch.Tensor) -> torch.Tensor:
+    """A new tensor of x's shape without gaps."""
+    return torch.empty_like(x, memory_format=torch.contiguous_format)
 
 
-def _problem(q: torch.Tensor, kv_heads: int, cu_seqlens: torch.Tensor, max_q: int, block: int, query_block: int,
-             n_select: int, causal: bool) -> SpammAttn:
+def _problem(q: torch.Tensor, q_strides, kv_heads: int, cu_seqlens: torch.Tensor, max_q: int, block: int, query_block: int,
+             causal: bool) -> SpammAttn:
+    tokens, heads, dim = q.shape
     if block not in _BLOCKS:
         raise ValueError(f"block must be one of {_BLOCKS}, got {block}")
-    if kv_heads < 1 or q.shape[1] % kv_heads or not 1 <= q.shape[1] // kv_heads <= 128:
-        raise ValueError(f"{q.shape[1]} query heads for {kv_heads} key heads: must be a multiple, 1 to 128 times")
-    a = SpammAttn()
+    if kv_heads < 1 or heads % kv_heads or not 1 <= heads // kv_heads <= 128:
+        raise ValueError(f"{heads} query heads for {kv_heads} key heads: must be a multiple, 1 to 128 times")
+    if not isinstance(cu_seqlens, torch.Tensor) or cu_seqlens.dim() != 1 or cu_seqlens.shape[0] < 1:
+        raise ValueError("cu_seqlens must be a tensor [batch + 1]")
+    _ints("cu_seqlens", cu_seqlens, cu_seqlens.shape, q.device)
+    a = SpammAttn()                          # all zeros
     a.dtype = _DTYPES[q.dtype]
-    a.batch = _batch(cu_seqlens, q.device)
-    a.heads, a.kv_heads, a.dim = q.shape[1], kv_heads, q.shape[2]
-    a.block, a.query_block, a.n_select = block, query_block, n_select
-    a.causal, a.max_q, a.tokens, a.zero_tail = bool(causal), max_q, q.shape[0], 1
+    a.batch = cu_seqlens.shape[0] - 1
+    a.heads = heads
+    a.kv_heads = kv_heads
+    a.dim = dim
+    a.block = block
+    a.query_block = query_block
+    a.causal = 1 if causal else 0
+    a.max_q = max_q
+    a.tokens = tokens
+    a.zero_tail = 1
     a.scale = 1.0
     a.d_cu = cu_seqlens.data_ptr()
     a.d_q = q.data_ptr()
-    a.q_token, a.q_head = _strides(q)
+    a.q_token, a.q_head = q_strides
     return a
 
 
-def _set_keys(a: SpammAttn, k: torch.Tensor, v: Optional[torch.Tensor]) -> None:
+def _set_keys(a: SpammAttn, k: torch.Tensor, k_strides, v: Optional[torch.Tensor] = None, v_strides=None) -> None:
     a.d_k = k.data_ptr()
-    a.k_token, a.k_head = _strides(k)
+    a.k_token, a.k_head = k_strides
     if v is not None:
         a.d_v = v.data_ptr()
-        a.v_token, a.v_head = _strides(v)
+        a.v_token, a.v_head = v_strides
 
 
 def _set_out(a: SpammAttn, o: torch.Tensor) -> None:
+    """o without gaps."""
     a.d_o = o.data_ptr()
-    a.o_token, a.o_head = _strides(o)
+    a.o_token = a.heads * a.dim
+    a.o_head = a.dim
 
 
 def _set_lists(a: SpammAttn, lists: torch.Tensor, device) -> None:
@@ -172,6 +180,7 @@ def _select(a: SpammAttn, q: torch.Tensor, key_sums: Optional[torch.Tensor], n_s
     forced = n_first + (n_local + (a.query_block + a.block - 2) // a.block if n_local else 0)
     if not 1 <= n_select <= 1024 or n_select < forced:
         raise ValueError(f"n_select must be 1 to 1024 and hold the {forced} first and local blocks, got {n_select}")
+    a.n_select = n_select
     _on_gpu(q)
     with _device(q.device):
         lists = torch.empty((a.batch, -(-a.max_q // a.query_block), a.kv_heads, n_select), dtype=torch.int32, device=q.device)
@@ -198,64 +207,71 @@ def select_blocks(q: torch.Tensor, k: torch.Tensor, cu_seqlens: torch.Tensor, ma
     of the key head) times the block's mean key; it is taken in double, ties go to the lower block.  The first `n_first`
     blocks and those from `n_local` - 1 before the first query's to the last query's own are always taken.  No sequence
     may be longer than `max_seqlen`.  The choice is not differentiable."""
-    _rows("q", q)
-    _rows("k", k)
-    _rows("k", k, like=q)
-    a = _problem(q, k.shape[1], cu_seqlens, _host_int("max_seqlen", max_seqlen), _host_int("block", block),
-                 _host_int("query_block", query_block, 1), _host_int("n_select", n_select, 1), causal)
-    _set_keys(a, k, None)
-    return _select(a, q, None, a.n_select, _host_int("n_first", n_first), _host_int("n_local", n_local))
+    q_strides = _rows("q", q)
+    k_strides = _rows("k", k, like=q)
+    a = _problem(q, q_strides, k.shape[1], cu_seqlens, _host_int("max_seqlen", max_seqlen), _host_int("block", block),
+                 _host_int("query_block", query_block, 1), causal)
+    _set_keys(a, k, k_strides)
+    return _select(a, q, None, _host_int("n_select", n_select, 1), _host_int("n_first", n_first), _host_int("n_local", n_local))
+
+
+def _own_strides(x: torch.Tensor):
+    (tokens, heads, _), (token, head, _) = x.shape, x.stride()
+    return token if tokens > 1 else 0, head if heads > 1 else 0
 
 
 class _BlockSparseAttention(torch.autograd.Function):
+    """`a` describes q, k, v, the lists and cu_seqlens, checked."""
+
     @staticmethod
-    def forward(ctx, q, k, v, lists, cu_seqlens, max_seqlen, block, query_block, causal, scale):
-        a = _problem(q, k.shape[1], cu_seqlens, max_seqlen, block, query_block, 0, causal)
-        a.scale = scale
-        _set_keys(a, k, v)
-        _set_lists(a, lists, q.device)
-        _on_gpu(q)
-        with _device(q.device):
-            o = q.new_empty(q.shape)
-            lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device)
+    def forward(ctx, q, k, v, lists, cu_seqlens, a, want_lse):
+        device = q.device
+        with _device(device):
+            o = _like(q)
+            lse = torch.empty((a.tokens, a.heads), dtype=torch.float32, device=device)
             _set_out(a, o)
             a.d_lse = lse.data_ptr()
             # what the rounding of o left, for the backward's do.o: only where there will be one
-            low = torch.empty_like(o) if any(ctx.needs_input_grad[:3]) else None
+            low = _like(q) if any(ctx.needs_input_grad[:3]) else None
             a.d_o_low = low.data_ptr() if low is not None else None
             if not a.batch or not a.max_q:
                 o.zero_()
                 lse.fill_(float("-inf"))
-            _forward(a, q.device)
-        ctx.save_for_backward(q, k, v, lists, cu_seqlens, o, low, lse)
-        ctx.how = (max_seqlen, block, query_block, causal, scale)
+            _forward(a, device)
+        if low is not None:
+            ctx.save_for_backward(q, k, v, lists, cu_seqlens, o, low, lse)
+            ctx.problem = a
+        if not want_lse:
+            return o
         ctx.mark_non_differentiable(lse)
         return o, lse
 
     @staticmethod
     @torch.autograd.function.once_differentiable
-    def backward(ctx, d_o, _):
+    def backward(ctx, d_o, *_):
         q, k, v, lists, cu_seqlens, o, low, lse = ctx.saved_tensors
-        max_seqlen, block, query_block, causal, scale = ctx.how
-        a = _problem(q, k.shape[1], cu_seqlens, max_seqlen, block, query_block, 0, causal)
-        a.scale = scale
-        _set_keys(a, k, v)
-        _set_lists(a, lists, q.device)
-        _set_out(a, o)
+        # the sizes are the forward's; the tensors may lie elsewhere by now (hooks on saved tensors)
+        a = SpammAttn.from_buffer_copy(ctx.problem)
+        a.d_q, a.d_o = q.data_ptr(), o.data_ptr()
+        a.q_token, a.q_head = _own_strides(q)
+        a.o_token, a.o_head = _own_strides(o)
+        _set_keys(a, k, _own_strides(k), v, _own_strides(v))
+        a.d_lists, a.d_cu = lists.data_ptr(), cu_seqlens.data_ptr()
         a.d_lse, a.d_o_low = lse.data_ptr(), low.data_ptr()
         # an expanded or oddly laid out gradient (the sum's, for one) is brought into rows first
-        if d_o.numel() and (d_o.stride(2) != 1 or d_o.data_ptr() % 16 or any(st % 8 for st in _strides(d_o))):
+        do_token, do_head = _own_strides(d_o)
+        if (d_o.stride(2) != 1 or d_o.data_ptr() % 16 or do_token % 8 or do_head % 8) and d_o.numel():
             d_o = d_o.contiguous()
+            do_token, do_head = _own_strides(d_o)
         lib = _lib.load()
-        with _device(q.device):
-            dq = q.new_empty(q.shape)
-            dk = k.new_empty(k.shape)
-            dv = v.new_empty(v.shape)
+        device = q.device
+        with _device(device):
+            dq, dk, dv = _like(q), _like(k), _like(k)
             n = lib.spamm_attn_backward_scratch_bytes(C.byref(a))
-            scratch, ptr = _scratch(n, q.device)
-            check(lib.spamm_attn_backward_dev(C.byref(a), d_o.data_ptr(), *_strides(d_o), dq.data_ptr(), dk.data_ptr(),
-                                              dv.data_ptr(), ptr, n, _stream(q.device)), "spamm_attn_backward_dev")
-        return dq, dk, dv, None, None, None, None, None, None, None
+            scratch, ptr = _scratch(n, device)
+            check(lib.spamm_attn_backward_dev(C.byref(a), d_o.data_ptr(), do_token, do_head, dq.data_ptr(), dk.data_ptr(),
+                                              dv.data_ptr(), ptr, n, _stream(device)), "spamm_attn_backward_dev")
+        return dq, dk, dv, None, None, None, None
 
 
 def block_sparse_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lists: torch.Tensor, cu_seqlens: torch.Tensor,
@@ -266,14 +282,16 @@ def block_sparse_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, li
     those up to its own position.  `scale` multiplies q.k (default head_dim ** -0.5).  A query that sees no key gets
     zeros.  Returns o [tokens, heads, head_dim], with `return_lse` also the log of the sum of exp(scale * q.k) per query
     and head (float, not differentiable).  Differentiable once in q, k and v; two backward passes give the same bits."""
-    _rows("q", q)
-    _rows("k", k)
-    _rows("k", k, like=q)
-    _rows("v", v, heads=k.shape[1], like=q)
-    o, lse = _BlockSparseAttention.apply(q, k, v, lists, cu_seqlens, _host_int("max_seqlen", max_seqlen),
-                                         _host_int("block", block), _host_int("query_block", query_block, 1), bool(causal),
-                                         _scale(scale, q.shape[2]))
-    return (o, lse) if return_lse else o
+    q_strides = _rows("q", q)
+    k_strides = _rows("k", k, like=q)
+    v_strides = _rows("v", v, heads=k.shape[1], like=q)
+    a = _problem(q, q_strides, k.shape[1], cu_seqlens, _host_int("max_seqlen", max_seqlen), _host_int("block", block),
+                 _host_int("query_block", query_block, 1), causal)
+    a.scale = _scale(scale, a.dim)
+    _set_keys(a, k, k_strides, v, v_strides)
+    _set_lists(a, lists, q.device)
+    _on_gpu(q)
+    return _BlockSparseAttention.apply(q, k, v, lists, cu_seqlens, a, return_lse)
 
 
 class PagedCache:
@@ -324,22 +342,29 @@ class PagedCache:
             self.status.zero_()
             raise SpammError(st, "PagedCache")
 
-    def _problem(self, q, cu_seqlens, max_new, page_table, lengths, query_block, n_select, causal) -> SpammAttn:
-        if q.dtype != self.k.dtype or q.shape[2] != self.k.shape[3] or q.device != self.k.device:
+    def _problem(self, q, q_strides, cu_seqlens, max_new, page_table, lengths, query_block) -> SpammAttn:
+        n_pages, kv_heads, page_size, dim = self.k.shape
+        device = self.k.device
+        if q.dtype != self.k.dtype or q.shape[2] != dim or q.device != device:
             raise ValueError("tokens must match the cache in dtype, head_dim and device")
-        a = _problem(q, self.k.shape[1], cu_seqlens, _host_int("max_new", max_new), self.page_size,
-                     _host_int("query_block", query_block, 1), n_select, causal)
-        _ints("lengths", lengths, (a.batch,), q.device)
+        a = _problem(q, q_strides, kv_heads, cu_seqlens, _host_int("max_new", max_new), page_size,
+                     _host_int("query_block", query_block, 1), True)
+        batch = a.batch
+        _ints("lengths", lengths, (batch,), device)
         if not isinstance(page_table, torch.Tensor) or page_table.dim() != 2 or page_table.dtype != torch.int32 \
-                or page_table.shape[0] != a.batch or page_table.device != q.device:
+                or page_table.shape[0] != batch or page_table.device != device:
             raise ValueError("page_table must be an int32 tensor [batch, pages of the longest sequence] beside the tokens")
-        if page_table.shape[1] > 1 and page_table.stride(1) != 1:
+        width, (row, column) = page_table.shape[1], page_table.stride()
+        if width > 1 and column != 1:
             raise ValueError("page_table: the last dimension must be contiguous")
-        if page_table.shape[0] > 1 and page_table.shape[1] and page_table.stride(0) < page_table.shape[1]:
+        if batch > 1 and width and row < width:
             raise ValueError("page_table: rows must not overlap")
-        a.n_pages, a.table_width = self.k.shape[0], page_table.shape[1]
-        a.table_stride = max(page_table.stride(0), page_table.shape[1]) if page_table.shape[0] > 1 else page_table.shape[1]
-        a.d_table, a.d_lengths, a.d_status = page_table.data_ptr(), lengths.data_ptr(), self.status.data_ptr()
+        a.n_pages = n_pages
+        a.table_width = width
+        a.table_stride = max(row, width) if batch > 1 else width
+        a.d_table = page_table.data_ptr()
+        a.d_lengths = lengths.data_ptr()
+        a.d_status = self.status.data_ptr()
         return a
 
     def append(self, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor, max_new: int, page_table: torch.Tensor,
@@ -350,23 +375,23 @@ class PagedCache:
         position * inv_freq on the way, pairs (j, j + n) of each head or, `interleaved`, (2j, 2j + 1); `q` is rotated
         likewise and returned as a new tensor.  The key sums of the touched pages are taken anew from all keys that they
         hold, so that tokens may be appended again after `lengths` went back."""
-        _rows("k", k, heads=self.k.shape[1])
-        _rows("v", v, heads=self.k.shape[1], like=k)
-        if q is not None:
-            _rows("q", q, like=k)
+        kv_heads = self.k.shape[1]
+        k_strides = _rows("k", k, heads=kv_heads)
+        v_strides = _rows("v", v, heads=kv_heads, like=k)
+        q_strides = _rows("q", q, like=k) if q is not None else k_strides
         if inv_freq is not None:
             if not isinstance(inv_freq, torch.Tensor) or inv_freq.dtype != torch.float32 or inv_freq.dim() != 1 \
                     or not inv_freq.is_contiguous() or inv_freq.device != k.device:
                 raise ValueError("inv_freq must be a contiguous float32 tensor beside the tokens")
             if inv_freq.shape[0] % 8 or 2 * inv_freq.shape[0] > k.shape[2] or not inv_freq.shape[0]:
                 raise ValueError(f"inv_freq must have a multiple of 8 values, at most head_dim / 2, got {inv_freq.shape[0]}")
-        a = self._problem(k if q is None else q, cu_seqlens, max_new, page_table, lengths, 1, 0, True)
-        _set_keys(a, k, v)
+        a = self._problem(k if q is None else q, q_strides, cu_seqlens, max_new, page_table, lengths, 1)
+        _set_keys(a, k, k_strides, v, v_strides)
         lib = _lib.load()
         with _device(k.device):
             out = None
             if q is not None:
-                out = q.new_empty(q.shape)
+                out = _like(q)
                 _set_out(a, out)
                 if not a.batch or not a.max_q:
                     out.zero_()
@@ -379,10 +404,10 @@ class PagedCache:
     def select(self, q: torch.Tensor, cu_seqlens: torch.Tensor, max_new: int, page_table: torch.Tensor, lengths: torch.Tensor,
                n_select: int, query_block: int = 1, n_first: int = 1, n_local: int = 1) -> torch.Tensor:
         """`select_blocks` for the newest tokens over the cached pages, by the cache's key sums."""
-        _rows("q", q)
-        a = self._problem(q, cu_seqlens, max_new, page_table, lengths, query_block, _host_int("n_select", n_select, 1), True)
+        a = self._problem(q, _rows("q", q), cu_seqlens, max_new, page_table, lengths, query_block)
         a.d_k = self.k.data_ptr()
-        return _select(a, q, self.key_sums, a.n_select, _host_int("n_first", n_first), _host_int("n_local", n_local))
+        return _select(a, q, self.key_sums, _host_int("n_select", n_select, 1), _host_int("n_first", n_first),
+                       _host_int("n_local", n_local))
 
     def attend(self, q: torch.Tensor, cu_seqlens: torch.Tensor, max_new: int, page_table: torch.Tensor, lengths: torch.Tensor,
                lists: Optional[torch.Tensor] = None, query_block: int = 1, scale: Optional[float] = None,
@@ -390,26 +415,27 @@ class PagedCache:
         """Attention of the newest tokens (one of each sequence or a whole chunk) over the cached keys up to their own,
         of all pages or, with `lists` (as `select` gives them, for the same `query_block`), of the listed ones.  With
         `out` the result goes there, and its rows that belong to no sequence are left as they are; else they are zero."""
-        _rows("q", q)
-        a = self._problem(q, cu_seqlens, max_new, page_table, lengths, query_block, 0, True)
-        a.scale = _scale(scale, q.shape[2])
+        a = self._problem(q, _rows("q", q), cu_seqlens, max_new, page_table, lengths, query_block)
+        a.scale = _scale(scale, a.dim)
         a.d_k, a.d_v = self.k.data_ptr(), self.v.data_ptr()
+        device = q.device
         if lists is not None:
-            _set_lists(a, lists, q.device)
-        with _device(q.device):
+            _set_lists(a, lists, device)
+        with _device(device):
             if out is None:
-                out = q.new_empty(q.shape)
+                out = _like(q)
                 if not a.batch or not a.max_q:
                     out.zero_()
+                _set_out(a, out)
             else:
-                _rows("out", out, heads=q.shape[1], like=q)
+                a.o_token, a.o_head = _rows("out", out, heads=a.heads, like=q)
                 if any(n > 1 and st == 0 for n, st in zip(out.shape, out.stride())):
                     raise ValueError("out: rows must not overlap")
+                a.d_o = out.data_ptr()
                 a.zero_tail = 0
-            _set_out(a, out)
             lse = None
             if return_lse:
-                lse = torch.full(q.shape[:2], float("-inf"), dtype=torch.float32, device=q.device)
+                lse = torch.full((a.tokens, a.heads), float("-inf"), dtype=torch.float32, device=device)
                 a.d_lse = lse.data_ptr()
-            _forward(a, q.device)
+            _forward(a, device)
         return (out, lse) if return_lse else out

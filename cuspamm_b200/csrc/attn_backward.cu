@@ -48,7 +48,7 @@ static BackwardPlan backward_plan(const spamm_attn &a)
     size_t at = 0;
     auto take = [&](size_t n) { const size_t o = at; at += (n + 255) / 256 * 256; return o; };
     p.delta = take((size_t)a.tokens * a.heads * 4);
-    p.bits = take((size_t)p.groups * p.nkb * p.words * 4);          // bits and counts are cleared together
+    p.bits = take((size_t)p.groups * p.nkb * p.words * 4);          // bits and counts lie together: attn_delta_kernel clears them
     p.counts = take((size_t)p.groups * p.nkb * 4);
     p.slots = take((size_t)p.groups * p.nkb * 4);
     p.items = take((size_t)p.groups * p.item_cap * sizeof(Item));
@@ -58,12 +58,14 @@ static BackwardPlan backward_plan(const spamm_attn &a)
     return p;
 }
 
-// delta = do.o for every row; a quarter of a warp for each.  Rows of no sequence get zero gradients here.  Bound by the reading
-// of do, o and the low part of o: 18000 tokens of 32 heads of 128 (440 MB) take 69 us, 6.4 TB/s.
+// delta = do.o for every row; a quarter of a warp for each.  Rows of no sequence get zero gradients here, and the bits
+// and counts of the lists that are turned over next are cleared (`clear`, one launch less).  Bound by the reading of do, o and the low part of o: 18000 tokens of 32 heads of 128 (440 MB) take 69 us, 6.4 TB/s.
 template <typename T, int D>
 __global__ __launch_bounds__(256) void attn_delta_kernel(const __grid_constant__ spamm_attn a, const T *d_do, int64_t do_token,
-                                                         int64_t do_head, float *delta, T *dq, T *dk, T *dv)
+                                                         int64_t do_head, float *delta, T *dq, T *dk, T *dv, uint4 *clear,
+                                                         size_t n_clear)
 {
+    for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < n_clear; i += (size_t)gridDim.x * 256) clear[i] = make_uint4(0, 0, 0, 0);
     const int sub = threadIdx.x & 7;
     const int64_t w = (int64_t)blockIdx.x * 32 + (threadIdx.x >> 3);
     if (w >= (int64_t)a.tokens * a.heads) return;
@@ -1174,8 +1176,8 @@ static int backward_launch(const spamm_attn &a, const BackwardPlan &p, const T *
         p.groups * p.nkb > INT32_MAX || (int64_t)bq * (a.heads / a.kv_heads) > (1 << 28))
         return attn_too_large();
 
-    SPAMM_CUDA_TRY(cudaMemsetAsync(bits, 0, p.slots - p.bits, stream));
-    attn_delta_kernel<T, D><<<(unsigned)((rows + 31) / 32), 256, 0, stream>>>(a, d_do, do_token, do_head, delta, dq, dk, dv);
+    attn_delta_kernel<T, D><<<(unsigned)((rows + 31) / 32), 256, 0, stream>>>(a, d_do, do_token, do_head, delta, dq, dk, dv,
+                                                                             reinterpret_cast<uint4 *>(bits), (p.slots - p.bits) / 16);
     attn_turn_kernel<<<(unsigned)((lists + 3) / 4), 128, 0, stream>>>(a, p.nqb, p.nkb, p.words, bits, counts);
     attn_items_kernel<<<(unsigned)p.groups, 1024, 0, stream>>>(a, p, counts, slots, items, n_items);
 
