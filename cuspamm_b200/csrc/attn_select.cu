@@ -358,6 +358,80 @@ static __device__ __noinline__ void pick_by_whole_keys(const unsigned long long 
     write_list(mine, n, threshold, left, n_select, out, lane);
 }
 
+// The same by the upper halves of the keys alone, which nearly always suffice: held in registers, R for each of the LANES lanes
+// of a list, 32 / LANES lists to a warp, whose searches are then under way together.  n_most: the warp's largest n, at most
+// LANES * R.  False, and nothing written, where upper halves are alike at the border.
+template <int LANES, int R>
+static __device__ __forceinline__ bool pick_by_upper_halves(const unsigned long long *mine, int n, int n_most, int n_select, bool wanted,
+                                                            int32_t *out, int lane)
+{
+    const int l = lane % LANES, group = lane - l;
+    constexpr unsigned MASK = LANES == 32 ? ~0u : (1u << (LANES % 32)) - 1;
+    uint32_t k[R], low = ~0u, high = 0;
+#pragma unroll
+    for (int x = 0; x < R; x++) {
+        const int b = x * LANES + l;
+        k[x] = b < n ? reinterpret_cast<const uint32_t *>(mine)[2 * b + 1] : 0;      // no branch: all are requested at once
+    }
+    // (groups of eight: a branch for each would cost more than what it skips)
+#pragma unroll
+    for (int x0 = 0; x0 < R; x0 += 8) {
+        if (x0 * LANES >= n_most) break;
+#pragma unroll
+        for (int x = x0; x < x0 + 8; x++) {
+            low = min(low, x * LANES + l < n ? k[x] : ~0u);
+            high = max(high, k[x] != ~0u ? k[x] : 0);
+        }
+    }
+#pragma unroll
+    for (int d = 1; d < LANES; d <<= 1) {
+        low = min(low, __shfl_xor_sync(~0u, low, d));
+        high = max(high, __shfl_xor_sync(~0u, high, d));
+    }
+    high++;
+    const bool all = n <= n_select;                          // every candidate is taken
+    bool exact = all;
+    for (int round = 0; __any_sync(~0u, !exact && low < high && high - low > 1); round++) {
+        uint32_t want = (uint32_t)(key_between((unsigned long long)low << 32, (unsigned long long)high << 32, round) >> 32);
+        if (want == low) want++;
+        int c = 0, c1 = 0;
+#pragma unroll
+        for (int x0 = 0; x0 < R; x0 += 8) {
+            if (x0 * LANES >= n_most) break;
+#pragma unroll
+            for (int x = x0; x < x0 + 8; x += 2) {
+                c += k[x] >= want;
+                c1 += k[x + 1] >= want;
+            }
+        }
+        c += c1;
+        if (LANES == 32) {
+            c = __reduce_add_sync(~0u, c);
+        } else {
+#pragma unroll
+            for (int d = 1; d < LANES; d <<= 1) c += __shfl_xor_sync(~0u, c, d);
+        }
+        if (!exact && low < high && high - low > 1) {
+            exact = c == n_select;
+            if (c >= n_select) low = want;
+            else high = want;
+        }
+    }
+    int count = 0;
+#pragma unroll
+    for (int x = 0; x < R; x++) {
+        if (x * LANES >= n_most) break;
+        const int b = x * LANES + l;
+        const bool keep = exact && b < n && (all ? mine[b] != 0 : k[x] >= low);
+        const unsigned m = __ballot_sync(~0u, keep) >> group & MASK;
+        if (keep && wanted) out[count + __popc(m & ((1u << l) - 1))] = b;
+        count += __popc(m);
+    }
+    if (exact && wanted)
+        for (int x = count + l; x < n_select; x += LANES) out[x] = -1;
+    return exact;
+}
+
 constexpr int SELECT_TILE32_BLOCKS = 256;      // blocks of a sequence up to which tiles of 32 query blocks are used
 
 // ---- many query blocks: QT of them and one key head per block of threads, scores as double products on the tensor cores
@@ -458,60 +532,12 @@ __global__ __launch_bounds__(256) void attn_select_tile_kernel(const __grid_cons
         __syncthreads();
     }
     if constexpr (QT == 32) {
-        // eight lanes for a list, four lists to a warp, which keeps four searches in flight; the upper halves of the keys,
-        // held in registers, nearly always suffice
-        const int g = lane >> 3, l = lane & 7, i = warp * 4 + g, qb = qt * QT + i, n = reach[i].n;
-        const unsigned long long *mine = keys + i * nkb;
-        constexpr int R = SELECT_TILE32_BLOCKS / 8;
-        uint32_t k[R], low = ~0u, high = 0;
-#pragma unroll
-        for (int x = 0; x < R; x++) {
-            const int b = x * 8 + l;
-            k[x] = 0;
-            if (x * 8 < n_most && b < n) {
-                k[x] = (uint32_t)(mine[b] >> 32);
-                low = min(low, k[x]);
-                if (k[x] != ~0u) high = max(high, k[x]);
-            }
-        }
-#pragma unroll
-        for (int d = 1; d < 8; d <<= 1) {
-            low = min(low, __shfl_xor_sync(~0u, low, d));
-            high = max(high, __shfl_xor_sync(~0u, high, d));
-        }
-        high++;
-        const bool all = n <= a.n_select;                    // every candidate is taken
-        bool exact = all;
-        for (int round = 0; __any_sync(~0u, !exact && low < high && high - low > 1); round++) {
-            uint32_t want = (uint32_t)(key_between((unsigned long long)low << 32, (unsigned long long)high << 32, round) >> 32);
-            if (want == low) want++;
-            int c = 0;
-#pragma unroll
-            for (int x = 0; x < R; x++)
-                if (x * 8 < n_most) c += k[x] >= want;
-#pragma unroll
-            for (int d = 1; d < 8; d <<= 1) c += __shfl_xor_sync(~0u, c, d);
-            if (!exact && low < high && high - low > 1) {
-                exact = c == a.n_select;
-                if (c >= a.n_select) low = want;
-                else high = want;
-            }
-        }
-        int32_t *out = lists + (((int64_t)s * nqb + qb) * a.kv_heads + h) * a.n_select;
-        int count = 0;
-#pragma unroll
-        for (int x = 0; x < R; x++) {
-            if (x * 8 >= n_most) break;
-            const int b = x * 8 + l;
-            const bool keep = exact && b < n && (all ? mine[b] != 0 : k[x] >= low);
-            const unsigned m = __ballot_sync(~0u, keep) >> (8 * g) & 255u;
-            if (keep && qb < nqb) out[count + __popc(m & ((1u << l) - 1))] = b;
-            count += __popc(m);
-        }
-        if (exact && qb < nqb)
-            for (int x = count + l; x < a.n_select; x += 8) out[x] = -1;
+        // four lists to a warp
+        const int i = warp * 4 + lane / 8, qb = qt * QT + i;
+        const bool exact = pick_by_upper_halves<8, SELECT_TILE32_BLOCKS / 8>(keys + i * nkb, reach[i].n, n_most, a.n_select, qb < nqb,
+                                                                             lists + (((int64_t)s * nqb + qb) * a.kv_heads + h) * a.n_select, lane);
         // the rest, where upper halves are alike at the border
-        unsigned rest = __ballot_sync(~0u, !exact && l == 0 && qb < nqb);
+        unsigned rest = __ballot_sync(~0u, !exact && lane % 8 == 0 && qb < nqb);
         while (rest) {
             const int slow = warp * 4 + (__ffs(rest) - 1) / 8;
             rest &= rest - 1;
@@ -639,18 +665,33 @@ __global__ __launch_bounds__(SPREAD_WARPS * 32, 4) void attn_spread_scores_kerne
     }
 }
 
-// The lists of spread scores.  The rounds of the search are what it takes: 128 lists over up to 1025 blocks 14 us.
+// The lists of spread scores: by one warp each up to LARGEST_WARP blocks, by a block of threads beyond.
+constexpr int LARGEST_WARP = 2048;
+
+static __device__ __forceinline__ int candidates(const spamm_attn &a, int nqb, int list)
+{
+    const int s = list / a.kv_heads / nqb, qb = list / a.kv_heads % nqb;
+    const Seq sq = attn_seq(a, s);
+    const int64_t q0 = (int64_t)qb * a.query_block;
+    return reach_of(a, sq, q0, (int)min((int64_t)a.query_block, sq.nq - q0), 0).n;
+}
+template <int R>
+__global__ __launch_bounds__(32) void attn_largest_warp_kernel(const __grid_constant__ spamm_attn a, int nqb, int nkb,
+                                                               const unsigned long long *keys, int32_t *lists)
+{
+    const int n = candidates(a, nqb, blockIdx.x);
+    const unsigned long long *mine = keys + (int64_t)blockIdx.x * nkb;
+    int32_t *out = lists + (int64_t)blockIdx.x * a.n_select;
+    if (!pick_by_upper_halves<32, R>(mine, n, n, a.n_select, true, out, threadIdx.x)) pick_by_whole_keys(mine, n, a.n_select, out, threadIdx.x);
+}
 template <int THREADS>
 __global__ __launch_bounds__(THREADS) void attn_largest_kernel(const __grid_constant__ spamm_attn a, int nqb, int nkb,
                                                                const unsigned long long *keys, int32_t *lists)
 {
     extern __shared__ __align__(16) unsigned long long copy[];
-    const int s = blockIdx.x / a.kv_heads / nqb, qb = blockIdx.x / a.kv_heads % nqb;
-    const Seq sq = attn_seq(a, s);
-    const int64_t q0 = (int64_t)qb * a.query_block;
-    const Reach reach = reach_of(a, sq, q0, (int)min((int64_t)a.query_block, sq.nq - q0), 0);
-    for (int i = threadIdx.x; i < reach.n; i += THREADS) copy[i] = keys[(int64_t)blockIdx.x * nkb + i];
-    write_largest<THREADS>(copy, reach.n, a.n_select, lists + (int64_t)blockIdx.x * a.n_select);
+    const int n = candidates(a, nqb, blockIdx.x);
+    for (int i = threadIdx.x; i < n; i += THREADS) copy[i] = keys[(int64_t)blockIdx.x * nkb + i];
+    write_largest<THREADS>(copy, n, a.n_select, lists + (int64_t)blockIdx.x * a.n_select);
 }
 
 // ---- many query blocks of sequences too long for that: one list per block of threads
@@ -768,9 +809,15 @@ static int select_launch(const spamm_attn &a, const float *key_sums, int n_first
         if (blocks > INT32_MAX) return attn_too_large();
         attn_spread_scores_kernel<T, D><<<(unsigned)blocks, SPREAD_WARPS * 32, 0, stream>>>(a, nqb, spans, nkb, n_first, n_local, key_sums,
                                                                               rows > SPREAD_ROWS ? query_sums : nullptr, keys);
-        st = attn_set_smem((const void *)attn_largest_kernel<256>, (size_t)nkb * 8);
-        if (st) return st;
-        attn_largest_kernel<256><<<(unsigned)grid, 256, (size_t)nkb * 8, stream>>>(a, nqb, nkb, keys, lists);
+        if (nkb <= LARGEST_WARP / 4) {
+            attn_largest_warp_kernel<LARGEST_WARP / 128><<<(unsigned)grid, 32, 0, stream>>>(a, nqb, nkb, keys, lists);
+        } else if (nkb <= LARGEST_WARP) {
+            attn_largest_warp_kernel<LARGEST_WARP / 32><<<(unsigned)grid, 32, 0, stream>>>(a, nqb, nkb, keys, lists);
+        } else {
+            st = attn_set_smem((const void *)attn_largest_kernel<256>, (size_t)nkb * 8);
+            if (st) return st;
+            attn_largest_kernel<256><<<(unsigned)grid, 256, (size_t)nkb * 8, stream>>>(a, nqb, nkb, keys, lists);
+        }
         break;
     }
     case SELECT_TILE32: st = select_tile_launch<D, 32>(a, nqb, nkb, n_first, n_local, key_sums, query_sums, lists, stream); break;

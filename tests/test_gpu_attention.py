@@ -708,3 +708,31 @@ def test_offsets_beyond_four_gigabytes():
                 near(listed[at:at + m, h], val["o"], tol["o"], "listed")
             at, src = at + m, src + n
     cache.check()
+
+
+@pytest.mark.parametrize("blocks", [300, 1025, 2048, 2049, 5000])
+@pytest.mark.parametrize("ties", [False, True])
+def test_select_of_new_tokens_over_many_pages(blocks, ties):
+    """A few query blocks over every range of lengths that has a way of its own, with scores that mostly tie as well."""
+    from cuspamm_b200 import PagedCache
+
+    page, HK, G, D, new, n_select = 16, 2, 2, 64, [1, 3, 1], 40
+    lens = [blocks * page, (blocks * page) // 3 + 1, 5]
+    g = torch.Generator().manual_seed(blocks)
+    k, v, table, lengths = build_cache(g, lens, HK, D, BF, page)
+    cache = PagedCache(k, v)
+    cache.key_sums.copy_(torch.randint(-1, 2, cache.key_sums.shape, generator=g) if ties else torch.randn(cache.key_sums.shape, generator=g))
+    q = tokens(g, sum(new), HK * G, D, BF)
+    if ties:
+        q = torch.zeros_like(q)
+        q[..., :2] = 1.0                     # scores of a few small whole numbers over 16
+    got = cache.select(q, cu_of(new), max(new), table, lengths, n_select)
+    cache.check()
+    want, at = torch.full(got.shape, -1, dtype=torch.int32), 0
+    for s, (n, m) in enumerate(zip(lens, new)):
+        nb = -(-n // page)
+        held = torch.tensor([min(page, n - b * page) for b in range(nb)])
+        x = plain.lists_of(q[at:at + m].cpu(), cache.key_sums[table[s, :nb].long()].cpu(), held, n, n - m, page, 1, n_select, 1, 1, True)
+        want[s, :x.shape[0]] = x
+        at += m
+    assert torch.equal(got.cpu(), want)
