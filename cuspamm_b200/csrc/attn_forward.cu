@@ -120,18 +120,44 @@ struct RowsPlan {
     int n_split;            // ranges of keys
     int split_keys;         // keys of a range, a multiple of the block
     int max_entries;        // blocks of a range
+    bool cluster;           // the ranges of 16 rows are a cluster's blocks of threads, which join them
     bool pairs;             // pairs of tiles of 128 rows to a block of threads
     TileShape shape;        // of a tile of 128 rows
 };
 
 constexpr int ROWS_STAGES = 3;
 constexpr int ROWS_WARPS = 4;
+constexpr int ROWS_CLUSTER = 8;
+
+__device__ __forceinline__ void cluster_barrier()
+{
+    asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+}
+// Shared memory of block `rank` of the cluster, at this block's address `p`.
+__device__ __forceinline__ uint32_t cluster_addr(const void *p, int rank)
+{
+    uint32_t there;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(smem_addr(p)), "r"(rank));
+    return there;
+}
+__device__ __forceinline__ float cluster_load(uint32_t at)
+{
+    float x;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x) : "r"(at) : "memory");
+    return x;
+}
+__device__ __forceinline__ float4 cluster_load4(uint32_t at)
+{
+    float4 x;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(x.x), "=f"(x.y), "=f"(x.z), "=f"(x.w) : "r"(at) : "memory");
+    return x;
+}
 
 // 16 rows (queries x heads) of one key head against one range of its keys.  Each of the four warps takes every fourth
 // chunk of 16 keys with a ring of three chunks of its own, so that nothing but the end synchronises the block; the four
 // results are joined in shared memory.  Bound by the reading of keys and values when rows are few: 32 sequences of up to 16384
 // keys, 8 key heads of 128 (1.43 GB), take 243 us, 5.9 TB/s, and 6 us to join the ranges; 16 lists of 32 pages of 64, 4 key
-// heads (68 MB), 22 us, 3.0 TB/s.  There every block of threads finds its list, then the pages, then the keys, one wait on
+// heads (68 MB), 23 us with the joining, 2.9 TB/s.  There every block of threads finds its list, then the pages, then the keys, one wait on
 // memory after the other, and has 28 chunks of 16 keys to hide them behind.
 template <typename T, int D>
 __global__ __launch_bounds__(128) void attn_rows_kernel(const __grid_constant__ spamm_attn a, const RowsPlan p,
@@ -175,20 +201,18 @@ __global__ __launch_bounds__(128) void attn_rows_kernel(const __grid_constant__ 
     cp_commit();
 
     const int n_blocks = ceil_div(limit_max, a.block);
-    const int per_split = p.split_keys / a.block;
-    int e0, e1;
+    int count = n_blocks;
     if (a.n_select) {
         if (warp == 0) {
             const int n = attn_load_list(a, s, qb, p.nqb, h, n_blocks, blk, lane);
             if (lane == 0) shared_count = n;
         }
         __syncthreads();
-        e0 = min(split * per_split, shared_count);
-        e1 = min(e0 + per_split, shared_count);
-    } else {
-        e0 = min(split * per_split, n_blocks);
-        e1 = min(e0 + per_split, n_blocks);
+        count = shared_count;
     }
+    // the blocks of a cluster wait for one another and share the keys evenly
+    const int per_split = p.cluster ? ceil_div(count, p.n_split) : p.split_keys / a.block;
+    const int e0 = min(split * per_split, count), e1 = min(e0 + per_split, count);
     // where each block's rows begin: for k; for v they begin at the same place in pages
     for (int e = e0 + tid; e < e1; e += 128) {
         const int b = a.n_select ? blk[e] : e;
@@ -316,6 +340,7 @@ __global__ __launch_bounds__(128) void attn_rows_kernel(const __grid_constant__ 
     // join the four warps: [warp][16][D] sums, then maxima and sums of the rows
     float *so = reinterpret_cast<float *>(ring);
     float *sm = so + ROWS_WARPS * 16 * D, *sl = sm + ROWS_WARPS * 16;
+    float *range_o = sl + ROWS_WARPS * 16, *range_lse = range_o + 16 * D;        // of the rows, for the cluster
 #pragma unroll
     for (int n = 0; n < D / 8; n++)
 #pragma unroll
@@ -366,17 +391,19 @@ __global__ __launch_bounds__(128) void attn_rows_kernel(const __grid_constant__ 
             if (a.d_lse && (tid & 7) == 0) a.d_lse[row * a.heads + head] = lse2 * LN2;
         } else {
             const int64_t at = (row * a.heads + head) * p.n_split + split;
+            float *dst = p.cluster ? range_o + r * D : part_o + at * D;
 #pragma unroll
-            for (int i = 0; i < D / 8; i++) part_o[at * D + c0 + i] = y[i] * inv;
-            if ((tid & 7) == 0) part_lse[at] = lse2;
+            for (int i = 0; i < D / 8; i += 4)
+                *reinterpret_cast<float4 *>(dst + c0 + i) = make_float4(y[i] * inv, y[i + 1] * inv, y[i + 2] * inv, y[i + 3] * inv);
+            if ((tid & 7) == 0) *(p.cluster ? range_lse + r : part_lse + at) = lse2;
         }
     }
-    if (!__syncthreads_or(odd)) return;
+    const bool any_odd = __syncthreads_or(odd);
     // rows that are not finite once more, over their own keys alone (see row_keys)
     if (odd) atomicOr(&odd_rows, 1u << r);
-    __syncthreads();
+    if (any_odd) __syncthreads();
 #pragma unroll 1
-    for (int sr = warp; sr < rows; sr += ROWS_WARPS) {
+    for (int sr = warp; sr < rows && any_odd; sr += ROWS_WARPS) {
         if (!(odd_rows >> sr & 1)) continue;
         const int x = tile * 16 + sr, query = qb * p.bq + x / G, head = h * G + x % G;
         const int64_t row = sq.row0 + query;
@@ -401,10 +428,42 @@ __global__ __launch_bounds__(128) void attn_rows_kernel(const __grid_constant__ 
                     *reinterpret_cast<uint32_t *>(static_cast<T *>(a.d_o_low) + (row * a.heads + head) * D + d) =
                         Pack<T>::two(y[i] * inv - back.x, y[i + 1] * inv - back.y);
             } else {
-                *reinterpret_cast<float2 *>(part_o + at * D + d) = make_float2(y[i] * inv, y[i + 1] * inv);
+                *reinterpret_cast<float2 *>((p.cluster ? range_o + sr * D : part_o + at * D) + d) = make_float2(y[i] * inv, y[i + 1] * inv);
             }
         }
     }
+    if (!p.cluster) return;
+    // the ranges joined as by attn_join_kernel, each block a share of the rows' pieces of eight values
+    cluster_barrier();
+    for (int i = split * 128 + tid; i < rows * (D / 8); i += p.n_split * 128) {
+        const int jr = i / (D / 8), d = i % (D / 8) * 8;
+        float lse[ROWS_CLUSTER], top = -CUDART_INF_F, total = 0.f, y[8] = {};
+#pragma unroll
+        for (int j = 0; j < ROWS_CLUSTER; j++) {
+            lse[j] = j < p.n_split ? cluster_load(cluster_addr(range_lse + jr, j)) : -CUDART_INF_F;
+            top = fmaxf(top, lse[j]);
+        }
+        const float t0 = top == -CUDART_INF_F ? 0.f : top;
+#pragma unroll
+        for (int j = 0; j < ROWS_CLUSTER; j++) {
+            if (lse[j] == -CUDART_INF_F) continue;
+            const float f = fast_exp2(lse[j] - t0);
+            const uint32_t from = cluster_addr(range_o + jr * D + d, j);
+            const float4 u = cluster_load4(from), v = cluster_load4(from + 16);
+            total += f;
+            y[0] += f * u.x; y[1] += f * u.y; y[2] += f * u.z; y[3] += f * u.w;
+            y[4] += f * v.x; y[5] += f * v.y; y[6] += f * v.z; y[7] += f * v.w;
+        }
+        const float inv = total == 0.f ? 0.f : 1.f / total;
+#pragma unroll
+        for (int k = 0; k < 8; k++) y[k] *= inv;
+        const int x = tile * 16 + jr, head = h * G + x % G;
+        const int64_t row = sq.row0 + qb * p.bq + x / G;
+        store8<T>(static_cast<T *>(a.d_o) + row * a.o_token + head * a.o_head + d,
+                  a.d_o_low ? static_cast<T *>(a.d_o_low) + (row * a.heads + head) * D + d : nullptr, y);
+        if (a.d_lse && d == 0) a.d_lse[row * a.heads + head] = total == 0.f ? -CUDART_INF_F : (t0 + log2f(total)) * LN2;
+    }
+    cluster_barrier();                       // no block leaves while another reads its shared memory
 }
 
 // ---- pairs of tiles of 128 rows on the tensor memory path
@@ -922,7 +981,7 @@ __global__ __launch_bounds__(TILES * 256 + 64, TILES == 1 ? 2 : 1) void attn_tc_
 
 // Joins the ranges of keys of every row: o = sum_i 2^(lse_i - lse) o_i.  One warp for a row and head.  Bound by the reading of
 // the ranges' floats: 1774 tokens of 32 heads of 128 in 3 ranges (102 MB) 28 us, 3.7 TB/s; one token for each of 32 sequences
-// 6 us, a launch's own time.
+// 6 us, a launch's own time.  (Few ranges of short rows are joined by a cluster instead, in attn_rows_kernel.)
 template <typename T, int D>
 __global__ __launch_bounds__(128) void attn_join_kernel(const __grid_constant__ spamm_attn a, int n_split,
                                                         const float *part_o, const float *part_lse)
@@ -1063,12 +1122,16 @@ static RowsPlan rows_plan(const spamm_attn &a)
     const int64_t units = (int64_t)a.batch * a.kv_heads * p.nqb * p.tiles;
     // Tiles of 128 rows: enough blocks of threads to fill 148 SMs several times over (with lists the work is short as it is:
     // once), ranges of 1024 keys at the least.  Tiles of 16: two blocks per SM; lists are of one length, so one wave of equal
-    // ranges does (296 blocks: 22 us against 30 us with 600 for 64 lists of 2048 keys), whole sequences are not, and two waves
+    // ranges does (296 blocks: 23 us against 37 us with 444 for 64 lists of 2048 keys), whole sequences are not, and two waves
     // even them out.
     int64_t want = (tc ? a.n_select ? 148 : 740 : a.n_select ? 296 : 600) / units + (tc || !a.n_select);
     want = max((int64_t)1, min(want, (blocks * a.block + (tc ? 1023 : 255)) / (tc ? 1024 : 256)));
     int64_t per = min(most, (blocks + want - 1) / want);
     p.n_split = (int)((blocks + per - 1) / per);
+    // Ranges of tiles of 16 as a cluster, joined in its shared memory, where all of them run at once: 64 lists of 2048 keys 23 us
+    // against 22 + 5.5 us with a kernel that joins.  In several waves the blocks of a cluster that are done hold room for which
+    // others wait: 32 sequences of up to 16384 keys 265 us (more ranges 256 us and 277 us) against 243 + 6 us.
+    p.cluster = !tc && p.n_split > 1 && p.n_split <= ROWS_CLUSTER && units * p.n_split <= 296;
     p.max_entries = (int)(tc && a.n_select ? min(per, listed) : per);
     p.split_keys = (int)(per * a.block);
     return p;
@@ -1102,9 +1165,24 @@ static int forward_launch(const spamm_attn &a, float *scratch, cudaStream_t stre
         const size_t smem = rows_smem(a, p);
         int st = attn_set_smem((const void *)attn_rows_kernel<T, D>, smem);
         if (st) return st;
-        attn_rows_kernel<T, D><<<(unsigned)grid, 128, smem, stream>>>(a, p, part_o, part_lse);
+        if (p.cluster) {
+            cudaLaunchConfig_t how = {};
+            cudaLaunchAttribute cluster = {};
+            cluster.id = cudaLaunchAttributeClusterDimension;
+            cluster.val.clusterDim.x = p.n_split;
+            cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
+            how.gridDim = dim3((unsigned)grid);
+            how.blockDim = dim3(128);
+            how.dynamicSmemBytes = smem;
+            how.stream = stream;
+            how.attrs = &cluster;
+            how.numAttrs = 1;
+            SPAMM_CUDA_TRY(cudaLaunchKernelEx(&how, attn_rows_kernel<T, D>, a, p, part_o, part_lse));
+        } else {
+            attn_rows_kernel<T, D><<<(unsigned)grid, 128, smem, stream>>>(a, p, part_o, part_lse);
+        }
     }
-    if (p.n_split > 1)
+    if (p.n_split > 1 && !p.cluster)
         attn_join_kernel<T, D><<<(unsigned)((rows + 3) / 4), 128, 0, stream>>>(a, p.n_split, part_o, part_lse);
     SPAMM_CUDA_TRY(cudaGetLastError());
     return SPAMM_OK;
@@ -1118,7 +1196,7 @@ extern "C" size_t spamm_attn_forward_scratch_bytes(const spamm_attn *a)
 {
     if (attn_check(a, false) || !a->batch || !a->max_q || !a->tokens) return 0;
     const RowsPlan p = rows_plan(*a);
-    return p.n_split > 1 ? (size_t)a->tokens * a->heads * p.n_split * (a->dim + 1) * sizeof(float) : 0;
+    return p.n_split > 1 && !p.cluster ? (size_t)a->tokens * a->heads * p.n_split * (a->dim + 1) * sizeof(float) : 0;
 }
 
 extern "C" int spamm_attn_forward_dev(const spamm_attn *a, void *d_scratch, size_t scratch_bytes, void *stream)

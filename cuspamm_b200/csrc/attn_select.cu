@@ -442,7 +442,7 @@ __device__ __forceinline__ void mma_double(double *c, double a, double b)
                  : "+d"(c[0]), "+d"(c[1]) : "d"(a), "d"(b));
 }
 
-// Bound by the double products for long sequences and by the searches for the lists: 32768 lists over up to 128 blocks 72 us, of
+// Bound by the double products for long sequences and by the searches for the lists: 32768 lists over up to 128 blocks 66 us, of
 // which the products (1.1 GFLOP in double, half of them masked) are less than half; 4512 lists over up to 256 blocks 33 us.
 template <int D, int QT>
 __global__ __launch_bounds__(256) void attn_select_tile_kernel(const __grid_constant__ spamm_attn a, int nqb, int nkb, int n_first,
@@ -559,12 +559,12 @@ __global__ __launch_bounds__(256) void attn_select_tile_kernel(const __grid_cons
 // One query block (the newest token): plain products, joined by two shuffles.  Several: m8n8k4, where a lane's four values
 // enter four products in turn (the sum then takes the values in another order, for both operands alike).  Sums of up to 16 rows
 // are taken here, by every block of threads for itself: one launch less, for a few kilobytes of q.  16 sequences of up to 65537
-// keys in pages of 64, 8 key heads of 128 (44 MB of key sums): 17 us, 2.6 TB/s.
+// keys in pages of 64, 8 key heads of 128 (44 MB of key sums): 16 us, 2.8 TB/s.
 constexpr int SPREAD_ROWS = 16;          // rows of a query block up to which their sums are taken here
 constexpr int SPREAD_BLOCKS = 32, SPREAD_WARPS = 4;
 
 template <typename T, int D>
-__global__ __launch_bounds__(SPREAD_WARPS * 32, 4) void attn_spread_scores_kernel(const __grid_constant__ spamm_attn a, int nqb, int spans,
+__global__ __launch_bounds__(SPREAD_WARPS * 32, 6) void attn_spread_scores_kernel(const __grid_constant__ spamm_attn a, int nqb, int spans,
                                                                                  int nkb, int n_first, int n_local,
                                                                                  const float *key_sums, const double *query_sums,
                                                                                  unsigned long long *keys)
@@ -665,7 +665,8 @@ __global__ __launch_bounds__(SPREAD_WARPS * 32, 4) void attn_spread_scores_kerne
     }
 }
 
-// The lists of spread scores: by one warp each up to LARGEST_WARP blocks, by a block of threads beyond.
+// The lists of spread scores: by one warp each up to LARGEST_WARP blocks (128 lists over up to 1025: 10 us, the
+// latency of its rounds), by a block of threads beyond (14 us).
 constexpr int LARGEST_WARP = 2048;
 
 static __device__ __forceinline__ int candidates(const spamm_attn &a, int nqb, int list)
@@ -738,7 +739,7 @@ __global__ __launch_bounds__(128) void attn_select_kernel(const __grid_constant_
 
 // Which of the four (times with the sums, 8 key heads of 128 unless noted).  A tile of eight query blocks wants eight in a
 // sequence, and tiles enough to fill the GPU when the blocks of keys are many: else the scores are spread (16 sequences of one
-// token over up to 1025 blocks: 17 us and 14 us for the lists; as tiles of one list each seven eighths of the products would be
+// token over up to 1025 blocks: 16 us and 10 us for the lists; as tiles of one list each seven eighths of the products would be
 // empty).  1024 lists over 32 blocks: tiles of 8 15 us, spread 24 us, one by one 19 us.  Tiles of 32 need 4096 lists: 2048
 // lists over 64 blocks 19 us against 17 us in tiles of 8, 8192 lists 30 us against 42 us (one by one 79 us, spread 103 us).
 // Beyond 1024 blocks the scores of eight query blocks do not fit shared memory.

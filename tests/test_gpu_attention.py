@@ -736,3 +736,52 @@ def test_select_of_new_tokens_over_many_pages(blocks, ties):
         want[s, :x.shape[0]] = x
         at += m
     assert torch.equal(got.cpu(), want)
+
+
+@pytest.mark.parametrize("lens,HK,G,n_select,block", [([2000, 1, 3000, 70], 2, 4, 16, 64), ([40, 900], 1, 16, 60, 16),
+                                                      ([700], 1, 3, 0, 16), ([130, 260, 390], 2, 2, 0, 32)])
+def test_ranges_joined_by_a_cluster(lens, HK, G, n_select, block):
+    """Few rows whose keys are cut into a handful of ranges, some of them without keys, a NaN in one key that some rows read."""
+    from cuspamm_b200 import PagedCache
+
+    D, new = 128, [min(2, n) for n in lens]
+    g = torch.Generator().manual_seed(sum(lens))
+    k, v, table, lengths = build_cache(g, lens, HK, D, BF, block)
+    last = int(table[0, (lens[0] - 1) // block])
+    k[last, 0, (lens[0] - 1) % block, 3] = torch.nan               # the last token's key: only its own row sees it
+    cache = PagedCache(k, v)
+    q = tokens(g, sum(new), HK * G, D, BF)
+    lists = None
+    if n_select:
+        lists = torch.full((len(lens), max(new), HK, n_select), -1, dtype=torch.int32)
+        for s, n in enumerate(lens):
+            nb = -(-n // block)
+            for i in range(max(new)):
+                for h in range(HK):
+                    m = min(n_select, nb)
+                    lists[s, i, h, :m] = torch.randperm(nb, generator=g)[:m].sort().values.int()
+        lists[0, :, :, -1] = (lens[0] - 1) // block
+        lists[0] = lists[0].sort(-1).values
+        lists = lists.to(DEV)
+    o, lse = cache.attend(q, cu_of(new), max(new), table, lengths, lists=lists, return_lse=True)
+    cache.check()
+    at = 0
+    for s, (n, m) in enumerate(zip(lens, new)):
+        pages = table[s, :-(-n // block)].long()
+        ks = k[pages].transpose(1, 2).reshape(-1, HK, D)[:n].double()
+        vs = v[pages].transpose(1, 2).reshape(-1, HK, D)[:n].double()
+        for i in range(m):
+            for h in range(HK):
+                ok = torch.arange(n, device=DEV) <= n - m + i
+                if n_select:
+                    ok &= torch.isin(torch.arange(n, device=DEV) // block, lists[s, i, h])
+                z = (q[at + i, h * G:(h + 1) * G].double() @ ks[ok, h].T) * D ** -0.5
+                want = torch.softmax(z, 1) @ vs[ok, h]
+                got = o[at + i, h * G:(h + 1) * G].double()
+                assert torch.equal(torch.isnan(got), torch.isnan(want))
+                # p and o are rounded to bf16 (2^-8 each, relative to the sum of |p v| and to |o|); sums and exponentials in float
+                bound = 2.0 ** -8 * (torch.softmax(z, 1) @ vs[ok, h].abs() + want.abs()) + 1e-4
+                assert torch.isnan(want).any() or bool(((got - want).abs() <= bound).all()), (s, i, h)
+                if not torch.isnan(z).any():
+                    torch.testing.assert_close(lse[at + i, h * G:(h + 1) * G].double(), torch.logsumexp(z, 1), rtol=0, atol=1e-4)
+        at += m
