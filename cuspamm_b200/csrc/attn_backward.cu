@@ -12,6 +12,8 @@
 
 namespace spamm {
 
+constexpr int TK_MAX_CHUNK = 640;            // query blocks of a work item: their list lies in what the tiles leave of shared memory
+
 struct BackwardPlan {
     int nqb, nkb, words;        // query blocks, blocks of keys, 32-bit words of a block's bits
     int chunk;                  // query blocks of a work item
@@ -34,7 +36,7 @@ static BackwardPlan backward_plan(const spamm_attn &a)
     p.nkb = ceil_div(a.max_q, a.block);
     p.words = ceil_div(p.nqb, 32);
     const int64_t rows = (int64_t)min(a.query_block, a.max_q) * G;
-    p.chunk = (int)max((int64_t)1, min((int64_t)1024, 8192 / rows));
+    p.chunk = (int)max((int64_t)1, min((int64_t)TK_MAX_CHUNK, 8192 / rows));
     p.per = fast_div((uint32_t)rows);
     p.G = fast_div((uint32_t)G);
     // a tensor copy takes the heads of a key head of as many queries as fit a tile or make up a query block, when that
@@ -749,13 +751,17 @@ constexpr int TK_ROWS = 128, TK_MAX_KEYS = 64, TK_SOFTMAX = 256, TK_THREADS = TK
 // Tensor memory columns, and blocks of threads per SM: short blocks of small heads leave room for two.
 __host__ __device__ constexpr int tk_cols(int keys) { return keys == 64 ? 512 : keys == 32 ? 256 : 128; }
 __host__ __device__ constexpr int tk_per_sm(int dim, int keys) { return dim == 64 && keys < 64 ? 2 : 1; }
+// Buffers of the ring that the tiles of dO and Q pass through in turn (dO of tile j is the ring's 2 j-th, Q its 2 j + 1-st).
+// An even number where the two of a tile must lie side by side.
+__host__ __device__ constexpr int tk_slots(int dim, int keys) { return dim == 128 ? 5 : keys < 64 ? 4 : 8; }
+constexpr int TK_MAX_SLOTS = 8;
 
 struct TkCtrl {
-    uint64_t kv_full, q_full[2], q_empty[2], do_full[2], do_empty[2], s_full[2], p_full, dv_done, ds_full, dk_done;
+    uint64_t kv_full, full[TK_MAX_SLOTS], empty[TK_MAX_SLOTS], s_full[2], p_full, dv_done, ds_full, dk_done;
     uint32_t tmem_base;
     uint32_t abort_flag;
     int32_t err;
-    int32_t pad;
+    int32_t warp_sum[TK_THREADS / 32];
 };
 
 template <typename T, int D, int TK_KEYS>
@@ -770,11 +776,11 @@ __global__ __launch_bounds__(TK_THREADS, tk_per_sm(D, TK_KEYS)) void attn_dkv_tc
     uint8_t *const smem = smem_tc;
     constexpr int KT = TK_KEYS * D * 2, RT = TK_ROWS * D * 2, PT = TK_ROWS * 128;     // rows of p and ds take a panel's 128 bytes
     constexpr int HALF = TK_KEYS / 2;                           // keys of a thread
-    const uint32_t k_tile = smem_u32(smem), v_tile = k_tile + KT, ring = v_tile + KT;      // ring: [stage][do | q]
-    const uint32_t p_tile = ring + 4 * RT, ds_tile = p_tile + PT;
-    TkCtrl *ctrl = reinterpret_cast<TkCtrl *>(smem + 2 * KT + 4 * RT + 2 * PT);
+    constexpr int SLOTS = tk_slots(D, TK_KEYS);
+    const uint32_t k_tile = smem_u32(smem), v_tile = k_tile + KT, ring = v_tile + KT;
+    const uint32_t p_tile = ring + SLOTS * RT, ds_tile = p_tile + PT;
+    TkCtrl *ctrl = reinterpret_cast<TkCtrl *>(smem + 2 * KT + SLOTS * RT + 2 * PT);
     int *list = reinterpret_cast<int *>(ctrl + 1);
-    __shared__ int warp_sum[TK_THREADS / 32];
 
     const int halves = a.block / TK_KEYS;
     const int half = blockIdx.x % halves;
@@ -794,13 +800,11 @@ __global__ __launch_bounds__(TK_THREADS, tk_per_sm(D, TK_KEYS)) void attn_dkv_tc
     if (warp == 8) {
         if (lane == 0) {
             mbar_init(smem_u32(&ctrl->kv_full), 128);
-            for (int i = 0; i < 2; i++) {
-                mbar_init(smem_u32(&ctrl->q_full[i]), 64);
-                mbar_init(smem_u32(&ctrl->do_full[i]), 64);
-                mbar_init(smem_u32(&ctrl->q_empty[i]), 1);
-                mbar_init(smem_u32(&ctrl->do_empty[i]), 1);
-                mbar_init(smem_u32(&ctrl->s_full[i]), 1);
+            for (int i = 0; i < SLOTS; i++) {
+                mbar_init(smem_u32(&ctrl->full[i]), 64);
+                mbar_init(smem_u32(&ctrl->empty[i]), 1);
             }
+            for (int i = 0; i < 2; i++) mbar_init(smem_u32(&ctrl->s_full[i]), 1);
             mbar_init(smem_u32(&ctrl->p_full), TK_SOFTMAX);
             mbar_init(smem_u32(&ctrl->ds_full), TK_SOFTMAX);
             mbar_init(smem_u32(&ctrl->dv_done), 1);
@@ -814,7 +818,7 @@ __global__ __launch_bounds__(TK_THREADS, tk_per_sm(D, TK_KEYS)) void attn_dkv_tc
         tc_fence_before();
     }
     const int n_list = expand_bits<TK_THREADS>(bits + (group * p.nkb + item.kb) * p.words, p.words, item.chunk * p.chunk, p.chunk,
-                                               list, warp_sum);
+                                               list, ctrl->warp_sum);
     tc_fence_after();
     const int bq = min(a.query_block, a.max_q), per = bq * G;
     // all listed query blocks are full but the sequence's last one, which can only be the last of the list
@@ -837,8 +841,12 @@ __global__ __launch_bounds__(TK_THREADS, tk_per_sm(D, TK_KEYS)) void attn_dkv_tc
         const bool is_q = tid - TK_SOFTMAX - 32 >= 64;
         const T *src = is_q ? static_cast<const T *>(a.d_q) : d_do;
         const int64_t token = is_q ? a.q_token : do_token, stride = is_q ? a.q_head : do_head;
-        uint64_t *full = is_q ? ctrl->q_full : ctrl->do_full, *empty = is_q ? ctrl->q_empty : ctrl->do_empty;
-        const uint32_t my_ring = ring + (is_q ? RT : 0);
+        // waits until the buffer of tile j is free: the n-th of the ring takes the place of the (n - SLOTS)-th
+        auto number = [&](int j) { return 2 * j + (is_q ? 1 : 0); };
+        auto buffer_free = [&](int j) {
+            const int n = number(j);
+            return n < SLOTS || __all_sync(~0u, ws.wait(smem_u32(&ctrl->empty[n % SLOTS]), n / SLOTS - 1, 1));
+        };
         {
             const T *kv = is_q ? static_cast<const T *>(a.d_k) : static_cast<const T *>(a.d_v);
             const int64_t kv_token = is_q ? a.k_token : a.v_token, kv_head = is_q ? a.k_head : a.v_head;
@@ -864,14 +872,15 @@ __global__ __launch_bounds__(TK_THREADS, tk_per_sm(D, TK_KEYS)) void attn_dkv_tc
             const int box_rows = p.box_tokens * G, boxes = TK_ROWS / box_rows;
             const int i = t % boxes, panel = t / boxes;
             for (int j = 0; j < by_map; j++) {
-                if (j > 1) fine = __all_sync(~0u, ws.wait(smem_u32(&empty[j & 1]), (j >> 1) - 1, 1));
+                fine = buffer_free(j);
                 if (!fine) break;
-                const uint32_t bar = smem_u32(&full[j & 1]);
+                const int slot = number(j) % SLOTS;
+                const uint32_t bar = smem_u32(&ctrl->full[slot]);
                 if (panel < D / 64) {
                     int query, head;
                     locate(j * TK_ROWS + i * box_rows, &query, &head);
                     mbar_expect_tx(bar, box_rows * 128);
-                    tma_box(my_ring + (j & 1) * 2 * RT + panel * (TK_ROWS * 128) + i * box_rows * 128, &map.map, panel * 64, head,
+                    tma_box(ring + slot * RT + panel * (TK_ROWS * 128) + i * box_rows * 128, &map.map, panel * 64, head,
                             sq.row0 + query, bar);
                 }
                 mbar_arrive(bar);
@@ -881,16 +890,21 @@ __global__ __launch_bounds__(TK_THREADS, tk_per_sm(D, TK_KEYS)) void attn_dkv_tc
                 }
             }
         }
+        int waiting = by_map ? -1 : -2;                         // what was requested and not announced: a tile, -2: K or V
+        auto announce = [&] {
+            if (waiting != -1) signal(waiting == -2 ? &ctrl->kv_full : &ctrl->full[number(waiting) % SLOTS]);
+            waiting = -1;
+        };
         for (int j = by_map; j <= n_tiles && fine; j++) {
-            if (j > 1 && j > by_map) {
-                // the buffer comes free only when the tile before has been worked on: announce that one first
-                cp_wait<0>();
-                signal(&full[(j - 1) & 1]);
-            }
             if (j < n_tiles) {
-                if (j > 1) fine = __all_sync(~0u, ws.wait(smem_u32(&empty[j & 1]), (j >> 1) - 1, 1));
+                if (number(j) >= SLOTS && waiting != -1) {
+                    // the buffer comes free only when tiles before have been worked on: announce them first
+                    cp_wait<0>();
+                    announce();
+                }
+                fine = buffer_free(j);
                 if (!fine) break;
-                const uint32_t dst = my_ring + (j & 1) * 2 * RT;
+                const uint32_t dst = ring + number(j) % SLOTS * RT;
 #pragma unroll 1
                 for (int half_tile = 0; half_tile < 2; half_tile++) {
                     // each lane finds one of 32 rows, the copies take the addresses from it
@@ -907,10 +921,11 @@ __global__ __launch_bounds__(TK_THREADS, tk_per_sm(D, TK_KEYS)) void attn_dkv_tc
                 }
             }
             cp_commit();
-            if (j <= 1 && !by_map) {
-                cp_wait<1>();                                   // the group before: K or V, or the rows of the first tile
-                signal(j ? &full[0] : &ctrl->kv_full);
+            if (waiting != -1) {
+                cp_wait<1>();                                   // the group before this one
+                announce();
             }
+            if (j < n_tiles) waiting = j;
         }
         cp_wait<0>();
     } else if (warp == 8) {
@@ -918,9 +933,9 @@ __global__ __launch_bounds__(TK_THREADS, tk_per_sm(D, TK_KEYS)) void attn_dkv_tc
         if (n_tiles) {
             constexpr uint32_t s_desc = mma_desc<T>(128, TK_KEYS, false, false), o_desc = mma_desc<T>(128, TK_KEYS, true, true);
             const uint32_t base = __shfl_sync(~0u, tmem, 0);
-            const uint64_t k_desc = desc_k_major(k_tile), v_desc = desc_k_major(v_tile), do_desc = desc_k_major(ring), q_desc = desc_k_major(ring + RT);
+            const uint64_t k_desc = desc_k_major(k_tile), v_desc = desc_k_major(v_tile), row_desc = desc_k_major(ring);
             // A of the second products: 128 values of dO (of Q) x 128 rows; with D = 64 the tiles of dO and Q one behind the other
-            const uint64_t dot_desc = desc_mn_major(ring, TK_ROWS), qt_desc = desc_mn_major(D == 64 ? ring : ring + RT, TK_ROWS);
+            const uint64_t turned_desc = desc_mn_major(ring, TK_ROWS);
             const uint64_t p_desc = desc_mn_major(p_tile, TK_ROWS), ds_desc = desc_mn_major(ds_tile, TK_ROWS);
             bool fine = __all_sync(~0u, ws.wait(smem_u32(&ctrl->kv_full), 0, 2));
             // Whichever is ready: dP of the next tile (at most one tile under way), its S, or the second products of the oldest
@@ -928,14 +943,16 @@ __global__ __launch_bounds__(TK_THREADS, tk_per_sm(D, TK_KEYS)) void attn_dkv_tc
             // order the second products would wait for the copies of the next tile, which wait for the buffers that they free.)
             int next_dp = 0, next_s = 0, second = 0;
             unsigned long long t0 = 0;
+            auto do_slot = [](int j) { return 2 * j % SLOTS; };
+            auto q_slot = [](int j) { return (2 * j + 1) % SLOTS; };
             while (second < n_tiles) {
-                const uint32_t dp_stage = (next_dp & 1) * (2 * RT >> 4), s_stage = (next_s & 1) * (2 * RT >> 4);
-                if (next_s < next_dp && __all_sync(~0u, mbar_test(smem_u32(&ctrl->q_full[next_s & 1]), (next_s >> 1) & 1))) {
+                const uint32_t dp_stage = do_slot(next_dp) * (RT >> 4), s_stage = q_slot(next_s) * (RT >> 4);
+                if (next_s < next_dp && __all_sync(~0u, mbar_test(smem_u32(&ctrl->full[q_slot(next_s)]), (2 * next_s + 1) / SLOTS & 1))) {
                     tc_fence_after();
                     if (elect_one()) {
 #pragma unroll
                         for (int ks = 0; ks < D / 16; ks++)
-                            mma_ss(base + (next_s & 1) * 2 * TK_KEYS, q_desc + s_stage + step_k_major(TK_ROWS, ks), k_desc + step_k_major(TK_KEYS, ks),
+                            mma_ss(base + (next_s & 1) * 2 * TK_KEYS, row_desc + s_stage + step_k_major(TK_ROWS, ks), k_desc + step_k_major(TK_KEYS, ks),
                                    s_desc, ks != 0);
                         umma_commit(smem_u32(&ctrl->s_full[next_s & 1]));
                     }
@@ -943,12 +960,12 @@ __global__ __launch_bounds__(TK_THREADS, tk_per_sm(D, TK_KEYS)) void attn_dkv_tc
                     next_s++;
                     t0 = 0;
                 } else if (next_dp < n_tiles && next_dp - second < 2 &&
-                           __all_sync(~0u, mbar_test(smem_u32(&ctrl->do_full[next_dp & 1]), (next_dp >> 1) & 1))) {
+                           __all_sync(~0u, mbar_test(smem_u32(&ctrl->full[do_slot(next_dp)]), 2 * next_dp / SLOTS & 1))) {
                     tc_fence_after();
                     if (elect_one()) {
 #pragma unroll
                         for (int ks = 0; ks < D / 16; ks++)
-                            mma_ss(base + (next_dp & 1) * 2 * TK_KEYS + TK_KEYS, do_desc + dp_stage + step_k_major(TK_ROWS, ks),
+                            mma_ss(base + (next_dp & 1) * 2 * TK_KEYS + TK_KEYS, row_desc + dp_stage + step_k_major(TK_ROWS, ks),
                                    v_desc + step_k_major(TK_KEYS, ks), s_desc, ks != 0);
                     }
                     __syncwarp();
@@ -956,12 +973,13 @@ __global__ __launch_bounds__(TK_THREADS, tk_per_sm(D, TK_KEYS)) void attn_dkv_tc
                     t0 = 0;
                 } else if (second < next_s && __all_sync(~0u, mbar_test(smem_u32(&ctrl->p_full), second & 1))) {
                     tc_fence_after();
-                    const uint32_t stage = (second & 1) * (2 * RT >> 4);
+                    const int do_at = do_slot(second), q_at = q_slot(second);
+                    const uint32_t do_stage = do_at * (RT >> 4), q_stage = (D == 64 ? do_at : q_at) * (RT >> 4);
                     if (elect_one()) {
 #pragma unroll
                         for (int ks = 0; ks < TK_ROWS / 16; ks++)
-                            mma_ss(base + 4 * TK_KEYS, dot_desc + stage + step_mn_major(ks), p_desc + step_mn_major(ks), o_desc, second || ks);
-                        if (D == 128) umma_commit(smem_u32(&ctrl->do_empty[second & 1]));
+                            mma_ss(base + 4 * TK_KEYS, turned_desc + do_stage + step_mn_major(ks), p_desc + step_mn_major(ks), o_desc, second || ks);
+                        if (D == 128) umma_commit(smem_u32(&ctrl->empty[do_at]));
                         umma_commit(smem_u32(&ctrl->dv_done));
                     }
                     __syncwarp();
@@ -971,9 +989,9 @@ __global__ __launch_bounds__(TK_THREADS, tk_per_sm(D, TK_KEYS)) void attn_dkv_tc
                     if (elect_one()) {
 #pragma unroll
                         for (int ks = 0; ks < TK_ROWS / 16; ks++)
-                            mma_ss(base + 5 * TK_KEYS, qt_desc + stage + step_mn_major(ks), ds_desc + step_mn_major(ks), o_desc, second || ks);
-                        if (D == 64) umma_commit(smem_u32(&ctrl->do_empty[second & 1]));      // dO is half of this A too
-                        umma_commit(smem_u32(&ctrl->q_empty[second & 1]));
+                            mma_ss(base + 5 * TK_KEYS, turned_desc + q_stage + step_mn_major(ks), ds_desc + step_mn_major(ks), o_desc, second || ks);
+                        if (D == 64) umma_commit(smem_u32(&ctrl->empty[do_at]));      // dO is half of this A too
+                        umma_commit(smem_u32(&ctrl->empty[q_at]));
                         umma_commit(smem_u32(&ctrl->dk_done));
                     }
                     __syncwarp();
@@ -1146,7 +1164,7 @@ static int dkv_launch(const spamm_attn &a, const BackwardPlan &p, const T *d_do,
                       const float *delta, const unsigned *bits, const Item *items, const int *n_items, float *partial, T *dk,
                       T *dv, cudaStream_t stream)
 {
-    const size_t smem = 2 * KEYS * D * 2 + 4 * TK_ROWS * D * 2 + 2 * TK_ROWS * 128 + sizeof(TkCtrl) + p.chunk * 4;
+    const size_t smem = 2 * KEYS * D * 2 + tk_slots(D, KEYS) * TK_ROWS * D * 2 + 2 * TK_ROWS * 128 + sizeof(TkCtrl) + p.chunk * 4;
     int st = attn_set_smem((const void *)attn_dkv_tc_kernel<T, D, KEYS>, smem);
     if (st) return st;
     RowMap q_map, do_map;
