@@ -941,7 +941,7 @@ __global__ __launch_bounds__(TK_THREADS, tk_per_sm(D, TK_KEYS)) void attn_dkv_tc
             // Whichever is ready: dP of the next tile (at most one tile under way), its S, or the second products of the oldest
             // tile under way.  dO comes free after dV, before Q does, and returns before it: hence dP before S.  (In a fixed
             // order the second products would wait for the copies of the next tile, which wait for the buffers that they free.)
-            int next_dp = 0, next_s = 0, second = 0;
+            int next_dp = 0, next_s = 0, second = 0, idle = 0;
             unsigned long long t0 = 0;
             auto do_slot = [](int j) { return 2 * j % SLOTS; };
             auto q_slot = [](int j) { return (2 * j + 1) % SLOTS; };
@@ -998,7 +998,8 @@ __global__ __launch_bounds__(TK_THREADS, tk_per_sm(D, TK_KEYS)) void attn_dkv_tc
                     second++;
                     t0 = 0;
                 } else {
-                    if (__any_sync(~0u, !fine || ctrl->abort_flag)) break;
+                    if (++idle & 63) continue;                   // the clock is slow to read
+                    if (__any_sync(~0u, !fine || *ws.abort_flag)) break;
                     if (!t0) t0 = global_ns();
                     if (__any_sync(~0u, global_ns() - t0 > WAIT_LIMIT_NS)) {
                         *ws.abort_flag = 1;
@@ -1014,27 +1015,28 @@ __global__ __launch_bounds__(TK_THREADS, tk_per_sm(D, TK_KEYS)) void attn_dkv_tc
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         const float scale2 = a.scale * LOG2E;
         const float2 sc2 = make_float2(scale2, scale2), sc = make_float2(a.scale, a.scale);
-        auto row_of = [&](int j, float *minus_lse, float *minus_delta, int *n_visible) {
+        // lse and delta of the row in tile j as they are, and how many of this thread's keys it sees: requested a tile ahead,
+        // and not touched before they are needed
+        auto row_of = [&](int j, float *lse, float *dl, int *n_visible) {
             int query, head;
-            *minus_lse = -CUDART_INF_F;                         // a row that is none, or has no keys: every p zero
-            *minus_delta = 0.f;
+            *lse = -CUDART_INF_F;                               // a row that is none, or has no keys: every p zero
+            *dl = 0.f;
             *n_visible = 0;
             if (j < n_tiles && locate(j * TK_ROWS + r, &query, &head)) {
                 const int64_t at = (int64_t)(sq.row0 + query) * a.heads + head;
-                const float z = a.d_lse[at];
-                if (z != -CUDART_INF_F) *minus_lse = -z * LOG2E;
-                *minus_delta = -delta[at] * a.scale;
+                *lse = a.d_lse[at];
+                *dl = delta[at];
                 *n_visible = min(a.causal ? query + 1 - pos0 : TK_KEYS, keys) - part * HALF;
             }
         };
-        float minus_lse, minus_delta;
+        float lse, dl;
         int n_visible;
-        row_of(0, &minus_lse, &minus_delta, &n_visible);
+        row_of(0, &lse, &dl, &n_visible);
         bool fine = true;
         for (int j = 0; j < n_tiles; j++) {
-            float next_lse, next_delta;
+            const float minus_lse = lse == -CUDART_INF_F ? lse : -lse * LOG2E, minus_delta = -dl * a.scale;
             int next_visible;
-            row_of(j + 1, &next_lse, &next_delta, &next_visible);
+            row_of(j + 1, &lse, &dl, &next_visible);
             fine = __all_sync(~0u, ws.wait(smem_u32(&ctrl->s_full[j & 1]), j >> 1, 6));
             if (!fine) break;
             tc_fence_after();
@@ -1083,8 +1085,6 @@ __global__ __launch_bounds__(TK_THREADS, tk_per_sm(D, TK_KEYS)) void attn_dkv_tc
             fence_async_smem();
             tc_fence_before();
             mbar_arrive(smem_u32(&ctrl->ds_full));
-            minus_lse = next_lse;
-            minus_delta = next_delta;
             n_visible = next_visible;
         }
         if (n_tiles && fine) fine = __all_sync(~0u, ws.wait(smem_u32(&ctrl->dk_done), n_tiles - 1, 9));
