@@ -60,8 +60,9 @@ static BackwardPlan backward_plan(const spamm_attn &a)
     return p;
 }
 
-// delta = do.o for every row; a quarter of a warp for each.  Rows of no sequence get zero gradients here, and the bits
-// and counts of the lists that are turned over next are cleared (`clear`, one launch less).  Bound by the reading of do, o and the low part of o: 18000 tokens of 32 heads of 128 (440 MB) take 69 us, 6.4 TB/s.
+// delta = do.o for every row; a quarter of a warp for each.  Rows of no sequence get zero gradients here, and the bits and
+// counts of the lists that are turned over next are cleared (`clear`, one launch less).  Bound by the reading of do, o and the
+// low part of o: 18000 tokens of 32 heads of 128 (440 MB) take 66 us, 6.7 TB/s.
 template <typename T, int D>
 __global__ __launch_bounds__(256) void attn_delta_kernel(const __grid_constant__ spamm_attn a, const T *d_do, int64_t do_token,
                                                          int64_t do_head, float *delta, T *dq, T *dk, T *dv, uint4 *clear,
@@ -743,10 +744,12 @@ __global__ __launch_bounds__(TQ_THREADS, 2) void attn_dq_tc_kernel(const __grid_
 // With D = 64 the tiles of dO and Q together are the 128 rows of the second products' A: dV^T comes out in the upper half
 // of one accumulator, dK^T in the lower half of the other (the other halves are not used).
 //
-// Bound by the products: with 64 keys an M = 128, N = 64 product takes 50 clocks where 32 would be the full rate (A is read
-// from shared memory for each), and a tile of 128 rows has 32 of them.  3 sequences of up to 8192, 32 heads of 128, lists of
-// 16 blocks of 64 (553 GFLOP): 905 us, 0.61 PFLOP/s.  Chunks of 8192 rows for one item; 4096 906 us and 2048 980 us there, 267,
-// 260 and 286 us with a list for each query.
+// Bound by the chain of a tile, scores to p and ds to the second products, whose steps the roles hand one another through
+// barriers: 3 sequences of up to 8192, 32 heads of 128, lists of 16 blocks of 64 (553 GFLOP) take 843 us, 0.66 PFLOP/s, and
+// with every product cut to a single step still about 690 us, with the exponentials left out 820 us (both measured on the
+// kernel at 892 us).  Four threads for a row 942 us; a few exponentials by the polynomial of attn_tc.cuh 880 us.  Five buffers
+// of rows instead of two pairs 905 -> 892 us.  Chunks of 8192 rows for one item: 4096 906 us and 2048 980 us against 909 us,
+// 269, 260 and 286 us with a list for each query.
 constexpr int TK_ROWS = 128, TK_MAX_KEYS = 64, TK_SOFTMAX = 256, TK_THREADS = TK_SOFTMAX + 32 + 128;
 // Tensor memory columns, and blocks of threads per SM: short blocks of small heads leave room for two.
 __host__ __device__ constexpr int tk_cols(int keys) { return keys == 64 ? 512 : keys == 32 ? 256 : 128; }
