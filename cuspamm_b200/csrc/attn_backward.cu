@@ -745,11 +745,11 @@ __global__ __launch_bounds__(TQ_THREADS, 2) void attn_dq_tc_kernel(const __grid_
 // of one accumulator, dK^T in the lower half of the other (the other halves are not used).
 //
 // Bound by the chain of a tile, scores to p and ds to the second products, whose steps the roles hand one another through
-// barriers: 3 sequences of up to 8192, 32 heads of 128, lists of 16 blocks of 64 (553 GFLOP) take 843 us, 0.66 PFLOP/s, and
-// with every product cut to a single step still about 690 us, with the exponentials left out 820 us (both measured on the
-// kernel at 892 us).  Four threads for a row 942 us; a few exponentials by the polynomial of attn_tc.cuh 880 us.  Five buffers
-// of rows instead of two pairs 905 -> 892 us.  Chunks of 8192 rows for one item: 4096 906 us and 2048 980 us against 909 us,
-// 269, 260 and 286 us with a list for each query.
+// barriers: 3 sequences of up to 8192, 32 heads of 128, lists of 16 blocks of 64 (553 GFLOP) take 843 to 891 us from run to
+// run, 0.62 to 0.66 PFLOP/s, and with every product cut to a single step still about 690 us, with the exponentials left out
+// 820 us.  Four threads for a row 942 us; a few exponentials by the polynomial of attn_tc.cuh 880 to 895 us, no gain.  Five
+// buffers of rows instead of two pairs 905 -> 892 us.  Chunks of 8192 rows for one item: 4096 906 us and 2048 980 us against
+// 909 us, 269, 260 and 286 us with a list for each query.
 constexpr int TK_ROWS = 128, TK_MAX_KEYS = 64, TK_SOFTMAX = 256, TK_THREADS = TK_SOFTMAX + 32 + 128;
 // Tensor memory columns, and blocks of threads per SM: short blocks of small heads leave room for two.
 __host__ __device__ constexpr int tk_cols(int keys) { return keys == 64 ? 512 : keys == 32 ? 256 : 128; }
