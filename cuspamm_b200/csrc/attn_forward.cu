@@ -6,6 +6,7 @@
 // maximum and sum (both float); p is rounded to the type of v for the product, as v itself is.
 #include <stdio.h>
 #include <string.h>
+#include <atomic>
 #include <cudaTypedefs.h>
 #include "attn.cuh"
 #include "attn_tc.cuh"
@@ -52,25 +53,31 @@ int attn_check(const spamm_attn *a, bool need_lists)
     return SPAMM_OK;
 }
 
-// The attribute is set once for a kernel, device and host thread as long as the size does not grow (the call costs about as
-// much as a launch).
+// The limit of dynamic shared memory belongs to a kernel and a device, whatever thread sets it: it is raised to all that the
+// device has beside the kernel's fixed part, once in the process, and never lowered, so that no call can undo another's.  (The
+// call costs about as much as a launch.)  Two threads may both raise it: to the same value.
 int attn_set_smem(const void *kernel, size_t bytes)
 {
     if (bytes <= 48 * 1024) return SPAMM_OK;
-    struct Known { const void *kernel; int device; size_t bytes; };
+    struct Raised { std::atomic<const void *> kernel; std::atomic<uint64_t> devices; };
     constexpr int ROOM = 64;
-    static thread_local Known known[ROOM];
-    static thread_local int n_known = 0;
+    static Raised raised[ROOM];
     int device = 0;
     SPAMM_CUDA_TRY(cudaGetDevice(&device));
-    int i = 0;
-    while (i < n_known && (known[i].kernel != kernel || known[i].device != device)) i++;
-    if (i < n_known && known[i].bytes >= bytes) return SPAMM_OK;
-    SPAMM_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
-    if (i < ROOM) {
-        known[i] = Known{kernel, device, bytes};
-        if (i == n_known) n_known++;
+    Raised *mine = nullptr;
+    for (int i = 0; i < ROOM && !mine; i++) {
+        const void *k = raised[i].kernel.load();
+        if (!k && raised[i].kernel.compare_exchange_strong(k, kernel)) k = kernel;     // (on failure k is the other thread's)
+        if (k == kernel) mine = &raised[i];
     }
+    const uint64_t bit = device < 64 ? 1ull << device : 0;
+    if (mine && mine->devices.load() & bit) return SPAMM_OK;
+    cudaFuncAttributes have;
+    int most = 0;
+    SPAMM_CUDA_TRY(cudaFuncGetAttributes(&have, kernel));
+    SPAMM_CUDA_TRY(cudaDeviceGetAttribute(&most, cudaDevAttrMaxSharedMemoryPerBlockOptin, device));
+    SPAMM_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most - (int)have.sharedSizeBytes));
+    if (mine) mine->devices.fetch_or(bit);
     return SPAMM_OK;
 }
 

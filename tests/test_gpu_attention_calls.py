@@ -1,0 +1,75 @@
+"""Calls of the attention operators that the parity tests do not make: several host threads, other streams, sizes at the
+borders of a launch, tensors with gradients, lengths beyond the table, kernels that only large problems reach."""
+import threading
+
+import pytest
+import torch
+
+import _attention_plain as plain
+from test_gpu_attention import BF, DEV, HF, build_cache, cu_of, expect, flat, near, random_lists, tokens
+
+pytestmark = pytest.mark.gpu
+
+
+# ------------------------------------------------------------------------------------------------ shared memory of a launch
+
+def calls_of_two_sizes(g):
+    """For every kernel whose shared memory depends on the call: the same call large and small."""
+    from cuspamm_b200 import PagedCache, block_sparse_attention, select_blocks
+
+    def listed_attend(n_select):
+        k, v, table, lengths = build_cache(g, [3000, 2000], 2, 128, BF, 16)
+        q, lists = tokens(g, 2, 8, 128, BF), random_lists(g, [1, 1], [3000, 2000], 2, 16, 1, n_select, True)
+        cache = PagedCache(k, v)
+        return lambda: (cache.attend(q, cu_of([1, 1]), 1, table, lengths, lists=lists),)
+
+    def select(n, block, query_block, heads, kv_heads):
+        q, k = tokens(g, n, heads, 128, BF), tokens(g, n, kv_heads, 128, BF)
+        return lambda: (select_blocks(q, k, cu_of([n]), n, 9, block=block, query_block=query_block, n_local=0),)
+
+    def train(n, query_block, n_select, G):
+        q, k, v, d_o = (tokens(g, n, h, 128, BF) for h in (2 * G, 2, 2, 2 * G))
+        lists = random_lists(g, [n], [n], 2, 16, query_block, n_select, True)
+        x = [t.requires_grad_() for t in (q, k, v)]
+
+        def call():
+            o = block_sparse_attention(*x, lists, cu_of([n]), n, block=16, query_block=query_block)
+            return (o.detach(), *torch.autograd.grad(o, x, d_o))
+        return call
+
+    return [(listed_attend(150), listed_attend(8)),
+            (select(16300, 16, 16, 2, 2), select(2100, 16, 16, 16, 16)),       # tiles of eight lists
+            (select(4000, 16, 1, 2, 2), select(1600, 16, 1, 4, 4)),            # tiles of 32
+            (select(130000, 16, 100, 1, 1), select(100000, 16, 80, 1, 1)),     # one list at a time
+            (select(130000, 16, 50000, 1, 1), select(100000, 16, 50000, 1, 1)),
+            (train(900, 16, 40, 4), train(200, 64, 4, 4)),
+            (train(20, 16, 200, 1), train(20, 16, 2, 1))]                      # tiles of 16 rows
+
+
+def test_two_host_threads_with_large_and_small_calls():
+    """A kernel's limit of shared memory belongs to the process: one thread's small call must not undo another's large one."""
+    g = torch.Generator().manual_seed(91)
+    pairs = calls_of_two_sizes(g)
+    want = [[call() for call in pair] for pair in pairs]
+    torch.cuda.synchronize(DEV)
+    trouble = []
+
+    def repeat(which, times):
+        try:
+            for _ in range(times):
+                for pair, results in zip(pairs, want):
+                    for x, y in zip(pair[which](), results[which]):
+                        assert torch.equal(x, y)
+        except Exception as e:                                  # noqa: BLE001: handed to the test's own thread
+            trouble.append(e)
+
+    other = threading.Thread(target=repeat, args=(1, 1))        # a new thread sets the small limits; the large calls follow
+    other.start()
+    other.join()
+    repeat(0, 1)
+    both = [threading.Thread(target=repeat, args=(i % 2, 5)) for i in range(4)]
+    for t in both:
+        t.start()
+    for t in both:
+        t.join()
+    assert not trouble, trouble
