@@ -16,7 +16,7 @@ bool attn_rows_ok(const void *p, int64_t token, int64_t head);   // 16-byte alig
 inline int attn_query_blocks(const spamm_attn &a) { return ceil_div(a.max_q, a.query_block); }
 // Blocks of the longest sequence that a call may meet.
 inline int attn_max_blocks(const spamm_attn &a) { return a.n_pages ? a.table_width : ceil_div(a.max_q, a.block); }
-int attn_set_smem(const void *kernel, size_t bytes);
+int attn_set_smem(const void *kernel);
 int attn_refuse(const char *why);     // records the text, gives SPAMM_ERR_INVALID
 int attn_too_large();                 // the same for a grid beyond 2^31 - 1, SPAMM_ERR_UNSUPPORTED
 

@@ -202,7 +202,7 @@ static int append_launch(const spamm_attn &a, void *k_pages, void *v_pages, floa
     const int tokens = min(a.max_q, a.block);
     const size_t turns = ((size_t)tokens * n_freq * sizeof(float2) + 15) / 16 * 16 + (size_t)(ceil_div(tokens, 8) + 7) * n_freq * sizeof(double2);
     const size_t smem = max(turns, (size_t)APPEND_THREADS * 8 * sizeof(double));
-    int st = attn_set_smem((const void *)attn_append_kernel<T, D>, smem);
+    int st = attn_set_smem((const void *)attn_append_kernel<T, D>);
     if (st) return st;
     attn_append_kernel<T, D><<<dim3((unsigned)grid, split), APPEND_THREADS, smem, stream>>>(
         a, (int)per, heads_per_cta, fast_div(heads_per_cta), fast_div(heads_per_cta * (a.heads / a.kv_heads)), static_cast<T *>(k_pages), static_cast<T *>(v_pages), key_sums, inv_freq, n_freq, interleaved != 0);

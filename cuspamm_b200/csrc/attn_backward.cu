@@ -1168,7 +1168,7 @@ static int dkv_launch(const spamm_attn &a, const BackwardPlan &p, const T *d_do,
                       T *dv, cudaStream_t stream)
 {
     const size_t smem = 2 * KEYS * D * 2 + tk_slots(D, KEYS) * TK_ROWS * D * 2 + 2 * TK_ROWS * 128 + sizeof(TkCtrl) + p.chunk * 4;
-    int st = attn_set_smem((const void *)attn_dkv_tc_kernel<T, D, KEYS>, smem);
+    int st = attn_set_smem((const void *)attn_dkv_tc_kernel<T, D, KEYS>);
     if (st) return st;
     RowMap q_map, do_map;
     const int G = a.heads / a.kv_heads;
@@ -1210,13 +1210,13 @@ static int backward_launch(const spamm_attn &a, const BackwardPlan &p, const T *
         attn_row_maps(a, min(a.block, TQ_KEYS), &k_map, &v_map);
         const int entries = (int)min((int64_t)p.nkb, (int64_t)attn_tile_lists(a) * a.n_select);
         const size_t smem = 2 * TQ_ROWS * D * 2 + 3 * TQ_KEYS * D * 2 + sizeof(TqCtrl) + 6 * (size_t)entries;
-        st = attn_set_smem((const void *)attn_dq_tc_kernel<T, D>, smem);
+        st = attn_set_smem((const void *)attn_dq_tc_kernel<T, D>);
         if (st) return st;
         attn_dq_tc_kernel<T, D><<<(unsigned)(p.groups * tq), TQ_THREADS, smem, stream>>>(
             a, tq, attn_tile_shape(a), entries, k_map, v_map, d_do, do_token, do_head, delta, dq);
     } else {
         const size_t smem = (size_t)DQ_WARPS * DQ_STAGES * 2 * 16 * D * 2 + 2 * 16 * D * 2 + a.n_select * 4;
-        st = attn_set_smem((const void *)attn_dq_rows_kernel<T, D>, smem);
+        st = attn_set_smem((const void *)attn_dq_rows_kernel<T, D>);
         if (st) return st;
         attn_dq_rows_kernel<T, D><<<(unsigned)dq_grid, 128, smem, stream>>>(a, p.nqb, tiles, d_do, do_token, do_head, delta, dq);
     }

@@ -53,12 +53,12 @@ int attn_check(const spamm_attn *a, bool need_lists)
     return SPAMM_OK;
 }
 
-// The limit of dynamic shared memory belongs to a kernel and a device, whatever thread sets it: it is raised to all that the
-// device has beside the kernel's fixed part, once in the process, and never lowered, so that no call can undo another's.  (The
-// call costs about as much as a launch.)  Two threads may both raise it: to the same value.
-int attn_set_smem(const void *kernel, size_t bytes)
+// The limit of dynamic shared memory, 48 KB less the kernel's fixed part at first, belongs to a kernel and a device, whatever
+// thread sets it: it is raised to all that the device has beside the fixed part, once in the process, and never lowered, so
+// that no call can undo another's.  (The call costs about as much as a launch.)  Two threads may both raise it: to the same
+// value.
+int attn_set_smem(const void *kernel)
 {
-    if (bytes <= 48 * 1024) return SPAMM_OK;
     struct Raised { std::atomic<const void *> kernel; std::atomic<uint64_t> devices; };
     constexpr int ROOM = 64;
     static Raised raised[ROOM];
@@ -1163,14 +1163,14 @@ static int forward_launch(const spamm_attn &a, float *scratch, cudaStream_t stre
         const int tiles = p.pairs ? 2 : 1;
         const size_t smem = tiles * 3 * TC_ROWS * D * 2 + sizeof(TcCtrl) + (a.n_select ? 6 * (size_t)p.max_entries : 0);
         const auto kernel = p.pairs ? attn_tc_kernel<T, D, 2> : attn_tc_kernel<T, D, 1>;
-        int st = attn_set_smem((const void *)kernel, smem);
+        int st = attn_set_smem((const void *)kernel);
         if (st) return st;
         RowMap k_map, v_map;
         attn_row_maps(a, a.block, &k_map, &v_map);
         kernel<<<(unsigned)grid, tiles * 256 + 64, smem, stream>>>(a, p, k_map, v_map, part_o, part_lse);
     } else {
         const size_t smem = rows_smem(a, p);
-        int st = attn_set_smem((const void *)attn_rows_kernel<T, D>, smem);
+        int st = attn_set_smem((const void *)attn_rows_kernel<T, D>);
         if (st) return st;
         if (p.cluster) {
             cudaLaunchConfig_t how = {};

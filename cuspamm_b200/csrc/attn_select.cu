@@ -758,7 +758,7 @@ static int select_tile_launch(const spamm_attn &a, int nqb, int nkb, int n_first
 {
     const size_t smem = (size_t)(QT + (QT == 8 ? 64 : 32)) * (D + 4) * 8 + (size_t)QT * nkb * 8;
     const int64_t grid = (int64_t)a.batch * a.kv_heads * ((nqb + QT - 1) / QT);
-    int st = attn_set_smem((const void *)attn_select_tile_kernel<D, QT>, smem);
+    int st = attn_set_smem((const void *)attn_select_tile_kernel<D, QT>);
     if (st) return st;
     attn_select_tile_kernel<D, QT><<<(unsigned)grid, 256, smem, stream>>>(a, nqb, nkb, n_first, n_local, key_sums, query_sums, lists);
     return SPAMM_OK;
@@ -815,7 +815,7 @@ static int select_launch(const spamm_attn &a, const float *key_sums, int n_first
         } else if (nkb <= LARGEST_WARP) {
             attn_largest_warp_kernel<LARGEST_WARP / 32><<<(unsigned)grid, 32, 0, stream>>>(a, nqb, nkb, keys, lists);
         } else {
-            st = attn_set_smem((const void *)attn_largest_kernel<256>, (size_t)nkb * 8);
+            st = attn_set_smem((const void *)attn_largest_kernel<256>);
             if (st) return st;
             attn_largest_kernel<256><<<(unsigned)grid, 256, (size_t)nkb * 8, stream>>>(a, nqb, nkb, keys, lists);
         }
@@ -824,7 +824,7 @@ static int select_launch(const spamm_attn &a, const float *key_sums, int n_first
     case SELECT_TILE32: st = select_tile_launch<D, 32>(a, nqb, nkb, n_first, n_local, key_sums, query_sums, lists, stream); break;
     case SELECT_TILE8: st = select_tile_launch<D, 8>(a, nqb, nkb, n_first, n_local, key_sums, query_sums, lists, stream); break;
     case SELECT_ONE:
-        st = attn_set_smem((const void *)attn_select_kernel<T, D>, (size_t)nkb * 8);
+        st = attn_set_smem((const void *)attn_select_kernel<T, D>);
         if (st) return st;
         attn_select_kernel<T, D><<<(unsigned)grid, 128, (size_t)nkb * 8, stream>>>(a, nqb, n_first, n_local, key_sums, query_sums, lists);
         break;

@@ -73,3 +73,31 @@ def test_two_host_threads_with_large_and_small_calls():
     for t in both:
         t.join()
     assert not trouble, trouble
+
+# D = 64: what the lists need beside the kernel's fixed shared memory comes to 48 KB and a little less
+BORDERS = [(b, 64, 64, 8, 8) for b in (153, 154, 156, 157)] + [(b, 64, 1, 2, 2) for b in (54, 55, 56, 57)] + \
+    [(b, 16, 64, 1, 1) for b in (6060, 6100, 6144, 6145)] + [(b, 16, 24576, 1, 1) for b in (6060, 6140, 6144, 6145)]
+
+
+@pytest.mark.parametrize("blocks,block,query_block,heads,kv_heads", BORDERS)
+def test_select_where_shared_memory_passes_48_kb(blocks, block, query_block, heads, kv_heads):
+    from cuspamm_b200 import select_blocks
+
+    n, D, n_select = blocks * block - 3, 64, 9
+    g = torch.Generator().manual_seed(blocks)
+    q, k = tokens(g, n, heads, D, BF), tokens(g, n, kv_heads, D, BF)
+    got = select_blocks(q, k, cu_of([n]), n, n_select, block=block, query_block=query_block, n_first=1, n_local=0)
+    sums = torch.zeros(blocks, kv_heads, D, dtype=torch.float64, device=DEV).index_add_(0, torch.arange(n, device=DEV) // block, k.double())
+    held = torch.full((blocks,), float(block), dtype=torch.float64, device=DEV)
+    held[-1] = block - 3
+    nqb = -(-n // query_block)
+    qs = torch.zeros(nqb, kv_heads, D, dtype=torch.float64, device=DEV).index_add_(0, torch.arange(n, device=DEV) // query_block, q.double())
+    last = torch.clamp((torch.arange(nqb, device=DEV) + 1) * query_block, max=n) - 1
+    seen = torch.arange(blocks, device=DEV)[None] * block <= last[:, None]
+    for h in range(kv_heads):
+        score = (qs[:, h] @ sums[:, h].float().double().T) / held
+        score[:, 0] = torch.inf
+        best = torch.where(seen, score, -torch.inf).topk(n_select, 1)
+        want = torch.where(best.values > -torch.inf, best.indices, blocks).sort(1).values
+        want = torch.where(want < blocks, want, -1)
+        assert torch.equal(got[0, :, h].long(), want)
