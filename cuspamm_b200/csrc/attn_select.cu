@@ -458,7 +458,7 @@ __global__ __launch_bounds__(256) void attn_select_tile_kernel(const __grid_cons
     __shared__ Reach reach[QT];
     __shared__ bool there[KT];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int q_tiles = (nqb + QT - 1) / QT;
+    const int q_tiles = ceil_div(nqb, QT);
     unsigned idx = blockIdx.x;
     const int qt = q_tiles - 1 - idx % q_tiles; idx /= q_tiles;
     const int h = idx % a.kv_heads, s = idx / a.kv_heads;
@@ -572,7 +572,7 @@ __global__ __launch_bounds__(SPREAD_WARPS * 32, 6) void attn_spread_scores_kerne
     constexpr int N = D / 16;            // groups of four values of a lane
     __shared__ __align__(16) double qs[8][D];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, row = lane >> 2, kk = lane & 3;
-    const int groups = (nqb + 7) / 8;
+    const int groups = ceil_div(nqb, 8);
     unsigned idx = blockIdx.x;
     const int span = idx % spans; idx /= spans;
     const int qg = idx % groups; idx /= groups;
@@ -757,7 +757,7 @@ static int select_tile_launch(const spamm_attn &a, int nqb, int nkb, int n_first
                               const double *query_sums, int32_t *lists, cudaStream_t stream)
 {
     const size_t smem = (size_t)(QT + (QT == 8 ? 64 : 32)) * (D + 4) * 8 + (size_t)QT * nkb * 8;
-    const int64_t grid = (int64_t)a.batch * a.kv_heads * ((nqb + QT - 1) / QT);
+    const int64_t grid = (int64_t)a.batch * a.kv_heads * ceil_div(nqb, QT);
     int st = attn_set_smem((const void *)attn_select_tile_kernel<D, QT>);
     if (st) return st;
     attn_select_tile_kernel<D, QT><<<(unsigned)grid, 256, smem, stream>>>(a, nqb, nkb, n_first, n_local, key_sums, query_sums, lists);
@@ -806,7 +806,7 @@ static int select_launch(const spamm_attn &a, const float *key_sums, int n_first
         if (!nkb) return clear_lists(a, lists, stream);
         unsigned long long *keys = reinterpret_cast<unsigned long long *>(query_sums + grid * D);
         const int spans = ceil_div(nkb, SPREAD_BLOCKS * SPREAD_WARPS);
-        const int64_t blocks = (int64_t)a.batch * a.kv_heads * ((nqb + 7) / 8) * spans;
+        const int64_t blocks = (int64_t)a.batch * a.kv_heads * ceil_div(nqb, 8) * spans;
         if (blocks > INT32_MAX) return attn_too_large();
         attn_spread_scores_kernel<T, D><<<(unsigned)blocks, SPREAD_WARPS * 32, 0, stream>>>(a, nqb, spans, nkb, n_first, n_local, key_sums,
                                                                               rows > SPREAD_ROWS ? query_sums : nullptr, keys);

@@ -26,7 +26,8 @@ __host__ __device__ inline uint32_t step_cols(uint32_t s) { return (s >> 20) & 0
 __host__ __device__ inline int step_count_of(int32_t v) { return v & SPAMM_STEPS_MASK; }
 __host__ __device__ inline bool step_list_dense(int32_t v) { return (v & SPAMM_STEPS_DENSE) != 0; }
 
-__host__ __device__ inline int ceil_div(int a, int b) { return (a + b - 1) / b; }
+// b > 0.  (Not (a + b - 1) / b: the sum may pass 2^31.)
+__host__ __device__ inline int ceil_div(int a, int b) { return a / b + (a % b > 0); }
 
 // Records a CUDA error for spamm_last_cuda_error and maps it to a status.
 int record_cuda_error(cudaError_t e, const char *what);

@@ -101,3 +101,33 @@ def test_select_where_shared_memory_passes_48_kb(blocks, block, query_block, hea
         want = torch.where(best.values > -torch.inf, best.indices, blocks).sort(1).values
         want = torch.where(want < blocks, want, -1)
         assert torch.equal(got[0, :, h].long(), want)
+
+
+# ------------------------------------------------------------------------------------------------ the largest numbers
+
+@pytest.mark.parametrize("lens", [[2, 2, 1], [30, 20], [300, 200, 1]])
+def test_one_list_for_the_whole_sequence(lens):
+    """query_block of 2^31 - 1 is the same as one of the longest sequence, for every sequence and in both passes."""
+    from cuspamm_b200 import PagedCache, block_sparse_attention, select_blocks
+
+    g = torch.Generator().manual_seed(sum(lens))
+    T, n, cu = sum(lens), max(lens), cu_of(lens)
+    q, k, v, d_o = (tokens(g, T, h, 64, BF) for h in (4, 2, 2, 4))
+    held = [x + 90 for x in lens]
+    pages = build_cache(g, held, 2, 64, BF, 16)
+    cache = PagedCache(*pages[:2])
+    cache.key_sums.copy_(torch.randn(cache.key_sums.shape, generator=g))
+    got = []
+    for query_block in (n, 2 ** 31 - 1):
+        lists = select_blocks(q, k, cu, n, 3, block=16, query_block=query_block, n_local=0)
+        assert lists.shape == (len(lens), 1, 2, 3)
+        x = [t.detach().requires_grad_() for t in (q, k, v)]
+        o = block_sparse_attention(*x, lists, cu, n, block=16, query_block=query_block)
+        of_pages = cache.select(q, cu, n, *pages[2:], 3, query_block=query_block, n_local=0)
+        got.append((lists, o.detach(), *torch.autograd.grad(o, x, d_o), of_pages,
+                    cache.attend(q, cu, n, *pages[2:], lists=of_pages, query_block=query_block)))
+    for a, b in zip(*got):
+        assert torch.equal(a, b)
+    val, tol = expect(q, k, v, got[0][0], lens, 16, n, True, 64 ** -0.5, d_o)
+    for name, x in zip(("o", "dq", "dk", "dv"), got[1][1:5]):
+        near(x, val[name], tol[name], name)
