@@ -28,6 +28,12 @@ struct Item {
     int kb, chunk, slot, pad;   // block of keys, which chunk of its query blocks, partial sum to write (-1: the rows)
 };
 
+// A plan counts the rows of a query block in 32 bits.
+static bool backward_fits(const spamm_attn &a)
+{
+    return (int64_t)min(a.query_block, a.max_q) * (a.heads / a.kv_heads) <= (1 << 28);
+}
+
 static BackwardPlan backward_plan(const spamm_attn &a)
 {
     BackwardPlan p;
@@ -1194,7 +1200,7 @@ static int backward_launch(const spamm_attn &a, const BackwardPlan &p, const T *
     const int tiles = (int)(((int64_t)bq * (a.heads / a.kv_heads) + 15) / 16);
     const int64_t dq_grid = p.groups * p.nqb * tiles;
     if ((rows + 31) / 32 > INT32_MAX || (lists + 3) / 4 > INT32_MAX || dq_grid > INT32_MAX || p.groups * p.item_cap > INT32_MAX / 2 ||
-        p.groups * p.nkb > INT32_MAX || (int64_t)bq * (a.heads / a.kv_heads) > (1 << 28))
+        p.groups * p.nkb > INT32_MAX)
         return attn_too_large();
 
     attn_delta_kernel<T, D><<<(unsigned)((rows + 31) / 32), 256, 0, stream>>>(a, d_do, do_token, do_head, delta, dq, dk, dv,
@@ -1239,7 +1245,7 @@ using namespace spamm;
 
 extern "C" size_t spamm_attn_backward_scratch_bytes(const spamm_attn *a)
 {
-    if (attn_check(a, false) || !a->batch || !a->max_q || !a->tokens) return 0;
+    if (attn_check(a, false) || !a->batch || !a->max_q || !a->tokens || !backward_fits(*a)) return 0;
     return backward_plan(*a).bytes;
 }
 
@@ -1265,6 +1271,7 @@ extern "C" int spamm_attn_backward_dev(const spamm_attn *a, const void *d_do, in
         return SPAMM_OK;
     }
     if (reinterpret_cast<uintptr_t>(a->d_o_low) & 15) return attn_refuse("d_o_low is not on a 16-byte boundary");
+    if (!backward_fits(*a)) return attn_too_large();
     const BackwardPlan p = backward_plan(*a);
     if (!d_scratch || scratch_bytes < p.bytes || (reinterpret_cast<uintptr_t>(d_scratch) & 15))
         return attn_refuse("scratch too small or not on a 16-byte boundary");

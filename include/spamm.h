@@ -568,7 +568,8 @@ int spamm_attn_forward_dev(const spamm_attn *a, void *d_scratch, size_t scratch_
 /*
  * Gradients for the output gradient d_do ([tokens][heads][dim], strides given): d_dq [tokens][heads][dim], d_dk and
  * d_dv [tokens][kv_heads][dim], without gaps.  `a` holds q, k, v, o, lse and the lists as the forward had them.  Sums
- * run in a fixed order: the same inputs give the same bits.
+ * run in a fixed order: the same inputs give the same bits.  A query block may have up to 2^28 rows (queries times heads of a
+ * key head).
  */
 size_t spamm_attn_backward_scratch_bytes(const spamm_attn *a);
 int spamm_attn_backward_dev(const spamm_attn *a, const void *d_do, int64_t do_token, int64_t do_head,

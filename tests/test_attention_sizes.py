@@ -40,3 +40,13 @@ def test_select_refuses_more_blocks_than_it_ranks_at_the_largest_bound(lib, max_
     r = C.byref(problem(max_q=max_q, query_block=2 ** 31 - 1))
     assert lib.spamm_attn_select_dev(r, None, 1, 0, P, P, 1 << 40, None) == 6
     assert b"16384" in lib.spamm_last_cuda_error()
+
+
+@pytest.mark.parametrize("max_q,heads,kv_heads", [(1 << 26, 64, 1), (2 ** 31 - 1, 2, 1), (2 ** 31 - 1, 128, 1), (1 << 28, 16, 8)])
+def test_backward_refuses_query_blocks_of_too_many_rows(lib, max_q, heads, kv_heads):
+    """Query blocks of 2^28 rows and more (queries times heads of a key head), up to counts that pass 32 bits."""
+    a = problem(max_q=max_q, query_block=2 ** 31 - 1, heads=heads, kv_heads=kv_heads, batch=1)
+    r = C.byref(a)
+    assert lib.spamm_attn_backward_scratch_bytes(r) == 0
+    assert lib.spamm_attn_backward_dev(r, P, heads * 128, 128, P, P, P, P, 1 << 60, None) == 6
+    assert lib.spamm_last_cuda_error().startswith(b"spamm_attn")
