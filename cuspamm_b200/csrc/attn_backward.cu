@@ -8,6 +8,13 @@
 // sums over its queries in ascending order and writes its rows once.  No atomics on gradients: the same inputs give the
 // same bits.  A block that very many queries list (the first one often is on every list) is cut into items of `chunk`
 // query blocks each, whose float partial sums a last kernel adds up in order.
+//
+// p and ds are rounded to the type for their products.  bf16 has float's range; half loses digits below 2^-14, where ds lies
+// for output gradients of 1e-3 already (4096 keys of like weight and output gradients of 1e-4: every digit), so half's
+// operands are multiplied by powers of two on the way, which the float results are divided by: p by 2^15 (p <= 1), ds without
+// its scale by the 2^n that brings its bound, twice the longest do times the longest v (o_i is a mean of rows of v), near half's
+// largest numbers.
+#include <type_traits>
 #include "attn_tc.cuh"
 
 namespace spamm {
@@ -21,7 +28,8 @@ struct BackwardPlan {
     int64_t groups;             // batch * kv_heads
     FastDiv per, G;             // rows of a full query block, heads of a key head
     int box_tokens;             // queries of a tensor copy of q and do (0: rows are copied one by one)
-    size_t delta, bits, counts, slots, items, n_items, partial, bytes;   // scratch offsets
+    int64_t n_norms;            // blocks of threads of attn_delta_kernel
+    size_t delta, bits, counts, slots, items, n_items, partial, norms, factor, bytes;   // scratch offsets (the last two: half)
 };
 
 struct Item {
@@ -62,70 +70,126 @@ static BackwardPlan backward_plan(const spamm_attn &a)
     p.items = take((size_t)p.groups * p.item_cap * sizeof(Item));
     p.n_items = take((size_t)p.groups * 4);
     p.partial = take((size_t)p.groups * p.slot_cap * a.block * a.dim * 2 * 4);
+    const bool half = a.dtype == SPAMM_ATTN_HALF;
+    p.n_norms = ((int64_t)a.tokens * a.heads + 31) / 32;
+    p.norms = take(half ? (size_t)p.n_norms * sizeof(float2) : 0);
+    p.factor = take(half ? 4 : 0);
     p.bytes = at;
     return p;
 }
 
 // delta = do.o for every row; a quarter of a warp for each.  Rows of no sequence get zero gradients here, and the bits and
-// counts of the lists that are turned over next are cleared (`clear`, one launch less).  Bound by the reading of do, o and the
-// low part of o: 18000 tokens of 32 heads of 128 (440 MB) take 66 us, 6.7 TB/s.
+// counts of the lists that are turned over next are cleared (`clear`, one launch less).  For half every block of threads leaves
+// the largest squared norms of its rows of do and of v.  (Rows with infinities and NaN do not count: what meets them is not
+// finite in any case.)  Bound by the reading of do, o and the low part of o: 18000 tokens of 32 heads of 128 (440 MB) take
+// 66 us, 6.7 TB/s.
 template <typename T, int D>
-__global__ __launch_bounds__(256) void attn_delta_kernel(const __grid_constant__ spamm_attn a, const T *d_do, int64_t do_token,
-                                                         int64_t do_head, float *delta, T *dq, T *dk, T *dv, uint4 *clear,
-                                                         size_t n_clear)
+__global__ __launch_bounds__(256) void attn_delta_kernel(const __grid_constant__ spamm_attn a, FastDiv div_heads, FastDiv div_g, const T *d_do,
+                                                         int64_t do_token, int64_t do_head, float *delta, T *dq, T *dk, T *dv,
+                                                         uint4 *clear, size_t n_clear, float2 *norms)
 {
+    constexpr bool HALF = std::is_same<T, __half>::value;
     for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < n_clear; i += (size_t)gridDim.x * 256) clear[i] = make_uint4(0, 0, 0, 0);
     const int sub = threadIdx.x & 7;
     const int64_t w = (int64_t)blockIdx.x * 32 + (threadIdx.x >> 3);
-    if (w >= (int64_t)a.tokens * a.heads) return;
-    const int row = (int)(w / a.heads), head = (int)(w % a.heads);
-    // the sequence that holds the row
-    int lo = 0, hi = a.batch;
-    while (lo < hi) {
-        const int mid = (lo + hi) >> 1;
-        if (a.d_cu[mid + 1] > row) hi = mid; else lo = mid + 1;
+    const bool there = w < (int64_t)a.tokens * a.heads;
+    const int row = w <= INT32_MAX ? (int)div_heads.quotient((uint32_t)w) : (int)(w / a.heads), head = (int)(w - (int64_t)row * a.heads);
+    const int h = (int)div_g.quotient(head);
+    const bool first = head == h * (int)div_g.d;      // of the heads of its key head
+    bool held = false;
+    if (there) {
+        // the sequence that holds the row
+        int lo = 0, hi = a.batch;
+        while (lo < hi) {
+            const int mid = (lo + hi) >> 1;
+            if (a.d_cu[mid + 1] > row) hi = mid; else lo = mid + 1;
+        }
+        if (lo < a.batch) {
+            const Seq sq = attn_seq(a, lo);
+            held = row >= sq.row0 && row < sq.row0 + sq.nq;
+        }
     }
-    bool held = lo < a.batch;
-    if (held) {
-        const Seq sq = attn_seq(a, lo);
-        held = row >= sq.row0 && row < sq.row0 + sq.nq;
-    }
-    if (!held) {
+    if (there && !held) {
         const uint4 z = make_uint4(0, 0, 0, 0);
-        const int G = a.heads / a.kv_heads;
         for (int c = sub; c < D / 8; c += 8) {
             reinterpret_cast<uint4 *>(dq + ((int64_t)row * a.heads + head) * D)[c] = z;
-            if (head % G == 0) {
-                reinterpret_cast<uint4 *>(dk + ((int64_t)row * a.kv_heads + head / G) * D)[c] = z;
-                reinterpret_cast<uint4 *>(dv + ((int64_t)row * a.kv_heads + head / G) * D)[c] = z;
+            if (first) {
+                reinterpret_cast<uint4 *>(dk + ((int64_t)row * a.kv_heads + h) * D)[c] = z;
+                reinterpret_cast<uint4 *>(dv + ((int64_t)row * a.kv_heads + h) * D)[c] = z;
             }
         }
-        return;
     }
-    float sum = 0.f;
+    float sum = 0.f, norm_do = 0.f, norm_v = 0.f;
+    if (held) {
 #pragma unroll
-    for (int c = 0; c < D / 64; c++) {
-        const int d = (c * 8 + sub) * 8;
-        const uint4 x = *reinterpret_cast<const uint4 *>(d_do + row * do_token + head * do_head + d);
-        const uint4 y = *reinterpret_cast<const uint4 *>(static_cast<const T *>(a.d_o) + row * a.o_token + head * a.o_head + d);
-        uint4 z = make_uint4(0, 0, 0, 0);
-        if (a.d_o_low) z = *reinterpret_cast<const uint4 *>(static_cast<const T *>(a.d_o_low) + w * D + d);
-        const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+        for (int c = 0; c < D / 64; c++) {
+            const int d = (c * 8 + sub) * 8;
+            const uint4 x = *reinterpret_cast<const uint4 *>(d_do + row * do_token + head * do_head + d);
+            const uint4 y = *reinterpret_cast<const uint4 *>(static_cast<const T *>(a.d_o) + row * a.o_token + head * a.o_head + d);
+            uint4 z = make_uint4(0, 0, 0, 0), k = z;
+            if (a.d_o_low) z = *reinterpret_cast<const uint4 *>(static_cast<const T *>(a.d_o_low) + w * D + d);
+            if (HALF && first) k = *reinterpret_cast<const uint4 *>(static_cast<const T *>(a.d_v) + row * a.v_token + h * a.v_head + d);
+            const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w}, ks[4] = {k.x, k.y, k.z, k.w};
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const float2 u = Pack<T>::to2(xs[i]);
-            float2 v = Pack<T>::to2(ys[i]);
-            if (a.d_o_low) {
-                const float2 w = Pack<T>::to2(reinterpret_cast<const uint32_t *>(&z)[i]);
-                v.x += w.x;
-                v.y += w.y;
+            for (int i = 0; i < 4; i++) {
+                const float2 u = Pack<T>::to2(xs[i]);
+                float2 v = Pack<T>::to2(ys[i]);
+                if (a.d_o_low) {
+                    const float2 w = Pack<T>::to2(reinterpret_cast<const uint32_t *>(&z)[i]);
+                    v.x += w.x;
+                    v.y += w.y;
+                }
+                sum = fmaf(u.x, v.x, fmaf(u.y, v.y, sum));
+                if constexpr (HALF) {
+                    norm_do = fmaf(u.x, u.x, fmaf(u.y, u.y, norm_do));
+                    if (first) {
+                        const float2 t = Pack<T>::to2(ks[i]);
+                        norm_v = fmaf(t.x, t.x, fmaf(t.y, t.y, norm_v));
+                    }
+                }
             }
-            sum = fmaf(u.x, v.x, fmaf(u.y, v.y, sum));
         }
     }
 #pragma unroll
     for (int d = 1; d < 8; d <<= 1) sum += __shfl_xor_sync(~0u, sum, d, 8);
-    if (sub == 0) delta[w] = sum;
+    if (held && sub == 0) delta[w] = sum;
+    if constexpr (HALF) {
+        __shared__ uint2 met[8];
+#pragma unroll
+        for (int d = 1; d < 8; d <<= 1) {
+            norm_do += __shfl_xor_sync(~0u, norm_do, d, 8);
+            norm_v += __shfl_xor_sync(~0u, norm_v, d, 8);
+        }
+        // floats from zero on are in the order of their bits
+        const uint32_t x = __reduce_max_sync(~0u, isfinite(norm_do) ? __float_as_uint(norm_do) : 0u);
+        const uint32_t y = __reduce_max_sync(~0u, isfinite(norm_v) ? __float_as_uint(norm_v) : 0u);
+        if ((threadIdx.x & 31) == 0) met[threadIdx.x >> 5] = make_uint2(x, y);
+        __syncthreads();
+        if (threadIdx.x < 8) {
+            const uint2 m = met[threadIdx.x];
+            const uint32_t most_do = __reduce_max_sync(0xffu, m.x), most_v = __reduce_max_sync(0xffu, m.y);
+            if (threadIdx.x == 0) norms[blockIdx.x] = make_float2(__uint_as_float(most_do), __uint_as_float(most_v));
+        }
+    }
+}
+
+// What half's ds is multiplied by: the power of two that brings its bound, 2 |do| |v|, to 2^14 .. 2^15, from the largest squared
+// norms.
+static __device__ float ds_factor(float norm_do, float norm_v)
+{
+    const float bound = 2.f * sqrtf(norm_do) * sqrtf(norm_v);
+    int e = 15;
+    if (bound > 0.f) frexpf(bound, &e);               // bound < 2^e
+    return ldexpf(1.f, 15 - e);
+}
+constexpr float P_UP = 15.f;                          // log2 of what half's p is multiplied by
+
+// How ds enters its products and what their results are multiplied by.
+struct DsScale { float in, out; };
+template <typename T> static __device__ __forceinline__ DsScale ds_scale(const spamm_attn &a, const float *factor)
+{
+    if constexpr (std::is_same<T, __half>::value) return {*factor, a.scale / *factor};
+    else return {a.scale, 1.f};
 }
 
 // Turns the lists over: one warp reads a list and sets the bit of its query block in every listed block of keys.  (The bits and
@@ -152,9 +216,10 @@ __global__ __launch_bounds__(128) void attn_turn_kernel(const __grid_constant__ 
 }
 
 // The work items of one (sequence, key head), in the order of the blocks: a running sum over the blocks of how many
-// items and partial sums each needs.
+// items and partial sums each needs.  The first block of threads also takes the factor of half's ds from `norms`.
 __global__ __launch_bounds__(1024) void attn_items_kernel(const __grid_constant__ spamm_attn a, const BackwardPlan p,
-                                                          const int *counts, int *slots, Item *items, int *n_items)
+                                                          const int *counts, int *slots, Item *items, int *n_items,
+                                                          const float2 *norms, float *factor)
 {
     __shared__ int2 warp_sum[32];
     __shared__ int2 carry;
@@ -162,6 +227,18 @@ __global__ __launch_bounds__(1024) void attn_items_kernel(const __grid_constant_
     const int64_t group = blockIdx.x;
     const int s = (int)(group / a.kv_heads);
     const int n_blocks = ceil_div(attn_seq(a, s).nk, a.block);
+    if (norms && blockIdx.x == 0) {
+        float2 most = make_float2(0.f, 0.f);
+        for (int64_t i = tid; i < p.n_norms; i += 1024) most = make_float2(fmaxf(most.x, norms[i].x), fmaxf(most.y, norms[i].y));
+        const uint32_t x = __reduce_max_sync(~0u, __float_as_uint(most.x)), y = __reduce_max_sync(~0u, __float_as_uint(most.y));
+        if (lane == 0) warp_sum[warp] = make_int2((int)x, (int)y);
+        __syncthreads();
+        if (warp == 0) {
+            const int2 m = warp_sum[lane];
+            const uint32_t most_do = __reduce_max_sync(~0u, (uint32_t)m.x), most_v = __reduce_max_sync(~0u, (uint32_t)m.y);
+            if (lane == 0) *factor = ds_factor(__uint_as_float(most_do), __uint_as_float(most_v));
+        }
+    }
     if (tid == 0) carry = make_int2(0, 0);
     __syncthreads();
     for (int b0 = 0; b0 < n_blocks; b0 += 1024) {
@@ -227,7 +304,8 @@ constexpr int DQ_WARPS = 4;
 // lists of up to 16 blocks of 64: 13 us (26 us in tiles of 128 rows).
 template <typename T, int D>
 __global__ __launch_bounds__(128) void attn_dq_rows_kernel(const __grid_constant__ spamm_attn a, int nqb, int tiles, const T *d_do,
-                                                           int64_t do_token, int64_t do_head, const float *delta, T *dq)
+                                                           int64_t do_token, int64_t do_head, const float *delta, const float *factor,
+                                                           T *dq)
 {
     extern __shared__ __align__(128) uint8_t smem[];
     constexpr int TILE16 = 16 * D * 2;
@@ -312,6 +390,7 @@ __global__ __launch_bounds__(128) void attn_dq_rows_kernel(const __grid_constant
         dl[x] = delta[at];
     }
     const float scale2 = a.scale * LOG2E;
+    const DsScale dss = ds_scale<T>(a, factor);
     float o[D / 8][4] = {};
     int stage = 0;
     for (int c = warp; c < n_chunks; c += DQ_WARPS) {
@@ -339,7 +418,7 @@ __global__ __launch_bounds__(128) void attn_dq_rows_kernel(const __grid_constant
             for (int i = 0; i < 4; i++) {
                 const int x = i >> 1;
                 float pr = fast_exp2(sc[nt][i] * scale2 - lse2[x]);
-                float ds = pr * (dp[nt][i] - dl[x]) * a.scale;
+                float ds = pr * (dp[nt][i] - dl[x]) * dss.in;
                 if (masked && p0 + nt * 8 + (lane & 3) * 2 + (i & 1) >= limit[x]) ds = 0.f;
                 sc[nt][i] = ds;
             }
@@ -374,6 +453,8 @@ __global__ __launch_bounds__(128) void attn_dq_rows_kernel(const __grid_constant
         for (int w = 0; w < DQ_WARPS; w++)
 #pragma unroll
             for (int i = 0; i < D / 8; i++) y[i] += so[(w * 16 + r) * D + c0 + i];
+#pragma unroll
+        for (int i = 0; i < D / 8; i++) y[i] *= dss.out;
 #pragma unroll
         for (int i = 0; i < D / 8; i++) odd |= not_finite(__float_as_uint(y[i]));
         uint32_t out[D / 16];
@@ -461,7 +542,8 @@ __global__ __launch_bounds__(TQ_THREADS, 2) void attn_dq_tc_kernel(const __grid_
                                                                    const TileShape shape, int max_entries,
                                                                    const __grid_constant__ RowMap k_map,
                                                                    const __grid_constant__ RowMap v_map, const T *d_do,
-                                                                   int64_t do_token, int64_t do_head, const float *delta, T *dq)
+                                                                   int64_t do_token, int64_t do_head, const float *delta,
+                                                                   const float *factor, T *dq)
 {
     extern __shared__ __align__(1024) uint8_t smem_tc[];
     uint8_t *const smem = smem_tc;
@@ -621,7 +703,8 @@ __global__ __launch_bounds__(TQ_THREADS, 2) void attn_dq_tc_kernel(const __grid_
         const int64_t at = (int64_t)(sq.row0 + my_query) * a.heads + h * G + y - my_query * G;
         const float z = a.d_lse[at];
         const float minus_lse = z == -CUDART_INF_F ? -CUDART_INF_F : -z * LOG2E;       // a row without keys: every p zero
-        const float minus_delta = -delta[at] * a.scale;
+        const DsScale dss = ds_scale<T>(a, factor);
+        const float minus_delta = -delta[at] * dss.in;
         cp_wait<0>();
         fence_async_smem();
         mbar_arrive(smem_u32(&ctrl->q_full));
@@ -629,7 +712,7 @@ __global__ __launch_bounds__(TQ_THREADS, 2) void attn_dq_tc_kernel(const __grid_
         const uint32_t lane_dq = tmem_dq + ((uint32_t)((warp & 3) * 32) << 16) + half * (D / 2);
         const float scale2 = a.scale * LOG2E;
         const float2 sc2 = make_float2(scale2, scale2), ml2 = make_float2(minus_lse, minus_lse);
-        const float2 sc = make_float2(a.scale, a.scale), md = make_float2(minus_delta, minus_delta);
+        const float2 sc = make_float2(dss.in, dss.in), md = make_float2(minus_delta, minus_delta);
         bool fine = true;
         for (int j = 0; j < n_tiles; j++) {
             // lanes 0 and 1: position and lists of this half's groups of 16 keys
@@ -689,7 +772,7 @@ __global__ __launch_bounds__(TQ_THREADS, 2) void attn_dq_tc_kernel(const __grid_
                 tmem_landed<32>(v);
             }
 #pragma unroll
-            for (int i = 0; i < 32; i++) v[i] = !fine ? 0x7fc00000u : n_tiles ? v[i] : 0u;
+            for (int i = 0; i < 32; i++) v[i] = !fine ? 0x7fc00000u : n_tiles ? __float_as_uint(__uint_as_float(v[i]) * dss.out) : 0u;
 #pragma unroll
             for (int i = 0; i < 32; i++) odd |= not_finite(v[i]);
 #pragma unroll
@@ -778,8 +861,8 @@ __global__ __launch_bounds__(TK_THREADS, tk_per_sm(D, TK_KEYS)) void attn_dkv_tc
                                                                     const __grid_constant__ RowMap q_map,
                                                                     const __grid_constant__ RowMap do_map,
                                                                     const T *d_do, int64_t do_token, int64_t do_head,
-                                                                    const float *delta, const unsigned *bits, const Item *items,
-                                                                    const int *n_items, float *partial, T *dk, T *dv)
+                                                                    const float *delta, const float *factor, const unsigned *bits,
+                                                                    const Item *items, const int *n_items, float *partial, T *dk, T *dv)
 {
     extern __shared__ __align__(1024) uint8_t smem_tc[];
     uint8_t *const smem = smem_tc;
@@ -1023,7 +1106,11 @@ __global__ __launch_bounds__(TK_THREADS, tk_per_sm(D, TK_KEYS)) void attn_dkv_tc
         const int r = tid & 127, part = warp >> 2;
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         const float scale2 = a.scale * LOG2E;
-        const float2 sc2 = make_float2(scale2, scale2), sc = make_float2(a.scale, a.scale);
+        // half: p times 2^P_UP, and ds = p (dP - delta) with it times the factor
+        constexpr bool IS_HALF = std::is_same<T, __half>::value;
+        const DsScale dss = ds_scale<T>(a, factor);
+        const float p_up = IS_HALF ? P_UP : 0.f, p_down = IS_HALF ? 0x1p-15f : 1.f, ds_in = dss.in * p_down;
+        const float2 sc2 = make_float2(scale2, scale2), sc = make_float2(ds_in, ds_in);
         // lse and delta of the row in tile j as they are, and how many of this thread's keys it sees: requested a tile ahead,
         // and not touched before they are needed
         auto row_of = [&](int j, float *lse, float *dl, int *n_visible) {
@@ -1043,7 +1130,7 @@ __global__ __launch_bounds__(TK_THREADS, tk_per_sm(D, TK_KEYS)) void attn_dkv_tc
         row_of(0, &lse, &dl, &n_visible);
         bool fine = true;
         for (int j = 0; j < n_tiles; j++) {
-            const float minus_lse = lse == -CUDART_INF_F ? lse : -lse * LOG2E, minus_delta = -dl * a.scale;
+            const float minus_lse = lse == -CUDART_INF_F ? lse : IS_HALF ? fmaf(-lse, LOG2E, p_up) : -lse * LOG2E, minus_delta = -dl * ds_in;
             int next_visible;
             row_of(j + 1, &lse, &dl, &next_visible);
             fine = __all_sync(~0u, ws.wait(smem_u32(&ctrl->s_full[j & 1]), j >> 1, 6));
@@ -1100,6 +1187,7 @@ __global__ __launch_bounds__(TK_THREADS, tk_per_sm(D, TK_KEYS)) void attn_dkv_tc
         tc_fence_after();
         // rows of the accumulators are the D values, columns the keys: four warps write dv, four dk
         const bool is_k = part != 0;
+        const float out = is_k ? dss.out : p_down;
         const int row = r, d0 = D == 64 && is_k ? row - 64 : row;
         const bool mine = D == 128 || (is_k ? row >= 64 : row < 64);            // whole warps
         constexpr int COLS = TK_KEYS < 32 ? TK_KEYS : 32;
@@ -1112,7 +1200,7 @@ __global__ __launch_bounds__(TK_THREADS, tk_per_sm(D, TK_KEYS)) void attn_dkv_tc
                 tmem_landed<COLS>(v);
             }
 #pragma unroll
-            for (int i = 0; i < COLS; i++) v[i] = !fine ? 0x7fc00000u : n_tiles ? v[i] : 0u;
+            for (int i = 0; i < COLS; i++) v[i] = !fine ? 0x7fc00000u : n_tiles ? __float_as_uint(__uint_as_float(v[i]) * out) : 0u;
             if (!mine) continue;
             if (item.slot >= 0) {
                 float *dst = partial + (group * p.slot_cap + item.slot) * (int64_t)(2 * a.block * D) + (is_k ? 0 : a.block * D) +
@@ -1170,8 +1258,8 @@ __global__ __launch_bounds__(128) void attn_dkv_join_kernel(const __grid_constan
 
 template <typename T, int D, int KEYS>
 static int dkv_launch(const spamm_attn &a, const BackwardPlan &p, const T *d_do, int64_t do_token, int64_t do_head,
-                      const float *delta, const unsigned *bits, const Item *items, const int *n_items, float *partial, T *dk,
-                      T *dv, cudaStream_t stream)
+                      const float *delta, const float *factor, const unsigned *bits, const Item *items, const int *n_items,
+                      float *partial, T *dk, T *dv, cudaStream_t stream)
 {
     const size_t smem = 2 * KEYS * D * 2 + tk_slots(D, KEYS) * TK_ROWS * D * 2 + 2 * TK_ROWS * 128 + sizeof(TkCtrl) + p.chunk * 4;
     int st = attn_set_smem((const void *)attn_dkv_tc_kernel<T, D, KEYS>);
@@ -1181,7 +1269,7 @@ static int dkv_launch(const spamm_attn &a, const BackwardPlan &p, const T *d_do,
     attn_row_map(a, a.d_q, a.q_token, a.q_head, a.heads, G, max(1, p.box_tokens), &q_map);
     attn_row_map(a, d_do, do_token, do_head, a.heads, G, max(1, p.box_tokens), &do_map);
     attn_dkv_tc_kernel<T, D, KEYS><<<(unsigned)(p.groups * p.item_cap * (a.block / KEYS)), TK_THREADS, smem, stream>>>(
-        a, p, q_map, do_map, d_do, do_token, do_head, delta, bits, items, n_items, partial, dk, dv);
+        a, p, q_map, do_map, d_do, do_token, do_head, delta, factor, bits, items, n_items, partial, dk, dv);
     return SPAMM_OK;
 }
 
@@ -1195,6 +1283,9 @@ static int backward_launch(const spamm_attn &a, const BackwardPlan &p, const T *
     Item *items = reinterpret_cast<Item *>(scratch + p.items);
     int *n_items = reinterpret_cast<int *>(scratch + p.n_items);
     float *partial = reinterpret_cast<float *>(scratch + p.partial);
+    const bool half = std::is_same<T, __half>::value;
+    float2 *norms = half ? reinterpret_cast<float2 *>(scratch + p.norms) : nullptr;
+    float *factor = half ? reinterpret_cast<float *>(scratch + p.factor) : nullptr;
     const int64_t rows = (int64_t)a.tokens * a.heads, lists = (int64_t)a.batch * p.nqb * a.kv_heads;
     const int bq = min(a.query_block, a.max_q);
     const int tiles = (int)(((int64_t)bq * (a.heads / a.kv_heads) + 15) / 16);
@@ -1203,10 +1294,10 @@ static int backward_launch(const spamm_attn &a, const BackwardPlan &p, const T *
         p.groups * p.nkb > INT32_MAX)
         return attn_too_large();
 
-    attn_delta_kernel<T, D><<<(unsigned)((rows + 31) / 32), 256, 0, stream>>>(a, d_do, do_token, do_head, delta, dq, dk, dv,
-                                                                             reinterpret_cast<uint4 *>(bits), (p.slots - p.bits) / 16);
+    attn_delta_kernel<T, D><<<(unsigned)((rows + 31) / 32), 256, 0, stream>>>(a, fast_div(a.heads), p.G, d_do, do_token, do_head, delta, dq, dk, dv,
+                                                                             reinterpret_cast<uint4 *>(bits), (p.slots - p.bits) / 16, norms);
     attn_turn_kernel<<<(unsigned)((lists + 3) / 4), 128, 0, stream>>>(a, p.nqb, p.nkb, p.words, bits, counts);
-    attn_items_kernel<<<(unsigned)p.groups, 1024, 0, stream>>>(a, p, counts, slots, items, n_items);
+    attn_items_kernel<<<(unsigned)p.groups, 1024, 0, stream>>>(a, p, counts, slots, items, n_items, norms, factor);
 
     // (over more blocks than a union is built over, tiles of 16 rows whatever their number)
     int st;
@@ -1219,18 +1310,18 @@ static int backward_launch(const spamm_attn &a, const BackwardPlan &p, const T *
         st = attn_set_smem((const void *)attn_dq_tc_kernel<T, D>);
         if (st) return st;
         attn_dq_tc_kernel<T, D><<<(unsigned)(p.groups * tq), TQ_THREADS, smem, stream>>>(
-            a, tq, attn_tile_shape(a), entries, k_map, v_map, d_do, do_token, do_head, delta, dq);
+            a, tq, attn_tile_shape(a), entries, k_map, v_map, d_do, do_token, do_head, delta, factor, dq);
     } else {
         const size_t smem = (size_t)DQ_WARPS * DQ_STAGES * 2 * 16 * D * 2 + 2 * 16 * D * 2 + a.n_select * 4;
         st = attn_set_smem((const void *)attn_dq_rows_kernel<T, D>);
         if (st) return st;
-        attn_dq_rows_kernel<T, D><<<(unsigned)dq_grid, 128, smem, stream>>>(a, p.nqb, tiles, d_do, do_token, do_head, delta, dq);
+        attn_dq_rows_kernel<T, D><<<(unsigned)dq_grid, 128, smem, stream>>>(a, p.nqb, tiles, d_do, do_token, do_head, delta, factor, dq);
     }
 
     switch (a.block) {
-    case 16: st = dkv_launch<T, D, 16>(a, p, d_do, do_token, do_head, delta, bits, items, n_items, partial, dk, dv, stream); break;
-    case 32: st = dkv_launch<T, D, 32>(a, p, d_do, do_token, do_head, delta, bits, items, n_items, partial, dk, dv, stream); break;
-    default: st = dkv_launch<T, D, TK_MAX_KEYS>(a, p, d_do, do_token, do_head, delta, bits, items, n_items, partial, dk, dv, stream); break;
+    case 16: st = dkv_launch<T, D, 16>(a, p, d_do, do_token, do_head, delta, factor, bits, items, n_items, partial, dk, dv, stream); break;
+    case 32: st = dkv_launch<T, D, 32>(a, p, d_do, do_token, do_head, delta, factor, bits, items, n_items, partial, dk, dv, stream); break;
+    default: st = dkv_launch<T, D, TK_MAX_KEYS>(a, p, d_do, do_token, do_head, delta, factor, bits, items, n_items, partial, dk, dv, stream); break;
     }
     if (st) return st;
     if (p.nqb > p.chunk)

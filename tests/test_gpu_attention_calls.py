@@ -131,3 +131,57 @@ def test_one_list_for_the_whole_sequence(lens):
     val, tol = expect(q, k, v, got[0][0], lens, 16, n, True, 64 ** -0.5, d_o)
     for name, x in zip(("o", "dq", "dk", "dv"), got[1][1:5]):
         near(x, val[name], tol[name], name)
+
+
+# ------------------------------------------------------------------------------------------------ small numbers in half
+
+@pytest.mark.parametrize("lens,H,HK,D,block,query_block,n_select", [([700, 90], 4, 2, 128, 64, 64, 8), ([300], 4, 4, 64, 16, 1, 6),
+                                                                    ([20, 9], 1, 1, 128, 16, 5, 2), ([500], 16, 1, 64, 32, 1, 4)])
+@pytest.mark.parametrize("size", [2.0 ** -13, 2.0 ** -7, 2.0 ** 11])
+def test_half_gradients_keep_their_digits_whatever_the_size_of_the_output_gradient(lens, H, HK, D, block, query_block, n_select, size):
+    """Output gradients of a small (or large) power of two times whole numbers: gradients are those of the whole numbers times
+    that power, but for the rounding of the results themselves."""
+    from cuspamm_b200 import block_sparse_attention
+
+    g = torch.Generator().manual_seed(101)
+    T, cu = sum(lens), cu_of(lens)
+    q, k, v = (tokens(g, T, h, D, HF) for h in (H, HK, HK))
+    whole = torch.randint(-8, 9, (T, H, D), generator=g).to(DEV)        # times 2^-3 to 2^-16 (half's last bit is 2^-24)
+    lists = random_lists(g, lens, lens, HK, block, query_block, n_select, True)
+
+    def gradients(d_o):
+        x = [t.detach().requires_grad_() for t in (q, k, v)]
+        o = block_sparse_attention(*x, lists, cu, max(lens), block=block, query_block=query_block)
+        return torch.autograd.grad(o, x, d_o)
+
+    unit, small = gradients((whole * 2.0 ** -3).to(HF)), gradients((whole * 2.0 ** -3 * size).to(HF))
+    u = plain.half_step(HF)
+    for name, x, y in zip(("dq", "dk", "dv"), unit, small):
+        # the roundings of the two results, and half's last bit (results near half's largest number are left out)
+        want = x.double() * size
+        near(torch.where(want.abs() < 6e4, y.double(), want), want, 2 * u * want.abs() + 2.0 ** -25 * (1 + size), name)
+
+
+def test_half_gradients_of_long_flat_rows():
+    """Rows over 4096 keys of nearly equal weight, output gradients of 1e-4: within roundings of the values, with nothing allowed
+    for what half cannot hold but the last bit of the results."""
+    from cuspamm_b200 import block_sparse_attention
+
+    g = torch.Generator().manual_seed(103)
+    n, D = 4096, 64
+    q, k, v = (tokens(g, n, 1, D, HF) for _ in range(3))
+    q *= 0.125
+    d_o = (torch.randn(n, 1, D, generator=g) * 1e-4).to(HF).to(DEV)
+    lists = torch.arange(64, dtype=torch.int32, device=DEV).expand(1, 64, 1, 64).contiguous()
+    x = [t.detach().requires_grad_() for t in (q, k, v)]
+    got = torch.autograd.grad(block_sparse_attention(*x, lists, cu_of([n]), n, causal=False), x, d_o)
+    ok = torch.ones(n, n, dtype=torch.bool, device=DEV)
+    q, k, v, d_o = (t[:, 0].double() for t in (q, k, v, d_o))
+    val, _ = plain.attend(q, k, v, ok, D ** -0.5, d_o)
+    # half's roundings of p and ds (u each) and the float sums, as in _attention_plain.py
+    u, p, dp, delta = plain.half_step(HF), torch.exp(q @ k.T * D ** -0.5 - val["lse"][:, None]), d_o @ v.T, (d_o * val["o"]).sum(1, keepdim=True)
+    off_delta = (d_o.abs() * ((u + plain.SLACK) * (p @ v.abs()) + u * val["o"].abs())).sum(1, keepdim=True)
+    off = u * (p * (dp - delta) * D ** -0.5).abs() + p * D ** -0.5 * (off_delta + 2 * plain.SLACK * (dp.abs() + delta.abs()))
+    bound = dict(dq=off @ k.abs(), dk=off.T @ q.abs(), dv=(u + plain.SLACK) * (p.T @ d_o.abs()))
+    for name, y in zip(("dq", "dk", "dv"), got):
+        near(y[:, 0], val[name], bound[name] + u * val[name].abs() + 2.0 ** -25, name)
