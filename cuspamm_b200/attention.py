@@ -294,6 +294,20 @@ def block_sparse_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, li
     return _BlockSparseAttention.apply(q, k, v, lists, cu_seqlens, a, return_lse)
 
 
+class _NoGradient(torch.autograd.Function):
+    """A result without a gradient of its own, of tensors that want one: a backward pass through it raises."""
+
+    @staticmethod
+    def forward(ctx, x, source, name):
+        ctx.name = name
+        return x.view_as(x)
+
+    @staticmethod
+    def backward(ctx, *_):
+        raise RuntimeError(f"{ctx.name} has no gradient (block_sparse_attention has); run it under torch.no_grad() or on "
+                           "detached tensors")
+
+
 class PagedCache:
     """Keys and values of many sequences in pages of `page_size` tokens, with the sum of the keys of every page.
 
@@ -305,7 +319,10 @@ class PagedCache:
     What the tables say is checked on the GPU: a page outside the cache is read as masked and never written, a length
     beyond the table's width is cut, more new tokens than `max_new` or than the length holds are left out; `check()`
     reports any of these since the last report.  No two sequences may append to the same page in one call; reading a
-    shared page is fine."""
+    shared page is fine.
+
+    The cache serves and does not train: a backward pass through a result of `append` or `attend`, when q or what was appended
+    required gradients, raises RuntimeError."""
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, key_sums: Optional[torch.Tensor] = None):
         for name, x in (("k", k), ("v", v)):
@@ -323,6 +340,7 @@ class PagedCache:
         self.k, self.v = k, v
         self.key_sums = torch.zeros(sums, dtype=torch.float32, device=k.device) if key_sums is None else key_sums
         self.status = torch.zeros(1, dtype=torch.int32, device=k.device)
+        self._wanted_gradients = False           # some appended key or value did
 
     @classmethod
     def empty(cls, n_pages: int, kv_heads: int, head_dim: int, page_size: int = 64, dtype=torch.bfloat16,
@@ -333,6 +351,11 @@ class PagedCache:
     @property
     def page_size(self) -> int:
         return self.k.shape[2]
+
+    def _without_gradient(self, x: torch.Tensor, q: torch.Tensor, name: str) -> torch.Tensor:
+        if not torch.is_grad_enabled() or not (q.requires_grad or self._wanted_gradients):
+            return x
+        return _NoGradient.apply(x, q if q.requires_grad else torch.empty(0, requires_grad=True), "PagedCache." + name)
 
     def check(self) -> None:
         """Waits for the GPU and raises SpammError when a call met a page, a length or a number of new tokens out of
@@ -387,6 +410,8 @@ class PagedCache:
                 raise ValueError(f"inv_freq must have a multiple of 8 values, at most head_dim / 2, got {inv_freq.shape[0]}")
         a = self._problem(k if q is None else q, q_strides, cu_seqlens, max_new, page_table, lengths, 1)
         _set_keys(a, k, k_strides, v, v_strides)
+        if (k.requires_grad or v.requires_grad) and torch.is_grad_enabled():
+            self._wanted_gradients = True
         lib = _lib.load()
         with _device(k.device):
             out = None
@@ -399,7 +424,7 @@ class PagedCache:
                                             inv_freq.data_ptr() if inv_freq is not None else None,
                                             inv_freq.shape[0] if inv_freq is not None else 0, int(bool(interleaved)),
                                             _stream(k.device)), "spamm_attn_append_dev")
-        return out
+        return self._without_gradient(out, q, "append") if q is not None else None
 
     def select(self, q: torch.Tensor, cu_seqlens: torch.Tensor, max_new: int, page_table: torch.Tensor, lengths: torch.Tensor,
                n_select: int, query_block: int = 1, n_first: int = 1, n_local: int = 1) -> torch.Tensor:
@@ -414,8 +439,11 @@ class PagedCache:
                out: Optional[torch.Tensor] = None, return_lse: bool = False):
         """Attention of the newest tokens (one of each sequence or a whole chunk) over the cached keys up to their own,
         of all pages or, with `lists` (as `select` gives them, for the same `query_block`), of the listed ones.  With
-        `out` the result goes there, and its rows that belong to no sequence are left as they are; else they are zero."""
+        `out` the result goes there, and its rows that belong to no sequence are left as they are; else they are zero.
+        (As torch's own functions with an `out` it is refused where gradients are recorded for q or for `out`.)"""
         a = self._problem(q, _rows("q", q), cu_seqlens, max_new, page_table, lengths, query_block)
+        if out is not None and torch.is_grad_enabled() and isinstance(out, torch.Tensor) and (q.requires_grad or out.requires_grad):
+            raise ValueError("out: not where gradients are recorded (q or out requires them); call under torch.no_grad()")
         a.scale = _scale(scale, a.dim)
         a.d_k, a.d_v = self.k.data_ptr(), self.v.data_ptr()
         device = q.device
@@ -438,4 +466,8 @@ class PagedCache:
                 lse = torch.full((a.tokens, a.heads), float("-inf"), dtype=torch.float32, device=device)
                 a.d_lse = lse.data_ptr()
             _forward(a, device)
+        if a.zero_tail:
+            out = self._without_gradient(out, q, "attend")
+        if return_lse:
+            lse = self._without_gradient(lse, q, "attend")
         return (out, lse) if return_lse else out

@@ -185,3 +185,43 @@ def test_half_gradients_of_long_flat_rows():
     bound = dict(dq=off @ k.abs(), dk=off.T @ q.abs(), dv=(u + plain.SLACK) * (p.T @ d_o.abs()))
     for name, y in zip(("dq", "dk", "dv"), got):
         near(y[:, 0], val[name], bound[name] + u * val[name].abs() + 2.0 ** -25, name)
+
+
+# ------------------------------------------------------------------------------------------------ gradients that do not exist
+
+def test_a_backward_pass_through_the_cache_raises():
+    """append and attend have no gradient: asking for it must not pass in silence."""
+    from cuspamm_b200 import PagedCache
+
+    g = torch.Generator().manual_seed(111)
+    table, lengths, cu = torch.arange(2, dtype=torch.int32, device=DEV)[None], torch.tensor([20], dtype=torch.int32, device=DEV), cu_of([20])
+    q, k, v = (tokens(g, 20, h, 64, BF) for h in (4, 2, 2))
+    inv = torch.ones(32, device=DEV)
+
+    def run(q, k, v, **kw):
+        cache = PagedCache.empty(2, 2, 64, page_size=16, device=DEV)
+        rq = cache.append(k, v, cu, 20, table, lengths, inv_freq=inv, q=q)
+        return rq, cache.attend(q.detach() if kw.pop("cut", False) else rq, cu, 20, table, lengths, **kw)
+
+    want = run(q, k, v)
+    assert not want[0].requires_grad and not want[1].requires_grad
+    with torch.no_grad():
+        for x, y in zip(run(q.clone().requires_grad_(), k.clone().requires_grad_(), v), want):
+            assert not x.requires_grad and torch.equal(x, y)
+    w = q.clone().requires_grad_()
+    got = run(w, k, v)
+    for x, y in zip(got, want):
+        assert torch.equal(x, y)
+        with pytest.raises(RuntimeError, match="no gradient"):
+            x.float().sum().backward()
+    assert w.grad is None
+    for kw in (dict(k=k.clone().requires_grad_(), v=v), dict(k=k, v=v.clone().requires_grad_())):
+        with pytest.raises(RuntimeError, match="no gradient"):      # what was appended wanted one
+            run(q, **kw, cut=True)[1].float().sum().backward()
+    with pytest.raises(ValueError):
+        run(w, k, v, out=torch.empty_like(q))
+    with torch.no_grad():
+        run(w, k, v, out=torch.empty_like(q))
+    for x in run(w, k, v, return_lse=True)[1]:
+        with pytest.raises(RuntimeError, match="no gradient"):
+            x.float().sum().backward()
