@@ -294,6 +294,16 @@ def block_sparse_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, li
     return _BlockSparseAttention.apply(q, k, v, lists, cu_seqlens, a, return_lse)
 
 
+def _report(status: torch.Tensor, name: str) -> None:
+    """Raises what the kernels of any stream left in a status word, and clears it."""
+    torch.cuda.synchronize(status.device)
+    st = int(status.item())
+    if st:
+        status.zero_()
+        torch.cuda.synchronize(status.device)    # no later call's report is cleared with this one's
+        raise SpammError(st, name)
+
+
 class _NoGradient(torch.autograd.Function):
     """A result without a gradient of its own, of tensors that want one: a backward pass through it raises."""
 
@@ -358,12 +368,9 @@ class PagedCache:
         return _NoGradient.apply(x, q if q.requires_grad else torch.empty(0, requires_grad=True), "PagedCache." + name)
 
     def check(self) -> None:
-        """Waits for the GPU and raises SpammError when a call met a page, a length or a number of new tokens out of
-        range since the last report."""
-        st = int(self.status.item())
-        if st:
-            self.status.zero_()
-            raise SpammError(st, "PagedCache")
+        """Waits for the GPU (for the work of all streams) and raises SpammError when a call met a page, a length or a number
+        of new tokens out of range since the last report."""
+        _report(self.status, "PagedCache")
 
     def _problem(self, q, q_strides, cu_seqlens, max_new, page_table, lengths, query_block) -> SpammAttn:
         n_pages, kv_heads, page_size, dim = self.k.shape

@@ -225,3 +225,25 @@ def test_a_backward_pass_through_the_cache_raises():
     for x in run(w, k, v, return_lse=True)[1]:
         with pytest.raises(RuntimeError, match="no gradient"):
             x.float().sum().backward()
+
+
+# ------------------------------------------------------------------------------------------------ reports
+
+def test_check_waits_for_every_stream():
+    """A bad page met on a stream that is not the current one, and that is busy when the report is asked for."""
+    from cuspamm_b200 import PagedCache, SpammError
+
+    g = torch.Generator().manual_seed(121)
+    k, v, table, lengths = build_cache(g, [40], 1, 64, BF, 16)
+    q, cu, cache = tokens(g, 1, 2, 64, BF), cu_of([1]), PagedCache(k, v)
+    cache.attend(q, cu, 1, table, lengths)
+    cache.check()
+    table[0, 1] = -7
+    torch.cuda.synchronize(DEV)
+    side = torch.cuda.Stream(DEV)
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(100_000_000)                              # some 50 ms
+        cache.attend(q, cu, 1, table, lengths)
+    with pytest.raises(SpammError):
+        cache.check()
+    cache.check()
