@@ -12,7 +12,7 @@ from .engine import (  # noqa: F401
 from ._lib import SpammError, SpammStats  # noqa: F401
 
 # attention over selected blocks works on torch tensors: torch is imported when one of these is first asked for
-_ATTENTION = ("PagedCache", "block_sparse_attention", "select_blocks")
+_ATTENTION = ("PagedCache", "block_sparse_attention", "check_attention", "select_blocks")
 
 
 def __getattr__(name):

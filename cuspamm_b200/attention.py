@@ -3,6 +3,7 @@ multiplying, products of the listed blocks only) for queries, keys and values on
 
     lists = select_blocks(q, k, cu_seqlens, max_seqlen, n_select)
     o = block_sparse_attention(q, k, v, lists, cu_seqlens, max_seqlen)        # differentiable in q, k and v
+    check_attention()                                                         # now and then: what the kernels reported
 
 and, for serving, over a paged cache whose pages are the blocks:
 
@@ -117,6 +118,32 @@ def _problem(q: torch.Tensor, q_strides, kv_heads: int, cu_seqlens: torch.Tensor
     return a
 
 
+_STATUS = {}           # device index -> the word in which the calls on packed tokens leave what went wrong
+
+
+def _packed_status(device) -> Optional[int]:
+    status = _STATUS.get(device.index)
+    if status is None:
+        if torch.cuda.is_current_stream_capturing():
+            return None              # a capture before any call outside one: its memory would belong to the graph
+        stream = torch.cuda.Stream(device)
+        with torch.cuda.stream(stream):
+            status = torch.zeros(1, dtype=torch.int32, device=device)
+        stream.synchronize()
+        status = _STATUS.setdefault(device.index, status)
+    return status.data_ptr()
+
+
+def check_attention(device=None) -> None:
+    """Waits for the GPU (for the work of all streams) and raises SpammError when a `select_blocks` or
+    `block_sparse_attention` call on it, or a backward pass of one, met a sequence longer than `max_seqlen`, or gave up a wait
+    inside a kernel (its result is then NaN), since the last report.  (PagedCache.check reports for the cache's calls.)"""
+    index = torch.device("cuda" if device is None else device).index
+    status = _STATUS.get(torch.cuda.current_device() if index is None else index)
+    if status is not None:
+        _report(status, "attention")
+
+
 def _set_keys(a: SpammAttn, k: torch.Tensor, k_strides, v: Optional[torch.Tensor] = None, v_strides=None) -> None:
     a.d_k = k.data_ptr()
     a.k_token, a.k_head = k_strides
@@ -183,6 +210,8 @@ def _select(a: SpammAttn, q: torch.Tensor, key_sums: Optional[torch.Tensor], n_s
     a.n_select = n_select
     _on_gpu(q)
     with _device(q.device):
+        if not a.n_pages:
+            a.d_status = _packed_status(q.device)
         lists = torch.empty((a.batch, -(-a.max_q // a.query_block), a.kv_heads, n_select), dtype=torch.int32, device=q.device)
         n = lib.spamm_attn_select_scratch_bytes(C.byref(a))
         scratch, ptr = _scratch(n, q.device)
@@ -206,7 +235,8 @@ def select_blocks(q: torch.Tensor, k: torch.Tensor, cu_seqlens: torch.Tensor, ma
     n_select], ascending, -1 behind.  The score of a block is the sum of the queries (over the query block and the heads
     of the key head) times the block's mean key; it is taken in double, ties go to the lower block.  The first `n_first`
     blocks and those from `n_local` - 1 before the first query's to the last query's own are always taken.  No sequence
-    may be longer than `max_seqlen`.  The choice is not differentiable."""
+    may be longer than `max_seqlen` (`check_attention` reports it; what is beyond is left out).  The choice is not
+    differentiable."""
     q_strides = _rows("q", q)
     k_strides = _rows("k", k, like=q)
     a = _problem(q, q_strides, k.shape[1], cu_seqlens, _host_int("max_seqlen", max_seqlen), _host_int("block", block),
@@ -227,6 +257,7 @@ class _BlockSparseAttention(torch.autograd.Function):
     def forward(ctx, q, k, v, lists, cu_seqlens, a, want_lse):
         device = q.device
         with _device(device):
+            a.d_status = _packed_status(device)
             o = _like(q)
             lse = torch.empty((a.tokens, a.heads), dtype=torch.float32, device=device)
             _set_out(a, o)
@@ -281,7 +312,8 @@ def block_sparse_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, li
     them; an entry that is no block of the sequence, or not above every entry before it, is skipped), with `causal` over
     those up to its own position.  `scale` multiplies q.k (default head_dim ** -0.5).  A query that sees no key gets
     zeros.  Returns o [tokens, heads, head_dim], with `return_lse` also the log of the sum of exp(scale * q.k) per query
-    and head (float, not differentiable).  Differentiable once in q, k and v; two backward passes give the same bits."""
+    and head (float, not differentiable).  Differentiable once in q, k and v; two backward passes give the same bits.
+    Tokens of a sequence from `max_seqlen` on are left out, with zeros for results and gradients; `check_attention` reports it."""
     q_strides = _rows("q", q)
     k_strides = _rows("k", k, like=q)
     v_strides = _rows("v", v, heads=k.shape[1], like=q)

@@ -484,7 +484,7 @@ int spamm_count_valid_static_max_blocks(void);
  * What device memory says is never trusted with an address: cu is clamped to [0, tokens], lengths to the table's width,
  * a page outside [0, n_pages) is treated as masked (append: not written) and SPAMM_ERR_INVALID is stored to *d_status;
  * a list entry that is no block of the sequence, or not above every entry before it, is skipped.  Queries of a
- * sequence from max_q on are not computed (their rows count as rows behind the last sequence).
+ * sequence from max_q on are not computed (their rows count as rows behind the last sequence) and reported likewise.
  *
  * A NaN or an infinity in a key or value reaches the rows that read it and no others: what lies behind the last key of a
  * sequence, in blocks that are not listed or behind a causal limit changes no result.  One in a query or in its output
@@ -530,7 +530,9 @@ typedef struct spamm_attn {
     void *d_o_low;              /* [tokens][heads][dim] without gaps, may be NULL: what the rounding of o left, rounded
                                    to the type; output of the forward, read by the backward, whose gradients of q and
                                    k are then as near as if o had been kept in float */
-    int32_t *d_status;          /* one word, kept until the caller clears it; may be NULL without pages */
+    int32_t *d_status;          /* one word, kept until the caller clears it: SPAMM_ERR_INVALID for what is said above,
+                                   SPAMM_ERR_DEVICE_WAIT where a kernel gave up a wait (its results are then NaN); may be
+                                   NULL without pages */
 } spamm_attn;
 
 /*

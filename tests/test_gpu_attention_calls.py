@@ -247,3 +247,35 @@ def test_check_waits_for_every_stream():
     with pytest.raises(SpammError):
         cache.check()
     cache.check()
+
+
+def test_calls_on_packed_tokens_report():
+    """A sequence longer than the bound, and a wait given up (its code put in by hand), come out of check_attention once."""
+    from cuspamm_b200 import SpammError, attention, block_sparse_attention, check_attention, select_blocks
+
+    g = torch.Generator().manual_seed(131)
+    q, k, v, d_o = (tokens(g, 50, h, 64, BF) for h in (2, 1, 1, 2))
+    cu, lists = cu_of([30, 20]), torch.zeros(2, 1, 1, 1, dtype=torch.int32, device=DEV)
+    check_attention()
+    x = [t.requires_grad_() for t in (q, k, v)]
+    grads = torch.autograd.grad(block_sparse_attention(*x, lists, cu, 30, block=16), x, d_o)
+    select_blocks(q, k, cu, 30, 3, block=16, query_block=16)
+    check_attention(DEV)
+    o = block_sparse_attention(*x, lists, cu, 20, block=16)
+    assert not bool(o[20:30].any()) and bool(o[30:].any())
+    with pytest.raises(SpammError):
+        check_attention()
+    check_attention()
+    cut = torch.autograd.grad(o, x, d_o)
+    assert not any(bool(t[20:30].any()) for t in cut) and torch.equal(cut[0][30:], grads[0][30:])
+    with pytest.raises(SpammError):
+        check_attention()
+    select_blocks(q, k, cu, 20, 3, block=16, query_block=16)
+    with pytest.raises(SpammError):
+        check_attention()
+    check_attention()
+    attention._STATUS[0].fill_(4)                                 # SPAMM_ERR_DEVICE_WAIT
+    with pytest.raises(SpammError) as e:
+        check_attention()
+    assert e.value.status == 4
+    check_attention()
