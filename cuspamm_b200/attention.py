@@ -309,10 +309,11 @@ def block_sparse_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, li
                            max_seqlen: int, *, block: int = 64, query_block: int = 64, causal: bool = True,
                            scale: Optional[float] = None, return_lse: bool = False):
     """Attention of every query over the keys of the blocks on its query block's list (`lists` as `select_blocks` gives
-    them; an entry that is no block of the sequence, or not above every entry before it, is skipped), with `causal` over
-    those up to its own position.  `scale` multiplies q.k (default head_dim ** -0.5).  A query that sees no key gets
-    zeros.  Returns o [tokens, heads, head_dim], with `return_lse` also the log of the sum of exp(scale * q.k) per query
-    and head (float, not differentiable).  Differentiable once in q, k and v; two backward passes give the same bits.
+    them; an entry that is no block which some query of the query block may see, or not above every such entry before it,
+    is skipped), with `causal` over those up to its own position.  `scale` multiplies q.k (default head_dim ** -0.5).  A
+    query that sees no key gets zeros.  Returns o [tokens, heads, head_dim], with `return_lse` also the log of the sum of
+    exp(scale * q.k) per query and head (float, not differentiable).  Differentiable once in q, k and v; two backward
+    passes give the same bits.
     Tokens of a sequence from `max_seqlen` on are left out, with zeros for results and gradients; `check_attention` reports it."""
     q_strides = _rows("q", q)
     k_strides = _rows("k", k, like=q)

@@ -117,10 +117,15 @@ __device__ __forceinline__ int attn_for_list(const spamm_attn &a, int s, int qb,
     __syncwarp();
     return count;
 }
-// The same into an array with room for n_select.
-__device__ __forceinline__ int attn_load_list(const spamm_attn &a, int s, int qb, int nqb, int h, int n_blocks, int *out, int lane)
+// The same into an array with room for n_select.  n_blocks: of the whole query block, as what counts must not depend on the
+// tile that asks; returns how many are below `reached`, those that the tile's rows may see.
+__device__ __forceinline__ int attn_load_list(const spamm_attn &a, int s, int qb, int nqb, int h, int n_blocks, int reached, int *out, int lane)
 {
-    return attn_for_list(a, s, qb, nqb, h, n_blocks, lane, [&](int v, int i) { out[i] = v; });
+    const int n = attn_for_list(a, s, qb, nqb, h, n_blocks, lane, [&](int v, int i) { out[i] = v; });
+    if (reached >= n_blocks) return n;
+    int below = 0;
+    for (int i = lane; i < n; i += 32) below += out[i] < reached;
+    return __reduce_add_sync(~0u, below);
 }
 
 // ---- types

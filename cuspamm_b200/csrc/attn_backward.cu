@@ -206,7 +206,8 @@ __global__ __launch_bounds__(128) void attn_turn_kernel(const __grid_constant__ 
     const Seq sq = attn_seq(a, s);
     const int last = min((int)min((int64_t)(qb + 1) * a.query_block, (int64_t)sq.nq), sq.nq) - 1;
     if ((int64_t)qb * a.query_block >= sq.nq) return;
-    const int n = attn_load_list(a, s, qb, nqb, h, ceil_div(attn_limit(a, sq, last), a.block), lists[warp], lane);
+    const int blocks = ceil_div(attn_limit(a, sq, last), a.block);
+    const int n = attn_load_list(a, s, qb, nqb, h, blocks, blocks, lists[warp], lane);
     const int64_t group = (int64_t)s * a.kv_heads + h;
     for (int i = lane; i < n; i += 32) {
         const int64_t at = group * nkb + lists[warp][i];
@@ -341,7 +342,8 @@ __global__ __launch_bounds__(128) void attn_dq_rows_kernel(const __grid_constant
     }
     cp_commit();
     if (warp == 0) {
-        const int n = attn_load_list(a, s, qb, nqb, h, ceil_div(limit_max, a.block), blk, lane);
+        const int all_blocks = ceil_div(attn_limit(a, sq, qb * bq + n_tok - 1), a.block);
+        const int n = attn_load_list(a, s, qb, nqb, h, all_blocks, ceil_div(limit_max, a.block), blk, lane);
         if (lane == 0) shared_count = n;
     }
     __syncthreads();

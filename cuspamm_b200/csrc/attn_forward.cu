@@ -211,7 +211,8 @@ __global__ __launch_bounds__(128) void attn_rows_kernel(const __grid_constant__ 
     int count = n_blocks;
     if (a.n_select) {
         if (warp == 0) {
-            const int n = attn_load_list(a, s, qb, p.nqb, h, n_blocks, blk, lane);
+            const int all_blocks = ceil_div(attn_limit(a, sq, sq.pos0 + qb * p.bq + n_tok - 1), a.block);
+            const int n = attn_load_list(a, s, qb, p.nqb, h, all_blocks, n_blocks, blk, lane);
             if (lane == 0) shared_count = n;
         }
         __syncthreads();

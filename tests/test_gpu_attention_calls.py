@@ -279,3 +279,26 @@ def test_calls_on_packed_tokens_report():
         check_attention()
     assert e.value.status == 4
     check_attention()
+
+
+# ------------------------------------------------------------------------------------------------ lists
+
+@pytest.mark.parametrize("lens,H,HK,query_block", [([32], 1, 1, 32), ([33, 20], 1, 1, 40), ([17, 5], 4, 2, 17), ([300], 4, 2, 100)])
+def test_unordered_lists_are_read_alike_by_every_tile_and_both_passes(lens, H, HK, query_block):
+    """An entry counts when it is above every one before it, whether or not the rows of a tile reach it: all queries of a query
+    block read the same blocks, up to their own position."""
+    from cuspamm_b200 import block_sparse_attention
+
+    g = torch.Generator().manual_seed(141)
+    T, D, block = sum(lens), 64, 16
+    q, k, v, d_o = (tokens(g, T, h, D, BF) for h in (H, HK, HK, H))
+    nqb = -(-max(lens) // query_block)
+    lists = torch.randint(-1, 1 + max(lens) // block, (len(lens), nqb, HK, 6), generator=g).int()
+    lists[0, 0, :, :2] = torch.tensor([1, 0])
+    lists = lists.to(DEV)
+    x = [t.clone().requires_grad_() for t in (q, k, v)]
+    o, lse = block_sparse_attention(*x, lists, cu_of(lens), max(lens), block=block, query_block=query_block, return_lse=True)
+    got = (o.detach(), lse, *torch.autograd.grad(o, x, d_o))
+    val, tol = expect(q, k, v, lists, lens, block, query_block, True, D ** -0.5, d_o)
+    for n, y in zip(("o", "lse", "dq", "dk", "dv"), got):
+        near(y, val[n], tol[n], n)
