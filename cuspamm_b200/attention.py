@@ -359,9 +359,9 @@ class PagedCache:
     lengths[s] (int32) tokens are held, counting the new ones of the call: the same two tensors serve `append`, `select`
     and `attend` of one step.
 
-    What the tables say is checked on the GPU: a page outside the cache is read as masked and never written, a length
-    beyond the table's width is cut, more new tokens than `max_new` or than the length holds are left out; `check()`
-    reports any of these since the last report.  No two sequences may append to the same page in one call; reading a
+    What the tables say is checked on the GPU: a page outside the cache is read as masked and never written, tokens beyond
+    the table's width, more new tokens than `max_new` or than the length holds are left out; `check()` reports any of these
+    since the last report.  No two sequences may append to the same page in one call; reading a
     shared page is fine.
 
     The cache serves and does not train: a backward pass through a result of `append` or `attend`, when q or what was appended

@@ -40,7 +40,7 @@ struct Seq {
     int row0;     // first row of q (and of packed k, v)
     int nq;       // queries that are computed
     int nk;       // keys held
-    int pos0;     // position of the first query
+    int pos0;     // position of the first query (may lie before 0, or behind nk)
 };
 
 __device__ __forceinline__ Seq attn_seq(const spamm_attn &a, int s)
@@ -55,7 +55,7 @@ __device__ __forceinline__ Seq attn_seq(const spamm_attn &a, int s)
         const int held = a.d_lengths[s];
         r.nk = (int)min((int64_t)max(held, 0), room);
         if (held != r.nk && a.d_status) *a.d_status = SPAMM_ERR_INVALID;
-        r.pos0 = r.nk - all;
+        r.pos0 = max(held, 0) - all;       // a length beyond the table moves no token from its position
     } else {
         r.nk = r.nq;
         r.pos0 = 0;

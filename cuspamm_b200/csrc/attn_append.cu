@@ -62,7 +62,8 @@ __global__ __launch_bounds__(APPEND_THREADS) void attn_append_kernel(const __gri
     if (a.d_o && a.zero_tail) {
         // rows of q that belong to no sequence, or to no position
         const int end = s == a.batch - 1 ? a.tokens : min(max(a.d_cu[s + 1], sq.row0), a.tokens);
-        const int lead = s == 0 ? sq.row0 : 0, begin = sq.row0 + sq.nq, head_rows = min(skip, sq.nq);
+        const int lead = s == 0 ? sq.row0 : 0, head_rows = min(skip, sq.nq);
+        const int begin = sq.row0 + min(sq.nq, max(sq.nk - sq.pos0, 0));
         const int rows = lead + head_rows + (end - begin), vecs = hn * G * V;
         for (int i = j; i < rows; i += pages_per_seq) {
             const int64_t row = i < lead ? i : i < lead + head_rows ? sq.row0 + i - lead : begin + (i - lead - head_rows);
@@ -71,9 +72,10 @@ __global__ __launch_bounds__(APPEND_THREADS) void attn_append_kernel(const __gri
                     make_uint4(0, 0, 0, 0);
         }
     }
-    const int first = max(sq.pos0, 0);                                // first position that is written
+    const int first = max(sq.pos0, 0), end = min(sq.pos0 + sq.nq, sq.nk);    // positions that are written
+    if (first >= end) return;
     const int b = first / a.block + j;
-    const int lo = max(first, b * a.block), hi = min(min(sq.pos0 + sq.nq, sq.nk), (b + 1) * a.block);
+    const int lo = max(first, b * a.block), hi = min(end, (b + 1) * a.block);
     if (lo >= hi) return;
     const int n = hi - lo;
     int page = a.d_table[(int64_t)s * a.table_stride + b];

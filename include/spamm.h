@@ -481,11 +481,11 @@ int spamm_count_valid_static_max_blocks(void);
  * k and v are [n_pages][kv_heads][block][dim] with no gaps, the page of block b of sequence s is table[s][b], and
  * lengths[s] keys are held, the new ones among them (query i of n new ones has position lengths[s] - n + i).
  *
- * What device memory says is never trusted with an address: cu is clamped to [0, tokens], lengths to the table's width,
- * a page outside [0, n_pages) is treated as masked (append: not written) and SPAMM_ERR_INVALID is stored to *d_status;
- * a list entry that is no block which some query of its query block may see, or not above every such entry before it, is
- * skipped.  Queries of a sequence from max_q on are not computed (their rows count as rows behind the last sequence) and
- * reported likewise.
+ * What device memory says is never trusted with an address: cu is clamped to [0, tokens], what lengths says beyond the
+ * table's width is not there (tokens at such positions are not written, and see what there is), a page outside [0, n_pages)
+ * is treated as masked (append: not written), and SPAMM_ERR_INVALID is stored to *d_status; a list entry that is no block
+ * which some query of its query block may see, or not above every such entry before it, is skipped.  Queries of a sequence
+ * from max_q on are not computed (their rows count as rows behind the last sequence) and reported likewise.
  *
  * A NaN or an infinity in a key or value reaches the rows that read it and no others: what lies behind the last key of a
  * sequence, in blocks that are not listed or behind a causal limit changes no result.  One in a query or in its output

@@ -302,3 +302,54 @@ def test_unordered_lists_are_read_alike_by_every_tile_and_both_passes(lens, H, H
     val, tol = expect(q, k, v, lists, lens, block, query_block, True, D ** -0.5, d_o)
     for n, y in zip(("o", "lse", "dq", "dk", "dv"), got):
         near(y, val[n], tol[n], n)
+
+
+# ------------------------------------------------------------------------------------------------ lengths beyond the table
+
+@pytest.mark.parametrize("new", [1, 5, 40])
+@pytest.mark.parametrize("beyond", [0, 1, 3, 100])
+def test_tokens_beyond_the_table_are_left_out(new, beyond):
+    """A sequence that outgrew its row of the table keeps what it holds: tokens without a page are not written (nor anything else
+    instead), the others go to their own positions, queries see what there is up to theirs, and the report comes."""
+    from cuspamm_b200 import PagedCache, SpammError
+
+    g = torch.Generator().manual_seed(151)
+    page, D, H, HK, room = 16, 64, 4, 2, 64
+    k, v, table, _ = build_cache(g, [room, 10], HK, D, BF, page, nan_behind=False)
+    cache = PagedCache(k.clone(), v.clone())
+    cache.key_sums.fill_(3.0)
+    held = [room + beyond, 10]
+    lengths, cu = torch.tensor(held, dtype=torch.int32, device=DEV), cu_of([new, 2])
+    q, nk, nv = (tokens(g, new + 2, h, D, BF) for h in (H, HK, HK))
+    inv = (1e4 ** (-torch.arange(32, dtype=torch.float64) / 32)).float().to(DEV)
+    rq = cache.append(nk, nv, cu, max(new, 2), table, lengths, inv_freq=inv, q=q)
+    if beyond:
+        with pytest.raises(SpammError):
+            cache.check()
+    want_k, want_v, want_s, want_q = k.clone(), v.clone(), torch.full_like(cache.key_sums, 3.0), torch.zeros_like(q)
+    at = 0
+    for s, n in enumerate((new, 2)):
+        first = held[s] - n
+        for i in range(n):
+            p, pos = first + i, torch.tensor([first + i], device=DEV)
+            if p >= room:
+                continue
+            want_q[at + i] = plain.rotate(q[at + i:at + i + 1], pos, inv, False)[0]
+            want_k[table[s, p // page].long(), :, p % page] = plain.rotate(nk[at + i:at + i + 1], pos, inv, False)[0]
+            want_v[table[s, p // page].long(), :, p % page] = nv[at + i]
+        for b in range(first // page, -(-min(held[s], room) // page) if first < room else 0):
+            want_s[table[s, b].long()] = want_k[table[s, b].long(), :, :min(page, held[s] - b * page)].double().sum(1).float()
+        at += n
+    assert torch.equal(cache.k, want_k) and torch.equal(cache.v, want_v) and torch.equal(rq, want_q)
+    assert torch.equal(cache.key_sums, want_s)
+    o = cache.attend(q, cu, max(new, 2), table, lengths)
+    lists = cache.select(q, cu, max(new, 2), table, lengths, 4, n_first=0, n_local=1)
+    at = 0
+    for s, n in enumerate((new, 2)):
+        have, first = min(held[s], room), held[s] - n
+        assert all((max(0, min(first + i + 1, have)) == 0) == (lists[s, i, 0, 0] < 0) for i in range(n))
+        for h in range(H):
+            ok = torch.arange(have, device=DEV)[None] <= first + torch.arange(n, device=DEV)[:, None]
+            val, tol = plain.attend(q[at:at + n, h], flat(cache.k, table, s, have, h // 2), flat(cache.v, table, s, have, h // 2), ok, D ** -0.5)
+            near(o[at:at + n, h], val["o"], tol["o"], "o")
+        at += n
