@@ -278,6 +278,9 @@ __global__ __launch_bounds__(1024) void attn_items_kernel(const __grid_constant_
     if (tid == 0) n_items[group] = min(carry.x, p.item_cap);
 }
 
+// Whether every ds of a row is NaN in any case.
+static __device__ __forceinline__ bool dq_is_nan(float lse, float delta) { return lse != lse || (delta != delta && lse != -CUDART_INF_F); }
+
 // dq of one row over its own keys alone, by one warp: y[0 .. D/32).
 template <typename T, int D, typename Block>
 static __device__ __forceinline__ void dq_row(const spamm_attn &a, const Seq &sq, int s, int h, int query, int head, const T *d_do,
@@ -463,7 +466,9 @@ __global__ __launch_bounds__(128) void attn_dq_rows_kernel(const __grid_constant
 #pragma unroll
         for (int i = 0; i < D / 16; i++) out[i] = Pack<T>::two(y[2 * i], y[2 * i + 1]);
         const int x = tile * 16 + r;
-        T *dst = dq + (((int64_t)sq.row0 + qb * bq + x / G) * a.heads + h * G + x % G) * D + c0;
+        const int64_t at = ((int64_t)sq.row0 + qb * bq + x / G) * a.heads + h * G + x % G;
+        if (odd) odd = !dq_is_nan(a.d_lse[at], delta[at]);
+        T *dst = dq + at * D + c0;
 #pragma unroll
         for (int i = 0; i < D / 64; i++) reinterpret_cast<uint4 *>(dst)[i] = *reinterpret_cast<uint4 *>(out + 4 * i);
     }
@@ -786,7 +791,7 @@ __global__ __launch_bounds__(TQ_THREADS, 2) void attn_dq_tc_kernel(const __grid_
                 *reinterpret_cast<uint4 *>(smem + row_piece(D * 2, r, half * (D / 16) + c * 4 + i)) = *reinterpret_cast<uint4 *>(x);
             }
         }
-        const unsigned rows_odd = __ballot_sync(~0u, odd && fine && r < rows);
+        const unsigned rows_odd = __ballot_sync(~0u, odd && fine && r < rows && !dq_is_nan(z, minus_delta));
         if (rows_odd && lane == 0) atomicOr(&ctrl->odd[warp & 3], rows_odd);
         asm volatile("bar.sync 1, 256;" ::: "memory");
         if (ctrl->odd[0] | ctrl->odd[1] | ctrl->odd[2] | ctrl->odd[3]) {

@@ -386,6 +386,7 @@ __global__ __launch_bounds__(128) void attn_rows_kernel(const __grid_constant__ 
             for (int i = 0; i < D / 8; i++) y[i] += so[(w * 16 + r) * D + c0 + i] * f[w];
 #pragma unroll
         for (int i = 0; i < D / 8; i++) odd |= not_finite(__float_as_uint(y[i] * inv));
+        odd = odd && total == total;
         const int x = tile * 16 + r;
         const int64_t row = sq.row0 + qb * p.bq + x / G;
         const int head = h * G + x % G;
@@ -918,7 +919,7 @@ __global__ __launch_bounds__(TILES * 256 + 64, TILES == 1 ? 2 : 1) void attn_tc_
             else if (a.d_lse) a.d_lse[row * a.heads + head] = fine ? lse2 * LN2 : CUDART_NAN_F;
         }
         {
-            const unsigned rows_odd = __ballot_sync(~0u, odd && fine && r < rows);
+            const unsigned rows_odd = __ballot_sync(~0u, odd && l == l && fine && r < rows);
             if (rows_odd && lane == 0) atomicOr(&ctrl->odd[x0][quad], rows_odd);
         }
         tile_barrier(x0);

@@ -353,3 +353,50 @@ def test_tokens_beyond_the_table_are_left_out(new, beyond):
             val, tol = plain.attend(q[at:at + n, h], flat(cache.k, table, s, have, h // 2), flat(cache.v, table, s, have, h // 2), ok, D ** -0.5)
             near(o[at:at + n, h], val["o"], tol["o"], "o")
         at += n
+
+
+# ------------------------------------------------------------------------------------------------ values that are not finite
+
+@pytest.mark.parametrize("what", ["q", "k", "qkv"])
+def test_a_model_gone_to_nan_costs_no_more(what):
+    """Rows whose own scores are NaN have NaN results and need no second look: a poisoned batch takes about its usual time."""
+    from cuspamm_b200 import PagedCache, block_sparse_attention
+
+    g = torch.Generator().manual_seed(161)
+    n, H, HK, D = 2048, 8, 2, 128
+    lists = random_lists(g, [n], [n], HK, 64, 64, 8, True)
+    lists[:, :, :, 0] = 0                                           # (every query sees a key: none is empty)
+    lists = lists.sort(-1).values.contiguous()
+    k_pages, v_pages, table, lengths = build_cache(g, [4000], HK, D, BF, 64, nan_behind=False)
+    cu, one = cu_of([n]), cu_of([1])
+
+    def once(poison):
+        q, k, v, d_o = (tokens(g, n, h, D, BF) for h in (H, HK, HK, H))
+        cache = PagedCache(k_pages.clone(), v_pages.clone())
+        if poison:
+            for name, x in (("q", q), ("k", k), ("v", v), ("k", cache.k), ("v", cache.v)):
+                if name in what:
+                    x.fill_(torch.nan)
+        x = [t.requires_grad_() for t in (q, k, v)]
+
+        def calls():
+            o = block_sparse_attention(*x, lists, cu, n)
+            with torch.no_grad():
+                return (o.detach(), *torch.autograd.grad(o, x[:1], d_o), cache.attend(q, cu, n, table, lengths),
+                        cache.attend(q[:1], one, 1, table, lengths))
+        return calls
+
+    times = []
+    for poison in (False, True):
+        calls = once(poison)
+        got = calls()
+        if poison:
+            assert all(bool(torch.isnan(y).all()) for y in got)
+        start, end = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+        start.record()
+        for _ in range(3):
+            calls()
+        end.record()
+        torch.cuda.synchronize(DEV)
+        times.append(start.elapsed_time(end))
+    assert times[1] < 4 * times[0] + 1, times
