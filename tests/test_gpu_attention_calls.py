@@ -79,11 +79,10 @@ BORDERS = [(b, 64, 64, 8, 8) for b in (153, 154, 156, 157)] + [(b, 64, 1, 2, 2) 
     [(b, 16, 64, 1, 1) for b in (6060, 6100, 6144, 6145)] + [(b, 16, 24576, 1, 1) for b in (6060, 6140, 6144, 6145)]
 
 
-@pytest.mark.parametrize("blocks,block,query_block,heads,kv_heads", BORDERS)
-def test_select_where_shared_memory_passes_48_kb(blocks, block, query_block, heads, kv_heads):
+def check_selection(blocks, block, query_block, heads, kv_heads, D):
     from cuspamm_b200 import select_blocks
 
-    n, D, n_select = blocks * block - 3, 64, 9
+    n, n_select = blocks * block - 3, 9
     g = torch.Generator().manual_seed(blocks)
     q, k = tokens(g, n, heads, D, BF), tokens(g, n, kv_heads, D, BF)
     got = select_blocks(q, k, cu_of([n]), n, n_select, block=block, query_block=query_block, n_first=1, n_local=0)
@@ -91,7 +90,8 @@ def test_select_where_shared_memory_passes_48_kb(blocks, block, query_block, hea
     held = torch.full((blocks,), float(block), dtype=torch.float64, device=DEV)
     held[-1] = block - 3
     nqb = -(-n // query_block)
-    qs = torch.zeros(nqb, kv_heads, D, dtype=torch.float64, device=DEV).index_add_(0, torch.arange(n, device=DEV) // query_block, q.double())
+    qs = torch.zeros(nqb, kv_heads, D, dtype=torch.float64, device=DEV).index_add_(0, torch.arange(n, device=DEV) // query_block,
+                                                                                             q.double().view(n, kv_heads, -1, D).sum(2))
     last = torch.clamp((torch.arange(nqb, device=DEV) + 1) * query_block, max=n) - 1
     seen = torch.arange(blocks, device=DEV)[None] * block <= last[:, None]
     for h in range(kv_heads):
@@ -101,6 +101,18 @@ def test_select_where_shared_memory_passes_48_kb(blocks, block, query_block, hea
         want = torch.where(best.values > -torch.inf, best.indices, blocks).sort(1).values
         want = torch.where(want < blocks, want, -1)
         assert torch.equal(got[0, :, h].long(), want)
+
+
+@pytest.mark.parametrize("blocks,block,query_block,heads,kv_heads", BORDERS)
+def test_select_where_shared_memory_passes_48_kb(blocks, block, query_block, heads, kv_heads):
+    check_selection(blocks, block, query_block, heads, kv_heads, 64)
+
+
+# D = 128: tiles of 32 lists (4096 lists and more), of eight, one by one, spread
+@pytest.mark.parametrize("blocks,block,query_block,heads,kv_heads", [(90, 64, 1, 2, 1), (255, 16, 1, 8, 2), (256, 32, 4, 4, 4), (1000, 16, 16, 4, 2),
+                                                                     (1200, 16, 16, 1, 1), (700, 16, 5000, 2, 1)])
+def test_select_with_heads_of_128(blocks, block, query_block, heads, kv_heads):
+    check_selection(blocks, block, query_block, heads, kv_heads, 128)
 
 
 # ------------------------------------------------------------------------------------------------ the largest numbers
@@ -400,3 +412,150 @@ def test_a_model_gone_to_nan_costs_no_more(what):
         torch.cuda.synchronize(DEV)
         times.append(start.elapsed_time(end))
     assert times[1] < 4 * times[0] + 1, times
+
+
+# ------------------------------------------------------------------------------------------------ kernels of larger problems
+
+@pytest.mark.parametrize("dtype,D,page", [(BF, 64, 16), (BF, 128, 64), (HF, 64, 128), (HF, 128, 32)])
+@pytest.mark.parametrize("held,new", [([900, 130], [300, 130]), ([3100, 260, 1], [70, 260, 1])])
+def test_chunks_in_pairs_of_tiles(dtype, D, page, held, new):
+    """Unlisted chunks of many key heads: two tiles of 128 rows to a block of threads (148 pairs and more), an odd number of tiles, one
+    range of keys or several, a page that is not there and a NaN in the last token's key and value."""
+    from cuspamm_b200 import PagedCache, SpammError
+
+    g = torch.Generator().manual_seed(171)
+    HK, G = 8, 8 if len(new) == 2 else 6
+    k, v, table, lengths = build_cache(g, held, HK, D, dtype, page)
+    last = held[0] - 1
+    k[table[0, last // page].long(), :, last % page, 1] = torch.nan
+    v[table[0, last // page].long(), :, last % page, 2] = torch.nan
+    gone = (held[0] - new[0]) // page // 2
+    kept_table, kept = table.clone(), torch.ones(held[0], dtype=torch.bool, device=DEV)
+    table[0, gone] = -3
+    kept[gone * page:(gone + 1) * page] = False
+    q, cu = tokens(g, sum(new), HK * G, D, dtype), cu_of(new)
+    cache = PagedCache(k, v)
+    o, lse = cache.attend(q, cu, max(new), table, lengths, return_lse=True)
+    with pytest.raises(SpammError):
+        cache.check()
+    at = 0
+    for s, (n, m) in enumerate(zip(held, new)):
+        ok = plain.mask_of(None, m, n, n - m, page, 1, True, 0).to(DEV)
+        rows = m
+        if s == 0:
+            ok &= kept[None]
+            rows = m - 1                                            # the last query reads the NaN
+            assert bool(torch.isnan(o[at + rows]).all()) and bool(torch.isnan(lse[at + rows]).all())
+        for h in range(HK * G):
+            kk, vv = (flat(x, kept_table, s, n, h // G).nan_to_num(0.0) for x in (k, v))
+            val, tol = plain.attend(q[at:at + rows, h], kk, vv, ok[:rows], D ** -0.5)
+            near(o[at:at + rows, h], val["o"], tol["o"], f"o {s} {h}")
+            near(lse[at:at + rows, h], val["lse"], tol["lse"], f"lse {s} {h}")
+        at += m
+
+
+@pytest.mark.parametrize("lens,H,HK,D,dtype,block,query_block,n_select,causal", [
+    ([1100], 16, 1, 128, BF, 64, 1, 3, True), ([1100], 16, 1, 64, HF, 128, 1, 2, True), ([1300, 40], 16, 1, 128, HF, 128, 1, 2, False),
+    ([700], 16, 1, 64, BF, 16, 1, 4, True), ([1200, 3], 32, 2, 128, BF, 32, 1, 3, True), ([700], 64, 2, 64, HF, 64, 2, 2, True)])
+def test_blocks_that_very_many_queries_list(lens, H, HK, D, dtype, block, query_block, n_select, causal):
+    """Every query lists block 0: its gradients are sums of several work items, joined."""
+    from cuspamm_b200 import block_sparse_attention
+
+    g = torch.Generator().manual_seed(181)
+    T = sum(lens)
+    q, k, v, d_o = (tokens(g, T, h, D, dtype) for h in (H, HK, HK, H))
+    lists = random_lists(g, lens, lens, HK, block, query_block, n_select, causal)
+    lists[..., 0] = 0
+    x = [t.clone().requires_grad_() for t in (q, k, v)]
+    o = block_sparse_attention(*x, lists, cu_of(lens), max(lens), block=block, query_block=query_block, causal=causal)
+    got = (o.detach(), *torch.autograd.grad(o, x, d_o))
+    val, tol = expect(q, k, v, lists, lens, block, query_block, causal, D ** -0.5, d_o)
+    for n, y in zip(("o", "dq", "dk", "dv"), got):
+        near(y, val[n], tol[n], n)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("block", [16, 32, 64, 128])
+@pytest.mark.parametrize("dtype,lens,H,HK,query_block,causal", [(BF, [300, 77], 4, 2, 32, True), (HF, [290], 3, 1, 128, False)])
+def test_every_block_and_head_size(dtype, D, block, lens, H, HK, query_block, causal):
+    from cuspamm_b200 import block_sparse_attention
+
+    g = torch.Generator().manual_seed(191 + D + block)
+    T = sum(lens)
+    q, k, v, d_o = (tokens(g, T, h, D, dtype) for h in (H, HK, HK, H))
+    lists = random_lists(g, lens, lens, HK, block, query_block, 4, causal)
+    x = [t.clone().requires_grad_() for t in (q, k, v)]
+    o = block_sparse_attention(*x, lists, cu_of(lens), max(lens), block=block, query_block=query_block, causal=causal)
+    got = (o.detach(), *torch.autograd.grad(o, x, d_o))
+    val, tol = expect(q, k, v, lists, lens, block, query_block, causal, D ** -0.5, d_o)
+    for n, y in zip(("o", "dq", "dk", "dv"), got):
+        near(y, val[n], tol[n], n)
+
+
+@pytest.mark.parametrize("D,dtype", [(64, BF), (128, HF)])
+def test_lists_over_more_blocks_than_one_union_holds(D, dtype):
+    """Ten thousand blocks of 16 keys: the tiles' unions in two ranges, dq in tiles of 16 rows. Sampled queries and blocks against
+    the plain form over the listed keys."""
+    from cuspamm_b200 import block_sparse_attention
+
+    g = torch.Generator().manual_seed(201)
+    n, block, query_block, n_select, G = 160005, 16, 48, 5, 2
+    q, k, v, d_o = (tokens(g, n, h, D, dtype) for h in (G, 1, 1, G))
+    nqb, nkb = -(-n // query_block), -(-n // block)
+    own = (torch.arange(nqb) * query_block + query_block - 1).clamp(max=n - 1) // block
+    lists = (torch.rand(nqb, n_select, generator=g) * own[:, None]).long()
+    lists[:, 0], lists[:, -1] = torch.randint(0, 3, (nqb,), generator=g), own
+    lists = lists.sort(1).values.int()
+    x = [t.clone().requires_grad_() for t in (q, k, v)]
+    o = block_sparse_attention(*x, lists[None, :, None].contiguous().to(DEV), cu_of([n]), n, block=block, query_block=query_block)
+    got = dict(zip(("o", "dq", "dk", "dv"), (o.detach(), *torch.autograd.grad(o, x, d_o))))
+    rows_of = lambda i: torch.arange(i * query_block, min((i + 1) * query_block, n), device=DEV)  # noqa: E731
+
+    def of_query_block(i, h):
+        keys = torch.cat([torch.arange(b * block, min((b + 1) * block, n), device=DEV) for b in sorted(set(lists[i].tolist()))])
+        rows = rows_of(i)
+        return rows, keys, *plain.attend(q[rows, h], k[keys, 0], v[keys, 0], keys[None] <= rows[:, None], D ** -0.5, d_o[rows, h])
+
+    for i in [0, 1, 2000, nqb // 2, nqb - 2, nqb - 1]:
+        for h in range(G):
+            rows, _, val, tol = of_query_block(i, h)
+            for name in ("o", "dq"):
+                near(got[name][rows, h], val[name], tol[name], f"{name} {i}")
+    for b in [3000, nkb // 2, nkb - 1]:
+        at = torch.arange(b * block, min((b + 1) * block, n), device=DEV)
+        val, tol = ({name: torch.zeros(len(at), D, dtype=torch.float64, device=DEV) for name in ("dk", "dv")} for _ in range(2))
+        for i in (lists == b).any(1).nonzero()[:, 0].tolist():
+            for h in range(G):
+                _, keys, x, t = of_query_block(i, h)
+                here = (keys // block == b).nonzero()[:, 0]
+                for name in ("dk", "dv"):
+                    val[name] += x[name][here]
+                    tol[name] += t[name][here]
+        for name in ("dk", "dv"):
+            near(got[name][at, 0], val[name], tol[name], f"{name} {b}")
+
+
+def test_the_exponential_by_polynomial():
+    """lse of rows with two keys that count, scores 0 and x: log(1 + e^x), the second key in every place of a tile."""
+    from cuspamm_b200 import PagedCache
+
+    g = torch.Generator().manual_seed(211)
+    held, new, D = 256, 64, 64
+    table, lengths, cu = torch.arange(4, dtype=torch.int32, device=DEV)[None], torch.tensor([held], dtype=torch.int32, device=DEV), cu_of([new])
+    k = torch.zeros(4, 1, 64, D, dtype=BF, device=DEV)
+    q = torch.zeros(new, 1, D, dtype=BF, device=DEV)
+    q[:, 0, 0] = 1.0
+    for place in range(1, 128):
+        k.zero_()
+        k[..., 0] = -1000.0                                         # e^-1000: nothing
+        k[0, 0, 0] = 0.0
+        k[place // 64, 0, place % 64, 0], k[place // 64, 0, place % 64, 1] = 0.0, 1.0
+        q[:, 0, 1] = (-15 * torch.rand(new, generator=g)).to(BF)
+        _, lse = PagedCache(k, k).attend(q, cu, new, table, lengths, scale=1.0, return_lse=True)
+        x = q[:, 0, 1].double()
+        e = torch.exp(x)
+        # 2.7e-6 of the polynomial, the exponent's rounding (two of 2^-24 of a number up to 22, times ln 2), two steps of a sum
+        # between 1 and 2, its logarithm and the product with ln 2
+        bound = e / (1 + e) * (2.7e-6 + 2.0 ** -23 * x.abs() + 2.0 ** -23) + 4 * 2.0 ** -24
+        off = (lse[:, 0].double() - torch.log1p(e)).abs() - bound
+        assert float(off.max()) <= 0, (place, float(off.max()))
