@@ -354,7 +354,8 @@ class _NoGradient(torch.autograd.Function):
 class PagedCache:
     """Keys and values of many sequences in pages of `page_size` tokens, with the sum of the keys of every page.
 
-    k, v: [n_pages, kv_heads, page_size, head_dim]; key_sums: float [n_pages, kv_heads, head_dim].  The caller hands out
+    k, v: [n_pages, kv_heads, page_size, head_dim]; key_sums: float [n_pages, kv_heads, head_dim] (zeros when not given: pages
+    that hold keys already need theirs for `select`).  The caller hands out
     the pages: the page of tokens b * page_size .. of sequence s is page_table[s, b] (int32 [batch, width]), and
     lengths[s] (int32) tokens are held, counting the new ones of the call: the same two tensors serve `append`, `select`
     and `attend` of one step.

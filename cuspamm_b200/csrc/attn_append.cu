@@ -5,7 +5,8 @@
 // position * inv_freq are taken in double (a float angle of position 10^5 is off by 0.004), their sine and cosine are
 // rounded to float and kept in shared memory for all heads.  A rotated pair is (a cos - b sin, b cos + a sin) with every
 // product and sum rounded by itself, not fused: the stored keys are then the same bits wherever they are computed, and
-// with them the key sums by which blocks are selected.
+// with them the key sums by which blocks are selected.  (But for about one cosine in 10^8, which lies so near the middle of two
+// floats that the way its angle was put together decides.)
 //
 // Bound by reading and writing the tokens where they are many: 5 prompts of up to 4001 tokens, 32 heads and 4 key heads of 128,
 // q with them (307 MB), 80 us, 3.8 TB/s: a block of threads turns, stores and sums one after the other.  One token for each of 64 sequences: 11 us,

@@ -11,9 +11,9 @@
 //
 // p and ds are rounded to the type for their products.  bf16 has float's range; half loses digits below 2^-14, where ds lies
 // for output gradients of 1e-3 already (4096 keys of like weight and output gradients of 1e-4: every digit), so half's
-// operands are multiplied by powers of two on the way, which the float results are divided by: p by 2^15 (p <= 1), ds without
-// its scale by the 2^n that brings its bound, twice the longest do times the longest v (o_i is a mean of rows of v), near half's
-// largest numbers.
+// operands are multiplied by powers of two on the way, which the float results are divided by: p by 2^10 (p <= 1, but for scores
+// so large, from 10^7 on, that their float error is felt in p: room for 2^6), ds without its scale by the 2^n that brings its
+// bound, twice the longest do times the longest v (o_i is a mean of rows of v), near half's largest numbers.
 #include <type_traits>
 #include "attn_tc.cuh"
 
@@ -173,16 +173,16 @@ __global__ __launch_bounds__(256) void attn_delta_kernel(const __grid_constant__
     }
 }
 
-// What half's ds is multiplied by: the power of two that brings its bound, 2 |do| |v|, to 2^14 .. 2^15, from the largest squared
+// What half's ds is multiplied by: the power of two that brings its bound, 2 |do| |v|, to 2^13 .. 2^14, from the largest squared
 // norms.
 static __device__ float ds_factor(float norm_do, float norm_v)
 {
     const float bound = 2.f * sqrtf(norm_do) * sqrtf(norm_v);
-    int e = 15;
+    int e = 14;
     if (bound > 0.f) frexpf(bound, &e);               // bound < 2^e
-    return ldexpf(1.f, 15 - e);
+    return ldexpf(1.f, 14 - e);
 }
-constexpr float P_UP = 15.f;                          // log2 of what half's p is multiplied by
+constexpr float P_UP = 10.f, P_DOWN = 0x1p-10f;       // log2 of what half's p is multiplied by, and what takes it back
 
 // How ds enters its products and what their results are multiplied by.
 struct DsScale { float in, out; };
@@ -1116,7 +1116,7 @@ __global__ __launch_bounds__(TK_THREADS, tk_per_sm(D, TK_KEYS)) void attn_dkv_tc
         // half: p times 2^P_UP, and ds = p (dP - delta) with it times the factor
         constexpr bool IS_HALF = std::is_same<T, __half>::value;
         const DsScale dss = ds_scale<T>(a, factor);
-        const float p_up = IS_HALF ? P_UP : 0.f, p_down = IS_HALF ? 0x1p-15f : 1.f, ds_in = dss.in * p_down;
+        const float p_up = IS_HALF ? P_UP : 0.f, p_down = IS_HALF ? P_DOWN : 1.f, ds_in = dss.in * p_down;
         const float2 sc2 = make_float2(scale2, scale2), sc = make_float2(ds_in, ds_in);
         // lse and delta of the row in tile j as they are, and how many of this thread's keys it sees: requested a tile ahead,
         // and not touched before they are needed

@@ -559,3 +559,28 @@ def test_the_exponential_by_polynomial():
         bound = e / (1 + e) * (2.7e-6 + 2.0 ** -23 * x.abs() + 2.0 ** -23) + 4 * 2.0 ** -24
         off = (lse[:, 0].double() - torch.log1p(e)).abs() - bound
         assert float(off.max()) <= 0, (place, float(off.max()))
+
+
+def test_half_gradients_with_very_large_scores():
+    """Scores of 10^7, where a float's last bit is one: the largest takes all the weight, and nothing overflows."""
+    from cuspamm_b200 import block_sparse_attention
+
+    g = torch.Generator().manual_seed(221)
+    n, D = 64, 64
+    q, k, v, d_o = (tokens(g, n, 1, D, HF) for _ in range(4))
+    q, k = q * 600, k * 600
+    lists = torch.tensor([0, 1, 2, 3], dtype=torch.int32, device=DEV).expand(1, 4, 1, 4).contiguous()
+    x = [t.detach().requires_grad_() for t in (q, k, v)]
+    o = block_sparse_attention(*x, lists, cu_of([n]), n, block=16, query_block=16, scale=1.0)
+    got = torch.autograd.grad(o, x, d_o)
+    z = (q[:, 0].double() @ k[:, 0].double().T).masked_fill(torch.ones(n, n, dtype=torch.bool, device=DEV).triu(1), -torch.inf)
+    best = z.argmax(1)
+    two = z.topk(2, 1).values
+    assert float((two[1:, 0] - two[1:, 1]).min()) > 2 ** 5 and float(z.max()) > 1e7
+    near(o[:, 0].detach(), v[best, 0], 2.0 ** -10 * v[best, 0].double().abs(), "o")
+    assert all(bool(torch.isfinite(y).all()) for y in got)
+    # p is one but for its exponent's roundings: below 2^24 in powers of two, each is off by one at the most, and there are four
+    # (the running maximum, lse in units of e and back, the difference): p is within 2^4 of one
+    want = torch.zeros(n, D, dtype=torch.float64, device=DEV).index_add_(0, best, d_o[:, 0].double().abs())
+    assert float(z.max()) * 1.4427 < 2 ** 24 + 2 ** 23
+    assert float((got[2][:, 0].double().abs() - 16 * want).max()) <= 2.0 ** -10
