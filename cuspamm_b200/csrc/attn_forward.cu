@@ -3,7 +3,9 @@
 //   o_i = sum_j p_ij v_j,  p_ij = exp(scale q_i.k_j - lse_i),  lse_i = log sum_j exp(scale q_i.k_j)
 //
 // over the keys j of the blocks on the list of query i's block that i may see.  One pass over the keys with a running
-// maximum and sum (both float); p is rounded to the type of v for the product, as v itself is.
+// maximum and sum (both float); p is rounded to the type of v for the product, as v itself is: the tensor cores take 16 bits,
+// and half a step of p, as independent from key to key as those of v, about doubles the square of the error of the result's own
+// rounding.
 #include <stdio.h>
 #include <string.h>
 #include <atomic>
@@ -492,11 +494,12 @@ __global__ __launch_bounds__(128) void attn_rows_kernel(const __grid_constant__ 
 // Where pairs would not fill the GPU, and wherever keys are listed, single tiles (TILES 1) with one buffer each for K and V:
 // two blocks of threads per SM.
 //
-// Bound by the exponentials beside the products: a step of 128 keys and two tiles is 2 x 8 products of N = 128 for S and as
-// many for O (about 66 clocks each, 2100 in all for D = 128), and 2 x 128 x 128 exponentials, 2048 clocks of the SM's
-// special-function units if those took all of them, beside the multiplications, maxima, sums and conversions.  Two chunks of
-// 1024 and 750 tokens over 32768 and 24006 keys, 32 heads of 128 (832 GFLOP): 870 us, 0.96 PFLOP/s.  Three of 16 pairs of exponentials by
-// the polynomial: 853 us; none 860, six 863, eight 885.  Listed keys, 3 sequences of up to 8192, 16 blocks of 64 (276 GFLOP):
+// A step of 128 keys and two tiles is 2 x 8 products of N = 128 for S and as many for O (about 66 clocks each, 2100 in all for
+// D = 128), and 2 x 128 x 128 exponentials, 2048 clocks of the SM's special-function units if those took all of them, beside the
+// multiplications, maxima, sums and conversions.  Bound by the chain of a step rather than by either: S has one buffer for a
+// tile, p lies over it, and O += P V waits for all of p.  Two chunks of 1024 and 750 tokens over 32768 and 24006 keys, 32 heads
+// of 128 (832 GFLOP): 870 to 882 us, 0.94 to 0.96 PFLOP/s.  Three of 16 pairs of exponentials by the polynomial: 853 us; none
+// 860, six 863, eight 885, one per cent for a fifth of the unit's work.  Listed keys, 3 sequences of up to 8192, 16 blocks of 64 (276 GFLOP):
 // 470 us, 0.59 PFLOP/s; a tile has 8 steps of 128 keys there, and its beginning and end weigh.
 constexpr int TC_ROWS = 128, TC_KEYS = 128, TC_HALF = TC_KEYS / 2;
 constexpr int TC_ENTRIES = 2048;        // blocks of a union, at most
