@@ -278,8 +278,11 @@ __global__ __launch_bounds__(1024) void attn_items_kernel(const __grid_constant_
     if (tid == 0) n_items[group] = min(carry.x, p.item_cap);
 }
 
-// Whether every ds of a row is NaN in any case.
-static __device__ __forceinline__ bool dq_is_nan(float lse, float delta) { return lse != lse || (delta != delta && lse != -CUDART_INF_F); }
+// Whether no ds of a row is finite in any case.
+static __device__ __forceinline__ bool no_finite_ds(float lse, float delta)
+{
+    return lse != lse || (not_finite(__float_as_uint(delta)) && lse != -CUDART_INF_F);
+}
 
 // dq of one row over its own keys alone, by one warp: y[0 .. D/32).
 template <typename T, int D, typename Block>
@@ -467,19 +470,29 @@ __global__ __launch_bounds__(128) void attn_dq_rows_kernel(const __grid_constant
         for (int i = 0; i < D / 16; i++) out[i] = Pack<T>::two(y[2 * i], y[2 * i + 1]);
         const int x = tile * 16 + r;
         const int64_t at = ((int64_t)sq.row0 + qb * bq + x / G) * a.heads + h * G + x % G;
-        if (odd) odd = !dq_is_nan(a.d_lse[at], delta[at]);
+        if (odd) odd = !no_finite_ds(a.d_lse[at], delta[at]);
         T *dst = dq + at * D + c0;
 #pragma unroll
         for (int i = 0; i < D / 64; i++) reinterpret_cast<uint4 *>(dst)[i] = *reinterpret_cast<uint4 *>(out + 4 * i);
     }
     if (!__syncthreads_or(odd)) return;
     // rows that are not finite once more, over their own keys alone (see row_keys)
+    __shared__ uint32_t sure[D];
     if (odd) atomicOr(&odd_rows, 1u << r);
+    if (tid < D) sure[tid] = 0;
+    __syncthreads();
+    sure_columns<T, D>(a, sq, s, h, static_cast<const T *>(a.d_k), a.k_token, a.k_head, shared_count, 0, nullptr, blk, nullptr, limit_min, sure,
+                       tid, 128);
     __syncthreads();
 #pragma unroll 1
     for (int sr = warp; sr < rows; sr += DQ_WARPS) {
         if (!(odd_rows >> sr & 1)) continue;
         const int x = tile * 16 + sr, query = qb * bq + x / G, head = h * G + x % G;
+        const uint32_t *got = reinterpret_cast<const uint32_t *>(dq + (((int64_t)sq.row0 + query) * a.heads + head) * D + lane * (D / 32));
+        bool open = false;
+#pragma unroll
+        for (int i = 0; i < D / 32; i += 2) open |= unsure(Pack<T>::to2(got[i / 2]), sure, lane * (D / 32) + i, ~0u);
+        if (!__any_sync(~0u, open)) continue;
         float y[D / 32] = {};
         dq_row<T, D>(a, sq, s, h, query, head, d_do, do_token, do_head, delta, shared_count, [&](int e) { return blk[e]; }, lane, y);
         T *dst = dq + (((int64_t)sq.row0 + query) * a.heads + head) * D + lane * (D / 32);
@@ -791,15 +804,28 @@ __global__ __launch_bounds__(TQ_THREADS, 2) void attn_dq_tc_kernel(const __grid_
                 *reinterpret_cast<uint4 *>(smem + row_piece(D * 2, r, half * (D / 16) + c * 4 + i)) = *reinterpret_cast<uint4 *>(x);
             }
         }
-        const unsigned rows_odd = __ballot_sync(~0u, odd && fine && r < rows && !dq_is_nan(z, minus_delta));
+        const unsigned rows_odd = __ballot_sync(~0u, odd && fine && r < rows && !no_finite_ds(z, minus_delta));
         if (rows_odd && lane == 0) atomicOr(&ctrl->odd[warp & 3], rows_odd);
         asm volatile("bar.sync 1, 256;" ::: "memory");
         if (ctrl->odd[0] | ctrl->odd[1] | ctrl->odd[2] | ctrl->odd[3]) {
+            uint32_t *const sure = reinterpret_cast<uint32_t *>(smem + RT);         // behind the rows
+            if (tid < D) sure[tid] = 0;
+            asm volatile("bar.sync 1, 256;" ::: "memory");
+            sure_columns<T, D>(a, sq, s, h, static_cast<const T *>(a.d_k), a.k_token, a.k_head, n_entries, 0, blk, nullptr, bits, limit_min, sure,
+                               tid, 256);
+            asm volatile("bar.sync 1, 256;" ::: "memory");
 #pragma unroll 1
             for (int sr = warp; sr < rows; sr += 8) {
                 if (!(ctrl->odd[sr >> 5] >> (sr & 31) & 1)) continue;
                 const int sy = tr.row0 + sr, tok = (int)shape.G.quotient(sy), head = h * G + sy - tok * G;
                 const uint32_t bit = 1u << (tok / a.query_block - tr.qb0);
+                bool open = false;
+#pragma unroll
+                for (int i = 0; i < D / 32; i += 2) {
+                    const int d = lane * (D / 32) + i, piece = d * 2;
+                    open |= unsure(Pack<T>::to2(*reinterpret_cast<const uint32_t *>(smem + row_piece(D * 2, sr, piece >> 4) + (piece & 15))), sure, d, bit);
+                }
+                if (!__any_sync(~0u, open)) continue;
                 float y2[D / 32] = {};
                 dq_row<T, D>(a, sq, s, h, tok, head, d_do, do_token, do_head, delta, n_entries,
                              [&](int e) { return bits[e] & bit ? (int)blk[e] : -1; }, lane, y2);

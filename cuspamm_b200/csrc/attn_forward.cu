@@ -411,13 +411,30 @@ __global__ __launch_bounds__(128) void attn_rows_kernel(const __grid_constant__ 
     }
     const bool any_odd = __syncthreads_or(odd);
     // rows that are not finite once more, over their own keys alone (see row_keys)
-    if (odd) atomicOr(&odd_rows, 1u << r);
-    if (any_odd) __syncthreads();
+    __shared__ uint32_t sure[D];
+    if (any_odd) {
+        if (odd) atomicOr(&odd_rows, 1u << r);
+        if (tid < D) sure[tid] = 0;
+        __syncthreads();
+        sure_columns<T, D>(a, sq, s, h, static_cast<const T *>(a.d_v), a.v_token, a.v_head, e1 - e0, e0, nullptr,
+                           a.n_select ? blk + e0 : nullptr, nullptr, limit_min, sure, tid, 128);
+        __syncthreads();
+    }
 #pragma unroll 1
     for (int sr = warp; sr < rows && any_odd; sr += ROWS_WARPS) {
         if (!(odd_rows >> sr & 1)) continue;
         const int x = tile * 16 + sr, query = qb * p.bq + x / G, head = h * G + x % G;
         const int64_t row = sq.row0 + query;
+        const int64_t at = (row * a.heads + head) * p.n_split + split;
+        bool open = false;
+#pragma unroll
+        for (int i = 0; i < D / 32; i += 2) {
+            const int d = lane * (D / 32) + i;
+            const float2 got = p.n_split == 1 ? Pack<T>::to2(*reinterpret_cast<const uint32_t *>(static_cast<const T *>(a.d_o) + row * a.o_token + head * a.o_head + d))
+                                              : *reinterpret_cast<const float2 *>((p.cluster ? range_o + sr * D : part_o + at * D) + d);
+            open |= unsure(got, sure, d, ~0u);
+        }
+        if (!__any_sync(~0u, open)) continue;
         float q[D / 32], k[D / 32], v[D / 32], y[D / 32] = {}, top = -CUDART_INF_F, sum = 0.f;
         row_load<T, D>(static_cast<const T *>(a.d_q) + row * a.q_token + head * a.q_head, lane, q);
         row_keys<T>(a, sq, s, h, e1 - e0, attn_limit(a, sq, sq.pos0 + query), [&](int e) { return a.n_select ? blk[e0 + e] : e0 + e; },
@@ -427,7 +444,6 @@ __global__ __launch_bounds__(128) void attn_rows_kernel(const __grid_constant__ 
                         online_row<D>(row_dot<D>(q, k) * scale2, v, y, &top, &sum);
                     });
         const float inv = sum == 0.f ? 0.f : 1.f / sum;
-        const int64_t at = (row * a.heads + head) * p.n_split + split;
 #pragma unroll
         for (int i = 0; i < D / 32; i += 2) {
             const int d = lane * (D / 32) + i;
@@ -927,12 +943,26 @@ __global__ __launch_bounds__(TILES * 256 + 64, TILES == 1 ? 2 : 1) void attn_tc_
         }
         tile_barrier(x0);
         if (ctrl->odd[x0][0] | ctrl->odd[x0][1] | ctrl->odd[x0][2] | ctrl->odd[x0][3]) {
+            uint32_t *const sure = reinterpret_cast<uint32_t *>(stage + 2 * TILE);     // behind the rows
+            if ((tid & 255) < D) sure[tid & 255] = 0;
+            tile_barrier(x0);
+            sure_columns<T, D>(a, sq, s, h, static_cast<const T *>(a.d_v), a.v_token, a.v_head, n_entries, b0, listed ? idx : nullptr, nullptr,
+                               listed ? bits : nullptr, limit_min, sure, tid & 255, 256);
+            tile_barrier(x0);
 #pragma unroll 1
             for (int sr = warp & 7; sr < rows; sr += 8) {
                 if (!(ctrl->odd[x0][sr >> 5] >> (sr & 31) & 1)) continue;
                 const int sy = mine.row0 + sr, tok = (int)p.shape.G.quotient(sy), head = h * G + sy - tok * G;
                 const int64_t row = sq.row0 + tok;
                 const uint32_t bit = listed ? 1u << (tok / a.query_block - mine.qb0) : 1u;
+                bool open = false;
+#pragma unroll
+                for (int i = 0; i < D / 32; i += 2) {
+                    const int d = lane * (D / 32) + i, piece = d * (whole ? 2 : 4);
+                    const uint8_t *from = stage + row_piece(whole ? D * 2 : D * 4, sr, piece >> 4) + (piece & 15);
+                    open |= unsure(whole ? Pack<T>::to2(*reinterpret_cast<const uint32_t *>(from)) : *reinterpret_cast<const float2 *>(from), sure, d, bit);
+                }
+                if (!__any_sync(~0u, open)) continue;
                 float q[D / 32], k[D / 32], v[D / 32], o[D / 32] = {}, top = -CUDART_INF_F, sum = 0.f;
                 row_load<T, D>(static_cast<const T *>(a.d_q) + row * a.q_token + head * a.q_head, lane, q);
                 row_keys<T>(a, sq, s, h, n_entries, attn_limit(a, sq, sq.pos0 + tok),

@@ -319,9 +319,13 @@ __device__ __forceinline__ uint32_t row_piece(int row_bytes, int r, int c) { ret
 //
 // A tile multiplies every row with every key of its steps, those that the row does not read with p (or ds) = 0: a NaN or an
 // infinity among their values would reach the row all the same, as 0 * NaN.  Rows whose result is not finite are therefore
-// taken again over their own keys alone, one warp for a row, some 0.3 us a key.  (Rows that read such a value themselves come
-// out the same.)  Not those whose own scores are NaN, as their sum over visible keys tells (in the backward lse, or delta
-// where they see a key): all their results are, and a model gone to NaN costs no more than another.
+// taken again over their own keys alone, one warp for a row, some 0.3 us a key.  As that would be minutes where every row of
+// long sequences reads such a value, it is done only where it can change a result:
+//   not for rows whose own scores are NaN, as their sum over visible keys tells (in the backward lse, or delta where they see a
+//   key): all their results are;
+//   not for rows whose results are not finite in columns alone where a value that they read is not either (sure_columns).
+
+__device__ __forceinline__ bool not_finite(uint32_t v) { return (v & 0x7f800000u) == 0x7f800000u; }
 
 // Elements lane * D/32 .. of a row of D values.
 template <typename T, int D> __device__ __forceinline__ void row_load(const T *p, int lane, float *x)
@@ -357,6 +361,47 @@ __device__ __forceinline__ void row_keys(const spamm_attn &a, const Seq &sq, int
         for (int i = 0; i < keys; i++) f(static_cast<const T *>(a.d_k) + k0 + i * k_tok, static_cast<const T *>(a.d_v) + v0 + i * v_tok);
     }
 }
+// For every column of k or v (`rows`) the lists, as bits, that read a value there that is not finite, at a position below `limit`,
+// which all rows of the tile see: sure[D], zeros before, by `threads` threads.  Entries are blocks b0 + idx[e], blk[e] or b0 + e, and
+// their lists bits[e], or all.
+template <typename T, int D>
+static __device__ __noinline__ void sure_columns(const spamm_attn &a, const Seq &sq, int s, int h, const T *rows, int64_t token, int64_t head,
+                                                 int n_entries, int b0, const uint16_t *idx, const int *blk, const uint32_t *bits, int limit,
+                                                 uint32_t *sure, int t, int threads)
+{
+    constexpr uint32_t ONE = IsBf<T>::value ? 0x00800080u : 0x04000400u;      // carries an exponent of all ones into the sign's place
+    constexpr int AHEAD = 4;
+    const int c = t % (D / 8), step = threads / (D / 8), log_block = 31 - __clz(a.block), n = n_entries << log_block;
+    for (int i0 = t / (D / 8); i0 < n; i0 += AHEAD * step) {
+        uint4 x[AHEAD];
+#pragma unroll
+        for (int u = 0; u < AHEAD; u++) {
+            const int i = i0 + u * step, e = i >> log_block, r = i & (a.block - 1);
+            x[u] = make_uint4(0, 0, 0, 0);
+            if (i >= n) continue;
+            const int b = idx ? b0 + idx[e] : blk ? blk[e] : b0 + e;
+            if (b * a.block + r >= limit) continue;
+            const int64_t at = attn_block_base(a, sq, s, h, b, token, head);
+            if (at >= 0) x[u] = *reinterpret_cast<const uint4 *>(rows + at + r * (a.n_pages ? (int64_t)D : token) + c * 8);
+        }
+#pragma unroll
+        for (int u = 0; u < AHEAD; u++) {
+            const uint32_t y[4] = {x[u].x & 0x7fff7fffu, x[u].y & 0x7fff7fffu, x[u].z & 0x7fff7fffu, x[u].w & 0x7fff7fffu};
+            if (!(((y[0] + ONE) | (y[1] + ONE) | (y[2] + ONE) | (y[3] + ONE)) & 0x80008000u)) continue;
+            const uint32_t who = bits ? bits[(i0 + u * step) >> log_block] : ~0u;
+            for (int k = 0; k < 4; k++) {
+                if ((y[k] + ONE) & 0x8000u) atomicOr(sure + c * 8 + 2 * k, who);
+                if ((y[k] + ONE) & 0x80000000u) atomicOr(sure + c * 8 + 2 * k + 1, who);
+            }
+        }
+    }
+}
+// Whether some of a pair of results, columns d and d + 1, is not finite and not for sure.
+__device__ __forceinline__ bool unsure(float2 x, const uint32_t *sure, int d, uint32_t bit)
+{
+    return (not_finite(__float_as_uint(x.x)) && !(sure[d] & bit)) || (not_finite(__float_as_uint(x.y)) && !(sure[d + 1] & bit));
+}
+
 // One key with the score z (times log2 e) joins a row's running maximum, sum and output.
 template <int D> __device__ __forceinline__ void online_row(float z, const float *v, float *o, float *top, float *sum)
 {
@@ -367,8 +412,6 @@ template <int D> __device__ __forceinline__ void online_row(float z, const float
 #pragma unroll
     for (int i = 0; i < D / 32; i++) o[i] = o[i] * f + w * v[i];
 }
-__device__ __forceinline__ bool not_finite(uint32_t v) { return (v & 0x7f800000u) == 0x7f800000u; }
-
 // Barriers of a kernel and its abort flag: a wait that runs out (never, unless the kernel is wrong) sets the flag, every
 // role leaves its loop, and the results of the tile become NaN.
 struct WaitState {

@@ -584,3 +584,72 @@ def test_half_gradients_with_very_large_scores():
     want = torch.zeros(n, D, dtype=torch.float64, device=DEV).index_add_(0, best, d_o[:, 0].double().abs())
     assert float(z.max()) * 1.4427 < 2 ** 24 + 2 ** 23
     assert float((got[2][:, 0].double().abs() - 16 * want).max()) <= 2.0 ** -10
+
+
+@pytest.mark.parametrize("what", ["v", "k"])
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_an_infinity_that_every_row_reads_costs_no_more(what, dtype):
+    """The first token's value (or key) is infinite in one column, and every query reads it: its column of o (of dq) is not finite,
+    the others are as they should be, and nothing takes much longer."""
+    from cuspamm_b200 import PagedCache, block_sparse_attention
+
+    g = torch.Generator().manual_seed(231)
+    n, H, HK, D, COL = 2048, 8, 2, 128, 5
+    lists = random_lists(g, [n], [n], HK, 64, 64, 8, True)
+    lists[..., 0] = 0
+    q, k, v, d_o = (tokens(g, n, h, D, dtype) for h in (H, HK, HK, H))
+    pages_k, pages_v, table, lengths = build_cache(g, [4000], HK, D, dtype, 64, nan_behind=False)
+    cu, one = cu_of([n]), cu_of([1])
+    finite = [t.clone() for t in (k, v, pages_k, pages_v)]
+    first = table[0, 0].long()
+
+    def times():
+        x = [t.detach().requires_grad_() for t in (q, k, v)]
+        cache = PagedCache(pages_k, pages_v)
+
+        def calls():
+            o = block_sparse_attention(*x, lists, cu, n)
+            with torch.no_grad():
+                return (o.detach(), *torch.autograd.grad(o, x[:1], d_o), cache.attend(q, cu, n, table, lengths),
+                        cache.attend(q[-1:], one, 1, table, lengths))
+        got = calls()
+        start, end = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+        start.record()
+        for _ in range(3):
+            calls()
+        end.record()
+        torch.cuda.synchronize(DEV)
+        return got, start.elapsed_time(end)
+
+    usual = times()[1]
+    for x in ((v[0], pages_v[first, :, 0]) if what == "v" else (k[0], pages_k[first, :, 0])):
+        x[..., COL] = torch.inf
+    got, took = times()
+    assert took < 4 * usual + 1, (took, usual)
+    rest = [c for c in range(D) if c != COL]
+    fk, fv, pk, pv = finite
+    for h in range(H):
+        hk = h // (H // HK)
+        ok = plain.mask_of(lists[0].cpu()[None][0], n, n, 0, 64, 64, True, hk).to(DEV)
+        over_pages = torch.arange(4000, device=DEV)[None] <= (4000 - n + torch.arange(n, device=DEV))[:, None]
+        rows = slice(0, n)
+        if what == "k":
+            # a score of minus infinity: the key has no weight (plus infinity: all is NaN)
+            rows = (q[:, h, COL] < 0) & (torch.arange(n, device=DEV) > 0)
+            lost = q[:, h, COL] >= 0
+            assert all(bool(torch.isnan(y[:, h][lost]).all()) for y in got[:3])
+            ok[:, 0], over_pages[:, 0] = False, False
+        val, tol = plain.attend(q[rows, h], fk[:, hk], fv[:, hk], ok[rows], D ** -0.5, d_o[rows, h])
+        if what == "v":
+            assert bool(got[0][:, h, COL].isinf().all()) and not bool(got[1][:, h].isfinite().any())
+            near(got[0][:, h][:, rest], val["o"][:, rest], tol["o"][:, rest], "o")
+        else:
+            near(got[0][rows, h], val["o"], tol["o"], "o")
+            near(got[1][rows, h][:, rest], val["dq"][:, rest], tol["dq"][:, rest], "dq")
+            assert not bool(got[1][rows, h, COL].isfinite().any())
+        val, tol = plain.attend(q[rows, h], flat(pk, table, 0, 4000, hk), flat(pv, table, 0, 4000, hk), over_pages[rows], D ** -0.5)
+        columns = rest if what == "v" else list(range(D))
+        near(got[2][rows, h][:, columns], val["o"][:, columns], tol["o"][:, columns], "over pages")
+        if what == "v" or bool(q[-1, h, COL] < 0):
+            near(got[3][0, h, columns], val["o"][-1, columns], tol["o"][-1, columns], "one token")
+            assert what == "k" or bool(got[3][0, h, COL].isinf())
