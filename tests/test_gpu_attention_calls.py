@@ -653,3 +653,55 @@ def test_an_infinity_that_every_row_reads_costs_no_more(what, dtype):
         if what == "v" or bool(q[-1, h, COL] < 0):
             near(got[3][0, h, columns], val["o"][-1, columns], tol["o"][-1, columns], "one token")
             assert what == "k" or bool(got[3][0, h, COL].isinf())
+
+
+# ------------------------------------------------------------------------------------------------ layouts
+
+def test_rows_before_between_and_behind_the_sequences():
+    """cu_seqlens that begins behind row 0 and ends before the last: rows of no sequence are zero, in results and gradients, and what
+    stands in them (NaN) changes nothing."""
+    from cuspamm_b200 import block_sparse_attention, select_blocks
+
+    g = torch.Generator().manual_seed(241)
+    lens, lead, tail, H, HK, D = [60, 0, 75], 5, 9, 4, 2, 64
+    T = lead + sum(lens) + tail
+    for dtype in (BF, HF):
+        q, k, v, d_o = (tokens(g, T, h, D, dtype) for h in (H, HK, HK, H))
+        inner = slice(lead, T - tail)
+        lists = random_lists(g, lens, lens, HK, 16, 16, 3, True)
+
+        def run(q, k, v, d_o, cu):
+            x = [t.detach().requires_grad_() for t in (q, k, v)]
+            o = block_sparse_attention(*x, lists, cu, 75, block=16, query_block=16)
+            return (o.detach(), *torch.autograd.grad(o, x, d_o)), select_blocks(q, k, cu, 75, 4, block=16, query_block=16)
+
+        want, picked = run(*(t[inner].clone() for t in (q, k, v, d_o)), cu_of(lens))
+        for t in (q, k, v, d_o):
+            t[:lead], t[T - tail:] = torch.nan, torch.inf
+        got, again = run(q, k, v, d_o, cu_of(lens) + lead)
+        assert torch.equal(picked, again)
+        for a, b in zip(want, got):
+            assert torch.equal(a, b[inner]) and not bool(b[:lead].any()) and not bool(b[T - tail:].any())
+
+
+@pytest.mark.parametrize("new,n_select", [([1, 1], 0), ([1, 1], 5), ([130, 70], 0), ([130, 70], 5)])
+def test_results_into_strided_rows_and_tables_cut_from_wider_ones(new, n_select):
+    """out= with gaps between rows and heads, out= over q itself, a page table whose rows are part of a wider one."""
+    from cuspamm_b200 import PagedCache
+
+    g = torch.Generator().manual_seed(251)
+    H, HK, D, page = 8, 2, 128, 16
+    k, v, table, lengths = build_cache(g, [700, 333], HK, D, BF, page)
+    wide = torch.full((2, table.shape[1] + 7), 2 ** 30, dtype=torch.int32, device=DEV)
+    wide[:, 3:3 + table.shape[1]] = table
+    q, cu, cache = tokens(g, sum(new), H, D, BF), cu_of(new), PagedCache(k, v)
+    lists = random_lists(g, new, [700, 333], HK, page, 1, n_select, True) if n_select else None
+    want = cache.attend(q, cu, max(new), table, lengths, lists=lists)
+    assert torch.equal(cache.attend(q, cu, max(new), wide[:, 3:3 + table.shape[1]], lengths, lists=lists), want)
+    room = torch.full((sum(new), 2 * H, D + 8), 7.0, dtype=BF, device=DEV)
+    out = room[:, ::2, :D]
+    assert cache.attend(q, cu, max(new), table, lengths, lists=lists, out=out) is out
+    assert torch.equal(out, want) and bool((room[:, 1::2] == 7.0).all()) and bool((room[..., D:] == 7.0).all())
+    same = q.clone()
+    assert torch.equal(cache.attend(same, cu, max(new), table, lengths, lists=lists, out=same), want)
+    cache.check()
